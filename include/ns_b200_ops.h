@@ -191,6 +191,108 @@ int nsb_op_index(const float* in, int axis, int rows, int cols, const long long*
 int nsb_op_scatter(const float* in, int axis, int rows, int cols, const long long* idx, int L, const float* upd,
                    float* out, void* stream);
 
+/* ---- Mixture of experts with k experts a token (no reference counterpart:
+ * its layer sends a token to one expert) --------------------------------- */
+#define NSB_SCORE_SOFTMAX 0
+#define NSB_SCORE_SIGMOID 1
+
+/* Routing. logits [M, ld] (F32 or BF16), scores s = softmax over the live
+ * experts or sigmoid, both in fp32; active[e] = 0 marks a dead expert, whose
+ * logit is not looked at (NULL = all live). The choice goes by s + bias
+ * (bias [E], may be NULL). With groups > 1 (a divisor of E, at least two
+ * experts each) a group's score is the sum of its two best s + bias (of live
+ * experts; of its one where only one lives), and only the topk_groups best
+ * groups stay. The k largest are chosen, in falling order; ties go to the
+ * lower expert, and group. idx [M, k] receives the experts, w [M, k] their
+ * weights
+ *   w = scale * s / (sum of the k chosen s + 1e-20)     (renorm)
+ *   w = scale * s                                       (otherwise).
+ * A row with fewer than k candidates has idx -1 and w 0 in the rest; an
+ * expert whose s + bias is NaN or -inf is no candidate (a softmax row with a
+ * NaN or +inf logit, or with -inf in every live one, has none).
+ * Limits: E <= 1024, k <= 32, k <= E. */
+int nsb_op_moe_topk_route(const void* logits, int dtype, long long ld, int M, int E, int k, int score,
+                          const float* bias, const unsigned char* active, int groups, int topk_groups, int renorm,
+                          float scale, int* idx, float* w, void* stream);
+/* Its gradient: dlogits [M, ld_dlogits] (the logits' type) from dw [M, k],
+ * the same logits and the choice idx, which is constant. Entries of dw beside
+ * idx -1 are not looked at; a row without any expert gets zeros. */
+int nsb_op_moe_topk_route_bwd(const float* dw, const void* logits, int dtype, long long ld, int M, int E, int k,
+                              int score, const unsigned char* active, int renorm, float scale, const int* idx,
+                              void* dlogits, long long ld_dlogits, void* stream);
+
+/* Order of the pairs (token t, choice j), numbered t * k + j, by expert:
+ * expert e owns rows [offsets[e], offsets[e] + counts[e]) in rising pair
+ * order, offsets[e] a multiple of align, offsets[E] the end of the last.
+ * rows[r] = the pair in row r or -1 (all of nsb_op_moe_dispatch_rows(...)
+ * rows are written), pos[t * k + j] = its row, -1 for idx outside [0, E).
+ * E <= 1024, k <= 32; more than 2^31 - 1 rows return -2. */
+size_t nsb_op_moe_dispatch_rows(int M, int k, int E, int align);
+int nsb_op_moe_dispatch(const int* idx, int M, int k, int E, int align, int* offsets, int* counts, int* rows, int* pos,
+                        void* stream);
+
+/* y[t] = sum over j of w[t,j] * o[pos[t,j]] in fp32, rounded once (w NULL:
+ * all 1, the gradient of a gather by rows; negative pos are left out). o, y:
+ * [*, D] of one dtype. */
+int nsb_op_moe_combine(const void* o, int dtype, long long ld_o, const int* pos, const float* w, int M, int k, int D,
+                       void* y, long long ld_y, void* stream);
+/* Its gradient: d_o[r] = w[pair] * dy[pair / k] for pair = rows[r], zeros for
+ * rows[r] = -1 (R rows), and dw[pair] = <o[r], dy[pair / k]>, 0 for pairs
+ * without a row (dw and o may be NULL together). */
+int nsb_op_moe_combine_bwd(const void* dy, const void* o, int dtype, long long ld_dy, long long ld_o, const int* rows,
+                           const int* pos, const float* w, int M, int k, int R, int D, void* d_o, long long ld_do,
+                           float* dw, void* stream);
+
+/* ---- 8-bit floating point (e4m3) with a scale for each block of 128 ------
+ * (no reference counterpart)
+ *   scale = max(max |x| * (1 / 448), 2^-100),  code = e4m3(x * (1 / scale)),
+ * rounded to nearest even, the value read back code * scale. NaN gives a NaN
+ * code and does not count in the maximum; an infinity turns its block to NaN.
+ * Code arrays: 16-byte aligned, rows on 16-byte boundaries (leading
+ * dimensions multiples of 16). Scales of rows are block-major: row r,
+ * columns [128 b, 128 b + 128) at s[b * ld_s + r]; scales of 128 x 128 blocks
+ * lie row by row.
+ *
+ * x [*, ld] (F32 or BF16, any alignment) with act(x) quantised (act 0: x
+ * itself): q [M, ld_q] with s (a scale for each 1 x 128), and / or the
+ * transpose qt [K, ld_qt] with st (a scale for each 128 rows of a column).
+ * rows (NULL: none) gathers first: row r of the result is row
+ * rows[r] / row_div of x (row_div 0: row r), zeros for a negative entry. */
+int nsb_op_fp8_quantize(const void* x, int dtype, long long ld, int M, int K, int act, const int* rows, int row_div,
+                        void* q, long long ld_q, float* s, long long ld_s, void* qt, long long ld_qt, float* st,
+                        long long ld_st, void* stream);
+/* A scale for each 128 x 128: q [M, ld_q], s [M / 128, ld_s], and / or the
+ * transpose of the same codes and scales, qt [K, ld_qt], st [K / 128, ld_st]. */
+int nsb_op_fp8_quantize_block(const void* x, int dtype, long long ld, int M, int K, void* q, long long ld_q, float* s,
+                              long long ld_s, void* qt, long long ld_qt, float* st, long long ld_st, void* stream);
+
+/* C[M,N] = A[M,K] B[N,K]^T of the values that codes and scales stand for:
+ * exact products, fp32 sums over 128 k, these scaled and added in fp32,
+ * rounded once to c_dtype. A has row scales; B 128 x 128 scales (b_rows 0: a
+ * weight; its transposed codes serve the input gradient) or row scales
+ * (b_rows 1: the weight gradient, from two transposed quantisations). */
+int nsb_op_gemm_fp8(int M, int N, int K, const void* A, long long lda, const float* sa, long long ld_sa,
+                    const void* B, long long ldb, const float* sb, long long ld_sb, int b_rows, void* C, int c_dtype,
+                    long long ldc, int* dev_err, void* stream);
+/* The experts' products: rows [offsets[e], offsets[e] + counts[e]) of C
+ * [R, ldc] are those of A times B[e]^T (b_stride codes and sb_stride scales
+ * from expert to expert, 128 x 128 scales); other rows of C are not written.
+ * rows (NULL: A is in C's order): row r reads row rows[r] / row_div of A,
+ * which has a_rows rows. E <= 1024. */
+int nsb_op_moe_gemm_fp8(int R, int E, int N, int K, const void* A, long long lda, int a_rows, const float* sa,
+                        long long ld_sa, const int* rows, int row_div, const int* offsets, const int* counts,
+                        const void* B, long long ldb, long long b_stride, const float* sb, long long ld_sb,
+                        long long sb_stride, void* C, int c_dtype, long long ldc, int* dev_err, void* stream);
+/* The experts' weight gradients: C[e] (c_stride elements apart) =
+ * sum over r in [offsets[e], offsets[e] + counts[e]) of A[:, r] B[:, r]^T, A
+ * [M, R] and B [N, R] with row scales, both zero in the columns between an
+ * expert's last row and the next multiple of 128; offsets multiples of 128.
+ * An expert without rows gets zeros. */
+int nsb_op_moe_wgrad_fp8(int M, int N, int R, int E, const void* A, long long lda, const float* sa, long long ld_sa,
+                         const void* B, long long ldb, const float* sb, long long ld_sb, const int* offsets,
+                         const int* counts, void* C, int c_dtype, long long ldc, long long c_stride, int* dev_err,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif

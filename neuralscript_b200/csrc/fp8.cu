@@ -1,0 +1,214 @@
+// Quantisation to 8-bit floating point (e4m3) with a scale for each block of
+// 128 (no counterpart in the reference).
+//
+//   scale = max(max |x| * (1 / 448), 2^-100),  code = e4m3(x * (1 / scale))
+//
+// 448 is the largest finite e4m3 value; its reciprocal is rounded to fp32, a
+// multiplication in place of a division, for the quotient's last bit does not
+// matter: code and scale are read back together. The floor keeps 1 / scale finite for
+// blocks of zeros and of numbers so small that their quotient underflows. A
+// NaN becomes a NaN code and leaves its block's scale alone; an infinity
+// makes the scale infinite and the whole block NaN when it is read back.
+//
+// One block of threads takes 128 x 128 values, so that one read of x serves
+// both orientations and all three forms of scales. A half-warp owns 8 rows: a
+// lane 8 columns (one 16-byte load of bf16 a row), so row maxima are 4
+// shuffles and the 8 codes of a column are one 8-byte word of the transpose,
+// which goes through 16 KB of shared memory, the words of a column exchanged
+// (unit ^ column / 8) so that neither side has bank conflicts.
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+
+#include "fp8.h"
+
+namespace nsb {
+
+namespace {
+
+constexpr unsigned kAll = 0xffffffffu;
+constexpr float kTopInv = 1.f / 448.f;
+constexpr float kFloor = 7.888609052210118e-31f;  // 2^-100
+
+__device__ __forceinline__ float scale_of(float amax) { return fmaxf(amax * kTopInv, kFloor); }
+
+__device__ __forceinline__ uint32_t code4(float a, float b, float c, float d) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
+}
+
+__device__ __forceinline__ void store8(uint8_t* dst, uint2 v, int n) {
+    if (n >= 8) {
+        *reinterpret_cast<uint2*>(dst) = v;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (i < n) dst[i] = (uint8_t)((i < 4 ? v.x >> 8 * i : v.y >> 8 * (i - 4)) & 0xff);
+}
+
+template <typename T, bool BLOCK, bool VEC>
+__global__ void __launch_bounds__(256, 2) quantize_kernel(const QuantDesc d) {
+    __shared__ uint2 tile[128 * 16];   // [column][unit of 8 rows]
+    __shared__ float part[16][128];    // column maxima of the 16 half-warps
+    __shared__ float inv[128];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int half = warp * 2 + (lane >> 4);  // 0..15: rows 8 half ..
+    const int cl = lane & 15;
+    const int r0 = blockIdx.y * 128 + half * 8, c0 = blockIdx.x * 128 + cl * 8;
+    float v[8][8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int r = r0 + i;
+        long long src = r;
+        if (d.rows && r < d.M) {
+            src = d.rows[r];
+            if (src >= 0) src = d.row_div ? src / d.row_div : r;
+        }
+        const bool in = r < d.M && src >= 0;
+        const T* p = reinterpret_cast<const T*>(d.x) + src * d.ld + c0;
+        if (VEC && in && c0 + 8 <= d.K) {
+            if constexpr (sizeof(T) == 2) {
+                const uint4 t = *reinterpret_cast<const uint4*>(p);
+                const __nv_bfloat16* h = reinterpret_cast<const __nv_bfloat16*>(&t);
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[i][j] = bf2f(h[j]);
+            } else {
+                const float4 t0 = reinterpret_cast<const float4*>(p)[0], t1 = reinterpret_cast<const float4*>(p)[1];
+                v[i][0] = t0.x, v[i][1] = t0.y, v[i][2] = t0.z, v[i][3] = t0.w;
+                v[i][4] = t1.x, v[i][5] = t1.y, v[i][6] = t1.z, v[i][7] = t1.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[i][j] = in && c0 + j < d.K ? (float)p[j] : 0.f;
+        }
+    }
+    if (d.act) {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[i][j] = act_fwd(v[i][j], d.act);
+    }
+    if constexpr (BLOCK) {
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(v[i][j]));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
+        if (lane == 0) part[0][warp] = m;
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < 8; q++) m = fmaxf(m, part[0][q]);
+        const float s = scale_of(m), k = 1.f / s;
+        if (threadIdx.x == 0) {
+            if (d.s) d.s[blockIdx.y * d.ld_s + blockIdx.x] = s;
+            if (d.st) d.st[blockIdx.x * d.ld_st + blockIdx.y] = s;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[i][j] *= k;
+        if (d.q) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (r0 + i < d.M)
+                    store8(d.q + (size_t)(r0 + i) * d.ld_q + c0,
+                           make_uint2(code4(v[i][0], v[i][1], v[i][2], v[i][3]),
+                                      code4(v[i][4], v[i][5], v[i][6], v[i][7])),
+                           d.K - c0);
+        }
+        if (!d.qt) return;
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            tile[(cl * 8 + j) * 16 + (half ^ cl)] = make_uint2(code4(v[0][j], v[1][j], v[2][j], v[3][j]),
+                                                              code4(v[4][j], v[5][j], v[6][j], v[7][j]));
+    } else {
+        if (d.q) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                float m = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(v[i][j]));
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
+                const float s = scale_of(m), k = 1.f / s;
+                if (r0 + i < d.M) {
+                    if (cl == 0) d.s[blockIdx.x * d.ld_s + r0 + i] = s;
+                    store8(d.q + (size_t)(r0 + i) * d.ld_q + c0,
+                           make_uint2(code4(v[i][0] * k, v[i][1] * k, v[i][2] * k, v[i][3] * k),
+                                      code4(v[i][4] * k, v[i][5] * k, v[i][6] * k, v[i][7] * k)),
+                           d.K - c0);
+                }
+            }
+        }
+        if (!d.qt) return;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[i][j]));
+            part[half][cl * 8 + j] = m;
+        }
+        __syncthreads();
+        if (threadIdx.x < 128) {
+            float m = 0.f;
+#pragma unroll
+            for (int q = 0; q < 16; q++) m = fmaxf(m, part[q][threadIdx.x]);
+            const float s = scale_of(m);
+            inv[threadIdx.x] = 1.f / s;
+            const int c = blockIdx.x * 128 + threadIdx.x;
+            if (c < d.K) d.st[blockIdx.y * d.ld_st + c] = s;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float k = inv[cl * 8 + j];
+            tile[(cl * 8 + j) * 16 + (half ^ cl)] =
+                make_uint2(code4(v[0][j] * k, v[1][j] * k, v[2][j] * k, v[3][j] * k),
+                           code4(v[4][j] * k, v[5][j] * k, v[6][j] * k, v[7][j] * k));
+        }
+    }
+    __syncthreads();
+    const int r = blockIdx.y * 128 + cl * 8;
+    for (int c = half; c < 128; c += 16) {
+        const int col = blockIdx.x * 128 + c;
+        if (col < d.K && r < d.M)
+            store8(d.qt + (size_t)col * d.ld_qt + r, tile[c * 16 + (cl ^ (c >> 3))], d.M - r);
+    }
+}
+
+template <bool BLOCK>
+int quantize(const QuantDesc& d, cudaStream_t st) {
+    const bool f = d.dtype == kF32;
+    if (d.M < 0 || d.K <= 0 || (!f && d.dtype != kBF16) || d.ld < d.K || d.act < 0 || d.act > kGeluMoe) return -1;
+    if (d.rows && d.row_div < 0) return -1;
+    if (!d.q && !d.qt) return -1;
+    if (d.M == 0) return 0;
+    if (!d.x) return -1;
+    auto codes = [](const void* p, long long ld, int cols) {
+        return !(reinterpret_cast<uintptr_t>(p) & 15) && ld % 16 == 0 && ld >= cols;
+    };
+    const int rb = (d.M + 127) / 128, cb = (d.K + 127) / 128;
+    if (d.q && (!codes(d.q, d.ld_q, d.K) || !d.s || d.ld_s < (BLOCK ? cb : d.M))) return -1;
+    if (d.qt && (!codes(d.qt, d.ld_qt, d.M) || !d.st || d.ld_st < (BLOCK ? rb : d.K))) return -1;
+    if (rb > 65535) return -2;
+    const dim3 grid((unsigned)cb, (unsigned)rb);
+    const bool vec = !(reinterpret_cast<uintptr_t>(d.x) & 15) && d.ld * (f ? 4 : 2) % 16 == 0;
+    if (f) {
+        if (vec) quantize_kernel<float, BLOCK, true><<<grid, 256, 0, st>>>(d);
+        else quantize_kernel<float, BLOCK, false><<<grid, 256, 0, st>>>(d);
+    } else {
+        if (vec) quantize_kernel<__nv_bfloat16, BLOCK, true><<<grid, 256, 0, st>>>(d);
+        else quantize_kernel<__nv_bfloat16, BLOCK, false><<<grid, 256, 0, st>>>(d);
+    }
+    return cudaGetLastError() == cudaSuccess ? 0 : -5;
+}
+
+}  // namespace
+
+int fp8_quantize(const QuantDesc& d, cudaStream_t s) { return quantize<false>(d, s); }
+int fp8_quantize_block(const QuantDesc& d, cudaStream_t s) { return quantize<true>(d, s); }
+
+}  // namespace nsb

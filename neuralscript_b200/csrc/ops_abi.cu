@@ -7,9 +7,11 @@
 #include "attention.h"
 #include "elementwise.h"
 #include "engine.h"
+#include "fp8.h"
 #include "gemm.h"
 #include "kernels.h"
 #include "moe.h"
+#include "moe_topk.h"
 
 using namespace nsb;
 
@@ -292,6 +294,199 @@ int nsb_op_gemm_layernorm(int M, int K, const void* A, int dtype, long long lda,
     d.ep.ln_rstd = rstd;
     launch_counter() += 1;
     return gemm(d, (cudaStream_t)stream, dev_err);
+}
+
+static RouteDesc make_route(const void* logits, int dtype, long long ld, int M, int E, int k, int score,
+                            const float* bias, const unsigned char* active, int groups, int topk_groups, int renorm,
+                            float scale) {
+    RouteDesc d;
+    d.logits = logits;
+    d.dtype = dtype;
+    d.ld = ld;
+    d.M = M;
+    d.E = E;
+    d.k = k;
+    d.sigmoid = score == NSB_SCORE_SIGMOID;
+    d.bias = bias;
+    d.active = active;
+    d.groups = groups;
+    d.topk_groups = topk_groups;
+    d.renorm = renorm != 0;
+    d.scale = scale;
+    return d;
+}
+
+int nsb_op_moe_topk_route(const void* logits, int dtype, long long ld, int M, int E, int k, int score,
+                          const float* bias, const unsigned char* active, int groups, int topk_groups, int renorm,
+                          float scale, int* idx, float* w, void* stream) {
+    if (score != NSB_SCORE_SOFTMAX && score != NSB_SCORE_SIGMOID) return -1;
+    launch_counter() += 1;
+    return moe_topk_route(make_route(logits, dtype, ld, M, E, k, score, bias, active, groups, topk_groups, renorm, scale),
+                          idx, w, (cudaStream_t)stream);
+}
+
+int nsb_op_moe_topk_route_bwd(const float* dw, const void* logits, int dtype, long long ld, int M, int E, int k,
+                              int score, const unsigned char* active, int renorm, float scale, const int* idx,
+                              void* dlogits, long long ld_dlogits, void* stream) {
+    if (score != NSB_SCORE_SOFTMAX && score != NSB_SCORE_SIGMOID) return -1;
+    launch_counter() += 1;
+    return moe_topk_route_bwd(make_route(logits, dtype, ld, M, E, k, score, nullptr, active, 1, 1, renorm, scale), dw,
+                              idx, dlogits, ld_dlogits, (cudaStream_t)stream);
+}
+
+size_t nsb_op_moe_dispatch_rows(int M, int k, int E, int align) { return moe_dispatch_rows(M, k, E, align); }
+
+int nsb_op_moe_dispatch(const int* idx, int M, int k, int E, int align, int* offsets, int* counts, int* rows, int* pos,
+                        void* stream) {
+    launch_counter() += 1;
+    return moe_dispatch(idx, M, k, E, align, offsets, counts, rows, pos, (cudaStream_t)stream);
+}
+
+int nsb_op_moe_combine(const void* o, int dtype, long long ld_o, const int* pos, const float* w, int M, int k, int D,
+                       void* y, long long ld_y, void* stream) {
+    launch_counter() += 1;
+    return moe_combine(o, dtype, ld_o, pos, w, M, k, D, y, ld_y, (cudaStream_t)stream);
+}
+
+int nsb_op_moe_combine_bwd(const void* dy, const void* o, int dtype, long long ld_dy, long long ld_o, const int* rows,
+                           const int* pos, const float* w, int M, int k, int R, int D, void* d_o, long long ld_do,
+                           float* dw, void* stream) {
+    launch_counter() += 1;
+    return moe_combine_bwd(dy, o, dtype, ld_dy, ld_o, rows, pos, w, M, k, R, D, d_o, ld_do, dw, (cudaStream_t)stream);
+}
+
+int nsb_op_fp8_quantize(const void* x, int dtype, long long ld, int M, int K, int act, const int* rows, int row_div,
+                        void* q, long long ld_q, float* s, long long ld_s, void* qt, long long ld_qt, float* st,
+                        long long ld_st, void* stream) {
+    QuantDesc d;
+    d.x = x;
+    d.dtype = dtype;
+    d.ld = ld;
+    d.M = M;
+    d.K = K;
+    d.act = act;
+    d.rows = rows;
+    d.row_div = row_div;
+    d.q = reinterpret_cast<uint8_t*>(q);
+    d.ld_q = ld_q;
+    d.s = s;
+    d.ld_s = ld_s;
+    d.qt = reinterpret_cast<uint8_t*>(qt);
+    d.ld_qt = ld_qt;
+    d.st = st;
+    d.ld_st = ld_st;
+    launch_counter() += 1;
+    return fp8_quantize(d, (cudaStream_t)stream);
+}
+
+int nsb_op_fp8_quantize_block(const void* x, int dtype, long long ld, int M, int K, void* q, long long ld_q, float* s,
+                              long long ld_s, void* qt, long long ld_qt, float* st, long long ld_st, void* stream) {
+    QuantDesc d;
+    d.x = x;
+    d.dtype = dtype;
+    d.ld = ld;
+    d.M = M;
+    d.K = K;
+    d.q = reinterpret_cast<uint8_t*>(q);
+    d.ld_q = ld_q;
+    d.s = s;
+    d.ld_s = ld_s;
+    d.qt = reinterpret_cast<uint8_t*>(qt);
+    d.ld_qt = ld_qt;
+    d.st = st;
+    d.ld_st = ld_st;
+    launch_counter() += 1;
+    return fp8_quantize_block(d, (cudaStream_t)stream);
+}
+
+int nsb_op_gemm_fp8(int M, int N, int K, const void* A, long long lda, const float* sa, long long ld_sa,
+                    const void* B, long long ldb, const float* sb, long long ld_sb, int b_rows, void* C, int c_dtype,
+                    long long ldc, int* dev_err, void* stream) {
+    Fp8Gemm d;
+    d.M = M;
+    d.N = N;
+    d.K = K;
+    d.a = reinterpret_cast<const uint8_t*>(A);
+    d.lda = lda;
+    d.a_rows = M;
+    d.sa = sa;
+    d.ld_sa = ld_sa;
+    d.b = reinterpret_cast<const uint8_t*>(B);
+    d.ldb = ldb;
+    d.sb = sb;
+    d.ld_sb = ld_sb;
+    d.b_rows = b_rows != 0;
+    d.c = C;
+    d.c_dtype = c_dtype;
+    d.ldc = ldc;
+    d.err = dev_err;
+    launch_counter() += 1;
+    return fp8_gemm(d, (cudaStream_t)stream);
+}
+
+int nsb_op_moe_gemm_fp8(int R, int E, int N, int K, const void* A, long long lda, int a_rows, const float* sa,
+                        long long ld_sa, const int* rows, int row_div, const int* offsets, const int* counts,
+                        const void* B, long long ldb, long long b_stride, const float* sb, long long ld_sb,
+                        long long sb_stride, void* C, int c_dtype, long long ldc, int* dev_err, void* stream) {
+    if (E <= 0 || a_rows < 0 || (!rows && a_rows < R)) return -1;
+    Fp8Gemm d;
+    d.M = R;
+    d.N = N;
+    d.K = K;
+    d.a = reinterpret_cast<const uint8_t*>(A);
+    d.lda = lda;
+    d.a_rows = a_rows;
+    d.sa = sa;
+    d.ld_sa = ld_sa;
+    d.b = reinterpret_cast<const uint8_t*>(B);
+    d.ldb = ldb;
+    d.b_stride = b_stride;
+    d.sb = sb;
+    d.ld_sb = ld_sb;
+    d.sb_stride = sb_stride;
+    d.c = C;
+    d.c_dtype = c_dtype;
+    d.ldc = ldc;
+    d.groups = E;
+    d.offsets = offsets;
+    d.counts = counts;
+    d.rows = rows;
+    d.row_div = row_div;
+    d.err = dev_err;
+    launch_counter() += 1;
+    return fp8_gemm(d, (cudaStream_t)stream);
+}
+
+int nsb_op_moe_wgrad_fp8(int M, int N, int R, int E, const void* A, long long lda, const float* sa, long long ld_sa,
+                         const void* B, long long ldb, const float* sb, long long ld_sb, const int* offsets,
+                         const int* counts, void* C, int c_dtype, long long ldc, long long c_stride, int* dev_err,
+                         void* stream) {
+    if (E <= 0) return -1;
+    Fp8Gemm d;
+    d.M = M;
+    d.N = N;
+    d.K = R;
+    d.a = reinterpret_cast<const uint8_t*>(A);
+    d.lda = lda;
+    d.a_rows = M;
+    d.sa = sa;
+    d.ld_sa = ld_sa;
+    d.b = reinterpret_cast<const uint8_t*>(B);
+    d.ldb = ldb;
+    d.sb = sb;
+    d.ld_sb = ld_sb;
+    d.b_rows = 1;
+    d.c = C;
+    d.c_dtype = c_dtype;
+    d.ldc = ldc;
+    d.c_stride = c_stride;
+    d.groups = E;
+    d.group_k = 1;
+    d.offsets = offsets;
+    d.counts = counts;
+    d.err = dev_err;
+    launch_counter() += 1;
+    return fp8_gemm(d, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,124 @@
+"""Argument checks of the top-k mixture-of-experts and 8-bit operators at the
+C entries: every refusal comes before anything is launched, so none needs a
+GPU."""
+
+import pytest
+
+from neuralscript_b200 import ops
+
+X = 0x10000  # an address that is never read
+
+
+def rc(name, *args):
+    return getattr(ops.L(), name)(*args, None)
+
+
+def route(**kw):
+    a = dict(logits=X, dtype=0, ld=16, M=4, E=16, k=2, score=0, bias=None, active=None, groups=1, topk_groups=1, renorm=1,
+             scale=1.0, idx=X, w=X) | kw
+    return rc("nsb_op_moe_topk_route", *a.values())
+
+
+@pytest.mark.parametrize("bad", [dict(k=0), dict(k=17), dict(E=0, ld=0), dict(E=1025, ld=1025), dict(k=33, E=64, ld=64),
+                                 dict(M=-1), dict(ld=15), dict(dtype=2), dict(score=2), dict(groups=3), dict(groups=0),
+                                 dict(groups=16), dict(groups=4, topk_groups=5), dict(topk_groups=0), dict(logits=None),
+                                 dict(idx=None), dict(w=None)])
+def test_route_refuses(bad):
+    assert route(**bad) == -1
+
+
+def test_route_of_no_tokens():
+    assert route(M=0) == 0
+
+
+def test_route_gradient_refuses():
+    ok = [X, X, 0, 16, 4, 16, 2, 0, None, 1, 1.0, X, X, 16]
+    for at, v in ((0, None), (1, None), (2, 5), (3, 8), (6, 0), (7, 9), (11, None), (12, None), (13, 15)):
+        a = list(ok)
+        a[at] = v
+        assert rc("nsb_op_moe_topk_route_bwd", *a) == -1, at
+
+
+def test_dispatch_refuses():
+    ok = [X, 4, 2, 8, 128, X, X, X, X]
+    for at, v in ((0, None), (1, -1), (2, 0), (2, 33), (3, 0), (3, 1025), (4, 0), (5, None), (6, None), (7, None), (8, None)):
+        a = list(ok)
+        a[at] = v
+        assert rc("nsb_op_moe_dispatch", *a) == -1, at
+    assert rc("nsb_op_moe_dispatch", X, 2 ** 30, 2, 8, 128, X, X, X, X) == -2
+
+
+@pytest.mark.parametrize("M,k,E,align,rows", [(3, 2, 8, 1, 6), (3, 2, 8, 128, 768), (100, 2, 8, 128, 1280),
+                                              (0, 2, 8, 128, 0), (1, 1, 8, 16, 16)])
+def test_dispatch_rows(M, k, E, align, rows):
+    got = ops.moe_dispatch_rows(M, k, E, align)
+    assert got % align == 0 and got >= M * k
+    assert got == rows
+
+
+def test_combine_refuses():
+    ok = [X, 0, 64, X, X, 4, 2, 64, X, 64]
+    for at, v in ((0, None), (1, 3), (2, 63), (3, None), (5, -1), (6, 0), (6, 33), (7, 0), (8, None), (9, 63)):
+        a = list(ok)
+        a[at] = v
+        assert rc("nsb_op_moe_combine", *a) == -1, at
+    ok = [X, X, 0, 64, 64, X, X, X, 4, 2, 8, 64, X, 64, X]
+    for at, v in ((0, None), (1, None), (2, 3), (3, 63), (4, 63), (5, None), (6, None), (8, -1), (9, 0), (10, -1), (11, 0),
+                  (12, None), (13, 63)):
+        a = list(ok)
+        a[at] = v
+        assert rc("nsb_op_moe_combine_bwd", *a) == -1, at
+
+
+def test_quantize_refuses():
+    ok = [X, 0, 64, 4, 64, 0, None, 1, X, 64, X, 4, X, 16, X, 64]
+    for at, v in ((0, None), (1, 2), (2, 63), (3, -1), (4, 0), (5, 8), (5, -1), (8, X + 8), (9, 48), (9, 72), (10, None),
+                  (11, 3), (12, X + 1), (13, 8), (14, None), (15, 63)):
+        a = list(ok)
+        a[at] = v
+        assert rc("nsb_op_fp8_quantize", *a) == -1, at
+    a = list(ok)
+    a[6], a[7] = X, -1
+    assert rc("nsb_op_fp8_quantize", *a) == -1
+    a = list(ok)
+    a[8] = a[12] = None
+    assert rc("nsb_op_fp8_quantize", *a) == -1
+    ok = [X, 0, 300, 200, 300, X, 304, X, 3, X, 208, X, 2]
+    for at, v in ((0, None), (1, 7), (2, 299), (4, 0), (6, 288), (7, None), (8, 2), (10, 192), (11, None), (12, 1)):
+        a = list(ok)
+        a[at] = v
+        assert rc("nsb_op_fp8_quantize_block", *a) == -1, at
+
+
+def test_products_refuse():
+    ok = [4, 200, 300, X, 304, X, 4, X, 304, X, 3, 0, X, 0, 200, None]
+    for at, v in ((0, -1), (1, -1), (2, -1), (3, None), (3, X + 4), (4, 288), (4, 308), (5, None), (6, 3), (7, None),
+                  (7, X + 8), (8, 300), (9, None), (10, 2), (12, None), (13, 2), (14, 199)):
+        a = list(ok)
+        a[at] = v
+        assert rc("nsb_op_gemm_fp8", *a) == -1, at
+    a = list(ok)
+    a[11], a[10] = 1, 199  # row scales
+    assert rc("nsb_op_gemm_fp8", *a) == -1
+    ok = [8, 4, 200, 300, X, 304, 8, X, 8, None, 1, X, X, X, 304, 304 * 200, X, 3, 6, X, 0, 200, None]
+    for at, v in ((1, 0), (4, None), (5, 300), (6, 7), (8, 7), (11, None), (12, None), (13, None), (15, 8), (17, 2), (19, None),
+                  (21, 199)):
+        a = list(ok)
+        a[at] = v
+        assert rc("nsb_op_moe_gemm_fp8", *a) == -1, at
+    a = list(ok)
+    a[1] = 1025
+    assert rc("nsb_op_moe_gemm_fp8", *a) == -2
+    a = list(ok)
+    a[9], a[10] = X, 0
+    assert rc("nsb_op_moe_gemm_fp8", *a) == -1
+    ok = [64, 48, 256, 4, X, 256, X, 64, X, 256, X, 48, X, X, X, 0, 48, 64 * 48, None]
+    for at, v in ((3, 0), (4, None), (5, 240), (7, 63), (8, None), (11, 47), (12, None), (13, None), (14, None), (16, 47)):
+        a = list(ok)
+        a[at] = v
+        assert rc("nsb_op_moe_wgrad_fp8", *a) == -1, at
+
+
+def test_products_of_nothing():
+    assert rc("nsb_op_gemm_fp8", 0, 200, 300, X, 304, X, 4, X, 304, X, 3, 0, X, 0, 200, None) == 0
+    assert rc("nsb_op_gemm_fp8", 4, 0, 300, X, 304, X, 4, X, 304, X, 3, 0, X, 0, 200, None) == 0
