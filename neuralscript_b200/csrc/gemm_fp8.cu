@@ -2,87 +2,442 @@
 // (no counterpart in the reference):
 //
 //   C[m,n] = sum over blocks b of 128 k of  sa(m,b) sb(n,b) sum_k A[m,k] B[n,k]
+//
+// The tensor cores sum a block's 128 exact products in fp32 (tcgen05
+// kind::f8f6f4, accumulators in TMEM); the scales vary from block to block, so
+// every block's sum is read back from TMEM, scaled and added to an fp32
+// accumulator in registers, while the tensor cores work on the next block in
+// another part of TMEM.
+#include <cuda.h>
 #include <cuda_fp8.h>
+#include <string.h>
+
+#include <mutex>
 
 #include "fp8.h"
 #include "gemm.h"
+#include "ptx.cuh"
 
 namespace nsb {
 
 namespace {
 
-__device__ __forceinline__ float value(uint8_t c) {
-    __nv_fp8_e4m3 t;
-    t.__x = c;
-    return (float)t;
+// ---------------------------------------------------------------------------
+// 128 x BN tiles, one persistent CTA an SM
+//   warp 0       TMA producer into a ring of stages (128 x 128 codes of A,
+//                BN x 128 of B, 128-byte swizzle)
+//   warp 1       MMA issuer: one k-block's product into one of TMEM's parts
+//   warps 4..11  a warp owns 32 rows and half the columns: scales and adds
+//                every k-block's part, stores the tile
+// The accumulators of a 128 x 256 tile are 128 registers a thread, so the
+// first four warps give theirs up: 56 + 2 * 224 of the 3 * 168 registers that
+// the three warpgroups are launched with.
+// ---------------------------------------------------------------------------
+struct TileParams {
+    int M, N, K;
+    const float* sa;
+    long long ld_sa;
+    const float* sb;
+    long long ld_sb, sb_stride;
+    void* c;
+    int c_dtype;
+    long long ldc, c_stride;
+    int groups;  // row groups (ROWS) or k groups; 0: one product
+    const int* offsets;
+    const int* counts;
+    const int* rows;
+    int row_div;
+    int m_tiles, n_tiles, nb;  // nb: 128-wide scale blocks along N
+    int tma_out, vec_out;
+    int* err;
+};
+
+constexpr int kBand = 16;  // n tiles whose m tiles run together
+constexpr int kEpi = 8;
+constexpr int kThreads = 128 + 32 * kEpi;
+constexpr int kMaxGroups = 1024;
+
+template <int BN, bool VEC, bool ROWS>
+struct TileCfg {
+    static constexpr int A_BYTES = 128 * 128;
+    static constexpr int STAGE = A_BYTES + BN * 128;
+    static constexpr int STAGES = BN == 256 ? 4 : 6;
+    static constexpr int PARTS = 512 / BN;   // TMEM parts
+    static constexpr int COLS = BN / 2;      // columns of a warp
+    static constexpr int NSTG = VEC || ROWS ? 1 : 2;  // output staging buffers of 2 KB a warp
+    static constexpr int STAGING = kEpi * NSTG * 2048;
+    static constexpr int VECS = VEC ? kEpi * 2 * COLS * 4 : 0;
+    static constexpr int TABLE = ROWS ? (kMaxGroups + 1) * 4 : 0;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + VECS + 256 + TABLE;
+    static_assert(SMEM <= 227 * 1024, "above the shared memory of a block");
+};
+
+struct Unit {
+    int g, m0, row_end, n0, kb0, kb1;
+};
+
+// Tile u of the work: tiles of a group run along n first, those of a single
+// product in bands of kBand n tiles, so that tiles in flight share operands.
+template <int BN, bool ROWS>
+__device__ __forceinline__ Unit unit_at(const TileParams& p, const int* start, int u) {
+    Unit w;
+    if (ROWS) {
+        int t = u / p.n_tiles;
+        int lo = 0, hi = p.groups;  // start[lo] <= t < start[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (start[mid] <= t) lo = mid;
+            else hi = mid;
+        }
+        w.g = lo;
+        const int off = p.offsets[lo];
+        w.m0 = off + (t - start[lo]) * 128;
+        w.row_end = min(p.M, off + p.counts[lo]);
+        w.n0 = u % p.n_tiles * BN;
+        w.kb0 = 0;
+        w.kb1 = (p.K + 127) / 128;
+        return w;
+    }
+    const int tiles = p.m_tiles * p.n_tiles;
+    w.g = u / tiles;
+    u -= w.g * tiles;
+    const int band = u / (kBand * p.m_tiles);
+    u -= band * kBand * p.m_tiles;
+    const int width = min(kBand, p.n_tiles - band * kBand);
+    w.m0 = u / width * 128;
+    w.n0 = (band * kBand + u % width) * BN;
+    w.row_end = p.M;
+    w.kb0 = 0;
+    w.kb1 = (p.K + 127) / 128;
+    if (p.groups) {
+        const int off = p.offsets[w.g];
+        w.kb0 = off / 128;
+        w.kb1 = min(w.kb1, (off + p.counts[w.g] + 127) / 128);
+    }
+    return w;
 }
 
-// 64 x 64 outputs a block of 256 threads, blocks of 128 k summed apart.
-__global__ void __launch_bounds__(256) fp8_simple_kernel(const Fp8Gemm d) {
-    __shared__ float As[16][65], Bs[16][65];
-    const int g = blockIdx.z;
-    int m0 = blockIdx.y * 64, m_end = d.M;
-    long long k0 = 0, k1 = d.K;
-    const uint8_t* b = d.b;
-    const float* sb = d.sb;
-    char* c = reinterpret_cast<char*>(d.c);
-    if (d.groups && d.group_k) {
-        k0 = d.offsets[g];
-        k1 = min((long long)d.K, k0 + d.counts[g]);
-        c += g * d.c_stride * (d.c_dtype == kBF16 ? 2 : 4);
-    } else if (d.groups) {
-        m0 += d.offsets[g];
-        m_end = min(d.M, d.offsets[g] + d.counts[g]);
-        b += g * d.b_stride;
-        sb += g * d.sb_stride;
-    }
-    if (m0 >= m_end) return;
-    const int n0 = blockIdx.x * 64, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    float acc[4][4] = {};
-    for (long long kb = k0 / 128; kb * 128 < k1; kb++) {
-        float part[4][4] = {};
-        for (int ks = 0; ks < 128; ks += 16) {
-            for (int e = threadIdx.x; e < 1024; e += 256) {
-                const int kk = e % 16, i = e / 16;
-                const long long k = kb * 128 + ks + kk;
-                const int m = m0 + i, n = n0 + i;
-                long long am = m;
-                if (d.rows && m < m_end) am = d.rows[m] < 0 ? -1 : d.rows[m] / d.row_div;
-                As[kk][i] = m < m_end && k < k1 && am >= 0 ? value(d.a[am * d.lda + k]) : 0.f;
-                Bs[kk][i] = n < d.N && k < k1 ? value(b[(long long)n * d.ldb + k]) : 0.f;
-            }
-            __syncthreads();
-            for (int kk = 0; kk < 16; kk++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) part[i][j] = fmaf(As[kk][ty + 16 * i], Bs[kk][tx + 16 * j], part[i][j]);
-            __syncthreads();
+template <int BN, bool VEC, bool ROWS>
+__global__ void __launch_bounds__(kThreads, 1)
+    fp8_tile_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
+                    const __grid_constant__ CUtensorMap tc, const TileParams p) {
+    using C = TileCfg<BN, VEC, ROWS>;
+    constexpr uint32_t IDESC = ptx::instr_desc(0, 0, 0, 128, BN);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* staging = smem + C::STAGES * C::STAGE;
+    float* vecs = reinterpret_cast<float*>(staging + C::STAGING);
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + C::STAGING + C::VECS);
+    uint64_t* empty = full + C::STAGES;
+    uint64_t* part_full = empty + C::STAGES;
+    uint64_t* part_empty = part_full + C::PARTS;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(part_empty + C::PARTS);
+    int* total_slot = reinterpret_cast<int*>(tmem_slot + 1);
+    int* start = reinterpret_cast<int*>(staging + C::STAGING + C::VECS + 256);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; s++) {
+            ptx::mbar_init(&full[s], 1);
+            ptx::mbar_init(&empty[s], 1);
         }
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-                if (m >= m_end || n >= d.N) continue;
-                long long am = m;
-                if (d.rows) am = d.rows[m] < 0 ? -1 : d.rows[m] / d.row_div;
-                if (am < 0) continue;
-                const float s = d.sa[kb * d.ld_sa + am] *
-                                (d.b_rows ? sb[kb * d.ld_sb + n] : sb[(long long)(n / 128) * d.ld_sb + kb]);
-                acc[i][j] = fmaf(part[i][j], s, acc[i][j]);
-            }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-            if (m >= m_end || n >= d.N) continue;
-            const size_t at = (size_t)m * d.ldc + n;
-            if (d.c_dtype == kBF16) reinterpret_cast<__nv_bfloat16*>(c)[at] = f2bf(acc[i][j]);
-            else reinterpret_cast<float*>(c)[at] = acc[i][j];
+        for (int s = 0; s < C::PARTS; s++) {
+            ptx::mbar_init(&part_full[s], 1);
+            ptx::mbar_init(&part_empty[s], kEpi);
         }
+        ptx::fence_mbar_init();
+        ptx::prefetch_tmap(&ta);
+        ptx::prefetch_tmap(&tb);
+        if (p.tma_out) ptx::prefetch_tmap(&tc);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc(tmem_slot, 512);
+        ptx::tmem_relinquish();
+    }
+    if (ROWS && warp == 4) {  // first tile of every group
+        int run = 0;
+        for (int g0 = 0; g0 < p.groups; g0 += 32) {
+            const int g = g0 + lane;
+            int n = 0;
+            if (g < p.groups) n = (max(0, min(p.counts[g], p.M - p.offsets[g])) + 127) / 128;
+            int inc = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int t = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += t;
+            }
+            if (g < p.groups) start[g] = run + inc - n;
+            run += __shfl_sync(0xffffffffu, inc, 31);
+        }
+        if (lane == 0) {
+            start[p.groups] = run;
+            *total_slot = run * p.n_tiles;
+        }
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int total = ROWS ? *total_slot : p.m_tiles * p.n_tiles * (p.groups ? p.groups : 1);
+
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        bool alive = true;
+        for (int u = blockIdx.x; alive && u < total; u += gridDim.x) {
+            const Unit w = unit_at<BN, ROWS>(p, start, u);
+            int4 src = make_int4(0, 0, 0, 0);  // this lane's four rows of A (gathered)
+            if (ROWS && p.rows) {
+                int* s4 = reinterpret_cast<int*>(&src);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int m = w.m0 + lane * 4 + i;
+                    // rows past the group's end read row 0 and are not stored
+                    s4[i] = m < w.row_end ? max(0, p.rows[m]) / p.row_div : 0;
+                }
+            }
+            for (int kb = w.kb0; kb < w.kb1; kb++) {
+                uint8_t* sa = smem + stage * C::STAGE;
+                if (ROWS && p.rows) {
+                    if (!__all_sync(0xffffffffu, ptx::mbar_wait(&empty[stage], phase ^ 1, p.err, kErrTimeoutProducer))) {
+                        alive = false;
+                        break;
+                    }
+                    if (lane == 0) ptx::mbar_arrive_expect_tx(&full[stage], C::STAGE);
+                    __syncwarp();
+                    ptx::tma_gather4(sa + lane * 512, &ta, &full[stage], kb * 128, src);
+                    if (lane == 0) ptx::tma_load_3d(sa + C::A_BYTES, &tb, &full[stage], kb * 128, w.n0, w.g);
+                } else if (lane == 0) {
+                    if (!ptx::mbar_wait(&empty[stage], phase ^ 1, p.err, kErrTimeoutProducer)) {
+                        alive = false;
+                        break;
+                    }
+                    ptx::mbar_arrive_expect_tx(&full[stage], C::STAGE);
+                    ptx::tma_load_2d(sa, &ta, &full[stage], kb * 128, w.m0);
+                    ptx::tma_load_3d(sa + C::A_BYTES, &tb, &full[stage], kb * 128, w.n0, ROWS ? w.g : 0);
+                }
+                if (++stage == C::STAGES) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+        }
+        __syncwarp();
+        // every load has landed and been used before the CTA exits (bounded)
+        if (lane == 0)
+            for (int s = 0; s < C::STAGES; s++) {
+                ptx::mbar_wait(&empty[stage], phase ^ 1, p.err, kErrTimeoutProducer);
+                if (++stage == C::STAGES) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int stage = 0, part = 0;
+            uint32_t phase = 0, part_phase = 0;
+            bool alive = true;
+            for (int u = blockIdx.x; alive && u < total; u += gridDim.x) {
+                const Unit w = unit_at<BN, ROWS>(p, start, u);
+                for (int kb = w.kb0; kb < w.kb1; kb++) {
+                    if (!ptx::mbar_wait(&part_empty[part], part_phase ^ 1, p.err, kErrTimeoutMma) ||
+                        !ptx::mbar_wait(&full[stage], phase, p.err, kErrTimeoutMma)) {
+                        alive = false;
+                        break;
+                    }
+                    ptx::tc_fence_after();
+                    const uint32_t sa = ptx::smem_u32(smem + stage * C::STAGE), sb = sa + C::A_BYTES;
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        ptx::mma_f8(tmem + part * BN, ptx::smem_desc(sa + k * 32, 16, 1024, 2),
+                                    ptx::smem_desc(sb + k * 32, 16, 1024, 2), IDESC, k > 0);
+                    ptx::mma_commit(&empty[stage]);
+                    ptx::mma_commit(&part_full[part]);
+                    if (++stage == C::STAGES) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                    if (++part == C::PARTS) {
+                        part = 0;
+                        part_phase ^= 1;
+                    }
+                }
+            }
+        }
+    }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        uint8_t* stg = staging + (warp - 4) * C::NSTG * 2048;
+        float* vec = vecs + (warp - 4) * 2 * C::COLS;
+        int part = 0, buf = 0;
+        uint32_t part_phase = 0;
+        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + half * C::COLS;
+        for (int u = blockIdx.x; u < total; u += gridDim.x) {
+            const Unit w = unit_at<BN, ROWS>(p, start, u);
+            const int row = w.m0 + quarter * 32 + lane;
+            const bool valid = row < w.row_end;
+            int arow = valid ? row : 0;
+            if (ROWS && p.rows && valid) arow = max(0, p.rows[row]) / p.row_div;
+            const int col0 = w.n0 + half * C::COLS;
+            const float* sa = p.sa + arow;
+            const float* sb = p.sb;
+            if (!VEC) sb += (ROWS ? w.g * p.sb_stride : 0) + min(col0 / 128, p.nb - 1) * p.ld_sb;
+            uint64_t acc[C::COLS / 2];
+#pragma unroll
+            for (int j = 0; j < C::COLS / 2; j++) acc[j] = 0;
+            float s_row = 0.f, s_blk = 0.f, s_col[C::COLS / 32];
+            auto fetch = [&](int kb) {
+                s_row = __ldg(sa + kb * p.ld_sa);
+                if (VEC) {
+#pragma unroll
+                    for (int i = 0; i < C::COLS / 32; i++) {
+                        const int n = col0 + i * 32 + lane;
+                        s_col[i] = n < p.N ? __ldg(sb + kb * p.ld_sb + n) : 0.f;
+                    }
+                } else {
+                    s_blk = __ldg(sb + kb);
+                }
+            };
+            if (w.kb0 < w.kb1) fetch(w.kb0);
+            bool alive = true;
+            for (int kb = w.kb0; kb < w.kb1; kb++) {
+                const float s = VEC ? s_row : s_row * s_blk;
+                const uint64_t s2 = f2_pack(s, s);
+                float* v = vec + (kb & 1) * C::COLS;
+                if (VEC) {
+#pragma unroll
+                    for (int i = 0; i < C::COLS / 32; i++) v[i * 32 + lane] = s_col[i];
+                    __syncwarp();
+                }
+                if (kb + 1 < w.kb1) fetch(kb + 1);
+                if (!ptx::mbar_wait(&part_full[part], part_phase, p.err, kErrTimeoutEpilogue)) alive = false;
+                alive = __all_sync(0xffffffffu, alive);
+                if (!alive) break;
+                ptx::tc_fence_after();
+                const uint32_t t = lane_base + part * BN;
+                uint32_t r[2][32];
+                ptx::tmem_ld32(t, r[0]);
+#pragma unroll
+                for (int c = 0; c < C::COLS / 32; c++) {
+                    ptx::tmem_ld_wait_regs32(r[c & 1]);
+                    if (c + 1 < C::COLS / 32) ptx::tmem_ld32(t + (c + 1) * 32, r[(c + 1) & 1]);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        const uint64_t x =
+                            f2_pack(__uint_as_float(r[c & 1][2 * j]), __uint_as_float(r[c & 1][2 * j + 1]));
+                        if (VEC) {
+                            const uint64_t m = reinterpret_cast<const uint64_t*>(v)[c * 16 + j];
+                            acc[c * 16 + j] = f2_fma(x, f2_mul(m, s2), acc[c * 16 + j]);
+                        } else {
+                            acc[c * 16 + j] = f2_fma(x, s2, acc[c * 16 + j]);
+                        }
+                    }
+                }
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&part_empty[part]);
+                if (++part == C::PARTS) {
+                    part = 0;
+                    part_phase ^= 1;
+                }
+            }
+            if (!alive) break;
+            // a slab of 32 rows leaves by TMA where all of them are the tile's
+            // (the store clips at the tensor's end), else row by row
+            const int y = w.m0 + quarter * 32;
+            const int gz = ROWS ? 0 : w.g;
+            const bool tma = p.tma_out && (!ROWS || y + 32 <= w.row_end);
+#pragma unroll
+            for (int c = 0; c < C::COLS / 32; c++) {
+                const int col = col0 + c * 32;
+                if (col >= p.N) continue;
+                float f[32];
+#pragma unroll
+                for (int j = 0; j < 16; j++) f2_unpack(acc[c * 16 + j], f[2 * j], f[2 * j + 1]);
+                if (tma) {
+                    if (y >= p.M) continue;
+                    const int boxes = p.c_dtype == kBF16 ? 1 : 2;
+#pragma unroll
+                    for (int b = 0; b < 2; b++) {
+                        const int x = col + b * 16;
+                        if (b >= boxes || (b && x >= p.N)) continue;
+                        uint8_t* dst = stg + buf * 2048;
+                        if (lane == 0) {
+                            if (C::NSTG == 2) ptx::bulk_wait_read1();
+                            else ptx::bulk_wait_read0();
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            uint4 o;
+                            if (p.c_dtype == kBF16) {
+                                __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&o);
+#pragma unroll
+                                for (int i = 0; i < 4; i++) h[i] = __floats2bfloat162_rn(f[8 * q + 2 * i], f[8 * q + 2 * i + 1]);
+                            } else {
+                                o = make_uint4(__float_as_uint(f[16 * b + 4 * q]), __float_as_uint(f[16 * b + 4 * q + 1]),
+                                               __float_as_uint(f[16 * b + 4 * q + 2]),
+                                               __float_as_uint(f[16 * b + 4 * q + 3]));
+                            }
+                            *reinterpret_cast<uint4*>(dst + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = o;
+                        }
+                        ptx::fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            ptx::tma_store_3d(&tc, dst, x, y, gz);
+                            ptx::bulk_commit();
+                        }
+                        if (C::NSTG == 2) buf ^= 1;
+                    }
+                } else if (valid) {
+                    const size_t at = (size_t)gz * p.c_stride + (size_t)row * p.ldc + col;
+                    const bool vec16 = p.vec_out && col + 32 <= p.N;
+                    if (p.c_dtype == kBF16) {
+                        __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(p.c) + at;
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            uint4 t;
+                            __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&t);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) h[i] = __floats2bfloat162_rn(f[8 * q + 2 * i], f[8 * q + 2 * i + 1]);
+                            if (vec16) {
+                                reinterpret_cast<uint4*>(o)[q] = t;
+                            } else {
+                                const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&t);
+#pragma unroll
+                                for (int i = 0; i < 8; i++)
+                                    if (col + 8 * q + i < p.N) o[8 * q + i] = e[i];
+                            }
+                        }
+                    } else {
+                        float* o = reinterpret_cast<float*>(p.c) + at;
+#pragma unroll
+                        for (int q = 0; q < 8; q++) {
+                            if (vec16) {
+                                reinterpret_cast<float4*>(o)[q] = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 4; i++)
+                                    if (col + 4 * q + i < p.N) o[4 * q + i] = f[4 * q + i];
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        if (lane == 0) ptx::bulk_wait_all();
+        __syncwarp();
+    }
+
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem, 512);
+    }
 }
 
 __global__ void fp8_zero_kernel(const Fp8Gemm d) {
@@ -92,6 +447,124 @@ __global__ void fp8_zero_kernel(const Fp8Gemm d) {
         if (d.c_dtype == kBF16) reinterpret_cast<__nv_bfloat16*>(d.c)[at] = f2bf(0.f);
         else reinterpret_cast<float*>(d.c)[at] = 0.f;
     }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encoder() {
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(f);
+    });
+    return fn;
+}
+
+// Codes [rows, cols] with ld bytes a row: boxes of 128 columns and box rows.
+bool map_codes2(CUtensorMap* m, const void* p, long long cols, long long rows, long long ld, int box) {
+    EncodeTiledFn enc = encoder();
+    if (!enc) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld};
+    cuuint32_t boxes[2] = {128, (cuuint32_t)box}, one[2] = {1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, boxes, one,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The same, one such array for each of z groups, stride bytes apart.
+bool map_codes3(CUtensorMap* m, const void* p, long long cols, long long rows, long long ld, long long z,
+                long long stride, int box) {
+    EncodeTiledFn enc = encoder();
+    if (!enc) return false;
+    cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)z};
+    cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)(z > 1 ? stride : ld * rows)};
+    cuuint32_t boxes[3] = {128, (cuuint32_t)box, 1}, one[3] = {1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(p), dims, strides, boxes, one,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Output boxes of 32 rows x 64 bytes, 64-byte swizzle.
+bool map_out(CUtensorMap* m, void* p, int dtype, long long cols, long long rows, long long ld, long long z,
+             long long stride) {
+    EncodeTiledFn enc = encoder();
+    if (!enc) return false;
+    const int es = dtype == kBF16 ? 2 : 4;
+    cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)z};
+    cuuint64_t strides[2] = {(cuuint64_t)(ld * es), (cuuint64_t)((z > 1 ? stride : ld * rows) * es)};
+    cuuint32_t boxes[3] = {(cuuint32_t)(64 / es), 32, 1}, one[3] = {1, 1, 1};
+    return enc(m, dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, p, dims,
+               strides, boxes, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The attribute belongs to the current device: set once for each.
+template <typename Kernel>
+bool allow_smem(Kernel k, int bytes, bool* done) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return false;
+    if (!done[dev]) {
+        if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+        done[dev] = true;
+    }
+    return true;
+}
+
+template <int BN, bool VEC, bool ROWS>
+int launch_tiles(const Fp8Gemm& d, cudaStream_t st) {
+    using C = TileCfg<BN, VEC, ROWS>;
+    static bool done[kMaxDevices] = {};
+    auto k = fp8_tile_kernel<BN, VEC, ROWS>;
+    if (!allow_smem(k, C::SMEM, done)) return -5;
+    const int es = d.c_dtype == kBF16 ? 2 : 4;
+    const bool aligned = !(reinterpret_cast<uintptr_t>(d.c) & 15) && d.ldc * es % 16 == 0 && d.c_stride * es % 16 == 0;
+    TileParams p;
+    p.M = d.M;
+    p.N = d.N;
+    p.K = d.K;
+    p.sa = d.sa;
+    p.ld_sa = d.ld_sa;
+    p.sb = d.sb;
+    p.ld_sb = d.ld_sb;
+    p.sb_stride = d.sb_stride;
+    p.c = d.c;
+    p.c_dtype = d.c_dtype;
+    p.ldc = d.ldc;
+    p.c_stride = d.c_stride;
+    p.groups = d.groups;
+    p.offsets = d.offsets;
+    p.counts = d.counts;
+    p.rows = d.rows;
+    p.row_div = d.row_div;
+    p.m_tiles = (d.M + 127) / 128;
+    p.n_tiles = (d.N + BN - 1) / BN;
+    p.nb = (d.N + 127) / 128;
+    p.vec_out = aligned;
+    p.err = d.err;
+    CUtensorMap ta, tb, tc;
+    memset(&tc, 0, sizeof(tc));
+    if (!map_codes2(&ta, d.a, d.K, d.a_rows, d.lda, d.rows ? 1 : 128)) return -2;
+    if (!map_codes3(&tb, d.b, d.K, d.N, d.ldb, ROWS ? d.groups : 1, d.b_stride, BN)) return -2;
+    // a TMA store clips rows to whole 16-byte pieces, so ragged ones go another way
+    p.tma_out = aligned && (long long)d.N * es % 16 == 0 &&
+                map_out(&tc, d.c, d.c_dtype, d.N, d.M, d.ldc, d.group_k ? d.groups : 1, d.c_stride);
+    long long units = (long long)p.m_tiles * p.n_tiles;
+    if (ROWS) units = ((long long)p.m_tiles + d.groups) * p.n_tiles;  // at most
+    else if (d.groups) units *= d.groups;
+    if (units > 0x7fffffff) return -2;
+    const int sms = num_sms();
+    k<<<(unsigned)(units < sms ? units : sms), kThreads, C::SMEM, st>>>(ta, tb, tc, p);
+    return cudaGetLastError() == cudaSuccess ? 0 : -5;
 }
 
 }  // namespace
@@ -114,9 +587,9 @@ int fp8_gemm(const Fp8Gemm& d, cudaStream_t st) {
     if (d.ld_sa < d.a_rows || d.ld_sb < (d.b_rows ? d.N : kb)) return -1;
     if (d.groups && (!d.offsets || !d.counts)) return -1;
     if (d.rows && d.row_div <= 0) return -1;
-    const dim3 grid((d.N + 63) / 64, (d.M + 63) / 64, d.groups ? d.groups : 1);
-    fp8_simple_kernel<<<grid, 256, 0, st>>>(d);
-    return cudaGetLastError() == cudaSuccess ? 0 : -5;
+    if (d.a_rows <= 0) return -1;
+    if (d.groups && !d.group_k) return launch_tiles<256, false, true>(d, st);
+    return d.b_rows ? launch_tiles<256, true, false>(d, st) : launch_tiles<256, false, false>(d, st);
 }
 
 }  // namespace nsb
