@@ -27,6 +27,10 @@ namespace {
 //   warp 0       TMA producer into a ring of stages (128 x 128 codes of A,
 //                BN x 128 of B, 128-byte swizzle)
 //   warp 1       MMA issuer: one k-block's product into one of TMEM's parts
+//   warps 2..3   copy the k-blocks' scales into a ring of their own, deep
+//                enough to cover a read from DRAM; with a row list also the
+//                rows of A (16-byte cp.async in the swizzled order; TMA's
+//                four-row gather took 2700 cycles for 128 rows)
 //   warps 4..11  a warp owns 32 rows and half the columns: scales and adds
 //                every k-block's part, stores the tile
 // The accumulators of a 128 x 256 tile are 128 registers a thread, so the
@@ -35,6 +39,9 @@ namespace {
 // ---------------------------------------------------------------------------
 struct TileParams {
     int M, N, K;
+    const uint8_t* a;
+    long long lda;
+    int a_rows;
     const float* sa;
     long long ld_sa;
     const float* sb;
@@ -56,6 +63,8 @@ constexpr int kBand = 16;  // n tiles whose m tiles run together
 constexpr int kEpi = 8;
 constexpr int kThreads = 128 + 32 * kEpi;
 constexpr int kMaxGroups = 1024;
+constexpr int kSlots = 8;  // k-blocks of scales in flight
+constexpr int kLag = 2;    // k-blocks of gathered rows in flight before the oldest is waited for
 
 template <int BN, bool VEC, bool ROWS>
 struct TileCfg {
@@ -64,11 +73,11 @@ struct TileCfg {
     static constexpr int STAGES = BN == 256 ? 4 : 6;
     static constexpr int PARTS = 512 / BN;   // TMEM parts
     static constexpr int COLS = BN / 2;      // columns of a warp
-    static constexpr int NSTG = VEC || ROWS ? 1 : 2;  // output staging buffers of 2 KB a warp
-    static constexpr int STAGING = kEpi * NSTG * 2048;
-    static constexpr int VECS = VEC ? kEpi * 2 * COLS * 4 : 0;
+    static constexpr int STAGING = kEpi * 2048;  // 32 rows x 64 bytes a warp
+    static constexpr int SLOT = 128 + (VEC ? BN : 2);  // row scales, then column or block scales
+    static constexpr int SCALES = kSlots * SLOT * 4;
     static constexpr int TABLE = ROWS ? (kMaxGroups + 1) * 4 : 0;
-    static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + VECS + 256 + TABLE;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + SCALES + 512 + TABLE;
     static_assert(SMEM <= 227 * 1024, "above the shared memory of a block");
 };
 
@@ -126,20 +135,26 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* staging = smem + C::STAGES * C::STAGE;
-    float* vecs = reinterpret_cast<float*>(staging + C::STAGING);
-    uint64_t* full = reinterpret_cast<uint64_t*>(staging + C::STAGING + C::VECS);
+    float* slots = reinterpret_cast<float*>(staging + C::STAGING);
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + C::STAGING + C::SCALES);
     uint64_t* empty = full + C::STAGES;
     uint64_t* part_full = empty + C::STAGES;
     uint64_t* part_empty = part_full + C::PARTS;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(part_empty + C::PARTS);
+    uint64_t* slot_full = part_empty + C::PARTS;
+    uint64_t* slot_empty = slot_full + kSlots;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(slot_empty + kSlots);
     int* total_slot = reinterpret_cast<int*>(tmem_slot + 1);
-    int* start = reinterpret_cast<int*>(staging + C::STAGING + C::VECS + 256);
+    int* start = reinterpret_cast<int*>(staging + C::STAGING + C::SCALES + 512);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; s++) {
-            ptx::mbar_init(&full[s], 1);
+            ptx::mbar_init(&full[s], ROWS && p.rows ? 3 : 1);
             ptx::mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < kSlots; s++) {
+            ptx::mbar_init(&slot_full[s], 64);
+            ptx::mbar_init(&slot_empty[s], kEpi);
         }
         for (int s = 0; s < C::PARTS; s++) {
             ptx::mbar_init(&part_full[s], 1);
@@ -183,50 +198,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0) {
-        int stage = 0;
-        uint32_t phase = 0;
-        bool alive = true;
-        for (int u = blockIdx.x; alive && u < total; u += gridDim.x) {
-            const Unit w = unit_at<BN, ROWS>(p, start, u);
-            int4 src = make_int4(0, 0, 0, 0);  // this lane's four rows of A (gathered)
-            if (ROWS && p.rows) {
-                int* s4 = reinterpret_cast<int*>(&src);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int m = w.m0 + lane * 4 + i;
-                    // rows past the group's end read row 0 and are not stored
-                    s4[i] = m < w.row_end ? max(0, p.rows[m]) / p.row_div : 0;
-                }
-            }
-            for (int kb = w.kb0; kb < w.kb1; kb++) {
-                uint8_t* sa = smem + stage * C::STAGE;
-                if (ROWS && p.rows) {
-                    if (!__all_sync(0xffffffffu, ptx::mbar_wait(&empty[stage], phase ^ 1, p.err, kErrTimeoutProducer))) {
-                        alive = false;
-                        break;
-                    }
-                    if (lane == 0) ptx::mbar_arrive_expect_tx(&full[stage], C::STAGE);
-                    __syncwarp();
-                    ptx::tma_gather4(sa + lane * 512, &ta, &full[stage], kb * 128, src);
-                    if (lane == 0) ptx::tma_load_3d(sa + C::A_BYTES, &tb, &full[stage], kb * 128, w.n0, w.g);
-                } else if (lane == 0) {
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool alive = true;
+            const bool gather = ROWS && p.rows;
+            for (int u = blockIdx.x; alive && u < total; u += gridDim.x) {
+                const Unit w = unit_at<BN, ROWS>(p, start, u);
+                for (int kb = w.kb0; kb < w.kb1; kb++) {
                     if (!ptx::mbar_wait(&empty[stage], phase ^ 1, p.err, kErrTimeoutProducer)) {
                         alive = false;
                         break;
                     }
-                    ptx::mbar_arrive_expect_tx(&full[stage], C::STAGE);
-                    ptx::tma_load_2d(sa, &ta, &full[stage], kb * 128, w.m0);
+                    uint8_t* sa = smem + stage * C::STAGE;
+                    ptx::mbar_arrive_expect_tx(&full[stage], gather ? C::STAGE - C::A_BYTES : C::STAGE);
+                    if (!gather) ptx::tma_load_2d(sa, &ta, &full[stage], kb * 128, w.m0);
                     ptx::tma_load_3d(sa + C::A_BYTES, &tb, &full[stage], kb * 128, w.n0, ROWS ? w.g : 0);
-                }
-                if (++stage == C::STAGES) {
-                    stage = 0;
-                    phase ^= 1;
+                    if (++stage == C::STAGES) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
                 }
             }
-        }
-        __syncwarp();
-        // every load has landed and been used before the CTA exits (bounded)
-        if (lane == 0)
+            // every load has landed and been used before the CTA exits (bounded)
             for (int s = 0; s < C::STAGES; s++) {
                 ptx::mbar_wait(&empty[stage], phase ^ 1, p.err, kErrTimeoutProducer);
                 if (++stage == C::STAGES) {
@@ -234,6 +228,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     phase ^= 1;
                 }
             }
+        }
     } else if (warp == 1) {
         if (lane == 0) {
             int stage = 0, part = 0;
@@ -266,79 +261,153 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         }
+    } else {
+        const int t = threadIdx.x - 64;  // 0..63
+        const bool gather = ROWS && p.rows;
+        int slot = 0, stage = 0, behind = 0, old = 0;
+        uint32_t slot_phase = 0, phase = 0;
+        bool alive = true;
+        for (int u = blockIdx.x; alive && u < total; u += gridDim.x) {
+            const Unit w = unit_at<BN, ROWS>(p, start, u);
+            // the rows whose scales this thread copies; rows past the end
+            // take the first one's, and are not stored
+            const float* srow[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int m = w.m0 + t + 64 * i;
+                const int r = m >= w.row_end ? 0 : gather ? min(max(0, p.rows[m]) / p.row_div, p.a_rows - 1) : m;
+                srow[i] = p.sa + r;
+            }
+            const float* sb = p.sb;
+            if (!VEC) sb += (ROWS ? w.g * p.sb_stride : 0) + (long long)min(w.n0 / 128 + (t & 1) * (BN / 256), p.nb - 1) * p.ld_sb;
+            int arow[16];  // rows of A that this thread copies a 16-byte piece of: t / 8, t / 8 + 8, ...
+            if (gather) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int m = w.m0 + t / 8 + 8 * i;
+                    arow[i] = m < w.row_end ? min(max(0, p.rows[m]) / p.row_div, p.a_rows - 1) : -1;
+                }
+            }
+            for (int kb = w.kb0; kb < w.kb1; kb++) {
+                if (!__all_sync(0xffffffffu,
+                                ptx::mbar_wait(&slot_empty[slot], slot_phase ^ 1, p.err, kErrTimeoutProducer))) {
+                    alive = false;
+                    break;
+                }
+                float* to = slots + slot * C::SLOT;
+#pragma unroll
+                for (int i = 0; i < 2; i++) ptx::cp_async4(to + t + 64 * i, srow[i] + kb * p.ld_sa);
+                if (VEC) {
+#pragma unroll
+                    for (int i = 0; i < BN / 64; i++) {
+                        const int n = w.n0 + t + 64 * i;
+                        if (n < p.N) ptx::cp_async4(to + 128 + t + 64 * i, sb + kb * p.ld_sb + n);
+                    }
+                } else if (t < 2) {
+                    ptx::cp_async4(to + 128 + t, sb + kb);
+                }
+                ptx::cp_async_arrive(&slot_full[slot]);
+                if (++slot == kSlots) {
+                    slot = 0;
+                    slot_phase ^= 1;
+                }
+                if (!gather) continue;
+                if (!__all_sync(0xffffffffu, ptx::mbar_wait(&empty[stage], phase ^ 1, p.err, kErrTimeoutProducer))) {
+                    alive = false;
+                    break;
+                }
+                uint8_t* sa = smem + stage * C::STAGE;
+                const int k = kb * 128 + (t & 7) * 16;
+                const int bytes = max(0, min(16, p.K - k));
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int r = t / 8 + 8 * i;  // r % 8 = t / 8: the swizzle's row
+                    const bool on = arow[i] >= 0 && bytes > 0;
+                    ptx::cp_async16(sa + r * 128 + (((t & 7) ^ (t >> 3)) << 4),
+                                    on ? p.a + (size_t)arow[i] * p.lda + k : p.a, on ? bytes : 0);
+                }
+                ptx::cp_async_commit();
+                if (++stage == C::STAGES) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+                if (behind < kLag) {
+                    behind++;
+                } else {
+                    ptx::cp_async_wait<kLag>();
+                    ptx::fence_proxy_async();  // the tensor cores read through the async proxy
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(&full[old]);
+                    if (++old == C::STAGES) old = 0;
+                }
+            }
+        }
+        ptx::cp_async_wait<0>();
+        if (gather) {
+            ptx::fence_proxy_async();
+            __syncwarp();
+            for (; behind > 0; behind--) {
+                if (lane == 0) ptx::mbar_arrive(&full[old]);
+                if (++old == C::STAGES) old = 0;
+            }
+        }
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int quarter = warp & 3, half = (warp - 4) >> 2;
-        uint8_t* stg = staging + (warp - 4) * C::NSTG * 2048;
-        float* vec = vecs + (warp - 4) * 2 * C::COLS;
-        int part = 0, buf = 0;
-        uint32_t part_phase = 0;
+        uint8_t* stg = staging + (warp - 4) * 2048;
+        int part = 0, slot = 0;
+        uint32_t part_phase = 0, slot_phase = 0;
         const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + half * C::COLS;
         for (int u = blockIdx.x; u < total; u += gridDim.x) {
             const Unit w = unit_at<BN, ROWS>(p, start, u);
             const int row = w.m0 + quarter * 32 + lane;
             const bool valid = row < w.row_end;
-            int arow = valid ? row : 0;
-            if (ROWS && p.rows && valid) arow = max(0, p.rows[row]) / p.row_div;
             const int col0 = w.n0 + half * C::COLS;
-            const float* sa = p.sa + arow;
-            const float* sb = p.sb;
-            if (!VEC) sb += (ROWS ? w.g * p.sb_stride : 0) + min(col0 / 128, p.nb - 1) * p.ld_sb;
             uint64_t acc[C::COLS / 2];
 #pragma unroll
             for (int j = 0; j < C::COLS / 2; j++) acc[j] = 0;
-            float s_row = 0.f, s_blk = 0.f, s_col[C::COLS / 32];
-            auto fetch = [&](int kb) {
-                s_row = __ldg(sa + kb * p.ld_sa);
-                if (VEC) {
-#pragma unroll
-                    for (int i = 0; i < C::COLS / 32; i++) {
-                        const int n = col0 + i * 32 + lane;
-                        s_col[i] = n < p.N ? __ldg(sb + kb * p.ld_sb + n) : 0.f;
-                    }
-                } else {
-                    s_blk = __ldg(sb + kb);
-                }
-            };
-            if (w.kb0 < w.kb1) fetch(w.kb0);
             bool alive = true;
             for (int kb = w.kb0; kb < w.kb1; kb++) {
-                const float s = VEC ? s_row : s_row * s_blk;
+                if (!ptx::mbar_wait(&slot_full[slot], slot_phase, p.err, kErrTimeoutEpilogue)) alive = false;
+                const float* sc = slots + slot * C::SLOT;
+                const float s = VEC ? sc[quarter * 32 + lane] : sc[quarter * 32 + lane] * sc[128 + half];
                 const uint64_t s2 = f2_pack(s, s);
-                float* v = vec + (kb & 1) * C::COLS;
-                if (VEC) {
-#pragma unroll
-                    for (int i = 0; i < C::COLS / 32; i++) v[i * 32 + lane] = s_col[i];
-                    __syncwarp();
-                }
-                if (kb + 1 < w.kb1) fetch(kb + 1);
+                const uint64_t* v = reinterpret_cast<const uint64_t*>(sc + 128 + half * C::COLS);
                 if (!ptx::mbar_wait(&part_full[part], part_phase, p.err, kErrTimeoutEpilogue)) alive = false;
                 alive = __all_sync(0xffffffffu, alive);
                 if (!alive) break;
                 ptx::tc_fence_after();
                 const uint32_t t = lane_base + part * BN;
-                uint32_t r[2][32];
-                ptx::tmem_ld32(t, r[0]);
+                uint32_t r[2][16];
+                ptx::tmem_ld16(t, r[0]);
 #pragma unroll
-                for (int c = 0; c < C::COLS / 32; c++) {
-                    ptx::tmem_ld_wait_regs32(r[c & 1]);
-                    if (c + 1 < C::COLS / 32) ptx::tmem_ld32(t + (c + 1) * 32, r[(c + 1) & 1]);
+                for (int c = 0; c < C::COLS / 16; c++) {
+                    uint64_t m[8];
+                    if (VEC) {
 #pragma unroll
-                    for (int j = 0; j < 16; j++) {
+                        for (int j = 0; j < 8; j++) m[j] = f2_mul(v[c * 8 + j], s2);
+                    }
+                    ptx::tmem_ld_wait_regs16(r[c & 1]);
+                    if (c + 1 < C::COLS / 16) ptx::tmem_ld16(t + (c + 1) * 16, r[(c + 1) & 1]);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        uint64_t& a = acc[c * 8 + j];
                         const uint64_t x =
                             f2_pack(__uint_as_float(r[c & 1][2 * j]), __uint_as_float(r[c & 1][2 * j + 1]));
-                        if (VEC) {
-                            const uint64_t m = reinterpret_cast<const uint64_t*>(v)[c * 16 + j];
-                            acc[c * 16 + j] = f2_fma(x, f2_mul(m, s2), acc[c * 16 + j]);
-                        } else {
-                            acc[c * 16 + j] = f2_fma(x, s2, acc[c * 16 + j]);
-                        }
+                        a = f2_fma(x, VEC ? m[j] : s2, a);
                     }
                 }
                 ptx::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(&part_empty[part]);
+                if (lane == 0) {
+                    ptx::mbar_arrive(&part_empty[part]);
+                    ptx::mbar_arrive(&slot_empty[slot]);
+                }
+                if (++slot == kSlots) {
+                    slot = 0;
+                    slot_phase ^= 1;
+                }
                 if (++part == C::PARTS) {
                     part = 0;
                     part_phase ^= 1;
@@ -364,11 +433,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int b = 0; b < 2; b++) {
                         const int x = col + b * 16;
                         if (b >= boxes || (b && x >= p.N)) continue;
-                        uint8_t* dst = stg + buf * 2048;
-                        if (lane == 0) {
-                            if (C::NSTG == 2) ptx::bulk_wait_read1();
-                            else ptx::bulk_wait_read0();
-                        }
+                        uint8_t* dst = stg;
+                        if (lane == 0) ptx::bulk_wait_read0();
                         __syncwarp();
 #pragma unroll
                         for (int q = 0; q < 4; q++) {
@@ -390,7 +456,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                             ptx::tma_store_3d(&tc, dst, x, y, gz);
                             ptx::bulk_commit();
                         }
-                        if (C::NSTG == 2) buf ^= 1;
                     }
                 } else if (valid) {
                     const size_t at = (size_t)gz * p.c_stride + (size_t)row * p.ldc + col;
@@ -532,6 +597,9 @@ int launch_tiles(const Fp8Gemm& d, cudaStream_t st) {
     p.M = d.M;
     p.N = d.N;
     p.K = d.K;
+    p.a = d.a;
+    p.lda = d.lda;
+    p.a_rows = (int)d.a_rows;
     p.sa = d.sa;
     p.ld_sa = d.ld_sa;
     p.sb = d.sb;
@@ -553,7 +621,7 @@ int launch_tiles(const Fp8Gemm& d, cudaStream_t st) {
     p.err = d.err;
     CUtensorMap ta, tb, tc;
     memset(&tc, 0, sizeof(tc));
-    if (!map_codes2(&ta, d.a, d.K, d.a_rows, d.lda, d.rows ? 1 : 128)) return -2;
+    if (!map_codes2(&ta, d.a, d.K, d.a_rows, d.lda, 128)) return -2;
     if (!map_codes3(&tb, d.b, d.K, d.N, d.ldb, ROWS ? d.groups : 1, d.b_stride, BN)) return -2;
     // a TMA store clips rows to whole 16-byte pieces, so ragged ones go another way
     p.tma_out = aligned && (long long)d.N * es % 16 == 0 &&
