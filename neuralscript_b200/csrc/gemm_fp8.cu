@@ -24,13 +24,15 @@ namespace {
 
 // ---------------------------------------------------------------------------
 // 128 x BN tiles, one persistent CTA an SM
-//   warp 0       TMA producer into a ring of stages (128 x 128 codes of A,
-//                BN x 128 of B, 128-byte swizzle)
-//   warp 1       MMA issuer: one k-block's product into one of TMEM's parts
-//   warps 2..3   copy the k-blocks' scales into a ring of their own, deep
-//                enough to cover a read from DRAM; with a row list also the
-//                rows of A (16-byte cp.async in the swizzled order; TMA's
-//                four-row gather took 2700 cycles for 128 rows)
+//   warps 0, 3   copy: A and B by TMA into a ring of stages (128 x 128 codes
+//                of A, BN x 128 of B, 128-byte swizzle), the k-blocks' scales
+//                into a ring of their own, deep enough to cover a read from
+//                DRAM; with a row list the rows of A by 16-byte cp.async in
+//                the swizzled order (TMA's four-row gather took 2700 cycles
+//                for 128 rows)
+//   warps 1, 2   MMA issuers, each one's k-blocks' products into parts of TMEM
+//                of its own: while one is held up by the tensor cores' queue
+//                or waits for a part, the other's products run
 //   warps 4..11  a warp owns 32 rows and half the columns: scales and adds
 //                every k-block's part, stores the tile
 // The accumulators of a 128 x 256 tile are 128 registers a thread, so the
@@ -63,22 +65,45 @@ constexpr int kBand = 16;  // n tiles whose m tiles run together
 constexpr int kEpi = 8;
 constexpr int kThreads = 128 + 32 * kEpi;
 constexpr int kMaxGroups = 1024;
-constexpr int kSlots = 8;  // k-blocks of scales in flight
-constexpr int kLag = 2;    // k-blocks of gathered rows in flight before the oldest is waited for
+constexpr int kSlots = 4;  // groups of k-blocks whose scales are in flight
 
 template <int BN, bool VEC, bool ROWS>
 struct TileCfg {
     static constexpr int A_BYTES = 128 * 128;
     static constexpr int STAGE = A_BYTES + BN * 128;
     static constexpr int STAGES = BN == 256 ? 4 : 6;
-    static constexpr int PARTS = 512 / BN;   // TMEM parts
+    static constexpr int PARTS = 512 / BN;   // parts of TMEM
     static constexpr int COLS = BN / 2;      // columns of a warp
     static constexpr int STAGING = kEpi * 2048;  // 32 rows x 64 bytes a warp
-    static constexpr int SLOT = 128 + (VEC ? BN : 2);  // row scales, then column or block scales
-    static constexpr int SCALES = kSlots * SLOT * 4;
+    static constexpr int SLOT = 128 + (VEC ? BN : 4);  // a k-block's row scales, then column or block scales
+    static constexpr int SLOTK = VEC ? 2 : 4;  // k-blocks of a group: one wait for all their scales
+    static constexpr int SCALES = kSlots * SLOTK * SLOT * 4;
     static constexpr int TABLE = ROWS ? (kMaxGroups + 1) * 4 : 0;
     static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + SCALES + 512 + TABLE;
     static_assert(SMEM <= 227 * 1024, "above the shared memory of a block");
+};
+
+// Waits of the pipeline. A wait that runs out of time records the error and
+// raises the CTA's flag; from then on no wait of the CTA lasts, so every role
+// runs to its end (on stale data) without having to leave its loops.
+struct Pipe {
+    volatile int* dead;
+    int* err;
+    int code;
+    __device__ __forceinline__ void slow(uint64_t* bar, uint32_t parity) const {
+        const long long t0 = clock64();
+        while (!ptx::mbar_try_wait(bar, parity)) {
+            if (*dead) return;
+            if (clock64() - t0 > ptx::kWaitCycles) {
+                *dead = 1;
+                if (err) atomicCAS(err, 0, code);
+                return;
+            }
+        }
+    }
+    __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity) const {
+        if (!ptx::mbar_try_wait(bar, parity)) slow(bar, parity);
+    }
 };
 
 struct Unit {
@@ -144,12 +169,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* slot_empty = slot_full + kSlots;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(slot_empty + kSlots);
     int* total_slot = reinterpret_cast<int*>(tmem_slot + 1);
+    int* dead = total_slot + 1;
     int* start = reinterpret_cast<int*>(staging + C::STAGING + C::SCALES + 512);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
+        *dead = 0;
         for (int s = 0; s < C::STAGES; s++) {
-            ptx::mbar_init(&full[s], ROWS && p.rows ? 3 : 1);
+            ptx::mbar_init(&full[s], ROWS && p.rows ? 65 : 1);
             ptx::mbar_init(&empty[s], 1);
         }
         for (int s = 0; s < kSlots; s++) {
@@ -195,53 +222,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = *tmem_slot;
     const int total = ROWS ? *total_slot : p.m_tiles * p.n_tiles * (p.groups ? p.groups : 1);
 
-    if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 0) {
+    if (warp == 1 || warp == 2) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (lane == 0) {
-            int stage = 0;
-            uint32_t phase = 0;
-            bool alive = true;
-            const bool gather = ROWS && p.rows;
-            for (int u = blockIdx.x; alive && u < total; u += gridDim.x) {
+            const int mine = warp - 1;
+            const Pipe pipe{dead, p.err, kErrTimeoutMma};
+            int it = 0;  // k-blocks so far: number `it` uses stage it % STAGES and part it % PARTS
+            for (int u = blockIdx.x; u < total; u += gridDim.x) {
                 const Unit w = unit_at<BN, ROWS>(p, start, u);
-                for (int kb = w.kb0; kb < w.kb1; kb++) {
-                    if (!ptx::mbar_wait(&empty[stage], phase ^ 1, p.err, kErrTimeoutProducer)) {
-                        alive = false;
-                        break;
-                    }
-                    uint8_t* sa = smem + stage * C::STAGE;
-                    ptx::mbar_arrive_expect_tx(&full[stage], gather ? C::STAGE - C::A_BYTES : C::STAGE);
-                    if (!gather) ptx::tma_load_2d(sa, &ta, &full[stage], kb * 128, w.m0);
-                    ptx::tma_load_3d(sa + C::A_BYTES, &tb, &full[stage], kb * 128, w.n0, ROWS ? w.g : 0);
-                    if (++stage == C::STAGES) {
-                        stage = 0;
-                        phase ^= 1;
-                    }
-                }
-            }
-            // every load has landed and been used before the CTA exits (bounded)
-            for (int s = 0; s < C::STAGES; s++) {
-                ptx::mbar_wait(&empty[stage], phase ^ 1, p.err, kErrTimeoutProducer);
-                if (++stage == C::STAGES) {
-                    stage = 0;
-                    phase ^= 1;
-                }
-            }
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            int stage = 0, part = 0;
-            uint32_t phase = 0, part_phase = 0;
-            bool alive = true;
-            for (int u = blockIdx.x; alive && u < total; u += gridDim.x) {
-                const Unit w = unit_at<BN, ROWS>(p, start, u);
-                for (int kb = w.kb0; kb < w.kb1; kb++) {
-                    if (!ptx::mbar_wait(&part_empty[part], part_phase ^ 1, p.err, kErrTimeoutMma) ||
-                        !ptx::mbar_wait(&full[stage], phase, p.err, kErrTimeoutMma)) {
-                        alive = false;
-                        break;
-                    }
+                for (int kb = w.kb0; kb < w.kb1; kb++, it++) {
+                    if ((it & 1) != mine) continue;
+                    const int stage = it % C::STAGES, part = it % C::PARTS;
+                    pipe.wait(&full[stage], it / C::STAGES & 1);
+                    pipe.wait(&part_empty[part], (it / C::PARTS & 1) ^ 1);
+                    // gathered rows came through the generic proxy; the fence is
+                    // here, where no copies are in flight that it would wait for
+                    if (ROWS && p.rows) ptx::fence_proxy_async();
                     ptx::tc_fence_after();
                     const uint32_t sa = ptx::smem_u32(smem + stage * C::STAGE), sb = sa + C::A_BYTES;
 #pragma unroll
@@ -250,24 +246,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                                     ptx::smem_desc(sb + k * 32, 16, 1024, 2), IDESC, k > 0);
                     ptx::mma_commit(&empty[stage]);
                     ptx::mma_commit(&part_full[part]);
-                    if (++stage == C::STAGES) {
-                        stage = 0;
-                        phase ^= 1;
-                    }
-                    if (++part == C::PARTS) {
-                        part = 0;
-                        part_phase ^= 1;
-                    }
                 }
             }
         }
-    } else {
-        const int t = threadIdx.x - 64;  // 0..63
+    } else if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        const int t = (warp == 0 ? 0 : 32) + lane;  // 0..63
         const bool gather = ROWS && p.rows;
-        int slot = 0, stage = 0, behind = 0, old = 0;
+        int slot = 0, stage = 0;
         uint32_t slot_phase = 0, phase = 0;
-        bool alive = true;
-        for (int u = blockIdx.x; alive && u < total; u += gridDim.x) {
+        const Pipe pipe{dead, p.err, kErrTimeoutProducer};
+        for (int u = blockIdx.x; u < total; u += gridDim.x) {
             const Unit w = unit_at<BN, ROWS>(p, start, u);
             // the rows whose scales this thread copies; rows past the end
             // take the first one's, and are not stored
@@ -289,12 +278,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             for (int kb = w.kb0; kb < w.kb1; kb++) {
-                if (!__all_sync(0xffffffffu,
-                                ptx::mbar_wait(&slot_empty[slot], slot_phase ^ 1, p.err, kErrTimeoutProducer))) {
-                    alive = false;
-                    break;
-                }
-                float* to = slots + slot * C::SLOT;
+                const int in = (kb - w.kb0) % C::SLOTK;
+                if (in == 0) pipe.wait(&slot_empty[slot], slot_phase ^ 1);
+                float* to = slots + (slot * C::SLOTK + in) * C::SLOT;
 #pragma unroll
                 for (int i = 0; i < 2; i++) ptx::cp_async4(to + t + 64 * i, srow[i] + kb * p.ld_sa);
                 if (VEC) {
@@ -306,17 +292,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                 } else if (t < 2) {
                     ptx::cp_async4(to + 128 + t, sb + kb);
                 }
-                ptx::cp_async_arrive(&slot_full[slot]);
-                if (++slot == kSlots) {
-                    slot = 0;
-                    slot_phase ^= 1;
+                if (in == C::SLOTK - 1 || kb + 1 == w.kb1) {
+                    ptx::cp_async_arrive(&slot_full[slot]);
+                    if (++slot == kSlots) {
+                        slot = 0;
+                        slot_phase ^= 1;
+                    }
+                }
+                if (!gather && warp != 0) continue;
+                pipe.wait(&empty[stage], phase ^ 1);
+                uint8_t* sa = smem + stage * C::STAGE;
+                if (t == 0) {
+                    ptx::mbar_arrive_expect_tx(&full[stage], gather ? C::STAGE - C::A_BYTES : C::STAGE);
+                    if (!gather) ptx::tma_load_2d(sa, &ta, &full[stage], kb * 128, w.m0);
+                    ptx::tma_load_3d(sa + C::A_BYTES, &tb, &full[stage], kb * 128, w.n0, ROWS ? w.g : 0);
+                }
+                uint64_t* landed = &full[stage];
+                if (++stage == C::STAGES) {
+                    stage = 0;
+                    phase ^= 1;
                 }
                 if (!gather) continue;
-                if (!__all_sync(0xffffffffu, ptx::mbar_wait(&empty[stage], phase ^ 1, p.err, kErrTimeoutProducer))) {
-                    alive = false;
-                    break;
-                }
-                uint8_t* sa = smem + stage * C::STAGE;
                 const int k = kb * 128 + (t & 7) * 16;
                 const int bytes = max(0, min(16, p.K - k));
 #pragma unroll
@@ -326,94 +322,91 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ptx::cp_async16(sa + r * 128 + (((t & 7) ^ (t >> 3)) << 4),
                                     on ? p.a + (size_t)arow[i] * p.lda + k : p.a, on ? bytes : 0);
                 }
-                ptx::cp_async_commit();
+                ptx::cp_async_arrive(landed);
+            }
+        }
+        ptx::cp_async_wait_all();
+        // every load has landed and been used before the CTA exits (bounded)
+        if (t == 0)
+            for (int s = 0; s < C::STAGES; s++) {
+                pipe.wait(&empty[stage], phase ^ 1);
                 if (++stage == C::STAGES) {
                     stage = 0;
                     phase ^= 1;
                 }
-                if (behind < kLag) {
-                    behind++;
-                } else {
-                    ptx::cp_async_wait<kLag>();
-                    ptx::fence_proxy_async();  // the tensor cores read through the async proxy
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(&full[old]);
-                    if (++old == C::STAGES) old = 0;
-                }
             }
-        }
-        ptx::cp_async_wait<0>();
-        if (gather) {
-            ptx::fence_proxy_async();
-            __syncwarp();
-            for (; behind > 0; behind--) {
-                if (lane == 0) ptx::mbar_arrive(&full[old]);
-                if (++old == C::STAGES) old = 0;
-            }
-        }
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         uint8_t* stg = staging + (warp - 4) * 2048;
         int part = 0, slot = 0;
         uint32_t part_phase = 0, slot_phase = 0;
+        const Pipe pipe{dead, p.err, kErrTimeoutEpilogue};
         const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + half * C::COLS;
         for (int u = blockIdx.x; u < total; u += gridDim.x) {
             const Unit w = unit_at<BN, ROWS>(p, start, u);
             const int row = w.m0 + quarter * 32 + lane;
             const bool valid = row < w.row_end;
             const int col0 = w.n0 + half * C::COLS;
-            uint64_t acc[C::COLS / 2];
+            float acc[C::COLS];
 #pragma unroll
-            for (int j = 0; j < C::COLS / 2; j++) acc[j] = 0;
-            bool alive = true;
+            for (int j = 0; j < C::COLS; j++) acc[j] = 0.f;
+            int in = 0;
+            float s_next[C::SLOTK];  // this row's scales of the group's k-blocks
             for (int kb = w.kb0; kb < w.kb1; kb++) {
-                if (!ptx::mbar_wait(&slot_full[slot], slot_phase, p.err, kErrTimeoutEpilogue)) alive = false;
-                const float* sc = slots + slot * C::SLOT;
-                const float s = VEC ? sc[quarter * 32 + lane] : sc[quarter * 32 + lane] * sc[128 + half];
-                const uint64_t s2 = f2_pack(s, s);
-                const uint64_t* v = reinterpret_cast<const uint64_t*>(sc + 128 + half * C::COLS);
-                if (!ptx::mbar_wait(&part_full[part], part_phase, p.err, kErrTimeoutEpilogue)) alive = false;
-                alive = __all_sync(0xffffffffu, alive);
-                if (!alive) break;
+                if (in == 0) {
+                    pipe.wait(&slot_full[slot], slot_phase);
+                    const float* sc = slots + slot * C::SLOTK * C::SLOT;
+#pragma unroll
+                    for (int i = 0; i < C::SLOTK; i++)
+                        s_next[i] = sc[i * C::SLOT + quarter * 32 + lane] * (VEC ? 1.f : sc[i * C::SLOT + 128 + half]);
+                }
+                const float s = s_next[0];
+#pragma unroll
+                for (int i = 0; i + 1 < C::SLOTK; i++) s_next[i] = s_next[i + 1];
+                const float4* v =
+                    reinterpret_cast<const float4*>(slots + (slot * C::SLOTK + in) * C::SLOT + 128 + half * C::COLS);
+                pipe.wait(&part_full[part], part_phase);
+                __syncwarp();
                 ptx::tc_fence_after();
                 const uint32_t t = lane_base + part * BN;
                 uint32_t r[2][16];
                 ptx::tmem_ld16(t, r[0]);
 #pragma unroll
                 for (int c = 0; c < C::COLS / 16; c++) {
-                    uint64_t m[8];
+                    float m[16];
                     if (VEC) {
 #pragma unroll
-                        for (int j = 0; j < 8; j++) m[j] = f2_mul(v[c * 8 + j], s2);
+                        for (int j = 0; j < 4; j++) {
+                            const float4 q = v[c * 4 + j];
+                            m[4 * j] = q.x * s;
+                            m[4 * j + 1] = q.y * s;
+                            m[4 * j + 2] = q.z * s;
+                            m[4 * j + 3] = q.w * s;
+                        }
                     }
                     ptx::tmem_ld_wait_regs16(r[c & 1]);
                     if (c + 1 < C::COLS / 16) ptx::tmem_ld16(t + (c + 1) * 16, r[(c + 1) & 1]);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        uint64_t& a = acc[c * 8 + j];
-                        const uint64_t x =
-                            f2_pack(__uint_as_float(r[c & 1][2 * j]), __uint_as_float(r[c & 1][2 * j + 1]));
-                        a = f2_fma(x, VEC ? m[j] : s2, a);
-                    }
+                    for (int j = 0; j < 16; j++)
+                        acc[c * 16 + j] = fmaf(__uint_as_float(r[c & 1][j]), VEC ? m[j] : s, acc[c * 16 + j]);
                 }
                 ptx::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) {
-                    ptx::mbar_arrive(&part_empty[part]);
-                    ptx::mbar_arrive(&slot_empty[slot]);
-                }
-                if (++slot == kSlots) {
-                    slot = 0;
-                    slot_phase ^= 1;
+                ptx::mbar_arrive_if(&part_empty[part], lane == 0);
+                if (++in == C::SLOTK || kb + 1 == w.kb1) {
+                    ptx::mbar_arrive_if(&slot_empty[slot], lane == 0);
+                    in = 0;
+                    if (++slot == kSlots) {
+                        slot = 0;
+                        slot_phase ^= 1;
+                    }
                 }
                 if (++part == C::PARTS) {
                     part = 0;
                     part_phase ^= 1;
                 }
             }
-            if (!alive) break;
             // a slab of 32 rows leaves by TMA where all of them are the tile's
             // (the store clips at the tensor's end), else row by row
             const int y = w.m0 + quarter * 32;
@@ -423,9 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int c = 0; c < C::COLS / 32; c++) {
                 const int col = col0 + c * 32;
                 if (col >= p.N) continue;
-                float f[32];
-#pragma unroll
-                for (int j = 0; j < 16; j++) f2_unpack(acc[c * 16 + j], f[2 * j], f[2 * j + 1]);
+                const float* f = acc + c * 32;
                 if (tma) {
                     if (y >= p.M) continue;
                     const int boxes = p.c_dtype == kBF16 ? 1 : 2;
