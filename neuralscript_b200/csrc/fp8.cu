@@ -19,6 +19,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "fp8.h"
 
 namespace nsb {
@@ -47,7 +49,14 @@ __device__ __forceinline__ void store8(uint8_t* dst, uint2 v, int n) {
         if (i < n) dst[i] = (uint8_t)((i < 4 ? v.x >> 8 * i : v.y >> 8 * (i - 4)) & 0xff);
 }
 
-template <typename T, bool BLOCK, bool VEC>
+// act_fwd with the code known, and GELU's division by sqrt(2) as a
+// multiplication (a last bit's difference, a third of the instructions)
+template <int ACT>
+__device__ __forceinline__ float activate(float x) {
+    return act_fwd(x, ACT == kGelu ? kGeluMoe : ACT);
+}
+
+template <typename T, bool BLOCK, bool VEC, int ACT>
 __global__ void __launch_bounds__(256, 2) quantize_kernel(const QuantDesc d) {
     __shared__ uint2 tile[128 * 16];   // [column][unit of 8 rows]
     __shared__ float part[16][128];    // column maxima of the 16 half-warps
@@ -83,11 +92,11 @@ __global__ void __launch_bounds__(256, 2) quantize_kernel(const QuantDesc d) {
             for (int j = 0; j < 8; j++) v[i][j] = in && c0 + j < d.K ? (float)p[j] : 0.f;
         }
     }
-    if (d.act) {
+    if (ACT) {
 #pragma unroll
         for (int i = 0; i < 8; i++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[i][j] = act_fwd(v[i][j], d.act);
+            for (int j = 0; j < 8; j++) v[i][j] = activate<ACT>(v[i][j]);
     }
     if constexpr (BLOCK) {
         float m = 0.f;
@@ -196,12 +205,29 @@ int quantize(const QuantDesc& d, cudaStream_t st) {
     if (rb > 65535) return -2;
     const dim3 grid((unsigned)cb, (unsigned)rb);
     const bool vec = !(reinterpret_cast<uintptr_t>(d.x) & 15) && d.ld * (f ? 4 : 2) % 16 == 0;
-    if (f) {
-        if (vec) quantize_kernel<float, BLOCK, true><<<grid, 256, 0, st>>>(d);
-        else quantize_kernel<float, BLOCK, false><<<grid, 256, 0, st>>>(d);
+    auto go = [&](auto act) {
+        constexpr int ACT = decltype(act)::value;
+        if (f) {
+            if (vec) quantize_kernel<float, BLOCK, true, ACT><<<grid, 256, 0, st>>>(d);
+            else quantize_kernel<float, BLOCK, false, ACT><<<grid, 256, 0, st>>>(d);
+        } else {
+            if (vec) quantize_kernel<__nv_bfloat16, BLOCK, true, ACT><<<grid, 256, 0, st>>>(d);
+            else quantize_kernel<__nv_bfloat16, BLOCK, false, ACT><<<grid, 256, 0, st>>>(d);
+        }
+    };
+    if constexpr (BLOCK) {
+        go(std::integral_constant<int, kIdentity>());
     } else {
-        if (vec) quantize_kernel<__nv_bfloat16, BLOCK, true><<<grid, 256, 0, st>>>(d);
-        else quantize_kernel<__nv_bfloat16, BLOCK, false><<<grid, 256, 0, st>>>(d);
+        switch (d.act) {
+            case kRelu: go(std::integral_constant<int, kRelu>()); break;
+            case kLeaky: go(std::integral_constant<int, kLeaky>()); break;
+            case kSigmoid: go(std::integral_constant<int, kSigmoid>()); break;
+            case kTanh: go(std::integral_constant<int, kTanh>()); break;
+            case kSilu: go(std::integral_constant<int, kSilu>()); break;
+            case kGelu:
+            case kGeluMoe: go(std::integral_constant<int, kGelu>()); break;
+            default: go(std::integral_constant<int, kIdentity>());
+        }
     }
     return cudaGetLastError() == cudaSuccess ? 0 : -5;
 }

@@ -4,6 +4,8 @@
 #include <cuda_bf16.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "gemm.h"
 #include "moe_topk.h"
 
@@ -41,20 +43,47 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
-// Scores of this lane's NV consecutive experts, from lane * NV on. Dead
-// experts score 0. The softmax's sum is held in 64 bits and rounded once, so
-// that the scores, and with them the choice, do not depend on the order of
-// the sum.
+// Logits of this lane's NV consecutive experts, from lane * NV on: 16-byte
+// loads where the rows allow them.
+template <int NV>
+__device__ __forceinline__ void load_logits(const RouteDesc& d, int row, int lane, float* x) {
+    const int e0 = lane * NV;
+    if (d.vec && e0 + NV <= d.E) {
+        if (d.dtype == kF32) {
+            const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(d.logits) + (size_t)row * d.ld + e0);
+#pragma unroll
+            for (int i = 0; i < NV / 4; i++) {
+                const float4 t = p[i];
+                x[4 * i] = t.x, x[4 * i + 1] = t.y, x[4 * i + 2] = t.z, x[4 * i + 3] = t.w;
+            }
+        } else {
+            const uint2* p = reinterpret_cast<const uint2*>(reinterpret_cast<const __nv_bfloat16*>(d.logits) + (size_t)row * d.ld + e0);
+#pragma unroll
+            for (int i = 0; i < NV / 4; i++) {
+                const uint2 t = p[i];
+                const __nv_bfloat16* h = reinterpret_cast<const __nv_bfloat16*>(&t);
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[4 * i + j] = bf2f(h[j]);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; i++) x[i] = e0 + i < d.E ? ld_any(d.logits, d.dtype, (size_t)row * d.ld + e0 + i) : 0.f;
+}
+
+// Their scores. Dead experts score 0. The softmax's sum is held in 64 bits
+// and rounded once, so that the scores, and with them the choice, do not
+// depend on the order of the sum.
 template <int NV>
 __device__ __forceinline__ void scores(const RouteDesc& d, int row, int lane, float* s, unsigned& live) {
     float x[NV];
+    load_logits<NV>(d, row, lane, x);
     live = 0;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
         const int e = lane * NV + i;
-        const bool on = e < d.E && (!d.active || d.active[e]);
-        x[i] = on ? ld_any(d.logits, d.dtype, (size_t)row * d.ld + e) : -INFINITY;
-        live |= on ? 1u << i : 0u;
+        live |= e < d.E && (!d.active || d.active[e]) ? 1u << i : 0u;
     }
     if (d.sigmoid) {
 #pragma unroll
@@ -63,7 +92,8 @@ __device__ __forceinline__ void scores(const RouteDesc& d, int row, int lane, fl
     }
     float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < NV; i++) m = fmaxf(m, x[i]);
+    for (int i = 0; i < NV; i++)
+        if (live >> i & 1) m = fmaxf(m, x[i]);
     m = warp_max(m);
     double sum = 0.;
 #pragma unroll
@@ -76,7 +106,15 @@ __device__ __forceinline__ void scores(const RouteDesc& d, int row, int lane, fl
     for (int i = 0; i < NV; i++) s[i] = s[i] / total;
 }
 
-// One warp a token; a lane holds NV consecutive experts.
+// A group's score is the sum of its two best keys b1 >= b2 (0: none there).
+__device__ __forceinline__ unsigned group_score(unsigned b1, unsigned b2) {
+    if (b1 == 0) return 0;
+    return ordered(b2 ? unordered(b1) + unordered(b2) : unordered(b1));
+}
+
+// One warp a token; a lane holds NV consecutive experts. The k choices are k
+// rounds of one warp maximum; only the lane that gave an expert away looks
+// for its next best.
 template <int NV>
 __global__ void __launch_bounds__(128) route_kernel(const RouteDesc d, int* __restrict__ idx, float* __restrict__ w) {
     const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -89,10 +127,37 @@ __global__ void __launch_bounds__(128) route_kernel(const RouteDesc d, int* __re
         const float v = s[i] + (d.bias && lane * NV + i < d.E ? d.bias[lane * NV + i] : 0.f);
         key[i] = (live >> i & 1) && v > -INFINITY ? ordered(v) : 0u;
     }
-    if (d.groups > 1) {
-        // A group's score is the sum of its two best keys; lane g (and g + 32,
-        // ...) keeps that of group g. The topk_groups best stay.
+    if (d.lanes > 0) {
+        // a group is the experts of `lanes` neighbouring lanes, a power of 2
+        unsigned b1 = 0, b2 = 0;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            b2 = max(b2, min(b1, key[i]));
+            b1 = max(b1, key[i]);
+        }
+        for (int o = 1; o < d.lanes; o <<= 1) {
+            const unsigned c1 = __shfl_xor_sync(kAll, b1, o), c2 = __shfl_xor_sync(kAll, b2, o);
+            b2 = max(min(b1, c1), max(b2, c2));
+            b1 = max(b1, c1);
+        }
+        const unsigned mine = group_score(b1, b2);
+        const int g = lane / d.lanes;
+        int better = 0;
+        for (int o = 0; o < d.groups; o++) {
+            const unsigned other = __shfl_sync(kAll, mine, o * d.lanes);
+            better += other > mine || (other == mine && o < g);
+        }
+        if (better >= d.topk_groups) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) key[i] = 0;
+        }
+    } else if (d.groups > 1) {
+        // any other size: group by group, lane g (and g + 32, ...) keeps the
+        // score of group g
         const int per = d.E / d.groups;
+        int of[NV];
+#pragma unroll
+        for (int i = 0; i < NV; i++) of[i] = (lane * NV + i) / per;
         unsigned gs[(kTopkMaxE / 2) / 32];
 #pragma unroll
         for (int q = 0; q < (kTopkMaxE / 2) / 32; q++) gs[q] = 0;
@@ -100,19 +165,17 @@ __global__ void __launch_bounds__(128) route_kernel(const RouteDesc d, int* __re
             unsigned b1 = 0, b2 = 0;
 #pragma unroll
             for (int i = 0; i < NV; i++) {
-                const int e = lane * NV + i;
-                const unsigned v = e / per == g ? key[i] : 0u;
+                const unsigned v = of[i] == g ? key[i] : 0u;
                 b2 = max(b2, min(b1, v));
                 b1 = max(b1, v);
             }
             const unsigned m1 = __reduce_max_sync(kAll, b1);
             const int owner = __ffs(__ballot_sync(kAll, b1 == m1)) - 1;
             const unsigned m2 = __reduce_max_sync(kAll, lane == owner ? b2 : b1);
-            float v = m1 ? unordered(m1) : 0.f;
-            if (m2) v += unordered(m2);
+            const unsigned v = group_score(m1, m2);
 #pragma unroll
             for (int q = 0; q < (kTopkMaxE / 2) / 32; q++)
-                if (q * 32 + lane == g) gs[q] = m1 ? ordered(v) : 0u;
+                if (q * 32 + lane == g) gs[q] = v;
         }
         for (int t = 0; t < d.groups; t++) {
             unsigned b = 0;
@@ -132,35 +195,40 @@ __global__ void __launch_bounds__(128) route_kernel(const RouteDesc d, int* __re
             if (t < d.topk_groups) continue;
 #pragma unroll
             for (int i = 0; i < NV; i++)
-                if ((lane * NV + i) / per == g) key[i] = 0;
+                if (of[i] == g) key[i] = 0;
         }
     }
     int mine = -1;
     float got = 0.f;
-    for (int j = 0; j < d.k; j++) {
-        unsigned b = 0;
-        int bi = 0;
+    unsigned b = 0;
+    int bi = 0;
+    float bs = 0.f;
+    auto best = [&] {
+        b = 0;
 #pragma unroll
         for (int i = 0; i < NV; i++)
             if (key[i] > b) {
                 b = key[i];
                 bi = i;
+                bs = s[i];
             }
+    };
+    best();
+    for (int j = 0; j < d.k; j++) {
         const unsigned m = __reduce_max_sync(kAll, b);
         if (m == 0) break;
         const int owner = __ffs(__ballot_sync(kAll, b == m)) - 1;
-        float sv = 0.f;
-#pragma unroll
-        for (int i = 0; i < NV; i++)
-            if (i == bi) {
-                sv = s[i];
-                if (lane == owner) key[i] = 0;
-            }
         const int e = __shfl_sync(kAll, lane * NV + bi, owner);
-        sv = __shfl_sync(kAll, sv, owner);
+        const float sv = __shfl_sync(kAll, bs, owner);
         if (lane == j) {
             mine = e;
             got = sv;
+        }
+        if (lane == owner) {
+#pragma unroll
+            for (int i = 0; i < NV; i++)
+                if (i == bi) key[i] = 0;
+            best();
         }
     }
     const float total = d.renorm ? warp_sum(got) + 1e-20f : 1.f;
@@ -175,30 +243,35 @@ __device__ __forceinline__ void st_any(void* p, int dtype, size_t i, float v) {
     else reinterpret_cast<float*>(p)[i] = v;
 }
 
-// One warp a token: the row's other experts first, then lane j the j-th
-// chosen one.
+// One warp a token: the row's other experts first (zeros for sigmoid scores,
+// which then need no more of the row than the chosen logits), then lane j
+// the j-th chosen one.
 template <int NV>
 __global__ void __launch_bounds__(128)
     route_bwd_kernel(const RouteDesc d, const float* __restrict__ dw, const int* __restrict__ idx, void* dlogits,
-                     long long ld_d) {
+                     long long ld_d, int vec_d) {
     const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (row >= d.M) return;
-    float s[NV];
-    unsigned live;
-    scores<NV>(d, row, lane, s, live);
     int e = lane < d.k ? idx[(size_t)row * d.k + lane] : -1;
     if (e >= d.E) e = -1;
-    float sj = 0.f;
-    for (int j = 0; j < d.k; j++) {
-        const int ej = __shfl_sync(kAll, e, j);
-        float v = 0.f;
-#pragma unroll
-        for (int i = 0; i < NV; i++)
-            if (ej >= 0 && i == ej % NV) v = s[i];
-        v = __shfl_sync(kAll, v, ej >= 0 ? ej / NV : 0);
-        if (lane == j) sj = v;
-    }
     const float g = e >= 0 ? dw[(size_t)row * d.k + lane] : 0.f;
+    float s[NV];
+    float sj = 0.f;
+    if (d.sigmoid) {
+        if (e >= 0) sj = 1.f / (1.f + expf(-ld_any(d.logits, d.dtype, (size_t)row * d.ld + e)));
+    } else {
+        unsigned live;
+        scores<NV>(d, row, lane, s, live);
+        for (int j = 0; j < d.k; j++) {
+            const int ej = __shfl_sync(kAll, e, j);
+            float v = 0.f;
+#pragma unroll
+            for (int i = 0; i < NV; i++)
+                if (ej >= 0 && i == ej % NV) v = s[i];
+            v = __shfl_sync(kAll, v, ej >= 0 ? ej / NV : 0);
+            if (lane == j) sj = v;
+        }
+    }
     float ds = d.scale * g;
     if (d.renorm) {
         const float total = warp_sum(sj) + 1e-20f;
@@ -208,9 +281,24 @@ __global__ void __launch_bounds__(128)
     const bool any = __any_sync(kAll, e >= 0);
     const float dot = d.sigmoid || !any ? 0.f : warp_sum(ds * sj);
     const size_t base = (size_t)row * ld_d;
+    if (d.sigmoid || !any) {
+        const size_t es = d.dtype == kBF16 ? 2 : 4;
+        char* p = reinterpret_cast<char*>(dlogits) + base * es;
+        if (vec_d) {
+            for (int i = lane; i < (int)(d.E * es / 16); i += 32) reinterpret_cast<uint4*>(p)[i] = make_uint4(0, 0, 0, 0);
+        } else {
+            for (int i = lane; i < d.E; i += 32) st_any(dlogits, d.dtype, base + i, 0.f);
+        }
+    } else if (vec_d && d.dtype == kF32 && NV % 4 == 0 && lane * NV + NV <= d.E) {
 #pragma unroll
-    for (int i = 0; i < NV; i++)
-        if (lane * NV + i < d.E) st_any(dlogits, d.dtype, base + lane * NV + i, dot == 0.f ? 0.f : -s[i] * dot);
+        for (int i = 0; i < NV / 4; i++)
+            reinterpret_cast<float4*>(reinterpret_cast<float*>(dlogits) + base + lane * NV)[i] =
+                make_float4(-s[4 * i] * dot, -s[4 * i + 1] * dot, -s[4 * i + 2] * dot, -s[4 * i + 3] * dot);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+            if (lane * NV + i < d.E) st_any(dlogits, d.dtype, base + lane * NV + i, -s[i] * dot);
+    }
     __syncwarp();
     if (e >= 0) st_any(dlogits, d.dtype, base + e, d.sigmoid ? ds * sj * (1.f - sj) : sj * (ds - dot));
 }
@@ -228,19 +316,46 @@ bool route_ok(const RouteDesc& d) {
 constexpr int kOrderThreads = 1024;
 constexpr int kOrderWarps = kOrderThreads / 32;
 
-// One block: every warp counts a contiguous share of the pairs, the counts
-// are summed over warps and experts, and every warp places its share in the
-// same order.
+__device__ __forceinline__ unsigned cluster_rank() {
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// the same word of the shared memory of CTA `rank` of the cluster
+__device__ __forceinline__ int cluster_load(const int* p, unsigned rank) {
+    uint32_t at;
+    int v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                 : "=r"(at)
+                 : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+
+// One cluster of CTAS blocks, one launch: every warp counts a contiguous
+// share of the pairs, the counts are summed over the warps of a block, the
+// blocks of the cluster (through each other's shared memory) and the experts,
+// and every warp places its share in the same order. A pair's rank among its
+// 32 neighbours of the same expert comes from a warp match, so nothing is
+// counted by atomics and the order is the pairs' own.
+template <int CTAS>
 __global__ void __launch_bounds__(kOrderThreads)
     dispatch_kernel(const int* __restrict__ idx, long long P, int E, int align, long long cap, int* offsets, int* counts,
                     int* rows, int* pos) {
-    extern __shared__ int sh[];  // [kOrderWarps][E] counts, [E + 1] starts
-    int* start = sh + kOrderWarps * E;
+    extern __shared__ int sh[];       // [kOrderWarps][E] counts of the warps
+    int* total = sh + kOrderWarps * E;  // [E] of the block
+    int* start = total + E;             // [E + 1] first row of an expert
+    int* base = start + E + 1;          // [E] this block's first row of it
+    int* sums = base + E;               // [kOrderWarps] scan over experts
+    const unsigned rank = CTAS > 1 ? cluster_rank() : 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int i = threadIdx.x; i < kOrderWarps * E; i += kOrderThreads) sh[i] = 0;
     __syncthreads();
-    const long long share = (P + kOrderThreads - 1) / kOrderThreads * 32;
-    const long long p0 = share * warp, p1 = min(P, p0 + share);
+    const long long share = (P + CTAS * kOrderThreads - 1) / (CTAS * kOrderThreads) * 32;
+    const long long p0 = share * (rank * kOrderWarps + warp), p1 = min(P, p0 + share);
     int* mine = sh + warp * E;
     for (long long p = p0; p < p1; p += 32) {
         const int e = p + lane < p1 ? idx[p + lane] : -1;
@@ -251,66 +366,169 @@ __global__ void __launch_bounds__(kOrderThreads)
     __syncthreads();
     for (int e = threadIdx.x; e < E; e += kOrderThreads) {
         int run = 0;
+#pragma unroll 8
         for (int q = 0; q < kOrderWarps; q++) {
             const int c = sh[q * E + e];
             sh[q * E + e] = run;
             run += c;
         }
-        start[e] = run;
-        counts[e] = run;
+        total[e] = run;
     }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        int at = 0;
-        for (int e = 0; e < E; e++) {
-            const int c = start[e];
-            start[e] = at;
-            offsets[e] = at;
-            at += (c + align - 1) / align * align;
+    if (CTAS > 1) cluster_sync();
+    else __syncthreads();
+    // E <= 1024 threads: thread e sums expert e over the blocks, then the
+    // padded counts are scanned over the experts
+    const int e = threadIdx.x;
+    int all = 0, before = 0;
+    if (e < E) {
+#pragma unroll
+        for (int c = 0; c < CTAS; c++) {
+            const int v = CTAS > 1 ? cluster_load(total + e, c) : total[e];
+            if (c < (int)rank) before += v;
+            all += v;
         }
-        start[E] = at;
-        offsets[E] = at;
     }
-    for (long long r = threadIdx.x; r < cap; r += kOrderThreads) rows[r] = -1;
+    const int padded = (all + align - 1) / align * align;
+    int inc = padded;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int n = __shfl_up_sync(kAll, inc, o);
+        if (lane >= o) inc += n;
+    }
+    if (lane == 31) sums[warp] = inc;
     __syncthreads();
+    if (warp == 0) {
+        int v = sums[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int n = __shfl_up_sync(kAll, v, o);
+            if (lane >= o) v += n;
+        }
+        sums[lane] = v;
+    }
+    __syncthreads();
+    if (e < E) {
+        const int first = inc - padded + (warp ? sums[warp - 1] : 0);
+        base[e] = first + before;
+        start[e] = first;
+        if (e == E - 1) start[E] = first + padded;
+        if (rank == 0) {
+            offsets[e] = first;
+            counts[e] = all;
+            if (e == E - 1) offsets[E] = first + padded;
+        }
+        // rows of the padding behind the expert's last pair
+        if (e % CTAS == (int)rank)
+            for (int r = first + all; r < first + padded; r++) rows[r] = -1;
+    }
+    __syncthreads();
+    for (long long r = start[E] + (long long)rank * kOrderThreads + threadIdx.x; r < cap; r += CTAS * kOrderThreads)
+        rows[r] = -1;
     for (long long p = p0; p < p1; p += 32) {
         const bool in = p + lane < p1;
-        int e = in ? idx[p + lane] : -1;
-        if (e >= E) e = -1;
-        const unsigned peers = __match_any_sync(kAll, e);
-        const int rank = __popc(peers & ((1u << lane) - 1u));
+        int x = in ? idx[p + lane] : -1;
+        if (x >= E) x = -1;
+        const unsigned peers = __match_any_sync(kAll, x);
+        const int place = __popc(peers & ((1u << lane) - 1u));
         int at = -1;
-        if (e >= 0) at = start[e] + mine[e] + rank;
+        if (x >= 0) at = base[x] + mine[x] + place;
         __syncwarp();
-        if (e >= 0 && rank == 0) mine[e] += __popc(peers);
+        if (x >= 0 && place == 0) mine[x] += __popc(peers);
         __syncwarp();
         if (in) pos[p + lane] = at;
         if (at >= 0) rows[at] = (int)(p + lane);
     }
+    if (CTAS > 1) cluster_sync();  // no block leaves while others read its counts
 }
 
 // ---------------------------------------------------------------------------
 // Weighted sum of the experts' outputs
 // ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(256)
-    combine_kernel(const void* o, int dtype, long long ld_o, const int* __restrict__ pos, const float* __restrict__ w,
-                   int k, int D, void* y, long long ld_y) {
-    const size_t t = blockIdx.x;
-    for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < D; c += gridDim.y * blockDim.x) {
-        float acc = 0.f;
-        for (int j = 0; j < k; j++) {
-            const int p = pos[t * k + j];
-            if (p >= 0) acc = fmaf(w ? w[t * k + j] : 1.f, ld_any(o, dtype, (size_t)p * ld_o + c), acc);
-        }
-        st_any(y, dtype, t * ld_y + c, acc);
+// 16 bytes of a row as floats and back
+template <typename T>
+struct Pack;
+template <>
+struct Pack<float> {
+    __device__ static void get(uint4 v, float* f) {
+        f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+    }
+    __device__ static uint4 put(const float* f) {
+        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+};
+template <>
+struct Pack<__nv_bfloat16> {
+    __device__ static void get(uint4 v, float* f) {
+        const __nv_bfloat16* h = reinterpret_cast<const __nv_bfloat16*>(&v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) f[i] = bf2f(h[i]);
+    }
+    __device__ static uint4 put(const float* f) {
+        uint4 v;
+        __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&v);
+#pragma unroll
+        for (int i = 0; i < 4; i++) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        return v;
+    }
+};
+
+// W columns (16 bytes, or 1 where rows do not start on 16-byte boundaries) of
+// a row: ncol of them there.
+template <typename T, int W>
+__device__ __forceinline__ void load_cols(const T* p, float* f) {
+    if constexpr (W == 1) f[0] = (float)*p;
+    else Pack<T>::get(__ldg(reinterpret_cast<const uint4*>(p)), f);
+}
+template <typename T, int W>
+__device__ __forceinline__ void store_cols(T* p, const float* f) {
+    if constexpr (W == 1) {
+        if constexpr (sizeof(T) == 2) *p = f2bf(f[0]);
+        else *p = f[0];
+    } else {
+        *reinterpret_cast<uint4*>(p) = Pack<T>::put(f);
     }
 }
 
-// One warp a row of the ordered outputs.
+// A thread sums W columns of a token; the rows of four choices are in flight
+// together.
+template <typename T, int W>
+__global__ void __launch_bounds__(128)
+    combine_kernel(const T* __restrict__ o, long long ld_o, const int* __restrict__ pos, const float* __restrict__ w,
+                   int k, int D, T* __restrict__ y, long long ld_y) {
+    const size_t t = blockIdx.x;
+    const int c = (blockIdx.y * blockDim.x + threadIdx.x) * W;
+    if (c >= D) return;
+    float acc[W];
+#pragma unroll
+    for (int i = 0; i < W; i++) acc[i] = 0.f;
+    for (int j0 = 0; j0 < k; j0 += 4) {
+        float f[4][W], wj[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int p = j0 + j < k ? pos[t * k + j0 + j] : -1;
+            wj[j] = p < 0 ? 0.f : w ? w[t * k + j0 + j] : 1.f;
+            if (p >= 0) {
+                load_cols<T, W>(o + (size_t)p * ld_o + c, f[j]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < W; i++) f[j][i] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int i = 0; i < W; i++) acc[i] = fmaf(wj[j], f[j][i], acc[i]);
+    }
+    store_cols<T, W>(y + t * ld_y + c, acc);
+}
+
+// One warp a row of the ordered outputs: o and d_o stream, the tokens' dy,
+// which k rows share, come out of L2. Four steps of the row in flight.
+template <typename T, int W>
 __global__ void __launch_bounds__(256)
-    combine_bwd_kernel(const void* dy, const void* o, int dtype, long long ld_dy, long long ld_o,
+    combine_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ o, long long ld_dy, long long ld_o,
                        const int* __restrict__ rows, const int* __restrict__ pos, const float* __restrict__ w,
-                       long long P, int k, int R, int D, void* d_o, long long ld_do, float* dw) {
+                       long long P, int k, int R, int D, T* __restrict__ d_o, long long ld_do, float* __restrict__ dw) {
     const long long gt = (long long)blockIdx.x * blockDim.x + threadIdx.x;
     const long long step = (long long)gridDim.x * blockDim.x;
     if (dw)
@@ -319,47 +537,92 @@ __global__ void __launch_bounds__(256)
     const int lane = threadIdx.x & 31;
     for (long long r = gt >> 5; r < R; r += step >> 5) {
         const int pair = rows[r];
-        const float wp = pair >= 0 && w ? w[pair] : 1.f;
-        const size_t t = pair >= 0 ? pair / k : 0;
-        float acc = 0.f;
-        for (int c = lane; c < D; c += 32) {
-            const float g = pair >= 0 ? ld_any(dy, dtype, t * ld_dy + c) : 0.f;
-            if (pair >= 0 && dw) acc = fmaf(g, ld_any(o, dtype, (size_t)r * ld_o + c), acc);
-            st_any(d_o, dtype, (size_t)r * ld_do + c, wp * g);
+        T* to = d_o + (size_t)r * ld_do;
+        if (pair < 0) {
+            float zero[W];
+#pragma unroll
+            for (int i = 0; i < W; i++) zero[i] = 0.f;
+            for (int c = lane * W; c < D; c += 32 * W) store_cols<T, W>(to + c, zero);
+            continue;
         }
-        acc = warp_sum(acc);
-        if (lane == 0 && pair >= 0 && dw) dw[pair] = acc;
+        const float wp = w ? w[pair] : 1.f;
+        const T* g = dy + (size_t)(pair / k) * ld_dy;
+        const T* f = o + (size_t)r * ld_o;
+        float acc = 0.f;
+        for (int c0 = lane * W; c0 < D; c0 += 4 * 32 * W) {
+            float gv[4][W], fv[4][W];
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int c = c0 + q * 32 * W;
+                if (c >= D) continue;
+                load_cols<T, W>(g + c, gv[q]);
+                if (dw) load_cols<T, W>(f + c, fv[q]);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int c = c0 + q * 32 * W;
+                if (c >= D) continue;
+                float out[W];
+#pragma unroll
+                for (int i = 0; i < W; i++) {
+                    if (dw) acc = fmaf(gv[q][i], fv[q][i], acc);
+                    out[i] = wp * gv[q][i];
+                }
+                store_cols<T, W>(to + c, out);
+            }
+        }
+        if (dw) {
+            acc = warp_sum(acc);
+            if (lane == 0) dw[pair] = acc;
+        }
     }
 }
 
 }  // namespace
 
-int moe_topk_route(const RouteDesc& d, int* idx, float* w, cudaStream_t st) {
-    if (!route_ok(d) || !idx || !w) return -1;
-    if (d.M == 0) return 0;
-    const unsigned grid = (unsigned)((d.M + 3) / 4);
-    const int nv = (d.E + 31) / 32;
-    if (nv <= 1) route_kernel<1><<<grid, 128, 0, st>>>(d, idx, w);
-    else if (nv <= 2) route_kernel<2><<<grid, 128, 0, st>>>(d, idx, w);
-    else if (nv <= 4) route_kernel<4><<<grid, 128, 0, st>>>(d, idx, w);
-    else if (nv <= 8) route_kernel<8><<<grid, 128, 0, st>>>(d, idx, w);
-    else if (nv <= 16) route_kernel<16><<<grid, 128, 0, st>>>(d, idx, w);
-    else route_kernel<32><<<grid, 128, 0, st>>>(d, idx, w);
+namespace {
+// f with the smallest of 1, 2, 4, ... experts a lane that holds them all
+template <typename F>
+void by_lane(int E, F f) {
+    const int nv = (E + 31) / 32;
+    if (nv <= 1) f(std::integral_constant<int, 1>());
+    else if (nv <= 2) f(std::integral_constant<int, 2>());
+    else if (nv <= 4) f(std::integral_constant<int, 4>());
+    else if (nv <= 8) f(std::integral_constant<int, 8>());
+    else if (nv <= 16) f(std::integral_constant<int, 16>());
+    else f(std::integral_constant<int, 32>());
+}
+
+bool rows16(const void* p, long long ld, int dtype) {
+    return !(reinterpret_cast<uintptr_t>(p) & 15) && ld * (dtype == kBF16 ? 2 : 4) % 16 == 0;
+}
+}  // namespace
+
+int moe_topk_route(const RouteDesc& d0, int* idx, float* w, cudaStream_t st) {
+    if (!route_ok(d0) || !idx || !w) return -1;
+    if (d0.M == 0) return 0;
+    RouteDesc d = d0;
+    by_lane(d.E, [&](auto n) {
+        constexpr int NV = decltype(n)::value;
+        d.vec = NV >= 4 && rows16(d.logits, d.ld, d.dtype);
+        const int per = d.E / d.groups;
+        if (d.groups > 1 && per % NV == 0 && (per / NV & (per / NV - 1)) == 0) d.lanes = per / NV;
+        route_kernel<NV><<<(unsigned)((d.M + 3) / 4), 128, 0, st>>>(d, idx, w);
+    });
     return launched();
 }
 
-int moe_topk_route_bwd(const RouteDesc& d, const float* dw, const int* idx, void* dl, long long ld_d,
+int moe_topk_route_bwd(const RouteDesc& d0, const float* dw, const int* idx, void* dl, long long ld_d,
                        cudaStream_t st) {
-    if (!route_ok(d) || !idx || !dw || !dl || ld_d < d.E) return -1;
-    if (d.M == 0) return 0;
-    const unsigned grid = (unsigned)((d.M + 3) / 4);
-    const int nv = (d.E + 31) / 32;
-    if (nv <= 1) route_bwd_kernel<1><<<grid, 128, 0, st>>>(d, dw, idx, dl, ld_d);
-    else if (nv <= 2) route_bwd_kernel<2><<<grid, 128, 0, st>>>(d, dw, idx, dl, ld_d);
-    else if (nv <= 4) route_bwd_kernel<4><<<grid, 128, 0, st>>>(d, dw, idx, dl, ld_d);
-    else if (nv <= 8) route_bwd_kernel<8><<<grid, 128, 0, st>>>(d, dw, idx, dl, ld_d);
-    else if (nv <= 16) route_bwd_kernel<16><<<grid, 128, 0, st>>>(d, dw, idx, dl, ld_d);
-    else route_bwd_kernel<32><<<grid, 128, 0, st>>>(d, dw, idx, dl, ld_d);
+    if (!route_ok(d0) || !idx || !dw || !dl || ld_d < d0.E) return -1;
+    if (d0.M == 0) return 0;
+    RouteDesc d = d0;
+    by_lane(d.E, [&](auto n) {
+        constexpr int NV = decltype(n)::value;
+        d.vec = NV >= 4 && rows16(d.logits, d.ld, d.dtype);
+        const int vec_d = rows16(dl, ld_d, d.dtype) && d.E * (d.dtype == kBF16 ? 2 : 4) % 16 == 0;
+        route_bwd_kernel<NV><<<(unsigned)((d.M + 3) / 4), 128, 0, st>>>(d, dw, idx, dl, ld_d, vec_d);
+    });
     return launched();
 }
 
@@ -376,12 +639,29 @@ int moe_dispatch(const int* idx, int M, int k, int E, int align, int* offsets, i
     if (M > 0 && (!idx || !rows || !pos)) return -1;
     const size_t cap = moe_dispatch_rows(M, k, E, align);
     if (cap > 0x7fffffffu) return -2;
-    const int smem = (kOrderWarps * E + E + 1) * (int)sizeof(int);
-    if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute(dispatch_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-        return -5;
-    dispatch_kernel<<<1, kOrderThreads, smem, st>>>(idx, (long long)M * k, E, align, (long long)cap, offsets, counts,
-                                                    rows, pos);
+    const long long P = (long long)M * k;
+    const int smem = (kOrderWarps * E + 3 * E + 1 + kOrderWarps) * (int)sizeof(int);
+    auto go = [&](auto ctas) {
+        constexpr int CTAS = decltype(ctas)::value;
+        auto f = dispatch_kernel<CTAS>;
+        if (smem > 48 * 1024 &&
+            cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+            return;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(CTAS);
+        cfg.blockDim = dim3(kOrderThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        cudaLaunchAttribute at;
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = CTAS;
+        at.val.clusterDim.y = at.val.clusterDim.z = 1;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+        cudaLaunchKernelEx(&cfg, f, idx, P, E, align, (long long)cap, offsets, counts, rows, pos);
+    };
+    if (P <= kOrderThreads) go(std::integral_constant<int, 1>());
+    else go(std::integral_constant<int, 8>());
     return launched();
 }
 
@@ -391,8 +671,21 @@ int moe_combine(const void* o, int dtype, long long ld_o, const int* pos, const 
         return -1;
     if (M == 0) return 0;
     if (!o || !pos || !y) return -1;
-    combine_kernel<<<dim3((unsigned)M, (unsigned)((D + 1023) / 1024)), 256, 0, st>>>(o, dtype, ld_o, pos, w, k, D, y,
-                                                                                 ld_y);
+    const bool vec = rows16(o, ld_o, dtype) && rows16(y, ld_y, dtype) && D % (dtype == kBF16 ? 8 : 4) == 0;
+    auto go = [&](auto zero, auto width) {
+        using T = decltype(zero);
+        constexpr int W = decltype(width)::value;
+        const int cols = (D + W - 1) / W, threads = cols < 128 ? (cols + 31) / 32 * 32 : 128;
+        combine_kernel<T, W><<<dim3((unsigned)M, (unsigned)((cols + threads - 1) / threads)), threads, 0, st>>>(
+            (const T*)o, ld_o, pos, w, k, D, (T*)y, ld_y);
+    };
+    if (dtype == kBF16) {
+        if (vec) go(__nv_bfloat16(), std::integral_constant<int, 8>());
+        else go(__nv_bfloat16(), std::integral_constant<int, 1>());
+    } else {
+        if (vec) go(0.f, std::integral_constant<int, 4>());
+        else go(0.f, std::integral_constant<int, 1>());
+    }
     return launched();
 }
 
@@ -405,8 +698,21 @@ int moe_combine_bwd(const void* dy, const void* o, int dtype, long long ld_dy, l
     if (!dy || !rows || !pos || !d_o || (dw && !o)) return -1;
     const long long warps = R > 0 ? R : 1;
     const long long blocks = (warps + 7) / 8, most = (long long)num_sms() * 8;
-    combine_bwd_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(
-        dy, o, dtype, ld_dy, ld_o, rows, pos, w, (long long)M * k, k, R, D, d_o, ld_do, dw);
+    const bool vec = rows16(dy, ld_dy, dtype) && (!o || rows16(o, ld_o, dtype)) && rows16(d_o, ld_do, dtype) &&
+                     D % (dtype == kBF16 ? 8 : 4) == 0;
+    auto go = [&](auto zero, auto width) {
+        using T = decltype(zero);
+        constexpr int W = decltype(width)::value;
+        combine_bwd_kernel<T, W><<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(
+            (const T*)dy, (const T*)o, ld_dy, ld_o, rows, pos, w, (long long)M * k, k, R, D, (T*)d_o, ld_do, dw);
+    };
+    if (dtype == kBF16) {
+        if (vec) go(__nv_bfloat16(), std::integral_constant<int, 8>());
+        else go(__nv_bfloat16(), std::integral_constant<int, 1>());
+    } else {
+        if (vec) go(0.f, std::integral_constant<int, 4>());
+        else go(0.f, std::integral_constant<int, 1>());
+    }
     return launched();
 }
 
