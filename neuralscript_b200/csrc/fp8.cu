@@ -11,11 +11,11 @@
 // makes the scale infinite and the whole block NaN when it is read back.
 //
 // One block of threads takes 128 x 128 values, so that one read of x serves
-// both orientations and all three forms of scales. A half-warp owns 8 rows: a
-// lane 8 columns (one 16-byte load of bf16 a row), so row maxima are 4
-// shuffles and the 8 codes of a column are one 8-byte word of the transpose,
-// which goes through 16 KB of shared memory, the words of a column exchanged
-// (unit ^ column / 8) so that neither side has bank conflicts.
+// both orientations and all three forms of scales. A half-warp owns 4 rows, a
+// lane 8 columns of them (one 16-byte load of bf16 a row), so row maxima are 4
+// shuffles and the 4 codes of a column are one word of the transpose, which
+// goes through 16 KB of shared memory, the words of a column exchanged
+// (word ^ 2 (column / 8)) so that neither side has bank conflicts.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
@@ -49,25 +49,64 @@ __device__ __forceinline__ void store8(uint8_t* dst, uint2 v, int n) {
         if (i < n) dst[i] = (uint8_t)((i < 4 ? v.x >> 8 * i : v.y >> 8 * (i - 4)) & 0xff);
 }
 
-// act_fwd with the code known, and GELU's division by sqrt(2) as a
-// multiplication (a last bit's difference, a third of the instructions)
-template <int ACT>
-__device__ __forceinline__ float activate(float x) {
-    return act_fwd(x, ACT == kGelu ? kGeluMoe : ACT);
+__device__ __forceinline__ float ex2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
+// x Phi(x) without erff's branches: Phi(-a) = erfc(z) / 2 for z = a / sqrt(2),
+// erfc(z) = exp(-z^2) erfcx(z), and erfcx(z) = t P(t) with t = 1 / (1 + 0.38 z)
+// and a polynomial of degree 6 fitted for this code (Lawson-weighted least
+// squares over z in [0, 10]; relative error below 1.4e-6, also far out on the
+// negative side, where 1 + erf would cancel).
+// Two values at a time on packed fp32 pairs, which halves the FMA
+// instructions that bound this pass.
+__device__ __forceinline__ void gelu_tail2(float& x0, float& x1) {
+    const uint64_t a = f2_pack(fabsf(x0), fabsf(x1));
+    const uint64_t z = f2_mul(a, f2_pack(0.70710678f, 0.70710678f));
+    float d0, d1, e0, e1;
+    f2_unpack(f2_fma(z, f2_pack(0.38f, 0.38f), f2_pack(1.f, 1.f)), d0, d1);
+    f2_unpack(f2_mul(f2_mul(z, z), f2_pack(-1.44269504f, -1.44269504f)), e0, e1);
+    const uint64_t t = f2_pack(rcp_approx(d0), rcp_approx(d1));
+    const uint64_t e = f2_pack(ex2_approx(e0), ex2_approx(e1));
+    auto c = [](float v) { return f2_pack(v, v); };
+    uint64_t q = c(-0.125199478f);
+    q = f2_fma(q, t, c(0.335197723f));
+    q = f2_fma(q, t, c(-0.068613310f));
+    q = f2_fma(q, t, c(0.246798871f));
+    q = f2_fma(q, t, c(0.181039411f));
+    q = f2_fma(q, t, c(0.216480016f));
+    q = f2_fma(q, t, c(0.214295747f));
+    q = f2_mul(q, f2_mul(t, e));
+    f2_unpack(f2_fma(f2_mul(a, c(-0.5f)), q, f2_pack(fmaxf(x0, 0.f), fmaxf(x1, 0.f))), x0, x1);
+}
+
+template <int ACT>
+__device__ __forceinline__ float activate(float x) {
+    if constexpr (ACT == kSilu) return x * rcp_approx(1.f + ex2_approx(x * -1.44269504f));
+    else return act_fwd(x, ACT);
+}
+
+constexpr int kThreads = 512;
+
 template <typename T, bool BLOCK, bool VEC, int ACT>
-__global__ void __launch_bounds__(256, 2) quantize_kernel(const QuantDesc d) {
-    __shared__ uint2 tile[128 * 16];   // [column][unit of 8 rows]
-    __shared__ float part[16][128];    // column maxima of the 16 half-warps
+__global__ void __launch_bounds__(kThreads, 2) quantize_kernel(const QuantDesc d) {
+    __shared__ __align__(8) uint32_t tile[128 * 32];  // [column][word of 4 rows]
+    __shared__ float part[16][128];      // column maxima of the 16 warps
     __shared__ float inv[128];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int half = warp * 2 + (lane >> 4);  // 0..15: rows 8 half ..
+    const int half = warp * 2 + (lane >> 4);  // 0..31: rows 4 half ..
     const int cl = lane & 15;
-    const int r0 = blockIdx.y * 128 + half * 8, c0 = blockIdx.x * 128 + cl * 8;
-    float v[8][8];
+    const int r0 = blockIdx.y * 128 + half * 4, c0 = blockIdx.x * 128 + cl * 8;
+    float v[4][8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < 4; i++) {
         const int r = r0 + i;
         long long src = r;
         if (d.rows && r < d.M) {
@@ -94,14 +133,21 @@ __global__ void __launch_bounds__(256, 2) quantize_kernel(const QuantDesc d) {
     }
     if (ACT) {
 #pragma unroll
-        for (int i = 0; i < 8; i++)
+        for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[i][j] = activate<ACT>(v[i][j]);
+            for (int j = 0; j < 8; j += 2) {
+                if constexpr (ACT == kGelu) {
+                    gelu_tail2(v[i][j], v[i][j + 1]);
+                } else {
+                    v[i][j] = activate<ACT>(v[i][j]);
+                    v[i][j + 1] = activate<ACT>(v[i][j + 1]);
+                }
+            }
     }
     if constexpr (BLOCK) {
         float m = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; i++)
+        for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(v[i][j]));
 #pragma unroll
@@ -109,19 +155,19 @@ __global__ void __launch_bounds__(256, 2) quantize_kernel(const QuantDesc d) {
         if (lane == 0) part[0][warp] = m;
         __syncthreads();
 #pragma unroll
-        for (int q = 0; q < 8; q++) m = fmaxf(m, part[0][q]);
+        for (int q = 0; q < kThreads / 32; q++) m = fmaxf(m, part[0][q]);
         const float s = scale_of(m), k = 1.f / s;
         if (threadIdx.x == 0) {
             if (d.s) d.s[blockIdx.y * d.ld_s + blockIdx.x] = s;
             if (d.st) d.st[blockIdx.x * d.ld_st + blockIdx.y] = s;
         }
 #pragma unroll
-        for (int i = 0; i < 8; i++)
+        for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int j = 0; j < 8; j++) v[i][j] *= k;
         if (d.q) {
 #pragma unroll
-            for (int i = 0; i < 8; i++)
+            for (int i = 0; i < 4; i++)
                 if (r0 + i < d.M)
                     store8(d.q + (size_t)(r0 + i) * d.ld_q + c0,
                            make_uint2(code4(v[i][0], v[i][1], v[i][2], v[i][3]),
@@ -131,25 +177,30 @@ __global__ void __launch_bounds__(256, 2) quantize_kernel(const QuantDesc d) {
         if (!d.qt) return;
 #pragma unroll
         for (int j = 0; j < 8; j++)
-            tile[(cl * 8 + j) * 16 + (half ^ cl)] = make_uint2(code4(v[0][j], v[1][j], v[2][j], v[3][j]),
-                                                              code4(v[4][j], v[5][j], v[6][j], v[7][j]));
+            tile[(cl * 8 + j) * 32 + (half ^ (cl * 2))] = code4(v[0][j], v[1][j], v[2][j], v[3][j]);
     } else {
         if (d.q) {
+            // lane i of the half-warp turns the maximum of row i into its scale
+            float mine = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
+            for (int i = 0; i < 4; i++) {
                 float m = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(v[i][j]));
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
-                const float s = scale_of(m), k = 1.f / s;
-                if (r0 + i < d.M) {
-                    if (cl == 0) d.s[blockIdx.x * d.ld_s + r0 + i] = s;
+                if (cl == i) mine = m;
+            }
+            const float s = scale_of(mine), inverse = 1.f / s;
+            if (cl < 4 && r0 + cl < d.M) d.s[blockIdx.x * d.ld_s + r0 + cl] = s;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float k = __shfl_sync(kAll, inverse, (lane & 16) + i);
+                if (r0 + i < d.M)
                     store8(d.q + (size_t)(r0 + i) * d.ld_q + c0,
                            make_uint2(code4(v[i][0] * k, v[i][1] * k, v[i][2] * k, v[i][3] * k),
                                       code4(v[i][4] * k, v[i][5] * k, v[i][6] * k, v[i][7] * k)),
                            d.K - c0);
-                }
             }
         }
         if (!d.qt) return;
@@ -157,34 +208,36 @@ __global__ void __launch_bounds__(256, 2) quantize_kernel(const QuantDesc d) {
         for (int j = 0; j < 8; j++) {
             float m = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[i][j]));
-            part[half][cl * 8 + j] = m;
+            for (int i = 0; i < 4; i++) m = fmaxf(m, fabsf(v[i][j]));
+            m = fmaxf(m, __shfl_xor_sync(kAll, m, 16));
+            if (lane < 16) part[warp][j * 16 + cl] = m;  // column cl * 8 + j
         }
         __syncthreads();
         if (threadIdx.x < 128) {
             float m = 0.f;
 #pragma unroll
-            for (int q = 0; q < 16; q++) m = fmaxf(m, part[q][threadIdx.x]);
+            for (int q = 0; q < kThreads / 32; q++) m = fmaxf(m, part[q][threadIdx.x]);
             const float s = scale_of(m);
             inv[threadIdx.x] = 1.f / s;
-            const int c = blockIdx.x * 128 + threadIdx.x;
+            const int c = blockIdx.x * 128 + (threadIdx.x & 15) * 8 + (threadIdx.x >> 4);
             if (c < d.K) d.st[blockIdx.y * d.ld_st + c] = s;
         }
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float k = inv[cl * 8 + j];
-            tile[(cl * 8 + j) * 16 + (half ^ cl)] =
-                make_uint2(code4(v[0][j] * k, v[1][j] * k, v[2][j] * k, v[3][j] * k),
-                           code4(v[4][j] * k, v[5][j] * k, v[6][j] * k, v[7][j] * k));
+            const float k = inv[j * 16 + cl];
+            tile[(cl * 8 + j) * 32 + (half ^ (cl * 2))] =
+                code4(v[0][j] * k, v[1][j] * k, v[2][j] * k, v[3][j] * k);
         }
     }
     __syncthreads();
     const int r = blockIdx.y * 128 + cl * 8;
-    for (int c = half; c < 128; c += 16) {
+#pragma unroll
+    for (int c = half; c < 128; c += kThreads / 16) {
         const int col = blockIdx.x * 128 + c;
         if (col < d.K && r < d.M)
-            store8(d.qt + (size_t)col * d.ld_qt + r, tile[c * 16 + (cl ^ (c >> 3))], d.M - r);
+            store8(d.qt + (size_t)col * d.ld_qt + r,
+                   *reinterpret_cast<const uint2*>(tile + c * 32 + ((cl * 2) ^ ((c >> 3) * 2))), d.M - r);
     }
 }
 
@@ -208,11 +261,11 @@ int quantize(const QuantDesc& d, cudaStream_t st) {
     auto go = [&](auto act) {
         constexpr int ACT = decltype(act)::value;
         if (f) {
-            if (vec) quantize_kernel<float, BLOCK, true, ACT><<<grid, 256, 0, st>>>(d);
-            else quantize_kernel<float, BLOCK, false, ACT><<<grid, 256, 0, st>>>(d);
+            if (vec) quantize_kernel<float, BLOCK, true, ACT><<<grid, kThreads, 0, st>>>(d);
+            else quantize_kernel<float, BLOCK, false, ACT><<<grid, kThreads, 0, st>>>(d);
         } else {
-            if (vec) quantize_kernel<__nv_bfloat16, BLOCK, true, ACT><<<grid, 256, 0, st>>>(d);
-            else quantize_kernel<__nv_bfloat16, BLOCK, false, ACT><<<grid, 256, 0, st>>>(d);
+            if (vec) quantize_kernel<__nv_bfloat16, BLOCK, true, ACT><<<grid, kThreads, 0, st>>>(d);
+            else quantize_kernel<__nv_bfloat16, BLOCK, false, ACT><<<grid, kThreads, 0, st>>>(d);
         }
     };
     if constexpr (BLOCK) {

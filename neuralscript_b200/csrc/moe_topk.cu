@@ -472,22 +472,25 @@ struct Pack<__nv_bfloat16> {
     }
 };
 
-// W columns (16 bytes, or 1 where rows do not start on 16-byte boundaries) of
-// a row: ncol of them there.
+// W columns of a row (16 bytes, or 1 column where rows do not start on 16-byte
+// boundaries) as they are loaded, and as floats.
 template <typename T, int W>
-__device__ __forceinline__ void load_cols(const T* p, float* f) {
-    if constexpr (W == 1) f[0] = (float)*p;
-    else Pack<T>::get(__ldg(reinterpret_cast<const uint4*>(p)), f);
-}
-template <typename T, int W>
-__device__ __forceinline__ void store_cols(T* p, const float* f) {
-    if constexpr (W == 1) {
+struct Cols {
+    uint4 v;
+    __device__ __forceinline__ void load(const T* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void get(float* f) const { Pack<T>::get(v, f); }
+    __device__ static __forceinline__ void store(T* p, const float* f) { *reinterpret_cast<uint4*>(p) = Pack<T>::put(f); }
+};
+template <typename T>
+struct Cols<T, 1> {
+    float v;
+    __device__ __forceinline__ void load(const T* p) { v = (float)*p; }
+    __device__ __forceinline__ void get(float* f) const { f[0] = v; }
+    __device__ static __forceinline__ void store(T* p, const float* f) {
         if constexpr (sizeof(T) == 2) *p = f2bf(f[0]);
         else *p = f[0];
-    } else {
-        *reinterpret_cast<uint4*>(p) = Pack<T>::put(f);
     }
-}
+};
 
 // A thread sums W columns of a token; the rows of four choices are in flight
 // together.
@@ -502,24 +505,27 @@ __global__ void __launch_bounds__(128)
 #pragma unroll
     for (int i = 0; i < W; i++) acc[i] = 0.f;
     for (int j0 = 0; j0 < k; j0 += 4) {
-        float f[4][W], wj[4];
+        Cols<T, W> in[4];
+        float wj[4];
+        int p[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const int p = j0 + j < k ? pos[t * k + j0 + j] : -1;
-            wj[j] = p < 0 ? 0.f : w ? w[t * k + j0 + j] : 1.f;
-            if (p >= 0) {
-                load_cols<T, W>(o + (size_t)p * ld_o + c, f[j]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < W; i++) f[j][i] = 0.f;
-            }
+            p[j] = j0 + j < k ? pos[t * k + j0 + j] : -1;
+            wj[j] = p[j] >= 0 && w ? w[t * k + j0 + j] : 1.f;
         }
 #pragma unroll
         for (int j = 0; j < 4; j++)
+            if (p[j] >= 0) in[j].load(o + (size_t)p[j] * ld_o + c);
 #pragma unroll
-            for (int i = 0; i < W; i++) acc[i] = fmaf(wj[j], f[j][i], acc[i]);
+        for (int j = 0; j < 4; j++) {
+            if (p[j] < 0) continue;
+            float f[W];
+            in[j].get(f);
+#pragma unroll
+            for (int i = 0; i < W; i++) acc[i] = fmaf(wj[j], f[i], acc[i]);
+        }
     }
-    store_cols<T, W>(y + t * ld_y + c, acc);
+    Cols<T, W>::store(y + t * ld_y + c, acc);
 }
 
 // One warp a row of the ordered outputs: o and d_o stream, the tokens' dy,
@@ -535,14 +541,16 @@ __global__ void __launch_bounds__(256)
         for (long long p = gt; p < P; p += step)
             if (pos[p] < 0) dw[p] = 0.f;
     const int lane = threadIdx.x & 31;
+    int next = gt >> 5 < R ? rows[gt >> 5] : -1;
     for (long long r = gt >> 5; r < R; r += step >> 5) {
-        const int pair = rows[r];
+        const int pair = next;
+        if (r + (step >> 5) < R) next = rows[r + (step >> 5)];
         T* to = d_o + (size_t)r * ld_do;
         if (pair < 0) {
             float zero[W];
 #pragma unroll
             for (int i = 0; i < W; i++) zero[i] = 0.f;
-            for (int c = lane * W; c < D; c += 32 * W) store_cols<T, W>(to + c, zero);
+            for (int c = lane * W; c < D; c += 32 * W) Cols<T, W>::store(to + c, zero);
             continue;
         }
         const float wp = w ? w[pair] : 1.f;
@@ -550,25 +558,29 @@ __global__ void __launch_bounds__(256)
         const T* f = o + (size_t)r * ld_o;
         float acc = 0.f;
         for (int c0 = lane * W; c0 < D; c0 += 4 * 32 * W) {
-            float gv[4][W], fv[4][W];
+            Cols<T, W> gv[4], fv[4];
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 const int c = c0 + q * 32 * W;
                 if (c >= D) continue;
-                load_cols<T, W>(g + c, gv[q]);
-                if (dw) load_cols<T, W>(f + c, fv[q]);
+                if (dw) fv[q].load(f + c);
+                gv[q].load(g + c);
             }
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 const int c = c0 + q * 32 * W;
                 if (c >= D) continue;
-                float out[W];
+                float gf[W], out[W];
+                gv[q].get(gf);
+                if (dw) {
+                    float ff[W];
+                    fv[q].get(ff);
 #pragma unroll
-                for (int i = 0; i < W; i++) {
-                    if (dw) acc = fmaf(gv[q][i], fv[q][i], acc);
-                    out[i] = wp * gv[q][i];
+                    for (int i = 0; i < W; i++) acc = fmaf(gf[i], ff[i], acc);
                 }
-                store_cols<T, W>(to + c, out);
+#pragma unroll
+                for (int i = 0; i < W; i++) out[i] = wp * gf[i];
+                Cols<T, W>::store(to + c, out);
             }
         }
         if (dw) {
