@@ -151,6 +151,26 @@ __device__ __forceinline__ Unit unit_at(const TileParams& p, const int* start, i
     return w;
 }
 
+// First tile of every group (tiles of `rows` rows) into start[0..groups], by
+// one warp.
+__device__ __forceinline__ void group_starts(const TileParams& p, int rows, int* start, int lane) {
+    int run = 0;
+    for (int g0 = 0; g0 < p.groups; g0 += 32) {
+        const int g = g0 + lane;
+        int n = 0;
+        if (g < p.groups) n = (max(0, min(p.counts[g], p.M - p.offsets[g])) + rows - 1) / rows;
+        int inc = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += t;
+        }
+        if (g < p.groups) start[g] = run + inc - n;
+        run += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) start[p.groups] = run;
+}
+
 template <int BN, bool VEC, bool ROWS>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_tile_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
@@ -168,8 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* slot_full = part_empty + C::PARTS;
     uint64_t* slot_empty = slot_full + kSlots;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(slot_empty + kSlots);
-    int* total_slot = reinterpret_cast<int*>(tmem_slot + 1);
-    int* dead = total_slot + 1;
+    int* dead = reinterpret_cast<int*>(tmem_slot + 1);
     int* start = reinterpret_cast<int*>(staging + C::STAGING + C::SCALES + 512);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -196,31 +215,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         ptx::tmem_alloc(tmem_slot, 512);
         ptx::tmem_relinquish();
     }
-    if (ROWS && warp == 4) {  // first tile of every group
-        int run = 0;
-        for (int g0 = 0; g0 < p.groups; g0 += 32) {
-            const int g = g0 + lane;
-            int n = 0;
-            if (g < p.groups) n = (max(0, min(p.counts[g], p.M - p.offsets[g])) + 127) / 128;
-            int inc = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int t = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += t;
-            }
-            if (g < p.groups) start[g] = run + inc - n;
-            run += __shfl_sync(0xffffffffu, inc, 31);
-        }
-        if (lane == 0) {
-            start[p.groups] = run;
-            *total_slot = run * p.n_tiles;
-        }
-    }
+    if (ROWS && warp == 4) group_starts(p, 128, start, lane);
     ptx::tc_fence_before();
     __syncthreads();
     ptx::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int total = ROWS ? *total_slot : p.m_tiles * p.n_tiles * (p.groups ? p.groups : 1);
+    const int total = ROWS ? start[p.groups] * p.n_tiles : p.m_tiles * p.n_tiles * (p.groups ? p.groups : 1);
 
     if (warp == 1 || warp == 2) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -496,6 +496,345 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
+// ---------------------------------------------------------------------------
+// Few rows of A (or few for each expert): the sides change places. 128 rows of
+// B, the weights, are the MMA's rows and BN rows of A its columns, so a tile
+// reads no more than the weights and what there is of A. What bounds it is
+// the stream of the weights, so everything serves loads in flight: a deep
+// ring, eight parts of TMEM, and for one product the k-blocks of a tile split
+// over a cluster of CTAs, whose sums meet in shared memory in rank order.
+//   warp 0       weights by TMA
+//   warp 1       MMA issuer
+//   warps 2..3   rows of A by cp.async (listed, or in order) and the scales
+//   warps 4..7   a warp owns 32 weight rows: scales and adds, stores
+// ---------------------------------------------------------------------------
+template <int BN, bool VEC>
+struct SmallCfg {
+    static constexpr int W_BYTES = 128 * 128;
+    static constexpr int STAGE = W_BYTES + BN * 128;
+    static constexpr int STAGES = BN == 64 ? 8 : (BN == 32 ? 9 : 10);
+    static constexpr int PARTS = 8;
+    static constexpr int SLOTK = 4;
+    static constexpr int SLOT = BN + (VEC ? 128 : 4);  // scales of A's rows, then of B's rows or block
+    static constexpr int SCALES = kSlots * SLOTK * SLOT * 4;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + SCALES + 512 + (kMaxGroups + 1) * 4;
+    static_assert(SMEM <= 227 * 1024, "above the shared memory of a block");
+    static_assert(BN * 128 * 4 <= STAGES * STAGE, "the cluster's sums take the ring's place");
+};
+
+struct SmallParams {
+    TileParams t;  // M: rows of A in order; N: weight rows
+    int split;     // CTAs of a cluster that share a tile's k-blocks
+};
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float cluster_loadf(const float* p, unsigned rank) {
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(ptx::smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+
+template <int BN>
+__device__ __forceinline__ Unit small_unit(const TileParams& p, const int* start, int u) {
+    Unit w;
+    int t = u / p.n_tiles;
+    w.n0 = u % p.n_tiles * 128;
+    w.kb0 = 0;
+    w.kb1 = (p.K + 127) / 128;
+    w.g = 0;
+    w.m0 = t * BN;
+    w.row_end = p.M;
+    if (p.groups) {
+        int lo = 0, hi = p.groups;  // start[lo] <= t < start[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (start[mid] <= t) lo = mid;
+            else hi = mid;
+        }
+        w.g = lo;
+        const int off = p.offsets[lo];
+        w.m0 = off + (t - start[lo]) * BN;
+        w.row_end = min(p.M, off + p.counts[lo]);
+    }
+    return w;
+}
+
+template <int BN, bool VEC>
+__global__ void __launch_bounds__(256, 1)
+    fp8_small_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ SmallParams sp) {
+    using C = SmallCfg<BN, VEC>;
+    const TileParams& p = sp.t;
+    constexpr uint32_t IDESC = ptx::instr_desc(0, 0, 0, 128, BN);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float* slots = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE + C::SCALES);
+    uint64_t* empty = full + C::STAGES;
+    uint64_t* part_full = empty + C::STAGES;
+    uint64_t* part_empty = part_full + C::PARTS;
+    uint64_t* slot_full = part_empty + C::PARTS;
+    uint64_t* slot_empty = slot_full + kSlots;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(slot_empty + kSlots);
+    int* dead = reinterpret_cast<int*>(tmem_slot + 1);
+    int* start = reinterpret_cast<int*>(smem + C::STAGES * C::STAGE + C::SCALES + 512);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        *dead = 0;
+        for (int s = 0; s < C::STAGES; s++) {
+            ptx::mbar_init(&full[s], 65);
+            ptx::mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < C::PARTS; s++) {
+            ptx::mbar_init(&part_full[s], 1);
+            ptx::mbar_init(&part_empty[s], 4);
+        }
+        for (int s = 0; s < kSlots; s++) {
+            ptx::mbar_init(&slot_full[s], 64);
+            ptx::mbar_init(&slot_empty[s], 4);
+        }
+        ptx::fence_mbar_init();
+        ptx::prefetch_tmap(&tw);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc(tmem_slot, C::PARTS * BN);
+        ptx::tmem_relinquish();
+    }
+    if (p.groups && warp == 4) group_starts(p, BN, start, lane);
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int total = (p.groups ? start[p.groups] : p.m_tiles) * p.n_tiles;
+    // a cluster takes one tile, rank r the r-th share of its k-blocks; without
+    // clusters the CTAs take tiles in turn
+    const int rank = sp.split > 1 ? blockIdx.x % sp.split : 0;
+    const int first = sp.split > 1 ? blockIdx.x / sp.split : blockIdx.x;
+    const int stride = sp.split > 1 ? total : gridDim.x;
+    const int kblocks = (p.K + 127) / 128, share = (kblocks + sp.split - 1) / sp.split;
+    const int kb0 = min(kblocks, rank * share), kb1 = min(kblocks, kb0 + share);
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const Pipe pipe{dead, p.err, kErrTimeoutProducer};
+            int stage = 0;
+            uint32_t phase = 0;
+            for (int u = first; u < total; u += stride) {
+                const Unit w = small_unit<BN>(p, start, u);
+                for (int kb = kb0; kb < kb1; kb++) {
+                    pipe.wait(&empty[stage], phase ^ 1);
+                    ptx::mbar_arrive_expect_tx(&full[stage], C::W_BYTES);
+                    ptx::tma_load_3d(smem + stage * C::STAGE, &tw, &full[stage], kb * 128, w.n0, w.g);
+                    if (++stage == C::STAGES) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+            // every load has landed and been used before the CTA exits (bounded)
+            for (int s = 0; s < C::STAGES; s++) {
+                pipe.wait(&empty[stage], phase ^ 1);
+                if (++stage == C::STAGES) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const Pipe pipe{dead, p.err, kErrTimeoutMma};
+            int stage = 0, part = 0;
+            uint32_t phase = 0, part_phase = 0;
+            for (int u = first; u < total; u += stride)
+                for (int kb = kb0; kb < kb1; kb++) {
+                    pipe.wait(&full[stage], phase);
+                    pipe.wait(&part_empty[part], part_phase ^ 1);
+                    ptx::fence_proxy_async();  // A's rows came through the generic proxy
+                    ptx::tc_fence_after();
+                    const uint32_t sw = ptx::smem_u32(smem + stage * C::STAGE), sa = sw + C::W_BYTES;
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        ptx::mma_f8(tmem + part * BN, ptx::smem_desc(sw + k * 32, 16, 1024, 2),
+                                    ptx::smem_desc(sa + k * 32, 16, 1024, 2), IDESC, k > 0);
+                    ptx::mma_commit(&empty[stage]);
+                    ptx::mma_commit(&part_full[part]);
+                    if (++stage == C::STAGES) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                    if (++part == C::PARTS) {
+                        part = 0;
+                        part_phase ^= 1;
+                    }
+                }
+        }
+        __syncwarp();
+    } else if (warp < 4) {
+        const Pipe pipe{dead, p.err, kErrTimeoutProducer};
+        const int t = threadIdx.x - 64;  // 0..63
+        int slot = 0, stage = 0;
+        uint32_t slot_phase = 0, phase = 0;
+        auto source = [&](const Unit& w, int i) {  // row of A behind row i of the tile, -1 past the end
+            const int m = w.m0 + i;
+            if (m >= w.row_end) return -1;
+            return p.rows ? min(max(0, p.rows[m]) / p.row_div, p.a_rows - 1) : m;
+        };
+        for (int u = first; u < total; u += stride) {
+            const Unit w = small_unit<BN>(p, start, u);
+            constexpr int PIECES = BN / 8;  // 16-byte pieces of a k-block that this thread copies
+            int arow[PIECES];
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) arow[i] = source(w, t / 8 + 8 * i);
+            const float* srow = p.sa + max(0, source(w, min(t, BN - 1)));
+            const float* sb = p.sb + w.g * p.sb_stride;
+            if (!VEC) sb += (long long)(w.n0 / 128) * p.ld_sb;
+            for (int kb = kb0; kb < kb1; kb++) {
+                const int in = (kb - kb0) % C::SLOTK;
+                if (in == 0) pipe.wait(&slot_empty[slot], slot_phase ^ 1);
+                float* to = slots + (slot * C::SLOTK + in) * C::SLOT;
+                if (t < BN) ptx::cp_async4(to + t, srow + kb * p.ld_sa);
+                if (VEC) {
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const int n = w.n0 + t + 64 * i;
+                        if (n < p.N) ptx::cp_async4(to + BN + t + 64 * i, sb + kb * p.ld_sb + n);
+                    }
+                } else if (t == 0) {
+                    ptx::cp_async4(to + BN, sb + kb);
+                }
+                if (in == C::SLOTK - 1 || kb + 1 == kb1) {
+                    ptx::cp_async_arrive(&slot_full[slot]);
+                    if (++slot == kSlots) {
+                        slot = 0;
+                        slot_phase ^= 1;
+                    }
+                }
+                pipe.wait(&empty[stage], phase ^ 1);
+                uint8_t* sa = smem + stage * C::STAGE + C::W_BYTES;
+                const int k = kb * 128 + (t & 7) * 16;
+                const int bytes = max(0, min(16, p.K - k));
+#pragma unroll
+                for (int i = 0; i < PIECES; i++) {
+                    const int r = t / 8 + 8 * i;  // r % 8 = t / 8: the swizzle's row
+                    const bool on = arow[i] >= 0 && bytes > 0;
+                    ptx::cp_async16(sa + r * 128 + (((t & 7) ^ (t >> 3)) << 4),
+                                    on ? p.a + (size_t)arow[i] * p.lda + k : p.a, on ? bytes : 0);
+                }
+                ptx::cp_async_arrive(&full[stage]);
+                if (++stage == C::STAGES) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+        }
+        ptx::cp_async_wait_all();
+        __syncwarp();
+    } else {
+        const Pipe pipe{dead, p.err, kErrTimeoutEpilogue};
+        const int quarter = warp & 3;
+        int part = 0, slot = 0;
+        uint32_t part_phase = 0, slot_phase = 0;
+        for (int u = first; u < total; u += stride) {
+            const Unit w = small_unit<BN>(p, start, u);
+            const int n_in = quarter * 32 + lane, n = w.n0 + n_in;
+            float acc[BN];
+#pragma unroll
+            for (int j = 0; j < BN; j++) acc[j] = 0.f;
+            int in = 0;
+            for (int kb = kb0; kb < kb1; kb++) {
+                if (in == 0) pipe.wait(&slot_full[slot], slot_phase);
+                const float* sc = slots + (slot * C::SLOTK + in) * C::SLOT;
+                const float s = VEC ? sc[BN + n_in] : sc[BN];
+                pipe.wait(&part_full[part], part_phase);
+                __syncwarp();
+                ptx::tc_fence_after();
+                const uint32_t t = tmem + ((uint32_t)(quarter * 32) << 16) + part * BN;
+                uint32_t r[2][16];
+                ptx::tmem_ld16(t, r[0]);
+#pragma unroll
+                for (int c = 0; c < BN / 16; c++) {
+                    float m[16];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float4 q = reinterpret_cast<const float4*>(sc)[c * 4 + j];
+                        m[4 * j] = q.x * s;
+                        m[4 * j + 1] = q.y * s;
+                        m[4 * j + 2] = q.z * s;
+                        m[4 * j + 3] = q.w * s;
+                    }
+                    ptx::tmem_ld_wait_regs16(r[c & 1]);
+                    if (c + 1 < BN / 16) ptx::tmem_ld16(t + (c + 1) * 16, r[(c + 1) & 1]);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) acc[c * 16 + j] = fmaf(__uint_as_float(r[c & 1][j]), m[j], acc[c * 16 + j]);
+                }
+                ptx::tc_fence_before();
+                __syncwarp();
+                ptx::mbar_arrive_if(&part_empty[part], lane == 0);
+                if (++in == C::SLOTK || kb + 1 == kb1) {
+                    ptx::mbar_arrive_if(&slot_empty[slot], lane == 0);
+                    in = 0;
+                    if (++slot == kSlots) {
+                        slot = 0;
+                        slot_phase ^= 1;
+                    }
+                }
+                if (++part == C::PARTS) {
+                    part = 0;
+                    part_phase ^= 1;
+                }
+            }
+            if (sp.split > 1) {
+                // (this CTA's loads have all been used: its last part was read)
+                float* sum = reinterpret_cast<float*>(smem);
+#pragma unroll
+                for (int j = 0; j < BN; j++) sum[j * 128 + n_in] = acc[j];
+                continue;
+            }
+#pragma unroll
+            for (int j = 0; j < BN; j++) {
+                const int m = w.m0 + j;
+                if (m < w.row_end && n < p.N) {
+                    if (p.c_dtype == kBF16) reinterpret_cast<__nv_bfloat16*>(p.c)[(size_t)m * p.ldc + n] = f2bf(acc[j]);
+                    else reinterpret_cast<float*>(p.c)[(size_t)m * p.ldc + n] = acc[j];
+                }
+            }
+        }
+    }
+
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem, C::PARTS * BN);
+    }
+    if (sp.split > 1) {
+        // the k-blocks' shares are added in rank order; rank r stores every
+        // split-th row of the tile
+        cluster_sync();
+        if (first < total) {
+            const Unit w = small_unit<BN>(p, start, first);
+            const float* sum = reinterpret_cast<const float*>(smem);
+            const int n_in = threadIdx.x & 127, n = w.n0 + n_in;
+            for (int j = rank * 2 + (threadIdx.x >> 7); j < BN; j += sp.split * 2) {
+                const int m = w.m0 + j;
+                if (m >= w.row_end) break;
+                float v = 0.f;
+                for (int r = 0; r < sp.split; r++) v += cluster_loadf(sum + j * 128 + n_in, r);
+                if (n < p.N) {
+                    if (p.c_dtype == kBF16) reinterpret_cast<__nv_bfloat16*>(p.c)[(size_t)m * p.ldc + n] = f2bf(v);
+                    else reinterpret_cast<float*>(p.c)[(size_t)m * p.ldc + n] = v;
+                }
+            }
+        }
+        cluster_sync();  // no CTA leaves while others read its sums
+    }
+}
+
 __global__ void fp8_zero_kernel(const Fp8Gemm d) {
     const size_t n = (size_t)d.M * d.N;
     for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) {
@@ -576,14 +915,7 @@ bool allow_smem(Kernel k, int bytes, bool* done) {
     return true;
 }
 
-template <int BN, bool VEC, bool ROWS>
-int launch_tiles(const Fp8Gemm& d, cudaStream_t st) {
-    using C = TileCfg<BN, VEC, ROWS>;
-    static bool done[kMaxDevices] = {};
-    auto k = fp8_tile_kernel<BN, VEC, ROWS>;
-    if (!allow_smem(k, C::SMEM, done)) return -5;
-    const int es = d.c_dtype == kBF16 ? 2 : 4;
-    const bool aligned = !(reinterpret_cast<uintptr_t>(d.c) & 15) && d.ldc * es % 16 == 0 && d.c_stride * es % 16 == 0;
+TileParams params(const Fp8Gemm& d, int bm, int bn) {
     TileParams p;
     p.M = d.M;
     p.N = d.N;
@@ -605,11 +937,56 @@ int launch_tiles(const Fp8Gemm& d, cudaStream_t st) {
     p.counts = d.counts;
     p.rows = d.rows;
     p.row_div = d.row_div;
-    p.m_tiles = (d.M + 127) / 128;
-    p.n_tiles = (d.N + BN - 1) / BN;
+    p.m_tiles = (d.M + bm - 1) / bm;
+    p.n_tiles = (d.N + bn - 1) / bn;
     p.nb = (d.N + 127) / 128;
-    p.vec_out = aligned;
+    p.tma_out = p.vec_out = 0;
     p.err = d.err;
+    return p;
+}
+
+template <int BN, bool VEC>
+int launch_small(const Fp8Gemm& d, cudaStream_t st) {
+    using C = SmallCfg<BN, VEC>;
+    static bool done[kMaxDevices] = {};
+    auto k = fp8_small_kernel<BN, VEC>;
+    if (!allow_smem(k, C::SMEM, done)) return -5;
+    SmallParams sp;
+    sp.t = params(d, BN, 128);
+    CUtensorMap tw;
+    if (!map_codes3(&tw, d.b, d.K, d.N, d.ldb, d.groups ? d.groups : 1, d.b_stride, 128)) return -2;
+    // tiles: of A's rows for each group at most one that is not full
+    const long long rows = d.groups ? (long long)d.M / BN + (d.M < d.groups ? d.M : d.groups) : sp.t.m_tiles;
+    const long long units = rows * sp.t.n_tiles;
+    if (units > 0x7fffffff) return -2;
+    const int sms = num_sms(), kblocks = (d.K + 127) / 128;
+    sp.split = 1;
+    if (!d.groups)
+        while (sp.split < 8 && units * sp.split * 2 <= sms && kblocks >= sp.split * 4) sp.split *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(sp.split > 1 ? units * sp.split : units < sms ? units : sms));
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = sp.split;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k, tw, sp) == cudaSuccess ? 0 : -5;
+}
+
+template <int BN, bool VEC, bool ROWS>
+int launch_tiles(const Fp8Gemm& d, cudaStream_t st) {
+    using C = TileCfg<BN, VEC, ROWS>;
+    static bool done[kMaxDevices] = {};
+    auto k = fp8_tile_kernel<BN, VEC, ROWS>;
+    if (!allow_smem(k, C::SMEM, done)) return -5;
+    const int es = d.c_dtype == kBF16 ? 2 : 4;
+    const bool aligned = !(reinterpret_cast<uintptr_t>(d.c) & 15) && d.ldc * es % 16 == 0 && d.c_stride * es % 16 == 0;
+    TileParams p = params(d, 128, BN);
+    p.vec_out = aligned;
     CUtensorMap ta, tb, tc;
     memset(&tc, 0, sizeof(tc));
     if (!map_codes2(&ta, d.a, d.K, d.a_rows, d.lda, 128)) return -2;
@@ -647,6 +1024,18 @@ int fp8_gemm(const Fp8Gemm& d, cudaStream_t st) {
     if (d.groups && (!d.offsets || !d.counts)) return -1;
     if (d.rows && d.row_div <= 0) return -1;
     if (d.a_rows <= 0) return -1;
+    if (!d.group_k) {
+        // Few rows: the weights' stream bounds the product. For one product,
+        // where 128 x 256 tiles would not fill half of the SMs; for groups,
+        // where the average one has no more than 64 rows.
+        const long long tiles = (long long)((d.M + 127) / 128) * ((d.N + 255) / 256);
+        const int rows = d.groups ? (d.M + d.groups - 1) / d.groups : d.M;
+        if (d.groups ? rows <= 64 : tiles * 2 <= num_sms()) {
+            if (rows <= 16) return d.b_rows ? launch_small<16, true>(d, st) : launch_small<16, false>(d, st);
+            if (rows <= 32) return d.b_rows ? launch_small<32, true>(d, st) : launch_small<32, false>(d, st);
+            return d.b_rows ? launch_small<64, true>(d, st) : launch_small<64, false>(d, st);
+        }
+    }
     if (d.groups && !d.group_k) return launch_tiles<256, false, true>(d, st);
     return d.b_rows ? launch_tiles<256, true, false>(d, st) : launch_tiles<256, false, false>(d, st);
 }
