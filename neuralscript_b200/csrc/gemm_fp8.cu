@@ -36,7 +36,7 @@ namespace {
 //   warps 4..11  a warp owns 32 rows and half the columns: scales and adds
 //                every k-block's part, stores the tile
 // The accumulators of a 128 x 256 tile are 128 registers a thread, so the
-// first four warps give theirs up: 56 + 2 * 224 of the 3 * 168 registers that
+// first four warps give theirs up: 72 + 2 * 216 of the 3 * 168 registers that
 // the three warpgroups are launched with.
 // ---------------------------------------------------------------------------
 struct TileParams {
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int total = ROWS ? start[p.groups] * p.n_tiles : p.m_tiles * p.n_tiles * (p.groups ? p.groups : 1);
 
     if (warp == 1 || warp == 2) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (lane == 0) {
             const int mine = warp - 1;
             const Pipe pipe{dead, p.err, kErrTimeoutMma};
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         const int t = (warp == 0 ? 0 : 32) + lane;  // 0..63
         const bool gather = ROWS && p.rows;
         int slot = 0, stage = 0;
@@ -269,12 +269,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const float* sb = p.sb;
             if (!VEC) sb += (ROWS ? w.g * p.sb_stride : 0) + (long long)min(w.n0 / 128 + (t & 1) * (BN / 256), p.nb - 1) * p.ld_sb;
-            int arow[16];  // rows of A that this thread copies a 16-byte piece of: t / 8, t / 8 + 8, ...
+            // gathered: pieces t % 4 and t % 4 + 4 (of 16 bytes) of rows t / 4,
+            // t / 4 + 16, ...; rows past the end read the first one's
+            const uint8_t* from[8];
             if (gather) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int m = w.m0 + t / 8 + 8 * i;
-                    arow[i] = m < w.row_end ? min(max(0, p.rows[m]) / p.row_div, p.a_rows - 1) : -1;
+                for (int i = 0; i < 8; i++) {
+                    const int m = w.m0 + t / 4 + 16 * i;
+                    const int r = m < w.row_end ? min(max(0, p.rows[m]) / p.row_div, p.a_rows - 1) : 0;
+                    from[i] = p.a + (size_t)r * p.lda + (t & 3) * 16;
                 }
             }
             for (int kb = w.kb0; kb < w.kb1; kb++) {
@@ -313,14 +316,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                     phase ^= 1;
                 }
                 if (!gather) continue;
-                const int k = kb * 128 + (t & 7) * 16;
-                const int bytes = max(0, min(16, p.K - k));
+                // row r's piece q lies at piece q ^ (r % 8)
+                uint8_t* lo = sa + (t >> 2) * 128 + (((t & 3) ^ (t >> 2 & 7)) << 4);
+                uint8_t* hi = sa + (t >> 2) * 128 + (((t & 3) ^ (t >> 2 & 7) ^ 4) << 4);
+                if (kb * 128 + 128 <= p.K) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int r = t / 8 + 8 * i;  // r % 8 = t / 8: the swizzle's row
-                    const bool on = arow[i] >= 0 && bytes > 0;
-                    ptx::cp_async16(sa + r * 128 + (((t & 7) ^ (t >> 3)) << 4),
-                                    on ? p.a + (size_t)arow[i] * p.lda + k : p.a, on ? bytes : 0);
+                    for (int i = 0; i < 8; i++) {
+                        ptx::cp_async16(lo + i * 2048, from[i]);
+                        ptx::cp_async16(hi + i * 2048, from[i] + 64);
+                        from[i] += 128;
+                    }
+                } else {
+                    const int k = kb * 128 + (t & 3) * 16;
+                    const int b0 = max(0, min(16, p.K - k)), b1 = max(0, min(16, p.K - k - 64));
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        ptx::cp_async16(lo + i * 2048, b0 ? from[i] : p.a, b0);
+                        ptx::cp_async16(hi + i * 2048, b1 ? from[i] + 64 : p.a, b1);
+                    }
                 }
                 ptx::cp_async_arrive(landed);
             }
@@ -336,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         uint8_t* stg = staging + (warp - 4) * 2048;
         int part = 0, slot = 0;
