@@ -67,11 +67,13 @@ constexpr int kThreads = 128 + 32 * kEpi;
 constexpr int kMaxGroups = 1024;
 constexpr int kSlots = 4;  // groups of k-blocks whose scales are in flight
 
-template <int BN, bool VEC, bool ROWS>
+template <int BN, bool VEC, bool ROWS, bool PAIR>
 struct TileCfg {
+    static constexpr int BM = PAIR ? 256 : 128;       // rows of a tile
+    static constexpr int BROWS = PAIR ? BN / 2 : BN;  // rows of B that this CTA loads
     static constexpr int A_BYTES = 128 * 128;
-    static constexpr int STAGE = A_BYTES + BN * 128;
-    static constexpr int STAGES = BN == 256 ? 4 : 6;
+    static constexpr int STAGE = A_BYTES + BROWS * 128;
+    static constexpr int STAGES = PAIR ? 6 : 4;
     static constexpr int PARTS = 512 / BN;   // parts of TMEM
     static constexpr int COLS = BN / 2;      // columns of a warp
     static constexpr int STAGING = kEpi * 2048;  // 32 rows x 64 bytes a warp
@@ -112,7 +114,7 @@ struct Unit {
 
 // Tile u of the work: tiles of a group run along n first, those of a single
 // product in bands of kBand n tiles, so that tiles in flight share operands.
-template <int BN, bool ROWS>
+template <int BM, int BN, bool ROWS>
 __device__ __forceinline__ Unit unit_at(const TileParams& p, const int* start, int u) {
     Unit w;
     if (ROWS) {
@@ -125,7 +127,7 @@ __device__ __forceinline__ Unit unit_at(const TileParams& p, const int* start, i
         }
         w.g = lo;
         const int off = p.offsets[lo];
-        w.m0 = off + (t - start[lo]) * 128;
+        w.m0 = off + (t - start[lo]) * BM;
         w.row_end = min(p.M, off + p.counts[lo]);
         w.n0 = u % p.n_tiles * BN;
         w.kb0 = 0;
@@ -138,7 +140,7 @@ __device__ __forceinline__ Unit unit_at(const TileParams& p, const int* start, i
     const int band = u / (kBand * p.m_tiles);
     u -= band * kBand * p.m_tiles;
     const int width = min(kBand, p.n_tiles - band * kBand);
-    w.m0 = u / width * 128;
+    w.m0 = u / width * BM;
     w.n0 = (band * kBand + u % width) * BN;
     w.row_end = p.M;
     w.kb0 = 0;
@@ -171,12 +173,12 @@ __device__ __forceinline__ void group_starts(const TileParams& p, int rows, int*
     if (lane == 0) start[p.groups] = run;
 }
 
-template <int BN, bool VEC, bool ROWS>
+template <int BN, bool VEC, bool ROWS, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_tile_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
                     const __grid_constant__ CUtensorMap tc, const TileParams p) {
-    using C = TileCfg<BN, VEC, ROWS>;
-    constexpr uint32_t IDESC = ptx::instr_desc(0, 0, 0, 128, BN);
+    using C = TileCfg<BN, VEC, ROWS, PAIR>;
+    constexpr uint32_t IDESC = ptx::instr_desc(0, 0, 0, C::BM, BN);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* staging = smem + C::STAGES * C::STAGE;
@@ -192,10 +194,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     int* start = reinterpret_cast<int*>(staging + C::STAGING + C::SCALES + 512);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = PAIR ? ptx::cluster_ctarank() : 0;  // rank 0 issues the pair's MMAs
+    const bool gather = ROWS && p.rows;
     if (threadIdx.x == 0) {
         *dead = 0;
         for (int s = 0; s < C::STAGES; s++) {
-            ptx::mbar_init(&full[s], ROWS && p.rows ? 65 : 1);
+            // TMA's arrival, with gathered rows every copying thread's, and the
+            // second CTA's once its rows are there
+            ptx::mbar_init(&full[s], gather ? (PAIR ? (rank ? 64 : 66) : 65) : 1);
             ptx::mbar_init(&empty[s], 1);
         }
         for (int s = 0; s < kSlots; s++) {
@@ -204,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int s = 0; s < C::PARTS; s++) {
             ptx::mbar_init(&part_full[s], 1);
-            ptx::mbar_init(&part_empty[s], kEpi);
+            ptx::mbar_init(&part_empty[s], PAIR ? 2 * kEpi : kEpi);
         }
         ptx::fence_mbar_init();
         ptx::prefetch_tmap(&ta);
@@ -212,24 +218,32 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (p.tma_out) ptx::prefetch_tmap(&tc);
     }
     if (warp == 1) {
-        ptx::tmem_alloc(tmem_slot, 512);
-        ptx::tmem_relinquish();
+        if (PAIR) {
+            ptx::tmem_alloc_pair(tmem_slot, 512);
+            ptx::tmem_relinquish_pair();
+        } else {
+            ptx::tmem_alloc(tmem_slot, 512);
+            ptx::tmem_relinquish();
+        }
     }
-    if (ROWS && warp == 4) group_starts(p, 128, start, lane);
+    if (ROWS && warp == 4) group_starts(p, C::BM, start, lane);
     ptx::tc_fence_before();
-    __syncthreads();
+    __syncwarp();
+    if (PAIR) ptx::cluster_sync();
+    else __syncthreads();
     ptx::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int total = ROWS ? start[p.groups] * p.n_tiles : p.m_tiles * p.n_tiles * (p.groups ? p.groups : 1);
+    const int first = PAIR ? blockIdx.x / 2 : blockIdx.x, stride = PAIR ? gridDim.x / 2 : gridDim.x;
 
     if (warp == 1 || warp == 2) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (lane == 0) {
+        if (lane == 0 && rank == 0) {
             const int mine = warp - 1;
             const Pipe pipe{dead, p.err, kErrTimeoutMma};
             int it = 0;  // k-blocks so far: number `it` uses stage it % STAGES and part it % PARTS
-            for (int u = blockIdx.x; u < total; u += gridDim.x) {
-                const Unit w = unit_at<BN, ROWS>(p, start, u);
+            for (int u = first; u < total; u += stride) {
+                const Unit w = unit_at<C::BM, BN, ROWS>(p, start, u);
                 for (int kb = w.kb0; kb < w.kb1; kb++, it++) {
                     if ((it & 1) != mine) continue;
                     const int stage = it % C::STAGES, part = it % C::PARTS;
@@ -237,27 +251,52 @@ __global__ void __launch_bounds__(kThreads, 1)
                     pipe.wait(&part_empty[part], (it / C::PARTS & 1) ^ 1);
                     // gathered rows came through the generic proxy; the fence is
                     // here, where no copies are in flight that it would wait for
-                    if (ROWS && p.rows) ptx::fence_proxy_async();
+                    if (gather) ptx::fence_proxy_async();
                     ptx::tc_fence_after();
                     const uint32_t sa = ptx::smem_u32(smem + stage * C::STAGE), sb = sa + C::A_BYTES;
 #pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        ptx::mma_f8(tmem + part * BN, ptx::smem_desc(sa + k * 32, 16, 1024, 2),
-                                    ptx::smem_desc(sb + k * 32, 16, 1024, 2), IDESC, k > 0);
-                    ptx::mma_commit(&empty[stage]);
-                    ptx::mma_commit(&part_full[part]);
+                    for (int k = 0; k < 4; k++) {
+                        const uint64_t da = ptx::smem_desc(sa + k * 32, 16, 1024, 2);
+                        const uint64_t db = ptx::smem_desc(sb + k * 32, 16, 1024, 2);
+                        if (PAIR) ptx::mma_f8_pair(tmem + part * BN, da, db, IDESC, k > 0);
+                        else ptx::mma_f8(tmem + part * BN, da, db, IDESC, k > 0);
+                    }
+                    if (PAIR) {
+                        ptx::mma_commit_pair(&empty[stage]);
+                        ptx::mma_commit_pair(&part_full[part]);
+                    } else {
+                        ptx::mma_commit(&empty[stage]);
+                        ptx::mma_commit(&part_full[part]);
+                    }
+                }
+            }
+        } else if (PAIR && gather && lane == 0 && warp == 1) {
+            // the second CTA tells the first when its gathered rows are there
+            const Pipe pipe{dead, p.err, kErrTimeoutMma};
+            int stage = 0;
+            uint32_t phase = 0;
+            for (int u = first; u < total; u += stride) {
+                const Unit w = unit_at<C::BM, BN, ROWS>(p, start, u);
+                for (int kb = w.kb0; kb < w.kb1; kb++) {
+                    pipe.wait(&full[stage], phase);
+                    ptx::fence_proxy_async();
+                    ptx::mbar_arrive_release(ptx::cluster_addr(&full[stage], 0));
+                    if (++stage == C::STAGES) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
                 }
             }
         }
     } else if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         const int t = (warp == 0 ? 0 : 32) + lane;  // 0..63
-        const bool gather = ROWS && p.rows;
         int slot = 0, stage = 0;
         uint32_t slot_phase = 0, phase = 0;
         const Pipe pipe{dead, p.err, kErrTimeoutProducer};
-        for (int u = blockIdx.x; u < total; u += gridDim.x) {
-            const Unit w = unit_at<BN, ROWS>(p, start, u);
+        for (int u = first; u < total; u += stride) {
+            Unit w = unit_at<C::BM, BN, ROWS>(p, start, u);
+            if (PAIR) w.m0 += rank * 128;
             // the rows whose scales this thread copies; rows past the end
             // take the first one's, and are not stored
             const float* srow[2];
@@ -306,9 +345,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 pipe.wait(&empty[stage], phase ^ 1);
                 uint8_t* sa = smem + stage * C::STAGE;
                 if (t == 0) {
-                    ptx::mbar_arrive_expect_tx(&full[stage], gather ? C::STAGE - C::A_BYTES : C::STAGE);
-                    if (!gather) ptx::tma_load_2d(sa, &ta, &full[stage], kb * 128, w.m0);
-                    ptx::tma_load_3d(sa + C::A_BYTES, &tb, &full[stage], kb * 128, w.n0, ROWS ? w.g : 0);
+                    constexpr int B_BYTES = C::STAGE - C::A_BYTES;
+                    if (PAIR) {
+                        // both CTAs' loads complete on the first one's barrier
+                        const uint32_t bar = ptx::cluster_addr(&full[stage], 0);
+                        if (rank == 0) ptx::mbar_arrive_expect_tx(&full[stage], 2 * (gather ? B_BYTES : C::STAGE));
+                        if (!gather) ptx::tma_load_2d_pair(sa, &ta, bar, kb * 128, w.m0);
+                        ptx::tma_load_3d_pair(sa + C::A_BYTES, &tb, bar, kb * 128, w.n0 + rank * C::BROWS, ROWS ? w.g : 0);
+                    } else {
+                        ptx::mbar_arrive_expect_tx(&full[stage], gather ? B_BYTES : C::STAGE);
+                        if (!gather) ptx::tma_load_2d(sa, &ta, &full[stage], kb * 128, w.m0);
+                        ptx::tma_load_3d(sa + C::A_BYTES, &tb, &full[stage], kb * 128, w.n0, ROWS ? w.g : 0);
+                    }
                 }
                 uint64_t* landed = &full[stage];
                 if (++stage == C::STAGES) {
@@ -356,8 +404,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t part_phase = 0, slot_phase = 0;
         const Pipe pipe{dead, p.err, kErrTimeoutEpilogue};
         const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + half * C::COLS;
-        for (int u = blockIdx.x; u < total; u += gridDim.x) {
-            const Unit w = unit_at<BN, ROWS>(p, start, u);
+        for (int u = first; u < total; u += stride) {
+            Unit w = unit_at<C::BM, BN, ROWS>(p, start, u);
+            if (PAIR) w.m0 += rank * 128;
             const int row = w.m0 + quarter * 32 + lane;
             const bool valid = row < w.row_end;
             const int col0 = w.n0 + half * C::COLS;
@@ -406,7 +455,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 ptx::tc_fence_before();
                 __syncwarp();
-                ptx::mbar_arrive_if(&part_empty[part], lane == 0);
+                if (PAIR) ptx::mbar_arrive_cluster_if(ptx::cluster_addr(&part_empty[part], 0), lane == 0);
+                else ptx::mbar_arrive_if(&part_empty[part], lane == 0);
                 if (++in == C::SLOTK || kb + 1 == w.kb1) {
                     ptx::mbar_arrive_if(&slot_empty[slot], lane == 0);
                     in = 0;
@@ -502,10 +552,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 
     ptx::tc_fence_before();
-    __syncthreads();
+    // (a pair leaves together: each other's shared memory is read and arrived at)
+    __syncwarp();
+    if (PAIR) ptx::cluster_sync();
+    else __syncthreads();
     if (warp == 1) {
         ptx::tc_fence_after();
-        ptx::tmem_dealloc(tmem, 512);
+        if (PAIR) ptx::tmem_dealloc_pair(tmem, 512);
+        else ptx::tmem_dealloc(tmem, 512);
     }
 }
 
@@ -540,9 +594,6 @@ struct SmallParams {
     int split;     // CTAs of a cluster that share a tile's k-blocks
 };
 
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
 __device__ __forceinline__ float cluster_loadf(const float* p, unsigned rank) {
     uint32_t at;
     float v;
@@ -828,7 +879,8 @@ __global__ void __launch_bounds__(256, 1)
     if (sp.split > 1) {
         // the k-blocks' shares are added in rank order; rank r stores every
         // split-th row of the tile
-        cluster_sync();
+        __syncwarp();
+        ptx::cluster_sync();
         if (first < total) {
             const Unit w = small_unit<BN>(p, start, first);
             const float* sum = reinterpret_cast<const float*>(smem);
@@ -844,7 +896,8 @@ __global__ void __launch_bounds__(256, 1)
                 }
             }
         }
-        cluster_sync();  // no CTA leaves while others read its sums
+        __syncwarp();
+        ptx::cluster_sync();  // no CTA leaves while others read its sums
     }
 }
 
@@ -990,20 +1043,20 @@ int launch_small(const Fp8Gemm& d, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, k, tw, sp) == cudaSuccess ? 0 : -5;
 }
 
-template <int BN, bool VEC, bool ROWS>
+template <int BN, bool VEC, bool ROWS, bool PAIR>
 int launch_tiles(const Fp8Gemm& d, cudaStream_t st) {
-    using C = TileCfg<BN, VEC, ROWS>;
+    using C = TileCfg<BN, VEC, ROWS, PAIR>;
     static bool done[kMaxDevices] = {};
-    auto k = fp8_tile_kernel<BN, VEC, ROWS>;
+    auto k = fp8_tile_kernel<BN, VEC, ROWS, PAIR>;
     if (!allow_smem(k, C::SMEM, done)) return -5;
     const int es = d.c_dtype == kBF16 ? 2 : 4;
     const bool aligned = !(reinterpret_cast<uintptr_t>(d.c) & 15) && d.ldc * es % 16 == 0 && d.c_stride * es % 16 == 0;
-    TileParams p = params(d, 128, BN);
+    TileParams p = params(d, C::BM, BN);
     p.vec_out = aligned;
     CUtensorMap ta, tb, tc;
     memset(&tc, 0, sizeof(tc));
     if (!map_codes2(&ta, d.a, d.K, d.a_rows, d.lda, 128)) return -2;
-    if (!map_codes3(&tb, d.b, d.K, d.N, d.ldb, ROWS ? d.groups : 1, d.b_stride, BN)) return -2;
+    if (!map_codes3(&tb, d.b, d.K, d.N, d.ldb, ROWS ? d.groups : 1, d.b_stride, C::BROWS)) return -2;
     // a TMA store clips rows to whole 16-byte pieces, so ragged ones go another way
     p.tma_out = aligned && (long long)d.N * es % 16 == 0 &&
                 map_out(&tc, d.c, d.c_dtype, d.N, d.M, d.ldc, d.group_k ? d.groups : 1, d.c_stride);
@@ -1011,9 +1064,30 @@ int launch_tiles(const Fp8Gemm& d, cudaStream_t st) {
     if (ROWS) units = ((long long)p.m_tiles + d.groups) * p.n_tiles;  // at most
     else if (d.groups) units *= d.groups;
     if (units > 0x7fffffff) return -2;
-    const int sms = num_sms();
-    k<<<(unsigned)(units < sms ? units : sms), kThreads, C::SMEM, st>>>(ta, tb, tc, p);
-    return cudaGetLastError() == cudaSuccess ? 0 : -5;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = PAIR ? 2 : 1;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    // one CTA an SM; of pairs as many as find two SMs of one cluster
+    long long slots = num_sms();
+    if (PAIR) {
+        static int pairs[kMaxDevices] = {};
+        int dev = 0;
+        cudaGetDevice(&dev);
+        if (pairs[dev] == 0) {
+            cfg.gridDim = dim3(2);
+            if (cudaOccupancyMaxActiveClusters(&pairs[dev], k, &cfg) != cudaSuccess || pairs[dev] < 1) return -5;
+        }
+        slots = pairs[dev];
+    }
+    cfg.gridDim = dim3((unsigned)((units < slots ? units : slots) * (PAIR ? 2 : 1)));
+    return cudaLaunchKernelEx(&cfg, k, ta, tb, tc, p) == cudaSuccess ? 0 : -5;
 }
 
 }  // namespace
@@ -1049,8 +1123,13 @@ int fp8_gemm(const Fp8Gemm& d, cudaStream_t st) {
             return d.b_rows ? launch_small<64, true>(d, st) : launch_small<64, false>(d, st);
         }
     }
-    if (d.groups && !d.group_k) return launch_tiles<256, false, true>(d, st);
-    return d.b_rows ? launch_tiles<256, true, false>(d, st) : launch_tiles<256, false, false>(d, st);
+    // Pairs of CTAs wherever a second 128 rows are there on average.
+    const int rows = d.groups && !d.group_k ? d.M / d.groups : d.M;
+    const bool pair = rows > (d.groups && !d.group_k ? 256 : 128);
+    if (d.groups && !d.group_k)
+        return pair ? launch_tiles<256, false, true, true>(d, st) : launch_tiles<256, false, true, false>(d, st);
+    if (d.b_rows) return pair ? launch_tiles<256, true, false, true>(d, st) : launch_tiles<256, true, false, false>(d, st);
+    return pair ? launch_tiles<256, false, false, true>(d, st) : launch_tiles<256, false, false, false>(d, st);
 }
 
 }  // namespace nsb
