@@ -71,6 +71,7 @@ template <int BN, bool VEC, bool ROWS, bool PAIR>
 struct TileCfg {
     static constexpr int BM = PAIR ? 256 : 128;       // rows of a tile
     static constexpr int BROWS = PAIR ? BN / 2 : BN;  // rows of B that this CTA loads
+    static_assert(!PAIR || (!VEC && !ROWS), "pairs take one product with block scales");
     static constexpr int A_BYTES = 128 * 128;
     static constexpr int STAGE = A_BYTES + BROWS * 128;
     static constexpr int STAGES = PAIR ? 6 : 4;
@@ -199,9 +200,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0) {
         *dead = 0;
         for (int s = 0; s < C::STAGES; s++) {
-            // TMA's arrival, with gathered rows every copying thread's, and the
-            // second CTA's once its rows are there
-            ptx::mbar_init(&full[s], gather ? (PAIR ? (rank ? 64 : 66) : 65) : 1);
+            // TMA's arrival and, with gathered rows, every copying thread's
+            ptx::mbar_init(&full[s], gather ? 65 : 1);
             ptx::mbar_init(&empty[s], 1);
         }
         for (int s = 0; s < kSlots; s++) {
@@ -270,23 +270,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-        } else if (PAIR && gather && lane == 0 && warp == 1) {
-            // the second CTA tells the first when its gathered rows are there
-            const Pipe pipe{dead, p.err, kErrTimeoutMma};
-            int stage = 0;
-            uint32_t phase = 0;
-            for (int u = first; u < total; u += stride) {
-                const Unit w = unit_at<C::BM, BN, ROWS>(p, start, u);
-                for (int kb = w.kb0; kb < w.kb1; kb++) {
-                    pipe.wait(&full[stage], phase);
-                    ptx::fence_proxy_async();
-                    ptx::mbar_arrive_release(ptx::cluster_addr(&full[stage], 0));
-                    if (++stage == C::STAGES) {
-                        stage = 0;
-                        phase ^= 1;
-                    }
-                }
-            }
         }
     } else if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -345,15 +328,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 pipe.wait(&empty[stage], phase ^ 1);
                 uint8_t* sa = smem + stage * C::STAGE;
                 if (t == 0) {
-                    constexpr int B_BYTES = C::STAGE - C::A_BYTES;
                     if (PAIR) {
                         // both CTAs' loads complete on the first one's barrier
                         const uint32_t bar = ptx::cluster_addr(&full[stage], 0);
-                        if (rank == 0) ptx::mbar_arrive_expect_tx(&full[stage], 2 * (gather ? B_BYTES : C::STAGE));
-                        if (!gather) ptx::tma_load_2d_pair(sa, &ta, bar, kb * 128, w.m0);
-                        ptx::tma_load_3d_pair(sa + C::A_BYTES, &tb, bar, kb * 128, w.n0 + rank * C::BROWS, ROWS ? w.g : 0);
+                        if (rank == 0) ptx::mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE);
+                        ptx::tma_load_2d_pair(sa, &ta, bar, kb * 128, w.m0);
+                        ptx::tma_load_3d_pair(sa + C::A_BYTES, &tb, bar, kb * 128, w.n0 + rank * C::BROWS, 0);
                     } else {
-                        ptx::mbar_arrive_expect_tx(&full[stage], gather ? B_BYTES : C::STAGE);
+                        ptx::mbar_arrive_expect_tx(&full[stage], gather ? C::STAGE - C::A_BYTES : C::STAGE);
                         if (!gather) ptx::tma_load_2d(sa, &ta, &full[stage], kb * 128, w.m0);
                         ptx::tma_load_3d(sa + C::A_BYTES, &tb, &full[stage], kb * 128, w.n0, ROWS ? w.g : 0);
                     }
@@ -414,44 +396,75 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int j = 0; j < C::COLS; j++) acc[j] = 0.f;
             int in = 0;
-            float s_next[C::SLOTK];  // this row's scales of the group's k-blocks
+            // block scales: this row's, times the block's, of the group's k-blocks;
+            // column scales: four rows' of one k-block (the fragment's)
+            constexpr int NS = VEC ? 4 : C::SLOTK;
+            float sr[NS];
             for (int kb = w.kb0; kb < w.kb1; kb++) {
-                if (in == 0) {
-                    pipe.wait(&slot_full[slot], slot_phase);
-                    const float* sc = slots + slot * C::SLOTK * C::SLOT;
+                const float* sc = slots + (slot * C::SLOTK + in) * C::SLOT;
+                if (in == 0) pipe.wait(&slot_full[slot], slot_phase);
+                if (VEC) {
 #pragma unroll
-                    for (int i = 0; i < C::SLOTK; i++)
-                        s_next[i] = sc[i * C::SLOT + quarter * 32 + lane] * (VEC ? 1.f : sc[i * C::SLOT + 128 + half]);
+                    for (int i = 0; i < 4; i++) sr[i] = sc[quarter * 32 + i * 8 + (lane >> 2)];
+                } else if (in == 0) {
+#pragma unroll
+                    for (int i = 0; i < NS; i++)
+                        sr[i] = sc[i * C::SLOT + quarter * 32 + lane] * sc[i * C::SLOT + 128 + half];
                 }
-                const float s = s_next[0];
+                const float s = sr[0];
+                if (!VEC) {
 #pragma unroll
-                for (int i = 0; i + 1 < C::SLOTK; i++) s_next[i] = s_next[i + 1];
-                const float4* v =
-                    reinterpret_cast<const float4*>(slots + (slot * C::SLOTK + in) * C::SLOT + 128 + half * C::COLS);
+                    for (int i = 0; i + 1 < NS; i++) sr[i] = sr[i + 1];
+                }
                 pipe.wait(&part_full[part], part_phase);
                 __syncwarp();
                 ptx::tc_fence_after();
                 const uint32_t t = lane_base + part * BN;
-                uint32_t r[2][16];
-                ptx::tmem_ld16(t, r[0]);
+                if constexpr (VEC) {
+                    // fragments of 16 rows x 32 columns: of each a thread has two
+                    // rows (lane / 4, + 8) and the columns 2 (lane % 4) of every 8,
+                    // so it needs 4 row and 32 column scales, not 1 and 128
+                    const uint64_t* v = reinterpret_cast<const uint64_t*>(sc + 128 + half * C::COLS) + (lane & 3);
+                    uint32_t r[2][16];
+                    ptx::tmem_ld_frag32(t, r[0]);
 #pragma unroll
-                for (int c = 0; c < C::COLS / 16; c++) {
-                    float m[16];
-                    if (VEC) {
+                    for (int c = 0; c < C::COLS / 32; c++) {
+                        uint64_t q[4];
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const float4 q = v[c * 4 + j];
-                            m[4 * j] = q.x * s;
-                            m[4 * j + 1] = q.y * s;
-                            m[4 * j + 2] = q.z * s;
-                            m[4 * j + 3] = q.w * s;
+                        for (int j = 0; j < 4; j++) q[j] = v[c * 16 + j * 4];
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            ptx::tmem_ld_wait_regs16(r[h]);
+                            if (h == 0) ptx::tmem_ld_frag32(t + (16u << 16) + c * 32, r[1]);
+                            else if (c + 1 < C::COLS / 32) ptx::tmem_ld_frag32(t + (c + 1) * 32, r[0]);
+#pragma unroll
+                            for (int j = 0; j < 8; j++) {
+                                float* o = acc + ((c * 2 + h) * 8 + j) * 2;
+                                const float sj = sr[h * 2 + (j & 1)];
+                                const uint64_t x =
+                                    f2_pack(__uint_as_float(r[h][2 * j]), __uint_as_float(r[h][2 * j + 1]));
+                                f2_unpack(f2_fma(f2_mul(x, q[j >> 1]), f2_pack(sj, sj), f2_pack(o[0], o[1])), o[0], o[1]);
+                            }
                         }
                     }
-                    ptx::tmem_ld_wait_regs16(r[c & 1]);
-                    if (c + 1 < C::COLS / 16) ptx::tmem_ld16(t + (c + 1) * 16, r[(c + 1) & 1]);
+                } else {
+                    // 16 columns at a time, the next 16 on their way; packed pairs
+                    // halve the FMA instructions
+                    uint32_t r[2][16];
+                    ptx::tmem_ld16(t, r[0]);
+                    const uint64_t s2 = f2_pack(s, s);
 #pragma unroll
-                    for (int j = 0; j < 16; j++)
-                        acc[c * 16 + j] = fmaf(__uint_as_float(r[c & 1][j]), VEC ? m[j] : s, acc[c * 16 + j]);
+                    for (int c = 0; c < C::COLS / 16; c++) {
+                        ptx::tmem_ld_wait_regs16(r[c & 1]);
+                        if (c + 1 < C::COLS / 16) ptx::tmem_ld16(t + (c + 1) * 16, r[(c + 1) & 1]);
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            float* o = acc + c * 16 + 2 * j;
+                            const uint64_t x =
+                                f2_pack(__uint_as_float(r[c & 1][2 * j]), __uint_as_float(r[c & 1][2 * j + 1]));
+                            f2_unpack(f2_fma(x, s2, f2_pack(o[0], o[1])), o[0], o[1]);
+                        }
+                    }
                 }
                 ptx::tc_fence_before();
                 __syncwarp();
@@ -469,6 +482,40 @@ __global__ void __launch_bounds__(kThreads, 1)
                     part = 0;
                     part_phase ^= 1;
                 }
+            }
+            if constexpr (VEC) {
+                // a row's 8 columns of four threads are one 32-byte (fp32) piece
+                const size_t base = (size_t)w.g * p.c_stride;
+#pragma unroll
+                for (int c = 0; c < C::COLS / 32; c++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const int m = w.m0 + quarter * 32 + h * 16 + (j & 1) * 8 + (lane >> 2);
+                            const int n = col0 + c * 32 + (j >> 1) * 8 + (lane & 3) * 2;
+                            const float* o = acc + ((c * 2 + h) * 8 + j) * 2;
+                            if (m >= w.row_end || n >= p.N) continue;
+                            const size_t at = base + (size_t)m * p.ldc + n;
+                            if (p.c_dtype == kBF16) {
+                                __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.c) + at;
+                                if (p.vec_out && n + 1 < p.N) {
+                                    *reinterpret_cast<__nv_bfloat162*>(dst) = __floats2bfloat162_rn(o[0], o[1]);
+                                } else {
+                                    dst[0] = f2bf(o[0]);
+                                    if (n + 1 < p.N) dst[1] = f2bf(o[1]);
+                                }
+                            } else {
+                                float* dst = reinterpret_cast<float*>(p.c) + at;
+                                if (p.vec_out && n + 1 < p.N) {
+                                    *reinterpret_cast<float2*>(dst) = make_float2(o[0], o[1]);
+                                } else {
+                                    dst[0] = o[0];
+                                    if (n + 1 < p.N) dst[1] = o[1];
+                                }
+                            }
+                        }
+                continue;
             }
             // a slab of 32 rows leaves by TMA where all of them are the tile's
             // (the store clips at the tensor's end), else row by row
@@ -1058,7 +1105,7 @@ int launch_tiles(const Fp8Gemm& d, cudaStream_t st) {
     if (!map_codes2(&ta, d.a, d.K, d.a_rows, d.lda, 128)) return -2;
     if (!map_codes3(&tb, d.b, d.K, d.N, d.ldb, ROWS ? d.groups : 1, d.b_stride, C::BROWS)) return -2;
     // a TMA store clips rows to whole 16-byte pieces, so ragged ones go another way
-    p.tma_out = aligned && (long long)d.N * es % 16 == 0 &&
+    p.tma_out = !VEC && aligned && (long long)d.N * es % 16 == 0 &&
                 map_out(&tc, d.c, d.c_dtype, d.N, d.M, d.ldc, d.group_k ? d.groups : 1, d.c_stride);
     long long units = (long long)p.m_tiles * p.n_tiles;
     if (ROWS) units = ((long long)p.m_tiles + d.groups) * p.n_tiles;  // at most
@@ -1123,13 +1170,14 @@ int fp8_gemm(const Fp8Gemm& d, cudaStream_t st) {
             return d.b_rows ? launch_small<64, true>(d, st) : launch_small<64, false>(d, st);
         }
     }
-    // Pairs of CTAs wherever a second 128 rows are there on average.
-    const int rows = d.groups && !d.group_k ? d.M / d.groups : d.M;
-    const bool pair = rows > (d.groups && !d.group_k ? 256 : 128);
-    if (d.groups && !d.group_k)
-        return pair ? launch_tiles<256, false, true, true>(d, st) : launch_tiles<256, false, true, false>(d, st);
-    if (d.b_rows) return pair ? launch_tiles<256, true, false, true>(d, st) : launch_tiles<256, true, false, false>(d, st);
-    return pair ? launch_tiles<256, false, false, true>(d, st) : launch_tiles<256, false, false, false>(d, st);
+    if (d.groups && !d.group_k) return launch_tiles<256, false, true, false>(d, st);
+    if (d.b_rows) return launch_tiles<256, true, false, false>(d, st);
+    // Pairs of CTAs read a third less from L2, but wait for one another: from
+    // two rounds of tiles on (8192 x 4096 x 4096: 133 us against 139; 2048 x
+    // 2048 x 2048, under one round: 15.1 against 14.2).
+    const long long tiles = (long long)((d.M + 255) / 256) * ((d.N + 255) / 256);
+    return tiles >= num_sms() ? launch_tiles<256, false, false, true>(d, st)
+                              : launch_tiles<256, false, false, false>(d, st);
 }
 
 }  // namespace nsb
