@@ -81,7 +81,7 @@ struct TileCfg {
     static constexpr int SLOT = 128 + (VEC ? BN : 4);  // a k-block's row scales, then column or block scales
     static constexpr int SLOTK = VEC ? 2 : 4;  // k-blocks of a group: one wait for all their scales
     static constexpr int SCALES = kSlots * SLOTK * SLOT * 4;
-    static constexpr int TABLE = ROWS ? (kMaxGroups + 1) * 4 : 0;
+    static constexpr int TABLE = ROWS ? (2 * kMaxGroups + 1) * 4 : 0;
     static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + SCALES + 512 + TABLE;
     static_assert(SMEM <= 227 * 1024, "above the shared memory of a block");
 };
@@ -127,9 +127,8 @@ __device__ __forceinline__ Unit unit_at(const TileParams& p, const int* start, i
             else hi = mid;
         }
         w.g = lo;
-        const int off = p.offsets[lo];
-        w.m0 = off + (t - start[lo]) * BM;
-        w.row_end = min(p.M, off + p.counts[lo]);
+        w.m0 = start[kMaxGroups + 1 + lo] + (t - start[lo]) * BM;
+        w.row_end = min(p.M, start[kMaxGroups + 1 + lo] + p.counts[lo]);
         w.n0 = u % p.n_tiles * BN;
         w.kb0 = 0;
         w.kb1 = (p.K + 127) / 128;
@@ -154,14 +153,18 @@ __device__ __forceinline__ Unit unit_at(const TileParams& p, const int* start, i
     return w;
 }
 
-// First tile of every group (tiles of `rows` rows) into start[0..groups], by
-// one warp.
+// First tile (of `rows` rows) of every group into start[0..groups], its first
+// row behind them. By one warp.
 __device__ __forceinline__ void group_starts(const TileParams& p, int rows, int* start, int lane) {
     int run = 0;
     for (int g0 = 0; g0 < p.groups; g0 += 32) {
         const int g = g0 + lane;
         int n = 0;
-        if (g < p.groups) n = (max(0, min(p.counts[g], p.M - p.offsets[g])) + rows - 1) / rows;
+        if (g < p.groups) {
+            const int off = p.offsets[g], end = max(off, min(p.M, off + p.counts[g]));
+            start[kMaxGroups + 1 + g] = off;
+            n = (end - off + rows - 1) / rows;
+        }
         int inc = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -618,10 +621,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ring, eight parts of TMEM, and for one product the k-blocks of a tile split
 // over a cluster of CTAs, whose sums meet in shared memory in rank order.
 //   warp 0       weights by TMA
-//   warp 1       MMA issuer
+//   warps 1, 8   MMA issuers, every other k-block each
 //   warps 2..3   rows of A by cp.async (listed, or in order) and the scales
 //   warps 4..7   a warp owns 32 weight rows: scales and adds, stores
 // ---------------------------------------------------------------------------
+constexpr int kSmallThreads = 288;
+
 template <int BN, bool VEC>
 struct SmallCfg {
     static constexpr int W_BYTES = 128 * 128;
@@ -631,7 +636,7 @@ struct SmallCfg {
     static constexpr int SLOTK = 4;
     static constexpr int SLOT = BN + (VEC ? 128 : 4);  // scales of A's rows, then of B's rows or block
     static constexpr int SCALES = kSlots * SLOTK * SLOT * 4;
-    static constexpr int SMEM = 1024 + STAGES * STAGE + SCALES + 512 + (kMaxGroups + 1) * 4;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + SCALES + 512 + (2 * kMaxGroups + 1) * 4;
     static_assert(SMEM <= 227 * 1024, "above the shared memory of a block");
     static_assert(BN * 128 * 4 <= STAGES * STAGE, "the cluster's sums take the ring's place");
 };
@@ -667,15 +672,14 @@ __device__ __forceinline__ Unit small_unit(const TileParams& p, const int* start
             else hi = mid;
         }
         w.g = lo;
-        const int off = p.offsets[lo];
-        w.m0 = off + (t - start[lo]) * BN;
-        w.row_end = min(p.M, off + p.counts[lo]);
+        w.m0 = start[kMaxGroups + 1 + lo] + (t - start[lo]) * BN;
+        w.row_end = min(p.M, start[kMaxGroups + 1 + lo] + p.counts[lo]);
     }
     return w;
 }
 
 template <int BN, bool VEC>
-__global__ void __launch_bounds__(256, 1)
+__global__ void __launch_bounds__(kSmallThreads, 1)
     fp8_small_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ SmallParams sp) {
     using C = SmallCfg<BN, VEC>;
     const TileParams& p = sp.t;
@@ -756,15 +760,17 @@ __global__ void __launch_bounds__(256, 1)
             }
         }
         __syncwarp();
-    } else if (warp == 1) {
+    } else if (warp == 1 || warp == 8) {
         if (lane == 0) {
             const Pipe pipe{dead, p.err, kErrTimeoutMma};
-            int stage = 0, part = 0;
-            uint32_t phase = 0, part_phase = 0;
+            const int mine = warp == 1 ? 0 : 1;
+            int it = 0;  // k-blocks so far: number `it` uses stage it % STAGES and part it % PARTS
             for (int u = first; u < total; u += stride)
-                for (int kb = kb0; kb < kb1; kb++) {
-                    pipe.wait(&full[stage], phase);
-                    pipe.wait(&part_empty[part], part_phase ^ 1);
+                for (int kb = kb0; kb < kb1; kb++, it++) {
+                    if ((it & 1) != mine) continue;
+                    const int stage = it % C::STAGES, part = it % C::PARTS;
+                    pipe.wait(&full[stage], it / C::STAGES & 1);
+                    pipe.wait(&part_empty[part], (it / C::PARTS & 1) ^ 1);
                     ptx::fence_proxy_async();  // A's rows came through the generic proxy
                     ptx::tc_fence_after();
                     const uint32_t sw = ptx::smem_u32(smem + stage * C::STAGE), sa = sw + C::W_BYTES;
@@ -774,14 +780,6 @@ __global__ void __launch_bounds__(256, 1)
                                     ptx::smem_desc(sa + k * 32, 16, 1024, 2), IDESC, k > 0);
                     ptx::mma_commit(&empty[stage]);
                     ptx::mma_commit(&part_full[part]);
-                    if (++stage == C::STAGES) {
-                        stage = 0;
-                        phase ^= 1;
-                    }
-                    if (++part == C::PARTS) {
-                        part = 0;
-                        part_phase ^= 1;
-                    }
                 }
         }
         __syncwarp();
@@ -795,13 +793,24 @@ __global__ void __launch_bounds__(256, 1)
             if (m >= w.row_end) return -1;
             return p.rows ? min(max(0, p.rows[m]) / p.row_div, p.a_rows - 1) : m;
         };
+        constexpr int PIECES = BN / 8;  // 16-byte pieces of a k-block that this thread copies
+        Unit next;
+        int ahead[PIECES + 1];  // the next tile's rows, looked up while this one's are copied
+        auto look = [&](int u) {
+            if (u >= total) return;
+            next = small_unit<BN>(p, start, u);
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) ahead[i] = source(next, t / 8 + 8 * i);
+            ahead[PIECES] = source(next, min(t, BN - 1));
+        };
+        look(first);
         for (int u = first; u < total; u += stride) {
-            const Unit w = small_unit<BN>(p, start, u);
-            constexpr int PIECES = BN / 8;  // 16-byte pieces of a k-block that this thread copies
+            const Unit w = next;
             int arow[PIECES];
 #pragma unroll
-            for (int i = 0; i < PIECES; i++) arow[i] = source(w, t / 8 + 8 * i);
-            const float* srow = p.sa + max(0, source(w, min(t, BN - 1)));
+            for (int i = 0; i < PIECES; i++) arow[i] = ahead[i];
+            const float* srow = p.sa + max(0, ahead[PIECES]);
+            look(u + stride);
             const float* sb = p.sb + w.g * p.sb_stride;
             if (!VEC) sb += (long long)(w.n0 / 128) * p.ld_sb;
             for (int kb = kb0; kb < kb1; kb++) {
@@ -932,7 +941,7 @@ __global__ void __launch_bounds__(256, 1)
             const Unit w = small_unit<BN>(p, start, first);
             const float* sum = reinterpret_cast<const float*>(smem);
             const int n_in = threadIdx.x & 127, n = w.n0 + n_in;
-            for (int j = rank * 2 + (threadIdx.x >> 7); j < BN; j += sp.split * 2) {
+            for (int j = rank * 2 + (threadIdx.x >> 7); threadIdx.x < 256 && j < BN; j += sp.split * 2) {
                 const int m = w.m0 + j;
                 if (m >= w.row_end) break;
                 float v = 0.f;
@@ -1078,7 +1087,7 @@ int launch_small(const Fp8Gemm& d, cudaStream_t st) {
         while (sp.split < 8 && units * sp.split * 2 <= sms && kblocks >= sp.split * 4) sp.split *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(sp.split > 1 ? units * sp.split : units < sms ? units : sms));
-    cfg.blockDim = dim3(256);
+    cfg.blockDim = dim3(kSmallThreads);
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = st;
     cudaLaunchAttribute at;

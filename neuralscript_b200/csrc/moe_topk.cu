@@ -87,7 +87,7 @@ __device__ __forceinline__ void scores(const RouteDesc& d, int row, int lane, fl
     }
     if (d.sigmoid) {
 #pragma unroll
-        for (int i = 0; i < NV; i++) s[i] = live >> i & 1 ? 1.f / (1.f + expf(-x[i])) : 0.f;
+        for (int i = 0; i < NV; i++) s[i] = live >> i & 1 ? __frcp_rn(1.f + expf(-x[i])) : 0.f;
         return;
     }
     float m = -INFINITY;
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(128)
     float s[NV];
     float sj = 0.f;
     if (d.sigmoid) {
-        if (e >= 0) sj = 1.f / (1.f + expf(-ld_any(d.logits, d.dtype, (size_t)row * d.ld + e)));
+        if (e >= 0) sj = __frcp_rn(1.f + expf(-ld_any(d.logits, d.dtype, (size_t)row * d.ld + e)));
     } else {
         unsigned live;
         scores<NV>(d, row, lane, s, live);

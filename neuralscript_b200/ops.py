@@ -196,76 +196,96 @@ def moe_route(x, Wg, active, best, pb, probs=None):
 # anything is launched; see include/ns_b200_ops.h for the definitions.
 # ---------------------------------------------------------------------------
 _SCORE = {"softmax": 0, "sigmoid": 1}
+_f32 = _bf16 = _i32 = _u8 = _f8 = _stream_of = _device = None
 
 
-def _is(t, what, dtype, *shape):
-    """t is a CUDA tensor of the dtype and shape (None: any size) whose last dimension is contiguous."""
-    if t.dtype is not dtype:
+def _torch():
+    """torch's names that every call below needs, looked up once (a decode step's kernels take a few microseconds)."""
+    global _f32, _bf16, _i32, _u8, _f8, _stream_of, _device
+    import torch
+    _stream_of, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+    _f32, _bf16, _i32, _u8, _f8 = torch.float32, torch.bfloat16, torch.int32, torch.uint8, torch.float8_e4m3fn
+    return L()
+
+
+def _refuse(t, what, dtype, shape):
+    if dtype is not None and t.dtype is not dtype:
         raise ValueError(f"{what}: {t.dtype} where {dtype} is wanted")
-    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
-        raise ValueError(f"{what}: shape {tuple(t.shape)} where {shape} is wanted")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: shape {tuple(t.shape)} where {tuple(shape)} is wanted")
     if not t.is_cuda:
         raise ValueError(f"{what}: not on a CUDA device")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{what}: its last dimension has stride {t.stride(-1)}")
+    raise ValueError(f"{what}: strides {t.stride()} are not those of contiguous rows (or of a dense tensor where one is "
+                     "wanted)")
+
+
+def _dense(t, what, dtype, shape):
+    """Address of a CUDA tensor of this dtype and shape without gaps."""
+    if t.dtype is not dtype or t.shape != shape or not t.is_cuda or not t.is_contiguous():
+        _refuse(t, what, dtype, shape)
     return t.data_ptr()
 
 
-def _dense(t, what, dtype, *shape):
-    """As _is, without gaps between rows."""
-    at = _is(t, what, dtype, *shape)
-    if not t.is_contiguous():
-        raise ValueError(f"{what}: not contiguous")
-    return at
+def _rows(t, what, dtype, shape):
+    """Address of a CUDA tensor of this dtype and shape whose last dimension is contiguous."""
+    if t.dtype is not dtype or t.shape != shape or not t.is_cuda or (t.stride(-1) != 1 and shape[-1] > 1):
+        _refuse(t, what, dtype, shape)
+    return t.data_ptr()
 
 
-def _float(t, what, *shape):
-    """As _is, fp32 or bf16; its address, type code and leading dimension."""
-    import torch
-    if t.dtype is not torch.float32 and t.dtype is not torch.bfloat16:
-        raise ValueError(f"{what}: {t.dtype} where float32 or bfloat16 is wanted")
-    return _is(t, what, t.dtype, *shape), F32 if t.dtype is torch.float32 else BF16, _ld(t)
+def _float(t, what, shape):
+    """As _rows, fp32 or bf16: address and type code."""
+    dt = t.dtype
+    if dt is not _f32 and dt is not _bf16:
+        raise ValueError(f"{what}: {dt} where float32 or bfloat16 is wanted")
+    return _rows(t, what, dt, shape), F32 if dt is _f32 else BF16
 
 
 def _ld(t, dim=0):
-    """Stride of a dimension (that of a single row is not looked at by torch, but is by the kernels)."""
-    return max(t.stride(dim), t.shape[-1] if t.shape[dim] < 2 else 0)
+    """Leading dimension; torch does not look at the stride of a single row, the kernels do."""
+    return t.stride(dim) if t.shape[dim] > 1 else max(t.stride(dim), t.shape[-1])
 
 
 def _ld16(t, dim=0):
-    """As _ld for codes: a single row has no stride of its own."""
+    """As _ld for codes, whose rows start on 16-byte boundaries."""
     return t.stride(dim) if t.shape[dim] > 1 else -(-t.shape[-1] // 16) * 16
 
 
-def _run(name, *args):
-    import torch
-    rc = getattr(L(), name)(*args, torch.cuda.current_stream().cuda_stream)
-    if rc != 0:
-        raise RuntimeError(f"{name} returned {rc}")
+def _here(t):
+    """The current stream; the kernels run on the current device."""
+    d = _device()
+    if t.get_device() != d:
+        raise ValueError(f"tensors are on {t.device}, the current device is {d}")
+    return _stream_of(d)
 
 
 def moe_topk_route(logits, idx, w, score="softmax", bias=None, active=None, groups=1, topk_groups=1, renorm=True,
                    scale=1.0):
     """idx, w [M, k] (int32, float32) <- the k experts of each row of logits [M, E] and their weights."""
-    import torch
+    lib = _bound if _f32 else _torch()
     M, E = logits.shape
     k = idx.shape[1]
-    at, dt, ld = _float(logits, "logits", M, E)
-    _run("nsb_op_moe_topk_route", at, dt, ld, M, E, k, _SCORE[score],
-         _dense(bias, "bias", torch.float32, E) if bias is not None else None,
-         _dense(active, "active", torch.uint8, E) if active is not None else None, groups, topk_groups, int(renorm),
-         scale, _dense(idx, "idx", torch.int32, M, k), _dense(w, "w", torch.float32, M, k))
+    at, dt = _float(logits, "logits", (M, E))
+    rc = lib.nsb_op_moe_topk_route(
+        at, dt, _ld(logits), M, E, k, _SCORE[score], None if bias is None else _dense(bias, "bias", _f32, (E,)),
+        None if active is None else _dense(active, "active", _u8, (E,)), groups, topk_groups, renorm, scale,
+        _dense(idx, "idx", _i32, (M, k)), _dense(w, "w", _f32, (M, k)), _here(logits))
+    if rc:
+        _check(rc, "nsb_op_moe_topk_route")
 
 
 def moe_topk_route_bwd(dw, logits, idx, dlogits, score="softmax", active=None, renorm=True, scale=1.0):
     """dlogits [M, E] (the logits' type) <- the gradient of moe_topk_route's w."""
-    import torch
+    lib = _bound if _f32 else _torch()
     M, E = logits.shape
     k = idx.shape[1]
-    at, dt, ld = _float(logits, "logits", M, E)
-    _run("nsb_op_moe_topk_route_bwd", _dense(dw, "dw", torch.float32, M, k), at, dt, ld, M, E, k, _SCORE[score],
-         _dense(active, "active", torch.uint8, E) if active is not None else None, int(renorm), scale,
-         _dense(idx, "idx", torch.int32, M, k), _is(dlogits, "dlogits", logits.dtype, M, E), _ld(dlogits))
+    at, dt = _float(logits, "logits", (M, E))
+    rc = lib.nsb_op_moe_topk_route_bwd(
+        _dense(dw, "dw", _f32, (M, k)), at, dt, _ld(logits), M, E, k, _SCORE[score],
+        None if active is None else _dense(active, "active", _u8, (E,)), renorm, scale,
+        _dense(idx, "idx", _i32, (M, k)), _rows(dlogits, "dlogits", logits.dtype, (M, E)), _ld(dlogits), _here(logits))
+    if rc:
+        _check(rc, "nsb_op_moe_topk_route_bwd")
 
 
 def moe_dispatch_rows(M, k, E, align=1) -> int:
@@ -275,38 +295,46 @@ def moe_dispatch_rows(M, k, E, align=1) -> int:
 
 def moe_dispatch(idx, E, offsets, counts, rows, pos, align=1):
     """offsets [E + 1], counts [E], rows [moe_dispatch_rows(...)], pos [M, k] (int32) <- the pairs of idx by expert."""
-    import torch
+    lib = _bound if _f32 else _torch()
     M, k = idx.shape
-    i32 = torch.int32
-    if rows.shape[0] != moe_dispatch_rows(M, k, E, align):
-        raise ValueError(f"rows: {rows.shape[0]} where {moe_dispatch_rows(M, k, E, align)} are wanted")
-    _run("nsb_op_moe_dispatch", _dense(idx, "idx", i32, M, k), M, k, E, align, _dense(offsets, "offsets", i32, E + 1),
-         _dense(counts, "counts", i32, E), _dense(rows, "rows", i32, None), _dense(pos, "pos", i32, M, k))
+    rc = lib.nsb_op_moe_dispatch(
+        _dense(idx, "idx", _i32, (M, k)), M, k, E, align, _dense(offsets, "offsets", _i32, (E + 1,)),
+        _dense(counts, "counts", _i32, (E,)),
+        _dense(rows, "rows", _i32, (lib.nsb_op_moe_dispatch_rows(M, k, E, align),)), _dense(pos, "pos", _i32, (M, k)),
+        _here(idx))
+    if rc:
+        _check(rc, "nsb_op_moe_dispatch")
 
 
 def moe_combine(o, pos, y, w=None):
     """y [M, D] <- sum over j of w[:, j] * o[pos[:, j]] (w None: 1)."""
-    import torch
+    lib = _bound if _f32 else _torch()
     M, k = pos.shape
-    D = y.shape[1]
-    at, dt, ld = _float(o, "o", None, D)
-    _run("nsb_op_moe_combine", at, dt, ld, _dense(pos, "pos", torch.int32, M, k),
-         _dense(w, "w", torch.float32, M, k) if w is not None else None, M, k, D, _is(y, "y", o.dtype, M, D), _ld(y))
+    R, D = o.shape
+    at, dt = _float(o, "o", (R, D))
+    rc = lib.nsb_op_moe_combine(
+        at, dt, _ld(o), _dense(pos, "pos", _i32, (M, k)), None if w is None else _dense(w, "w", _f32, (M, k)), M, k, D,
+        _rows(y, "y", o.dtype, (M, D)), _ld(y), _here(o))
+    if rc:
+        _check(rc, "nsb_op_moe_combine")
 
 
 def moe_combine_bwd(dy, o, rows, pos, w, do, dw=None):
     """do [R, D], dw [M, k] <- the gradients of moe_combine's o and w (dw None: do alone; o may be None then)."""
-    import torch
+    lib = _bound if _f32 else _torch()
     M, k = pos.shape
     D = dy.shape[1]
     R = rows.shape[0]
-    at, dt, ld = _float(dy, "dy", M, D)
+    at, dt = _float(dy, "dy", (M, D))
     if dw is not None and o is None:
         raise ValueError("dw needs o")
-    _run("nsb_op_moe_combine_bwd", at, _is(o, "o", dy.dtype, R, D) if o is not None else None, dt, ld,
-         _ld(o) if o is not None else 0, _dense(rows, "rows", torch.int32, R), _dense(pos, "pos", torch.int32, M, k),
-         _dense(w, "w", torch.float32, M, k) if w is not None else None, M, k, R, D, _is(do, "do", dy.dtype, R, D),
-         _ld(do), _dense(dw, "dw", torch.float32, M, k) if dw is not None else None)
+    rc = lib.nsb_op_moe_combine_bwd(
+        at, None if o is None else _rows(o, "o", dy.dtype, (R, D)), dt, _ld(dy), 0 if o is None else _ld(o),
+        _dense(rows, "rows", _i32, (R,)), _dense(pos, "pos", _i32, (M, k)),
+        None if w is None else _dense(w, "w", _f32, (M, k)), M, k, R, D, _rows(do, "do", dy.dtype, (R, D)), _ld(do),
+        None if dw is None else _dense(dw, "dw", _f32, (M, k)), _here(dy))
+    if rc:
+        _check(rc, "nsb_op_moe_combine_bwd")
 
 
 def fp8_ld(n) -> int:
@@ -314,82 +342,92 @@ def fp8_ld(n) -> int:
     return -(-n // 16) * 16
 
 
-def _quantized(q, s, what, rows, cols, srows, scols):
-    import torch
-    if q is None:
-        return None, 0, None, 0
-    return (_is(q, what, torch.float8_e4m3fn, rows, cols), _ld16(q),
-            _is(s, what + "'s scales", torch.float32, srows, scols), _ld(s))
-
-
 def fp8_quantize(x, q=None, s=None, qt=None, st=None, act=0, rows=None, row_div=1):
     """q [M, K] with s [ceil(K / 128), M], and / or qt [K, M] with st [ceil(M / 128), K] <- codes and scales of act(x).
 
     q, qt: float8_e4m3fn with rows on 16-byte boundaries. rows [M] (int32) gathers rows[r] / row_div of x first
     (row_div 0: only puts zeros where rows is negative)."""
-    import torch
+    lib = _bound if _f32 else _torch()
     n, K = x.shape
     M = n if rows is None else rows.shape[0]
     if rows is not None and row_div == 0 and n < M:
         raise ValueError(f"x: {n} rows where {M} are wanted")
-    at, dt, ld = _float(x, "x", n, K)
-    _run("nsb_op_fp8_quantize", at, dt, ld, M, K, act,
-         _dense(rows, "rows", torch.int32, M) if rows is not None else None, row_div,
-         *_quantized(q, s, "q", M, K, -(-K // 128), M), *_quantized(qt, st, "qt", K, M, -(-M // 128), K))
+    at, dt = _float(x, "x", (n, K))
+    rc = lib.nsb_op_fp8_quantize(
+        at, dt, _ld(x), M, K, act, None if rows is None else _dense(rows, "rows", _i32, (M,)), row_div,
+        *((None, 0, None, 0) if q is None else (_rows(q, "q", _f8, (M, K)), _ld16(q),
+                                                _rows(s, "s", _f32, (-(-K // 128), M)), _ld(s))),
+        *((None, 0, None, 0) if qt is None else (_rows(qt, "qt", _f8, (K, M)), _ld16(qt),
+                                                 _rows(st, "st", _f32, (-(-M // 128), K)), _ld(st))), _here(x))
+    if rc:
+        _check(rc, "nsb_op_fp8_quantize")
 
 
 def fp8_quantize_block(x, q=None, s=None, qt=None, st=None):
     """q [M, K] with s [ceil(M / 128), ceil(K / 128)], and / or their transposes qt, st <- codes and scales of x."""
+    lib = _bound if _f32 else _torch()
     M, K = x.shape
     mb, kb = -(-M // 128), -(-K // 128)
-    at, dt, ld = _float(x, "x", M, K)
-    _run("nsb_op_fp8_quantize_block", at, dt, ld, M, K, *_quantized(q, s, "q", M, K, mb, kb),
-         *_quantized(qt, st, "qt", K, M, kb, mb))
+    at, dt = _float(x, "x", (M, K))
+    rc = lib.nsb_op_fp8_quantize_block(
+        at, dt, _ld(x), M, K,
+        *((None, 0, None, 0) if q is None else (_rows(q, "q", _f8, (M, K)), _ld16(q), _rows(s, "s", _f32, (mb, kb)),
+                                                _ld(s))),
+        *((None, 0, None, 0) if qt is None else (_rows(qt, "qt", _f8, (K, M)), _ld16(qt),
+                                                 _rows(st, "st", _f32, (kb, mb)), _ld(st))), _here(x))
+    if rc:
+        _check(rc, "nsb_op_fp8_quantize_block")
 
 
 def gemm_fp8(a, sa, b, sb, c, err=None):
     """c [M, N] (fp32 or bf16) <- A B^T of codes a [M, K] with row scales sa, b [N, K] with scales sb: of rows
-    [ceil(K / 128), N], or of blocks [ceil(N / 128), ceil(K / 128)]. Where both have that shape (K > 128 and N both
-    in one block: N = ceil(N / 128) = ceil(K / 128) = 1) they are the same."""
-    import torch
-    f8, f32 = torch.float8_e4m3fn, torch.float32
+    [ceil(K / 128), N], or of blocks [ceil(N / 128), ceil(K / 128)] (both have that shape only where they are the same:
+    N = 1 and K at most 128)."""
+    lib = _bound if _f32 else _torch()
     M, K = a.shape
     N = b.shape[0]
     kb = -(-K // 128)
-    by_rows = tuple(sb.shape) == (kb, N)
-    c_at, c_dt, ldc = _float(c, "c", M, N)
-    _run("nsb_op_gemm_fp8", M, N, K, _is(a, "a", f8, M, K), _ld16(a), _is(sa, "sa", f32, kb, M), _ld(sa),
-         _is(b, "b", f8, N, K), _ld16(b),
-         _is(sb, "sb", f32, kb, N) if by_rows else _is(sb, "sb", f32, -(-N // 128), kb), _ld(sb), int(by_rows),
-         c_at, c_dt, ldc, p(err))
+    by_rows = sb.shape == (kb, N)
+    at, dt = _float(c, "c", (M, N))
+    rc = lib.nsb_op_gemm_fp8(
+        M, N, K, _rows(a, "a", _f8, (M, K)), _ld16(a), _rows(sa, "sa", _f32, (kb, M)), _ld(sa),
+        _rows(b, "b", _f8, (N, K)), _ld16(b), _rows(sb, "sb", _f32, (kb, N) if by_rows else (-(-N // 128), kb)),
+        _ld(sb), by_rows, at, dt, _ld(c), None if err is None else err.data_ptr(), _here(a))
+    if rc:
+        _check(rc, "nsb_op_gemm_fp8")
 
 
 def moe_gemm_fp8(a, sa, offsets, counts, b, sb, c, rows=None, row_div=1, err=None):
     """Rows of c [R, N] of each expert e <- those of A times B[e]^T: a [R, K] (with rows [R]: [any, K], of which
     row r takes rows[r] / row_div) with row scales sa, b [E, N, K] with block scales sb."""
-    import torch
-    f8, f32, i32 = torch.float8_e4m3fn, torch.float32, torch.int32
+    lib = _bound if _f32 else _torch()
     n, K = a.shape
     E, N, _ = b.shape
     R = c.shape[0]
     kb = -(-K // 128)
-    c_at, c_dt, ldc = _float(c, "c", R, N)
-    _run("nsb_op_moe_gemm_fp8", R, E, N, K, _is(a, "a", f8, n if rows is not None else R, K), _ld16(a), n,
-         _is(sa, "sa", f32, kb, n), _ld(sa), _dense(rows, "rows", i32, R) if rows is not None else None, row_div,
-         _dense(offsets, "offsets", i32, E + 1), _dense(counts, "counts", i32, E), _is(b, "b", f8, E, N, K),
-         _ld16(b, 1), b.stride(0), _is(sb, "sb", f32, E, -(-N // 128), kb), _ld(sb, 1), sb.stride(0), c_at, c_dt, ldc,
-         p(err))
+    at, dt = _float(c, "c", (R, N))
+    rc = lib.nsb_op_moe_gemm_fp8(
+        R, E, N, K, _rows(a, "a", _f8, (n if rows is not None else R, K)), _ld16(a), n,
+        _rows(sa, "sa", _f32, (kb, n)), _ld(sa), None if rows is None else _dense(rows, "rows", _i32, (R,)), row_div,
+        _dense(offsets, "offsets", _i32, (E + 1,)), _dense(counts, "counts", _i32, (E,)),
+        _rows(b, "b", _f8, (E, N, K)), _ld16(b, 1), b.stride(0), _rows(sb, "sb", _f32, (E, -(-N // 128), kb)),
+        _ld(sb, 1), sb.stride(0), at, dt, _ld(c), None if err is None else err.data_ptr(), _here(a))
+    if rc:
+        _check(rc, "nsb_op_moe_gemm_fp8")
 
 
 def moe_wgrad_fp8(a, sa, b, sb, offsets, counts, c, err=None):
     """c [E, M, N] <- for each expert the sum over its columns of a [M, R] and b [N, R] (row scales sa, sb)."""
-    import torch
-    f8, f32, i32 = torch.float8_e4m3fn, torch.float32, torch.int32
+    lib = _bound if _f32 else _torch()
     M, R = a.shape
     N = b.shape[0]
     E = c.shape[0]
     rb = -(-R // 128)
-    c_at, c_dt, _ = _float(c, "c", E, M, N)
-    _run("nsb_op_moe_wgrad_fp8", M, N, R, E, _is(a, "a", f8, M, R), _ld16(a), _is(sa, "sa", f32, rb, M), _ld(sa),
-         _is(b, "b", f8, N, R), _ld16(b), _is(sb, "sb", f32, rb, N), _ld(sb), _dense(offsets, "offsets", i32, E + 1),
-         _dense(counts, "counts", i32, E), c_at, c_dt, _ld(c, 1), c.stride(0), p(err))
+    at, dt = _float(c, "c", (E, M, N))
+    rc = lib.nsb_op_moe_wgrad_fp8(
+        M, N, R, E, _rows(a, "a", _f8, (M, R)), _ld16(a), _rows(sa, "sa", _f32, (rb, M)), _ld(sa),
+        _rows(b, "b", _f8, (N, R)), _ld16(b), _rows(sb, "sb", _f32, (rb, N)), _ld(sb),
+        _dense(offsets, "offsets", _i32, (E + 1,)), _dense(counts, "counts", _i32, (E,)), at, dt, _ld(c, 1),
+        c.stride(0), None if err is None else err.data_ptr(), _here(a))
+    if rc:
+        _check(rc, "nsb_op_moe_wgrad_fp8")
