@@ -1,0 +1,68 @@
+"""The top-k mixture-of-experts layer on the GPU: forward, gradients and
+serving against the same layer in 64 bits on the values that the 8-bit
+weights stand for."""
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from neuralscript_b200.moe_topk import MoETopk  # noqa: E402
+
+
+def values(q, s):
+    E, N, K = q.shape
+    return q.double() * s.double().repeat_interleave(128, 1)[:, :N].repeat_interleave(128, 2)[:, :, :K]
+
+
+def reference(layer, x, idx):
+    """y, and the leaves x, gate, w1, w2, with the choice held."""
+    x = x.double().requires_grad_(True)
+    gate = layer.gate16.double().requires_grad_(True)
+    w1, w2 = values(*layer.q1).requires_grad_(True), values(*layer.q2).requires_grad_(True)
+    p = torch.sigmoid(x @ gate.t()).gather(1, idx.long())
+    w = p / p.sum(1, keepdim=True)
+    y = 0
+    for j in range(idx.shape[1]):
+        e = idx[:, j].long()
+        h = torch.nn.functional.gelu(torch.einsum("thd,td->th", w1[e], x))
+        y = y + w[:, j:j + 1] * torch.einsum("tdh,th->td", w2[e], h)
+    return y, (x, gate, w1, w2)
+
+
+def off(a, b):
+    return float((a.double() - b.detach()).norm() / b.detach().norm())
+
+
+# An e4m3 rounding is off by at most 2^-4, on average over a step's range about
+# 2^-5.5 = 0.022 of a value; a product's error is that of its two operands (one
+# exact here on the weights' side in forward and input gradient), and at most
+# four roundings lie one after another.
+ONE = 0.03
+
+
+@pytest.mark.parametrize("M,E,k", [(1, 4, 2), (200, 8, 2), (333, 5, 3)])
+def test_layer_against_64_bits(M, E, k):
+    layer = MoETopk(128, 256, E, k, seed=M)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    x = torch.randn(M, 128, device="cuda", generator=g).to(torch.bfloat16)
+    dy = torch.randn(M, 128, device="cuda", generator=g)
+    y, kept = layer.forward(x, align=128)
+    ref, leaves = reference(layer, x, kept["idx"])
+    assert off(y, ref) < 2 * ONE
+    (ref * dy.double()).sum().backward()
+    for got, leaf in zip(layer.backward(dy, kept), leaves):
+        assert off(got, leaf.grad) < 4 * ONE
+    served, _ = layer.forward(x)  # without padding
+    assert off(served, y.double()) < 1e-5
+
+
+def test_layer_trains_and_serves_single_tokens():
+    layer, teacher = MoETopk(128, 128, 8, 2, groups=4, topk_groups=2, seed=1), MoETopk(128, 128, 8, 2, seed=2)
+    x = torch.randn(512, 128, device="cuda", dtype=torch.bfloat16)
+    target, _ = teacher.forward(x)
+    losses = [float(layer.train_step(x, target, 3e-3)) for _ in range(40)]
+    assert losses[-1] < 0.5 * losses[0]
+    y, _ = layer.forward(x)
+    one, _ = layer.forward(x[17:18])
+    assert off(one[0], y[17].double()) < 1e-5
