@@ -72,38 +72,63 @@ __device__ __forceinline__ void load_logits(const RouteDesc& d, int row, int lan
     for (int i = 0; i < NV; i++) x[i] = e0 + i < d.E ? ld_any(d.logits, d.dtype, (size_t)row * d.ld + e0 + i) : 0.f;
 }
 
-// Their scores. Dead experts score 0. The softmax's sum is held in 64 bits
-// and rounded once, so that the scores, and with them the choice, do not
-// depend on the order of the sum.
+// Which of them live, a bit each.
 template <int NV>
-__device__ __forceinline__ void scores(const RouteDesc& d, int row, int lane, float* s, unsigned& live) {
-    float x[NV];
-    load_logits<NV>(d, row, lane, x);
-    live = 0;
+__device__ __forceinline__ unsigned living(const RouteDesc& d, int lane) {
+    const int e0 = lane * NV;
+    const unsigned there = e0 >= d.E ? 0u : d.E - e0 >= NV ? (NV < 32 ? (1u << NV % 32) - 1 : ~0u) : (1u << (d.E - e0)) - 1;
+    if (!d.active) return there;
+    unsigned live = 0;
+    if (NV % 4 == 0 && d.vec_e && e0 + NV <= d.E) {
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int e = lane * NV + i;
-        live |= e < d.E && (!d.active || d.active[e]) ? 1u << i : 0u;
+        for (int i = 0; i < NV / 4; i++) {
+            const unsigned t = reinterpret_cast<const unsigned*>(d.active + e0)[i];
+#pragma unroll
+            for (int j = 0; j < 4; j++) live |= t >> 8 * j & 0xff ? 1u << (4 * i + j) : 0u;
+        }
+        return live;
     }
+#pragma unroll
+    for (int i = 0; i < NV; i++) live |= (there >> i & 1) && d.active[e0 + i] ? 1u << i : 0u;
+    return live;
+}
+
+// Scores: sigmoid(x), or exp(x - top) / total over the living. The softmax's
+// sum is held in 64 bits and rounded once, so that the scores, and with them
+// the choice, do not depend on the order of the sum.
+struct Softmax {
+    float top = 0.f, total = 1.f;
+};
+__device__ __forceinline__ float score(const RouteDesc& d, const Softmax& m, float x) {
+    return d.sigmoid ? __frcp_rn(1.f + expf(-x)) : expf(x - m.top) / m.total;
+}
+
+// Those of this lane's experts; dead ones score 0.
+template <int NV>
+__device__ __forceinline__ Softmax scores(const RouteDesc& d, int row, int lane, unsigned live, float* s) {
+    float x[NV];
+    Softmax m;
+    load_logits<NV>(d, row, lane, x);
     if (d.sigmoid) {
 #pragma unroll
-        for (int i = 0; i < NV; i++) s[i] = live >> i & 1 ? __frcp_rn(1.f + expf(-x[i])) : 0.f;
-        return;
+        for (int i = 0; i < NV; i++) s[i] = live >> i & 1 ? score(d, m, x[i]) : 0.f;
+        return m;
     }
-    float m = -INFINITY;
+    m.top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < NV; i++)
-        if (live >> i & 1) m = fmaxf(m, x[i]);
-    m = warp_max(m);
+        if (live >> i & 1) m.top = fmaxf(m.top, x[i]);
+    m.top = warp_max(m.top);
     double sum = 0.;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-        s[i] = live >> i & 1 ? expf(x[i] - m) : 0.f;
+        s[i] = live >> i & 1 ? expf(x[i] - m.top) : 0.f;
         sum += s[i];
     }
-    const float total = (float)warp_sum(sum);
+    m.total = (float)warp_sum(sum);
 #pragma unroll
-    for (int i = 0; i < NV; i++) s[i] = s[i] / total;
+    for (int i = 0; i < NV; i++) s[i] = s[i] / m.total;
+    return m;
 }
 
 // A group's score is the sum of its two best keys b1 >= b2 (0: none there).
@@ -113,20 +138,31 @@ __device__ __forceinline__ unsigned group_score(unsigned b1, unsigned b2) {
 }
 
 // One warp a token; a lane holds NV consecutive experts. The k choices are k
-// rounds of one warp maximum; only the lane that gave an expert away looks
-// for its next best.
+// rounds of one warp maximum; only the lane that gave an expert away moves on
+// to its next best.
 template <int NV>
 __global__ void __launch_bounds__(128) route_kernel(const RouteDesc d, int* __restrict__ idx, float* __restrict__ w) {
     const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (row >= d.M) return;
+    const unsigned live = living<NV>(d, lane);
     float s[NV];
-    unsigned live, key[NV];
-    scores<NV>(d, row, lane, s, live);
+    unsigned key[NV];
+    const Softmax m = scores<NV>(d, row, lane, live, s);
+    if (d.bias) {
+        if (NV % 4 == 0 && d.vec_e && lane * NV + NV <= d.E) {
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const float v = s[i] + (d.bias && lane * NV + i < d.E ? d.bias[lane * NV + i] : 0.f);
-        key[i] = (live >> i & 1) && v > -INFINITY ? ordered(v) : 0u;
+            for (int i = 0; i < NV / 4; i++) {
+                const float4 t = reinterpret_cast<const float4*>(d.bias + lane * NV)[i];
+                s[4 * i] += t.x, s[4 * i + 1] += t.y, s[4 * i + 2] += t.z, s[4 * i + 3] += t.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; i++)
+                if (lane * NV + i < d.E) s[i] += d.bias[lane * NV + i];
+        }
     }
+#pragma unroll
+    for (int i = 0; i < NV; i++) key[i] = (live >> i & 1) && s[i] > -INFINITY ? ordered(s[i]) : 0u;
     if (d.lanes > 0) {
         // a group is the experts of `lanes` neighbouring lanes, a power of 2
         unsigned b1 = 0, b2 = 0;
@@ -198,39 +234,45 @@ __global__ void __launch_bounds__(128) route_kernel(const RouteDesc d, int* __re
                 if (of[i] == g) key[i] = 0;
         }
     }
-    int mine = -1;
-    float got = 0.f;
-    unsigned b = 0;
-    int bi = 0;
-    float bs = 0.f;
-    auto best = [&] {
-        b = 0;
+    // this lane's best key b1 of expert i1, and its second best while it is
+    // known (two rounds of a lane to one search)
+    unsigned b1 = 0, b2 = 0, gone = 0;
+    int i1 = 0, i2 = 0;
+    auto search = [&] {
+        b1 = b2 = 0;
 #pragma unroll
-        for (int i = 0; i < NV; i++)
-            if (key[i] > b) {
-                b = key[i];
-                bi = i;
-                bs = s[i];
+        for (int i = 0; i < NV; i++) {
+            const unsigned v = gone >> i & 1 ? 0u : key[i];
+            if (v > b1) {
+                b2 = b1, i2 = i1;
+                b1 = v, i1 = i;
+            } else if (v > b2) {
+                b2 = v, i2 = i;
             }
-    };
-    best();
-    for (int j = 0; j < d.k; j++) {
-        const unsigned m = __reduce_max_sync(kAll, b);
-        if (m == 0) break;
-        const int owner = __ffs(__ballot_sync(kAll, b == m)) - 1;
-        const int e = __shfl_sync(kAll, lane * NV + bi, owner);
-        const float sv = __shfl_sync(kAll, bs, owner);
-        if (lane == j) {
-            mine = e;
-            got = sv;
         }
+    };
+    search();
+    bool second = true;
+    int mine = -1;
+    for (int j = 0; j < d.k; j++) {
+        const unsigned top = __reduce_max_sync(kAll, b1);
+        if (top == 0) break;
+        const int owner = __ffs(__ballot_sync(kAll, b1 == top)) - 1;
+        const int e = __shfl_sync(kAll, lane * NV + i1, owner);
+        if (lane == j) mine = e;
         if (lane == owner) {
-#pragma unroll
-            for (int i = 0; i < NV; i++)
-                if (i == bi) key[i] = 0;
-            best();
+            gone |= 1u << i1;
+            if (second) {
+                b1 = b2, i1 = i2;
+                second = false;
+            } else {
+                search();
+                second = true;
+            }
         }
     }
+    float got = 0.f;  // the chosen one's score, once more from its logit
+    if (mine >= 0) got = score(d, m, ld_any(d.logits, d.dtype, (size_t)row * d.ld + mine));
     const float total = d.renorm ? warp_sum(got) + 1e-20f : 1.f;
     if (lane < d.k) {
         idx[(size_t)row * d.k + lane] = mine;
@@ -258,19 +300,10 @@ __global__ void __launch_bounds__(128)
     float s[NV];
     float sj = 0.f;
     if (d.sigmoid) {
-        if (e >= 0) sj = __frcp_rn(1.f + expf(-ld_any(d.logits, d.dtype, (size_t)row * d.ld + e)));
+        if (e >= 0) sj = score(d, Softmax(), ld_any(d.logits, d.dtype, (size_t)row * d.ld + e));
     } else {
-        unsigned live;
-        scores<NV>(d, row, lane, s, live);
-        for (int j = 0; j < d.k; j++) {
-            const int ej = __shfl_sync(kAll, e, j);
-            float v = 0.f;
-#pragma unroll
-            for (int i = 0; i < NV; i++)
-                if (ej >= 0 && i == ej % NV) v = s[i];
-            v = __shfl_sync(kAll, v, ej >= 0 ? ej / NV : 0);
-            if (lane == j) sj = v;
-        }
+        const Softmax m = scores<NV>(d, row, lane, living<NV>(d, lane), s);
+        if (e >= 0) sj = score(d, m, ld_any(d.logits, d.dtype, (size_t)row * d.ld + e));
     }
     float ds = d.scale * g;
     if (d.renorm) {
@@ -315,6 +348,7 @@ bool route_ok(const RouteDesc& d) {
 // ---------------------------------------------------------------------------
 constexpr int kOrderThreads = 1024;
 constexpr int kOrderWarps = kOrderThreads / 32;
+constexpr int kOrderAhead = 8;
 
 __device__ __forceinline__ unsigned cluster_rank() {
     unsigned r;
@@ -350,6 +384,7 @@ __global__ void __launch_bounds__(kOrderThreads)
     int* start = total + E;             // [E + 1] first row of an expert
     int* base = start + E + 1;          // [E] this block's first row of it
     int* sums = base + E;               // [kOrderWarps] scan over experts
+    int* ends = sums + kOrderWarps;     // [E] row behind an expert's last pair
     const unsigned rank = CTAS > 1 ? cluster_rank() : 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int i = threadIdx.x; i < kOrderWarps * E; i += kOrderThreads) sh[i] = 0;
@@ -357,11 +392,23 @@ __global__ void __launch_bounds__(kOrderThreads)
     const long long share = (P + CTAS * kOrderThreads - 1) / (CTAS * kOrderThreads) * 32;
     const long long p0 = share * (rank * kOrderWarps + warp), p1 = min(P, p0 + share);
     int* mine = sh + warp * E;
-    for (long long p = p0; p < p1; p += 32) {
-        const int e = p + lane < p1 ? idx[p + lane] : -1;
-        const unsigned peers = __match_any_sync(kAll, e);
-        if (e >= 0 && e < E && lane == __ffs(peers) - 1) mine[e] += __popc(peers);
-        __syncwarp();
+    int x[kOrderAhead];  // 32 pairs each, all loads in flight before the first is counted
+    auto load = [&](long long p) {
+#pragma unroll
+        for (int i = 0; i < kOrderAhead; i++) {
+            x[i] = p + 32 * i + lane < p1 ? idx[p + 32 * i + lane] : -1;
+            if (x[i] >= E) x[i] = -1;
+        }
+    };
+    for (long long p = p0; p < p1; p += 32 * kOrderAhead) {
+        load(p);
+#pragma unroll
+        for (int i = 0; i < kOrderAhead; i++) {
+            if (p + 32 * i >= p1) break;
+            const unsigned peers = __match_any_sync(kAll, x[i]);
+            if (x[i] >= 0 && lane == __ffs(peers) - 1) mine[x[i]] += __popc(peers);
+            __syncwarp();
+        }
     }
     __syncthreads();
     for (int e = threadIdx.x; e < E; e += kOrderThreads) {
@@ -417,26 +464,31 @@ __global__ void __launch_bounds__(kOrderThreads)
             counts[e] = all;
             if (e == E - 1) offsets[E] = first + padded;
         }
-        // rows of the padding behind the expert's last pair
-        if (e % CTAS == (int)rank)
-            for (int r = first + all; r < first + padded; r++) rows[r] = -1;
+        ends[e] = first + all;
     }
     __syncthreads();
     for (long long r = start[E] + (long long)rank * kOrderThreads + threadIdx.x; r < cap; r += CTAS * kOrderThreads)
         rows[r] = -1;
-    for (long long p = p0; p < p1; p += 32) {
-        const bool in = p + lane < p1;
-        int x = in ? idx[p + lane] : -1;
-        if (x >= E) x = -1;
-        const unsigned peers = __match_any_sync(kAll, x);
-        const int place = __popc(peers & ((1u << lane) - 1u));
-        int at = -1;
-        if (x >= 0) at = base[x] + mine[x] + place;
-        __syncwarp();
-        if (x >= 0 && place == 0) mine[x] += __popc(peers);
-        __syncwarp();
-        if (in) pos[p + lane] = at;
-        if (at >= 0) rows[at] = (int)(p + lane);
+    // rows of the padding behind an expert's last pair, a warp an expert
+    if (align > 1)
+        for (int g = rank * kOrderWarps + warp; g < E; g += CTAS * kOrderWarps)
+            for (int r = ends[g] + lane; r < start[g + 1]; r += 32) rows[r] = -1;
+    for (long long p = p0; p < p1; p += 32 * kOrderAhead) {
+        if (share > 32 * kOrderAhead) load(p);  // (else they are still there)
+#pragma unroll
+        for (int i = 0; i < kOrderAhead; i++) {
+            if (p + 32 * i >= p1) break;
+            const unsigned peers = __match_any_sync(kAll, x[i]);
+            const int place = __popc(peers & ((1u << lane) - 1u));
+            int at = -1;
+            if (x[i] >= 0) at = base[x[i]] + mine[x[i]] + place;
+            __syncwarp();
+            if (x[i] >= 0 && place == 0) mine[x[i]] += __popc(peers);
+            __syncwarp();
+            const long long pair = p + 32 * i + lane;
+            if (pair < p1) pos[pair] = at;
+            if (at >= 0) rows[at] = (int)pair;
+        }
     }
     if (CTAS > 1) cluster_sync();  // no block leaves while others read its counts
 }
@@ -608,6 +660,9 @@ void by_lane(int E, F f) {
 bool rows16(const void* p, long long ld, int dtype) {
     return !(reinterpret_cast<uintptr_t>(p) & 15) && ld * (dtype == kBF16 ? 2 : 4) % 16 == 0;
 }
+bool experts16(const RouteDesc& d) {
+    return !((reinterpret_cast<uintptr_t>(d.bias) | reinterpret_cast<uintptr_t>(d.active)) & 15);
+}
 }  // namespace
 
 int moe_topk_route(const RouteDesc& d0, int* idx, float* w, cudaStream_t st) {
@@ -617,6 +672,7 @@ int moe_topk_route(const RouteDesc& d0, int* idx, float* w, cudaStream_t st) {
     by_lane(d.E, [&](auto n) {
         constexpr int NV = decltype(n)::value;
         d.vec = NV >= 4 && rows16(d.logits, d.ld, d.dtype);
+        d.vec_e = experts16(d);
         const int per = d.E / d.groups;
         if (d.groups > 1 && per % NV == 0 && (per / NV & (per / NV - 1)) == 0) d.lanes = per / NV;
         route_kernel<NV><<<(unsigned)((d.M + 3) / 4), 128, 0, st>>>(d, idx, w);
@@ -632,6 +688,7 @@ int moe_topk_route_bwd(const RouteDesc& d0, const float* dw, const int* idx, voi
     by_lane(d.E, [&](auto n) {
         constexpr int NV = decltype(n)::value;
         d.vec = NV >= 4 && rows16(d.logits, d.ld, d.dtype);
+        d.vec_e = experts16(d);
         const int vec_d = rows16(dl, ld_d, d.dtype) && d.E * (d.dtype == kBF16 ? 2 : 4) % 16 == 0;
         route_bwd_kernel<NV><<<(unsigned)((d.M + 3) / 4), 128, 0, st>>>(d, dw, idx, dl, ld_d, vec_d);
     });
@@ -652,7 +709,7 @@ int moe_dispatch(const int* idx, int M, int k, int E, int align, int* offsets, i
     const size_t cap = moe_dispatch_rows(M, k, E, align);
     if (cap > 0x7fffffffu) return -2;
     const long long P = (long long)M * k;
-    const int smem = (kOrderWarps * E + 3 * E + 1 + kOrderWarps) * (int)sizeof(int);
+    const int smem = (kOrderWarps * E + 4 * E + 1 + kOrderWarps) * (int)sizeof(int);
     auto go = [&](auto ctas) {
         constexpr int CTAS = decltype(ctas)::value;
         auto f = dispatch_kernel<CTAS>;

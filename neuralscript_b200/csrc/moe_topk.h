@@ -24,9 +24,9 @@ struct RouteDesc {
     int groups = 1, topk_groups = 1;
     int renorm = 1;
     float scale = 1.f;
-    // set by the launch: 16-byte rows; lanes that hold a group (0: groups do not
-    // fall on whole lanes)
-    int vec = 0, lanes = 0;
+    // set by the launch: 16-byte rows of logits; bias and active on 16-byte
+    // boundaries; lanes that hold a group (0: groups do not fall on whole lanes)
+    int vec = 0, vec_e = 0, lanes = 0;
 };
 
 int moe_topk_route(const RouteDesc& d, int* idx, float* w, cudaStream_t s);
