@@ -198,6 +198,18 @@ def test_product(M, N, K, out, by_rows):
     assert c[0].isnan().all() and c[M + 1].isnan().all()
 
 
+@pytest.mark.parametrize("M,N,K", [(3900, 2500, 300), (4096, 2304, 128), (2900, 3400, 1000)])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+def test_product_of_many_tiles(M, N, K, out):
+    """Sizes from which pairs of CTAs share tiles, some of whose second halves are empty."""
+    a, sa = rows_of(wild(M, K, 1), 3)
+    b, sb = block_of(wild(N, K, 2))
+    c = torch.full((M + 1, N), math.nan, dtype=out, device=DEV)
+    ops.gemm_fp8(a, sa, b, sb, c[:M])
+    assert near(c[:M], values_rows(a, sa), values_block(b, sb), K)
+    assert c[M].isnan().all()
+
+
 @pytest.mark.parametrize("M", [3, 200])
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
 def test_product_into_rows_of_a_wider_buffer(M, out):
@@ -339,6 +351,35 @@ def test_product_on_a_side_stream_and_in_a_graph():
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(c, want)
+
+
+def test_offsets_beyond_32_bits():
+    """Rows so far apart that an element's number passes 2^31 (and a byte's 2^32)."""
+    far = 2 ** 30
+    x = torch.empty(3 * far + 256, dtype=torch.bfloat16, device=DEV).as_strided((4, 256), (far, 1))
+    x.copy_(wild(4, 256, 1))
+    q = torch.empty(3 * far + 256, dtype=torch.uint8, device=DEV).view(F8).as_strided((4, 256), (far, 1))
+    s = scales(2, 4)
+    ops.fp8_quantize(x, q, s)
+    rq, rs = ref_rows(x)
+    assert torch.equal(s, rs) and same(q, rq)
+    b, sb = block_of(wild(72, 256, 2))
+    c = x[:, :72]  # the same storage
+    ops.gemm_fp8(q, s, b, sb, c)
+    assert near(c, values_rows(q, s), values_block(b, sb), 256)
+    del x, c
+    b = torch.empty(2 * far + 300 * 256, dtype=torch.uint8, device=DEV).view(F8).as_strided((3, 72, 256), (far, 256, 1))
+    sb = torch.empty(3, 1, 2, device=DEV)
+    for e in range(3):
+        qe, se = block_of(wild(72, 256, 3 + e))
+        b[e].view(torch.uint8).copy_(qe.view(torch.uint8))
+        sb[e] = se
+    offsets, counts, rows, _ = order(torch.arange(6, device=DEV, dtype=torch.int32).view(6, 1) % 3, 3, 1)
+    c = torch.empty(6, 72, device=DEV)
+    a, sa = rows_of(wild(6, 256, 9))
+    ops.moe_gemm_fp8(a, sa, offsets, counts, b, sb, c, rows=rows)
+    for e in range(3):
+        assert near(c[2 * e:2 * e + 2], values_rows(a, sa)[rows[2 * e:2 * e + 2].long()], values_block(b[e], sb[e]), 256)
 
 
 def test_refusals():

@@ -291,6 +291,30 @@ def test_route_to_combine_on_a_side_stream():
     assert torch.all((y - 1).abs() <= 8 * EPS)  # renormalised weights of ones
 
 
+def test_offsets_beyond_32_bits():
+    """Rows so far apart that an element's number passes 2^31."""
+    far = 2 ** 30
+    wide = torch.empty(3 * far + 64, dtype=torch.bfloat16, device=DEV)
+    x = wide.as_strided((4, 64), (far, 1))
+    x.copy_(torch.randn(4, 64, device=DEV, generator=gen(1)))
+    idx, w = route(x, 3)
+    ref, ref_w = route(x.contiguous(), 3)
+    assert torch.equal(idx, ref) and torch.equal(w, ref_w)
+    pos = torch.tensor([[3, 0], [2, -1]], dtype=torch.int32, device=DEV)
+    w = torch.randn(2, 2, device=DEV, generator=gen(2))
+    y, near = torch.empty(2, 64, dtype=torch.bfloat16, device=DEV), torch.empty(2, 64, dtype=torch.bfloat16, device=DEV)
+    ops.moe_combine(x, pos, y, w=w)
+    ops.moe_combine(x.contiguous(), pos, near, w=w)
+    assert torch.equal(y, near)
+    rows = torch.tensor([1, -1, 2, 0], dtype=torch.int32, device=DEV)
+    dw, dw_near = torch.empty(2, 2, device=DEV), torch.empty(2, 2, device=DEV)
+    do = torch.empty(4, 64, dtype=torch.bfloat16, device=DEV)
+    ops.moe_combine_bwd(y, x.contiguous(), rows, pos, w, do, dw_near)
+    far_do = torch.empty(3 * far + 64, dtype=torch.bfloat16, device=DEV).as_strided((4, 64), (far, 1))
+    ops.moe_combine_bwd(y, x, rows, pos, w, far_do, dw)
+    assert torch.equal(far_do, do) and torch.equal(dw, dw_near)
+
+
 def test_refusals():
     x = torch.zeros(4, 8, device=DEV)
     idx = torch.zeros(4, 2, dtype=torch.int32, device=DEV)
