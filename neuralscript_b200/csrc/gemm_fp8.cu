@@ -72,10 +72,12 @@ struct TileCfg {
     static constexpr int BM = PAIR ? 256 : 128;       // rows of a tile
     static constexpr int BROWS = PAIR ? BN / 2 : BN;  // rows of B that this CTA loads
     static_assert(!PAIR || (!VEC && !ROWS), "pairs take one product with block scales");
+    static_assert(BN == 128 || BN == 256 || (BN == 192 && VEC), "a warp's columns lie in one scale block");
     static constexpr int A_BYTES = 128 * 128;
     static constexpr int STAGE = A_BYTES + BROWS * 128;
-    static constexpr int STAGES = PAIR ? 6 : 4;
-    static constexpr int PARTS = 512 / BN;   // parts of TMEM
+    static constexpr int STAGES = BROWS == 128 ? 6 : 4;
+    static constexpr int PCOLS = BN == 128 ? 128 : 256;  // columns of a part of TMEM
+    static constexpr int PARTS = 512 / PCOLS;
     static constexpr int COLS = BN / 2;      // columns of a warp
     static constexpr int STAGING = kEpi * 2048;  // 32 rows x 64 bytes a warp
     static constexpr int SLOT = 128 + (VEC ? BN : 4);  // a k-block's row scales, then column or block scales
@@ -261,8 +263,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int k = 0; k < 4; k++) {
                         const uint64_t da = ptx::smem_desc(sa + k * 32, 16, 1024, 2);
                         const uint64_t db = ptx::smem_desc(sb + k * 32, 16, 1024, 2);
-                        if (PAIR) ptx::mma_f8_pair(tmem + part * BN, da, db, IDESC, k > 0);
-                        else ptx::mma_f8(tmem + part * BN, da, db, IDESC, k > 0);
+                        if (PAIR) ptx::mma_f8_pair(tmem + part * C::PCOLS, da, db, IDESC, k > 0);
+                        else ptx::mma_f8(tmem + part * C::PCOLS, da, db, IDESC, k > 0);
                     }
                     if (PAIR) {
                         ptx::mma_commit_pair(&empty[stage]);
@@ -422,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 pipe.wait(&part_full[part], part_phase);
                 __syncwarp();
                 ptx::tc_fence_after();
-                const uint32_t t = lane_base + part * BN;
+                const uint32_t t = lane_base + part * C::PCOLS;
                 if constexpr (VEC) {
                     // fragments of 16 rows x 32 columns: of each a thread has two
                     // rows (lane / 4, + 8) and the columns 2 (lane % 4) of every 8,
@@ -1167,26 +1169,33 @@ int fp8_gemm(const Fp8Gemm& d, cudaStream_t st) {
     if (d.groups && (!d.offsets || !d.counts)) return -1;
     if (d.rows && d.row_div <= 0) return -1;
     if (d.a_rows <= 0) return -1;
-    if (!d.group_k) {
-        // Few rows: the weights' stream bounds the product. For one product,
-        // where 128 x 256 tiles would not fill half of the SMs; for groups,
-        // where the average one has no more than 64 rows.
-        const long long tiles = (long long)((d.M + 127) / 128) * ((d.N + 255) / 256);
-        const int rows = d.groups ? (d.M + d.groups - 1) / d.groups : d.M;
-        if (d.groups ? rows <= 64 : tiles * 2 <= num_sms()) {
-            if (rows <= 16) return d.b_rows ? launch_small<16, true>(d, st) : launch_small<16, false>(d, st);
-            if (rows <= 32) return d.b_rows ? launch_small<32, true>(d, st) : launch_small<32, false>(d, st);
-            return d.b_rows ? launch_small<64, true>(d, st) : launch_small<64, false>(d, st);
-        }
+    const int sms = num_sms();
+    const int rows = d.groups && !d.group_k ? (d.M + d.groups - 1) / d.groups : d.M;
+    // Few rows (of the average group): the weights' stream bounds the product.
+    if (!d.group_k && rows <= 64) {
+        if (rows <= 16) return d.b_rows ? launch_small<16, true>(d, st) : launch_small<16, false>(d, st);
+        if (rows <= 32) return d.b_rows ? launch_small<32, true>(d, st) : launch_small<32, false>(d, st);
+        return d.b_rows ? launch_small<64, true>(d, st) : launch_small<64, false>(d, st);
     }
-    if (d.groups && !d.group_k) return launch_tiles<256, false, true, false>(d, st);
-    if (d.b_rows) return launch_tiles<256, true, false, false>(d, st);
+    // The tile's width with the least rounds x time of a k-block, which goes
+    // about as width + 64.
+    const long long m_tiles = (d.M + 127) / 128 * (long long)(d.group_k ? d.groups : 1);
+    auto cost = [&](int bn) { return (m_tiles * ((d.N + bn - 1) / bn) + sms - 1) / sms * (bn + 64); };
+    if (d.groups && !d.group_k)
+        return cost(128) < cost(256) ? launch_tiles<128, false, true, false>(d, st)
+                                     : launch_tiles<256, false, true, false>(d, st);
+    if (d.b_rows) {
+        if (cost(192) < cost(256) && cost(192) <= cost(128)) return launch_tiles<192, true, false, false>(d, st);
+        return cost(128) < cost(256) ? launch_tiles<128, true, false, false>(d, st)
+                                     : launch_tiles<256, true, false, false>(d, st);
+    }
     // Pairs of CTAs read a third less from L2, but wait for one another: from
     // two rounds of tiles on (8192 x 4096 x 4096: 133 us against 139; 2048 x
     // 2048 x 2048, under one round: 15.1 against 14.2).
-    const long long tiles = (long long)((d.M + 255) / 256) * ((d.N + 255) / 256);
-    return tiles >= num_sms() ? launch_tiles<256, false, false, true>(d, st)
-                              : launch_tiles<256, false, false, false>(d, st);
+    const long long pairs = (long long)((d.M + 255) / 256) * ((d.N + 255) / 256);
+    if (pairs >= sms) return launch_tiles<256, false, false, true>(d, st);
+    return cost(128) < cost(256) ? launch_tiles<128, false, false, false>(d, st)
+                                 : launch_tiles<256, false, false, false>(d, st);
 }
 
 }  // namespace nsb
