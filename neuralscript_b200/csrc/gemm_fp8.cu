@@ -57,6 +57,7 @@ struct TileParams {
     const int* rows;
     int row_div;
     int m_tiles, n_tiles, nb;  // nb: 128-wide scale blocks along N
+    int split;                 // CTAs of a cluster that share a tile's k-blocks
     int tma_out, vec_out;
     int* err;
 };
@@ -83,6 +84,11 @@ struct TileCfg {
     static constexpr int SLOT = 128 + (VEC ? BN : 4);  // a k-block's row scales, then column or block scales
     static constexpr int SLOTK = VEC ? 2 : 4;  // k-blocks of a group: one wait for all their scales
     static constexpr int SCALES = kSlots * SLOTK * SLOT * 4;
+    // tiles that are few share their k-blocks over a cluster; the sums meet in
+    // the ring's place, rows 4 floats apart in banks
+    static constexpr bool SPLITS = BN == 128 && !ROWS;
+    static constexpr int SUM_LD = BN + 4;
+    static_assert(!SPLITS || 128 * SUM_LD * 4 <= STAGES * STAGE, "a tile's sums fit the ring");
     static constexpr int TABLE = ROWS ? (2 * kMaxGroups + 1) * 4 : 0;
     static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + SCALES + 512 + TABLE;
     static_assert(SMEM <= 227 * 1024, "above the shared memory of a block");
@@ -179,6 +185,15 @@ __device__ __forceinline__ void group_starts(const TileParams& p, int rows, int*
     if (lane == 0) start[p.groups] = run;
 }
 
+__device__ __forceinline__ float4 cluster_load4(const float* p, unsigned rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(ptx::cluster_addr(p, rank))
+                 : "memory");
+    return v;
+}
+
 template <int BN, bool VEC, bool ROWS, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_tile_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
@@ -200,7 +215,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     int* start = reinterpret_cast<int*>(staging + C::STAGING + C::SCALES + 512);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = PAIR ? ptx::cluster_ctarank() : 0;  // rank 0 issues the pair's MMAs
+    // a pair's first CTA issues its MMAs; CTA r of a splitting cluster takes the
+    // r-th share of the k-blocks
+    const uint32_t rank = PAIR ? ptx::cluster_ctarank() : 0;
+    const int split = C::SPLITS ? p.split : 1, share_of = split > 1 ? (int)ptx::cluster_ctarank() : 0;
     const bool gather = ROWS && p.rows;
     if (threadIdx.x == 0) {
         *dead = 0;
@@ -239,7 +257,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     ptx::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int total = ROWS ? start[p.groups] * p.n_tiles : p.m_tiles * p.n_tiles * (p.groups ? p.groups : 1);
-    const int first = PAIR ? blockIdx.x / 2 : blockIdx.x, stride = PAIR ? gridDim.x / 2 : gridDim.x;
+    const int first = PAIR ? blockIdx.x / 2 : blockIdx.x / split;
+    const int stride = PAIR ? gridDim.x / 2 : gridDim.x / split;
+    auto unit = [&](int u) {
+        Unit w = unit_at<C::BM, BN, ROWS>(p, start, u);
+        if (C::SPLITS && split > 1) {
+            const int share = (w.kb1 - w.kb0 + split - 1) / split;
+            w.kb0 = min(w.kb1, w.kb0 + share_of * share);
+            w.kb1 = min(w.kb1, w.kb0 + share);
+        }
+        return w;
+    };
 
     if (warp == 1 || warp == 2) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -248,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const Pipe pipe{dead, p.err, kErrTimeoutMma};
             int it = 0;  // k-blocks so far: number `it` uses stage it % STAGES and part it % PARTS
             for (int u = first; u < total; u += stride) {
-                const Unit w = unit_at<C::BM, BN, ROWS>(p, start, u);
+                const Unit w = unit(u);
                 for (int kb = w.kb0; kb < w.kb1; kb++, it++) {
                     if ((it & 1) != mine) continue;
                     const int stage = it % C::STAGES, part = it % C::PARTS;
@@ -283,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t slot_phase = 0, phase = 0;
         const Pipe pipe{dead, p.err, kErrTimeoutProducer};
         for (int u = first; u < total; u += stride) {
-            Unit w = unit_at<C::BM, BN, ROWS>(p, start, u);
+            Unit w = unit(u);
             if (PAIR) w.m0 += rank * 128;
             // the rows whose scales this thread copies; rows past the end
             // take the first one's, and are not stored
@@ -392,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const Pipe pipe{dead, p.err, kErrTimeoutEpilogue};
         const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + half * C::COLS;
         for (int u = first; u < total; u += stride) {
-            Unit w = unit_at<C::BM, BN, ROWS>(p, start, u);
+            Unit w = unit(u);
             if (PAIR) w.m0 += rank * 128;
             const int row = w.m0 + quarter * 32 + lane;
             const bool valid = row < w.row_end;
@@ -486,6 +514,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (++part == C::PARTS) {
                     part = 0;
                     part_phase ^= 1;
+                }
+            }
+            if constexpr (C::SPLITS) {
+                if (split > 1) {
+                    // (this CTA's loads have all been used: its last part was read)
+                    float* sum = reinterpret_cast<float*>(smem) + half * C::COLS;
+                    if constexpr (VEC) {
+#pragma unroll
+                        for (int j = 0; j < C::COLS / 2; j++)
+                            *reinterpret_cast<float2*>(
+                                sum + (quarter * 32 + (j >> 3 & 1) * 16 + (j & 1) * 8 + (lane >> 2)) * C::SUM_LD +
+                                (j >> 4) * 32 + (j >> 1 & 3) * 8 + (lane & 3) * 2) = make_float2(acc[2 * j], acc[2 * j + 1]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < C::COLS / 4; j++)
+                            *reinterpret_cast<float4*>(sum + (quarter * 32 + lane) * C::SUM_LD + 4 * j) =
+                                make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+                    }
+                    continue;
                 }
             }
             if constexpr (VEC) {
@@ -612,6 +659,47 @@ __global__ void __launch_bounds__(kThreads, 1)
         ptx::tc_fence_after();
         if (PAIR) ptx::tmem_dealloc_pair(tmem, 512);
         else ptx::tmem_dealloc(tmem, 512);
+    }
+    if constexpr (C::SPLITS) {
+        if (split > 1) {
+            // the shares are added in rank order; rank r stores every split-th row
+            __syncwarp();
+            ptx::cluster_sync();
+            const Unit w = unit_at<C::BM, BN, ROWS>(p, start, first);
+            const float* sum = reinterpret_cast<const float*>(smem);
+            constexpr int QUADS = BN / 4;
+            for (int i = threadIdx.x; i < 128 / split * QUADS; i += kThreads) {
+                const int r = i / QUADS * split + share_of, n = w.n0 + i % QUADS * 4, m = w.m0 + r;
+                if (m >= w.row_end || n >= p.N) continue;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int q = 0; q < split; q++) {
+                    const float4 t = cluster_load4(sum + r * C::SUM_LD + i % QUADS * 4, q);
+                    v.x += t.x, v.y += t.y, v.z += t.z, v.w += t.w;
+                }
+                const size_t at = (size_t)m * p.ldc + n;
+                const float f[4] = {v.x, v.y, v.z, v.w};
+                if (p.c_dtype == kBF16) {
+                    __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(p.c) + at;
+                    if (p.vec_out && n + 4 <= p.N) {
+                        reinterpret_cast<__nv_bfloat162*>(o)[0] = __floats2bfloat162_rn(v.x, v.y);
+                        reinterpret_cast<__nv_bfloat162*>(o)[1] = __floats2bfloat162_rn(v.z, v.w);
+                    } else {
+                        for (int j = 0; j < 4; j++)
+                            if (n + j < p.N) o[j] = f2bf(f[j]);
+                    }
+                } else {
+                    float* o = reinterpret_cast<float*>(p.c) + at;
+                    if (p.vec_out && n + 4 <= p.N) {
+                        *reinterpret_cast<float4*>(o) = v;
+                    } else {
+                        for (int j = 0; j < 4; j++)
+                            if (n + j < p.N) o[j] = f[j];
+                    }
+                }
+            }
+            __syncwarp();
+            ptx::cluster_sync();  // no CTA leaves while others read its sums
+        }
     }
 }
 
@@ -1065,6 +1153,7 @@ TileParams params(const Fp8Gemm& d, int bm, int bn) {
     p.n_tiles = (d.N + bn - 1) / bn;
     p.nb = (d.N + 127) / 128;
     p.tma_out = p.vec_out = 0;
+    p.split = 1;
     p.err = d.err;
     return p;
 }
@@ -1128,7 +1217,10 @@ int launch_tiles(const Fp8Gemm& d, cudaStream_t st) {
     cfg.stream = st;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = PAIR ? 2 : 1;
+    // (a tile's group of rows or of k-blocks is not split)
+    if (C::SPLITS && !d.groups)
+        while (p.split < 8 && units * p.split * 2 <= num_sms() && (d.K + 127) / 128 >= p.split * 4) p.split *= 2;
+    at.val.clusterDim.x = PAIR ? 2 : p.split;
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
@@ -1144,7 +1236,8 @@ int launch_tiles(const Fp8Gemm& d, cudaStream_t st) {
         }
         slots = pairs[dev];
     }
-    cfg.gridDim = dim3((unsigned)((units < slots ? units : slots) * (PAIR ? 2 : 1)));
+    if (p.split > 1) cfg.gridDim = dim3((unsigned)(units * p.split));  // one tile a cluster
+    else cfg.gridDim = dim3((unsigned)((units < slots ? units : slots) * (PAIR ? 2 : 1)));
     return cudaLaunchKernelEx(&cfg, k, ta, tb, tc, p) == cudaSuccess ? 0 : -5;
 }
 
