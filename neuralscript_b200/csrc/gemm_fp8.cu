@@ -323,7 +323,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 srow[i] = p.sa + r;
             }
             const float* sb = p.sb;
-            if (!VEC) sb += (ROWS ? w.g * p.sb_stride : 0) + (long long)min(w.n0 / 128 + (t & 1) * (BN / 256), p.nb - 1) * p.ld_sb;
+            if (!VEC)
+                sb += (ROWS ? w.g * p.sb_stride : 0) +
+                      (long long)min(w.n0 / 128 + (t & 1) * (BN / 256), p.nb - 1) * p.ld_sb;
             // gathered: pieces t % 4 and t % 4 + 4 (of 16 bytes) of rows t / 4,
             // t / 4 + 16, ...; rows past the end read the first one's
             const uint8_t* from[8];

@@ -241,14 +241,14 @@ def _float(t, what, shape):
     return _rows(t, what, dt, shape), F32 if dt is _f32 else BF16
 
 
-def _ld(t, dim=0):
+def _ld(t, rows, cols, dim=0):
     """Leading dimension; torch does not look at the stride of a single row, the kernels do."""
-    return t.stride(dim) if t.shape[dim] > 1 else max(t.stride(dim), t.shape[-1])
+    return t.stride(dim) if rows > 1 else max(t.stride(dim), cols)
 
 
-def _ld16(t, dim=0):
+def _ld16(t, rows, cols, dim=0):
     """As _ld for codes, whose rows start on 16-byte boundaries."""
-    return t.stride(dim) if t.shape[dim] > 1 else -(-t.shape[-1] // 16) * 16
+    return t.stride(dim) if rows > 1 else -(-cols // 16) * 16
 
 
 def _here(t):
@@ -267,7 +267,7 @@ def moe_topk_route(logits, idx, w, score="softmax", bias=None, active=None, grou
     k = idx.shape[1]
     at, dt = _float(logits, "logits", (M, E))
     rc = lib.nsb_op_moe_topk_route(
-        at, dt, _ld(logits), M, E, k, _SCORE[score], None if bias is None else _dense(bias, "bias", _f32, (E,)),
+        at, dt, _ld(logits, M, E), M, E, k, _SCORE[score], None if bias is None else _dense(bias, "bias", _f32, (E,)),
         None if active is None else _dense(active, "active", _u8, (E,)), groups, topk_groups, renorm, scale,
         _dense(idx, "idx", _i32, (M, k)), _dense(w, "w", _f32, (M, k)), _here(logits))
     if rc:
@@ -281,9 +281,9 @@ def moe_topk_route_bwd(dw, logits, idx, dlogits, score="softmax", active=None, r
     k = idx.shape[1]
     at, dt = _float(logits, "logits", (M, E))
     rc = lib.nsb_op_moe_topk_route_bwd(
-        _dense(dw, "dw", _f32, (M, k)), at, dt, _ld(logits), M, E, k, _SCORE[score],
+        _dense(dw, "dw", _f32, (M, k)), at, dt, _ld(logits, M, E), M, E, k, _SCORE[score],
         None if active is None else _dense(active, "active", _u8, (E,)), renorm, scale,
-        _dense(idx, "idx", _i32, (M, k)), _rows(dlogits, "dlogits", logits.dtype, (M, E)), _ld(dlogits), _here(logits))
+        _dense(idx, "idx", _i32, (M, k)), _rows(dlogits, "dlogits", logits.dtype, (M, E)), _ld(dlogits, M, E), _here(logits))
     if rc:
         _check(rc, "nsb_op_moe_topk_route_bwd")
 
@@ -313,8 +313,8 @@ def moe_combine(o, pos, y, w=None):
     R, D = o.shape
     at, dt = _float(o, "o", (R, D))
     rc = lib.nsb_op_moe_combine(
-        at, dt, _ld(o), _dense(pos, "pos", _i32, (M, k)), None if w is None else _dense(w, "w", _f32, (M, k)), M, k, D,
-        _rows(y, "y", o.dtype, (M, D)), _ld(y), _here(o))
+        at, dt, _ld(o, R, D), _dense(pos, "pos", _i32, (M, k)), None if w is None else _dense(w, "w", _f32, (M, k)), M, k, D,
+        _rows(y, "y", o.dtype, (M, D)), _ld(y, M, D), _here(o))
     if rc:
         _check(rc, "nsb_op_moe_combine")
 
@@ -329,9 +329,9 @@ def moe_combine_bwd(dy, o, rows, pos, w, do, dw=None):
     if dw is not None and o is None:
         raise ValueError("dw needs o")
     rc = lib.nsb_op_moe_combine_bwd(
-        at, None if o is None else _rows(o, "o", dy.dtype, (R, D)), dt, _ld(dy), 0 if o is None else _ld(o),
+        at, None if o is None else _rows(o, "o", dy.dtype, (R, D)), dt, _ld(dy, M, D), 0 if o is None else _ld(o, R, D),
         _dense(rows, "rows", _i32, (R,)), _dense(pos, "pos", _i32, (M, k)),
-        None if w is None else _dense(w, "w", _f32, (M, k)), M, k, R, D, _rows(do, "do", dy.dtype, (R, D)), _ld(do),
+        None if w is None else _dense(w, "w", _f32, (M, k)), M, k, R, D, _rows(do, "do", dy.dtype, (R, D)), _ld(do, R, D),
         None if dw is None else _dense(dw, "dw", _f32, (M, k)), _here(dy))
     if rc:
         _check(rc, "nsb_op_moe_combine_bwd")
@@ -354,11 +354,12 @@ def fp8_quantize(x, q=None, s=None, qt=None, st=None, act=0, rows=None, row_div=
         raise ValueError(f"x: {n} rows where {M} are wanted")
     at, dt = _float(x, "x", (n, K))
     rc = lib.nsb_op_fp8_quantize(
-        at, dt, _ld(x), M, K, act, None if rows is None else _dense(rows, "rows", _i32, (M,)), row_div,
-        *((None, 0, None, 0) if q is None else (_rows(q, "q", _f8, (M, K)), _ld16(q),
-                                                _rows(s, "s", _f32, (-(-K // 128), M)), _ld(s))),
-        *((None, 0, None, 0) if qt is None else (_rows(qt, "qt", _f8, (K, M)), _ld16(qt),
-                                                 _rows(st, "st", _f32, (-(-M // 128), K)), _ld(st))), _here(x))
+        at, dt, _ld(x, n, K), M, K, act, None if rows is None else _dense(rows, "rows", _i32, (M,)), row_div,
+        *((None, 0, None, 0) if q is None else (_rows(q, "q", _f8, (M, K)), _ld16(q, M, K),
+                                                _rows(s, "s", _f32, (-(-K // 128), M)), _ld(s, -(-K // 128), M))),
+        *((None, 0, None, 0) if qt is None else (_rows(qt, "qt", _f8, (K, M)), _ld16(qt, K, M),
+                                                 _rows(st, "st", _f32, (-(-M // 128), K)), _ld(st, -(-M // 128), K))),
+        _here(x))
     if rc:
         _check(rc, "nsb_op_fp8_quantize")
 
@@ -370,11 +371,11 @@ def fp8_quantize_block(x, q=None, s=None, qt=None, st=None):
     mb, kb = -(-M // 128), -(-K // 128)
     at, dt = _float(x, "x", (M, K))
     rc = lib.nsb_op_fp8_quantize_block(
-        at, dt, _ld(x), M, K,
-        *((None, 0, None, 0) if q is None else (_rows(q, "q", _f8, (M, K)), _ld16(q), _rows(s, "s", _f32, (mb, kb)),
-                                                _ld(s))),
-        *((None, 0, None, 0) if qt is None else (_rows(qt, "qt", _f8, (K, M)), _ld16(qt),
-                                                 _rows(st, "st", _f32, (kb, mb)), _ld(st))), _here(x))
+        at, dt, _ld(x, M, K), M, K,
+        *((None, 0, None, 0) if q is None else (_rows(q, "q", _f8, (M, K)), _ld16(q, M, K), _rows(s, "s", _f32, (mb, kb)),
+                                                _ld(s, mb, kb))),
+        *((None, 0, None, 0) if qt is None else (_rows(qt, "qt", _f8, (K, M)), _ld16(qt, K, M),
+                                                 _rows(st, "st", _f32, (kb, mb)), _ld(st, kb, mb))), _here(x))
     if rc:
         _check(rc, "nsb_op_fp8_quantize_block")
 
@@ -389,10 +390,11 @@ def gemm_fp8(a, sa, b, sb, c, err=None):
     kb = -(-K // 128)
     by_rows = sb.shape == (kb, N)
     at, dt = _float(c, "c", (M, N))
+    sr, sc = (kb, N) if by_rows else (-(-N // 128), kb)
     rc = lib.nsb_op_gemm_fp8(
-        M, N, K, _rows(a, "a", _f8, (M, K)), _ld16(a), _rows(sa, "sa", _f32, (kb, M)), _ld(sa),
-        _rows(b, "b", _f8, (N, K)), _ld16(b), _rows(sb, "sb", _f32, (kb, N) if by_rows else (-(-N // 128), kb)),
-        _ld(sb), by_rows, at, dt, _ld(c), None if err is None else err.data_ptr(), _here(a))
+        M, N, K, _rows(a, "a", _f8, (M, K)), _ld16(a, M, K), _rows(sa, "sa", _f32, (kb, M)), _ld(sa, kb, M),
+        _rows(b, "b", _f8, (N, K)), _ld16(b, N, K), _rows(sb, "sb", _f32, (sr, sc)), _ld(sb, sr, sc), by_rows, at, dt,
+        _ld(c, M, N), None if err is None else err.data_ptr(), _here(a))
     if rc:
         _check(rc, "nsb_op_gemm_fp8")
 
@@ -407,11 +409,11 @@ def moe_gemm_fp8(a, sa, offsets, counts, b, sb, c, rows=None, row_div=1, err=Non
     kb = -(-K // 128)
     at, dt = _float(c, "c", (R, N))
     rc = lib.nsb_op_moe_gemm_fp8(
-        R, E, N, K, _rows(a, "a", _f8, (n if rows is not None else R, K)), _ld16(a), n,
-        _rows(sa, "sa", _f32, (kb, n)), _ld(sa), None if rows is None else _dense(rows, "rows", _i32, (R,)), row_div,
+        R, E, N, K, _rows(a, "a", _f8, (n if rows is not None else R, K)), _ld16(a, n, K), n,
+        _rows(sa, "sa", _f32, (kb, n)), _ld(sa, kb, n), None if rows is None else _dense(rows, "rows", _i32, (R,)), row_div,
         _dense(offsets, "offsets", _i32, (E + 1,)), _dense(counts, "counts", _i32, (E,)),
-        _rows(b, "b", _f8, (E, N, K)), _ld16(b, 1), b.stride(0), _rows(sb, "sb", _f32, (E, -(-N // 128), kb)),
-        _ld(sb, 1), sb.stride(0), at, dt, _ld(c), None if err is None else err.data_ptr(), _here(a))
+        _rows(b, "b", _f8, (E, N, K)), _ld16(b, N, K, 1), b.stride(0), _rows(sb, "sb", _f32, (E, -(-N // 128), kb)),
+        _ld(sb, -(-N // 128), kb, 1), sb.stride(0), at, dt, _ld(c, R, N), None if err is None else err.data_ptr(), _here(a))
     if rc:
         _check(rc, "nsb_op_moe_gemm_fp8")
 
@@ -425,9 +427,9 @@ def moe_wgrad_fp8(a, sa, b, sb, offsets, counts, c, err=None):
     rb = -(-R // 128)
     at, dt = _float(c, "c", (E, M, N))
     rc = lib.nsb_op_moe_wgrad_fp8(
-        M, N, R, E, _rows(a, "a", _f8, (M, R)), _ld16(a), _rows(sa, "sa", _f32, (rb, M)), _ld(sa),
-        _rows(b, "b", _f8, (N, R)), _ld16(b), _rows(sb, "sb", _f32, (rb, N)), _ld(sb),
-        _dense(offsets, "offsets", _i32, (E + 1,)), _dense(counts, "counts", _i32, (E,)), at, dt, _ld(c, 1),
+        M, N, R, E, _rows(a, "a", _f8, (M, R)), _ld16(a, M, R), _rows(sa, "sa", _f32, (rb, M)), _ld(sa, rb, M),
+        _rows(b, "b", _f8, (N, R)), _ld16(b, N, R), _rows(sb, "sb", _f32, (rb, N)), _ld(sb, rb, N),
+        _dense(offsets, "offsets", _i32, (E + 1,)), _dense(counts, "counts", _i32, (E,)), at, dt, _ld(c, M, N, 1),
         c.stride(0), None if err is None else err.data_ptr(), _here(a))
     if rc:
         _check(rc, "nsb_op_moe_wgrad_fp8")
