@@ -226,29 +226,40 @@ def _dense(t, what, dtype, shape):
     return t.data_ptr()
 
 
-def _rows(t, what, dtype, shape):
-    """Address of a CUDA tensor of this dtype and shape whose last dimension is contiguous."""
-    if t.dtype is not dtype or t.shape != shape or not t.is_cuda or (t.stride(-1) != 1 and shape[-1] > 1):
-        _refuse(t, what, dtype, shape)
-    return t.data_ptr()
+def _rows(t, what, dtype, rows, cols):
+    """Address and leading dimension of a CUDA matrix of this dtype and shape whose rows are contiguous. (torch does
+    not look at the stride of a single row; the kernels do.)"""
+    if t.dtype is not dtype or t.shape != (rows, cols) or not t.is_cuda:
+        _refuse(t, what, dtype, (rows, cols))
+    ld, one = t.stride()
+    if one != 1 and cols > 1:
+        _refuse(t, what, dtype, (rows, cols))
+    return t.data_ptr(), ld if rows > 1 else max(ld, cols)
 
 
-def _float(t, what, shape):
-    """As _rows, fp32 or bf16: address and type code."""
+def _float(t, what, rows, cols):
+    """As _rows, fp32 or bf16: address, type code and leading dimension."""
     dt = t.dtype
     if dt is not _f32 and dt is not _bf16:
         raise ValueError(f"{what}: {dt} where float32 or bfloat16 is wanted")
-    return _rows(t, what, dt, shape), F32 if dt is _f32 else BF16
+    at, ld = _rows(t, what, dt, rows, cols)
+    return at, F32 if dt is _f32 else BF16, ld
 
 
-def _ld(t, rows, cols, dim=0):
-    """Leading dimension; torch does not look at the stride of a single row, the kernels do."""
-    return t.stride(dim) if rows > 1 else max(t.stride(dim), cols)
+def _codes(t, what, rows, cols):
+    """As _rows for codes, whose rows start on 16-byte boundaries."""
+    at, ld = _rows(t, what, _f8, rows, cols)
+    return at, ld if rows > 1 else -(-cols // 16) * 16
 
 
-def _ld16(t, rows, cols, dim=0):
-    """As _ld for codes, whose rows start on 16-byte boundaries."""
-    return t.stride(dim) if rows > 1 else -(-cols // 16) * 16
+def _stack(t, what, dtype, n, rows, cols):
+    """As _rows for n matrices: address, leading dimension and the stride from one to the next."""
+    if t.dtype is not dtype or t.shape != (n, rows, cols) or not t.is_cuda:
+        _refuse(t, what, dtype, (n, rows, cols))
+    apart, ld, one = t.stride()
+    if one != 1 and cols > 1:
+        _refuse(t, what, dtype, (n, rows, cols))
+    return t.data_ptr(), ld if rows > 1 else max(ld, -(-cols // 16) * 16 if dtype is _f8 else cols), apart
 
 
 def _here(t):
@@ -265,9 +276,9 @@ def moe_topk_route(logits, idx, w, score="softmax", bias=None, active=None, grou
     lib = _bound if _f32 else _torch()
     M, E = logits.shape
     k = idx.shape[1]
-    at, dt = _float(logits, "logits", (M, E))
     rc = lib.nsb_op_moe_topk_route(
-        at, dt, _ld(logits, M, E), M, E, k, _SCORE[score], None if bias is None else _dense(bias, "bias", _f32, (E,)),
+        *_float(logits, "logits", M, E), M, E, k, _SCORE[score],
+        None if bias is None else _dense(bias, "bias", _f32, (E,)),
         None if active is None else _dense(active, "active", _u8, (E,)), groups, topk_groups, renorm, scale,
         _dense(idx, "idx", _i32, (M, k)), _dense(w, "w", _f32, (M, k)), _here(logits))
     if rc:
@@ -279,11 +290,10 @@ def moe_topk_route_bwd(dw, logits, idx, dlogits, score="softmax", active=None, r
     lib = _bound if _f32 else _torch()
     M, E = logits.shape
     k = idx.shape[1]
-    at, dt = _float(logits, "logits", (M, E))
     rc = lib.nsb_op_moe_topk_route_bwd(
-        _dense(dw, "dw", _f32, (M, k)), at, dt, _ld(logits, M, E), M, E, k, _SCORE[score],
+        _dense(dw, "dw", _f32, (M, k)), *_float(logits, "logits", M, E), M, E, k, _SCORE[score],
         None if active is None else _dense(active, "active", _u8, (E,)), renorm, scale,
-        _dense(idx, "idx", _i32, (M, k)), _rows(dlogits, "dlogits", logits.dtype, (M, E)), _ld(dlogits, M, E), _here(logits))
+        _dense(idx, "idx", _i32, (M, k)), *_rows(dlogits, "dlogits", logits.dtype, M, E), _here(logits))
     if rc:
         _check(rc, "nsb_op_moe_topk_route_bwd")
 
@@ -311,10 +321,9 @@ def moe_combine(o, pos, y, w=None):
     lib = _bound if _f32 else _torch()
     M, k = pos.shape
     R, D = o.shape
-    at, dt = _float(o, "o", (R, D))
     rc = lib.nsb_op_moe_combine(
-        at, dt, _ld(o, R, D), _dense(pos, "pos", _i32, (M, k)), None if w is None else _dense(w, "w", _f32, (M, k)), M, k, D,
-        _rows(y, "y", o.dtype, (M, D)), _ld(y, M, D), _here(o))
+        *_float(o, "o", R, D), _dense(pos, "pos", _i32, (M, k)),
+        None if w is None else _dense(w, "w", _f32, (M, k)), M, k, D, *_rows(y, "y", o.dtype, M, D), _here(o))
     if rc:
         _check(rc, "nsb_op_moe_combine")
 
@@ -325,13 +334,13 @@ def moe_combine_bwd(dy, o, rows, pos, w, do, dw=None):
     M, k = pos.shape
     D = dy.shape[1]
     R = rows.shape[0]
-    at, dt = _float(dy, "dy", (M, D))
     if dw is not None and o is None:
         raise ValueError("dw needs o")
+    at, dt, ld = _float(dy, "dy", M, D)
+    o_at, o_ld = (None, 0) if o is None else _rows(o, "o", dy.dtype, R, D)
     rc = lib.nsb_op_moe_combine_bwd(
-        at, None if o is None else _rows(o, "o", dy.dtype, (R, D)), dt, _ld(dy, M, D), 0 if o is None else _ld(o, R, D),
-        _dense(rows, "rows", _i32, (R,)), _dense(pos, "pos", _i32, (M, k)),
-        None if w is None else _dense(w, "w", _f32, (M, k)), M, k, R, D, _rows(do, "do", dy.dtype, (R, D)), _ld(do, R, D),
+        at, o_at, dt, ld, o_ld, _dense(rows, "rows", _i32, (R,)), _dense(pos, "pos", _i32, (M, k)),
+        None if w is None else _dense(w, "w", _f32, (M, k)), M, k, R, D, *_rows(do, "do", dy.dtype, R, D),
         None if dw is None else _dense(dw, "dw", _f32, (M, k)), _here(dy))
     if rc:
         _check(rc, "nsb_op_moe_combine_bwd")
@@ -340,6 +349,9 @@ def moe_combine_bwd(dy, o, rows, pos, w, do, dw=None):
 def fp8_ld(n) -> int:
     """Leading dimension of n codes a row: rows start on 16-byte boundaries."""
     return -(-n // 16) * 16
+
+
+_NOTHING = (None, 0, None, 0)
 
 
 def fp8_quantize(x, q=None, s=None, qt=None, st=None, act=0, rows=None, row_div=1):
@@ -352,14 +364,10 @@ def fp8_quantize(x, q=None, s=None, qt=None, st=None, act=0, rows=None, row_div=
     M = n if rows is None else rows.shape[0]
     if rows is not None and row_div == 0 and n < M:
         raise ValueError(f"x: {n} rows where {M} are wanted")
-    at, dt = _float(x, "x", (n, K))
     rc = lib.nsb_op_fp8_quantize(
-        at, dt, _ld(x, n, K), M, K, act, None if rows is None else _dense(rows, "rows", _i32, (M,)), row_div,
-        *((None, 0, None, 0) if q is None else (_rows(q, "q", _f8, (M, K)), _ld16(q, M, K),
-                                                _rows(s, "s", _f32, (-(-K // 128), M)), _ld(s, -(-K // 128), M))),
-        *((None, 0, None, 0) if qt is None else (_rows(qt, "qt", _f8, (K, M)), _ld16(qt, K, M),
-                                                 _rows(st, "st", _f32, (-(-M // 128), K)), _ld(st, -(-M // 128), K))),
-        _here(x))
+        *_float(x, "x", n, K), M, K, act, None if rows is None else _dense(rows, "rows", _i32, (M,)), row_div,
+        *(_NOTHING if q is None else _codes(q, "q", M, K) + _rows(s, "s", _f32, -(-K // 128), M)),
+        *(_NOTHING if qt is None else _codes(qt, "qt", K, M) + _rows(st, "st", _f32, -(-M // 128), K)), _here(x))
     if rc:
         _check(rc, "nsb_op_fp8_quantize")
 
@@ -369,13 +377,10 @@ def fp8_quantize_block(x, q=None, s=None, qt=None, st=None):
     lib = _bound if _f32 else _torch()
     M, K = x.shape
     mb, kb = -(-M // 128), -(-K // 128)
-    at, dt = _float(x, "x", (M, K))
     rc = lib.nsb_op_fp8_quantize_block(
-        at, dt, _ld(x, M, K), M, K,
-        *((None, 0, None, 0) if q is None else (_rows(q, "q", _f8, (M, K)), _ld16(q, M, K), _rows(s, "s", _f32, (mb, kb)),
-                                                _ld(s, mb, kb))),
-        *((None, 0, None, 0) if qt is None else (_rows(qt, "qt", _f8, (K, M)), _ld16(qt, K, M),
-                                                 _rows(st, "st", _f32, (kb, mb)), _ld(st, kb, mb))), _here(x))
+        *_float(x, "x", M, K), M, K,
+        *(_NOTHING if q is None else _codes(q, "q", M, K) + _rows(s, "s", _f32, mb, kb)),
+        *(_NOTHING if qt is None else _codes(qt, "qt", K, M) + _rows(st, "st", _f32, kb, mb)), _here(x))
     if rc:
         _check(rc, "nsb_op_fp8_quantize_block")
 
@@ -389,12 +394,11 @@ def gemm_fp8(a, sa, b, sb, c, err=None):
     N = b.shape[0]
     kb = -(-K // 128)
     by_rows = sb.shape == (kb, N)
-    at, dt = _float(c, "c", (M, N))
-    sr, sc = (kb, N) if by_rows else (-(-N // 128), kb)
+    at, dt, ld = _float(c, "c", M, N)
     rc = lib.nsb_op_gemm_fp8(
-        M, N, K, _rows(a, "a", _f8, (M, K)), _ld16(a, M, K), _rows(sa, "sa", _f32, (kb, M)), _ld(sa, kb, M),
-        _rows(b, "b", _f8, (N, K)), _ld16(b, N, K), _rows(sb, "sb", _f32, (sr, sc)), _ld(sb, sr, sc), by_rows, at, dt,
-        _ld(c, M, N), None if err is None else err.data_ptr(), _here(a))
+        M, N, K, *_codes(a, "a", M, K), *_rows(sa, "sa", _f32, kb, M), *_codes(b, "b", N, K),
+        *(_rows(sb, "sb", _f32, kb, N) if by_rows else _rows(sb, "sb", _f32, -(-N // 128), kb)), by_rows, at, dt, ld,
+        None if err is None else err.data_ptr(), _here(a))
     if rc:
         _check(rc, "nsb_op_gemm_fp8")
 
@@ -407,13 +411,13 @@ def moe_gemm_fp8(a, sa, offsets, counts, b, sb, c, rows=None, row_div=1, err=Non
     E, N, _ = b.shape
     R = c.shape[0]
     kb = -(-K // 128)
-    at, dt = _float(c, "c", (R, N))
+    at, dt, ld = _float(c, "c", R, N)
     rc = lib.nsb_op_moe_gemm_fp8(
-        R, E, N, K, _rows(a, "a", _f8, (n if rows is not None else R, K)), _ld16(a, n, K), n,
-        _rows(sa, "sa", _f32, (kb, n)), _ld(sa, kb, n), None if rows is None else _dense(rows, "rows", _i32, (R,)), row_div,
+        R, E, N, K, *_codes(a, "a", n if rows is not None else R, K), n, *_rows(sa, "sa", _f32, kb, n),
+        None if rows is None else _dense(rows, "rows", _i32, (R,)), row_div,
         _dense(offsets, "offsets", _i32, (E + 1,)), _dense(counts, "counts", _i32, (E,)),
-        _rows(b, "b", _f8, (E, N, K)), _ld16(b, N, K, 1), b.stride(0), _rows(sb, "sb", _f32, (E, -(-N // 128), kb)),
-        _ld(sb, -(-N // 128), kb, 1), sb.stride(0), at, dt, _ld(c, R, N), None if err is None else err.data_ptr(), _here(a))
+        *_stack(b, "b", _f8, E, N, K), *_stack(sb, "sb", _f32, E, -(-N // 128), kb), at, dt, ld,
+        None if err is None else err.data_ptr(), _here(a))
     if rc:
         _check(rc, "nsb_op_moe_gemm_fp8")
 
@@ -425,11 +429,13 @@ def moe_wgrad_fp8(a, sa, b, sb, offsets, counts, c, err=None):
     N = b.shape[0]
     E = c.shape[0]
     rb = -(-R // 128)
-    at, dt = _float(c, "c", (E, M, N))
+    if c.dtype is not _f32 and c.dtype is not _bf16:
+        raise ValueError(f"c: {c.dtype} where float32 or bfloat16 is wanted")
+    at, ld, apart = _stack(c, "c", c.dtype, E, M, N)
     rc = lib.nsb_op_moe_wgrad_fp8(
-        M, N, R, E, _rows(a, "a", _f8, (M, R)), _ld16(a, M, R), _rows(sa, "sa", _f32, (rb, M)), _ld(sa, rb, M),
-        _rows(b, "b", _f8, (N, R)), _ld16(b, N, R), _rows(sb, "sb", _f32, (rb, N)), _ld(sb, rb, N),
-        _dense(offsets, "offsets", _i32, (E + 1,)), _dense(counts, "counts", _i32, (E,)), at, dt, _ld(c, M, N, 1),
-        c.stride(0), None if err is None else err.data_ptr(), _here(a))
+        M, N, R, E, *_codes(a, "a", M, R), *_rows(sa, "sa", _f32, rb, M), *_codes(b, "b", N, R),
+        *_rows(sb, "sb", _f32, rb, N), _dense(offsets, "offsets", _i32, (E + 1,)),
+        _dense(counts, "counts", _i32, (E,)), at, F32 if c.dtype is _f32 else BF16, ld, apart,
+        None if err is None else err.data_ptr(), _here(a))
     if rc:
         _check(rc, "nsb_op_moe_wgrad_fp8")
