@@ -96,6 +96,9 @@ struct TileCfg {
     static constexpr int TABLE = ROWS ? (2 * kMaxGroups + 1) * 4 : 0;
     static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + SCALES + 512 + TABLE;
     static_assert(SMEM <= 227 * 1024, "above the shared memory of a block");
+    // (a wait on parity is only good for a phase whose predecessor the waiter
+    // has seen complete, so an issuer must come by at every phase of a barrier)
+    static_assert(STAGES % 2 == 0 && PARTS % 2 == 0, "a stage and a part always meet the same one of two issuers");
 };
 
 // Waits of the pipeline. A wait that runs out of time records the error and
@@ -729,13 +732,14 @@ template <int BN, bool VEC>
 struct SmallCfg {
     static constexpr int W_BYTES = 128 * 128;
     static constexpr int STAGE = W_BYTES + BN * 128;
-    static constexpr int STAGES = BN == 64 ? 8 : (BN == 32 ? 9 : 10);
+    static constexpr int STAGES = BN == 16 ? 10 : 8;
     static constexpr int PARTS = 8;
     static constexpr int SLOTK = 4;
     static constexpr int SLOT = BN + (VEC ? 128 : 4);  // scales of A's rows, then of B's rows or block
     static constexpr int SCALES = kSlots * SLOTK * SLOT * 4;
     static constexpr int SMEM = 1024 + STAGES * STAGE + SCALES + 512 + (2 * kMaxGroups + 1) * 4;
     static_assert(SMEM <= 227 * 1024, "above the shared memory of a block");
+    static_assert(STAGES % 2 == 0 && PARTS % 2 == 0, "a stage and a part always meet the same one of two issuers");
     static_assert(BN * 128 * 4 <= STAGES * STAGE, "the cluster's sums take the ring's place");
 };
 
