@@ -732,13 +732,18 @@ template <int BN, bool VEC>
 struct SmallCfg {
     static constexpr int W_BYTES = 128 * 128;
     static constexpr int STAGE = W_BYTES + BN * 128;
-    static constexpr int STAGES = BN == 16 ? 10 : 8;
+    // two CTAs an SM, whose copies and sums hide one another, as long as their
+    // accumulators fit (64 columns: 213 registers; at 112 they spill, 53 -> 83 us
+    // for 64 groups of 38 rows)
+    static constexpr int CTAS = BN == 64 ? 1 : 2;
+    static constexpr int STAGES = 8 / CTAS;
     static constexpr int PARTS = 8;
     static constexpr int SLOTK = 4;
     static constexpr int SLOT = BN + (VEC ? 128 : 4);  // scales of A's rows, then of B's rows or block
     static constexpr int SCALES = kSlots * SLOTK * SLOT * 4;
     static constexpr int SMEM = 1024 + STAGES * STAGE + SCALES + 512 + (2 * kMaxGroups + 1) * 4;
-    static_assert(SMEM <= 227 * 1024, "above the shared memory of a block");
+    static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "above the shared memory of an SM");
+    static_assert(CTAS * PARTS * BN <= 512, "above the columns of TMEM");
     static_assert(STAGES % 2 == 0 && PARTS % 2 == 0, "a stage and a part always meet the same one of two issuers");
     static_assert(BN * 128 * 4 <= STAGES * STAGE, "the cluster's sums take the ring's place");
 };
@@ -781,7 +786,7 @@ __device__ __forceinline__ Unit small_unit(const TileParams& p, const int* start
 }
 
 template <int BN, bool VEC>
-__global__ void __launch_bounds__(kSmallThreads, 1)
+__global__ void __launch_bounds__(kSmallThreads, SmallCfg<BN, VEC>::CTAS)
     fp8_small_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ SmallParams sp) {
     using C = SmallCfg<BN, VEC>;
     const TileParams& p = sp.t;
@@ -1184,7 +1189,7 @@ int launch_small(const Fp8Gemm& d, cudaStream_t st) {
     const long long rows = d.groups ? (long long)d.M / BN + (d.M < d.groups ? d.M : d.groups) : sp.t.m_tiles;
     const long long units = rows * sp.t.n_tiles;
     if (units > 0x7fffffff) return -2;
-    const int sms = num_sms(), kblocks = (d.K + 127) / 128;
+    const int sms = num_sms() * C::CTAS, kblocks = (d.K + 127) / 128;
     sp.split = 1;
     if (!d.groups)
         while (sp.split < 8 && units * sp.split * 2 <= sms && kblocks >= sp.split * 4) sp.split *= 2;
