@@ -732,11 +732,8 @@ template <int BN, bool VEC>
 struct SmallCfg {
     static constexpr int W_BYTES = 128 * 128;
     static constexpr int STAGE = W_BYTES + BN * 128;
-    // two CTAs an SM, whose copies and sums hide one another, as long as their
-    // accumulators fit (64 columns: 213 registers; at 112 they spill, 53 -> 83 us
-    // for 64 groups of 38 rows)
-    static constexpr int CTAS = BN == 64 ? 1 : 2;
-    static constexpr int STAGES = 8 / CTAS;
+    static constexpr int CTAS = 2;  // an SM: the copies and sums of one hide the other's
+    static constexpr int STAGES = 4;
     static constexpr int PARTS = 8;
     static constexpr int SLOTK = 4;
     static constexpr int SLOT = BN + (VEC ? 128 : 4);  // scales of A's rows, then of B's rows or block
@@ -1282,13 +1279,12 @@ int fp8_gemm(const Fp8Gemm& d, cudaStream_t st) {
     const int sms = num_sms();
     const int rows = d.groups && !d.group_k ? (d.M + d.groups - 1) / d.groups : d.M;
     // Few rows: the weights' stream bounds the product. (One product of 4096 x
-    // 4096: 16 rows 8.4 us here and 9.7 on tiles, 33 rows 11.4 and 9.7; 64
-    // groups of 1024 x 2048 with 38 rows on average 53 us and 92, with 62
-    // rows 65 and 77.)
-    if (!d.groups && rows <= 16) return d.b_rows ? launch_small<16, true>(d, st) : launch_small<16, false>(d, st);
-    if (d.groups && !d.group_k && rows <= 64) {
-        if (rows <= 16) return launch_small<16, false>(d, st);
-        return rows <= 32 ? launch_small<32, false>(d, st) : launch_small<64, false>(d, st);
+    // 4096: 16 rows 8.3 us here and 9.7 on tiles, 24 rows 9.4 and 10.5, 48 rows
+    // 11.1 and 10.1; groups of 1024 x 2048 with 38 rows on average 40 us and 92,
+    // with 100 rows 75 and 110, of 1024 x 1024 with 112 rows 19.8 and 22.3.)
+    if (!d.group_k && rows <= (d.groups ? 128 : 32)) {
+        if (rows <= 16) return d.b_rows ? launch_small<16, true>(d, st) : launch_small<16, false>(d, st);
+        return d.b_rows ? launch_small<32, true>(d, st) : launch_small<32, false>(d, st);
     }
     // The tile's width with the least rounds x time of a k-block, which goes
     // about as width + 64.
