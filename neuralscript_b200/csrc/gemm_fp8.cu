@@ -161,7 +161,7 @@ __device__ __forceinline__ Unit unit_at(const TileParams& p, const int* start, i
     w.kb0 = 0;
     w.kb1 = (p.K + 127) / 128;
     if (p.groups) {
-        const int off = p.offsets[w.g];
+        const int off = max(0, p.offsets[w.g]);
         w.kb0 = off / 128;
         w.kb1 = min(w.kb1, (off + p.counts[w.g] + 127) / 128);
     }
@@ -176,7 +176,7 @@ __device__ __forceinline__ void group_starts(const TileParams& p, int rows, int*
         const int g = g0 + lane;
         int n = 0;
         if (g < p.groups) {
-            const int off = p.offsets[g], end = max(off, min(p.M, off + p.counts[g]));
+            const int off = max(0, p.offsets[g]), end = max(off, min(p.M, off + p.counts[g]));
             start[kMaxGroups + 1 + g] = off;
             n = (end - off + rows - 1) / rows;
         }
@@ -719,8 +719,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 // the stream of the weights, so everything serves loads in flight: a deep
 // ring, eight parts of TMEM, and for one product the k-blocks of a tile split
 // over a cluster of CTAs, whose sums meet in shared memory in rank order.
-// 1 x 4096 x 4096: 7.9 us (2.6 us of HBM time, the rest latency); 24 tokens x 4
-// of 64 experts, 2048 x 1024: 28 us (3.8 TB/s, 5 to 7 tiles an SM).
+// 1 x 4096 x 4096: 7.5 us (2.6 us of HBM time, the rest latency); 24 tokens x 4
+// of 64 experts, 2048 x 1024: 22.3 us (4.8 TB/s, 5 to 7 tiles an SM; 28 us with
+// one CTA an SM).
 //   warp 0       weights by TMA
 //   warps 1, 8   MMA issuers, every other k-block each
 //   warps 2..3   rows of A by cp.async (listed, or in order) and the scales
