@@ -752,10 +752,8 @@ struct SmallParams {
 };
 
 __device__ __forceinline__ float cluster_loadf(const float* p, unsigned rank) {
-    uint32_t at;
     float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(ptx::smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ptx::cluster_addr(p, rank)) : "memory");
     return v;
 }
 

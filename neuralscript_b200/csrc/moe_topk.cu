@@ -8,6 +8,7 @@
 
 #include "gemm.h"
 #include "moe_topk.h"
+#include "ptx.cuh"
 
 namespace nsb {
 
@@ -353,22 +354,10 @@ constexpr int kOrderThreads = 1024;
 constexpr int kOrderWarps = kOrderThreads / 32;
 constexpr int kOrderAhead = 8;
 
-__device__ __forceinline__ unsigned cluster_rank() {
-    unsigned r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
 // the same word of the shared memory of CTA `rank` of the cluster
 __device__ __forceinline__ int cluster_load(const int* p, unsigned rank) {
-    uint32_t at;
     int v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
-                 : "=r"(at)
-                 : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(ptx::cluster_addr(p, rank)) : "memory");
     return v;
 }
 
@@ -403,7 +392,7 @@ __global__ void __launch_bounds__(kOrderThreads)
     int* base = start + E + 1;          // [E] this block's first row of it
     int* sums = base + E;               // [kOrderWarps] scan over experts
     int* ends = sums + kOrderWarps;     // [E] row behind an expert's last pair
-    const unsigned rank = CTAS > 1 ? cluster_rank() : 0;
+    const unsigned rank = CTAS > 1 ? ptx::cluster_ctarank() : 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int i = threadIdx.x; i < kOrderWarps * E; i += kOrderThreads) sh[i] = 0;
     __syncthreads();
@@ -440,7 +429,7 @@ __global__ void __launch_bounds__(kOrderThreads)
         }
         total[e] = run;
     }
-    if (CTAS > 1) cluster_sync();
+    if (CTAS > 1) ptx::cluster_sync();
     else __syncthreads();
     // E <= 1024 threads: thread e sums expert e over the blocks, then the
     // padded counts are scanned over the experts
@@ -509,7 +498,7 @@ __global__ void __launch_bounds__(kOrderThreads)
             if (at >= 0) rows[at] = (int)pair;
         }
     }
-    if (CTAS > 1) cluster_sync();  // no block leaves while others read its counts
+    if (CTAS > 1) ptx::cluster_sync();  // no block leaves while others read its counts
 }
 
 // ---------------------------------------------------------------------------

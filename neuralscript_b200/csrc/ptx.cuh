@@ -165,10 +165,6 @@ __device__ __forceinline__ void mbar_arrive_cluster_if(uint32_t bar, bool on) {
         "r"((uint32_t)on)
         : "memory");
 }
-// The same, releasing what this thread has seen and written to the cluster.
-__device__ __forceinline__ void mbar_arrive_release(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
 // Loads into this CTA's shared memory that complete on a barrier of either CTA.
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
     asm volatile(
