@@ -545,7 +545,51 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             if constexpr (VEC) {
-                // a row's 8 columns of four threads are one 32-byte (fp32) piece
+                if (p.tma_out) {
+                    const int y = w.m0 + quarter * 32;
+                    // 64 bytes of this warp's 32 rows, written into its staging buffer by
+                    // `fill`, leave by TMA (which clips at the tensor's end)
+                    auto leave = [&](int x, int z, auto fill) {
+                        if (lane == 0) ptx::bulk_wait_read0();
+                        __syncwarp();
+                        fill();
+                        ptx::fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            ptx::tma_store_3d(&tc, stg, x, y, z);
+                            ptx::bulk_commit();
+                        }
+                    };
+                    // (staging's 16-byte piece q of row r lies at q ^ (r / 2 % 4))
+                    const int es = p.c_dtype == kBF16 ? 2 : 4;
+#pragma unroll
+                    for (int c = 0; c < C::COLS / 32; c++)
+#pragma unroll
+                        for (int b = 0; b < 2; b++) {
+                            const int x = col0 + c * 32 + b * 16;
+                            if ((es == 2 && b) || x >= p.N || y >= p.M) continue;
+                            leave(x, w.g, [&] {
+#pragma unroll
+                                for (int h = 0; h < 2; h++)
+#pragma unroll
+                                    for (int j = 0; j < 8; j++) {
+                                        const int r = h * 16 + (j & 1) * 8 + (lane >> 2);
+                                        const float* o = acc + ((c * 2 + h) * 8 + j) * 2;
+                                        if (es == 2) {  // columns 8 (j / 2) + 2 (lane % 4)
+                                            *reinterpret_cast<__nv_bfloat162*>(
+                                                stg + r * 64 + (((j >> 1) ^ (r >> 1 & 3)) << 4) + (lane & 3) * 4) =
+                                                __floats2bfloat162_rn(o[0], o[1]);
+                                        } else if (j >> 2 == b) {  // 8 (j / 2 % 2) + 2 (lane % 4)
+                                            const int q = (j >> 1 & 1) * 2 + ((lane & 3) >> 1);
+                                            *reinterpret_cast<float2*>(stg + r * 64 + ((q ^ (r >> 1 & 3)) << 4) +
+                                                                       (lane & 1) * 8) = make_float2(o[0], o[1]);
+                                        }
+                                    }
+                            });
+                        }
+                    continue;
+                }
+                // row by row, two columns a thread
                 const size_t base = (size_t)w.g * p.c_stride;
 #pragma unroll
                 for (int c = 0; c < C::COLS / 32; c++)
@@ -556,24 +600,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const int m = w.m0 + quarter * 32 + h * 16 + (j & 1) * 8 + (lane >> 2);
                             const int n = col0 + c * 32 + (j >> 1) * 8 + (lane & 3) * 2;
                             const float* o = acc + ((c * 2 + h) * 8 + j) * 2;
-                            if (m >= w.row_end || n >= p.N) continue;
-                            const size_t at = base + (size_t)m * p.ldc + n;
-                            if (p.c_dtype == kBF16) {
-                                __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.c) + at;
-                                if (p.vec_out && n + 1 < p.N) {
-                                    *reinterpret_cast<__nv_bfloat162*>(dst) = __floats2bfloat162_rn(o[0], o[1]);
-                                } else {
-                                    dst[0] = f2bf(o[0]);
-                                    if (n + 1 < p.N) dst[1] = f2bf(o[1]);
-                                }
-                            } else {
-                                float* dst = reinterpret_cast<float*>(p.c) + at;
-                                if (p.vec_out && n + 1 < p.N) {
-                                    *reinterpret_cast<float2*>(dst) = make_float2(o[0], o[1]);
-                                } else {
-                                    dst[0] = o[0];
-                                    if (n + 1 < p.N) dst[1] = o[1];
-                                }
+                            if (m >= w.row_end) continue;
+#pragma unroll
+                            for (int i = 0; i < 2; i++) {
+                                if (n + i >= p.N) continue;
+                                const size_t at = base + (size_t)m * p.ldc + n + i;
+                                if (p.c_dtype == kBF16) reinterpret_cast<__nv_bfloat16*>(p.c)[at] = f2bf(o[i]);
+                                else reinterpret_cast<float*>(p.c)[at] = o[i];
                             }
                         }
                 continue;
@@ -1218,7 +1251,7 @@ int launch_tiles(const Fp8Gemm& d, cudaStream_t st) {
     if (!map_codes2(&ta, d.a, d.K, d.a_rows, d.lda, 128)) return -2;
     if (!map_codes3(&tb, d.b, d.K, d.N, d.ldb, ROWS ? d.groups : 1, d.b_stride, C::BROWS)) return -2;
     // a TMA store clips rows to whole 16-byte pieces, so ragged ones go another way
-    p.tma_out = !VEC && aligned && (long long)d.N * es % 16 == 0 &&
+    p.tma_out = aligned && (long long)d.N * es % 16 == 0 &&
                 map_out(&tc, d.c, d.c_dtype, d.N, d.M, d.ldc, d.group_k ? d.groups : 1, d.c_stride);
     long long units = (long long)p.m_tiles * p.n_tiles;
     if (ROWS) units = ((long long)p.m_tiles + d.groups) * p.n_tiles;  // at most
