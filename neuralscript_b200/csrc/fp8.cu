@@ -40,6 +40,14 @@ __device__ __forceinline__ uint32_t code4(float a, float b, float c, float d) {
     return lo | hi << 16;
 }
 
+// the same of four values times k, two at a time
+__device__ __forceinline__ uint32_t code4(float a, float b, float c, float d, float k) {
+    const uint64_t kk = f2_pack(k, k);
+    f2_unpack(f2_mul(f2_pack(a, b), kk), a, b);
+    f2_unpack(f2_mul(f2_pack(c, d), kk), c, d);
+    return code4(a, b, c, d);
+}
+
 __device__ __forceinline__ void store8(uint8_t* dst, uint2 v, int n) {
     if (n >= 8) {
         *reinterpret_cast<uint2*>(dst) = v;
@@ -223,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 2) quantize_kernel(const QuantDesc d
                 for (int i = 0; i < 4; i++) {
                     float m = 0.f;
 #pragma unroll
-                    for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(v[i][j]));
+                    for (int j = 0; j < 8; j += 2) m = max3(m, fabsf(v[i][j]), fabsf(v[i][j + 1]));
 #pragma unroll
                     for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
                     if (cl == i) mine = m;
@@ -235,17 +243,16 @@ __global__ void __launch_bounds__(kThreads, 2) quantize_kernel(const QuantDesc d
                     const float k = __shfl_sync(kAll, inverse, (lane & 16) + i);
                     if (r0 + i < d.M)
                         store8(d.q + (size_t)(r0 + i) * d.ld_q + c0,
-                               make_uint2(code4(v[i][0] * k, v[i][1] * k, v[i][2] * k, v[i][3] * k),
-                                          code4(v[i][4] * k, v[i][5] * k, v[i][6] * k, v[i][7] * k)),
+                               make_uint2(code4(v[i][0], v[i][1], v[i][2], v[i][3], k),
+                                          code4(v[i][4], v[i][5], v[i][6], v[i][7], k)),
                                d.K - c0);
                 }
             }
             if (!d.qt) continue;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                float m = 0.f;
-#pragma unroll
-                for (int i = 0; i < 4; i++) m = fmaxf(m, fabsf(v[i][j]));
+                float m = max3(0.f, fabsf(v[0][j]), fabsf(v[1][j]));
+                m = max3(m, fabsf(v[2][j]), fabsf(v[3][j]));
                 m = fmaxf(m, __shfl_xor_sync(kAll, m, 16));
                 if (lane < 16) part[warp][j * 16 + cl] = m;  // column cl * 8 + j
             }
@@ -264,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 2) quantize_kernel(const QuantDesc d
             for (int j = 0; j < 8; j++) {
                 const float k = inv[j * 16 + cl];
                 tile[(cl * 8 + j) * 32 + (half ^ (cl * 2))] =
-                    code4(v[0][j] * k, v[1][j] * k, v[2][j] * k, v[3][j] * k);
+                    code4(v[0][j], v[1][j], v[2][j], v[3][j], k);
             }
         }
         __syncthreads();
