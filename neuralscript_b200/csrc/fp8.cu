@@ -292,9 +292,8 @@ int quantize(const QuantDesc& d, cudaStream_t st) {
     const bool f = d.dtype == kF32;
     if (d.M < 0 || d.K <= 0 || (!f && d.dtype != kBF16) || d.ld < d.K || d.act < 0 || d.act > kGeluMoe) return -1;
     if (d.rows && d.row_div < 0) return -1;
-    if (!d.q && !d.qt) return -1;
-    if (d.M == 0) return 0;
-    if (!d.x) return -1;
+    if (d.M == 0) return 0;  // (what has no elements has no address)
+    if (!d.x || (!d.q && !d.qt)) return -1;
     auto codes = [](const void* p, long long ld, int cols) {
         return !(reinterpret_cast<uintptr_t>(p) & 15) && ld % 16 == 0 && ld >= cols;
     };

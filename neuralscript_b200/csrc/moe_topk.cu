@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(128)
 
 bool route_ok(const RouteDesc& d) {
     if (d.M < 0 || d.E <= 0 || d.E > kTopkMaxE || d.k <= 0 || d.k > kTopkMaxK || d.k > d.E) return false;
-    if (!d.logits || d.ld < d.E || (d.dtype != kF32 && d.dtype != kBF16)) return false;
+    if ((d.M && !d.logits) || d.ld < d.E || (d.dtype != kF32 && d.dtype != kBF16)) return false;
     if (d.groups < 1 || d.E % d.groups || d.topk_groups < 1 || d.topk_groups > d.groups) return false;
     return d.groups == 1 || d.E / d.groups >= 2;
 }
@@ -676,8 +676,9 @@ bool experts16(const RouteDesc& d) {
 }  // namespace
 
 int moe_topk_route(const RouteDesc& d0, int* idx, float* w, cudaStream_t st) {
-    if (!route_ok(d0) || !idx || !w) return -1;
+    if (!route_ok(d0)) return -1;
     if (d0.M == 0) return 0;
+    if (!idx || !w) return -1;
     RouteDesc d = d0;
     by_lane(d.E, [&](auto n) {
         constexpr int NV = decltype(n)::value;
@@ -692,8 +693,9 @@ int moe_topk_route(const RouteDesc& d0, int* idx, float* w, cudaStream_t st) {
 
 int moe_topk_route_bwd(const RouteDesc& d0, const float* dw, const int* idx, void* dl, long long ld_d,
                        cudaStream_t st) {
-    if (!route_ok(d0) || !idx || !dw || !dl || ld_d < d0.E) return -1;
+    if (!route_ok(d0) || ld_d < d0.E) return -1;
     if (d0.M == 0) return 0;
+    if (!idx || !dw || !dl) return -1;
     RouteDesc d = d0;
     by_lane(d.E, [&](auto n) {
         constexpr int NV = decltype(n)::value;

@@ -341,3 +341,28 @@ def test_refusals():
         ops.moe_combine(torch.zeros(8, 4, device=DEV), idx, torch.zeros(4, 4, device=DEV, dtype=torch.bfloat16), w=w)
     with pytest.raises(ValueError):
         ops.moe_combine_bwd(torch.zeros(4, 4, device=DEV), None, idx.view(-1), idx, w, torch.zeros(8, 4, device=DEV), w)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_no_tokens(dtype):
+    """Every operator of the path takes a batch of no tokens."""
+    f8, i32 = torch.float8_e4m3fn, dict(dtype=torch.int32, device=DEV)
+    x, logits = torch.empty(0, 64, dtype=dtype, device=DEV), torch.empty(0, 16, dtype=dtype, device=DEV)
+    idx, w, dw = torch.empty(0, 2, **i32), torch.empty(0, 2, device=DEV), torch.empty(0, 2, device=DEV)
+    ops.moe_topk_route(logits, idx, w)
+    ops.moe_topk_route_bwd(dw, logits, idx, torch.empty_like(logits))
+    offsets, counts = torch.full((17,), -7, **i32), torch.full((16,), -7, **i32)
+    rows, pos = torch.empty(0, **i32), torch.empty(0, 2, **i32)
+    ops.moe_dispatch(idx, 16, offsets, counts, rows, pos, align=128)
+    assert (offsets == 0).all() and (counts == 0).all()
+    q, s = torch.empty(0, 64, dtype=f8, device=DEV), torch.empty(1, 0, device=DEV)
+    qt, st = torch.empty(64, 0, dtype=f8, device=DEV), torch.empty(0, 64, device=DEV)
+    ops.fp8_quantize(x, q, s, qt, st)
+    ops.fp8_quantize(x, qt=qt, st=st, rows=rows, row_div=2)
+    ops.fp8_quantize_block(x, q, torch.empty(0, 1, device=DEV), qt, torch.empty(1, 0, device=DEV))
+    c = torch.empty(0, 32, dtype=dtype, device=DEV)
+    ops.gemm_fp8(q, s, torch.zeros(32, 64, device=DEV).to(f8), torch.ones(1, 1, device=DEV), c)
+    y = torch.empty(0, 32, dtype=dtype, device=DEV)
+    ops.moe_combine(c, pos, y, w)
+    ops.moe_combine_bwd(y, c, rows, pos, w, torch.empty_like(c), dw)
+    torch.cuda.synchronize()

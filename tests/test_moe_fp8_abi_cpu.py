@@ -122,3 +122,13 @@ def test_products_refuse():
 def test_products_of_nothing():
     assert rc("nsb_op_gemm_fp8", 0, 200, 300, X, 304, X, 4, X, 304, X, 3, 0, X, 0, 200, None) == 0
     assert rc("nsb_op_gemm_fp8", 4, 0, 300, X, 304, X, 4, X, 304, X, 3, 0, X, 0, 200, None) == 0
+
+
+def test_nothing_has_no_address():
+    """A tensor without elements has the address 0: no refusal."""
+    assert route(M=0, logits=None, idx=None, w=None) == 0
+    assert rc("nsb_op_moe_topk_route_bwd", None, None, 0, 16, 0, 16, 2, 0, None, 1, 1.0, None, None, 16) == 0
+    assert rc("nsb_op_moe_combine", None, 0, 64, None, None, 0, 2, 64, None, 64) == 0
+    assert rc("nsb_op_moe_combine_bwd", None, None, 0, 64, 64, None, None, None, 0, 2, 0, 64, None, 64, None) == 0
+    assert rc("nsb_op_fp8_quantize", None, 0, 64, 0, 64, 0, None, 1, None, 64, None, 0, None, 0, None, 64) == 0
+    assert rc("nsb_op_fp8_quantize_block", None, 0, 64, 0, 64, None, 64, None, 1, None, 0, None, 0) == 0
