@@ -303,6 +303,7 @@ int quantize(const QuantDesc& d, cudaStream_t st) {
     if ((long long)rb * cb > 0x7fffffff) return -2;
     const int tiles = rb * cb, most = 2 * num_sms(), grid = tiles < most ? tiles : most;
     const bool vec = !(reinterpret_cast<uintptr_t>(d.x) & 15) && d.ld * (f ? 4 : 2) % 16 == 0;
+    bool ok = true;
     auto go = [&](auto act) {
         constexpr int ACT = decltype(act)::value;
         if (f && vec) {
@@ -316,7 +317,10 @@ int quantize(const QuantDesc& d, cudaStream_t st) {
             constexpr int smem = 8 * kThreads * (int)sizeof(uint4);
             static bool done[kMaxDevices] = {};  // the attribute belongs to the current device
             int dev = 0;
-            if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return;
+            if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) {
+                ok = false;
+                return;
+            }
             if (!done[dev])
                 done[dev] = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess;
             k<<<grid, kThreads, smem, st>>>(d, cb, tiles);
@@ -336,7 +340,7 @@ int quantize(const QuantDesc& d, cudaStream_t st) {
             default: go(std::integral_constant<int, kIdentity>());
         }
     }
-    return cudaGetLastError() == cudaSuccess ? 0 : -5;
+    return cudaGetLastError() == cudaSuccess && ok ? 0 : -5;
 }
 
 }  // namespace
