@@ -69,6 +69,13 @@ __device__ __forceinline__ float rcp_approx(float x) {
     return y;
 }
 
+// the smaller one, NaN where either is
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
 // x Phi(x) without erff's branches: Phi(-a) = erfc(z) / 2 for z = a / sqrt(2),
 // erfc(z) = exp(-z^2) erfcx(z), and erfcx(z) = t P(t) with t = 1 / (1 + 0.38 z)
 // and a polynomial of degree 6 fitted for this code (Lawson-weighted least
@@ -76,8 +83,10 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // negative side, where 1 + erf would cancel).
 // Two values at a time on packed fp32 pairs, which halves the FMA
 // instructions that bound this pass.
+// a stops at 20, where Phi(-a) is long 0 in fp32, so that +inf meets no
+// inf * 0 and stays +inf; -inf gives NaN as it does in x Phi(x), and NaN NaN.
 __device__ __forceinline__ void gelu_tail2(float& x0, float& x1) {
-    const uint64_t a = f2_pack(fabsf(x0), fabsf(x1));
+    const uint64_t a = f2_pack(fabsf(min_nan(x0, 20.f)), fabsf(min_nan(x1, 20.f)));
     const uint64_t z = f2_mul(a, f2_pack(0.70710678f, 0.70710678f));
     float d0, d1, e0, e1;
     f2_unpack(f2_fma(z, f2_pack(0.38f, 0.38f), f2_pack(1.f, 1.f)), d0, d1);

@@ -110,6 +110,64 @@ def test_quantize_behind_an_activation(act):
         assert torch.all((v.double() * wide - ref).abs() <= step * (1 + 1e-5) + 1e-6 * ref.abs())
 
 
+def activated(x, act):
+    """The activations in 64 bits, as the fp32 ones treat infinities and NaN."""
+    x = x.double()
+    if act == 1:
+        return torch.where(x > 0, x, 0)
+    if act == 2:
+        return torch.where(x > 0, x, 0.01 * x)
+    if act == 3:
+        return 1 / (1 + torch.exp(-x))
+    if act == 4:
+        return torch.tanh(x)
+    if act == 5:
+        return x / (1 + torch.exp(-x))
+    return 0.5 * x * (1 + torch.erf(x / math.sqrt(2))) if act else x
+
+
+def read_back_ok(q, s, z):
+    """Codes and scales (of 128 along a row) of z: an infinity turns its block to NaN, a NaN only itself, all else is
+    within half a step of e4m3 and 1e-5 (above what the fp32 activations are off by) of its value."""
+    R, K = z.shape
+    wide = s.t().double().repeat_interleave(128, 1)[:, :K]
+    v = q.double() * wide
+    blocks = torch.nn.functional.pad(z, (0, up(K, 128) - K)).view(R, -1, 128)
+    lost = blocks.isinf().any(2).repeat_interleave(128, 1)[:, :K] | z.isnan()
+    ok = torch.where(lost, v.isnan(), (v - z).abs() <= torch.maximum(z.abs() * 2.0 ** -4, wide * 2.0 ** -10) + 1e-5 * z.abs())
+    return ok.all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("act", range(8))
+def test_quantize_infinities_and_nan_behind_activations(act, dtype):
+    M, K = 300, 270
+    x = torch.randn(M, K, device=DEV, generator=gen(act)).to(dtype)
+    for i, bad in enumerate((math.inf, -math.inf, math.nan)):
+        x[3 + i, 5 + i] = x[140 + i, 100 + 40 * i] = x[299 - i, 269 - i] = bad
+    x[200, 200], x[210, 210] = torch.finfo(dtype).max, -torch.finfo(dtype).max
+    for a in (x, torch.cat([x, x], 1)[:, 1:K + 1]):  # on 16-byte boundaries and off them
+        z = activated(a, act)
+        q, s, qt, st = codes(M, K), scales(up(K, 128) // 128, M), codes(K, M), scales(up(M, 128) // 128, K)
+        ops.fp8_quantize(a, q, s, qt, st, act=act)
+        assert read_back_ok(q, s, z) and read_back_ok(qt, st, z.t())
+
+
+def test_quantize_block_infinities_and_nan():
+    x = torch.randn(300, 400, device=DEV, generator=gen(1))
+    x[130, 7], x[5, 300], x[299, 399], x[0, 0] = math.inf, -math.inf, math.nan, math.nan
+    q, s, qt, st = codes(300, 400), scales(3, 4), codes(400, 300), scales(4, 3)
+    ops.fp8_quantize_block(x, q, s, qt, st)
+    wide = s.double().repeat_interleave(128, 0)[:300].repeat_interleave(128, 1)[:, :400]
+    v = q.double() * wide
+    lost = x.isnan()
+    lost[128:256, :128] = True
+    lost[:128, 256:384] = True
+    near = (v - x.double()).abs() <= torch.maximum(x.double().abs() * 2.0 ** -4, wide * 2.0 ** -10) * (1 + 1e-6)
+    assert torch.where(lost, v.isnan(), near).all()
+    assert same(qt, q.t()) and torch.equal(st, s.t())
+
+
 def test_quantize_gathered_rows():
     x = torch.randn(50, 90, device=DEV, generator=gen(3)).to(torch.bfloat16)
     rows = torch.randint(-1, 150, (300,), device=DEV, generator=gen(4), dtype=torch.int32)
