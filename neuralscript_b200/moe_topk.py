@@ -89,11 +89,14 @@ class MoETopk:
         o = self._product(hq, hs, order, self.q2, D)
         y = _floats(M, D)
         ops.moe_combine(o, order["pos"], y, w=w)
-        return y, dict(x=x, logits=logits, idx=idx, w=w, order=order, z=z, o=o)
+        return y, dict(x=x, logits=logits, idx=idx, w=w, order=order, z=z, o=o, align=align)
 
     def backward(self, dy, kept):
         """Gradients (dx [M, D], dgate, dw1, dw2) of the loss whose gradient in y is dy [M, D] (fp32); the forward
-        pass ran with align=128."""
+        pass ran with align=128 (the weight gradients sum whole blocks of 128 rows: without padding a block holds
+        rows of two experts)."""
+        if kept["align"] % 128:
+            raise ValueError(f"backward after a forward pass with align={kept['align']}, which is no multiple of 128")
         x, order, k, E, D, H = kept["x"], kept["order"], self.k, self.E, self.D, self.H
         rows, M = order["rows"], x.shape[0]
         R = rows.numel()

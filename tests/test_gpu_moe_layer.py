@@ -66,3 +66,13 @@ def test_layer_trains_and_serves_single_tokens():
     y, _ = layer.forward(x)
     one, _ = layer.forward(x[17:18])
     assert off(one[0], y[17].double()) < 1e-5
+
+
+@pytest.mark.parametrize("align", [1, 64])
+def test_backward_refuses_unaligned_segments(align):
+    """64 tokens, 2 experts each: 128 pairs, so that every buffer's shape fits and only the sums would be wrong."""
+    layer = MoETopk(128, 128, 4, 2, seed=3)
+    x = torch.randn(64, 128, device="cuda").to(torch.bfloat16)
+    y, kept = layer.forward(x, align=align)
+    with pytest.raises(ValueError, match="align"):
+        layer.backward(torch.ones_like(y), kept)
