@@ -79,8 +79,11 @@ __device__ __forceinline__ float min_nan(float a, float b) {
 // x Phi(x) without erff's branches: Phi(-a) = erfc(z) / 2 for z = a / sqrt(2),
 // erfc(z) = exp(-z^2) erfcx(z), and erfcx(z) = t P(t) with t = 1 / (1 + 0.38 z)
 // and a polynomial of degree 6 fitted for this code (Lawson-weighted least
-// squares over z in [0, 10]; relative error below 1.4e-6, also far out on the
-// negative side, where 1 + erf would cancel).
+// squares over z in [0, 10]), so that nothing cancels on the negative side.
+// Largest relative error, measured against 64 bits: 1.5e-6 for |x| up to 1,
+// 2.1e-6 down to -4, 6.5e-6 to -8, 1.9e-5 to -13: the polynomial's 1.4e-6, and
+// z^2 log2(e), whose roundings the exponential multiplies by z^2. Below about
+// -13.2 the result is 0, as its code is: 2^-100 is a block's smallest scale.
 // Two values at a time on packed fp32 pairs, which halves the FMA
 // instructions that bound this pass.
 // a stops at 20, where Phi(-a) is long 0 in fp32, so that +inf meets no

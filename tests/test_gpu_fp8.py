@@ -153,6 +153,21 @@ def test_quantize_infinities_and_nan_behind_activations(act, dtype):
         assert read_back_ok(q, s, z) and read_back_ok(qt, st, z.t())
 
 
+def test_quantize_behind_gelu_far_out():
+    """Blocks of one value, so that the scale tells GELU's own error. Roundings of x^2 / 2 log2(e) (constants and
+    operations: seven halves of an ulp) are multiplied by x^2 / 2; the rest is below 3e-6."""
+    x = torch.cat([torch.linspace(-13, -1e-3, 4000), torch.linspace(1e-3, 30, 1000)]).to(DEV)[:, None]
+    q, s = codes(5000, 1), scales(1, 5000)
+    ops.fp8_quantize(x, q, s, act=6)
+    z = 0.5 * x.double() * torch.special.erfc(-x.double() / math.sqrt(2))
+    want = torch.clamp(z.abs() / 448, min=2.0 ** -100)[:, 0]
+    assert ((s[0].double() - want).abs() <= want * (x[:, 0].double() ** 2 / 2 * 7 * EPS + 3e-6)).all()
+    far = torch.tensor([[-13.3], [-20.0], [-1e10], [-torch.finfo(torch.float32).max]], device=DEV)
+    q, s = codes(4, 1), scales(1, 4)
+    ops.fp8_quantize(far, q, s, act=6)
+    assert (q.float() == 0).all() and (s == 2.0 ** -100).all()
+
+
 def test_quantize_block_infinities_and_nan():
     x = torch.randn(300, 400, device=DEV, generator=gen(1))
     x[130, 7], x[5, 300], x[299, 399], x[0, 0] = math.inf, -math.inf, math.nan, math.nan
