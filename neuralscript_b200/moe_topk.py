@@ -70,8 +70,12 @@ class MoETopk:
         return out
 
     def forward(self, x, align=1):
-        """y [M, D] of x [M, D] (bf16), and what the backward pass needs."""
-        M, D, E, k = x.shape[0], self.D, self.E, self.k
+        """y [M, D] of x [M, D] (bf16, contiguous rows), and what the backward pass needs."""
+        D, E, k = self.D, self.E, self.k
+        if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != D or x.stride(1) != 1 or x.device != self.gate.device:
+            raise ValueError(f"x: {x.dtype} {tuple(x.shape)} with strides {x.stride()} on {x.device} where rows of {D} "
+                             f"bfloat16 on {self.gate.device} are wanted")
+        M = x.shape[0]
         i32 = dict(dtype=torch.int32, device="cuda")
         logits = _floats(M, E)
         ops.gemm(x, self.gate16, M, E, D, x.stride(0), 0, D, 0, c32=logits)

@@ -76,3 +76,12 @@ def test_backward_refuses_unaligned_segments(align):
     y, kept = layer.forward(x, align=align)
     with pytest.raises(ValueError, match="align"):
         layer.backward(torch.ones_like(y), kept)
+
+
+def test_forward_refuses_other_inputs():
+    layer = MoETopk(128, 128, 4, 2, seed=4)
+    x = torch.randn(256, 256, device="cuda").to(torch.bfloat16)
+    for bad in (x, x[:, :64], x[:, :128].float(), x[:128].t()[:, :128], x[0, :128], x[:, :128].cpu()):
+        with pytest.raises(ValueError, match="wanted"):
+            layer.forward(bad)
+    assert torch.equal(layer.forward(x[:, 64:192])[0], layer.forward(x[:, 64:192].contiguous())[0])
