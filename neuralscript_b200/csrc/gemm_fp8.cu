@@ -1093,10 +1093,17 @@ __global__ void __launch_bounds__(kSmallThreads, SmallCfg<BN, VEC>::CTAS)
     }
 }
 
+// An empty sum (K = 0): zeros into C, of row groups into their own rows alone.
 __global__ void fp8_zero_kernel(const Fp8Gemm d) {
-    const size_t n = (size_t)d.M * d.N;
-    for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) {
-        const size_t at = blockIdx.y * (size_t)d.c_stride + i / d.N * d.ldc + i % d.N;
+    const int g = blockIdx.y;
+    long long r0 = 0, r1 = d.M;
+    if (d.groups && !d.group_k) {
+        r0 = max(0, d.offsets[g]);
+        r1 = min((long long)d.M, r0 + d.counts[g]);
+    }
+    const long long n = (r1 - r0) * d.N, at0 = g * (d.group_k ? d.c_stride : 0) + r0 * d.ldc;
+    for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
+        const long long at = at0 + i / d.N * d.ldc + i % d.N;
         if (d.c_dtype == kBF16) reinterpret_cast<__nv_bfloat16*>(d.c)[at] = f2bf(0.f);
         else reinterpret_cast<float*>(d.c)[at] = 0.f;
     }
@@ -1294,8 +1301,9 @@ int fp8_gemm(const Fp8Gemm& d, cudaStream_t st) {
     if (d.groups > 1024) return -2;
     if (d.M == 0 || d.N == 0) return 0;
     if (!d.c || d.ldc < d.N) return -1;
+    if (d.groups && (!d.offsets || !d.counts)) return -1;
     if (d.K == 0) {  // an empty sum (a weight gradient of no tokens)
-        fp8_zero_kernel<<<dim3(64, d.group_k ? d.groups : 1), 256, 0, st>>>(d);
+        fp8_zero_kernel<<<dim3(64, d.groups ? d.groups : 1), 256, 0, st>>>(d);
         return cudaGetLastError() == cudaSuccess ? 0 : -5;
     }
     if (!d.a || !d.sa || !d.b || !d.sb) return -1;
@@ -1305,7 +1313,6 @@ int fp8_gemm(const Fp8Gemm& d, cudaStream_t st) {
     if (!codes(d.a, d.lda, d.K) || !codes(d.b, d.ldb, d.K) || d.b_stride % 16) return -1;
     const int kb = (d.K + 127) / 128;
     if (d.ld_sa < d.a_rows || d.ld_sb < (d.b_rows ? d.N : kb)) return -1;
-    if (d.groups && (!d.offsets || !d.counts)) return -1;
     if (d.rows && d.row_div <= 0) return -1;
     if (d.a_rows <= 0) return -1;
     const int sms = num_sms();

@@ -410,6 +410,24 @@ def test_experts_without_tokens():
                      torch.empty(0, 16, device=DEV))
 
 
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+def test_sums_of_nothing(out):
+    """K = 0: zeros, in the experts' own rows alone."""
+    i32 = dict(dtype=torch.int32, device=DEV)
+    c = torch.full((9, 40), 7.0, dtype=out, device=DEV)
+    ops.gemm_fp8(codes(5, 0), scales(0, 5), codes(24, 0), scales(1, 0), c[2:7, 8:32])
+    want = torch.full_like(c, 7)
+    want[2:7, 8:32] = 0
+    assert torch.equal(c, want)
+    offsets, counts = torch.tensor([0, 128, 256, 384], **i32), torch.tensor([5, 0, 100], **i32)
+    c = torch.full((384, 24), 7.0, dtype=out, device=DEV)
+    ops.moe_gemm_fp8(codes(384, 0), scales(0, 384), offsets, counts, codes(72, 0).view(3, 24, 0),
+                     torch.empty(3, 1, 0, device=DEV), c)
+    want = torch.full_like(c, 7)
+    want[:5] = want[256:356] = 0
+    assert torch.equal(c, want)
+
+
 def test_product_on_a_side_stream_and_in_a_graph():
     a, sa = rows_of(wild(20, 512, 1))
     b, sb = block_of(wild(256, 512, 2))
