@@ -266,6 +266,12 @@ int nsb_op_fp8_quantize(const void* x, int dtype, long long ld, int M, int K, in
 int nsb_op_fp8_quantize_block(const void* x, int dtype, long long ld, int M, int K, void* q, long long ld_q, float* s,
                               long long ld_s, void* qt, long long ld_qt, float* st, long long ld_st, void* stream);
 
+/* What went wrong on the current device in a product below whose caller gave
+ * no dev_err, since the last call: 0, or the first error's code (101 to 103: a
+ * bounded wait ran out and the product's result is not to be used), which is
+ * cleared. Waits for the stream; not inside a capture. */
+int nsb_op_device_error(int* code, void* stream);
+
 /* C[M,N] = A[M,K] B[N,K]^T of the values that codes and scales stand for:
  * exact products, fp32 sums over 128 k, these scaled and added in fp32,
  * rounded once to c_dtype. A has row scales; B 128 x 128 scales (b_rows 0: a

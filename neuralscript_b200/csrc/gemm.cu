@@ -40,6 +40,20 @@ int num_sms() {
     return n;
 }
 
+static __device__ int g_op_error;  // one on every device
+
+int* op_error_word() {
+    static int* word[kMaxDevices] = {};  // (two threads at once find the same address)
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return nullptr;
+    if (!word[dev]) {
+        void* p = nullptr;
+        if (cudaGetSymbolAddress(&p, g_op_error) != cudaSuccess) return nullptr;
+        word[dev] = reinterpret_cast<int*>(p);
+    }
+    return word[dev];
+}
+
 // ---------------------------------------------------------------------------
 // Epilogue helpers (shared by all paths)
 // ---------------------------------------------------------------------------

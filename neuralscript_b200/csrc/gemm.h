@@ -65,5 +65,8 @@ bool gemm_uses_tensor_cores(const GemmDesc& d);
 
 // Number of SMs of the current device (cached).
 int num_sms();
+// The current device's own error word, for kernels whose caller passes none;
+// NULL where there is no device.
+int* op_error_word();
 
 }  // namespace nsb

@@ -355,6 +355,17 @@ int nsb_op_moe_combine_bwd(const void* dy, const void* o, int dtype, long long l
     return moe_combine_bwd(dy, o, dtype, ld_dy, ld_o, rows, pos, w, M, k, R, D, d_o, ld_do, dw, (cudaStream_t)stream);
 }
 
+int nsb_op_device_error(int* code, void* stream) {
+    int* word = op_error_word();
+    cudaStream_t st = (cudaStream_t)stream;
+    if (!code) return -1;
+    if (!word || cudaMemcpyAsync(code, word, sizeof(int), cudaMemcpyDeviceToHost, st) != cudaSuccess ||
+        cudaStreamSynchronize(st) != cudaSuccess)
+        return -5;
+    if (*code && cudaMemsetAsync(word, 0, sizeof(int), st) != cudaSuccess) return -5;
+    return 0;
+}
+
 int nsb_op_fp8_quantize(const void* x, int dtype, long long ld, int M, int K, int act, const int* rows, int row_div,
                         void* q, long long ld_q, float* s, long long ld_s, void* qt, long long ld_qt, float* st,
                         long long ld_st, void* stream) {
@@ -419,7 +430,7 @@ int nsb_op_gemm_fp8(int M, int N, int K, const void* A, long long lda, const flo
     d.c = C;
     d.c_dtype = c_dtype;
     d.ldc = ldc;
-    d.err = dev_err;
+    d.err = dev_err ? dev_err : op_error_word();
     launch_counter() += 1;
     return fp8_gemm(d, (cudaStream_t)stream);
 }
@@ -452,7 +463,7 @@ int nsb_op_moe_gemm_fp8(int R, int E, int N, int K, const void* A, long long lda
     d.counts = counts;
     d.rows = rows;
     d.row_div = row_div;
-    d.err = dev_err;
+    d.err = dev_err ? dev_err : op_error_word();
     launch_counter() += 1;
     return fp8_gemm(d, (cudaStream_t)stream);
 }
@@ -484,7 +495,7 @@ int nsb_op_moe_wgrad_fp8(int M, int N, int R, int E, const void* A, long long ld
     d.group_k = 1;
     d.offsets = offsets;
     d.counts = counts;
-    d.err = dev_err;
+    d.err = dev_err ? dev_err : op_error_word();
     launch_counter() += 1;
     return fp8_gemm(d, (cudaStream_t)stream);
 }

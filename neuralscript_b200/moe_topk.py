@@ -45,6 +45,7 @@ class MoETopk:
         draw = lambda *s: torch.randn(*s, device="cuda", generator=g) / s[-1] ** 0.5  # noqa: E731
         self.gate, self.w1, self.w2 = draw(E, D), draw(E, H, D), draw(E, D, H)
         self.step = 0
+        self.err = torch.zeros(1, dtype=torch.int32, device="cuda")  # the gate's products'
         self._moments = [(torch.zeros_like(w), torch.zeros_like(w)) for w in (self.gate, self.w1, self.w2)]
         self.refresh()
 
@@ -64,6 +65,15 @@ class MoETopk:
         self.q1, self.q1t = self._blocks(self.w1)
         self.q2, self.q2t = self._blocks(self.w2)
 
+    def check(self):
+        """Waits for the current stream and raises RuntimeError where a product gave up a bounded wait since the last
+        check. train_step calls it; who serves calls it where the results are read."""
+        ops.check_errors()
+        code = int(self.err)
+        if code:
+            self.err.zero_()
+            raise RuntimeError(f"device error {code} in the gate's product")
+
     def _product(self, a, sa, order, b, N, rows=None):
         out = torch.zeros(order["rows"].numel(), N, device="cuda")
         ops.moe_gemm_fp8(a, sa, order["offsets"], order["counts"], *b, out, rows=rows, row_div=self.k)
@@ -78,7 +88,7 @@ class MoETopk:
         M = x.shape[0]
         i32 = dict(dtype=torch.int32, device="cuda")
         logits = _floats(M, E)
-        ops.gemm(x, self.gate16, M, E, D, x.stride(0), 0, D, 0, c32=logits)
+        ops.gemm(x, self.gate16, M, E, D, x.stride(0), 0, D, 0, c32=logits, err=self.err)
         idx, w = torch.empty(M, k, **i32), _floats(M, k)
         ops.moe_topk_route(logits, idx, w, **self.choice, **self.how)
         order = dict(offsets=torch.empty(E + 1, **i32), counts=torch.empty(E, **i32),
@@ -131,9 +141,9 @@ class MoETopk:
         ops.moe_combine(self._product(zq, zs, order, self.q1t, D), order["pos"], dx)
         x32 = x.float()
         dgate = _floats(E, D)
-        ops.gemm(dlogits, x32, E, D, M, E, 1, D, 1, c32=dgate)
+        ops.gemm(dlogits, x32, E, D, M, E, 1, D, 1, c32=dgate, err=self.err)
         total = _floats(M, D)
-        ops.gemm(dlogits, self.gate, M, D, E, E, 0, D, 1, add=dx, c32=total)
+        ops.gemm(dlogits, self.gate, M, D, E, E, 0, D, 1, add=dx, c32=total, err=self.err)
         return total, dgate, dw1, dw2
 
     def update(self, grads, lr):
@@ -144,11 +154,12 @@ class MoETopk:
         self.refresh()
 
     def train_step(self, x, target, lr):
-        """Mean squared error before the step."""
+        """Mean squared error before the step. A step whose products failed changes no weight."""
         y, kept = self.forward(x, align=128)
         diff = y - target
         loss = diff.square().mean()
         _, *grads = self.backward(diff * (2 / diff.numel()), kept)
+        self.check()
         self.update(grads, lr)
         return loss
 
@@ -166,6 +177,7 @@ def main():
         y, _ = layer.forward(x[t:t + 1])
         off = float((y - whole[t]).norm() / whole[t].norm())
         print(f"serving token {t}: {off:.1e} off its row in the batch")
+    layer.check()
 
 
 if __name__ == "__main__":

@@ -60,6 +60,7 @@ _sigs = {
                                       C.c_int] + [C.c_void_p, C.c_longlong] * 4 + [C.c_void_p]),
     "nsb_op_fp8_quantize_block": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_int]
                                   + [C.c_void_p, C.c_longlong] * 4 + [C.c_void_p]),
+    "nsb_op_device_error": (C.c_int, [C.POINTER(C.c_int), C.c_void_p]),
     "nsb_op_gemm_fp8": (C.c_int, [C.c_int, C.c_int, C.c_int] + [C.c_void_p, C.c_longlong] * 4
                         + [C.c_int, C.c_void_p, C.c_int, C.c_longlong, C.c_void_p, C.c_void_p]),
     "nsb_op_moe_gemm_fp8": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_longlong, C.c_int,
@@ -385,10 +386,26 @@ def fp8_quantize_block(x, q=None, s=None, qt=None, st=None):
         _check(rc, "nsb_op_fp8_quantize_block")
 
 
+def _word(err):
+    """Address of a caller's error word; None for the device's own."""
+    return None if err is None else _dense(err, "err", _i32, (1,))
+
+
+def check_errors():
+    """Waits for the current stream and raises RuntimeError where a product since the last call, without an `err` of
+    its own, gave up a bounded wait: its result is not to be used."""
+    lib = _bound if _f32 else _torch()
+    code = C.c_int(0)
+    _check(lib.nsb_op_device_error(C.byref(code), _stream_of(_device())), "nsb_op_device_error")
+    if code.value:
+        raise RuntimeError(f"device error {code.value} since the last check")
+
+
 def gemm_fp8(a, sa, b, sb, c, err=None):
     """c [M, N] (fp32 or bf16) <- A B^T of codes a [M, K] with row scales sa, b [N, K] with scales sb: of rows
     [ceil(K / 128), N], or of blocks [ceil(N / 128), ceil(K / 128)] (both have that shape only where they are the same:
-    N = 1 and K at most 128)."""
+    N = 1 and K at most 128). err (one int32): receives the code of a wait that ran out, in place of the word that
+    check_errors reads."""
     lib = _bound if _f32 else _torch()
     M, K = a.shape
     N = b.shape[0]
@@ -398,7 +415,7 @@ def gemm_fp8(a, sa, b, sb, c, err=None):
     rc = lib.nsb_op_gemm_fp8(
         M, N, K, *_codes(a, "a", M, K), *_rows(sa, "sa", _f32, kb, M), *_codes(b, "b", N, K),
         *(_rows(sb, "sb", _f32, kb, N) if by_rows else _rows(sb, "sb", _f32, -(-N // 128), kb)), by_rows, at, dt, ld,
-        None if err is None else err.data_ptr(), _here(a))
+        _word(err), _here(a))
     if rc:
         _check(rc, "nsb_op_gemm_fp8")
 
@@ -417,7 +434,7 @@ def moe_gemm_fp8(a, sa, offsets, counts, b, sb, c, rows=None, row_div=1, err=Non
         None if rows is None else _dense(rows, "rows", _i32, (R,)), row_div,
         _dense(offsets, "offsets", _i32, (E + 1,)), _dense(counts, "counts", _i32, (E,)),
         *_stack(b, "b", _f8, E, N, K), *_stack(sb, "sb", _f32, E, -(-N // 128), kb), at, dt, ld,
-        None if err is None else err.data_ptr(), _here(a))
+        _word(err), _here(a))
     if rc:
         _check(rc, "nsb_op_moe_gemm_fp8")
 
@@ -436,6 +453,6 @@ def moe_wgrad_fp8(a, sa, b, sb, offsets, counts, c, err=None):
         M, N, R, E, *_codes(a, "a", M, R), *_rows(sa, "sa", _f32, rb, M), *_codes(b, "b", N, R),
         *_rows(sb, "sb", _f32, rb, N), _dense(offsets, "offsets", _i32, (E + 1,)),
         _dense(counts, "counts", _i32, (E,)), at, F32 if c.dtype is _f32 else BF16, ld, apart,
-        None if err is None else err.data_ptr(), _here(a))
+        _word(err), _here(a))
     if rc:
         _check(rc, "nsb_op_moe_wgrad_fp8")

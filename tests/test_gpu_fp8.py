@@ -494,3 +494,41 @@ def test_refusals():
         ops.gemm_fp8(codes(4, 64), f(1, 4), codes(8, 64), f(1, 1), f(4, 8).half())
     with pytest.raises(ValueError):
         ops.moe_gemm_fp8(codes(4, 64), f(1, 4), f(3).int(), f(2).int(), codes(8, 64).view(1, 8, 64), f(1, 1, 1), f(4, 8))
+
+
+def test_error_words():
+    a, sa = rows_of(wild(20, 512, 1))
+    b, sb = block_of(wild(256, 512, 2))
+    c = torch.empty(20, 256, device=DEV)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    ops.gemm_fp8(a, sa, b, sb, c, err=err)
+    assert int(err) == 0
+    ops.gemm_fp8(a, sa, b, sb, c)
+    ops.check_errors()
+    for bad in (err.long(), torch.zeros(2, dtype=torch.int32, device=DEV), err.cpu(), err.view(())):
+        with pytest.raises(ValueError):
+            ops.gemm_fp8(a, sa, b, sb, c, err=bad)
+
+
+def test_first_call_of_a_process_may_be_captured():
+    """Loading, attributes and the error word's address are no allocation of the stream's."""
+    code = """
+import torch
+from neuralscript_b200 import ops
+f8 = torch.float8_e4m3fn
+a, b = torch.ones(20, 512, device="cuda").to(f8), torch.ones(256, 512, device="cuda").to(f8)
+sa, sb, c = torch.ones(4, 20, device="cuda"), torch.ones(2, 4, device="cuda"), torch.zeros(20, 256, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    ops.gemm_fp8(a, sa, b, sb, c)
+g.replay()
+ops.check_errors()
+assert (c == 512).all()
+"""
+    import pathlib
+    import subprocess
+    import sys
+    root = pathlib.Path(__file__).resolve().parent.parent
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]

@@ -85,3 +85,24 @@ def test_forward_refuses_other_inputs():
         with pytest.raises(ValueError, match="wanted"):
             layer.forward(bad)
     assert torch.equal(layer.forward(x[:, 64:192])[0], layer.forward(x[:, 64:192].contiguous())[0])
+
+
+def test_failed_products_stop_the_step(monkeypatch):
+    layer = MoETopk(128, 128, 4, 2, seed=5)
+    x = torch.randn(64, 128, device="cuda").to(torch.bfloat16)
+    layer.err.fill_(102)  # (no product runs while it is set)
+    with pytest.raises(RuntimeError, match="102"):
+        layer.check()
+    layer.check()  # read once
+    before = [w.clone() for w in (layer.gate, layer.w1, layer.w2)]
+
+    def failed():
+        raise RuntimeError("device error 101")
+
+    monkeypatch.setattr(layer, "check", failed)
+    with pytest.raises(RuntimeError, match="101"):
+        layer.train_step(x, x.float(), 1e-3)
+    assert all(torch.equal(a, b) for a, b in zip(before, (layer.gate, layer.w1, layer.w2)))
+    monkeypatch.undo()
+    layer.train_step(x, x.float(), 1e-3)
+    assert not torch.equal(before[1], layer.w1)

@@ -132,3 +132,30 @@ def test_nothing_has_no_address():
     assert rc("nsb_op_moe_combine_bwd", None, None, 0, 64, 64, None, None, None, 0, 2, 0, 64, None, 64, None) == 0
     assert rc("nsb_op_fp8_quantize", None, 0, 64, 0, 64, 0, None, 1, None, 64, None, 0, None, 0, None, 64) == 0
     assert rc("nsb_op_fp8_quantize_block", None, 0, 64, 0, 64, None, 64, None, 1, None, 0, None, 0) == 0
+
+
+def test_device_error_refuses():
+    assert ops.L().nsb_op_device_error(None, None) == -1
+
+
+def test_check_errors_raises(monkeypatch):
+    """A code in the device's word is raised, and a failure to read it."""
+    class Lib:
+        code, rc = 0, 0
+
+        def nsb_op_device_error(self, code, stream):
+            code._obj.value = self.code
+            return self.rc
+
+    lib = Lib()
+    monkeypatch.setattr(ops, "_bound", lib)
+    monkeypatch.setattr(ops, "_f32", object())
+    monkeypatch.setattr(ops, "_device", lambda: 0)
+    monkeypatch.setattr(ops, "_stream_of", lambda d: 0)
+    ops.check_errors()
+    lib.code = 102
+    with pytest.raises(RuntimeError, match="102"):
+        ops.check_errors()
+    lib.code, lib.rc = 0, -5
+    with pytest.raises(RuntimeError, match="-5"):
+        ops.check_errors()
