@@ -236,9 +236,14 @@ int nsb_op_moe_dispatch(const int* idx, int M, int k, int E, int align, int* off
  * [*, D] of one dtype. */
 int nsb_op_moe_combine(const void* o, int dtype, long long ld_o, const int* pos, const float* w, int M, int k, int D,
                        void* y, long long ld_y, void* stream);
+/* The same where o has R rows: a pos past them is left out, and reported by
+ * nsb_op_device_error (above, pos is trusted). */
+int nsb_op_moe_combine_rows(const void* o, int dtype, long long ld_o, int R, const int* pos, const float* w, int M,
+                            int k, int D, void* y, long long ld_y, void* stream);
 /* Its gradient: d_o[r] = w[pair] * dy[pair / k] for pair = rows[r], zeros for
- * rows[r] = -1 (R rows), and dw[pair] = <o[r], dy[pair / k]>, 0 for pairs
- * without a row (dw and o may be NULL together). */
+ * a negative rows[r], or one past the last pair, which is reported (R rows),
+ * and dw[pair] = <o[r], dy[pair / k]>, 0 for pairs without a row (dw and o may
+ * be NULL together). */
 int nsb_op_moe_combine_bwd(const void* dy, const void* o, int dtype, long long ld_dy, long long ld_o, const int* rows,
                            const int* pos, const float* w, int M, int k, int R, int D, void* d_o, long long ld_do,
                            float* dw, void* stream);
@@ -261,15 +266,22 @@ int nsb_op_moe_combine_bwd(const void* dy, const void* o, int dtype, long long l
 int nsb_op_fp8_quantize(const void* x, int dtype, long long ld, int M, int K, int act, const int* rows, int row_div,
                         void* q, long long ld_q, float* s, long long ld_s, void* qt, long long ld_qt, float* st,
                         long long ld_st, void* stream);
+/* The same where x has x_rows rows (at least M of them with row_div 0): an
+ * entry of rows past them counts as a negative one, and is reported by
+ * nsb_op_device_error (above, rows is trusted). */
+int nsb_op_fp8_quantize_rows(const void* x, int dtype, long long ld, int x_rows, int M, int K, int act, const int* rows,
+                             int row_div, void* q, long long ld_q, float* s, long long ld_s, void* qt, long long ld_qt,
+                             float* st, long long ld_st, void* stream);
 /* A scale for each 128 x 128: q [M, ld_q], s [M / 128, ld_s], and / or the
  * transpose of the same codes and scales, qt [K, ld_qt], st [K / 128, ld_st]. */
 int nsb_op_fp8_quantize_block(const void* x, int dtype, long long ld, int M, int K, void* q, long long ld_q, float* s,
                               long long ld_s, void* qt, long long ld_qt, float* st, long long ld_st, void* stream);
 
-/* What went wrong on the current device in a product below whose caller gave
- * no dev_err, since the last call: 0, or the first error's code (101 to 103: a
- * bounded wait ran out and the product's result is not to be used), which is
- * cleared. Waits for the stream; not inside a capture. */
+/* What went wrong on the current device since the last call, in a product
+ * below whose caller gave no dev_err or with an index past its tensor's rows:
+ * 0, or the first error's code, which is cleared (101 to 103: a bounded wait
+ * ran out and the product's result is not to be used; 111: an index was left
+ * out). Waits for the stream; not inside a capture. */
 int nsb_op_device_error(int* code, void* stream);
 
 /* C[M,N] = A[M,K] B[N,K]^T of the values that codes and scales stand for:
@@ -284,7 +296,7 @@ int nsb_op_gemm_fp8(int M, int N, int K, const void* A, long long lda, const flo
  * [R, ldc] are those of A times B[e]^T (b_stride codes and sb_stride scales
  * from expert to expert, 128 x 128 scales); other rows of C are not written.
  * rows (NULL: A is in C's order): row r reads row rows[r] / row_div of A,
- * which has a_rows rows. E <= 1024. */
+ * which has a_rows rows (the last one where the entry is past it). E <= 1024. */
 int nsb_op_moe_gemm_fp8(int R, int E, int N, int K, const void* A, long long lda, int a_rows, const float* sa,
                         long long ld_sa, const int* rows, int row_div, const int* offsets, const int* counts,
                         const void* B, long long ldb, long long b_stride, const float* sb, long long ld_sb,

@@ -20,6 +20,7 @@ enum DevErr : int {
     kErrTimeoutEpilogue = 103,
     kErrTimeoutAttn = 104,
     kErrBadShape = 110,
+    kErrBadIndex = 111,  // an index past its tensor's rows, which was left out
 };
 
 // Operand element types.

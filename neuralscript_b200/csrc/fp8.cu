@@ -135,7 +135,11 @@ __global__ void __launch_bounds__(kThreads, 2) quantize_kernel(const QuantDesc d
         if (r >= d.M) return -1;
         if (!d.rows) return r;
         const int at = d.rows[r];
-        return at < 0 ? -1 : d.row_div ? at / d.row_div : r;
+        if (at < 0) return -1;
+        const int src = d.row_div ? at / d.row_div : r;
+        if (src < d.x_rows) return src;
+        if (d.err) atomicCAS(d.err, 0, kErrBadIndex);
+        return -1;
     };
     auto fetch = [&](int t, int b) {
         const int r0 = t / cb * 128 + half * 4, c0 = t % cb * 128 + cl * 8;
@@ -303,7 +307,7 @@ template <bool BLOCK>
 int quantize(const QuantDesc& d, cudaStream_t st) {
     const bool f = d.dtype == kF32;
     if (d.M < 0 || d.K <= 0 || (!f && d.dtype != kBF16) || d.ld < d.K || d.act < 0 || d.act > kGeluMoe) return -1;
-    if (d.rows && d.row_div < 0) return -1;
+    if (d.rows && (d.row_div < 0 || d.x_rows < (d.row_div ? 0 : d.M))) return -1;
     if (d.M == 0) return 0;  // (what has no elements has no address)
     if (!d.x || (!d.q && !d.qt)) return -1;
     auto codes = [](const void* p, long long ld, int cols) {

@@ -21,9 +21,12 @@ struct QuantDesc {
     int M = 0, K = 0;  // rows of the result (gathered ones with `rows`) and columns
     int act = 0;       // activation applied first
     // Row r of the result is row rows[r] / row_div of x, row r itself where
-    // row_div is 0, and zeros for a negative entry
+    // row_div is 0, and zeros for a negative entry, or one past the x_rows rows
+    // of x, which goes into err
     const int* rows = nullptr;
     int row_div = 1;
+    int x_rows = 0x7fffffff;
+    int* err = nullptr;
     uint8_t* q = nullptr;  // [M, ld_q]
     long long ld_q = 0;
     float* s = nullptr;

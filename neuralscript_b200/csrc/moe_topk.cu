@@ -556,8 +556,8 @@ struct Cols<T, 1> {
 // together. HBM bounds it: 8192 x 4 rows of 2048 bf16 in 29 us (5.8 TB/s).
 template <typename T, int W>
 __global__ void __launch_bounds__(128)
-    combine_kernel(const T* __restrict__ o, long long ld_o, const int* __restrict__ pos, const float* __restrict__ w,
-                   int k, int D, T* __restrict__ y, long long ld_y) {
+    combine_kernel(const T* __restrict__ o, long long ld_o, int R, const int* __restrict__ pos,
+                   const float* __restrict__ w, int k, int D, T* __restrict__ y, long long ld_y, int* err) {
     const size_t t = blockIdx.x;
     const int c = (blockIdx.y * blockDim.x + threadIdx.x) * W;
     if (c >= D) return;
@@ -571,6 +571,10 @@ __global__ void __launch_bounds__(128)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             p[j] = j0 + j < k ? pos[t * k + j0 + j] : -1;
+            if (p[j] >= R) {
+                if (err) atomicCAS(err, 0, kErrBadIndex);
+                p[j] = -1;
+            }
             wj[j] = p[j] >= 0 && w ? w[t * k + j0 + j] : 1.f;
         }
 #pragma unroll
@@ -596,7 +600,8 @@ template <typename T, int W>
 __global__ void __launch_bounds__(256)
     combine_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ o, long long ld_dy, long long ld_o,
                        const int* __restrict__ rows, const int* __restrict__ pos, const float* __restrict__ w,
-                       long long P, int k, int R, int D, T* __restrict__ d_o, long long ld_do, float* __restrict__ dw) {
+                       long long P, int k, int R, int D, T* __restrict__ d_o, long long ld_do, float* __restrict__ dw,
+                       int* err) {
     const long long gt = (long long)blockIdx.x * blockDim.x + threadIdx.x;
     const long long step = (long long)gridDim.x * blockDim.x;
     if (dw)
@@ -605,7 +610,11 @@ __global__ void __launch_bounds__(256)
     const int lane = threadIdx.x & 31;
     int next = gt >> 5 < R ? rows[gt >> 5] : -1;
     for (long long r = gt >> 5; r < R; r += step >> 5) {
-        const int pair = next;
+        int pair = next;
+        if (pair >= P) {
+            if (err && lane == 0) atomicCAS(err, 0, kErrBadIndex);
+            pair = -1;
+        }
         if (r + (step >> 5) < R) next = rows[r + (step >> 5)];
         T* to = d_o + (size_t)r * ld_do;
         if (pair < 0) {
@@ -754,19 +763,19 @@ int moe_dispatch(const int* idx, int M, int k, int E, int align, int* offsets, i
     return go(std::integral_constant<int, 8>()) ? 0 : -5;
 }
 
-int moe_combine(const void* o, int dtype, long long ld_o, const int* pos, const float* w, int M, int k, int D,
-                void* y, long long ld_y, cudaStream_t st) {
-    if (M < 0 || k <= 0 || k > kTopkMaxK || D <= 0 || (dtype != kF32 && dtype != kBF16) || ld_o < D || ld_y < D)
+int moe_combine(const void* o, int dtype, long long ld_o, int R, const int* pos, const float* w, int M, int k, int D,
+                void* y, long long ld_y, int* err, cudaStream_t st) {
+    if (M < 0 || R < 0 || k <= 0 || k > kTopkMaxK || D <= 0 || (dtype != kF32 && dtype != kBF16) || ld_o < D || ld_y < D)
         return -1;
     if (M == 0) return 0;
-    if (!o || !pos || !y) return -1;
+    if ((R && !o) || !pos || !y) return -1;
     const bool vec = rows16(o, ld_o, dtype) && rows16(y, ld_y, dtype) && D % (dtype == kBF16 ? 8 : 4) == 0;
     auto go = [&](auto zero, auto width) {
         using T = decltype(zero);
         constexpr int W = decltype(width)::value;
         const int cols = (D + W - 1) / W, threads = cols < 128 ? (cols + 31) / 32 * 32 : 128;
         combine_kernel<T, W><<<dim3((unsigned)M, (unsigned)((cols + threads - 1) / threads)), threads, 0, st>>>(
-            (const T*)o, ld_o, pos, w, k, D, (T*)y, ld_y);
+            (const T*)o, ld_o, R, pos, w, k, D, (T*)y, ld_y, err);
     };
     if (dtype == kBF16) {
         if (vec) go(__nv_bfloat16(), std::integral_constant<int, 8>());
@@ -780,7 +789,7 @@ int moe_combine(const void* o, int dtype, long long ld_o, const int* pos, const 
 
 int moe_combine_bwd(const void* dy, const void* o, int dtype, long long ld_dy, long long ld_o, const int* rows,
                     const int* pos, const float* w, int M, int k, int R, int D, void* d_o, long long ld_do, float* dw,
-                    cudaStream_t st) {
+                    int* err, cudaStream_t st) {
     if (M < 0 || R < 0 || k <= 0 || k > kTopkMaxK || D <= 0 || (dtype != kF32 && dtype != kBF16)) return -1;
     if (ld_dy < D || ld_do < D || (dw && ld_o < D)) return -1;
     if (M == 0 && R == 0) return 0;
@@ -793,7 +802,8 @@ int moe_combine_bwd(const void* dy, const void* o, int dtype, long long ld_dy, l
         using T = decltype(zero);
         constexpr int W = decltype(width)::value;
         combine_bwd_kernel<T, W><<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(
-            (const T*)dy, (const T*)o, ld_dy, ld_o, rows, pos, w, (long long)M * k, k, R, D, (T*)d_o, ld_do, dw);
+            (const T*)dy, (const T*)o, ld_dy, ld_o, rows, pos, w, (long long)M * k, k, R, D, (T*)d_o, ld_do, dw,
+            err);
     };
     if (dtype == kBF16) {
         if (vec) go(__nv_bfloat16(), std::integral_constant<int, 8>());

@@ -38,10 +38,12 @@ size_t moe_dispatch_rows(long long M, int k, int E, int align);
 int moe_dispatch(const int* idx, int M, int k, int E, int align, int* offsets, int* counts, int* rows, int* pos,
                  cudaStream_t s);
 
-int moe_combine(const void* o, int dtype, long long ld_o, const int* pos, const float* w, int M, int k, int D,
-                void* y, long long ld_y, cudaStream_t s);
+// o has R rows; a place past them, and in the gradient a pair past the last,
+// is left out and goes into err.
+int moe_combine(const void* o, int dtype, long long ld_o, int R, const int* pos, const float* w, int M, int k, int D,
+                void* y, long long ld_y, int* err, cudaStream_t s);
 int moe_combine_bwd(const void* dy, const void* o, int dtype, long long ld_dy, long long ld_o, const int* rows,
                     const int* pos, const float* w, int M, int k, int R, int D, void* d_o, long long ld_do, float* dw,
-                    cudaStream_t s);
+                    int* err, cudaStream_t s);
 
 }  // namespace nsb

@@ -344,15 +344,21 @@ int nsb_op_moe_dispatch(const int* idx, int M, int k, int E, int align, int* off
 
 int nsb_op_moe_combine(const void* o, int dtype, long long ld_o, const int* pos, const float* w, int M, int k, int D,
                        void* y, long long ld_y, void* stream) {
+    return nsb_op_moe_combine_rows(o, dtype, ld_o, 0x7fffffff, pos, w, M, k, D, y, ld_y, stream);
+}
+
+int nsb_op_moe_combine_rows(const void* o, int dtype, long long ld_o, int R, const int* pos, const float* w, int M,
+                            int k, int D, void* y, long long ld_y, void* stream) {
     launch_counter() += 1;
-    return moe_combine(o, dtype, ld_o, pos, w, M, k, D, y, ld_y, (cudaStream_t)stream);
+    return moe_combine(o, dtype, ld_o, R, pos, w, M, k, D, y, ld_y, op_error_word(), (cudaStream_t)stream);
 }
 
 int nsb_op_moe_combine_bwd(const void* dy, const void* o, int dtype, long long ld_dy, long long ld_o, const int* rows,
                            const int* pos, const float* w, int M, int k, int R, int D, void* d_o, long long ld_do,
                            float* dw, void* stream) {
     launch_counter() += 1;
-    return moe_combine_bwd(dy, o, dtype, ld_dy, ld_o, rows, pos, w, M, k, R, D, d_o, ld_do, dw, (cudaStream_t)stream);
+    return moe_combine_bwd(dy, o, dtype, ld_dy, ld_o, rows, pos, w, M, k, R, D, d_o, ld_do, dw, op_error_word(),
+                           (cudaStream_t)stream);
 }
 
 int nsb_op_device_error(int* code, void* stream) {
@@ -369,10 +375,19 @@ int nsb_op_device_error(int* code, void* stream) {
 int nsb_op_fp8_quantize(const void* x, int dtype, long long ld, int M, int K, int act, const int* rows, int row_div,
                         void* q, long long ld_q, float* s, long long ld_s, void* qt, long long ld_qt, float* st,
                         long long ld_st, void* stream) {
+    return nsb_op_fp8_quantize_rows(x, dtype, ld, 0x7fffffff, M, K, act, rows, row_div, q, ld_q, s, ld_s, qt, ld_qt, st,
+                                    ld_st, stream);
+}
+
+int nsb_op_fp8_quantize_rows(const void* x, int dtype, long long ld, int x_rows, int M, int K, int act, const int* rows,
+                             int row_div, void* q, long long ld_q, float* s, long long ld_s, void* qt, long long ld_qt,
+                             float* st, long long ld_st, void* stream) {
     QuantDesc d;
     d.x = x;
     d.dtype = dtype;
     d.ld = ld;
+    d.x_rows = x_rows;
+    d.err = rows ? op_error_word() : nullptr;
     d.M = M;
     d.K = K;
     d.act = act;

@@ -53,11 +53,15 @@ _sigs = {
                                       C.c_void_p, C.c_void_p, C.c_void_p]),
     "nsb_op_moe_combine": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
                                      C.c_int, C.c_void_p, C.c_longlong, C.c_void_p]),
+    "nsb_op_moe_combine_rows": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_void_p, C.c_void_p, C.c_int,
+                                          C.c_int, C.c_int, C.c_void_p, C.c_longlong, C.c_void_p]),
     "nsb_op_moe_combine_bwd": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_longlong, C.c_longlong, C.c_void_p,
                                          C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p,
                                          C.c_longlong, C.c_void_p, C.c_void_p]),
     "nsb_op_fp8_quantize": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_void_p,
                                       C.c_int] + [C.c_void_p, C.c_longlong] * 4 + [C.c_void_p]),
+    "nsb_op_fp8_quantize_rows": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_int,
+                                           C.c_void_p, C.c_int] + [C.c_void_p, C.c_longlong] * 4 + [C.c_void_p]),
     "nsb_op_fp8_quantize_block": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_int]
                                   + [C.c_void_p, C.c_longlong] * 4 + [C.c_void_p]),
     "nsb_op_device_error": (C.c_int, [C.POINTER(C.c_int), C.c_void_p]),
@@ -318,15 +322,16 @@ def moe_dispatch(idx, E, offsets, counts, rows, pos, align=1):
 
 
 def moe_combine(o, pos, y, w=None):
-    """y [M, D] <- sum over j of w[:, j] * o[pos[:, j]] (w None: 1)."""
+    """y [M, D] <- sum over j of w[:, j] * o[pos[:, j]] (w None: 1). Negative entries of pos are left out, and so are
+    those past o's rows, which check_errors raises."""
     lib = _bound if _f32 else _torch()
     M, k = pos.shape
     R, D = o.shape
-    rc = lib.nsb_op_moe_combine(
-        *_float(o, "o", R, D), _dense(pos, "pos", _i32, (M, k)),
+    rc = lib.nsb_op_moe_combine_rows(
+        *_float(o, "o", R, D), R, _dense(pos, "pos", _i32, (M, k)),
         None if w is None else _dense(w, "w", _f32, (M, k)), M, k, D, *_rows(y, "y", o.dtype, M, D), _here(o))
     if rc:
-        _check(rc, "nsb_op_moe_combine")
+        _check(rc, "nsb_op_moe_combine_rows")
 
 
 def moe_combine_bwd(dy, o, rows, pos, w, do, dw=None):
@@ -359,18 +364,19 @@ def fp8_quantize(x, q=None, s=None, qt=None, st=None, act=0, rows=None, row_div=
     """q [M, K] with s [ceil(K / 128), M], and / or qt [K, M] with st [ceil(M / 128), K] <- codes and scales of act(x).
 
     q, qt: float8_e4m3fn with rows on 16-byte boundaries. rows [M] (int32) gathers rows[r] / row_div of x first
-    (row_div 0: only puts zeros where rows is negative)."""
+    (row_div 0: only puts zeros where rows is negative); an entry past x's rows gives zeros, and check_errors raises
+    it."""
     lib = _bound if _f32 else _torch()
     n, K = x.shape
     M = n if rows is None else rows.shape[0]
     if rows is not None and row_div == 0 and n < M:
         raise ValueError(f"x: {n} rows where {M} are wanted")
-    rc = lib.nsb_op_fp8_quantize(
-        *_float(x, "x", n, K), M, K, act, None if rows is None else _dense(rows, "rows", _i32, (M,)), row_div,
+    rc = lib.nsb_op_fp8_quantize_rows(
+        *_float(x, "x", n, K), n, M, K, act, None if rows is None else _dense(rows, "rows", _i32, (M,)), row_div,
         *(_NOTHING if q is None else _codes(q, "q", M, K) + _rows(s, "s", _f32, -(-K // 128), M)),
         *(_NOTHING if qt is None else _codes(qt, "qt", K, M) + _rows(st, "st", _f32, -(-M // 128), K)), _here(x))
     if rc:
-        _check(rc, "nsb_op_fp8_quantize")
+        _check(rc, "nsb_op_fp8_quantize_rows")
 
 
 def fp8_quantize_block(x, q=None, s=None, qt=None, st=None):
@@ -392,13 +398,14 @@ def _word(err):
 
 
 def check_errors():
-    """Waits for the current stream and raises RuntimeError where a product since the last call, without an `err` of
-    its own, gave up a bounded wait: its result is not to be used."""
+    """Waits for the current stream and raises RuntimeError where since the last call a product without an `err` of
+    its own gave up a bounded wait (its result is not to be used), or an index was past its tensor's rows."""
     lib = _bound if _f32 else _torch()
     code = C.c_int(0)
     _check(lib.nsb_op_device_error(C.byref(code), _stream_of(_device())), "nsb_op_device_error")
     if code.value:
-        raise RuntimeError(f"device error {code.value} since the last check")
+        why = "an index past its tensor's rows" if code.value == 111 else "a product's wait ran out"
+        raise RuntimeError(f"device error {code.value} since the last check: {why}")
 
 
 def gemm_fp8(a, sa, b, sb, c, err=None):

@@ -366,3 +366,38 @@ def test_no_tokens(dtype):
     ops.moe_combine(c, pos, y, w)
     ops.moe_combine_bwd(y, c, rows, pos, w, torch.empty_like(c), dw)
     torch.cuda.synchronize()
+
+
+def test_indices_past_the_rows_are_left_out_and_reported():
+    """Guarded by the kernels' own comparison with the number of rows."""
+    f8, i32 = torch.float8_e4m3fn, dict(dtype=torch.int32, device=DEV)
+    ops.check_errors()
+    o = torch.randn(6, 40, device=DEV, generator=gen(1))
+    pos = torch.tensor([[0, 6], [5, 2 ** 31 - 1], [1000000, -1]], **i32)
+    y = torch.empty(3, 40, device=DEV)
+    ops.moe_combine(o, pos, y)
+    assert torch.equal(y[0], o[0]) and torch.equal(y[1], o[5]) and (y[2] == 0).all()
+    with pytest.raises(RuntimeError, match="111"):
+        ops.check_errors()
+    ops.check_errors()  # read once
+    dy, do, dw = torch.randn(3, 40, device=DEV, generator=gen(2)), torch.empty(4, 40, device=DEV), torch.empty(3, 2, device=DEV)
+    rows, pos = torch.tensor([0, 6, 2 ** 31 - 1, 5], **i32), torch.tensor([[0, -1], [-1, -1], [-1, 3]], **i32)
+    ops.moe_combine_bwd(dy, o[:4], rows, pos, None, do, dw)
+    assert torch.equal(do[0], dy[0]) and torch.equal(do[3], dy[2]) and (do[1:3] == 0).all()
+    assert (dw.flatten()[1:5] == 0).all() and dw[0, 0] != 0 and dw[2, 1] != 0
+    with pytest.raises(RuntimeError, match="111"):
+        ops.check_errors()
+    for dtype in (torch.float32, torch.bfloat16):
+        x = torch.randn(5, 48, device=DEV, generator=gen(3)).to(dtype)
+        rows = torch.tensor([9, 10, 2 ** 31 - 1, 0, -1], **i32)
+        q, s, qt, st = (torch.empty(5, 48, device=DEV).to(f8), torch.empty(1, 5, device=DEV),
+                        torch.empty(48, 16, device=DEV).to(f8)[:, :5], torch.empty(1, 48, device=DEV))
+        ops.fp8_quantize(x, q, s, qt, st, rows=rows, row_div=2)
+        with pytest.raises(RuntimeError, match="111"):
+            ops.check_errors()
+        want, ws = torch.empty(2, 48, device=DEV).to(f8), torch.empty(1, 2, device=DEV)
+        ops.fp8_quantize(x[[4, 0]], want, ws)
+        assert torch.equal(q[[0, 3]].float(), want.float()) and torch.equal(s[:, [0, 3]], ws)
+        assert (q[[1, 2, 4]].float() == 0).all() and (qt[:, [1, 2, 4]].float() == 0).all()
+        assert (s[0, [1, 2, 4]] == 2.0 ** -100).all()
+    ops.check_errors()

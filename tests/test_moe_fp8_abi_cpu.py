@@ -159,3 +159,16 @@ def test_check_errors_raises(monkeypatch):
     lib.code, lib.rc = 0, -5
     with pytest.raises(RuntimeError, match="-5"):
         ops.check_errors()
+
+
+def test_bounded_entries_refuse():
+    ok = [X, 0, 64, 8, X, X, 4, 2, 64, X, 64]
+    for at, v in ((0, None), (1, 3), (2, 63), (3, -1), (4, None), (6, -1), (7, 0), (7, 33), (8, 0), (9, None), (10, 63)):
+        a = list(ok)
+        a[at] = v
+        assert rc("nsb_op_moe_combine_rows", *a) == -1, at
+    ok = [X, 0, 64, 4, 4, 64, 0, X, 0, X, 64, X, 4, X, 16, X, 64]
+    for at, v in ((0, None), (3, 3), (3, -1), (8, -1), (9, X + 8), (10, 48), (11, None)):
+        a = list(ok)
+        a[at] = v
+        assert rc("nsb_op_fp8_quantize_rows", *a) == -1, at
