@@ -730,15 +730,22 @@ int moe_dispatch(const int* idx, int M, int k, int E, int align, int* offsets, i
     const size_t cap = moe_dispatch_rows(M, k, E, align);
     if (cap > 0x7fffffffu) return -2;
     const long long P = (long long)M * k;
-    const int smem = (kOrderWarps * E + 4 * E + 1 + kOrderWarps) * (int)sizeof(int);
+    auto bytes = [](int experts) { return (kOrderWarps * experts + 4 * experts + 1 + kOrderWarps) * (int)sizeof(int); };
+    const int smem = bytes(E);
     auto go = [&](auto ctas) {
         constexpr int CTAS = decltype(ctas)::value;
         auto f = dispatch_kernel<CTAS>;
-        if (smem > 48 * 1024 &&
-            cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-            return false;
-        if (CTAS > 8 && cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-            return false;
+        // Once a device, to the most that any E takes: a limit set for this E
+        // would be another thread's, which launches with more.
+        static bool done[kMaxDevices] = {};
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return false;
+        if (!done[dev]) {
+            if (cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes(kTopkMaxE)) != cudaSuccess ||
+                (CTAS > 8 && cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess))
+                return false;
+            done[dev] = true;
+        }
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(CTAS);
         cfg.blockDim = dim3(kOrderThreads);

@@ -401,3 +401,28 @@ def test_indices_past_the_rows_are_left_out_and_reported():
         assert (q[[1, 2, 4]].float() == 0).all() and (qt[:, [1, 2, 4]].float() == 0).all()
         assert (s[0, [1, 2, 4]] == 2.0 ** -100).all()
     ops.check_errors()
+
+
+def test_dispatch_from_two_threads():
+    """Orders of few and of many experts, whose launches take different amounts of shared memory, at the same time."""
+    import threading
+    errors = []
+
+    def work(E, calls=3000):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                idx = torch.randint(0, E, (40, 2), device=DEV, dtype=torch.int32)
+                i32 = dict(dtype=torch.int32, device=DEV)
+                out = [torch.empty(E + 1, **i32), torch.empty(E, **i32), torch.empty(80, **i32), torch.empty(40, 2, **i32)]
+                for _ in range(calls):
+                    ops.moe_dispatch(idx, E, *out)
+                assert int(out[1].sum()) == 80
+        except Exception as e:
+            errors.append((E, e))
+
+    threads = [threading.Thread(target=work, args=(E,)) for E in (1024, 400, 1000, 512)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
