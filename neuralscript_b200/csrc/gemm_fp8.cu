@@ -276,150 +276,153 @@ __global__ void __launch_bounds__(kThreads, 1)
         return w;
     };
 
-    if (warp == 1 || warp == 2) {
+    if (warp < 4) {
+        // (all four warps of the group at one instruction, and the registers
+        // that the compiler counts on in the branch itself)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (lane == 0 && rank == 0) {
-            const int mine = warp - 1;
-            const Pipe pipe{dead, p.err, kErrTimeoutMma};
-            int it = 0;  // k-blocks so far: number `it` uses stage it % STAGES and part it % PARTS
+        if (warp == 1 || warp == 2) {
+            if (lane == 0 && rank == 0) {
+                const int mine = warp - 1;
+                const Pipe pipe{dead, p.err, kErrTimeoutMma};
+                int it = 0;  // k-blocks so far: number `it` uses stage it % STAGES and part it % PARTS
+                for (int u = first; u < total; u += stride) {
+                    const Unit w = unit(u);
+                    for (int kb = w.kb0; kb < w.kb1; kb++, it++) {
+                        if ((it & 1) != mine) continue;
+                        const int stage = it % C::STAGES, part = it % C::PARTS;
+                        pipe.wait(&full[stage], it / C::STAGES & 1);
+                        pipe.wait(&part_empty[part], (it / C::PARTS & 1) ^ 1);
+                        // gathered rows came through the generic proxy; the fence is
+                        // here, where no copies are in flight that it would wait for
+                        if (gather) ptx::fence_proxy_async();
+                        ptx::tc_fence_after();
+                        const uint32_t sa = ptx::smem_u32(smem + stage * C::STAGE), sb = sa + C::A_BYTES;
+    #pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const uint64_t da = ptx::smem_desc(sa + k * 32, 16, 1024, 2);
+                            const uint64_t db = ptx::smem_desc(sb + k * 32, 16, 1024, 2);
+                            if (PAIR) ptx::mma_f8_pair(tmem + part * C::PCOLS, da, db, IDESC, k > 0);
+                            else ptx::mma_f8(tmem + part * C::PCOLS, da, db, IDESC, k > 0);
+                        }
+                        if (PAIR) {
+                            ptx::mma_commit_pair(&empty[stage]);
+                            ptx::mma_commit_pair(&part_full[part]);
+                        } else {
+                            ptx::mma_commit(&empty[stage]);
+                            ptx::mma_commit(&part_full[part]);
+                        }
+                    }
+                }
+            }
+        } else {
+            const int t = (warp == 0 ? 0 : 32) + lane;  // 0..63
+            int slot = 0, stage = 0;
+            uint32_t slot_phase = 0, phase = 0;
+            const Pipe pipe{dead, p.err, kErrTimeoutProducer};
             for (int u = first; u < total; u += stride) {
-                const Unit w = unit(u);
-                for (int kb = w.kb0; kb < w.kb1; kb++, it++) {
-                    if ((it & 1) != mine) continue;
-                    const int stage = it % C::STAGES, part = it % C::PARTS;
-                    pipe.wait(&full[stage], it / C::STAGES & 1);
-                    pipe.wait(&part_empty[part], (it / C::PARTS & 1) ^ 1);
-                    // gathered rows came through the generic proxy; the fence is
-                    // here, where no copies are in flight that it would wait for
-                    if (gather) ptx::fence_proxy_async();
-                    ptx::tc_fence_after();
-                    const uint32_t sa = ptx::smem_u32(smem + stage * C::STAGE), sb = sa + C::A_BYTES;
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint64_t da = ptx::smem_desc(sa + k * 32, 16, 1024, 2);
-                        const uint64_t db = ptx::smem_desc(sb + k * 32, 16, 1024, 2);
-                        if (PAIR) ptx::mma_f8_pair(tmem + part * C::PCOLS, da, db, IDESC, k > 0);
-                        else ptx::mma_f8(tmem + part * C::PCOLS, da, db, IDESC, k > 0);
-                    }
-                    if (PAIR) {
-                        ptx::mma_commit_pair(&empty[stage]);
-                        ptx::mma_commit_pair(&part_full[part]);
-                    } else {
-                        ptx::mma_commit(&empty[stage]);
-                        ptx::mma_commit(&part_full[part]);
-                    }
+                Unit w = unit(u);
+                if (PAIR) w.m0 += rank * 128;
+                // the rows whose scales this thread copies; rows past the end
+                // take the first one's, and are not stored
+                const float* srow[2];
+    #pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int m = w.m0 + t + 64 * i;
+                    const int r = m >= w.row_end ? 0 : gather ? min(max(0, p.rows[m]) / p.row_div, p.a_rows - 1) : m;
+                    srow[i] = p.sa + r;
                 }
-            }
-        }
-    } else if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        const int t = (warp == 0 ? 0 : 32) + lane;  // 0..63
-        int slot = 0, stage = 0;
-        uint32_t slot_phase = 0, phase = 0;
-        const Pipe pipe{dead, p.err, kErrTimeoutProducer};
-        for (int u = first; u < total; u += stride) {
-            Unit w = unit(u);
-            if (PAIR) w.m0 += rank * 128;
-            // the rows whose scales this thread copies; rows past the end
-            // take the first one's, and are not stored
-            const float* srow[2];
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int m = w.m0 + t + 64 * i;
-                const int r = m >= w.row_end ? 0 : gather ? min(max(0, p.rows[m]) / p.row_div, p.a_rows - 1) : m;
-                srow[i] = p.sa + r;
-            }
-            const float* sb = p.sb;
-            if (!VEC)
-                sb += (ROWS ? w.g * p.sb_stride : 0) +
-                      (long long)min(w.n0 / 128 + (t & 1) * (BN / 256), p.nb - 1) * p.ld_sb;
-            // gathered: pieces t % 4 and t % 4 + 4 (of 16 bytes) of rows t / 4,
-            // t / 4 + 16, ...; rows past the end read the first one's
-            const uint8_t* from[8];
-            if (gather) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int m = w.m0 + t / 4 + 16 * i;
-                    const int r = m < w.row_end ? min(max(0, p.rows[m]) / p.row_div, p.a_rows - 1) : 0;
-                    from[i] = p.a + (size_t)r * p.lda + (t & 3) * 16;
-                }
-            }
-            for (int kb = w.kb0; kb < w.kb1; kb++) {
-                const int in = (kb - w.kb0) % C::SLOTK;
-                if (in == 0) pipe.wait(&slot_empty[slot], slot_phase ^ 1);
-                float* to = slots + (slot * C::SLOTK + in) * C::SLOT;
-#pragma unroll
-                for (int i = 0; i < 2; i++) ptx::cp_async4(to + t + 64 * i, srow[i] + kb * p.ld_sa);
-                if (VEC) {
-#pragma unroll
-                    for (int i = 0; i < BN / 64; i++) {
-                        const int n = w.n0 + t + 64 * i;
-                        if (n < p.N) ptx::cp_async4(to + 128 + t + 64 * i, sb + kb * p.ld_sb + n);
-                    }
-                } else if (t < 2) {
-                    ptx::cp_async4(to + 128 + t, sb + kb);
-                }
-                if (in == C::SLOTK - 1 || kb + 1 == w.kb1) {
-                    ptx::cp_async_arrive(&slot_full[slot]);
-                    if (++slot == kSlots) {
-                        slot = 0;
-                        slot_phase ^= 1;
-                    }
-                }
-                if (!gather && warp != 0) continue;
-                pipe.wait(&empty[stage], phase ^ 1);
-                uint8_t* sa = smem + stage * C::STAGE;
-                if (t == 0) {
-                    if (PAIR) {
-                        // both CTAs' loads complete on the first one's barrier
-                        const uint32_t bar = ptx::cluster_addr(&full[stage], 0);
-                        if (rank == 0) ptx::mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE);
-                        ptx::tma_load_2d_pair(sa, &ta, bar, kb * 128, w.m0);
-                        ptx::tma_load_3d_pair(sa + C::A_BYTES, &tb, bar, kb * 128, w.n0 + rank * C::BROWS, 0);
-                    } else {
-                        ptx::mbar_arrive_expect_tx(&full[stage], gather ? C::STAGE - C::A_BYTES : C::STAGE);
-                        if (!gather) ptx::tma_load_2d(sa, &ta, &full[stage], kb * 128, w.m0);
-                        ptx::tma_load_3d(sa + C::A_BYTES, &tb, &full[stage], kb * 128, w.n0, ROWS ? w.g : 0);
-                    }
-                }
-                uint64_t* landed = &full[stage];
-                if (++stage == C::STAGES) {
-                    stage = 0;
-                    phase ^= 1;
-                }
-                if (!gather) continue;
-                // row r's piece q lies at piece q ^ (r % 8)
-                uint8_t* lo = sa + (t >> 2) * 128 + (((t & 3) ^ (t >> 2 & 7)) << 4);
-                uint8_t* hi = sa + (t >> 2) * 128 + (((t & 3) ^ (t >> 2 & 7) ^ 4) << 4);
-                if (kb * 128 + 128 <= p.K) {
-#pragma unroll
+                const float* sb = p.sb;
+                if (!VEC)
+                    sb += (ROWS ? w.g * p.sb_stride : 0) +
+                          (long long)min(w.n0 / 128 + (t & 1) * (BN / 256), p.nb - 1) * p.ld_sb;
+                // gathered: pieces t % 4 and t % 4 + 4 (of 16 bytes) of rows t / 4,
+                // t / 4 + 16, ...; rows past the end read the first one's
+                const uint8_t* from[8];
+                if (gather) {
+    #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        ptx::cp_async16(lo + i * 2048, from[i]);
-                        ptx::cp_async16(hi + i * 2048, from[i] + 64);
-                        from[i] += 128;
-                    }
-                } else {
-                    const int k = kb * 128 + (t & 3) * 16;
-                    const int b0 = max(0, min(16, p.K - k)), b1 = max(0, min(16, p.K - k - 64));
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        ptx::cp_async16(lo + i * 2048, b0 ? from[i] : p.a, b0);
-                        ptx::cp_async16(hi + i * 2048, b1 ? from[i] + 64 : p.a, b1);
+                        const int m = w.m0 + t / 4 + 16 * i;
+                        const int r = m < w.row_end ? min(max(0, p.rows[m]) / p.row_div, p.a_rows - 1) : 0;
+                        from[i] = p.a + (size_t)r * p.lda + (t & 3) * 16;
                     }
                 }
-                ptx::cp_async_arrive(landed);
+                for (int kb = w.kb0; kb < w.kb1; kb++) {
+                    const int in = (kb - w.kb0) % C::SLOTK;
+                    if (in == 0) pipe.wait(&slot_empty[slot], slot_phase ^ 1);
+                    float* to = slots + (slot * C::SLOTK + in) * C::SLOT;
+    #pragma unroll
+                    for (int i = 0; i < 2; i++) ptx::cp_async4(to + t + 64 * i, srow[i] + kb * p.ld_sa);
+                    if (VEC) {
+    #pragma unroll
+                        for (int i = 0; i < BN / 64; i++) {
+                            const int n = w.n0 + t + 64 * i;
+                            if (n < p.N) ptx::cp_async4(to + 128 + t + 64 * i, sb + kb * p.ld_sb + n);
+                        }
+                    } else if (t < 2) {
+                        ptx::cp_async4(to + 128 + t, sb + kb);
+                    }
+                    if (in == C::SLOTK - 1 || kb + 1 == w.kb1) {
+                        ptx::cp_async_arrive(&slot_full[slot]);
+                        if (++slot == kSlots) {
+                            slot = 0;
+                            slot_phase ^= 1;
+                        }
+                    }
+                    if (!gather && warp != 0) continue;
+                    pipe.wait(&empty[stage], phase ^ 1);
+                    uint8_t* sa = smem + stage * C::STAGE;
+                    if (t == 0) {
+                        if (PAIR) {
+                            // both CTAs' loads complete on the first one's barrier
+                            const uint32_t bar = ptx::cluster_addr(&full[stage], 0);
+                            if (rank == 0) ptx::mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE);
+                            ptx::tma_load_2d_pair(sa, &ta, bar, kb * 128, w.m0);
+                            ptx::tma_load_3d_pair(sa + C::A_BYTES, &tb, bar, kb * 128, w.n0 + rank * C::BROWS, 0);
+                        } else {
+                            ptx::mbar_arrive_expect_tx(&full[stage], gather ? C::STAGE - C::A_BYTES : C::STAGE);
+                            if (!gather) ptx::tma_load_2d(sa, &ta, &full[stage], kb * 128, w.m0);
+                            ptx::tma_load_3d(sa + C::A_BYTES, &tb, &full[stage], kb * 128, w.n0, ROWS ? w.g : 0);
+                        }
+                    }
+                    uint64_t* landed = &full[stage];
+                    if (++stage == C::STAGES) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                    if (!gather) continue;
+                    // row r's piece q lies at piece q ^ (r % 8)
+                    uint8_t* lo = sa + (t >> 2) * 128 + (((t & 3) ^ (t >> 2 & 7)) << 4);
+                    uint8_t* hi = sa + (t >> 2) * 128 + (((t & 3) ^ (t >> 2 & 7) ^ 4) << 4);
+                    if (kb * 128 + 128 <= p.K) {
+    #pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            ptx::cp_async16(lo + i * 2048, from[i]);
+                            ptx::cp_async16(hi + i * 2048, from[i] + 64);
+                            from[i] += 128;
+                        }
+                    } else {
+                        const int k = kb * 128 + (t & 3) * 16;
+                        const int b0 = max(0, min(16, p.K - k)), b1 = max(0, min(16, p.K - k - 64));
+    #pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            ptx::cp_async16(lo + i * 2048, b0 ? from[i] : p.a, b0);
+                            ptx::cp_async16(hi + i * 2048, b1 ? from[i] + 64 : p.a, b1);
+                        }
+                    }
+                    ptx::cp_async_arrive(landed);
+                }
             }
+            ptx::cp_async_wait_all();
+            // every load has landed and been used before the CTA exits (bounded)
+            if (t == 0)
+                for (int s = 0; s < C::STAGES; s++) {
+                    pipe.wait(&empty[stage], phase ^ 1);
+                    if (++stage == C::STAGES) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
         }
-        ptx::cp_async_wait_all();
-        // every load has landed and been used before the CTA exits (bounded)
-        if (t == 0)
-            for (int s = 0; s < C::STAGES; s++) {
-                pipe.wait(&empty[stage], phase ^ 1);
-                if (++stage == C::STAGES) {
-                    stage = 0;
-                    phase ^= 1;
-                }
-            }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int quarter = warp & 3, half = (warp - 4) >> 2;
@@ -705,7 +708,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     if constexpr (C::SPLITS) {
         if (split > 1) {
             // the shares are added in rank order; rank r stores every split-th row
-            __syncwarp();
             ptx::cluster_sync();
             const Unit w = unit_at<C::BM, BN, ROWS>(p, start, first);
             const float* sum = reinterpret_cast<const float*>(smem);
@@ -739,7 +741,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-            __syncwarp();
             ptx::cluster_sync();  // no CTA leaves while others read its sums
         }
     }
@@ -1071,7 +1072,6 @@ __global__ void __launch_bounds__(kSmallThreads, SmallCfg<BN, VEC>::CTAS)
     if (sp.split > 1) {
         // the k-blocks' shares are added in rank order; rank r stores every
         // split-th row of the tile
-        __syncwarp();
         ptx::cluster_sync();
         if (first < total) {
             const Unit w = small_unit<BN>(p, start, first);
@@ -1088,7 +1088,6 @@ __global__ void __launch_bounds__(kSmallThreads, SmallCfg<BN, VEC>::CTAS)
                 }
             }
         }
-        __syncwarp();
         ptx::cluster_sync();  // no CTA leaves while others read its sums
     }
 }

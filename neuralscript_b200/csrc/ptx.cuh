@@ -152,7 +152,10 @@ __device__ __forceinline__ uint32_t cluster_ctarank() {
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
+// (.aligned: all lanes of a warp come together, which loops of unequal length
+// do not promise)
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 // Arrive at a barrier of any CTA of the cluster where `on` holds; what it
