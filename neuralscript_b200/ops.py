@@ -208,9 +208,11 @@ def _torch():
     """torch's names that every call below needs, looked up once (a decode step's kernels take a few microseconds)."""
     global _f32, _bf16, _i32, _u8, _f8, _stream_of, _device
     import torch
+    lib = L()  # raises where the library is missing, in this call and in the next
     _stream_of, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
-    _f32, _bf16, _i32, _u8, _f8 = torch.float32, torch.bfloat16, torch.int32, torch.uint8, torch.float8_e4m3fn
-    return L()
+    _bf16, _i32, _u8, _f8 = torch.bfloat16, torch.int32, torch.uint8, torch.float8_e4m3fn
+    _f32 = torch.float32  # last: where it is set, other threads find all the rest
+    return lib
 
 
 def _refuse(t, what, dtype, shape):

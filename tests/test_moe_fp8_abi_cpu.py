@@ -172,3 +172,30 @@ def test_bounded_entries_refuse():
         a = list(ok)
         a[at] = v
         assert rc("nsb_op_fp8_quantize_rows", *a) == -1, at
+
+
+def test_missing_library_is_reported_by_every_call(monkeypatch):
+    torch = pytest.importorskip("torch")
+    monkeypatch.setattr(ops, "_bound", None)
+    monkeypatch.setattr(ops, "_f32", None)
+
+    def missing():
+        raise RuntimeError("libns_b200.so missing")
+
+    monkeypatch.setattr(ops, "_core_lib", missing)
+    idx, w = torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 2)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="missing"):
+            ops.moe_topk_route(torch.zeros(4, 8), idx, w)
+        with pytest.raises(RuntimeError, match="missing"):
+            ops.check_errors()
+
+
+def test_names_are_published_behind_the_library(monkeypatch):
+    """A thread that comes while another one loads the library sees all names or none."""
+    monkeypatch.setattr(ops, "_f32", None)
+    monkeypatch.setattr(ops, "_f8", None)
+    seen = []
+    load = ops.L
+    monkeypatch.setattr(ops, "L", lambda: (seen.append(ops._f32), load())[1])
+    assert ops._torch() is load() and seen == [None] and ops._f8 is not None
