@@ -220,23 +220,23 @@ def _refuse(t, what, dtype, shape):
         raise ValueError(f"{what}: {t.dtype} where {dtype} is wanted")
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{what}: shape {tuple(t.shape)} where {tuple(shape)} is wanted")
-    if not t.is_cuda:
-        raise ValueError(f"{what}: not on a CUDA device")
+    if t.get_device() != _device():
+        raise ValueError(f"{what}: on {t.device}, where the current CUDA device ({_device()}), whose kernels run, is wanted")
     raise ValueError(f"{what}: strides {t.stride()} are not those of contiguous rows (or of a dense tensor where one is "
                      "wanted)")
 
 
 def _dense(t, what, dtype, shape):
-    """Address of a CUDA tensor of this dtype and shape without gaps."""
-    if t.dtype is not dtype or t.shape != shape or not t.is_cuda or not t.is_contiguous():
+    """Address of a tensor of this dtype and shape without gaps, on the current device."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != _device() or not t.is_contiguous():
         _refuse(t, what, dtype, shape)
     return t.data_ptr()
 
 
 def _rows(t, what, dtype, rows, cols):
-    """Address and leading dimension of a CUDA matrix of this dtype and shape whose rows are contiguous. (torch does
-    not look at the stride of a single row; the kernels do.)"""
-    if t.dtype is not dtype or t.shape != (rows, cols) or not t.is_cuda:
+    """Address and leading dimension of a matrix of this dtype and shape, on the current device, whose rows are
+    contiguous. (torch does not look at the stride of a single row; the kernels do.)"""
+    if t.dtype is not dtype or t.shape != (rows, cols) or t.get_device() != _device():
         _refuse(t, what, dtype, (rows, cols))
     ld, one = t.stride()
     if one != 1 and cols > 1:
@@ -261,7 +261,7 @@ def _codes(t, what, rows, cols):
 
 def _stack(t, what, dtype, n, rows, cols):
     """As _rows for n matrices: address, leading dimension and the stride from one to the next."""
-    if t.dtype is not dtype or t.shape != (n, rows, cols) or not t.is_cuda:
+    if t.dtype is not dtype or t.shape != (n, rows, cols) or t.get_device() != _device():
         _refuse(t, what, dtype, (n, rows, cols))
     apart, ld, one = t.stride()
     if one != 1 and cols > 1:
@@ -269,12 +269,9 @@ def _stack(t, what, dtype, n, rows, cols):
     return t.data_ptr(), ld if rows > 1 else max(ld, -(-cols // 16) * 16 if dtype is _f8 else cols), apart
 
 
-def _here(t):
-    """The current stream; the kernels run on the current device."""
-    d = _device()
-    if t.get_device() != d:
-        raise ValueError(f"tensors are on {t.device}, the current device is {d}")
-    return _stream_of(d)
+def _here():
+    """The current stream."""
+    return _stream_of(_device())
 
 
 def moe_topk_route(logits, idx, w, score="softmax", bias=None, active=None, groups=1, topk_groups=1, renorm=True,
@@ -287,7 +284,7 @@ def moe_topk_route(logits, idx, w, score="softmax", bias=None, active=None, grou
         *_float(logits, "logits", M, E), M, E, k, _SCORE[score],
         None if bias is None else _dense(bias, "bias", _f32, (E,)),
         None if active is None else _dense(active, "active", _u8, (E,)), groups, topk_groups, renorm, scale,
-        _dense(idx, "idx", _i32, (M, k)), _dense(w, "w", _f32, (M, k)), _here(logits))
+        _dense(idx, "idx", _i32, (M, k)), _dense(w, "w", _f32, (M, k)), _here())
     if rc:
         _check(rc, "nsb_op_moe_topk_route")
 
@@ -300,7 +297,7 @@ def moe_topk_route_bwd(dw, logits, idx, dlogits, score="softmax", active=None, r
     rc = lib.nsb_op_moe_topk_route_bwd(
         _dense(dw, "dw", _f32, (M, k)), *_float(logits, "logits", M, E), M, E, k, _SCORE[score],
         None if active is None else _dense(active, "active", _u8, (E,)), renorm, scale,
-        _dense(idx, "idx", _i32, (M, k)), *_rows(dlogits, "dlogits", logits.dtype, M, E), _here(logits))
+        _dense(idx, "idx", _i32, (M, k)), *_rows(dlogits, "dlogits", logits.dtype, M, E), _here())
     if rc:
         _check(rc, "nsb_op_moe_topk_route_bwd")
 
@@ -318,7 +315,7 @@ def moe_dispatch(idx, E, offsets, counts, rows, pos, align=1):
         _dense(idx, "idx", _i32, (M, k)), M, k, E, align, _dense(offsets, "offsets", _i32, (E + 1,)),
         _dense(counts, "counts", _i32, (E,)),
         _dense(rows, "rows", _i32, (lib.nsb_op_moe_dispatch_rows(M, k, E, align),)), _dense(pos, "pos", _i32, (M, k)),
-        _here(idx))
+        _here())
     if rc:
         _check(rc, "nsb_op_moe_dispatch")
 
@@ -331,7 +328,7 @@ def moe_combine(o, pos, y, w=None):
     R, D = o.shape
     rc = lib.nsb_op_moe_combine_rows(
         *_float(o, "o", R, D), R, _dense(pos, "pos", _i32, (M, k)),
-        None if w is None else _dense(w, "w", _f32, (M, k)), M, k, D, *_rows(y, "y", o.dtype, M, D), _here(o))
+        None if w is None else _dense(w, "w", _f32, (M, k)), M, k, D, *_rows(y, "y", o.dtype, M, D), _here())
     if rc:
         _check(rc, "nsb_op_moe_combine_rows")
 
@@ -349,7 +346,7 @@ def moe_combine_bwd(dy, o, rows, pos, w, do, dw=None):
     rc = lib.nsb_op_moe_combine_bwd(
         at, o_at, dt, ld, o_ld, _dense(rows, "rows", _i32, (R,)), _dense(pos, "pos", _i32, (M, k)),
         None if w is None else _dense(w, "w", _f32, (M, k)), M, k, R, D, *_rows(do, "do", dy.dtype, R, D),
-        None if dw is None else _dense(dw, "dw", _f32, (M, k)), _here(dy))
+        None if dw is None else _dense(dw, "dw", _f32, (M, k)), _here())
     if rc:
         _check(rc, "nsb_op_moe_combine_bwd")
 
@@ -376,7 +373,7 @@ def fp8_quantize(x, q=None, s=None, qt=None, st=None, act=0, rows=None, row_div=
     rc = lib.nsb_op_fp8_quantize_rows(
         *_float(x, "x", n, K), n, M, K, act, None if rows is None else _dense(rows, "rows", _i32, (M,)), row_div,
         *(_NOTHING if q is None else _codes(q, "q", M, K) + _rows(s, "s", _f32, -(-K // 128), M)),
-        *(_NOTHING if qt is None else _codes(qt, "qt", K, M) + _rows(st, "st", _f32, -(-M // 128), K)), _here(x))
+        *(_NOTHING if qt is None else _codes(qt, "qt", K, M) + _rows(st, "st", _f32, -(-M // 128), K)), _here())
     if rc:
         _check(rc, "nsb_op_fp8_quantize_rows")
 
@@ -389,7 +386,7 @@ def fp8_quantize_block(x, q=None, s=None, qt=None, st=None):
     rc = lib.nsb_op_fp8_quantize_block(
         *_float(x, "x", M, K), M, K,
         *(_NOTHING if q is None else _codes(q, "q", M, K) + _rows(s, "s", _f32, mb, kb)),
-        *(_NOTHING if qt is None else _codes(qt, "qt", K, M) + _rows(st, "st", _f32, kb, mb)), _here(x))
+        *(_NOTHING if qt is None else _codes(qt, "qt", K, M) + _rows(st, "st", _f32, kb, mb)), _here())
     if rc:
         _check(rc, "nsb_op_fp8_quantize_block")
 
@@ -404,7 +401,7 @@ def check_errors():
     its own gave up a bounded wait (its result is not to be used), or an index was past its tensor's rows."""
     lib = _bound if _f32 else _torch()
     code = C.c_int(0)
-    _check(lib.nsb_op_device_error(C.byref(code), _stream_of(_device())), "nsb_op_device_error")
+    _check(lib.nsb_op_device_error(C.byref(code), _here()), "nsb_op_device_error")
     if code.value:
         why = "an index past its tensor's rows" if code.value == 111 else "a product's wait ran out"
         raise RuntimeError(f"device error {code.value} since the last check: {why}")
@@ -424,7 +421,7 @@ def gemm_fp8(a, sa, b, sb, c, err=None):
     rc = lib.nsb_op_gemm_fp8(
         M, N, K, *_codes(a, "a", M, K), *_rows(sa, "sa", _f32, kb, M), *_codes(b, "b", N, K),
         *(_rows(sb, "sb", _f32, kb, N) if by_rows else _rows(sb, "sb", _f32, -(-N // 128), kb)), by_rows, at, dt, ld,
-        _word(err), _here(a))
+        _word(err), _here())
     if rc:
         _check(rc, "nsb_op_gemm_fp8")
 
@@ -443,7 +440,7 @@ def moe_gemm_fp8(a, sa, offsets, counts, b, sb, c, rows=None, row_div=1, err=Non
         None if rows is None else _dense(rows, "rows", _i32, (R,)), row_div,
         _dense(offsets, "offsets", _i32, (E + 1,)), _dense(counts, "counts", _i32, (E,)),
         *_stack(b, "b", _f8, E, N, K), *_stack(sb, "sb", _f32, E, -(-N // 128), kb), at, dt, ld,
-        _word(err), _here(a))
+        _word(err), _here())
     if rc:
         _check(rc, "nsb_op_moe_gemm_fp8")
 
@@ -462,6 +459,6 @@ def moe_wgrad_fp8(a, sa, b, sb, offsets, counts, c, err=None):
         M, N, R, E, *_codes(a, "a", M, R), *_rows(sa, "sa", _f32, rb, M), *_codes(b, "b", N, R),
         *_rows(sb, "sb", _f32, rb, N), _dense(offsets, "offsets", _i32, (E + 1,)),
         _dense(counts, "counts", _i32, (E,)), at, F32 if c.dtype is _f32 else BF16, ld, apart,
-        _word(err), _here(a))
+        _word(err), _here())
     if rc:
         _check(rc, "nsb_op_moe_wgrad_fp8")

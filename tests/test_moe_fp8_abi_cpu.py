@@ -6,6 +6,8 @@ import pytest
 
 from neuralscript_b200 import ops
 
+torch = pytest.importorskip("torch")
+
 X = 0x10000  # an address that is never read
 
 
@@ -175,7 +177,6 @@ def test_bounded_entries_refuse():
 
 
 def test_missing_library_is_reported_by_every_call(monkeypatch):
-    torch = pytest.importorskip("torch")
     monkeypatch.setattr(ops, "_bound", None)
     monkeypatch.setattr(ops, "_f32", None)
 
@@ -199,3 +200,72 @@ def test_names_are_published_behind_the_library(monkeypatch):
     load = ops.L
     monkeypatch.setattr(ops, "L", lambda: (seen.append(ops._f32), load())[1])
     assert ops._torch() is load() and seen == [None] and ops._f8 is not None
+
+
+class Far:
+    """What the entries ask of a tensor, of one that no process here could hold."""
+
+    def __init__(self, shape, dtype, device=0):
+        self.shape, self.dtype, self.device = torch.Size(shape), dtype, f"cuda:{device}"
+        self.at = device
+
+    def get_device(self):
+        return self.at
+
+    is_cuda = True
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return X
+
+    def stride(self):
+        out = [1]
+        for n in reversed(self.shape[1:]):
+            out.insert(0, out[0] * n)
+        return tuple(out)
+
+
+def calls():
+    """Every entry with all its tensors: (name, function of a device for each tensor, how many tensors)."""
+    f, i, q, u, h = torch.float32, torch.int32, torch.float8_e4m3fn, torch.uint8, torch.bfloat16
+    o = ops
+    yield o.moe_topk_route, [((4, 16), f), ((4, 2), i), ((4, 2), f)], dict(bias=((16,), f), active=((16,), u))
+    yield o.moe_topk_route_bwd, [((4, 2), f), ((4, 16), h), ((4, 2), i), ((4, 16), h)], dict(active=((16,), u))
+    yield o.moe_dispatch, [((4, 2), i), 8, ((9,), i), ((8,), i), ((8,), i), ((4, 2), i)], {}
+    yield o.moe_combine, [((8, 64), f), ((4, 2), i), ((4, 64), f)], dict(w=((4, 2), f))
+    yield o.moe_combine_bwd, [((4, 64), h), ((8, 64), h), ((8,), i), ((4, 2), i), ((4, 2), f), ((8, 64), h)], dict(dw=((4, 2), f))
+    yield o.fp8_quantize, [((8, 64), f)], dict(q=((4, 64), q), s=((1, 4), f), qt=((64, 4), q), st=((1, 64), f), rows=((4,), i))
+    yield o.fp8_quantize_block, [((4, 64), f)], dict(q=((4, 64), q), s=((1, 1), f), qt=((64, 4), q), st=((1, 1), f))
+    yield o.gemm_fp8, [((4, 64), q), ((1, 4), f), ((8, 64), q), ((1, 8), f), ((4, 8), h)], dict(err=((1,), i))
+    yield (o.moe_gemm_fp8, [((4, 64), q), ((1, 4), f), ((3,), i), ((2,), i), ((2, 8, 64), q), ((2, 1, 1), f), ((6, 8), f)],
+           dict(rows=((6,), i), err=((1,), i)))
+    yield (o.moe_wgrad_fp8, [((8, 256), q), ((2, 8), f), ((16, 256), q), ((2, 16), f), ((3,), i), ((2,), i), ((2, 8, 16), f)],
+           dict(err=((1,), i)))
+
+
+def test_every_tensor_is_on_the_current_device(monkeypatch):
+    class Lib:
+        def nsb_op_moe_dispatch_rows(self, M, k, E, align):
+            return M * k
+
+        def __getattr__(self, name):
+            return lambda *a: 0
+
+    ops._torch()
+    monkeypatch.setattr(ops, "_bound", Lib())
+    monkeypatch.setattr(ops, "_device", lambda: 0)
+    monkeypatch.setattr(ops, "_stream_of", lambda d: 0)
+    for f, args, named in calls():
+        every = list(enumerate(args)) + list(named.items())
+
+        def call(elsewhere):
+            make = lambda at, a: Far(*a, 1 if at == elsewhere else 0) if isinstance(a, tuple) else a  # noqa: E731
+            f(*(make(n, a) for n, a in enumerate(args)), **{n: make(n, a) for n, a in named.items()})
+
+        call(None)
+        for at, a in every:
+            if isinstance(a, tuple):
+                with pytest.raises(ValueError, match="cuda:1"):
+                    call(at)
