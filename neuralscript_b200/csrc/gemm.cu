@@ -1376,7 +1376,11 @@ static int gemm_tc(const GemmDesc& d, cudaStream_t s, int* dev_err) {
     // (row-grouped GEMMs too: a tile never crosses an expert's 128-row
     // padded segment, and padding rows, whose operand rows are zero, store
     // zeros)
-    if (p.vec_ok && !d.group_k && p.splits == 1 && !d.ep.out_rows && !d.ep.col_block &&
+    // A TMA store clips rows to whole 16-byte pieces: rows of 16-bit values that
+    // end inside one (N % 8 = 4; their leading dimension is a multiple of 8, so
+    // there is a gap behind them) would zero what follows.
+    const bool half_out = d.ep.c16 || (d.ep.z && d.ep.z_dtype != kF32);
+    if (p.vec_ok && !(half_out && d.N % 8) && !d.group_k && p.splits == 1 && !d.ep.out_rows && !d.ep.col_block &&
         (d.ep.z || d.ep.c32 || d.ep.c16)) {
         bool okm = true;
         if (d.ep.z) okm = okm && make_out_map(&om.z, d.ep.z, d.ep.z_dtype, d.N, d.M, d.ep.ld_z);

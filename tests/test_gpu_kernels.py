@@ -465,3 +465,23 @@ def test_cross_entropy_finish_from_fp16_logits(M, C):
     assert relerr(got, seed) < 4e-3
     # each element within bf16 rounding of the fp64 value
     assert np.all(np.abs(got - seed) <= np.abs(seed) * (2.0 ** -8 + 1e-4) + 1e-12)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,N,K,gap", [(64, 100, 64, 4), (200, 132, 96, 12), (300, 260, 128, 4), (130, 4, 64, 4),
+                                       (64, 100, 64, 0), (150, 264, 64, 8)])
+def test_gemm_writes_nothing_beside_its_rows(dt, M, N, K, gap):
+    """fp32 and bf16 outputs that are rows of wider buffers, whose other columns stay as they are."""
+    g = torch.Generator(device=DEV).manual_seed(M + N)
+    A, B = torch.randn(M, K, device=DEV, generator=g).to(dt), torch.randn(N, K, device=DEV, generator=g).to(dt)
+    c16 = torch.full((M + 1, N + gap), 7.0, dtype=torch.bfloat16, device=DEV)
+    c32 = torch.full((M + 1, N + gap), 7.0, device=DEV)
+    for out in (dict(c16=c16[:M, :N]), dict(c32=c32[:M, :N]), dict(c16=c16[:M, :N], c32=c32[:M, :N])):
+        c16.fill_(7.0)
+        c32.fill_(7.0)
+        O.gemm(A, B, M, N, K, K, 0, K, 0, **out)
+        ref = A.double() @ B.double().t()
+        for name, c in (("c16", c16), ("c32", c32)):
+            assert (c[:, N:] == 7).all() and (c[M] == 7).all(), name
+            if name in out:
+                assert relerr(c[:M, :N].float().cpu(), ref.cpu()) < (5e-3 if name == "c16" else 1e-3)
