@@ -532,3 +532,197 @@ assert (c == 512).all()
     root = pathlib.Path(__file__).resolve().parent.parent
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+# --------------------------------------------------------------------------
+# Blocks that take several tiles in turn: what a tile leaves behind (rings,
+# parts of TMEM, staging, shared memory) is the next one's start. Each case
+# says how many tiles there are, by the rules of the launches.
+# --------------------------------------------------------------------------
+SMS = torch.cuda.get_device_properties(0).multi_processor_count if torch.cuda.is_available() else 148
+
+
+def tiles_of(m_tiles, N, by_rows=False):
+    """Width and number of the large products' tiles: the least rounds x (width + 64)."""
+    cost = lambda bn: -(-m_tiles * -(-N // bn) // SMS) * (bn + 64)  # noqa: E731
+    if by_rows and cost(192) < cost(256) and cost(192) <= cost(128):
+        bn = 192
+    else:
+        bn = 128 if cost(128) < cost(256) else 256
+    return bn, m_tiles * -(-N // bn)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,K", [(2500, 2184), (5001, 2184), (3000, 2179)])
+@pytest.mark.parametrize("gathered", [False, True])
+def test_quantize_many_tiles(dtype, M, K, gathered):
+    assert up(M, 128) // 128 * (up(K, 128) // 128) > 2 * SMS  # two blocks an SM
+    x = wild(M, K, M).to(dtype)
+    full, how = x, {}
+    if gathered:
+        rows = torch.randint(-1, 2 * M, (M,), device=DEV, generator=gen(4), dtype=torch.int32)
+        full, how = torch.where((rows >= 0)[:, None], x[rows.long().clamp(min=0) // 2], 0), dict(rows=rows, row_div=2)
+    rq, rs = ref_rows(full)
+    rqt, rst = ref_rows(full.t())
+    for both in ("q", "qt", "both"):
+        q, s, qt, st = codes(M, K), scales(up(K, 128) // 128, M), codes(K, M), scales(up(M, 128) // 128, K)
+        out = (dict(q=q, s=s) if both != "qt" else {}) | (dict(qt=qt, st=st) if both != "q" else {})
+        ops.fp8_quantize(x, **out, **how)
+        if both != "qt":
+            assert same(q, rq) and torch.equal(s, rs), both
+        if both != "q":
+            assert same(qt, rqt) and torch.equal(st, rst), both
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,K", [(2500, 2184), (5001, 2179)])
+@pytest.mark.parametrize("transposed", [False, True])
+def test_quantize_block_many_tiles(dtype, M, K, transposed):
+    x = wild(M, K, M).to(dtype)
+    MB, KB = up(M, 128) // 128, up(K, 128) // 128
+    assert MB * KB > 2 * SMS
+    q, s, qt, st = codes(M, K), scales(MB, KB), codes(K, M), scales(KB, MB)
+    ops.fp8_quantize_block(x, q, s, *((qt, st) if transposed else ()))
+    b = torch.nn.functional.pad(x.float(), (0, KB * 128 - K, 0, MB * 128 - M)).view(MB, 128, KB, 128)
+    rs = torch.clamp(b.abs().amax((1, 3)) / 448, min=2.0 ** -100)
+    rq = (b * (1 / rs)[:, None, :, None]).to(F8).view(MB * 128, KB * 128)[:M, :K]
+    assert torch.equal(s, rs) and same(q, rq)
+    if transposed:
+        assert torch.equal(st, rs.t()) and same(qt, rq.t())
+
+
+@pytest.mark.parametrize("M,N,K,bn", [(3500, 2800, 300, 192), (5000, 2000, 136, 192), (3000, 3500, 260, 256),
+                                      (4000, 4100, 130, 256), (20000, 120, 300, 128)])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+def test_product_scaled_by_rows_of_many_tiles(M, N, K, bn, out):
+    width, tiles = tiles_of(up(M, 128) // 128, N, True)
+    assert width == bn and tiles > SMS
+    a, sa = rows_of(wild(M, K, 1), 3)
+    b, sb = rows_of(wild(N, K, 2), 1)
+    c = torch.full((M + 1, N), math.nan, dtype=out, device=DEV)
+    ops.gemm_fp8(a, sa, b, sb, c[:M])
+    assert near(c[:M], values_rows(a, sa), values_rows(b, sb), K)
+    assert c[M].isnan().all()
+
+
+@pytest.mark.parametrize("M,N,K", [(4096, 2560, 128), (4000, 2570, 100), (4100, 2560, 272)])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+def test_product_on_pairs(M, N, K, out):
+    """From one 256 x 256 tile an SM on: one k-block, a ragged one, and a last pair whose second half is empty."""
+    assert up(M, 256) // 256 * (up(N, 256) // 256) >= SMS
+    a, sa = rows_of(wild(M, K, 1), 3)
+    b, sb = block_of(wild(N, K, 2))
+    c = torch.full((M + 1, N), math.nan, dtype=out, device=DEV)
+    ops.gemm_fp8(a, sa, b, sb, c[:M])
+    assert near(c[:M], values_rows(a, sa), values_block(b, sb), K)
+    assert c[M].isnan().all()
+
+
+@pytest.mark.parametrize("M,N", [(5, 1000), (30, 300), (100, 1000), (40, 72)])
+@pytest.mark.parametrize("by_rows", [False, True])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+def test_product_split_with_empty_shares(M, N, by_rows, out):
+    """17 k-blocks over 8 CTAs in shares of 3: the last two have none."""
+    K = 17 * 128 - 5
+    rows, slots = (16 if M <= 16 else 32, 2 * SMS) if M <= 32 else (128, SMS)
+    assert up(M, rows) // rows * (up(N, 128) // 128) * 8 <= slots
+    a, sa = rows_of(wild(M, K, 1))
+    b, sb = rows_of(wild(N, K, 2)) if by_rows else block_of(wild(N, K, 2))
+    c = torch.full((M + 1, N), math.nan, dtype=out, device=DEV)
+    ops.gemm_fp8(a, sa, b, sb, c[:M])
+    assert near(c[:M], values_rows(a, sa), values_rows(b, sb) if by_rows else values_block(b, sb), K)
+    assert c[M].isnan().all()
+
+
+@pytest.mark.parametrize("M", [3, 30])
+@pytest.mark.parametrize("by_rows", [False, True])
+def test_small_product_of_many_tiles(M, by_rows):
+    N, K = 40000, 5 * 128 + 16
+    assert up(N, 128) // 128 > 2 * SMS
+    a, sa = rows_of(wild(M, K, 1))
+    b, sb = rows_of(wild(N, K, 2)) if by_rows else block_of(wild(N, K, 2))
+    c = torch.full((M + 1, N), math.nan, device=DEV)
+    ops.gemm_fp8(a, sa, b, sb, c[:M])
+    assert near(c[:M], values_rows(a, sa), values_rows(b, sb) if by_rows else values_block(b, sb), K)
+    assert c[M].isnan().all()
+
+
+def uneven(pairs, E, seed):
+    """One choice a token: expert 1 has none, expert 0 one, and the others shares that differ by powers of two."""
+    g = gen(seed)
+    share = torch.exp2(-torch.arange(E, device=DEV).float() / 2)
+    share[:2] = 0
+    idx = torch.multinomial(share, pairs, replacement=True, generator=g).to(torch.int32)
+    idx[pairs // 2] = 0
+    return idx[:, None].contiguous()
+
+
+@pytest.mark.parametrize("pairs,E,N,K,align,bn", [(8000, 6, 2056, 272, 1, 256), (7000, 6, 2050, 136, 128, 256),
+                                                  (19000, 7, 120, 400, 128, 128), (2000, 40, 2100, 200, 1, 0),
+                                                  (500, 40, 2104, 272, 1, 0)])
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+def test_experts_product_of_many_tiles(pairs, E, N, K, align, bn, gather, out):
+    """bn 0: the small kernel, for up to 128 rows an expert."""
+    offsets, counts, rows, pos = order(uneven(pairs, E, N), E, align)
+    R = rows.numel()
+    n = counts.tolist()
+    if bn:
+        assert R > 128 * E and tiles_of(up(R, 128) // 128, N)[0] == bn
+        assert sum(-(-v // 128) for v in n) * -(-N // bn) > SMS
+    else:
+        wide = 16 if -(-R // E) <= 16 else 32
+        assert -(-R // E) <= 128 and sum(-(-v // wide) for v in n) * -(-N // 128) > 2 * SMS
+    a, sa = rows_of(wild(pairs if gather else R, K, 1), 2)
+    ws = [block_of(wild(N, K, 10 + e)) for e in range(E)]
+    b = torch.zeros(E, N, up(K, 16), dtype=torch.uint8, device=DEV)
+    b[:, :, :K] = torch.stack([q.view(torch.uint8) for q, _ in ws])
+    b, sb = b.view(F8)[:, :, :K], torch.stack([s for _, s in ws])
+    c = torch.full((R, N), 7.0, dtype=out, device=DEV)
+    ops.moe_gemm_fp8(a, sa, offsets, counts, b, sb, c, rows=rows if gather else None)
+    av = values_rows(a, sa)
+    written = torch.zeros(R, dtype=torch.bool, device=DEV)
+    for e in range(E):
+        o = int(offsets[e])
+        src = rows[o:o + n[e]].long() if gather else torch.arange(o, o + n[e], device=DEV)
+        assert near(c[o:o + n[e]], av[src], values_block(*ws[e]), K), e
+        written[o:o + n[e]] = True
+    assert (c[~written] == 7).all()
+
+
+@pytest.mark.parametrize("M,N,E,bn", [(520, 1000, 16, 256), (260, 600, 33, 192), (260, 120, 100, 128), (258, 602, 33, 192)])
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+def test_experts_weight_gradient_of_many_tiles(M, N, E, bn, out):
+    width, tiles = tiles_of(up(M, 128) // 128 * E, N, True)
+    assert width == bn and tiles > 2 * SMS
+    offsets, counts, rows, pos = order(uneven(6000, E, M), E, 128)
+    R = rows.numel()
+    x, dz = wild(6000, N, 1), torch.randn(R, M, device=DEV, generator=gen(2))
+    xt, sx, gt, sg = codes(N, R), scales(R // 128, N), codes(M, R), scales(R // 128, M)
+    ops.fp8_quantize(x, qt=xt, st=sx, rows=rows)
+    ops.fp8_quantize(dz, qt=gt, st=sg, rows=rows, row_div=0)
+    c = torch.full((E, M, N), math.nan, dtype=out, device=DEV)
+    ops.moe_wgrad_fp8(gt, sg, xt, sx, offsets, counts, c)
+    gv, xv = values_rows(gt, sg), values_rows(xt, sx)
+    for e in range(E):
+        o, n = int(offsets[e]), int(counts[e])
+        assert near(c[e], gv[:, o:o + n], xv[:, o:o + n], n), e
+    assert (c[1] == 0).all()  # no rows
+
+
+def test_products_on_another_stream_than_the_current_one_before():
+    """Inputs made late on a side stream: a launch on any other stream would read what was there before."""
+    s = torch.cuda.Stream()
+    for M, N, K in ((20, 256, 512), (300, 512, 640)):
+        x, w = wild(M, K, 1), wild(N, K, 2)
+        a, sa = rows_of(torch.zeros_like(x))
+        b, sb = block_of(torch.zeros_like(w))
+        c = torch.full((M, N), math.nan, device=DEV)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(20_000_000)
+            ops.fp8_quantize(x, a, sa)
+            ops.fp8_quantize_block(w, b, sb)
+            ops.gemm_fp8(a, sa, b, sb, c)
+        s.synchronize()
+        assert near(c, values_rows(a, sa), values_block(b, sb), K) and (c != 0).any()

@@ -426,3 +426,40 @@ def test_dispatch_from_two_threads():
     for t in threads:
         t.join()
     assert not errors
+
+
+def test_dispatch_of_more_pairs_than_a_block_holds():
+    """From 16 blocks x 32 warps x 256 pairs on a warp loads its pairs a second time to place them."""
+    M, k, E = 40000, 4, 96
+    assert M * k > 16 * 32 * 256
+    idx = torch.randint(-1, E, (M, k), device=DEV, generator=gen(1), dtype=torch.int32)
+    offsets, counts, rows, pos = dispatch(idx, E, 16)
+    flat = idx.reshape(-1).long()
+    key = torch.where(flat >= 0, flat, E)
+    perm = torch.argsort(key, stable=True)
+    n = torch.bincount(key, minlength=E + 1)[:E]
+    start = torch.cat([torch.zeros(1, dtype=torch.long, device=DEV), ((n + 15) // 16 * 16).cumsum(0)])
+    assert torch.equal(offsets.long(), start) and torch.equal(counts.long(), n)
+    first = torch.cat([torch.zeros(1, dtype=torch.long, device=DEV), n.cumsum(0)])
+    e = key[perm]
+    there = e < E
+    at = start[e[there]] + torch.arange(M * k, device=DEV)[there] - first[e[there]]
+    want_rows, want_pos = torch.full_like(rows, -1), torch.full((M * k,), -1, dtype=torch.int32, device=DEV)
+    want_rows[at] = perm[there].to(torch.int32)
+    want_pos[perm[there]] = at.to(torch.int32)
+    assert torch.equal(rows, want_rows) and torch.equal(pos.reshape(-1), want_pos)
+
+
+def test_dispatch_in_a_graph():
+    """One block, 8 and 16 of them, of few and of many experts, replayed on other choices."""
+    for M, E in ((100, 8), (1000, 1024), (9000, 1024)):
+        idx = torch.randint(0, E, (M, 2), device=DEV, generator=gen(M), dtype=torch.int32)
+        out = dispatch(idx, E, 1)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ops.moe_dispatch(idx, E, *out)
+        idx.copy_(torch.randint(0, E, (M, 2), device=DEV, generator=gen(M + 1), dtype=torch.int32))
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, dispatch(idx, E, 1)))
