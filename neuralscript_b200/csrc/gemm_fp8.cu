@@ -101,26 +101,38 @@ struct TileCfg {
     static_assert(STAGES % 2 == 0 && PARTS % 2 == 0, "a stage and a part always meet the same one of two issuers");
 };
 
-// Waits of the pipeline. A wait that runs out of time records the error and
-// raises the CTA's flag; from then on no wait of the CTA lasts, so every role
-// runs to its end (on stale data) without having to leave its loops.
+// Waits of the pipeline. A wait that runs out of time records the error,
+// raises the CTA's flag and returns false; from then on no wait of the CTA
+// lasts. Copying warps and MMA issuers then stop issuing and drain what they
+// have in flight, so that nothing lands in shared memory or TMEM that is no
+// longer theirs; the scaling warps run to their end on stale data.
 struct Pipe {
     volatile int* dead;
     int* err;
     int code;
-    __device__ __forceinline__ void slow(uint64_t* bar, uint32_t parity) const {
+    __device__ __forceinline__ bool slow(uint64_t* bar, uint32_t parity) const {
         const long long t0 = clock64();
         while (!ptx::mbar_try_wait(bar, parity)) {
-            if (*dead) return;
+            if (*dead) return false;
             if (clock64() - t0 > ptx::kWaitCycles) {
                 *dead = 1;
                 if (err) atomicCAS(err, 0, code);
-                return;
+                return false;
             }
         }
+        return true;
     }
-    __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity) const {
-        if (!ptx::mbar_try_wait(bar, parity)) slow(bar, parity);
+    __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) const {
+        return ptx::mbar_try_wait(bar, parity) || slow(bar, parity);
+    }
+    // Where the CTA gave up: waits, with a limit of its own, for the phases of
+    // `bars` that the last `most` of `uses` uses of a ring complete.
+    __device__ __forceinline__ void drain(uint64_t* bars, int ring, int uses, int most) const {
+        if (!*dead) return;
+        const long long t0 = clock64();
+        for (int i = max(0, uses - most); i < uses; i++)
+            while (!ptx::mbar_try_wait(&bars[i % ring], i / ring & 1))
+                if (clock64() - t0 > ptx::kWaitCycles) return;
     }
 };
 
@@ -285,13 +297,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int mine = warp - 1;
                 const Pipe pipe{dead, p.err, kErrTimeoutMma};
                 int it = 0;  // k-blocks so far: number `it` uses stage it % STAGES and part it % PARTS
+                int last = -1;
                 for (int u = first; u < total; u += stride) {
                     const Unit w = unit(u);
                     for (int kb = w.kb0; kb < w.kb1; kb++, it++) {
                         if ((it & 1) != mine) continue;
                         const int stage = it % C::STAGES, part = it % C::PARTS;
-                        pipe.wait(&full[stage], it / C::STAGES & 1);
-                        pipe.wait(&part_empty[part], (it / C::PARTS & 1) ^ 1);
+                        if (!pipe.wait(&full[stage], it / C::STAGES & 1)) goto issued;
+                        if (!pipe.wait(&part_empty[part], (it / C::PARTS & 1) ^ 1)) goto issued;
+                        last = it;
                         // gathered rows came through the generic proxy; the fence is
                         // here, where no copies are in flight that it would wait for
                         if (gather) ptx::fence_proxy_async();
@@ -313,10 +327,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
+            issued:
+                // the MMAs are done before TMEM is freed (else the scaling warps
+                // have waited for them)
+                pipe.drain(empty, C::STAGES, last + 1, 1);
+                pipe.drain(part_full, C::PARTS, last + 1, 1);
             }
         } else {
             const int t = (warp == 0 ? 0 : 32) + lane;  // 0..63
-            int slot = 0, stage = 0;
+            int slot = 0, stage = 0, loads = 0;
             uint32_t slot_phase = 0, phase = 0;
             const Pipe pipe{dead, p.err, kErrTimeoutProducer};
             for (int u = first; u < total; u += stride) {
@@ -348,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 for (int kb = w.kb0; kb < w.kb1; kb++) {
                     const int in = (kb - w.kb0) % C::SLOTK;
-                    if (in == 0) pipe.wait(&slot_empty[slot], slot_phase ^ 1);
+                    if (in == 0 && !pipe.wait(&slot_empty[slot], slot_phase ^ 1)) goto copied;
                     float* to = slots + (slot * C::SLOTK + in) * C::SLOT;
     #pragma unroll
                     for (int i = 0; i < 2; i++) ptx::cp_async4(to + t + 64 * i, srow[i] + kb * p.ld_sa);
@@ -369,9 +388,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                     if (!gather && warp != 0) continue;
-                    pipe.wait(&empty[stage], phase ^ 1);
+                    if (!pipe.wait(&empty[stage], phase ^ 1)) goto copied;
                     uint8_t* sa = smem + stage * C::STAGE;
                     if (t == 0) {
+                        loads++;
                         if (PAIR) {
                             // both CTAs' loads complete on the first one's barrier
                             const uint32_t bar = ptx::cluster_addr(&full[stage], 0);
@@ -412,16 +432,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ptx::cp_async_arrive(landed);
                 }
             }
-            ptx::cp_async_wait_all();
             // every load has landed and been used before the CTA exits (bounded)
             if (t == 0)
                 for (int s = 0; s < C::STAGES; s++) {
-                    pipe.wait(&empty[stage], phase ^ 1);
+                    if (!pipe.wait(&empty[stage], phase ^ 1)) break;
                     if (++stage == C::STAGES) {
                         stage = 0;
                         phase ^= 1;
                     }
                 }
+        copied:
+            ptx::cp_async_wait_all();
+            // or at least landed, where the CTA gave up (those of a pair's second
+            // CTA complete on the first one's barriers, and the two leave together)
+            if (t == 0 && rank == 0) pipe.drain(full, C::STAGES, loads, C::STAGES);
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -873,12 +897,12 @@ __global__ void __launch_bounds__(kSmallThreads, SmallCfg<BN, VEC>::CTAS)
     if (warp == 0) {
         if (lane == 0) {
             const Pipe pipe{dead, p.err, kErrTimeoutProducer};
-            int stage = 0;
+            int stage = 0, loads = 0;
             uint32_t phase = 0;
             for (int u = first; u < total; u += stride) {
                 const Unit w = small_unit<BN>(p, start, u);
-                for (int kb = kb0; kb < kb1; kb++) {
-                    pipe.wait(&empty[stage], phase ^ 1);
+                for (int kb = kb0; kb < kb1; kb++, loads++) {
+                    if (!pipe.wait(&empty[stage], phase ^ 1)) goto loaded;
                     ptx::mbar_arrive_expect_tx(&full[stage], C::W_BYTES);
                     ptx::tma_load_3d(smem + stage * C::STAGE, &tw, &full[stage], kb * 128, w.n0, w.g);
                     if (++stage == C::STAGES) {
@@ -889,12 +913,14 @@ __global__ void __launch_bounds__(kSmallThreads, SmallCfg<BN, VEC>::CTAS)
             }
             // every load has landed and been used before the CTA exits (bounded)
             for (int s = 0; s < C::STAGES; s++) {
-                pipe.wait(&empty[stage], phase ^ 1);
+                if (!pipe.wait(&empty[stage], phase ^ 1)) break;
                 if (++stage == C::STAGES) {
                     stage = 0;
                     phase ^= 1;
                 }
             }
+        loaded:
+            pipe.drain(full, C::STAGES, loads, C::STAGES);  // or at least landed, where the CTA gave up
         }
         __syncwarp();
     } else if (warp == 1 || warp == 8) {
@@ -902,12 +928,14 @@ __global__ void __launch_bounds__(kSmallThreads, SmallCfg<BN, VEC>::CTAS)
             const Pipe pipe{dead, p.err, kErrTimeoutMma};
             const int mine = warp == 1 ? 0 : 1;
             int it = 0;  // k-blocks so far: number `it` uses stage it % STAGES and part it % PARTS
+            int last = -1;
             for (int u = first; u < total; u += stride)
                 for (int kb = kb0; kb < kb1; kb++, it++) {
                     if ((it & 1) != mine) continue;
                     const int stage = it % C::STAGES, part = it % C::PARTS;
-                    pipe.wait(&full[stage], it / C::STAGES & 1);
-                    pipe.wait(&part_empty[part], (it / C::PARTS & 1) ^ 1);
+                    if (!pipe.wait(&full[stage], it / C::STAGES & 1)) goto issued;
+                    if (!pipe.wait(&part_empty[part], (it / C::PARTS & 1) ^ 1)) goto issued;
+                    last = it;
                     ptx::fence_proxy_async();  // A's rows came through the generic proxy
                     ptx::tc_fence_after();
                     const uint32_t sw = ptx::smem_u32(smem + stage * C::STAGE), sa = sw + C::W_BYTES;
@@ -918,6 +946,11 @@ __global__ void __launch_bounds__(kSmallThreads, SmallCfg<BN, VEC>::CTAS)
                     ptx::mma_commit(&empty[stage]);
                     ptx::mma_commit(&part_full[part]);
                 }
+        issued:
+            // the MMAs are done before TMEM is freed (else the scaling warps have
+            // waited for them)
+            pipe.drain(empty, C::STAGES, last + 1, 1);
+            pipe.drain(part_full, C::PARTS, last + 1, 1);
         }
         __syncwarp();
     } else if (warp < 4) {
@@ -952,7 +985,7 @@ __global__ void __launch_bounds__(kSmallThreads, SmallCfg<BN, VEC>::CTAS)
             if (!VEC) sb += (long long)(w.n0 / 128) * p.ld_sb;
             for (int kb = kb0; kb < kb1; kb++) {
                 const int in = (kb - kb0) % C::SLOTK;
-                if (in == 0) pipe.wait(&slot_empty[slot], slot_phase ^ 1);
+                if (in == 0 && !pipe.wait(&slot_empty[slot], slot_phase ^ 1)) goto copied;
                 float* to = slots + (slot * C::SLOTK + in) * C::SLOT;
                 if (t < BN) ptx::cp_async4(to + t, srow + kb * p.ld_sa);
                 if (VEC) {
@@ -971,7 +1004,7 @@ __global__ void __launch_bounds__(kSmallThreads, SmallCfg<BN, VEC>::CTAS)
                         slot_phase ^= 1;
                     }
                 }
-                pipe.wait(&empty[stage], phase ^ 1);
+                if (!pipe.wait(&empty[stage], phase ^ 1)) goto copied;
                 uint8_t* sa = smem + stage * C::STAGE + C::W_BYTES;
                 const int k = kb * 128 + (t & 7) * 16;
                 const int bytes = max(0, min(16, p.K - k));
@@ -989,6 +1022,7 @@ __global__ void __launch_bounds__(kSmallThreads, SmallCfg<BN, VEC>::CTAS)
                 }
             }
         }
+    copied:
         ptx::cp_async_wait_all();
         __syncwarp();
     } else {
