@@ -221,22 +221,22 @@ def _refuse(t, what, dtype, shape):
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{what}: shape {tuple(t.shape)} where {tuple(shape)} is wanted")
     if t.get_device() != _device():
-        raise ValueError(f"{what}: on {t.device}, where the current CUDA device ({_device()}), whose kernels run, is wanted")
+        raise ValueError(f"{what}: on {t.device}, but the kernels run on the current CUDA device, {_device()}")
     raise ValueError(f"{what}: strides {t.stride()} are not those of contiguous rows (or of a dense tensor where one is "
                      "wanted)")
 
 
-def _dense(t, what, dtype, shape):
-    """Address of a tensor of this dtype and shape without gaps, on the current device."""
-    if t.dtype is not dtype or t.shape != shape or t.get_device() != _device() or not t.is_contiguous():
+def _dense(d, t, what, dtype, shape):
+    """Address of a tensor of this dtype and shape without gaps, on device d."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != d or not t.is_contiguous():
         _refuse(t, what, dtype, shape)
     return t.data_ptr()
 
 
-def _rows(t, what, dtype, rows, cols):
-    """Address and leading dimension of a matrix of this dtype and shape, on the current device, whose rows are
+def _rows(d, t, what, dtype, rows, cols):
+    """Address and leading dimension of a matrix of this dtype and shape, on device d, whose rows are
     contiguous. (torch does not look at the stride of a single row; the kernels do.)"""
-    if t.dtype is not dtype or t.shape != (rows, cols) or t.get_device() != _device():
+    if t.dtype is not dtype or t.shape != (rows, cols) or t.get_device() != d:
         _refuse(t, what, dtype, (rows, cols))
     ld, one = t.stride()
     if one != 1 and cols > 1:
@@ -244,24 +244,24 @@ def _rows(t, what, dtype, rows, cols):
     return t.data_ptr(), ld if rows > 1 else max(ld, cols)
 
 
-def _float(t, what, rows, cols):
+def _float(d, t, what, rows, cols):
     """As _rows, fp32 or bf16: address, type code and leading dimension."""
     dt = t.dtype
     if dt is not _f32 and dt is not _bf16:
         raise ValueError(f"{what}: {dt} where float32 or bfloat16 is wanted")
-    at, ld = _rows(t, what, dt, rows, cols)
+    at, ld = _rows(d, t, what, dt, rows, cols)
     return at, F32 if dt is _f32 else BF16, ld
 
 
-def _codes(t, what, rows, cols):
+def _codes(d, t, what, rows, cols):
     """As _rows for codes, whose rows start on 16-byte boundaries."""
-    at, ld = _rows(t, what, _f8, rows, cols)
+    at, ld = _rows(d, t, what, _f8, rows, cols)
     return at, ld if rows > 1 else -(-cols // 16) * 16
 
 
-def _stack(t, what, dtype, n, rows, cols):
+def _stack(d, t, what, dtype, n, rows, cols):
     """As _rows for n matrices: address, leading dimension and the stride from one to the next."""
-    if t.dtype is not dtype or t.shape != (n, rows, cols) or t.get_device() != _device():
+    if t.dtype is not dtype or t.shape != (n, rows, cols) or t.get_device() != d:
         _refuse(t, what, dtype, (n, rows, cols))
     apart, ld, one = t.stride()
     if one != 1 and cols > 1:
@@ -269,22 +269,18 @@ def _stack(t, what, dtype, n, rows, cols):
     return t.data_ptr(), ld if rows > 1 else max(ld, -(-cols // 16) * 16 if dtype is _f8 else cols), apart
 
 
-def _here():
-    """The current stream."""
-    return _stream_of(_device())
-
-
 def moe_topk_route(logits, idx, w, score="softmax", bias=None, active=None, groups=1, topk_groups=1, renorm=True,
                    scale=1.0):
     """idx, w [M, k] (int32, float32) <- the k experts of each row of logits [M, E] and their weights."""
     lib = _bound if _f32 else _torch()
+    d = _device()
     M, E = logits.shape
     k = idx.shape[1]
     rc = lib.nsb_op_moe_topk_route(
-        *_float(logits, "logits", M, E), M, E, k, _SCORE[score],
-        None if bias is None else _dense(bias, "bias", _f32, (E,)),
-        None if active is None else _dense(active, "active", _u8, (E,)), groups, topk_groups, renorm, scale,
-        _dense(idx, "idx", _i32, (M, k)), _dense(w, "w", _f32, (M, k)), _here())
+        *_float(d, logits, "logits", M, E), M, E, k, _SCORE[score],
+        None if bias is None else _dense(d, bias, "bias", _f32, (E,)),
+        None if active is None else _dense(d, active, "active", _u8, (E,)), groups, topk_groups, renorm, scale,
+        _dense(d, idx, "idx", _i32, (M, k)), _dense(d, w, "w", _f32, (M, k)), _stream_of(d))
     if rc:
         _check(rc, "nsb_op_moe_topk_route")
 
@@ -292,12 +288,13 @@ def moe_topk_route(logits, idx, w, score="softmax", bias=None, active=None, grou
 def moe_topk_route_bwd(dw, logits, idx, dlogits, score="softmax", active=None, renorm=True, scale=1.0):
     """dlogits [M, E] (the logits' type) <- the gradient of moe_topk_route's w."""
     lib = _bound if _f32 else _torch()
+    d = _device()
     M, E = logits.shape
     k = idx.shape[1]
     rc = lib.nsb_op_moe_topk_route_bwd(
-        _dense(dw, "dw", _f32, (M, k)), *_float(logits, "logits", M, E), M, E, k, _SCORE[score],
-        None if active is None else _dense(active, "active", _u8, (E,)), renorm, scale,
-        _dense(idx, "idx", _i32, (M, k)), *_rows(dlogits, "dlogits", logits.dtype, M, E), _here())
+        _dense(d, dw, "dw", _f32, (M, k)), *_float(d, logits, "logits", M, E), M, E, k, _SCORE[score],
+        None if active is None else _dense(d, active, "active", _u8, (E,)), renorm, scale,
+        _dense(d, idx, "idx", _i32, (M, k)), *_rows(d, dlogits, "dlogits", logits.dtype, M, E), _stream_of(d))
     if rc:
         _check(rc, "nsb_op_moe_topk_route_bwd")
 
@@ -310,12 +307,13 @@ def moe_dispatch_rows(M, k, E, align=1) -> int:
 def moe_dispatch(idx, E, offsets, counts, rows, pos, align=1):
     """offsets [E + 1], counts [E], rows [moe_dispatch_rows(...)], pos [M, k] (int32) <- the pairs of idx by expert."""
     lib = _bound if _f32 else _torch()
+    d = _device()
     M, k = idx.shape
     rc = lib.nsb_op_moe_dispatch(
-        _dense(idx, "idx", _i32, (M, k)), M, k, E, align, _dense(offsets, "offsets", _i32, (E + 1,)),
-        _dense(counts, "counts", _i32, (E,)),
-        _dense(rows, "rows", _i32, (lib.nsb_op_moe_dispatch_rows(M, k, E, align),)), _dense(pos, "pos", _i32, (M, k)),
-        _here())
+        _dense(d, idx, "idx", _i32, (M, k)), M, k, E, align, _dense(d, offsets, "offsets", _i32, (E + 1,)),
+        _dense(d, counts, "counts", _i32, (E,)),
+        _dense(d, rows, "rows", _i32, (lib.nsb_op_moe_dispatch_rows(M, k, E, align),)),
+        _dense(d, pos, "pos", _i32, (M, k)), _stream_of(d))
     if rc:
         _check(rc, "nsb_op_moe_dispatch")
 
@@ -324,11 +322,13 @@ def moe_combine(o, pos, y, w=None):
     """y [M, D] <- sum over j of w[:, j] * o[pos[:, j]] (w None: 1). Negative entries of pos are left out, and so are
     those past o's rows, which check_errors raises."""
     lib = _bound if _f32 else _torch()
+    d = _device()
     M, k = pos.shape
     R, D = o.shape
     rc = lib.nsb_op_moe_combine_rows(
-        *_float(o, "o", R, D), R, _dense(pos, "pos", _i32, (M, k)),
-        None if w is None else _dense(w, "w", _f32, (M, k)), M, k, D, *_rows(y, "y", o.dtype, M, D), _here())
+        *_float(d, o, "o", R, D), R, _dense(d, pos, "pos", _i32, (M, k)),
+        None if w is None else _dense(d, w, "w", _f32, (M, k)), M, k, D, *_rows(d, y, "y", o.dtype, M, D),
+        _stream_of(d))
     if rc:
         _check(rc, "nsb_op_moe_combine_rows")
 
@@ -336,17 +336,18 @@ def moe_combine(o, pos, y, w=None):
 def moe_combine_bwd(dy, o, rows, pos, w, do, dw=None):
     """do [R, D], dw [M, k] <- the gradients of moe_combine's o and w (dw None: do alone; o may be None then)."""
     lib = _bound if _f32 else _torch()
+    d = _device()
     M, k = pos.shape
     D = dy.shape[1]
     R = rows.shape[0]
     if dw is not None and o is None:
         raise ValueError("dw needs o")
-    at, dt, ld = _float(dy, "dy", M, D)
-    o_at, o_ld = (None, 0) if o is None else _rows(o, "o", dy.dtype, R, D)
+    at, dt, ld = _float(d, dy, "dy", M, D)
+    o_at, o_ld = (None, 0) if o is None else _rows(d, o, "o", dy.dtype, R, D)
     rc = lib.nsb_op_moe_combine_bwd(
-        at, o_at, dt, ld, o_ld, _dense(rows, "rows", _i32, (R,)), _dense(pos, "pos", _i32, (M, k)),
-        None if w is None else _dense(w, "w", _f32, (M, k)), M, k, R, D, *_rows(do, "do", dy.dtype, R, D),
-        None if dw is None else _dense(dw, "dw", _f32, (M, k)), _here())
+        at, o_at, dt, ld, o_ld, _dense(d, rows, "rows", _i32, (R,)), _dense(d, pos, "pos", _i32, (M, k)),
+        None if w is None else _dense(d, w, "w", _f32, (M, k)), M, k, R, D, *_rows(d, do, "do", dy.dtype, R, D),
+        None if dw is None else _dense(d, dw, "dw", _f32, (M, k)), _stream_of(d))
     if rc:
         _check(rc, "nsb_op_moe_combine_bwd")
 
@@ -366,14 +367,16 @@ def fp8_quantize(x, q=None, s=None, qt=None, st=None, act=0, rows=None, row_div=
     (row_div 0: only puts zeros where rows is negative); an entry past x's rows gives zeros, and check_errors raises
     it."""
     lib = _bound if _f32 else _torch()
+    d = _device()
     n, K = x.shape
     M = n if rows is None else rows.shape[0]
     if rows is not None and row_div == 0 and n < M:
         raise ValueError(f"x: {n} rows where {M} are wanted")
     rc = lib.nsb_op_fp8_quantize_rows(
-        *_float(x, "x", n, K), n, M, K, act, None if rows is None else _dense(rows, "rows", _i32, (M,)), row_div,
-        *(_NOTHING if q is None else _codes(q, "q", M, K) + _rows(s, "s", _f32, -(-K // 128), M)),
-        *(_NOTHING if qt is None else _codes(qt, "qt", K, M) + _rows(st, "st", _f32, -(-M // 128), K)), _here())
+        *_float(d, x, "x", n, K), n, M, K, act, None if rows is None else _dense(d, rows, "rows", _i32, (M,)), row_div,
+        *(_NOTHING if q is None else _codes(d, q, "q", M, K) + _rows(d, s, "s", _f32, -(-K // 128), M)),
+        *(_NOTHING if qt is None else _codes(d, qt, "qt", K, M) + _rows(d, st, "st", _f32, -(-M // 128), K)),
+        _stream_of(d))
     if rc:
         _check(rc, "nsb_op_fp8_quantize_rows")
 
@@ -381,27 +384,29 @@ def fp8_quantize(x, q=None, s=None, qt=None, st=None, act=0, rows=None, row_div=
 def fp8_quantize_block(x, q=None, s=None, qt=None, st=None):
     """q [M, K] with s [ceil(M / 128), ceil(K / 128)], and / or their transposes qt, st <- codes and scales of x."""
     lib = _bound if _f32 else _torch()
+    d = _device()
     M, K = x.shape
     mb, kb = -(-M // 128), -(-K // 128)
     rc = lib.nsb_op_fp8_quantize_block(
-        *_float(x, "x", M, K), M, K,
-        *(_NOTHING if q is None else _codes(q, "q", M, K) + _rows(s, "s", _f32, mb, kb)),
-        *(_NOTHING if qt is None else _codes(qt, "qt", K, M) + _rows(st, "st", _f32, kb, mb)), _here())
+        *_float(d, x, "x", M, K), M, K,
+        *(_NOTHING if q is None else _codes(d, q, "q", M, K) + _rows(d, s, "s", _f32, mb, kb)),
+        *(_NOTHING if qt is None else _codes(d, qt, "qt", K, M) + _rows(d, st, "st", _f32, kb, mb)), _stream_of(d))
     if rc:
         _check(rc, "nsb_op_fp8_quantize_block")
 
 
-def _word(err):
+def _word(d, err):
     """Address of a caller's error word; None for the device's own."""
-    return None if err is None else _dense(err, "err", _i32, (1,))
+    return None if err is None else _dense(d, err, "err", _i32, (1,))
 
 
 def check_errors():
     """Waits for the current stream and raises RuntimeError where since the last call a product without an `err` of
     its own gave up a bounded wait (its result is not to be used), or an index was past its tensor's rows."""
     lib = _bound if _f32 else _torch()
+    d = _device()
     code = C.c_int(0)
-    _check(lib.nsb_op_device_error(C.byref(code), _here()), "nsb_op_device_error")
+    _check(lib.nsb_op_device_error(C.byref(code), _stream_of(d)), "nsb_op_device_error")
     if code.value:
         why = "an index past its tensor's rows" if code.value == 111 else "a product's wait ran out"
         raise RuntimeError(f"device error {code.value} since the last check: {why}")
@@ -413,15 +418,16 @@ def gemm_fp8(a, sa, b, sb, c, err=None):
     N = 1 and K at most 128). err (one int32): receives the code of a wait that ran out, in place of the word that
     check_errors reads."""
     lib = _bound if _f32 else _torch()
+    d = _device()
     M, K = a.shape
     N = b.shape[0]
     kb = -(-K // 128)
     by_rows = sb.shape == (kb, N)
-    at, dt, ld = _float(c, "c", M, N)
+    at, dt, ld = _float(d, c, "c", M, N)
     rc = lib.nsb_op_gemm_fp8(
-        M, N, K, *_codes(a, "a", M, K), *_rows(sa, "sa", _f32, kb, M), *_codes(b, "b", N, K),
-        *(_rows(sb, "sb", _f32, kb, N) if by_rows else _rows(sb, "sb", _f32, -(-N // 128), kb)), by_rows, at, dt, ld,
-        _word(err), _here())
+        M, N, K, *_codes(d, a, "a", M, K), *_rows(d, sa, "sa", _f32, kb, M), *_codes(d, b, "b", N, K),
+        *(_rows(d, sb, "sb", _f32, kb, N) if by_rows else _rows(d, sb, "sb", _f32, -(-N // 128), kb)), by_rows,
+        at, dt, ld, _word(d, err), _stream_of(d))
     if rc:
         _check(rc, "nsb_op_gemm_fp8")
 
@@ -430,17 +436,18 @@ def moe_gemm_fp8(a, sa, offsets, counts, b, sb, c, rows=None, row_div=1, err=Non
     """Rows of c [R, N] of each expert e <- those of A times B[e]^T: a [R, K] (with rows [R]: [any, K], of which
     row r takes rows[r] / row_div) with row scales sa, b [E, N, K] with block scales sb."""
     lib = _bound if _f32 else _torch()
+    d = _device()
     n, K = a.shape
     E, N, _ = b.shape
     R = c.shape[0]
     kb = -(-K // 128)
-    at, dt, ld = _float(c, "c", R, N)
+    at, dt, ld = _float(d, c, "c", R, N)
     rc = lib.nsb_op_moe_gemm_fp8(
-        R, E, N, K, *_codes(a, "a", n if rows is not None else R, K), n, *_rows(sa, "sa", _f32, kb, n),
-        None if rows is None else _dense(rows, "rows", _i32, (R,)), row_div,
-        _dense(offsets, "offsets", _i32, (E + 1,)), _dense(counts, "counts", _i32, (E,)),
-        *_stack(b, "b", _f8, E, N, K), *_stack(sb, "sb", _f32, E, -(-N // 128), kb), at, dt, ld,
-        _word(err), _here())
+        R, E, N, K, *_codes(d, a, "a", n if rows is not None else R, K), n, *_rows(d, sa, "sa", _f32, kb, n),
+        None if rows is None else _dense(d, rows, "rows", _i32, (R,)), row_div,
+        _dense(d, offsets, "offsets", _i32, (E + 1,)), _dense(d, counts, "counts", _i32, (E,)),
+        *_stack(d, b, "b", _f8, E, N, K), *_stack(d, sb, "sb", _f32, E, -(-N // 128), kb), at, dt, ld,
+        _word(d, err), _stream_of(d))
     if rc:
         _check(rc, "nsb_op_moe_gemm_fp8")
 
@@ -448,17 +455,18 @@ def moe_gemm_fp8(a, sa, offsets, counts, b, sb, c, rows=None, row_div=1, err=Non
 def moe_wgrad_fp8(a, sa, b, sb, offsets, counts, c, err=None):
     """c [E, M, N] <- for each expert the sum over its columns of a [M, R] and b [N, R] (row scales sa, sb)."""
     lib = _bound if _f32 else _torch()
+    d = _device()
     M, R = a.shape
     N = b.shape[0]
     E = c.shape[0]
     rb = -(-R // 128)
     if c.dtype is not _f32 and c.dtype is not _bf16:
         raise ValueError(f"c: {c.dtype} where float32 or bfloat16 is wanted")
-    at, ld, apart = _stack(c, "c", c.dtype, E, M, N)
+    at, ld, apart = _stack(d, c, "c", c.dtype, E, M, N)
     rc = lib.nsb_op_moe_wgrad_fp8(
-        M, N, R, E, *_codes(a, "a", M, R), *_rows(sa, "sa", _f32, rb, M), *_codes(b, "b", N, R),
-        *_rows(sb, "sb", _f32, rb, N), _dense(offsets, "offsets", _i32, (E + 1,)),
-        _dense(counts, "counts", _i32, (E,)), at, F32 if c.dtype is _f32 else BF16, ld, apart,
-        _word(err), _here())
+        M, N, R, E, *_codes(d, a, "a", M, R), *_rows(d, sa, "sa", _f32, rb, M), *_codes(d, b, "b", N, R),
+        *_rows(d, sb, "sb", _f32, rb, N), _dense(d, offsets, "offsets", _i32, (E + 1,)),
+        _dense(d, counts, "counts", _i32, (E,)), at, F32 if c.dtype is _f32 else BF16, ld, apart,
+        _word(d, err), _stream_of(d))
     if rc:
         _check(rc, "nsb_op_moe_wgrad_fp8")
