@@ -45,7 +45,7 @@ class MoETopk:
         draw = lambda *s: torch.randn(*s, device="cuda", generator=g) / s[-1] ** 0.5  # noqa: E731
         self.gate, self.w1, self.w2 = draw(E, D), draw(E, H, D), draw(E, D, H)
         self.step = 0
-        self.err = torch.zeros(1, dtype=torch.int32, device="cuda")  # the gate's products'
+        self.err = torch.zeros(1, dtype=torch.int32, device="cuda")  # of all its products
         self._moments = [(torch.zeros_like(w), torch.zeros_like(w)) for w in (self.gate, self.w1, self.w2)]
         self.refresh()
 
@@ -68,15 +68,15 @@ class MoETopk:
     def check(self):
         """Waits for the current stream and raises RuntimeError where a product gave up a bounded wait since the last
         check. train_step calls it; who serves calls it where the results are read."""
-        ops.check_errors()
         code = int(self.err)
         if code:
             self.err.zero_()
-            raise RuntimeError(f"device error {code} in the gate's product")
+            raise RuntimeError(f"device error {code} in a product of the layer")
 
     def _product(self, a, sa, order, b, N, rows=None):
         out = torch.zeros(order["rows"].numel(), N, device="cuda")
-        ops.moe_gemm_fp8(a, sa, order["offsets"], order["counts"], *b, out, rows=rows, row_div=self.k)
+        ops.moe_gemm_fp8(a, sa, order["offsets"], order["counts"], *b, out, rows=rows, row_div=self.k,
+                         err=self.err)
         return out
 
     def forward(self, x, align=1):
@@ -130,13 +130,13 @@ class MoETopk:
         (dq, ds), dt = both(do, 0)
         _, ht = both(kept["z"], 0, act=GELU, by_rows=False)
         dw2 = _floats(E, D, H)
-        ops.moe_wgrad_fp8(*dt, *ht, order["offsets"], order["counts"], dw2)
+        ops.moe_wgrad_fp8(*dt, *ht, order["offsets"], order["counts"], dw2, err=self.err)
         dz = _floats(R, H)
         ops.act_bwd(self._product(dq, ds, order, self.q2t, H), kept["z"], GELU, dz)
         (zq, zs), zt = both(dz, 0)
         _, xt = both(x, k, by_rows=False)
         dw1 = _floats(E, H, D)
-        ops.moe_wgrad_fp8(*zt, *xt, order["offsets"], order["counts"], dw1)
+        ops.moe_wgrad_fp8(*zt, *xt, order["offsets"], order["counts"], dw1, err=self.err)
         dx = _floats(M, D)
         ops.moe_combine(self._product(zq, zs, order, self.q1t, D), order["pos"], dx)
         x32 = x.float()
