@@ -561,6 +561,7 @@ __global__ void __launch_bounds__(128)
     const size_t t = blockIdx.x;
     const int c = (blockIdx.y * blockDim.x + threadIdx.x) * W;
     if (c >= D) return;
+    bool past = false;
     float acc[W];
 #pragma unroll
     for (int i = 0; i < W; i++) acc[i] = 0.f;
@@ -571,10 +572,8 @@ __global__ void __launch_bounds__(128)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             p[j] = j0 + j < k ? pos[t * k + j0 + j] : -1;
-            if (p[j] >= R) {
-                if (err) atomicCAS(err, 0, kErrBadIndex);
-                p[j] = -1;
-            }
+            past |= p[j] >= R;
+            if (p[j] >= R) p[j] = -1;
             wj[j] = p[j] >= 0 && w ? w[t * k + j0 + j] : 1.f;
         }
 #pragma unroll
@@ -590,6 +589,7 @@ __global__ void __launch_bounds__(128)
         }
     }
     Cols<T, W>::store(y + t * ld_y + c, acc);
+    if (past && err) atomicCAS(err, 0, kErrBadIndex);
 }
 
 // One warp a row of the ordered outputs: o and d_o stream, the tokens' dy,
