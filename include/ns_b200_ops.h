@@ -285,8 +285,9 @@ int nsb_op_fp8_quantize_block(const void* x, int dtype, long long ld, int M, int
 int nsb_op_device_error(int* code, void* stream);
 
 /* C[M,N] = A[M,K] B[N,K]^T of the values that codes and scales stand for:
- * exact products, fp32 sums over 128 k, these scaled and added in fp32,
- * rounded once to c_dtype. A has row scales; B 128 x 128 scales (b_rows 0: a
+ * exact products, fp32 sums over 128 k, these scaled and added in fp32 (the
+ * product of two blocks' scales is to be a finite fp32 number), rounded once
+ * to c_dtype. A has row scales; B 128 x 128 scales (b_rows 0: a
  * weight; its transposed codes serve the input gradient) or row scales
  * (b_rows 1: the weight gradient, from two transposed quantisations). */
 int nsb_op_gemm_fp8(int M, int N, int K, const void* A, long long lda, const float* sa, long long ld_sa,

@@ -36,9 +36,12 @@ namespace {
 //   warps 4..11  a warp owns 32 rows and half the columns: scales and adds
 //                every k-block's part, stores the tile
 // The scaling bounds it: a k-block of 128 x 256 takes the tensor cores 512
-// cycles and the eight warps about 1080, most of them the latencies of eight
-// reads of TMEM, each behind the FMAs of the one before. 8192 x 4096 x 4096
-// into bf16: 133 us, 2.07 PFLOP/s; under the power cap 158.
+// cycles and the eight warps about 1080, in which each issues some 220
+// instructions, 64 of them packed FMAs. 8192 x 4096 x 4096 into bf16: 133 us,
+// 2.07 PFLOP/s; under the power cap 155 to 160. In copies of the kernel: 131 us
+// with the FMAs but no reads of TMEM, 116 with the reads alone, 108 with
+// neither, where 84 would be the tensor cores' (at twice the bf16 rate); what
+// holds the 108 is not known.
 // The accumulators of a 128 x 256 tile are 128 registers a thread, so the
 // first four warps give theirs up: 72 + 2 * 216 of the 3 * 168 registers that
 // the three warpgroups are launched with.
@@ -1350,7 +1353,11 @@ int fp8_gemm(const Fp8Gemm& d, cudaStream_t st) {
     if (d.a_rows <= 0) return -1;
     const int sms = num_sms();
     const int rows = d.groups && !d.group_k ? (d.M + d.groups - 1) / d.groups : d.M;
-    // Few rows: the weights' stream bounds the product. (One product of 4096 x
+    // Few rows: the weights' stream bounds the product. Of groups the host knows
+    // the rows of C, padding included, not their numbers, so segments that start
+    // on multiples of 128 count as full ones and take the tiles (608 x 4 of 64
+    // experts, 1024 x 2048, 38 rows each: 94 us there, 40 without padding).
+    // (One product of 4096 x
     // 4096: 16 rows 8.3 us here and 9.7 on tiles, 24 rows 9.4 and 10.5, 48 rows
     // 11.1 and 10.1; groups of 1024 x 2048 with 38 rows on average 40 us and 92,
     // with 100 rows 75 and 110, of 1024 x 1024 with 112 rows 19.8 and 22.3.)
