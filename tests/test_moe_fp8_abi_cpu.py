@@ -6,8 +6,6 @@ import pytest
 
 from neuralscript_b200 import ops
 
-torch = pytest.importorskip("torch")
-
 X = 0x10000  # an address that is never read
 
 
@@ -177,6 +175,7 @@ def test_bounded_entries_refuse():
 
 
 def test_missing_library_is_reported_by_every_call(monkeypatch):
+    torch = pytest.importorskip("torch")
     monkeypatch.setattr(ops, "_bound", None)
     monkeypatch.setattr(ops, "_f32", None)
 
@@ -206,7 +205,7 @@ class Far:
     """What the entries ask of a tensor, of one that no process here could hold."""
 
     def __init__(self, shape, dtype, device=0):
-        self.shape, self.dtype, self.device = torch.Size(shape), dtype, f"cuda:{device}"
+        self.shape, self.dtype, self.device = tuple(shape), dtype, f"cuda:{device}"
         self.at = device
 
     def get_device(self):
@@ -228,7 +227,8 @@ class Far:
 
 
 def calls():
-    """Every entry with all its tensors: (name, function of a device for each tensor, how many tensors)."""
+    """Every entry with shapes and types of all its tensors: (entry, arguments, named arguments)."""
+    torch = pytest.importorskip("torch")
     f, i, q, u, h = torch.float32, torch.int32, torch.float8_e4m3fn, torch.uint8, torch.bfloat16
     o = ops
     yield o.moe_topk_route, [((4, 16), f), ((4, 2), i), ((4, 2), f)], dict(bias=((16,), f), active=((16,), u))
