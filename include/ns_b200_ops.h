@@ -266,9 +266,9 @@ int nsb_op_moe_combine_bwd(const void* dy, const void* o, int dtype, long long l
 int nsb_op_fp8_quantize(const void* x, int dtype, long long ld, int M, int K, int act, const int* rows, int row_div,
                         void* q, long long ld_q, float* s, long long ld_s, void* qt, long long ld_qt, float* st,
                         long long ld_st, void* stream);
-/* The same where x has x_rows rows (at least M of them with row_div 0): an
- * entry of rows past them counts as a negative one, and is reported by
- * nsb_op_device_error (above, rows is trusted). */
+/* The same where x has x_rows rows (at least M of them without a row list or
+ * with row_div 0): an entry of rows past them counts as a negative one, and is
+ * reported by nsb_op_device_error (above, rows is trusted). */
 int nsb_op_fp8_quantize_rows(const void* x, int dtype, long long ld, int x_rows, int M, int K, int act, const int* rows,
                              int row_div, void* q, long long ld_q, float* s, long long ld_s, void* qt, long long ld_qt,
                              float* st, long long ld_st, void* stream);

@@ -307,7 +307,8 @@ template <bool BLOCK>
 int quantize(const QuantDesc& d, cudaStream_t st) {
     const bool f = d.dtype == kF32;
     if (d.M < 0 || d.K <= 0 || (!f && d.dtype != kBF16) || d.ld < d.K || d.act < 0 || d.act > kGeluMoe) return -1;
-    if (d.rows && (d.row_div < 0 || d.x_rows < (d.row_div ? 0 : d.M))) return -1;
+    if (d.rows && d.row_div < 0) return -1;
+    if (d.x_rows < (d.rows && d.row_div ? 0 : d.M)) return -1;
     if (d.M == 0) return 0;  // (what has no elements has no address)
     if (!d.x || (!d.q && !d.qt)) return -1;
     auto codes = [](const void* p, long long ld, int cols) {

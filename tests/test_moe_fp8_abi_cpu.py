@@ -172,6 +172,9 @@ def test_bounded_entries_refuse():
         a = list(ok)
         a[at] = v
         assert rc("nsb_op_fp8_quantize_rows", *a) == -1, at
+    a = list(ok)
+    a[3], a[7], a[8] = 3, None, 1  # no list: the rows themselves
+    assert rc("nsb_op_fp8_quantize_rows", *a) == -1
 
 
 def test_missing_library_is_reported_by_every_call(monkeypatch):
