@@ -312,6 +312,93 @@ int nsb_op_moe_wgrad_fp8(int M, int N, int R, int E, const void* A, long long ld
                          const int* counts, void* C, int c_dtype, long long ldc, long long c_stride, int* dev_err,
                          void* stream);
 
+/* ---- Attention that answers token by token (no reference counterpart: its
+ * attention is bidirectional, without positions, and keeps nothing between
+ * calls) --------------------------------------------------------------------
+ * Tensors of heads [rows, heads, dh]: `_row` and `_head` are the strides in
+ * elements from row to row and head to head, a head's columns lie side by
+ * side. Hq query heads share Hkv key heads (a divisor of Hq): query head h
+ * reads key head h / (Hq / Hkv). dtype is that of every tensor of heads.
+ *
+ * A cache of keys (of values) has `pages` pages of `page` places: place p of
+ * page n, head h, at n * _page + p * _slot + h * _head. table [B, ld_table]
+ * lists the pages of every sequence (`width` of them): key j of sequence b is
+ * at place j % page of page table[b, j / page]. */
+
+/* Rotary positions. Pair i < pairs of a head of x [T, H, dh] is columns
+ * (i, i + pairs), or (2 i, 2 i + 1) where interleaved, and becomes
+ *   scale * (x0 cos a - x1 sin a, x1 cos a + x0 sin a),  a = pos[axis, t] * freq[i],
+ * the angle in 64 bits. pos [axes, ld_pos] holds up to four coordinates of
+ * each token; the first sections[0] pairs turn by the first, the next
+ * sections[1] by the second and so on (sections: `axes` ints in host memory
+ * whose sum is pairs; NULL with one axis). Columns from 2 * pairs on are
+ * copied. y may be x. dh is even, at most 1024, H * dh at most 2^26. */
+int nsb_op_rope(const void* x, int dtype, long long x_row, long long x_head, int T, int H, int dh, const int* pos,
+                long long ld_pos, int axes, const int* sections, const float* freq, int pairs, int interleaved, float scale,
+                void* y, long long y_row, long long y_head, void* stream);
+/* Its gradient: dx from dy, the rotation back. */
+int nsb_op_rope_bwd(const void* dy, int dtype, long long dy_row, long long dy_head, int T, int H, int dh, const int* pos,
+                    long long ld_pos, int axes, const int* sections, const float* freq, int pairs, int interleaved,
+                    float scale, void* dx, long long dx_row, long long dx_head, void* stream);
+
+/* Keys k and values v [T, Hkv, dh] into their caches, token t at key at[t] of
+ * sequence seq[t], keys rotated as above on the way (pairs 0: as they are),
+ * and queries q [T, Hq, dh], rotated, to q_out (both may be NULL; q_out may be
+ * q). A token with a negative seq[t] is padding: nothing of it is read or
+ * written. One whose place is outside the table or the cache is left out too,
+ * and reported by nsb_op_device_error. No two tokens of one call go to the
+ * same place. */
+int nsb_op_kv_append(const void* k, long long k_row, long long k_head, const void* v, long long v_row, long long v_head,
+                     int dtype, int T, int Hkv, int dh, const int* seq, const int* at, const int* table, long long ld_table,
+                     int B, int width, int pages, int page, void* k_cache, long long kc_page, long long kc_slot,
+                     long long kc_head, void* v_cache, long long vc_page, long long vc_slot, long long vc_head,
+                     const int* pos, long long ld_pos, int axes, const int* sections, const float* freq, int pairs,
+                     int interleaved, float scale, const void* q, long long q_row, long long q_head, int Hq, void* q_out,
+                     long long qo_row, long long qo_head, void* stream);
+
+/* Attention of one new token a sequence: q, out [B, Hq, dh] over the first
+ * lens[b] keys of the cache (the new token's own among them),
+ *   out = sum_j p_j v_j,  p = softmax(scale * q . k_j),  lse = log sum_j exp(scale * q . k_j)
+ * over j < lens[b] and, where window > 0, j >= lens[b] - window or j < sinks.
+ * lse [B, Hq] may be NULL. Without a key (or with none but scores of -inf):
+ * zeros and -inf. A length that the table has no room for is cut, and a page
+ * outside the cache left out; both are reported by nsb_op_device_error. What
+ * the cache holds behind a sequence's end is not looked at. dh <= 128,
+ * B <= 8192, scale > 0. workspace (16-byte aligned) of at least
+ * nsb_op_attention_paged_workspace_bytes(...) bytes: of this call alone until
+ * it is done. */
+size_t nsb_op_attention_paged_workspace_bytes(int B, int Hq, int Hkv, int dh);
+int nsb_op_attention_paged(const void* q, long long q_row, long long q_head, int dtype, int B, int Hq, int Hkv, int dh,
+                           const void* k_cache, long long kc_page, long long kc_slot, long long kc_head, const void* v_cache,
+                           long long vc_page, long long vc_slot, long long vc_head, int pages, int page, const int* table,
+                           long long ld_table, int width, const int* lens, int window, int sinks, float scale, void* out,
+                           long long out_row, long long out_head, float* lse, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
+/* Causal attention of packed sequences: rows [offsets[b], offsets[b + 1]) of
+ * q, out [T, Hq, dh] and k, v [T, Hkv, dh] are sequence b (offsets [B + 1]
+ * rising from 0 on, at most T; NULL with B = 1: one of T rows), in which
+ * query i sees key j where
+ *   j <= i  and  (window == 0  or  i - j < window  or  j < sinks).
+ * lse [Hq, ld_lse] receives the log-sum-exp (may be NULL). Rows behind the
+ * last sequence are neither read nor written. Offsets that do not rise are
+ * cut and reported by nsb_op_device_error. dh <= 128, scale > 0. A value of a
+ * sequence that is infinite or NaN can reach its queries before it too. */
+int nsb_op_attention_window(const void* q, long long q_row, long long q_head, const void* k, long long k_row,
+                            long long k_head, const void* v, long long v_row, long long v_head, int dtype, int T, int Hq,
+                            int Hkv, int dh, const int* offsets, int B, int window, int sinks, float scale, void* out,
+                            long long out_row, long long out_head, float* lse, long long ld_lse, void* stream);
+/* Its gradients from dout, the forward pass's out and lse: dq, and dk, dv
+ * summed over the query heads that share a key head, in a fixed order. dvec:
+ * scratch of Hq * T floats. */
+int nsb_op_attention_window_bwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row,
+                                long long k_head, const void* v, long long v_row, long long v_head, int dtype, int T,
+                                int Hq, int Hkv, int dh, const int* offsets, int B, int window, int sinks, float scale,
+                                const void* out, long long out_row, long long out_head, const float* lse, long long ld_lse,
+                                const void* dout, long long do_row, long long do_head, void* dq, long long dq_row,
+                                long long dq_head, void* dk, long long dk_row, long long dk_head, void* dv,
+                                long long dv_row, long long dv_head, float* dvec, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,6 +5,7 @@
 
 #include "../../include/ns_b200_ops.h"
 #include "attention.h"
+#include "attention_cache.h"
 #include "elementwise.h"
 #include "engine.h"
 #include "fp8.h"
@@ -513,6 +514,193 @@ int nsb_op_moe_wgrad_fp8(int M, int N, int R, int E, const void* A, long long ld
     d.err = dev_err ? dev_err : op_error_word();
     launch_counter() += 1;
     return fp8_gemm(d, (cudaStream_t)stream);
+}
+
+static Heads heads(const void* p, long long row, long long head) {
+    Heads h;
+    h.p = const_cast<void*>(p);
+    h.row = row;
+    h.head = head;
+    return h;
+}
+static Pages cache(const void* p, long long page, long long slot, long long head) {
+    Pages c;
+    c.p = const_cast<void*>(p);
+    c.page = page;
+    c.slot = slot;
+    c.head = head;
+    return c;
+}
+
+// Sections become the pairs' ends, axis by axis; false where they do not add up.
+static bool make_turn(Turn* t, const int* pos, long long ld_pos, int axes, const int* sections, const float* freq, int pairs,
+                      int interleaved, float scale, float sign) {
+    t->n = pairs;
+    if (pairs == 0) return true;
+    if (axes < 1 || axes > kMaxAxes || (!sections && axes > 1)) return false;
+    long long end = 0;
+    for (int i = 0; i < axes; i++) {
+        if (sections && sections[i] < 0) return false;
+        end += sections ? sections[i] : pairs;
+        if (end > pairs) return false;
+        t->end[i] = (int)end;
+    }
+    t->pos = pos;
+    t->ld_pos = ld_pos;
+    t->axes = axes;
+    t->freq = freq;
+    t->interleaved = interleaved != 0;
+    t->scale = scale;
+    t->sign = sign;
+    return end == pairs;
+}
+
+static int turn_heads(const void* x, int dtype, long long x_row, long long x_head, int T, int H, int dh, const int* pos,
+                      long long ld_pos, int axes, const int* sections, const float* freq, int pairs, int interleaved,
+                      float scale, float sign, void* y, long long y_row, long long y_head, void* stream) {
+    Turn t;
+    if (!make_turn(&t, pos, ld_pos, axes, sections, freq, pairs, interleaved, scale, sign)) return -1;
+    launch_counter() += 1;
+    return rope(t, dtype, heads(x, x_row, x_head), heads(y, y_row, y_head), T, H, dh, (cudaStream_t)stream);
+}
+
+int nsb_op_rope(const void* x, int dtype, long long x_row, long long x_head, int T, int H, int dh, const int* pos,
+                long long ld_pos, int axes, const int* sections, const float* freq, int pairs, int interleaved, float scale,
+                void* y, long long y_row, long long y_head, void* stream) {
+    return turn_heads(x, dtype, x_row, x_head, T, H, dh, pos, ld_pos, axes, sections, freq, pairs, interleaved, scale, 1.f, y,
+                      y_row, y_head, stream);
+}
+
+int nsb_op_rope_bwd(const void* dy, int dtype, long long dy_row, long long dy_head, int T, int H, int dh, const int* pos,
+                    long long ld_pos, int axes, const int* sections, const float* freq, int pairs, int interleaved,
+                    float scale, void* dx, long long dx_row, long long dx_head, void* stream) {
+    return turn_heads(dy, dtype, dy_row, dy_head, T, H, dh, pos, ld_pos, axes, sections, freq, pairs, interleaved, scale,
+                      -1.f, dx, dx_row, dx_head, stream);
+}
+
+int nsb_op_kv_append(const void* k, long long k_row, long long k_head, const void* v, long long v_row, long long v_head,
+                     int dtype, int T, int Hkv, int dh, const int* seq, const int* at, const int* table, long long ld_table,
+                     int B, int width, int pages, int page, void* k_cache, long long kc_page, long long kc_slot,
+                     long long kc_head, void* v_cache, long long vc_page, long long vc_slot, long long vc_head,
+                     const int* pos, long long ld_pos, int axes, const int* sections, const float* freq, int pairs,
+                     int interleaved, float scale, const void* q, long long q_row, long long q_head, int Hq, void* q_out,
+                     long long qo_row, long long qo_head, void* stream) {
+    AppendDesc d;
+    if (!make_turn(&d.turn, pos, ld_pos, axes, sections, freq, pairs, interleaved, scale, 1.f)) return -1;
+    d.dtype = dtype;
+    d.T = T;
+    d.dh = dh;
+    d.Hkv = Hkv;
+    d.Hq = Hq;
+    d.k = heads(k, k_row, k_head);
+    d.v = heads(v, v_row, v_head);
+    d.q = heads(q, q_row, q_head);
+    d.q_out = heads(q_out, qo_row, qo_head);
+    d.seq = seq;
+    d.at = at;
+    d.table = table;
+    d.ld_table = ld_table;
+    d.B = B;
+    d.width = width;
+    d.pages = pages;
+    d.page = page;
+    d.kc = cache(k_cache, kc_page, kc_slot, kc_head);
+    d.vc = cache(v_cache, vc_page, vc_slot, vc_head);
+    d.err = op_error_word();
+    launch_counter() += 1;
+    return kv_append(d, (cudaStream_t)stream);
+}
+
+size_t nsb_op_attention_paged_workspace_bytes(int B, int Hq, int Hkv, int dh) {
+    return attention_paged_workspace(B, Hq, Hkv, dh);
+}
+
+int nsb_op_attention_paged(const void* q, long long q_row, long long q_head, int dtype, int B, int Hq, int Hkv, int dh,
+                           const void* k_cache, long long kc_page, long long kc_slot, long long kc_head, const void* v_cache,
+                           long long vc_page, long long vc_slot, long long vc_head, int pages, int page, const int* table,
+                           long long ld_table, int width, const int* lens, int window, int sinks, float scale, void* out,
+                           long long out_row, long long out_head, float* lse, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+    PagedDesc d;
+    d.dtype = dtype;
+    d.B = B;
+    d.Hq = Hq;
+    d.Hkv = Hkv;
+    d.dh = dh;
+    d.q = heads(q, q_row, q_head);
+    d.out = heads(out, out_row, out_head);
+    d.kc = cache(k_cache, kc_page, kc_slot, kc_head);
+    d.vc = cache(v_cache, vc_page, vc_slot, vc_head);
+    d.pages = pages;
+    d.page = page;
+    d.table = table;
+    d.ld_table = ld_table;
+    d.width = width;
+    d.lens = lens;
+    d.window = window;
+    d.sinks = sinks;
+    d.scale = scale;
+    d.lse = lse;
+    d.workspace = workspace;
+    d.workspace_bytes = workspace_bytes;
+    d.err = op_error_word();
+    launch_counter() += attention_paged_launches();
+    return attention_paged(d, (cudaStream_t)stream);
+}
+
+static WindowDesc make_window(const void* q, long long q_row, long long q_head, const void* k, long long k_row,
+                              long long k_head, const void* v, long long v_row, long long v_head, int dtype, int T, int Hq,
+                              int Hkv, int dh, const int* offsets, int B, int window, int sinks, float scale) {
+    WindowDesc d;
+    d.dtype = dtype;
+    d.T = T;
+    d.Hq = Hq;
+    d.Hkv = Hkv;
+    d.dh = dh;
+    d.offsets = offsets;
+    d.B = B;
+    d.window = window;
+    d.sinks = sinks;
+    d.scale = scale;
+    d.q = heads(q, q_row, q_head);
+    d.k = heads(k, k_row, k_head);
+    d.v = heads(v, v_row, v_head);
+    d.err = op_error_word();
+    return d;
+}
+
+int nsb_op_attention_window(const void* q, long long q_row, long long q_head, const void* k, long long k_row,
+                            long long k_head, const void* v, long long v_row, long long v_head, int dtype, int T, int Hq,
+                            int Hkv, int dh, const int* offsets, int B, int window, int sinks, float scale, void* out,
+                            long long out_row, long long out_head, float* lse, long long ld_lse, void* stream) {
+    WindowDesc d = make_window(q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, dtype, T, Hq, Hkv, dh, offsets, B,
+                               window, sinks, scale);
+    d.out = heads(out, out_row, out_head);
+    d.lse = lse;
+    d.ld_lse = ld_lse;
+    launch_counter() += 1;
+    return attention_window(d, (cudaStream_t)stream);
+}
+
+int nsb_op_attention_window_bwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row,
+                                long long k_head, const void* v, long long v_row, long long v_head, int dtype, int T,
+                                int Hq, int Hkv, int dh, const int* offsets, int B, int window, int sinks, float scale,
+                                const void* out, long long out_row, long long out_head, const float* lse, long long ld_lse,
+                                const void* dout, long long do_row, long long do_head, void* dq, long long dq_row,
+                                long long dq_head, void* dk, long long dk_row, long long dk_head, void* dv,
+                                long long dv_row, long long dv_head, float* dvec, void* stream) {
+    WindowDesc d = make_window(q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, dtype, T, Hq, Hkv, dh, offsets, B,
+                               window, sinks, scale);
+    d.out = heads(out, out_row, out_head);
+    d.lse = const_cast<float*>(lse);
+    d.ld_lse = ld_lse;
+    d.dout = heads(dout, do_row, do_head);
+    d.dq = heads(dq, dq_row, dq_head);
+    d.dk = heads(dk, dk_row, dk_head);
+    d.dv = heads(dv, dv_row, dv_head);
+    d.dvec = dvec;
+    launch_counter() += 2;
+    return attention_window_bwd(d, (cudaStream_t)stream);
 }
 
 }  // extern "C"

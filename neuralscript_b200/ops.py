@@ -9,6 +9,12 @@ from . import lib as _core_lib
 F32, BF16 = 0, 1
 AUTO, SIMT, TENSOR = 0, 1, 2
 
+# arguments that several entries have: a tensor of heads, a cache, a rotation, packed attention
+_heads_args = [C.c_void_p, C.c_longlong, C.c_longlong]
+_cache_args = [C.c_void_p] + [C.c_longlong] * 3
+_turn_args = [C.c_void_p, C.c_longlong, C.c_int, C.POINTER(C.c_int), C.c_void_p, C.c_int, C.c_int, C.c_float]
+_window_args = _heads_args * 3 + [C.c_int] * 5 + [C.c_void_p] + [C.c_int] * 3 + [C.c_float]
+
 _sigs = {
     "nsb_op_gemm": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_void_p,
                               C.c_int, C.c_longlong, C.c_int, C.c_float, C.c_void_p, C.c_longlong, C.c_int,
@@ -74,6 +80,19 @@ _sigs = {
     "nsb_op_moe_wgrad_fp8": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int] + [C.c_void_p, C.c_longlong] * 4
                              + [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_longlong, C.c_longlong, C.c_void_p,
                                 C.c_void_p]),
+    "nsb_op_rope": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_longlong, C.c_int, C.c_int, C.c_int] + _turn_args
+                    + _heads_args + [C.c_void_p]),
+    "nsb_op_rope_bwd": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_longlong, C.c_int, C.c_int, C.c_int] + _turn_args
+                        + _heads_args + [C.c_void_p]),
+    "nsb_op_kv_append": (C.c_int, _heads_args * 2 + [C.c_int] * 4 + [C.c_void_p] * 3 + [C.c_longlong] + [C.c_int] * 4
+                         + _cache_args * 2 + _turn_args + _heads_args + [C.c_int] + _heads_args + [C.c_void_p]),
+    "nsb_op_attention_paged_workspace_bytes": (C.c_size_t, [C.c_int] * 4),
+    "nsb_op_attention_paged": (C.c_int, _heads_args + [C.c_int] * 5 + _cache_args * 2
+                               + [C.c_int, C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_void_p, C.c_int, C.c_int,
+                                  C.c_float] + _heads_args + [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "nsb_op_attention_window": (C.c_int, _window_args + _heads_args + [C.c_void_p, C.c_longlong, C.c_void_p]),
+    "nsb_op_attention_window_bwd": (C.c_int, _window_args + _heads_args + [C.c_void_p, C.c_longlong] + _heads_args * 4
+                                    + [C.c_void_p, C.c_void_p]),
 }
 _bound = None
 
@@ -470,3 +489,189 @@ def moe_wgrad_fp8(a, sa, b, sb, offsets, counts, c, err=None):
         _word(d, err), _stream_of(d))
     if rc:
         _check(rc, "nsb_op_moe_wgrad_fp8")
+
+
+# ---------------------------------------------------------------------------
+# Attention that answers token by token: rotary positions, a paged cache of
+# keys and values, one new token over it, and packed sequences with a window.
+# Tensors of heads are [rows, heads, dh], fp32 or bf16, with any strides but a
+# head's columns side by side. Tensors that do not fit raise ValueError before
+# anything is launched; see include/ns_b200_ops.h for the definitions.
+# ---------------------------------------------------------------------------
+def _heads(d, t, what, dtype, rows, heads, dh):
+    """Address and strides (row, head) of a tensor of heads of this dtype and shape, on device d."""
+    if t.dtype is not dtype or t.shape != (rows, heads, dh) or t.get_device() != d:
+        _refuse(t, what, dtype, (rows, heads, dh))
+    row, head, one = t.stride()
+    if one != 1 and dh > 1:
+        _refuse(t, what, dtype, (rows, heads, dh))
+    return t.data_ptr(), row, head
+
+
+def _kind(t, what):
+    dt = t.dtype
+    if dt is not _f32 and dt is not _bf16:
+        raise ValueError(f"{what}: {dt} where float32 or bfloat16 is wanted")
+    return F32 if dt is _f32 else BF16
+
+
+def _ints(d, t, what, rows, cols):
+    """Address and leading dimension of an int32 matrix whose rows are contiguous."""
+    return _rows(d, t, what, _i32, rows, cols)
+
+
+_NO_TURN = (None, 0, 0, None, None, 0, 0, 1.0)
+
+
+def _turn(d, pos, freq, T, sections, interleaved, scale):
+    """The arguments of a rotation: pos [T] or [axes, T], freq [pairs], sections: pairs of each axis."""
+    if pos.dim() == 1:
+        pos = pos[None]
+    axes = pos.shape[0]
+    pairs = freq.shape[0]
+    at, ld = _ints(d, pos, "pos", axes, T)
+    if sections is None:
+        if axes != 1:
+            raise ValueError(f"pos has {axes} axes: sections say how many pairs belong to each")
+    else:
+        sections = tuple(sections)
+        if len(sections) != axes or sum(sections) != pairs or min(sections) < 0:
+            raise ValueError(f"sections {sections} where {axes} of sum {pairs} are wanted")
+        sections = (C.c_int * axes)(*sections)
+    return at, ld, axes, sections, _dense(d, freq, "freq", _f32, (pairs,)), pairs, interleaved, scale
+
+
+def _rope(name, x, pos, freq, y, sections, interleaved, scale):
+    lib = _bound if _f32 else _torch()
+    d = _device()
+    kind = _kind(x, "x")
+    T, H, dh = x.shape
+    at, row, head = _heads(d, x, "x", x.dtype, T, H, dh)
+    rc = getattr(lib, name)(at, kind, row, head, T, H, dh, *_turn(d, pos, freq, T, sections, interleaved, scale),
+                            *_heads(d, y, "y", x.dtype, T, H, dh), _stream_of(d))
+    if rc:
+        _check(rc, name)
+
+
+def rope(x, pos, freq, y, sections=None, interleaved=False, scale=1.0):
+    """y [T, H, dh] <- x with the pairs of its heads turned by pos * freq: pos [T] or [axes, T] (int32), freq [pairs]
+    (float32), a pair (i, i + pairs), or (2 i, 2 i + 1) where interleaved; sections: pairs of each axis. y may be x."""
+    _rope("nsb_op_rope", x, pos, freq, y, sections, interleaved, scale)
+
+
+def rope_bwd(dy, pos, freq, dx, sections=None, interleaved=False, scale=1.0):
+    """dx [T, H, dh] <- the gradient of rope's x. dx may be dy."""
+    _rope("nsb_op_rope_bwd", dy, pos, freq, dx, sections, interleaved, scale)
+
+
+def _pages(d, t, what, dtype, pages, page, heads, dh):
+    """Address and strides (page, place, head) of a cache."""
+    if t.dtype is not dtype or t.shape != (pages, page, heads, dh) or t.get_device() != d:
+        _refuse(t, what, dtype, (pages, page, heads, dh))
+    a, b, c, one = t.stride()
+    if one != 1 and dh > 1:
+        _refuse(t, what, dtype, (pages, page, heads, dh))
+    return t.data_ptr(), a, b, c
+
+
+def kv_append(k, v, seq, at, table, k_cache, v_cache, pos=None, freq=None, sections=None, interleaved=False, scale=1.0,
+              q=None, q_out=None):
+    """k, v [T, Hkv, dh] into k_cache, v_cache [pages, page, Hkv, dh] at key at[t] of sequence seq[t], by table [B, width]
+    (all int32); with freq the keys are turned as by rope, and q_out [T, Hq, dh] <- q turned. Tokens with a negative seq
+    are left out, and so are those without a place, which check_errors raises."""
+    lib = _bound if _f32 else _torch()
+    d = _device()
+    kind = _kind(k, "k")
+    dt = k.dtype
+    T, Hkv, dh = k.shape
+    B, width = table.shape
+    pages, page = k_cache.shape[:2]
+    if (q is None) != (q_out is None) or (pos is None) != (freq is None):
+        raise ValueError("q goes with q_out, and pos with freq")
+    Hq = 0 if q is None else q.shape[1]
+    rc = lib.nsb_op_kv_append(
+        *_heads(d, k, "k", dt, T, Hkv, dh), *_heads(d, v, "v", dt, T, Hkv, dh), kind, T, Hkv, dh,
+        _dense(d, seq, "seq", _i32, (T,)), _dense(d, at, "at", _i32, (T,)), *_ints(d, table, "table", B, width), B, width,
+        pages, page, *_pages(d, k_cache, "k_cache", dt, pages, page, Hkv, dh),
+        *_pages(d, v_cache, "v_cache", dt, pages, page, Hkv, dh),
+        *(_NO_TURN if freq is None else _turn(d, pos, freq, T, sections, interleaved, scale)),
+        *((None, 0, 0) if q is None else _heads(d, q, "q", dt, T, Hq, dh)), Hq,
+        *((None, 0, 0) if q is None else _heads(d, q_out, "q_out", dt, T, Hq, dh)), _stream_of(d))
+    if rc:
+        _check(rc, "nsb_op_kv_append")
+
+
+def attention_paged_workspace(B, Hq, Hkv, dh) -> int:
+    """Bytes that attention_paged works in."""
+    return L().nsb_op_attention_paged_workspace_bytes(B, Hq, Hkv, dh)
+
+
+def attention_paged(q, k_cache, v_cache, table, lens, out, lse=None, window=0, sinks=0, scale=None, workspace=None):
+    """out [B, Hq, dh] (and lse [B, Hq]) <- attention of one token a sequence, q [B, Hq, dh], over the first lens[b] keys
+    of caches [pages, page, Hkv, dh] by table [B, width]: with window the last `window` of them and the first `sinks`.
+    scale: 1 / sqrt(dh). workspace (uint8): attention_paged_workspace(...) bytes, allocated where it is not given."""
+    import torch
+    lib = _bound if _f32 else _torch()
+    d = _device()
+    kind = _kind(q, "q")
+    dt = q.dtype
+    B, Hq, dh = q.shape
+    pages, page, Hkv, _ = k_cache.shape
+    width = table.shape[1]
+    need = lib.nsb_op_attention_paged_workspace_bytes(B, Hq, Hkv, dh)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=_u8, device=q.device)
+    have = workspace.numel()
+    rc = lib.nsb_op_attention_paged(
+        *_heads(d, q, "q", dt, B, Hq, dh), kind, B, Hq, Hkv, dh, *_pages(d, k_cache, "k_cache", dt, pages, page, Hkv, dh),
+        *_pages(d, v_cache, "v_cache", dt, pages, page, Hkv, dh), pages, page, *_ints(d, table, "table", B, width), width,
+        _dense(d, lens, "lens", _i32, (B,)), window, sinks, dh ** -0.5 if scale is None else scale,
+        *_heads(d, out, "out", dt, B, Hq, dh), None if lse is None else _dense(d, lse, "lse", _f32, (B, Hq)),
+        _dense(d, workspace, "workspace", _u8, (have,)), have, _stream_of(d))
+    if rc:
+        _check(rc, "nsb_op_attention_paged")
+
+
+def _packed(d, q, k, v, offsets, window, sinks, scale):
+    kind = _kind(q, "q")
+    dt = q.dtype
+    T, Hq, dh = q.shape
+    Hkv = k.shape[1]
+    B = 1 if offsets is None else offsets.shape[0] - 1
+    return (*_heads(d, q, "q", dt, T, Hq, dh), *_heads(d, k, "k", dt, T, Hkv, dh), *_heads(d, v, "v", dt, T, Hkv, dh), kind,
+            T, Hq, Hkv, dh, None if offsets is None else _dense(d, offsets, "offsets", _i32, (B + 1,)), B, window, sinks,
+            dh ** -0.5 if scale is None else scale)
+
+
+def attention_window(q, k, v, out, lse=None, offsets=None, window=0, sinks=0, scale=None):
+    """out [T, Hq, dh] (and lse [Hq, T]) <- causal attention of packed sequences, q [T, Hq, dh] and k, v [T, Hkv, dh]:
+    rows offsets[b] to offsets[b + 1] (int32, [B + 1]; None: one sequence) are sequence b. With window a query sees the
+    last `window` keys up to its own, and the first `sinks`. Rows behind the last sequence are left as they are."""
+    lib = _bound if _f32 else _torch()
+    d = _device()
+    T, Hq, dh = q.shape
+    rc = lib.nsb_op_attention_window(
+        *_packed(d, q, k, v, offsets, window, sinks, scale), *_heads(d, out, "out", q.dtype, T, Hq, dh),
+        *((None, 0) if lse is None else _rows(d, lse, "lse", _f32, Hq, T)), _stream_of(d))
+    if rc:
+        _check(rc, "nsb_op_attention_window")
+
+
+def attention_window_bwd(q, k, v, out, lse, dout, dq, dk, dv, offsets=None, window=0, sinks=0, scale=None, dvec=None):
+    """dq [T, Hq, dh], dk, dv [T, Hkv, dh] <- the gradients of attention_window's q, k, v for out's gradient dout, from
+    its out and lse. dvec (float32, Hq * T): scratch, allocated where it is not given."""
+    import torch
+    lib = _bound if _f32 else _torch()
+    d = _device()
+    dt = q.dtype
+    T, Hq, dh = q.shape
+    Hkv = k.shape[1]
+    args = _packed(d, q, k, v, offsets, window, sinks, scale)
+    if dvec is None:
+        dvec = torch.empty(Hq * T, dtype=_f32, device=q.device)
+    rc = lib.nsb_op_attention_window_bwd(
+        *args, *_heads(d, out, "out", dt, T, Hq, dh), *_rows(d, lse, "lse", _f32, Hq, T),
+        *_heads(d, dout, "dout", dt, T, Hq, dh), *_heads(d, dq, "dq", dt, T, Hq, dh), *_heads(d, dk, "dk", dt, T, Hkv, dh),
+        *_heads(d, dv, "dv", dt, T, Hkv, dh), _dense(d, dvec, "dvec", _f32, (Hq * T,)), _stream_of(d))
+    if rc:
+        _check(rc, "nsb_op_attention_window_bwd")
