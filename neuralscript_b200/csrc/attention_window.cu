@@ -350,6 +350,7 @@ int attention_window(const WindowDesc& d, cudaStream_t st) {
     if (d.T == 0 || d.B == 0) return 0;
     if (!d.q.p || !d.k.p || !d.v.p || !d.out.p || (d.lse && d.ld_lse < d.T)) return -1;
     if (!d.err) return -5;
+    if (attention_window_tc_supported(d)) return attention_window_tc(d, st);
     return by_type(d, [&](auto zero, auto wide) {
         using T = decltype(zero);
         constexpr int DHP = decltype(wide)::value, bytes = smem_of<DHP>(3, 1);
