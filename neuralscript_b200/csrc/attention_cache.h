@@ -104,6 +104,8 @@ int attention_window(const WindowDesc& d, cudaStream_t s);
 // on the tensor cores (attention_window_tc.cu): bf16, 16-byte rows
 bool attention_window_tc_supported(const WindowDesc& d);
 int attention_window_tc(const WindowDesc& d, cudaStream_t s);
+bool attention_window_bwd_tc_supported(const WindowDesc& d);
+int attention_window_bwd_tc(const WindowDesc& d, cudaStream_t s);
 int attention_window_bwd(const WindowDesc& d, cudaStream_t s);
 
 }  // namespace nsb

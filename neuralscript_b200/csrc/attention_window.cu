@@ -367,6 +367,7 @@ int attention_window_bwd(const WindowDesc& d, cudaStream_t st) {
         !d.dvec)
         return -1;
     if (!d.err) return -5;
+    if (attention_window_bwd_tc_supported(d)) return attention_window_bwd_tc(d, st);
     return by_type(d, [&](auto zero, auto wide) {
         using T = decltype(zero);
         constexpr int DHP = decltype(wide)::value, bq = smem_of<DHP>(4, 1), bk = smem_of<DHP>(4, 2);
