@@ -389,15 +389,19 @@ int nsb_op_attention_window(const void* q, long long q_row, long long q_head, co
                             int Hkv, int dh, const int* offsets, int B, int window, int sinks, float scale, void* out,
                             long long out_row, long long out_head, float* lse, long long ld_lse, void* stream);
 /* Its gradients from dout, the forward pass's out and lse: dq, and dk, dv
- * summed over the query heads that share a key head, in a fixed order. dvec:
- * scratch of Hq * T floats. */
+ * summed over the query heads that share a key head, in a fixed order.
+ * workspace (16-byte aligned) of at least
+ * nsb_op_attention_window_bwd_workspace_bytes(...) bytes: of this call alone
+ * until it is done. */
+size_t nsb_op_attention_window_bwd_workspace_bytes(int T, int Hq, int Hkv, int dh, int dtype);
 int nsb_op_attention_window_bwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row,
                                 long long k_head, const void* v, long long v_row, long long v_head, int dtype, int T,
                                 int Hq, int Hkv, int dh, const int* offsets, int B, int window, int sinks, float scale,
                                 const void* out, long long out_row, long long out_head, const float* lse, long long ld_lse,
                                 const void* dout, long long do_row, long long do_head, void* dq, long long dq_row,
                                 long long dq_head, void* dk, long long dk_row, long long dk_head, void* dv,
-                                long long dv_row, long long dv_head, float* dvec, void* stream);
+                                long long dv_row, long long dv_head, void* workspace, size_t workspace_bytes,
+                                void* stream);
 
 #ifdef __cplusplus
 }

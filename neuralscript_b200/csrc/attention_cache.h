@@ -97,7 +97,10 @@ struct WindowDesc {
     float* lse = nullptr;  // [Hq, ld_lse]
     long long ld_lse = 0;
     Heads dout, dq, dk, dv;   // backward
-    float* dvec = nullptr;    // [Hq, T] scratch: rowdot(dout, out)
+    void* workspace = nullptr;
+    size_t workspace_bytes = 0;
+    float* dvec = nullptr;    // in the workspace: [Hq, T] rowdot(dout, out)
+    float* parts = nullptr;   // and sums of tiles that several blocks share
     int* err = nullptr;
 };
 int attention_window(const WindowDesc& d, cudaStream_t s);
@@ -105,7 +108,10 @@ int attention_window(const WindowDesc& d, cudaStream_t s);
 bool attention_window_tc_supported(const WindowDesc& d);
 int attention_window_tc(const WindowDesc& d, cudaStream_t s);
 bool attention_window_bwd_tc_supported(const WindowDesc& d);
+size_t attention_window_bwd_tc_parts(int dh);
 int attention_window_bwd_tc(const WindowDesc& d, cudaStream_t s);
+size_t attention_window_bwd_workspace(int T, int Hq, int Hkv, int dh, int dtype);
 int attention_window_bwd(const WindowDesc& d, cudaStream_t s);
+int attention_window_bwd_launches(const WindowDesc& d);
 
 }  // namespace nsb

@@ -360,13 +360,27 @@ int attention_window(const WindowDesc& d, cudaStream_t st) {
     });
 }
 
-int attention_window_bwd(const WindowDesc& d, cudaStream_t st) {
+static size_t dvec_bytes(int T, int Hq) { return ((size_t)Hq * T * sizeof(float) + 15) / 16 * 16; }
+
+size_t attention_window_bwd_workspace(int T, int Hq, int Hkv, int dh, int dtype) {
+    if (T <= 0 || Hkv <= 0 || Hq < Hkv || Hq % Hkv || dh <= 0 || dh > kAttnMaxHead) return 0;
+    return dvec_bytes(T, Hq) + (dtype == kBF16 && dh % 8 == 0 ? attention_window_bwd_tc_parts(dh) : 0);
+}
+
+int attention_window_bwd_launches(const WindowDesc& d) { return attention_window_bwd_tc_supported(d) ? 3 : 2; }
+
+int attention_window_bwd(const WindowDesc& given, cudaStream_t st) {
+    WindowDesc d = given;
     if (const int bad = check(d)) return bad;
     if (d.T == 0 || d.B == 0) return 0;
-    if (!d.q.p || !d.k.p || !d.v.p || !d.out.p || !d.lse || d.ld_lse < d.T || !d.dout.p || !d.dq.p || !d.dk.p || !d.dv.p ||
-        !d.dvec)
+    if (!d.q.p || !d.k.p || !d.v.p || !d.out.p || !d.lse || d.ld_lse < d.T || !d.dout.p || !d.dq.p || !d.dk.p || !d.dv.p)
+        return -1;
+    if (!d.workspace || reinterpret_cast<uintptr_t>(d.workspace) % 16 ||
+        d.workspace_bytes < attention_window_bwd_workspace(d.T, d.Hq, d.Hkv, d.dh, d.dtype))
         return -1;
     if (!d.err) return -5;
+    d.dvec = reinterpret_cast<float*>(d.workspace);
+    d.parts = reinterpret_cast<float*>(reinterpret_cast<char*>(d.workspace) + dvec_bytes(d.T, d.Hq));
     if (attention_window_bwd_tc_supported(d)) return attention_window_bwd_tc(d, st);
     return by_type(d, [&](auto zero, auto wide) {
         using T = decltype(zero);

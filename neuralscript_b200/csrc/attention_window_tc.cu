@@ -86,10 +86,11 @@ __device__ __forceinline__ void mma_dot(uint32_t d, uint32_t a, uint32_t b) {
     }
 }
 
-// 32 columns of an output row.
-__device__ __forceinline__ void store32(__nv_bfloat16* to, const uint32_t* v, float mul, int cols) {
+// N columns of an output row, `cols` of which there are.
+template <int N>
+__device__ __forceinline__ void store_cols(__nv_bfloat16* to, const uint32_t* v, float mul, int cols) {
 #pragma unroll
-    for (int g = 0; g < 4; g++) {
+    for (int g = 0; g < N / 8; g++) {
         if (8 * g >= cols) break;
         uint4 pk;
         __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&pk);
@@ -350,7 +351,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                 uint32_t v[32];
                 ptx::tmem_ld32(o_at + c, v);
                 ptx::tmem_ld_wait_regs32(v);
-                if (i < w.n) store32(to + c, v, mul, d.dh - c);
+                if (i < w.n) store_cols<32>(to + c, v, mul, d.dh - c);
             }
             if (i < w.n && d.lse) d.lse[h * d.ld_lse + w.row0 + i] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * kLn2;
         }
@@ -366,22 +367,23 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 // ---------------------------------------------------------------------------
 // Gradient of the queries. A block has 128 queries of one head and walks the
 // tiles of keys that they see:
-//   warp 9     TMA: queries and dout, then keys and values through a ring
-//   warp 8     every MMA: S = Q K^T into TMEM columns [0, 128),
+//   warp 17    TMA: queries and dout, then keys and values through a ring
+//   warp 16    every MMA: S = Q K^T into TMEM columns [0, 128),
 //              dP = dout V^T into [128, 256), dQ += dS K into [256, ...), dS
 //              (bf16) read from [384, 448). The next tile's S and dP run while
 //              this one's dS is computed.
-//   warps 0..7 dS = P (dP - D), two threads a query with 64 keys each. Before
-//              the first tile they form D = rowdot(dout, out), which the second
+//   warps 0..15   dS = P (dP - D), four threads a query with 32 keys each: their
+//              registers hold both scores at once, and four warps a scheduler
+//              hide each other's latencies. Before the first tile they form D = rowdot(dout, out), which the second
 //              kernel reads too.
 // ---------------------------------------------------------------------------
-constexpr int kBwdQThreads = 320;
+constexpr int kBwdQThreads = 576;
 
 template <int DHP>
 struct BwdQ {
     static constexpr int TILE = DHP / 64 * kChunk;
     static constexpr int SLOTS = DHP == 128 ? 4 : 8;
-    static constexpr int SMEM = (2 + SLOTS) * TILE + 256 * 4 + 512 + 1024;
+    static constexpr int SMEM = (2 + SLOTS) * TILE + 512 * 4 + 512 + 1024;
 };
 
 template <int DHP>
@@ -393,13 +395,13 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* ring = smem + 2 * F::TILE;
-    float* sums = reinterpret_cast<float*>(ring + F::SLOTS * F::TILE);  // [2][128] halves of D
-    uint64_t* q_full = reinterpret_cast<uint64_t*>(sums + 256);
+    float* sums = reinterpret_cast<float*>(ring + F::SLOTS * F::TILE);  // [4][128] quarters of D
+    uint64_t* q_full = reinterpret_cast<uint64_t*>(sums + 512);
     uint64_t* full = q_full + 1;
     uint64_t* empty = full + F::SLOTS;
     uint64_t* s_bar = empty + F::SLOTS;  // S and dP of a tile in TMEM
-    uint64_t* r_bar = s_bar + 1;         // both read (256 arrivals)
-    uint64_t* p_bar = r_bar + 1;         // dS in TMEM (256 arrivals)
+    uint64_t* r_bar = s_bar + 1;         // both read (512 arrivals)
+    uint64_t* p_bar = r_bar + 1;         // dS in TMEM (512 arrivals)
     uint64_t* o_bar = p_bar + 1;         // product added to dQ
     uint64_t* drain = o_bar + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -418,14 +420,14 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
             ptx::mbar_init(&empty[i], 1);
         }
         ptx::mbar_init(s_bar, 1);
-        ptx::mbar_init(r_bar, 256);
-        ptx::mbar_init(p_bar, 256);
+        ptx::mbar_init(r_bar, 512);
+        ptx::mbar_init(p_bar, 512);
         ptx::mbar_init(o_bar, 1);
         ptx::mbar_init(drain, 1);
         *failed = 0;
         ptx::fence_mbar_init();
     }
-    if (warp == 8) {
+    if (warp == 16) {
         ptx::tmem_alloc(tmem_slot, 512);
         ptx::tmem_relinquish();
     }
@@ -437,7 +439,7 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
     bool ok = true;
     const KeyTiles tiles(d, q0, min(q0 + kT, w.n), kT);
 
-    if (warp == 9) {
+    if (warp == 17) {
         if ((t & 31) == 0) {
             ptx::mbar_arrive_expect_tx(q_full, 2 * F::TILE);
             for (int c = 0; c < DHP / 64; c++) {
@@ -457,7 +459,7 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
             for (int i = max(0, it - F::SLOTS); i < it; i++)
                 ptx::mbar_wait(&full[i % F::SLOTS], (i / F::SLOTS) & 1, nullptr, 0);
         }
-    } else if (warp == 8) {
+    } else if (warp == 16) {
         const bool one = (t & 31) == 0;
         const uint32_t aQ = ptx::smem_u32(smem), aG = aQ + F::TILE, aR = ptx::smem_u32(ring);
         constexpr uint32_t idesc = ptx::instr_desc(1, 0, 1, kT, DHP);
@@ -496,7 +498,7 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
             ptx::mbar_wait(drain, 0, nullptr, 0);
         }
     } else {
-        const int lg = warp & 3, half = warp >> 2, r = lg * 32 + (t & 31);
+        const int lg = warp & 3, part = warp >> 2, r = lg * 32 + (t & 31);
         const int i = q0 + r;
         const uint32_t base = tmem + ((uint32_t)(lg * 32) << 16);
         const float sl2 = d.scale * kLog2e;
@@ -507,8 +509,8 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
             const __nv_bfloat16* g = (const __nv_bfloat16*)d.dout.p + (w.row0 + i) * d.dout.row + h * d.dout.head;
             const __nv_bfloat16* o = (const __nv_bfloat16*)d.out.p + (w.row0 + i) * d.out.row + h * d.out.head;
 #pragma unroll
-            for (int c = 0; c < DHP / 2; c += 8) {
-                const int at = half * (DHP / 2) + c;
+            for (int c = 0; c < DHP / 4; c += 8) {
+                const int at = part * (DHP / 4) + c;
                 if (at < d.dh) {
                     const uint4 x = *reinterpret_cast<const uint4*>(g + at), y = *reinterpret_cast<const uint4*>(o + at);
                     const __nv_bfloat162* x2 = reinterpret_cast<const __nv_bfloat162*>(&x);
@@ -522,41 +524,35 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
                 }
             }
         }
-        sums[half * 128 + r] = D;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        D = sums[r] + sums[128 + r];
-        if (half == 0 && i < w.n) d.dvec[(long long)h * d.T + w.row0 + i] = D;
+        sums[part * 128 + r] = D;
+        asm volatile("bar.sync 1, 512;" ::: "memory");
+        D = (sums[r] + sums[128 + r]) + (sums[256 + r] + sums[384 + r]);
+        if (part == 0 && i < w.n) d.dvec[(long long)h * d.T + w.row0 + i] = D;
         const uint64_t SL2 = f2_pack(sl2, sl2), NEG = f2_pack(-lse2, -lse2), ND = f2_pack(-D, -D);
         for (int x = 0; x < tiles.count; x++) {
             const int k0 = tiles.at(x) * kT;
             if (!(ok = wait(s_bar, x))) break;
             ptx::tc_fence_after();
-            uint32_t a[64], g[64];
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                ptx::tmem_ld32(base + half * 64 + 32 * c, a + 32 * c);
-                ptx::tmem_ld32(base + 128 + half * 64 + 32 * c, g + 32 * c);
-            }
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                ptx::tmem_ld_wait_regs32(a + 32 * c);
-                ptx::tmem_ld_wait_regs32(g + 32 * c);
-            }
+            uint32_t a[32], g[32];
+            ptx::tmem_ld32(base + part * 32, a);
+            ptx::tmem_ld32(base + 128 + part * 32, g);
+            ptx::tmem_ld_wait_regs32(a);
+            ptx::tmem_ld_wait_regs32(g);
             ptx::tc_fence_before();
             ptx::mbar_arrive(r_bar);
             const bool whole = all_seen(d, q0, k0);
             const Cols on(d, i, k0);
-            uint32_t pk[32];
+            uint32_t pk[16];
 #pragma unroll
-            for (int e = 0; e < 32; e++) {
+            for (int e = 0; e < 16; e++) {
                 float x0, x1, y0, y1;
                 f2_unpack(f2_fma(f2_pack(__uint_as_float(a[2 * e]), __uint_as_float(a[2 * e + 1])), SL2, NEG), x0, x1);
                 f2_unpack(f2_mul(f2_pack(ex2(x0), ex2(x1)),
                                  f2_add(f2_pack(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1])), ND)),
                           y0, y1);
                 if (!whole) {
-                    y0 = on(half * 64 + 2 * e) ? y0 : 0.f;
-                    y1 = on(half * 64 + 2 * e + 1) ? y1 : 0.f;
+                    y0 = on(part * 32 + 2 * e) ? y0 : 0.f;
+                    y1 = on(part * 32 + 2 * e + 1) ? y1 : 0.f;
                 }
                 const __nv_bfloat162 p = __floats2bfloat162_rn(y0, y1);
                 pk[e] = *reinterpret_cast<const uint32_t*>(&p);
@@ -565,8 +561,7 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
                 if (!(ok = wait(o_bar, x - 1))) break;  // the product before has read its dS
                 ptx::tc_fence_after();
             }
-            ptx::tmem_st16(base + 384 + half * 32, pk);
-            ptx::tmem_st16(base + 384 + half * 32 + 16, pk + 16);
+            ptx::tmem_st16(base + 384 + part * 16, pk);
             ptx::tmem_st_wait();
             ptx::tc_fence_before();
             ptx::mbar_arrive(p_bar);
@@ -575,40 +570,51 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
         ptx::tc_fence_after();
         if (ok) {
             __nv_bfloat16* to = (__nv_bfloat16*)d.dq.p + (w.row0 + i) * d.dq.row + h * d.dq.head;
-#pragma unroll 1
-            for (int c = half * (DHP / 2); c < (half + 1) * (DHP / 2); c += 32) {
+            if constexpr (DHP == 128) {
                 uint32_t v[32];
-                ptx::tmem_ld32(base + 256 + c, v);
+                ptx::tmem_ld32(base + 256 + part * 32, v);
                 ptx::tmem_ld_wait_regs32(v);
-                if (i < w.n) store32(to + c, v, d.scale, d.dh - c);
+                if (i < w.n) store_cols<32>(to + part * 32, v, d.scale, d.dh - part * 32);
+            } else {
+                uint32_t v[16];
+                ptx::tmem_ld16(base + 256 + part * 16, v);
+                ptx::tmem_ld_wait_regs16(v);
+                if (i < w.n) store_cols<16>(to + part * 16, v, d.scale, d.dh - part * 16);
             }
         }
     }
     ptx::tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 16) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc(tmem, 512);
     }
 }
 
 // ---------------------------------------------------------------------------
-// Gradients of keys and values. A block has 128 keys of one key head and walks
-// the tiles of queries, of all heads that share it, that see any of them. The
-// scores stand transposed, a key a row, so that both sums run over TMEM's
+// Gradients of keys and values. For 128 keys of one key head the tiles of
+// queries, of all heads that share it, that see any of them are walked. How
+// many these are differs by far (the first keys stay visible to all queries;
+// without a window the last keys are seen by few), so all steps (a tile of
+// keys with one of queries) of all tiles stand in one line that is cut into
+// equal shares, one a block; a tile of keys that is cut leaves fp32 sums in
+// the workspace, which a last kernel joins in the order of the blocks.
+//
+// The scores stand transposed, a key a row, so that both sums run over TMEM's
 // columns:
-//   warp 9     TMA: keys and values, then queries and dout through a ring
-//   warp 10    lse and D of each tile of queries, into a ring of their own
-//   warp 8     every MMA: S^T = K Q^T into TMEM columns [0, 128), dP^T = V dout^T
+//   warp 17    TMA: keys and values, then queries and dout through a ring
+//   warp 18    lse and D of each tile of queries, into a ring of their own
+//   warp 16    every MMA: S^T = K Q^T into TMEM columns [0, 128), dP^T = V dout^T
 //              into [128, 256), dV += P^T dout into [256, ...), dK += dS^T Q into
 //              [384, ...). P^T and dS^T (bf16) take the columns of the scores
 //              that they come from.
-//   warps 0..7 P and dS, two threads a key with 64 queries each: while P is
+//   warps 0..15   P and dS, four threads a key with 32 queries each: while P is
 //              computed the tensor cores run dK and the next dP, while dS is,
 //              dV and the next S.
 // ---------------------------------------------------------------------------
-constexpr int kBwdKvThreads = 352;
-constexpr int kStats = 4;  // tiles of lse and D held
+constexpr int kBwdKvThreads = 608;
+constexpr int kStats = 4;      // tiles of lse and D held
+constexpr int kMinSteps = 4;   // least steps a block: cutting a tile costs about two
 
 template <int DHP>
 struct BwdKv {
@@ -616,6 +622,108 @@ struct BwdKv {
     static constexpr int SLOTS = DHP == 128 ? 4 : 8;
     static constexpr int SMEM = (2 + SLOTS) * TILE + kStats * 2 * kT * 4 + 512 + 1024;
 };
+
+// Steps of a sequence, of one query head: tile t of nt has
+// min(nt - t, reach), the `front` first nt - t.
+struct Steps {
+    long long nt, front, reach;
+    __device__ __forceinline__ Steps(const WindowDesc& d, int n) {
+        nt = (n + kT - 1) / kT;
+        front = d.window ? min(nt, (long long)d.sinks / kT + (d.sinks % kT != 0)) : nt;
+        reach = ((long long)d.window + 2 * kT - 2) / kT;
+    }
+    __device__ __forceinline__ long long of(int t) const { return t < front ? nt - t : min(nt - t, reach); }
+    // those of the tiles before t
+    __device__ __forceinline__ long long before(long long t) const {
+        const long long f = min(t, front), s = f * nt - f * (f - 1) / 2;
+        if (t <= front) return s;
+        const long long u = nt - front, v = nt - t;  // tiles behind the front, and from t on: their steps v, v - 1 .. 1, or reach
+        auto tail = [&](long long k) { return k <= reach ? k * (k + 1) / 2 : reach * (reach + 1) / 2 + (k - reach) * reach; };
+        return s + tail(u) - tail(v);
+    }
+    __device__ __forceinline__ long long all() const { return before(nt); }
+};
+
+// The sequence b with its rows and the steps of one query head before it.
+struct Seq {
+    int row0, n;
+    long long before;
+};
+// The first sequence for which less(steps up to its end, tiles up to its end)
+// no longer holds; `all` receives the steps of every sequence where none is
+// found. By whole warps.
+template <typename F>
+__device__ __forceinline__ bool find_seq(const WindowDesc& d, Seq* out, long long* tiles, long long* all, F past) {
+    const int lane = threadIdx.x & 31;
+    long long steps = 0, rows = 0;
+    for (int b0 = 0; b0 < d.B; b0 += 32) {
+        int lo = 0, n = 0;
+        if (b0 + lane < d.B) {
+            lo = d.offsets ? min(max(d.offsets[b0 + lane], 0), d.T) : 0;
+            n = d.offsets ? min(max(d.offsets[b0 + lane + 1], lo), d.T) - lo : d.T;
+        }
+        const long long own = Steps(d, n).all(), nt = (n + kT - 1) / kT;
+        long long s = own, r = nt;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, s, o), v = __shfl_up_sync(0xffffffffu, r, o);
+            if (lane >= o) s += u, r += v;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, past(steps + s, rows + r));
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            *out = Seq{__shfl_sync(0xffffffffu, lo, src), __shfl_sync(0xffffffffu, n, src),
+                       steps + __shfl_sync(0xffffffffu, s - own, src)};
+            *tiles = rows + __shfl_sync(0xffffffffu, r - nt, src);
+            return true;
+        }
+        steps += __shfl_sync(0xffffffffu, s, 31);
+        rows += __shfl_sync(0xffffffffu, r, 31);
+    }
+    *all = steps;
+    return false;
+}
+// Steps of all heads, and a block's share of them.
+__device__ __forceinline__ long long all_steps(const WindowDesc& d) {
+    Seq q;
+    long long tiles, all = 0;
+    find_seq(d, &q, &tiles, &all, [](long long, long long) { return false; });
+    return all * d.Hq;
+}
+__device__ __forceinline__ long long share(long long all, int blocks) {
+    return max((long long)kMinSteps, (all + blocks - 1) / blocks);
+}
+
+// A piece of a block's share: steps [x0, x1) of `count` of one tile of keys.
+struct Piece {
+    int row0, n, k0, hk;
+    int first, each;  // first tile of queries, and how many a head
+    int x0, x1, count;
+};
+__device__ __forceinline__ Piece piece_at(const WindowDesc& d, long long at, long long end) {
+    Seq q{0, 0, 0};
+    long long tiles, all;
+    const int group = d.Hq / d.Hkv;
+    find_seq(d, &q, &tiles, &all, [&](long long steps, long long) { return steps * d.Hq > at; });
+    const Steps s(d, q.n);
+    long long rest = at - q.before * d.Hq;
+    const long long head = s.all() * group;
+    Piece p;
+    p.row0 = q.row0;
+    p.n = q.n;
+    p.hk = (int)(rest / head);
+    rest -= p.hk * head;
+    int t = 0;  // the last tile whose steps begin at or before `rest`
+    for (int step = 1 << 24; step; step >>= 1)
+        if (t + step < s.nt && s.before(t + step) * group <= rest) t += step;
+    p.k0 = t * kT;
+    p.first = t;
+    p.each = (int)s.of(t);
+    p.count = p.each * group;
+    p.x0 = (int)(rest - s.before(t) * group);
+    p.x1 = (int)min((long long)p.count, p.x0 + (end - at));
+    return p;
+}
 
 template <int DHP>
 __global__ void __launch_bounds__(kBwdKvThreads, 1)
@@ -628,44 +736,49 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
     uint8_t* ring = smem + 2 * F::TILE;
     float* stats = reinterpret_cast<float*>(ring + F::SLOTS * F::TILE);  // [kStats][lse | D][128]
     uint64_t* k_full = reinterpret_cast<uint64_t*>(stats + kStats * 2 * kT);
-    uint64_t* full = k_full + 1;
+    uint64_t* k_empty = k_full + 1;        // keys and values read by the last scores of a piece
+    uint64_t* full = k_empty + 1;
     uint64_t* empty = full + F::SLOTS;
     uint64_t* st_full = empty + F::SLOTS;  // (32 arrivals)
-    uint64_t* st_empty = st_full + kStats; // (256 arrivals)
+    uint64_t* st_empty = st_full + kStats; // (512 arrivals)
     uint64_t* s_bar = st_empty + kStats;   // S^T in TMEM
     uint64_t* g_bar = s_bar + 1;           // dP^T in TMEM
-    uint64_t* p_bar = g_bar + 1;           // P^T in TMEM (256 arrivals)
-    uint64_t* ds_bar = p_bar + 1;          // dS^T in TMEM (256 arrivals)
-    uint64_t* drain = ds_bar + 1;          // every product done
+    uint64_t* p_bar = g_bar + 1;           // P^T in TMEM (512 arrivals)
+    uint64_t* ds_bar = p_bar + 1;          // dS^T in TMEM (512 arrivals)
+    uint64_t* sum_bar = ds_bar + 1;        // a piece's sums in TMEM
+    uint64_t* out_bar = sum_bar + 1;       // and read (512 arrivals)
+    uint64_t* drain = out_bar + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     int* failed = reinterpret_cast<int*>(tmem_slot + 1);
 
     const int t = threadIdx.x, warp = t >> 5;
-    const int hk = blockIdx.x % d.Hkv, group = d.Hq / d.Hkv;
-    const Rows w = find_rows(d, blockIdx.x / d.Hkv, kT);
-    if (w.n <= 0) return;
-    const int k0 = w.first, row0 = (int)w.row0;
-    const int first = k0 / kT, each = query_tiles_end(d, k0, w.n, kT) - first, count = each * group;
+    const int group = d.Hq / d.Hkv;
+    const long long all = all_steps(d), per = share(all, gridDim.x);
+    const long long begin = blockIdx.x * per, end = min(all, begin + per);
+    if (begin >= end) return;
 
     if (t == 0) {
         ptx::mbar_init(k_full, 1);
+        ptx::mbar_init(k_empty, 1);
         for (int i = 0; i < F::SLOTS; i++) {
             ptx::mbar_init(&full[i], 1);
             ptx::mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < kStats; i++) {
             ptx::mbar_init(&st_full[i], 32);
-            ptx::mbar_init(&st_empty[i], 256);
+            ptx::mbar_init(&st_empty[i], 512);
         }
         ptx::mbar_init(s_bar, 1);
         ptx::mbar_init(g_bar, 1);
-        ptx::mbar_init(p_bar, 256);
-        ptx::mbar_init(ds_bar, 256);
+        ptx::mbar_init(p_bar, 512);
+        ptx::mbar_init(ds_bar, 512);
+        ptx::mbar_init(sum_bar, 1);
+        ptx::mbar_init(out_bar, 512);
         ptx::mbar_init(drain, 1);
         *failed = 0;
         ptx::fence_mbar_init();
     }
-    if (warp == 8) {
+    if (warp == 16) {
         ptx::tmem_alloc(tmem_slot, 512);
         ptx::tmem_relinquish();
     }
@@ -675,220 +788,291 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
     const uint32_t tmem = *tmem_slot;
     const Waits wait{failed, d.err};
     bool ok = true;
+    // step: counted over all pieces; piece: likewise
+    int step = 0, piece = 0;
 
-    if (warp == 9) {
-        if ((t & 31) == 0) {
-            ptx::mbar_arrive_expect_tx(k_full, 2 * F::TILE);
-            for (int c = 0; c < DHP / 64; c++) {
-                ptx::tma_load_3d(smem + c * kChunk, &tk, k_full, c * 64, hk, row0 + k0);
-                ptx::tma_load_3d(smem + F::TILE + c * kChunk, &tv, k_full, c * 64, hk, row0 + k0);
-            }
-            int it = 0;
-            for (int x = 0; x < count && ok; x++) {
-                const int h = hk * group + x / each, row = row0 + (first + x % each) * kT;
-                for (int qg = 0; qg < 2; qg++, it++) {
-                    const int slot = it % F::SLOTS, round = it / F::SLOTS;
-                    if (round && !(ok = wait.lane(&empty[slot], round - 1))) break;
-                    load_rows<DHP>(ring + slot * F::TILE, qg ? &tg : &tq, &full[slot], h, row);
+    if (warp == 17) {
+        const bool one = (t & 31) == 0;
+        int keys = 0, copies = 0;  // loads started
+        for (long long at = begin; at < end && ok; piece++) {
+            const Piece p = piece_at(d, at, end);
+            at += p.x1 - p.x0;
+            if (piece && !(ok = wait(k_empty, piece - 1))) break;
+            keys = piece + 1;
+            if (one) {
+                ptx::mbar_arrive_expect_tx(k_full, 2 * F::TILE);
+                for (int c = 0; c < DHP / 64; c++) {
+                    ptx::tma_load_3d(smem + c * kChunk, &tk, k_full, c * 64, p.hk, p.row0 + p.k0);
+                    ptx::tma_load_3d(smem + F::TILE + c * kChunk, &tv, k_full, c * 64, p.hk, p.row0 + p.k0);
                 }
             }
-            ptx::mbar_wait(k_full, 0, nullptr, 0);
-            for (int i = max(0, it - F::SLOTS); i < it; i++)
+            for (int x = p.x0; x < p.x1 && ok; x++, step++) {
+                const int h = p.hk * group + x / p.each, row = p.row0 + (p.first + x % p.each) * kT;
+                for (int qg = 0; qg < 2; qg++) {
+                    const int i = 2 * step + qg, slot = i % F::SLOTS, round = i / F::SLOTS;
+                    if (round && !(ok = wait(&empty[slot], round - 1))) break;
+                    if (one) load_rows<DHP>(ring + slot * F::TILE, qg ? &tg : &tq, &full[slot], h, row);
+                    copies = i + 1;
+                }
+            }
+        }
+        // no copy may land after the block has left
+        if (one) {
+            if (keys) ptx::mbar_wait(k_full, (keys - 1) & 1, nullptr, 0);
+            for (int i = max(0, copies - F::SLOTS); i < copies; i++)
                 ptx::mbar_wait(&full[i % F::SLOTS], (i / F::SLOTS) & 1, nullptr, 0);
         }
-    } else if (warp == 10) {
-        for (int x = 0; x < count && ok; x++) {
-            const int slot = x % kStats, h = hk * group + x / each, q0 = (first + x % each) * kT;
-            float l[4], D[4];
+    } else if (warp == 18) {
+        for (long long at = begin; at < end && ok;) {
+            const Piece p = piece_at(d, at, end);
+            at += p.x1 - p.x0;
+            for (int x = p.x0; x < p.x1 && ok; x++, step++) {
+                const int slot = step % kStats, h = p.hk * group + x / p.each, q0 = (p.first + x % p.each) * kT;
+                float l[4], D[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int i = q0 + (t & 31) + 32 * e;
-                // a query that saw nothing, or is none, has weights of 0
-                l[e] = INFINITY;
-                D[e] = 0.f;
-                if (i < w.n) {
-                    const float lse = d.lse[h * d.ld_lse + w.row0 + i];
-                    if (lse != -INFINITY) l[e] = lse * kLog2e;
-                    D[e] = d.dvec[(long long)h * d.T + w.row0 + i];
+                for (int e = 0; e < 4; e++) {
+                    const int i = q0 + (t & 31) + 32 * e;
+                    // a query that saw nothing, or is none, has weights of 0
+                    l[e] = INFINITY;
+                    D[e] = 0.f;
+                    if (i < p.n) {
+                        const float lse = d.lse[h * d.ld_lse + p.row0 + i];
+                        if (lse != -INFINITY) l[e] = lse * kLog2e;
+                        D[e] = d.dvec[(long long)h * d.T + p.row0 + i];
+                    }
                 }
-            }
-            if (x >= kStats && !(ok = wait(&st_empty[slot], x / kStats - 1))) break;
+                if (step >= kStats && !(ok = wait(&st_empty[slot], step / kStats - 1))) break;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                stats[slot * 2 * kT + (t & 31) + 32 * e] = l[e];
-                stats[slot * 2 * kT + kT + (t & 31) + 32 * e] = D[e];
+                for (int e = 0; e < 4; e++) {
+                    stats[slot * 2 * kT + (t & 31) + 32 * e] = l[e];
+                    stats[slot * 2 * kT + kT + (t & 31) + 32 * e] = D[e];
+                }
+                ptx::mbar_arrive(&st_full[slot]);
             }
-            ptx::mbar_arrive(&st_full[slot]);
         }
-    } else if (warp == 8) {
+    } else if (warp == 16) {
         const bool one = (t & 31) == 0;
         const uint32_t aK = ptx::smem_u32(smem), aV = aK + F::TILE, aR = ptx::smem_u32(ring);
         constexpr uint32_t idesc = ptx::instr_desc(1, 0, 1, kT, DHP);
-        // the slot that a tile's queries (0) or dout (1) are in, with zeros behind the sequence's end
-        auto ready = [&](int x, int qg) {
-            const int i = 2 * x + qg, slot = i % F::SLOTS, q0 = (first + x % each) * kT;
-            ok = wait(&full[slot], i / F::SLOTS);
-            if (ok && q0 + kT > w.n) zero_rows<DHP>(ring + slot * F::TILE, w.n - q0);
-            return aR + slot * F::TILE;
-        };
-        // d += A (bf16 of 128 queries in 2 x 32 columns, 64 apart) times the rows at b
+        // d += A (bf16 of 128 queries in 4 x 16 columns, 32 apart) times the rows at b
         auto add = [&](uint32_t d0, uint32_t a, uint32_t b, bool more) {
 #pragma unroll
             for (int s = 0; s < kT / 16; s++)
-                ptx::mma_bf16_ts(d0, a + 64 * (s >> 2) + 8 * (s & 3), ptx::smem_desc(b + s * 2048, kChunk, 1024, 2), idesc,
+                ptx::mma_bf16_ts(d0, a + 32 * (s >> 1) + 8 * (s & 1), ptx::smem_desc(b + s * 2048, kChunk, 1024, 2), idesc,
                                  more || s > 0);
         };
-        ok = wait(k_full, 0);
-        uint32_t aQ = 0, aG = 0;  // of the tile whose weights are awaited
-        if (ok) aQ = ready(0, 0);
-        if (ok) aG = ready(0, 1);
-        if (ok && one) {
-            ptx::tc_fence_after();
-            mma_dot<DHP>(tmem, aK, aQ);
-            ptx::mma_commit(s_bar);
-            mma_dot<DHP>(tmem + 128, aV, aG);
-            ptx::mma_commit(g_bar);
-        }
-        for (int x = 0; x < count && ok; x++) {
-            const bool more = x + 1 < count;
-            uint32_t nQ = 0, nG = 0;
-            if (more) nQ = ready(x + 1, 0);
-            if (!ok || !(ok = wait(p_bar, x))) break;
-            if (one) {
+        for (long long at = begin; at < end && ok; piece++) {
+            const Piece p = piece_at(d, at, end);
+            at += p.x1 - p.x0;
+            // the slot that a step's queries (0) or dout (1) are in, with zeros behind the sequence's end
+            auto ready = [&](int x, int qg) {
+                const int i = 2 * (step + x - p.x0) + qg, slot = i % F::SLOTS, q0 = (p.first + x % p.each) * kT;
+                ok = wait(&full[slot], i / F::SLOTS);
+                if (ok && q0 + kT > p.n) zero_rows<DHP>(ring + slot * F::TILE, p.n - q0);
+                return aR + slot * F::TILE;
+            };
+            uint32_t aQ = 0, aG = 0;  // of the step whose weights are awaited
+            ok = wait(k_full, piece);
+            if (ok) aQ = ready(p.x0, 0);
+            if (ok) aG = ready(p.x0, 1);
+            if (ok && one) {
                 ptx::tc_fence_after();
-                add(tmem + 256, tmem, aG, x > 0);
-                ptx::mma_commit(&empty[(2 * x + 1) % F::SLOTS]);
-                if (more) {
-                    mma_dot<DHP>(tmem, aK, nQ);
-                    ptx::mma_commit(s_bar);
-                }
+                mma_dot<DHP>(tmem, aK, aQ);
+                ptx::mma_commit(s_bar);
+                mma_dot<DHP>(tmem + 128, aV, aG);
+                ptx::mma_commit(g_bar);
             }
             __syncwarp();
-            if (more) nG = ready(x + 1, 1);
-            if (!ok || !(ok = wait(ds_bar, x))) break;
-            if (one) {
-                ptx::tc_fence_after();
-                add(tmem + 384, tmem + 128, aQ, x > 0);
-                ptx::mma_commit(&empty[2 * x % F::SLOTS]);
-                if (more) {
-                    mma_dot<DHP>(tmem + 128, aV, nG);
-                    ptx::mma_commit(g_bar);
+            for (int x = p.x0; x < p.x1 && ok; x++) {
+                const bool more = x + 1 < p.x1;
+                const int i = 2 * (step + x - p.x0);
+                uint32_t nQ = 0, nG = 0;
+                if (more) nQ = ready(x + 1, 0);
+                if (!ok || !(ok = wait(p_bar, i / 2))) break;
+                // the piece before has been read out of the sums
+                if (x == p.x0 && piece && !(ok = wait(out_bar, piece - 1))) break;
+                if (one) {
+                    ptx::tc_fence_after();
+                    add(tmem + 256, tmem, aG, x > p.x0);
+                    ptx::mma_commit(&empty[(i + 1) % F::SLOTS]);
+                    if (more) {
+                        mma_dot<DHP>(tmem, aK, nQ);
+                        ptx::mma_commit(s_bar);
+                    }
                 }
+                __syncwarp();
+                if (more) nG = ready(x + 1, 1);
+                if (!ok || !(ok = wait(ds_bar, i / 2))) break;
+                if (one) {
+                    ptx::tc_fence_after();
+                    add(tmem + 384, tmem + 128, aQ, x > p.x0);
+                    ptx::mma_commit(&empty[i % F::SLOTS]);
+                    if (more) {
+                        mma_dot<DHP>(tmem + 128, aV, nG);
+                        ptx::mma_commit(g_bar);
+                    }
+                    if (x + 2 >= p.x1 && (more || p.x1 - p.x0 == 1)) ptx::mma_commit(k_empty);
+                    if (!more) ptx::mma_commit(sum_bar);
+                }
+                __syncwarp();
+                aQ = nQ;
+                aG = nG;
             }
-            __syncwarp();
-            aQ = nQ;
-            aG = nG;
+            step += p.x1 - p.x0;
         }
         if (one) {
             ptx::mma_commit(drain);
             ptx::mbar_wait(drain, 0, nullptr, 0);
         }
     } else {
-        const int lg = warp & 3, half = warp >> 2;
-        const int j = k0 + lg * 32 + (t & 31);  // key of the sequence
-        const uint32_t base = tmem + ((uint32_t)(lg * 32) << 16) + 64 * half;
+        const int lg = warp & 3, part = warp >> 2;
+        const uint32_t row = tmem + ((uint32_t)(lg * 32) << 16), base = row + 32 * part;
         const float sl2 = d.scale * kLog2e;
         const uint64_t SL2 = f2_pack(sl2, sl2), MINUS = f2_pack(-1.f, -1.f);
-        const bool no_end = d.window == 0 || d.window >= w.n || j < d.sinks;
-        for (int x = 0; x < count; x++) {
-            const int slot = x % kStats, q0 = (first + x % each) * kT;
-            const float4* l4 = reinterpret_cast<const float4*>(stats + slot * 2 * kT + half * 64);
-            const float4* d4 = l4 + kT / 4;
-            const bool whole = all_seen(d, q0, k0);
-            // queries q0 + c that see key j: lo <= c < hi
-            const int lo = j - q0 - half * 64, hi = no_end ? kT : j + d.window - q0 - half * 64;
-            if (!(ok = wait(&st_full[slot], x / kStats) && wait(s_bar, x))) break;
-            ptx::tc_fence_after();
-            uint32_t a[64], g[64];
+        for (long long at = begin; at < end && ok; piece++) {
+            const Piece p = piece_at(d, at, end);
+            const int slot_of_part = at == begin ? 0 : 1;
+            at += p.x1 - p.x0;
+            const int j = p.k0 + lg * 32 + (t & 31);  // key of the sequence
+            const bool no_end = d.window == 0 || d.window >= p.n || j < d.sinks;
+            for (int x = p.x0; x < p.x1; x++, step++) {
+                const int slot = step % kStats, q0 = (p.first + x % p.each) * kT;
+                const float4* l4 = reinterpret_cast<const float4*>(stats + slot * 2 * kT + part * 32);
+                const float4* d4 = l4 + kT / 4;
+                const bool whole = all_seen(d, q0, p.k0);
+                // queries q0 + c that see key j: lo <= c < hi
+                const int lo = j - q0 - part * 32, hi = no_end ? kT : j + d.window - q0 - part * 32;
+                if (!(ok = wait(&st_full[slot], step / kStats) && wait(s_bar, step))) break;
+                ptx::tc_fence_after();
+                uint32_t a[32], g[32], pk[16];
+                ptx::tmem_ld32(base, a);
+                ptx::tmem_ld_wait_regs32(a);
 #pragma unroll
-            for (int c = 0; c < 2; c++) ptx::tmem_ld32(base + 32 * c, a + 32 * c);
+                for (int e = 0; e < 16; e += 2) {
+                    const float4 l = l4[e / 2];
 #pragma unroll
-            for (int c = 0; c < 2; c++) ptx::tmem_ld_wait_regs32(a + 32 * c);
-            uint32_t pk[32];
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-                const float4 l = l4[e / 2];
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const int c = 2 * (e + u);
-                    float x0, x1;
-                    f2_unpack(f2_fma(f2_pack(__uint_as_float(a[c]), __uint_as_float(a[c + 1])), SL2,
-                                     f2_mul(u ? f2_pack(l.z, l.w) : f2_pack(l.x, l.y), MINUS)),
-                              x0, x1);
-                    x0 = ex2(x0);
-                    x1 = ex2(x1);
-                    if (!whole) {
-                        x0 = c >= lo && c < hi ? x0 : 0.f;
-                        x1 = c + 1 >= lo && c + 1 < hi ? x1 : 0.f;
+                    for (int u = 0; u < 2; u++) {
+                        const int c = 2 * (e + u);
+                        float x0, x1;
+                        f2_unpack(f2_fma(f2_pack(__uint_as_float(a[c]), __uint_as_float(a[c + 1])), SL2,
+                                         f2_mul(u ? f2_pack(l.z, l.w) : f2_pack(l.x, l.y), MINUS)),
+                                  x0, x1);
+                        x0 = ex2(x0);
+                        x1 = ex2(x1);
+                        if (!whole) {
+                            x0 = c >= lo && c < hi ? x0 : 0.f;
+                            x1 = c + 1 >= lo && c + 1 < hi ? x1 : 0.f;
+                        }
+                        a[c] = __float_as_uint(x0);
+                        a[c + 1] = __float_as_uint(x1);
+                        const __nv_bfloat162 h2 = __floats2bfloat162_rn(x0, x1);
+                        pk[e + u] = *reinterpret_cast<const uint32_t*>(&h2);
                     }
-                    a[c] = __float_as_uint(x0);
-                    a[c + 1] = __float_as_uint(x1);
-                    const __nv_bfloat162 p = __floats2bfloat162_rn(x0, x1);
-                    pk[e + u] = *reinterpret_cast<const uint32_t*>(&p);
                 }
-            }
-            ptx::tmem_st16(base, pk);
-            ptx::tmem_st16(base + 16, pk + 16);
-            ptx::tmem_st_wait();
-            ptx::tc_fence_before();
-            ptx::mbar_arrive(p_bar);
-            if (!(ok = wait(g_bar, x))) break;
-            ptx::tc_fence_after();
+                ptx::tmem_st16(base, pk);
+                ptx::tmem_st_wait();
+                ptx::tc_fence_before();
+                ptx::mbar_arrive(p_bar);
+                if (!(ok = wait(g_bar, step))) break;
+                ptx::tc_fence_after();
+                ptx::tmem_ld32(base + 128, g);
+                ptx::tmem_ld_wait_regs32(g);
 #pragma unroll
-            for (int c = 0; c < 2; c++) ptx::tmem_ld32(base + 128 + 32 * c, g + 32 * c);
+                for (int e = 0; e < 16; e += 2) {
+                    const float4 D = d4[e / 2];
 #pragma unroll
-            for (int c = 0; c < 2; c++) ptx::tmem_ld_wait_regs32(g + 32 * c);
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-                const float4 D = d4[e / 2];
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const int c = 2 * (e + u);
-                    float y0, y1;
-                    f2_unpack(f2_mul(f2_pack(__uint_as_float(a[c]), __uint_as_float(a[c + 1])),
-                                     f2_fma(u ? f2_pack(D.z, D.w) : f2_pack(D.x, D.y), MINUS,
-                                            f2_pack(__uint_as_float(g[c]), __uint_as_float(g[c + 1])))),
-                              y0, y1);
-                    if (!whole) {  // a hidden place stays 0 whatever dP is
-                        y0 = c >= lo && c < hi ? y0 : 0.f;
-                        y1 = c + 1 >= lo && c + 1 < hi ? y1 : 0.f;
+                    for (int u = 0; u < 2; u++) {
+                        const int c = 2 * (e + u);
+                        float y0, y1;
+                        f2_unpack(f2_mul(f2_pack(__uint_as_float(a[c]), __uint_as_float(a[c + 1])),
+                                         f2_fma(u ? f2_pack(D.z, D.w) : f2_pack(D.x, D.y), MINUS,
+                                                f2_pack(__uint_as_float(g[c]), __uint_as_float(g[c + 1])))),
+                                  y0, y1);
+                        if (!whole) {  // a hidden place stays 0 whatever dP is
+                            y0 = c >= lo && c < hi ? y0 : 0.f;
+                            y1 = c + 1 >= lo && c + 1 < hi ? y1 : 0.f;
+                        }
+                        const __nv_bfloat162 h2 = __floats2bfloat162_rn(y0, y1);
+                        pk[e + u] = *reinterpret_cast<const uint32_t*>(&h2);
                     }
-                    const __nv_bfloat162 p = __floats2bfloat162_rn(y0, y1);
-                    pk[e + u] = *reinterpret_cast<const uint32_t*>(&p);
                 }
+                ptx::tmem_st16(base + 128, pk);
+                ptx::tmem_st_wait();
+                ptx::tc_fence_before();
+                ptx::mbar_arrive(ds_bar);
+                ptx::mbar_arrive(&st_empty[slot]);
             }
-            ptx::tmem_st16(base + 128, pk);
-            ptx::tmem_st16(base + 144, pk + 16);
-            ptx::tmem_st_wait();
-            ptx::tc_fence_before();
-            ptx::mbar_arrive(ds_bar);
-            ptx::mbar_arrive(&st_empty[slot]);
-        }
-        ok = ok && wait(drain, 0);
-        ptx::tc_fence_after();
-        if (ok && !*(volatile int*)failed) {
-            const uint32_t row = tmem + ((uint32_t)(lg * 32) << 16);
-            __nv_bfloat16* dv = (__nv_bfloat16*)d.dv.p + (w.row0 + j) * d.dv.row + hk * d.dv.head;
-            __nv_bfloat16* dk = (__nv_bfloat16*)d.dk.p + (w.row0 + j) * d.dk.row + hk * d.dk.head;
+            if (!ok || !(ok = wait(sum_bar, piece))) break;
+            ptx::tc_fence_after();
+            const bool alone = p.x1 - p.x0 == p.count;
+            __nv_bfloat16* dv = (__nv_bfloat16*)d.dv.p + (p.row0 + j) * d.dv.row + p.hk * d.dv.head;
+            __nv_bfloat16* dk = (__nv_bfloat16*)d.dk.p + (p.row0 + j) * d.dk.row + p.hk * d.dk.head;
+            // [dv | dk][column][key]
+            float* rest = d.parts + ((long long)blockIdx.x * 2 + slot_of_part) * (2 * DHP * kT) + lg * 32 + (t & 31);
 #pragma unroll 1
-            for (int c = half * (DHP / 2); c < (half + 1) * (DHP / 2); c += 32) {
-                uint32_t v[32], k[32];
-                ptx::tmem_ld32(row + 256 + c, v);
-                ptx::tmem_ld32(row + 384 + c, k);
-                ptx::tmem_ld_wait_regs32(v);
-                ptx::tmem_ld_wait_regs32(k);
-                if (j < w.n) {
-                    store32(dv + c, v, 1.f, d.dh - c);
-                    store32(dk + c, k, d.scale, d.dh - c);
+            for (int c = part * (DHP / 4); c < (part + 1) * (DHP / 4); c += 16) {
+                uint32_t v[16], k[16];
+                ptx::tmem_ld16(row + 256 + c, v);
+                ptx::tmem_ld16(row + 384 + c, k);
+                ptx::tmem_ld_wait_regs16(v);
+                ptx::tmem_ld_wait_regs16(k);
+                if (!alone) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        rest[(c + e) * kT] = __uint_as_float(v[e]);
+                        rest[(DHP + c + e) * kT] = __uint_as_float(k[e]);
+                    }
+                } else if (j < p.n) {
+                    store_cols<16>(dv + c, v, 1.f, d.dh - c);
+                    store_cols<16>(dk + c, k, d.scale, d.dh - c);
                 }
             }
+            ptx::tc_fence_before();
+            ptx::mbar_arrive(out_bar);
         }
     }
     ptx::tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 16) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc(tmem, 512);
+    }
+}
+
+// Joins the sums of a tile of keys that several blocks share: eight columns of
+// a key a thread, of dv and dk, block after block. grid (tiles of keys, Hkv).
+template <int DHP>
+__global__ void __launch_bounds__(256) window_tc_join_kernel(const __grid_constant__ WindowDesc d, int blocks) {
+    cudaGridDependencySynchronize();
+    const int group = d.Hq / d.Hkv, hk = blockIdx.y;
+    const long long per = share(all_steps(d), blocks);
+    Seq q;
+    long long tiles, all;
+    if (!find_seq(d, &q, &tiles, &all, [&](long long, long long r) { return r > (long long)blockIdx.x; })) return;
+    const Steps s(d, q.n);
+    const int t = (int)(blockIdx.x - tiles);
+    const long long from = q.before * d.Hq + hk * s.all() * group + s.before(t) * group, to = from + s.of(t) * group;
+    const int c0 = (int)(from / per), c1 = (int)((to - 1) / per);
+    if (c0 == c1) return;
+    const int r = threadIdx.x & (kT - 1), j = t * kT + r;
+    for (int at = threadIdx.x / kT; at < 2 * (DHP / 8); at += 2) {
+        const int which = at / (DHP / 8), c = at % (DHP / 8) * 8;
+        float sum[8] = {};
+        for (int b = c0; b <= c1; b++) {
+            const float* rest = d.parts + ((long long)b * 2 + (b == c0 && from != b * per ? 1 : 0)) * (2 * DHP * kT) +
+                                (which * DHP + c) * kT + r;
+#pragma unroll
+            for (int e = 0; e < 8; e++) sum[e] += rest[e * kT];
+        }
+        if (j < q.n && c < d.dh) {
+            const Heads& x = which ? d.dk : d.dv;
+            const float mul = which ? d.scale : 1.f;
+            uint4 pk;
+            __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&pk);
+#pragma unroll
+            for (int e = 0; e < 4; e++) h[e] = __floats2bfloat162_rn(sum[2 * e] * mul, sum[2 * e + 1] * mul);
+            *reinterpret_cast<uint4*>((__nv_bfloat16*)x.p + (q.row0 + j) * x.row + hk * x.head + c) = pk;
+        }
     }
 }
 
@@ -959,9 +1143,21 @@ int bwd(const WindowDesc& d, cudaStream_t s) {
         return -5;
     const long long tiles = tiles_of(d, kT);
     if (tiles * d.Hq > 0x7fffffff) return -2;
+    const int blocks = num_sms();
     window_tc_bwd_q_kernel<DHP><<<(unsigned)(tiles * d.Hq), kBwdQThreads, BwdQ<DHP>::SMEM, s>>>(q, k, v, g, d);
-    window_tc_bwd_kv_kernel<DHP><<<(unsigned)(tiles * d.Hkv), kBwdKvThreads, BwdKv<DHP>::SMEM, s>>>(q, k, v, g, d);
-    return cudaGetLastError() == cudaSuccess ? 0 : -5;
+    window_tc_bwd_kv_kernel<DHP><<<blocks, kBwdKvThreads, BwdKv<DHP>::SMEM, s>>>(q, k, v, g, d);
+    if (cudaGetLastError() != cudaSuccess) return -5;
+    // launched while the kernel before runs, and waits for it
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)tiles, d.Hkv);
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, window_tc_join_kernel<DHP>, d, blocks) == cudaSuccess ? 0 : -5;
 }
 
 }  // namespace
@@ -976,6 +1172,11 @@ int attention_window_tc(const WindowDesc& d, cudaStream_t s) { return d.dh <= 64
 bool attention_window_bwd_tc_supported(const WindowDesc& d) {
     return attention_window_tc_supported(d) && rows16(d.dout, d.T, d.Hq) && rows16(d.dq, d.T, d.Hq) &&
            rows16(d.dk, d.T, d.Hkv) && rows16(d.dv, d.T, d.Hkv);
+}
+
+// Two pieces of each block may be cut: [dv | dk][columns][128 keys] of each.
+size_t attention_window_bwd_tc_parts(int dh) {
+    return (size_t)num_sms() * 2 * 2 * (dh <= 64 ? 64 : 128) * kT * sizeof(float);
 }
 
 int attention_window_bwd_tc(const WindowDesc& d, cudaStream_t s) { return d.dh <= 64 ? bwd<64>(d, s) : bwd<128>(d, s); }

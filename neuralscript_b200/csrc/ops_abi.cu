@@ -682,13 +682,18 @@ int nsb_op_attention_window(const void* q, long long q_row, long long q_head, co
     return attention_window(d, (cudaStream_t)stream);
 }
 
+size_t nsb_op_attention_window_bwd_workspace_bytes(int T, int Hq, int Hkv, int dh, int dtype) {
+    return attention_window_bwd_workspace(T, Hq, Hkv, dh, dtype);
+}
+
 int nsb_op_attention_window_bwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row,
                                 long long k_head, const void* v, long long v_row, long long v_head, int dtype, int T,
                                 int Hq, int Hkv, int dh, const int* offsets, int B, int window, int sinks, float scale,
                                 const void* out, long long out_row, long long out_head, const float* lse, long long ld_lse,
                                 const void* dout, long long do_row, long long do_head, void* dq, long long dq_row,
                                 long long dq_head, void* dk, long long dk_row, long long dk_head, void* dv,
-                                long long dv_row, long long dv_head, float* dvec, void* stream) {
+                                long long dv_row, long long dv_head, void* workspace, size_t workspace_bytes,
+                                void* stream) {
     WindowDesc d = make_window(q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, dtype, T, Hq, Hkv, dh, offsets, B,
                                window, sinks, scale);
     d.out = heads(out, out_row, out_head);
@@ -698,8 +703,9 @@ int nsb_op_attention_window_bwd(const void* q, long long q_row, long long q_head
     d.dq = heads(dq, dq_row, dq_head);
     d.dk = heads(dk, dk_row, dk_head);
     d.dv = heads(dv, dv_row, dv_head);
-    d.dvec = dvec;
-    launch_counter() += 2;
+    d.workspace = workspace;
+    d.workspace_bytes = workspace_bytes;
+    launch_counter() += attention_window_bwd_launches(d);
     return attention_window_bwd(d, (cudaStream_t)stream);
 }
 

@@ -92,7 +92,8 @@ _sigs = {
                                   C.c_float] + _heads_args + [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "nsb_op_attention_window": (C.c_int, _window_args + _heads_args + [C.c_void_p, C.c_longlong, C.c_void_p]),
     "nsb_op_attention_window_bwd": (C.c_int, _window_args + _heads_args + [C.c_void_p, C.c_longlong] + _heads_args * 4
-                                    + [C.c_void_p, C.c_void_p]),
+                                    + [C.c_void_p, C.c_size_t, C.c_void_p]),
+    "nsb_op_attention_window_bwd_workspace_bytes": (C.c_size_t, [C.c_int] * 5),
 }
 _bound = None
 
@@ -657,9 +658,16 @@ def attention_window(q, k, v, out, lse=None, offsets=None, window=0, sinks=0, sc
         _check(rc, "nsb_op_attention_window")
 
 
-def attention_window_bwd(q, k, v, out, lse, dout, dq, dk, dv, offsets=None, window=0, sinks=0, scale=None, dvec=None):
+def attention_window_bwd_workspace(T, Hq, Hkv, dh, dtype) -> int:
+    """Bytes that attention_window_bwd works in; dtype: the tensors'."""
+    lib = _bound if _f32 else _torch()
+    return lib.nsb_op_attention_window_bwd_workspace_bytes(T, Hq, Hkv, dh, F32 if dtype is _f32 else BF16)
+
+
+def attention_window_bwd(q, k, v, out, lse, dout, dq, dk, dv, offsets=None, window=0, sinks=0, scale=None,
+                         workspace=None):
     """dq [T, Hq, dh], dk, dv [T, Hkv, dh] <- the gradients of attention_window's q, k, v for out's gradient dout, from
-    its out and lse. dvec (float32, Hq * T): scratch, allocated where it is not given."""
+    its out and lse. workspace (uint8): attention_window_bwd_workspace(...) bytes, allocated where it is not given."""
     import torch
     lib = _bound if _f32 else _torch()
     d = _device()
@@ -667,11 +675,13 @@ def attention_window_bwd(q, k, v, out, lse, dout, dq, dk, dv, offsets=None, wind
     T, Hq, dh = q.shape
     Hkv = k.shape[1]
     args = _packed(d, q, k, v, offsets, window, sinks, scale)
-    if dvec is None:
-        dvec = torch.empty(Hq * T, dtype=_f32, device=q.device)
+    if workspace is None:
+        need = lib.nsb_op_attention_window_bwd_workspace_bytes(T, Hq, Hkv, dh, F32 if dt is _f32 else BF16)
+        workspace = torch.empty(need, dtype=_u8, device=q.device)
+    have = workspace.numel()
     rc = lib.nsb_op_attention_window_bwd(
         *args, *_heads(d, out, "out", dt, T, Hq, dh), *_rows(d, lse, "lse", _f32, Hq, T),
         *_heads(d, dout, "dout", dt, T, Hq, dh), *_heads(d, dq, "dq", dt, T, Hq, dh), *_heads(d, dk, "dk", dt, T, Hkv, dh),
-        *_heads(d, dv, "dv", dt, T, Hkv, dh), _dense(d, dvec, "dvec", _f32, (Hq * T,)), _stream_of(d))
+        *_heads(d, dv, "dv", dt, T, Hkv, dh), _dense(d, workspace, "workspace", _u8, (have,)), have, _stream_of(d))
     if rc:
         _check(rc, "nsb_op_attention_window_bwd")

@@ -77,7 +77,8 @@ def test_paged_limits():
 
 WINDOW = dict(q=X, q_row=64, q_head=64, k=X, k_row=64, k_head=64, v=X, v_row=64, v_head=64, dtype=1, T=4, Hq=4, Hkv=2, dh=64, offsets=X, B=2,
               window=0, sinks=0, scale=0.125, out=X, o_row=64, o_head=64, lse=X, ld_lse=4)
-GRADS = WINDOW | dict(dout=X, do_row=64, do_head=64, dq=X, dq_row=64, dq_head=64, dk=X, dk_row=64, dk_head=64, dv=X, dv_row=64, dv_head=64, dvec=X)
+GRADS = WINDOW | dict(dout=X, do_row=64, do_head=64, dq=X, dq_row=64, dq_head=64, dk=X, dk_row=64, dk_head=64, dv=X, dv_row=64, dv_head=64, workspace=X,
+                      bytes=1 << 30)
 BAD = [dict(q=None), dict(k=None), dict(v=None), dict(dtype=2), dict(T=-1), dict(Hq=3), dict(Hkv=0), dict(dh=0), dict(dh=129),
        dict(offsets=None), dict(B=-1), dict(window=-1), dict(sinks=-1), dict(scale=0.0), dict(scale=float("nan")), dict(out=None),
        dict(ld_lse=3)]
@@ -88,7 +89,8 @@ def test_window_refuses(bad):
     assert call("nsb_op_attention_window", WINDOW, bad) == -1
 
 
-@pytest.mark.parametrize("bad", BAD + [dict(lse=None), dict(dout=None), dict(dq=None), dict(dk=None), dict(dv=None), dict(dvec=None)])
+@pytest.mark.parametrize("bad", BAD + [dict(lse=None), dict(dout=None), dict(dq=None), dict(dk=None), dict(dv=None), dict(workspace=None),
+                                       dict(workspace=X + 8), dict(bytes=63)])
 def test_window_gradient_refuses(bad):
     assert call("nsb_op_attention_window_bwd", GRADS, bad) == -1
 
