@@ -54,6 +54,12 @@ struct Waits {
     }
 };
 
+// One arrival for a whole warp, behind what all of its lanes did.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(bar);
+}
+
 // 128 rows of a head from row `row` on, 64 columns a chunk.
 template <int DHP>
 __device__ __forceinline__ void load_rows(uint8_t* to, const CUtensorMap* map, uint64_t* bar, int head, int row) {
@@ -101,14 +107,20 @@ __device__ __forceinline__ void store_cols(__nv_bfloat16* to, const uint32_t* v,
     }
 }
 
-// Columns of a tile of 128 keys from k0 on that query i sees:
-// c <= hi and (c > lo or c < front).
-struct Cols {
-    int hi, lo, front;
-    __device__ __forceinline__ Cols(const WindowDesc& d, int i, int k0)
-        : hi(i - k0), lo(d.window && i >= d.window ? i - d.window - k0 : -1), front(d.sinks - k0) {}
-    __device__ __forceinline__ bool operator()(int c) const { return c <= hi && (c > lo || c < front); }
-};
+// Bits 0 .. m - 1 of 32. Masks are words of bits: a test of a constant bit is
+// one instruction a score, comparing columns took five (3200 cycles a tile of
+// the queries' gradients in place of 1200 without a mask).
+__device__ __forceinline__ uint32_t below(int m) { return m <= 0 ? 0u : m >= 32 ? ~0u : (1u << m) - 1; }
+// Of 32 keys from j0 on those that query i sees.
+__device__ __forceinline__ uint32_t keys_seen(const WindowDesc& d, int i, int j0) {
+    const uint32_t hidden = d.window && i >= d.window ? below(i - d.window - j0 + 1) & ~below(d.sinks - j0) : 0u;
+    return below(i - j0 + 1) & ~hidden;
+}
+// Of 32 queries from i0 on those that see key j (n: the sequence's rows).
+__device__ __forceinline__ uint32_t queries_seeing(const WindowDesc& d, int j, int i0, int n) {
+    const uint32_t past = d.window == 0 || d.window >= n || j < d.sinks ? 0u : ~below(j + d.window - i0);
+    return ~below(j - i0) & ~past;
+}
 // Whether queries q0 .. q0 + 127 all see every key of the tile.
 __device__ __forceinline__ bool all_seen(const WindowDesc& d, int q0, int k0) {
     return k0 + kT - 1 <= q0 && (d.window == 0 || q0 + kT - 1 - k0 < d.window || k0 + kT - 1 < d.sinks);
@@ -153,7 +165,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     uint64_t* full = q_full + 1;
     uint64_t* empty = full + F::SLOTS;
     uint64_t* s_bar = empty + F::SLOTS;  // [2] scores of group g in TMEM
-    uint64_t* p_bar = s_bar + 2;         // [2] weights of group g in TMEM (128 arrivals)
+    uint64_t* p_bar = s_bar + 2;         // [2] weights of group g in TMEM (4 arrivals)
     uint64_t* o_bar = p_bar + 2;         // [2] product of group g added to O
     uint64_t* drain = o_bar + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -175,7 +187,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         }
         for (int g = 0; g < 2; g++) {
             ptx::mbar_init(&s_bar[g], 1);
-            ptx::mbar_init(&p_bar[g], 128);
+            ptx::mbar_init(&p_bar[g], 4);
             ptx::mbar_init(&o_bar[g], 1);
         }
         ptx::mbar_init(drain, 1);
@@ -286,10 +298,13 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 #pragma unroll
             for (int c = 0; c < 4; c++) ptx::tmem_ld_wait_regs32(a + 32 * c);
             if (!all_seen(d, q0 + g * kT, k0)) {
-                const Cols on(d, i, k0);
 #pragma unroll
-                for (int c = 0; c < 128; c++)
-                    if (!on(c)) a[c] = 0xff800000u;
+                for (int c = 0; c < 128; c += 32) {
+                    const uint32_t on = keys_seen(d, i, k0 + c);
+#pragma unroll
+                    for (int e = 0; e < 32; e++)
+                        if (!(on >> e & 1)) a[c + e] = 0xff800000u;
+                }
             }
             float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -338,7 +353,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             sum += s0 + s1;
             ptx::tmem_st_wait();
             ptx::tc_fence_before();
-            ptx::mbar_arrive(&p_bar[g]);
+            warp_arrive(&p_bar[g]);
             done++;
         }
         ok = ok && wait(&o_bar[g], done - 1);  // a query's own tile is always among its tiles
@@ -382,8 +397,8 @@ constexpr int kBwdQThreads = 576;
 template <int DHP>
 struct BwdQ {
     static constexpr int TILE = DHP / 64 * kChunk;
-    static constexpr int SLOTS = DHP == 128 ? 4 : 8;
-    static constexpr int SMEM = (2 + SLOTS) * TILE + 512 * 4 + 512 + 1024;
+    static constexpr int SLOTS = DHP == 128 ? 5 : 8;
+    static constexpr int SMEM = (2 + SLOTS) * TILE + 128 * 4 + 512 + 1024;
 };
 
 template <int DHP>
@@ -395,13 +410,13 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* ring = smem + 2 * F::TILE;
-    float* sums = reinterpret_cast<float*>(ring + F::SLOTS * F::TILE);  // [4][128] quarters of D
-    uint64_t* q_full = reinterpret_cast<uint64_t*>(sums + 512);
+    float* sums = reinterpret_cast<float*>(ring + F::SLOTS * F::TILE);  // [128] D
+    uint64_t* q_full = reinterpret_cast<uint64_t*>(sums + 128);
     uint64_t* full = q_full + 1;
     uint64_t* empty = full + F::SLOTS;
     uint64_t* s_bar = empty + F::SLOTS;  // S and dP of a tile in TMEM
-    uint64_t* r_bar = s_bar + 1;         // both read (512 arrivals)
-    uint64_t* p_bar = r_bar + 1;         // dS in TMEM (512 arrivals)
+    uint64_t* r_bar = s_bar + 1;         // both read (16 arrivals)
+    uint64_t* p_bar = r_bar + 1;         // dS in TMEM (16 arrivals)
     uint64_t* o_bar = p_bar + 1;         // product added to dQ
     uint64_t* drain = o_bar + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -420,8 +435,8 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
             ptx::mbar_init(&empty[i], 1);
         }
         ptx::mbar_init(s_bar, 1);
-        ptx::mbar_init(r_bar, 512);
-        ptx::mbar_init(p_bar, 512);
+        ptx::mbar_init(r_bar, 16);
+        ptx::mbar_init(p_bar, 16);
         ptx::mbar_init(o_bar, 1);
         ptx::mbar_init(drain, 1);
         *failed = 0;
@@ -524,9 +539,11 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
                 }
             }
         }
-        sums[part * 128 + r] = D;
-        asm volatile("bar.sync 1, 512;" ::: "memory");
-        D = (sums[r] + sums[128 + r]) + (sums[256 + r] + sums[384 + r]);
+        for (int p = 0; p < 4; p++) {  // the quarters in order
+            if (p == part) sums[r] = p ? sums[r] + D : D;
+            asm volatile("bar.sync 1, 512;" ::: "memory");
+        }
+        D = sums[r];
         if (part == 0 && i < w.n) d.dvec[(long long)h * d.T + w.row0 + i] = D;
         const uint64_t SL2 = f2_pack(sl2, sl2), NEG = f2_pack(-lse2, -lse2), ND = f2_pack(-D, -D);
         for (int x = 0; x < tiles.count; x++) {
@@ -539,9 +556,7 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
             ptx::tmem_ld_wait_regs32(a);
             ptx::tmem_ld_wait_regs32(g);
             ptx::tc_fence_before();
-            ptx::mbar_arrive(r_bar);
-            const bool whole = all_seen(d, q0, k0);
-            const Cols on(d, i, k0);
+            warp_arrive(r_bar);
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 16; e++) {
@@ -550,11 +565,18 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
                 f2_unpack(f2_mul(f2_pack(ex2(x0), ex2(x1)),
                                  f2_add(f2_pack(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1])), ND)),
                           y0, y1);
-                if (!whole) {
-                    y0 = on(part * 32 + 2 * e) ? y0 : 0.f;
-                    y1 = on(part * 32 + 2 * e + 1) ? y1 : 0.f;
-                }
-                const __nv_bfloat162 p = __floats2bfloat162_rn(y0, y1);
+                g[2 * e] = __float_as_uint(y0);
+                g[2 * e + 1] = __float_as_uint(y1);
+            }
+            if (!all_seen(d, q0, k0)) {  // a hidden place is 0 whatever its dP is
+                const uint32_t on = keys_seen(d, i, k0 + part * 32);
+#pragma unroll
+                for (int e = 0; e < 32; e++)
+                    if (!(on >> e & 1)) g[e] = 0u;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const __nv_bfloat162 p = __floats2bfloat162_rn(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]));
                 pk[e] = *reinterpret_cast<const uint32_t*>(&p);
             }
             if (x > 0) {
@@ -564,7 +586,7 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
             ptx::tmem_st16(base + 384 + part * 16, pk);
             ptx::tmem_st_wait();
             ptx::tc_fence_before();
-            ptx::mbar_arrive(p_bar);
+            warp_arrive(p_bar);
         }
         ok = ok && wait(o_bar, tiles.count - 1);
         ptx::tc_fence_after();
@@ -739,14 +761,14 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
     uint64_t* k_empty = k_full + 1;        // keys and values read by the last scores of a piece
     uint64_t* full = k_empty + 1;
     uint64_t* empty = full + F::SLOTS;
-    uint64_t* st_full = empty + F::SLOTS;  // (32 arrivals)
-    uint64_t* st_empty = st_full + kStats; // (512 arrivals)
+    uint64_t* st_full = empty + F::SLOTS;
+    uint64_t* st_empty = st_full + kStats; // (16 arrivals)
     uint64_t* s_bar = st_empty + kStats;   // S^T in TMEM
     uint64_t* g_bar = s_bar + 1;           // dP^T in TMEM
-    uint64_t* p_bar = g_bar + 1;           // P^T in TMEM (512 arrivals)
-    uint64_t* ds_bar = p_bar + 1;          // dS^T in TMEM (512 arrivals)
+    uint64_t* p_bar = g_bar + 1;           // P^T in TMEM (16 arrivals)
+    uint64_t* ds_bar = p_bar + 1;          // dS^T in TMEM (16 arrivals)
     uint64_t* sum_bar = ds_bar + 1;        // a piece's sums in TMEM
-    uint64_t* out_bar = sum_bar + 1;       // and read (512 arrivals)
+    uint64_t* out_bar = sum_bar + 1;       // and read (16 arrivals)
     uint64_t* drain = out_bar + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     int* failed = reinterpret_cast<int*>(tmem_slot + 1);
@@ -765,15 +787,15 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
             ptx::mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < kStats; i++) {
-            ptx::mbar_init(&st_full[i], 32);
-            ptx::mbar_init(&st_empty[i], 512);
+            ptx::mbar_init(&st_full[i], 1);
+            ptx::mbar_init(&st_empty[i], 16);
         }
         ptx::mbar_init(s_bar, 1);
         ptx::mbar_init(g_bar, 1);
-        ptx::mbar_init(p_bar, 512);
-        ptx::mbar_init(ds_bar, 512);
+        ptx::mbar_init(p_bar, 16);
+        ptx::mbar_init(ds_bar, 16);
         ptx::mbar_init(sum_bar, 1);
-        ptx::mbar_init(out_bar, 512);
+        ptx::mbar_init(out_bar, 16);
         ptx::mbar_init(drain, 1);
         *failed = 0;
         ptx::fence_mbar_init();
@@ -832,13 +854,13 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const int i = q0 + (t & 31) + 32 * e;
-                    // a query that saw nothing, or is none, has weights of 0
-                    l[e] = INFINITY;
+                    // (both negated.) A query that saw nothing, or is none, has weights of 0
+                    l[e] = -INFINITY;
                     D[e] = 0.f;
                     if (i < p.n) {
                         const float lse = d.lse[h * d.ld_lse + p.row0 + i];
-                        if (lse != -INFINITY) l[e] = lse * kLog2e;
-                        D[e] = d.dvec[(long long)h * d.T + p.row0 + i];
+                        if (lse != -INFINITY) l[e] = -lse * kLog2e;
+                        D[e] = -d.dvec[(long long)h * d.T + p.row0 + i];
                     }
                 }
                 if (step >= kStats && !(ok = wait(&st_empty[slot], step / kStats - 1))) break;
@@ -847,7 +869,7 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
                     stats[slot * 2 * kT + (t & 31) + 32 * e] = l[e];
                     stats[slot * 2 * kT + kT + (t & 31) + 32 * e] = D[e];
                 }
-                ptx::mbar_arrive(&st_full[slot]);
+                warp_arrive(&st_full[slot]);
             }
         }
     } else if (warp == 16) {
@@ -928,20 +950,16 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
         const int lg = warp & 3, part = warp >> 2;
         const uint32_t row = tmem + ((uint32_t)(lg * 32) << 16), base = row + 32 * part;
         const float sl2 = d.scale * kLog2e;
-        const uint64_t SL2 = f2_pack(sl2, sl2), MINUS = f2_pack(-1.f, -1.f);
+        const uint64_t SL2 = f2_pack(sl2, sl2);
         for (long long at = begin; at < end && ok; piece++) {
             const Piece p = piece_at(d, at, end);
             const int slot_of_part = at == begin ? 0 : 1;
             at += p.x1 - p.x0;
             const int j = p.k0 + lg * 32 + (t & 31);  // key of the sequence
-            const bool no_end = d.window == 0 || d.window >= p.n || j < d.sinks;
             for (int x = p.x0; x < p.x1; x++, step++) {
                 const int slot = step % kStats, q0 = (p.first + x % p.each) * kT;
                 const float4* l4 = reinterpret_cast<const float4*>(stats + slot * 2 * kT + part * 32);
                 const float4* d4 = l4 + kT / 4;
-                const bool whole = all_seen(d, q0, p.k0);
-                // queries q0 + c that see key j: lo <= c < hi
-                const int lo = j - q0 - part * 32, hi = no_end ? kT : j + d.window - q0 - part * 32;
                 if (!(ok = wait(&st_full[slot], step / kStats) && wait(s_bar, step))) break;
                 ptx::tc_fence_after();
                 uint32_t a[32], g[32], pk[16];
@@ -955,24 +973,27 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
                         const int c = 2 * (e + u);
                         float x0, x1;
                         f2_unpack(f2_fma(f2_pack(__uint_as_float(a[c]), __uint_as_float(a[c + 1])), SL2,
-                                         f2_mul(u ? f2_pack(l.z, l.w) : f2_pack(l.x, l.y), MINUS)),
+                                         u ? f2_pack(l.z, l.w) : f2_pack(l.x, l.y)),
                                   x0, x1);
-                        x0 = ex2(x0);
-                        x1 = ex2(x1);
-                        if (!whole) {
-                            x0 = c >= lo && c < hi ? x0 : 0.f;
-                            x1 = c + 1 >= lo && c + 1 < hi ? x1 : 0.f;
-                        }
-                        a[c] = __float_as_uint(x0);
-                        a[c + 1] = __float_as_uint(x1);
-                        const __nv_bfloat162 h2 = __floats2bfloat162_rn(x0, x1);
-                        pk[e + u] = *reinterpret_cast<const uint32_t*>(&h2);
+                        a[c] = __float_as_uint(ex2(x0));
+                        a[c + 1] = __float_as_uint(ex2(x1));
                     }
+                }
+                if (!all_seen(d, q0, p.k0)) {
+                    const uint32_t on = queries_seeing(d, j, q0 + part * 32, p.n);
+#pragma unroll
+                    for (int e = 0; e < 32; e++)
+                        if (!(on >> e & 1)) a[e] = 0u;
+                }
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const __nv_bfloat162 h2 = __floats2bfloat162_rn(__uint_as_float(a[2 * e]), __uint_as_float(a[2 * e + 1]));
+                    pk[e] = *reinterpret_cast<const uint32_t*>(&h2);
                 }
                 ptx::tmem_st16(base, pk);
                 ptx::tmem_st_wait();
                 ptx::tc_fence_before();
-                ptx::mbar_arrive(p_bar);
+                warp_arrive(p_bar);
                 if (!(ok = wait(g_bar, step))) break;
                 ptx::tc_fence_after();
                 ptx::tmem_ld32(base + 128, g);
@@ -985,13 +1006,9 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
                         const int c = 2 * (e + u);
                         float y0, y1;
                         f2_unpack(f2_mul(f2_pack(__uint_as_float(a[c]), __uint_as_float(a[c + 1])),
-                                         f2_fma(u ? f2_pack(D.z, D.w) : f2_pack(D.x, D.y), MINUS,
+                                         f2_add(u ? f2_pack(D.z, D.w) : f2_pack(D.x, D.y),
                                                 f2_pack(__uint_as_float(g[c]), __uint_as_float(g[c + 1])))),
                                   y0, y1);
-                        if (!whole) {  // a hidden place stays 0 whatever dP is
-                            y0 = c >= lo && c < hi ? y0 : 0.f;
-                            y1 = c + 1 >= lo && c + 1 < hi ? y1 : 0.f;
-                        }
                         const __nv_bfloat162 h2 = __floats2bfloat162_rn(y0, y1);
                         pk[e + u] = *reinterpret_cast<const uint32_t*>(&h2);
                     }
@@ -999,8 +1016,8 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
                 ptx::tmem_st16(base + 128, pk);
                 ptx::tmem_st_wait();
                 ptx::tc_fence_before();
-                ptx::mbar_arrive(ds_bar);
-                ptx::mbar_arrive(&st_empty[slot]);
+                warp_arrive(ds_bar);
+                warp_arrive(&st_empty[slot]);
             }
             if (!ok || !(ok = wait(sum_bar, piece))) break;
             ptx::tc_fence_after();
@@ -1028,7 +1045,7 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
                 }
             }
             ptx::tc_fence_before();
-            ptx::mbar_arrive(out_bar);
+            warp_arrive(out_bar);
         }
     }
     ptx::tc_fence_before();
