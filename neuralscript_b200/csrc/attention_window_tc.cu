@@ -54,6 +54,15 @@ struct Waits {
     }
 };
 
+// One lane of the warp (of all its lanes).
+__device__ __forceinline__ bool elect() {
+    uint32_t on;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(on));
+    return on;
+}
+
 // One arrival for a whole warp, behind what all of its lanes did.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
     __syncwarp();
@@ -81,15 +90,29 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int from) {
     __syncwarp();
 }
 
-// D (+)= A B^T over the heads' columns, both K-major tiles.
+// Descriptors of a tile at shared address `at`: K-major (its rows are the rows
+// or columns of the product) and MN-major (its rows are summed over).
+__device__ __forceinline__ uint64_t k_major(uint32_t at) { return ptx::smem_desc(at, 16, 1024, 2); }
+__device__ __forceinline__ uint64_t mn_major(uint32_t at) { return ptx::smem_desc(at, kChunk, 1024, 2); }
+
+// D = A B^T over the heads' columns, 16 a step, both K-major tiles.
 template <int DHP>
-__device__ __forceinline__ void mma_dot(uint32_t d, uint32_t a, uint32_t b) {
+__device__ __forceinline__ void mma_dot(uint32_t d, uint64_t a, uint64_t b) {
     constexpr uint32_t idesc = ptx::instr_desc(1, 0, 0, kT, kT);
 #pragma unroll
     for (int s = 0; s < DHP / 16; s++) {
-        const uint32_t at = (s >> 2) * kChunk + (s & 3) * 32;
-        ptx::mma_bf16(d, ptx::smem_desc(a + at, 16, 1024, 2), ptx::smem_desc(b + at, 16, 1024, 2), idesc, s > 0);
+        const uint32_t at = ((s >> 2) * kChunk + (s & 3) * 32) >> 4;
+        ptx::mma_bf16(d, a + at, b + at, idesc, s > 0);
     }
+}
+// D (+)= A B, A [128, 128] in TMEM (16 of its columns in 8, `apart` from
+// sixteen to sixteen where two lie side by side), B an MN-major tile.
+template <int DHP>
+__device__ __forceinline__ void mma_add(uint32_t d, uint32_t a, int apart, uint64_t b, bool more) {
+    constexpr uint32_t idesc = ptx::instr_desc(1, 0, 1, kT, DHP);
+#pragma unroll
+    for (int s = 0; s < kT / 16; s++)
+        ptx::mma_bf16_ts(d, a + (s >> 1) * (8 + apart) + (s & 1) * 8, b + s * (2048 >> 4), idesc, more || s > 0);
 }
 
 // N columns of an output row, `cols` of which there are.
@@ -234,9 +257,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                 ptx::mbar_wait(&full[i % F::SLOTS], (i / F::SLOTS) & 1, nullptr, 0);
         }
     } else if (warp == 8) {
-        const bool one = (t & 31) == 0;
         const uint32_t aQ = ptx::smem_u32(smem), aR = ptx::smem_u32(ring);
-        constexpr uint32_t idesc = ptx::instr_desc(1, 0, 1, kT, DHP);
         uint32_t given[2] = {0, 0};  // weights taken, by group
         ok = wait(q_full, 0);
         for (int x = 0; x <= tiles.count && ok; x++) {
@@ -253,29 +274,25 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                 if (x > 0 && uses(g, before)) {
                     if (!(ok = wait(&p_bar[g], given[g]))) break;
                     ptx::tc_fence_after();
-                    if (one) {
-#pragma unroll
-                        for (int s = 0; s < kT / 16; s++)
-                            ptx::mma_bf16_ts(tmem + 256 + 128 * g, tmem + 128 * g + 8 * s,
-                                             ptx::smem_desc(aR + sv * F::TILE + s * 2048, kChunk, 1024, 2), idesc,
-                                             given[g] > 0 || s > 0);
+                    if (elect()) {
+                        mma_add<DHP>(tmem + 256 + 128 * g, tmem + 128 * g, 8, mn_major(aR + sv * F::TILE), given[g] > 0);
                         ptx::mma_commit(&o_bar[g]);
                     }
                     given[g]++;
                 }
-                if (x < tiles.count && uses(g, kt) && one) {
+                if (x < tiles.count && uses(g, kt) && elect()) {
                     ptx::tc_fence_after();
-                    mma_dot<DHP>(tmem + 128 * g, aQ + g * F::TILE, aR + sk * F::TILE);
+                    mma_dot<DHP>(tmem + 128 * g, k_major(aQ + g * F::TILE), k_major(aR + sk * F::TILE));
                     ptx::mma_commit(&s_bar[g]);
                 }
             }
-            if (ok && one) {
+            if (ok && elect()) {
                 if (x > 0) ptx::mma_commit(&empty[sv]);
                 if (x < tiles.count) ptx::mma_commit(&empty[sk]);
             }
             __syncwarp();
         }
-        if (one) {
+        if (elect()) {
             ptx::mma_commit(drain);
             ptx::mbar_wait(drain, 0, nullptr, 0);
         }
@@ -475,9 +492,7 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
                 ptx::mbar_wait(&full[i % F::SLOTS], (i / F::SLOTS) & 1, nullptr, 0);
         }
     } else if (warp == 16) {
-        const bool one = (t & 31) == 0;
         const uint32_t aQ = ptx::smem_u32(smem), aG = aQ + F::TILE, aR = ptx::smem_u32(ring);
-        constexpr uint32_t idesc = ptx::instr_desc(1, 0, 1, kT, DHP);
         ok = wait(q_full, 0);
         for (int x = 0; x <= tiles.count && ok; x++) {
             if (x < tiles.count) {
@@ -486,9 +501,9 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
                 if ((kt + 1) * kT > w.n) zero_rows<DHP>(ring + sk * F::TILE, w.n - kt * kT);
                 if (x > 0 && !(ok = wait(r_bar, x - 1))) break;
                 ptx::tc_fence_after();
-                if (one) {
-                    mma_dot<DHP>(tmem, aQ, aR + sk * F::TILE);
-                    mma_dot<DHP>(tmem + 128, aG, aR + sv * F::TILE);
+                if (elect()) {
+                    mma_dot<DHP>(tmem, k_major(aQ), k_major(aR + sk * F::TILE));
+                    mma_dot<DHP>(tmem + 128, k_major(aG), k_major(aR + sv * F::TILE));
                     ptx::mma_commit(s_bar);
                     ptx::mma_commit(&empty[sv]);
                 }
@@ -497,18 +512,15 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
                 const int sk = 2 * (x - 1) % F::SLOTS;
                 if (!(ok = wait(p_bar, x - 1))) break;
                 ptx::tc_fence_after();
-                if (one) {
-#pragma unroll
-                    for (int s = 0; s < kT / 16; s++)
-                        ptx::mma_bf16_ts(tmem + 256, tmem + 384 + 8 * s,
-                                         ptx::smem_desc(aR + sk * F::TILE + s * 2048, kChunk, 1024, 2), idesc, x > 1 || s > 0);
+                if (elect()) {
+                    mma_add<DHP>(tmem + 256, tmem + 384, 8, mn_major(aR + sk * F::TILE), x > 1);
                     ptx::mma_commit(o_bar);
                     ptx::mma_commit(&empty[sk]);
                 }
             }
             __syncwarp();
         }
-        if (one) {
+        if (elect()) {
             ptx::mma_commit(drain);
             ptx::mbar_wait(drain, 0, nullptr, 0);
         }
@@ -873,16 +885,7 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
             }
         }
     } else if (warp == 16) {
-        const bool one = (t & 31) == 0;
         const uint32_t aK = ptx::smem_u32(smem), aV = aK + F::TILE, aR = ptx::smem_u32(ring);
-        constexpr uint32_t idesc = ptx::instr_desc(1, 0, 1, kT, DHP);
-        // d += A (bf16 of 128 queries in 4 x 16 columns, 32 apart) times the rows at b
-        auto add = [&](uint32_t d0, uint32_t a, uint32_t b, bool more) {
-#pragma unroll
-            for (int s = 0; s < kT / 16; s++)
-                ptx::mma_bf16_ts(d0, a + 32 * (s >> 1) + 8 * (s & 1), ptx::smem_desc(b + s * 2048, kChunk, 1024, 2), idesc,
-                                 more || s > 0);
-        };
         for (long long at = begin; at < end && ok; piece++) {
             const Piece p = piece_at(d, at, end);
             at += p.x1 - p.x0;
@@ -897,11 +900,11 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
             ok = wait(k_full, piece);
             if (ok) aQ = ready(p.x0, 0);
             if (ok) aG = ready(p.x0, 1);
-            if (ok && one) {
+            if (ok && elect()) {
                 ptx::tc_fence_after();
-                mma_dot<DHP>(tmem, aK, aQ);
+                mma_dot<DHP>(tmem, k_major(aK), k_major(aQ));
                 ptx::mma_commit(s_bar);
-                mma_dot<DHP>(tmem + 128, aV, aG);
+                mma_dot<DHP>(tmem + 128, k_major(aV), k_major(aG));
                 ptx::mma_commit(g_bar);
             }
             __syncwarp();
@@ -913,24 +916,24 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
                 if (!ok || !(ok = wait(p_bar, i / 2))) break;
                 // the piece before has been read out of the sums
                 if (x == p.x0 && piece && !(ok = wait(out_bar, piece - 1))) break;
-                if (one) {
+                if (elect()) {
                     ptx::tc_fence_after();
-                    add(tmem + 256, tmem, aG, x > p.x0);
+                    mma_add<DHP>(tmem + 256, tmem, 24, mn_major(aG), x > p.x0);
                     ptx::mma_commit(&empty[(i + 1) % F::SLOTS]);
                     if (more) {
-                        mma_dot<DHP>(tmem, aK, nQ);
+                        mma_dot<DHP>(tmem, k_major(aK), k_major(nQ));
                         ptx::mma_commit(s_bar);
                     }
                 }
                 __syncwarp();
                 if (more) nG = ready(x + 1, 1);
                 if (!ok || !(ok = wait(ds_bar, i / 2))) break;
-                if (one) {
+                if (elect()) {
                     ptx::tc_fence_after();
-                    add(tmem + 384, tmem + 128, aQ, x > p.x0);
+                    mma_add<DHP>(tmem + 384, tmem + 128, 24, mn_major(aQ), x > p.x0);
                     ptx::mma_commit(&empty[i % F::SLOTS]);
                     if (more) {
-                        mma_dot<DHP>(tmem + 128, aV, nG);
+                        mma_dot<DHP>(tmem + 128, k_major(aV), k_major(nG));
                         ptx::mma_commit(g_bar);
                     }
                     if (x + 2 >= p.x1 && (more || p.x1 - p.x0 == 1)) ptx::mma_commit(k_empty);
@@ -942,7 +945,7 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
             }
             step += p.x1 - p.x0;
         }
-        if (one) {
+        if (elect()) {
             ptx::mma_commit(drain);
             ptx::mbar_wait(drain, 0, nullptr, 0);
         }
