@@ -37,7 +37,17 @@ struct Waits {
     volatile int* failed;  // shared memory
     int* err;
     __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t phase) const {
-        return __all_sync(0xffffffffu, lane(bar, phase));
+        if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, phase & 1))) return true;
+        const long long t0 = clock64();
+        while (!__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, phase & 1))) {
+            const bool late = clock64() - t0 > ptx::kWaitCycles;
+            if (late) {
+                *failed = 1;
+                atomicCAS(err, 0, kErrTimeoutAttn);
+            }
+            if (__any_sync(0xffffffffu, late || *failed)) return false;
+        }
+        return true;
     }
     __device__ __forceinline__ bool lane(uint64_t* bar, uint32_t phase) const {
         if (ptx::mbar_try_wait(bar, phase & 1)) return true;
