@@ -6,14 +6,15 @@
 // that share it. One pass with the running maximum and sum of the softmax.
 //
 // Work is cut without regard to where sequences end: the visible keys of every
-// (sequence, key head), counted in tiles of 64, stand in one line, and every
-// block takes the same number of neighbouring tiles of it. (A cut into equal
+// (sequence, key head), counted in units of 16, stand in one line, and every
+// warp takes the same number of neighbouring units of it. (A cut into equal
 // parts a sequence leaves the blocks of short ones idle: the lengths of a
 // batch differ by a factor of ten and more.) The lengths are on the device,
-// so each block sums them up itself. A block writes what it covers whole; of
-// a head that other blocks share it leaves maximum, sum and weighted values
-// in the workspace, and a second kernel joins those in the order of the keys.
-// Nothing depends on timing.
+// so each block sums them up itself. A warp writes what it covers whole; of a
+// head that others share it leaves maximum, sum and weighted values in the
+// workspace (a block all of whose warps are in one head leaves one for all),
+// and a second kernel joins those in the order of the keys. Nothing depends
+// on timing.
 #include <cuda_bf16.h>
 #include <math.h>
 
@@ -27,19 +28,23 @@ namespace nsb {
 
 namespace {
 
-constexpr int kTile = 64;        // keys a tile
+constexpr int kKeys = 16;        // a unit
 constexpr int kThreads = 128;
-constexpr int kPerSm = 2;        // blocks an SM that the grid is made for
-constexpr int kMinTiles = 2;     // least tiles a block: below, joining costs more than a block saves
+constexpr int kWarps = kThreads / 32;
+constexpr int kPerSm = 2;        // most blocks an SM that the grid is made for
+constexpr int kMinUnits = 2;     // least units a warp: below, joining costs more than a warp saves
+constexpr int kSlots = 2 * kWarps + 1;  // parts that a block may leave: two a warp, or one
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct PagedArgs {
     PagedDesc d;
     int group;   // query heads that share a key head
-    int chunks;  // blocks' shares of a group
-    int* plan;   // [0]: tiles a block, [1 + b]: tiles before sequence b
-    float* part; // [grid][2] maxima, sums [HB] and values [HB][DHP]
+    int chunks;  // shares of a group
+    int blocks;
+    int shift;   // log2 of a page's places, -1: no power of two
+    int* plan;   // [0]: units a warp, [1 + b]: units before sequence b
+    float* part; // [blocks][kSlots] maxima, sums [HB] and values [HB][DHP]
 };
 
 // Visible keys of a sequence, numbered 0 .. n - 1: the first `front` are the
@@ -62,16 +67,16 @@ __device__ __forceinline__ Seen seen_of(const PagedDesc& d, int b) {
     }
     return s;
 }
-__device__ __forceinline__ int tiles_of(int n) { return n > 0 ? (n + kTile - 1) / kTile : 1; }
+__device__ __forceinline__ int units_of(int n) { return n > 0 ? (n + kKeys - 1) / kKeys : 1; }
 
-// pre[b] = tiles of the sequences before b, of one key head (pre: B + 1 ints).
+// pre[b] = units of the sequences before b, of one key head (pre: B + 1 ints).
 __device__ __forceinline__ void sum_up(const PagedDesc& d, int* pre) {
     __shared__ int s_warp[kThreads / 32];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     int carry = 0;
     if (t == 0) pre[0] = 0;
     for (int b0 = 0; b0 < d.B; b0 += kThreads) {
-        int v = b0 + t < d.B ? tiles_of(seen_of(d, b0 + t).n) : 0;
+        int v = b0 + t < d.B ? units_of(seen_of(d, b0 + t).n) : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int u = __shfl_up_sync(0xffffffffu, v, o);
@@ -91,6 +96,30 @@ __device__ __forceinline__ void sum_up(const PagedDesc& d, int* pre) {
     }
 }
 
+// Units a warp, and where the line's unit `at` is: in sequence b, share hc of
+// its heads, unit i of `units`.
+__device__ __forceinline__ long long share(long long all, int warps) {
+    const long long each = all < 0x7fffffff - warps ? ((int)all + warps - 1) / warps : (all + warps - 1) / warps;
+    return max((long long)kMinUnits, each);
+}
+struct Place {
+    int b, hc, i, units;
+};
+__device__ __forceinline__ Place locate(const int* pre, int B, int Hc, long long at) {
+    Place p;
+    p.b = 0;
+    for (int step = 1 << (31 - __clz(B)); step; step >>= 1)
+        if (p.b + step < B && (long long)pre[p.b + step] * Hc <= at) p.b += step;
+    p.units = pre[p.b + 1] - pre[p.b];
+    const long long in = at - (long long)pre[p.b] * Hc;
+    p.hc = in < 0x7fffffff ? (int)in / p.units : (int)(in / p.units);
+    p.i = (int)(in - (long long)p.hc * p.units);
+    return p;
+}
+
+__device__ __forceinline__ void put_lse(const PagedDesc& d, int b, int h, float m, float l) {
+    if (d.lse) d.lse[(long long)b * d.Hq + h] = l > 0.f ? (m + log2f(l)) * kLn2 : l == 0.f ? -INFINITY : l;
+}
 // Output of one head from its maximum (in powers of two), sum and values.
 template <typename T>
 __device__ __forceinline__ void put(const PagedDesc& d, int b, int h, int c, float m, float l, float o) {
@@ -100,7 +129,7 @@ __device__ __forceinline__ void put(const PagedDesc& d, int b, int h, int c, flo
         if constexpr (std::is_same<T, float>::value) *to = v;
         else *to = __float2bfloat16_rn(v);
     }
-    if (c == 0 && d.lse) d.lse[(long long)b * d.Hq + h] = l > 0.f ? (m + log2f(l)) * kLn2 : l == 0.f ? -INFINITY : l;
+    if (c == 0) put_lse(d, b, h, m, l);
 }
 
 __device__ __forceinline__ float ldf(const float* p) { return *p; }
@@ -115,45 +144,36 @@ __device__ __forceinline__ void load_dims(float* r, const T* p, int sub, int dh)
 
 // Any type, head size and alignment, on the fp32 units: eight lanes hold a
 // key, four keys a warp at a time, each with a softmax of its own over every
-// sixteenth key of a tile; the sixteen of a block meet at its end. HB query
-// heads share what is read.
+// fourth key of the warp's; the four meet where its keys of a head end. HB
+// query heads share what is read.
 template <typename T, int DHP, int HB>
 __global__ void __launch_bounds__(kThreads) paged_kernel(const __grid_constant__ PagedArgs a) {
     constexpr int DIMS = DHP / 8;
-    constexpr int STREAMS = kThreads / 8;
     extern __shared__ int pre[];
-    __shared__ float s_m[STREAMS][HB], s_l[STREAMS][HB];
-    __shared__ float s_o[STREAMS][DHP];
     const PagedDesc& d = a.d;
-    const int t = threadIdx.x, sub = t & 7, stream = t >> 3;
+    const int t = threadIdx.x, sub = t & 7, warp = t >> 5;
     sum_up(d, pre);
     __syncthreads();
     const int Hc = d.Hkv * a.chunks;
-    const long long W = (long long)pre[d.B] * Hc;
-    const long long per = max((long long)kMinTiles, (W + gridDim.x - 1) / gridDim.x);
+    const long long W = (long long)pre[d.B] * Hc, per = share(W, a.blocks * kWarps);
     if (blockIdx.x == 0) {
         for (int b = t; b <= d.B; b += kThreads) a.plan[1 + b] = pre[b];
         if (t == 0) a.plan[0] = (int)per;
     }
-    const long long begin = blockIdx.x * per, end = min(W, begin + per);
+    const long long begin = ((long long)blockIdx.x * kWarps + warp) * per, end = min(W, begin + per);
     const float s2 = d.scale * kLog2e;
 
     for (long long at = begin; at < end;) {
-        int b = 0;
-        for (int step = 1 << 13; step; step >>= 1)
-            if (b + step < d.B && (long long)pre[b + step] * Hc <= at) b += step;
-        const int tiles = pre[b + 1] - pre[b];
-        const long long in = at - (long long)pre[b] * Hc;
-        const int hc = (int)(in / tiles), i0 = (int)(in - (long long)hc * tiles);
-        const int i1 = (int)min((long long)tiles, i0 + (end - at));
-        const int hk = hc / a.chunks, g0 = (hc - hk * a.chunks) * HB, h0 = hk * a.group + g0;
+        const Place w = locate(pre, d.B, Hc, at);
+        const int i1 = (int)min((long long)w.units, w.i + (end - at));
+        const int hk = w.hc / a.chunks, g0 = (w.hc - hk * a.chunks) * HB, h0 = hk * a.group + g0;
         const int heads = min(HB, a.group - g0);
-        const Seen s = seen_of(d, b);
+        const Seen s = seen_of(d, w.b);
 
         float q[HB][DIMS], o[HB][DIMS], m[HB], l[HB];
 #pragma unroll
         for (int g = 0; g < HB; g++) {
-            if (g < heads) load_dims<T, DIMS>(q[g], (const T*)d.q.p + b * d.q.row + (h0 + g) * d.q.head, sub, d.dh);
+            if (g < heads) load_dims<T, DIMS>(q[g], (const T*)d.q.p + w.b * d.q.row + (h0 + g) * d.q.head, sub, d.dh);
             m[g] = -INFINITY;
             l[g] = 0.f;
 #pragma unroll
@@ -162,20 +182,20 @@ __global__ void __launch_bounds__(kThreads) paged_kernel(const __grid_constant__
                 o[g][j] = 0.f;
             }
         }
-        const int last = min(s.n, i1 * kTile);
-        for (int x = i0 * kTile + stream; x < last; x += STREAMS) {
+        const int last = min(s.n, i1 * kKeys);
+        for (int x = w.i * kKeys + (t >> 3 & 3); x < last; x += 4) {
             const int key = x < s.front ? x : x - s.front + s.back;
             const int pi = key / d.page;
-            const int page = d.table[b * d.ld_table + pi];
+            const int page = d.table[w.b * d.ld_table + pi];
             if (page < 0 || page >= d.pages) {  // no such page: its keys are left out
                 atomicCAS(d.err, 0, kErrBadIndex);
                 continue;
             }
             float k[DIMS], v[DIMS];
-            load_dims<T, DIMS>(k, (const T*)d.kc.p + page * d.kc.page + (key - pi * d.page) * d.kc.slot + hk * d.kc.head,
-                                    sub, d.dh);
-            load_dims<T, DIMS>(v, (const T*)d.vc.p + page * d.vc.page + (key - pi * d.page) * d.vc.slot + hk * d.vc.head,
-                                    sub, d.dh);
+            load_dims<T, DIMS>(k, (const T*)d.kc.p + page * d.kc.page + (key - pi * d.page) * d.kc.slot + hk * d.kc.head, sub,
+                               d.dh);
+            load_dims<T, DIMS>(v, (const T*)d.vc.p + page * d.vc.page + (key - pi * d.page) * d.vc.slot + hk * d.vc.head, sub,
+                               d.dh);
             const uint32_t mates = 0xffu << (threadIdx.x & 24);
 #pragma unroll
             for (int g = 0; g < HB; g++) {
@@ -194,46 +214,38 @@ __global__ void __launch_bounds__(kThreads) paged_kernel(const __grid_constant__
                 for (int j = 0; j < DIMS; j++) o[g][j] = fmaf(p, v[j], o[g][j] * turn);
             }
         }
-        // the block's streams meet, head by head
-        const bool whole = i0 == 0 && i1 == tiles;
-        float* part = a.part + ((long long)blockIdx.x * 2 + (at == begin ? 0 : 1)) * (HB * (DHP + 2));
-        __syncthreads();
-        if (sub == 0) {
-#pragma unroll
-            for (int g = 0; g < HB; g++) s_m[stream][g] = m[g], s_l[stream][g] = l[g];
-        }
+        __syncwarp();
+        const bool whole = w.i == 0 && i1 == w.units;
+        float* part = a.part + ((long long)blockIdx.x * kSlots + 2 * warp + (at == begin ? 0 : 1)) * (HB * (DHP + 2));
 #pragma unroll
         for (int g = 0; g < HB; g++) {
-            __syncthreads();
+            float top = m[g];
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            const float f = exp2f(m[g] - (top == -INFINITY ? 0.f : top));
+            float sum = l[g] * f;
+            sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
 #pragma unroll
-            for (int j = 0; j < DIMS; j++) s_o[stream][j * 8 + sub] = o[g][j];
-            __syncthreads();
-            if (t < DHP && g < heads) {
-                float top = -INFINITY, sum = 0.f, val = 0.f;
-                for (int i = 0; i < STREAMS; i++) top = fmaxf(top, s_m[i][g]);
-                const float safe = top == -INFINITY ? 0.f : top;
-                for (int i = 0; i < STREAMS; i++) {
-                    const float w = exp2f(s_m[i][g] - safe);
-                    sum = fmaf(s_l[i][g], w, sum);
-                    val = fmaf(s_o[i][t], w, val);
-                }
-                if (whole) {
-                    put<T>(d, b, h0 + g, t, top, sum, val);
-                } else {
-                    part[2 * HB + g * DHP + t] = val;
-                    if (t == 0) part[g] = top, part[HB + g] = sum;
-                }
+            for (int j = 0; j < DIMS; j++) {
+                float val = o[g][j] * f;
+                val += __shfl_xor_sync(0xffffffffu, val, 8);
+                val += __shfl_xor_sync(0xffffffffu, val, 16);
+                const int col = j * 8 + sub;
+                if (g >= heads || (t & 31) >= 8) continue;
+                if (whole) put<T>(d, w.b, h0 + g, col, top, sum, val);
+                else part[2 * HB + g * DHP + col] = val;
             }
+            if (!whole && g < heads && (t & 31) == 0) part[g] = top, part[HB + g] = sum;
         }
-        at += i1 - i0;
+        at += i1 - w.i;
     }
 }
 
 // ---------------------------------------------------------------------------
-// The same from 16-byte pieces. Each of four warps takes 16 keys of every
-// tile, through a ring of its own in shared memory that cp.async fills some
-// tiles ahead, over the borders of heads and sequences too: no barrier of the
-// block stands between two tiles. Pieces of a row are exchanged by the row's
+// The same from 16-byte pieces. Each warp has a ring of its own in shared
+// memory that cp.async fills some units ahead, over the borders of heads and
+// sequences too; no barrier of the block stands between two units. Pieces of a row are exchanged by the row's
 // lowest three bits, so that neither reading rows nor columns meets a bank
 // twice. What is behind a sequence's end, or on no page, arrives as zeros.
 //
@@ -245,9 +257,6 @@ __global__ void __launch_bounds__(kThreads) paged_kernel(const __grid_constant__
 // fp32: on the fp32 units, two lanes a key for the scores, and four columns a
 // lane for the values.
 // ---------------------------------------------------------------------------
-constexpr int kWarps = kThreads / 32;
-constexpr int kKeys = kTile / kWarps;  // of a warp in a tile: 16
-
 template <typename T, int DHP>
 struct Ring {
     static constexpr int ROW = DHP * (int)sizeof(T);
@@ -258,38 +267,49 @@ struct Ring {
     static constexpr int PER_SM = BYTES <= 108 * 1024 ? 2 : 1;
 };
 
-// Where a warp's next tile is; `offset`: of this lane's row, -1 for none
-// (lanes 0 .. 15 the keys', 16 .. 31 the values' rows).
-struct Cursor {
-    int b, hc, i, tiles;
-    Seen s;
-    int page;  // of the row, from the table; -1: no such key
-    int place;
+// Of a unit to fetch, the page (from the table; -1: no such key) and the place
+// of this lane's row (lanes 0 .. 15 the keys', 16 .. 31 the values').
+struct Row {
+    int page, place, hk;
+    bool real;
 };
-
-__device__ __forceinline__ void look_up(const PagedArgs& a, Cursor& c, bool real) {
-    const int x = c.i * kTile + (threadIdx.x >> 5) * kKeys + (threadIdx.x & (kKeys - 1));
-    c.page = -1;
-    if (real && x < c.s.n) {
-        const int key = x < c.s.front ? x : x - c.s.front + c.s.back;
-        const int pi = key / a.d.page;
-        c.place = key - pi * a.d.page;
-        c.page = a.d.table[c.b * a.d.ld_table + pi];
-        if (c.page < 0 || c.page >= a.d.pages) {
-            c.page = -1;
-            atomicCAS(a.d.err, 0, kErrBadIndex);
+// Where a warp's next unit is.
+struct Cursor {
+    Place w;
+    Seen s;
+    __device__ __forceinline__ void next(const PagedArgs& a, const int* pre, int Hc) {
+        if (++w.i < w.units) return;
+        w.i = 0;
+        if (++w.hc < Hc) return;
+        w.hc = 0;
+        if (++w.b < a.d.B) {
+            w.units = pre[w.b + 1] - pre[w.b];
+            s = seen_of(a.d, w.b);
         }
     }
-}
+    __device__ __forceinline__ Row look_up(const PagedArgs& a) const {
+        Row r{-1, 0, w.hc / a.chunks, false};
+        const int x = w.i * kKeys + (threadIdx.x & (kKeys - 1));
+        if (x < s.n) {
+            const int key = x < s.front ? x : x - s.front + s.back;
+            const int pi = a.shift >= 0 ? key >> a.shift : key / a.d.page;
+            r.place = key - pi * a.d.page;
+            r.page = a.d.table[w.b * a.d.ld_table + pi];
+            r.real = true;
+        }
+        return r;
+    }
+};
 
 template <typename T, int DHP>
-__device__ __forceinline__ void fetch(const PagedArgs& a, const Cursor& c, uint8_t* stage, uint32_t* mask) {
+__device__ __forceinline__ void fetch(const PagedArgs& a, Row c, uint8_t* stage, uint32_t* mask) {
     constexpr int PIECES = DHP * (int)sizeof(T) / 16, ROWS = 32 / PIECES > 0 ? 32 / PIECES : 1;
     const int lane = threadIdx.x & 31;
-    const int hk = c.hc / a.chunks;
     const Pages& mine = lane < kKeys ? a.d.kc : a.d.vc;
-    const long long offset = c.page < 0 ? -1 : c.page * mine.page + c.place * mine.slot + hk * mine.head;
-    const uint32_t there = __ballot_sync(0xffffffffu, c.page >= 0);
+    const bool there_is = c.page >= 0 && c.page < a.d.pages;
+    const long long offset = there_is ? c.page * mine.page + c.place * mine.slot + c.hk * mine.head : -1;
+    const uint32_t there = __ballot_sync(0xffffffffu, there_is);
+    if (c.real && !there_is) atomicCAS(a.d.err, 0, kErrBadIndex);  // no such page: its keys are left out
     if (lane == 0) *mask = there;
     const int piece = lane % PIECES;
     const bool inside = piece * 16 < a.d.dh * (int)sizeof(T);
@@ -417,6 +437,63 @@ struct State {
             for (int n = 0; n < NT; n++) mma16816(o[k][n], a, p[n][0], p[n][1]);
         }
     }
+    __device__ __forceinline__ float total(int n, int e) const {
+        float sum = l[n][e];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        return sum + __shfl_xor_sync(0xffffffffu, sum, 16);
+    }
+    // the heads' outputs
+    __device__ __forceinline__ void finish(const PagedDesc& d, int b, int h0, int heads) const {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            float mul[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const float sum = total(n, e);
+                mul[e] = sum == 0.f ? 0.f : 1.f / sum;
+                const int h = n * 8 + 2 * (lane & 3) + e;
+                if (lane < 4 && h < heads) put_lse(d, b, h0 + h, m[n][e], sum);
+            }
+            const int h = n * 8 + (lane >> 2);  // behind the transpose
+            __nv_bfloat16* to = (__nv_bfloat16*)d.out.p + b * d.out.row + (h0 + h) * d.out.head + 2 * (lane & 3);
+            const bool pairs = (reinterpret_cast<uintptr_t>(to) & 3) == 0;
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const __nv_bfloat162 v = __floats2bfloat162_rn(o[k][n][2 * e] * mul[0], o[k][n][2 * e + 1] * mul[1]);
+                    const uint32_t w = turned(*reinterpret_cast<const uint32_t*>(&v));
+                    const int c = 16 * k + 8 * e;
+                    if (h >= heads || c + 2 * (lane & 3) >= d.dh) continue;
+                    if (pairs) {
+                        *reinterpret_cast<uint32_t*>(to + c) = w;
+                    } else {
+                        const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&w);
+                        to[c] = x.x;
+                        to[c + 1] = x.y;
+                    }
+                }
+        }
+    }
+    // what others join
+    __device__ __forceinline__ void part(float* to) const {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const float sum = total(n, e);
+                const int h = n * 8 + 2 * (lane & 3) + e;
+                if (lane < 4) to[h] = m[n][e], to[HB + h] = sum;
+#pragma unroll
+                for (int k = 0; k < KS; k++) {
+                    to[2 * HB + h * DHP + 16 * k + (lane >> 2)] = o[k][n][e];
+                    to[2 * HB + h * DHP + 16 * k + (lane >> 2) + 8] = o[k][n][2 + e];
+                }
+            }
+    }
     // maxima [4], sums [4] and values [4][DHP] of heads 4 round .. + 3
     __device__ __forceinline__ void leave(float* to, int round) {
         const int lane = threadIdx.x & 31;
@@ -425,10 +502,7 @@ struct State {
             if (n != round >> 1) continue;
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                float sum = l[n][e];
-                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                const float sum = total(n, e);
                 const int h = 2 * (lane & 1) + e;
                 if ((lane >> 1 & 1) != (round & 1)) continue;
                 if (lane < 4) to[h] = m[n][e], to[4 + h] = sum;
@@ -509,20 +583,43 @@ struct State<float, DHP, HB> {
             }
         }
     }
-    __device__ __forceinline__ void leave(float* to, int) {
-        const int lane = threadIdx.x & 31;
+    template <typename F>
+    __device__ __forceinline__ void each_head(F use) const {  // use(head, sum, value e of this lane's columns ..)
 #pragma unroll
         for (int g = 0; g < HB; g++) {
-            float sum = l[g];
+            float sum = l[g], v[4];
 #pragma unroll
             for (int x = 1; x < 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-            if (lane == 0) to[g] = m[g], to[4 + g] = sum;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (SHARE == 2) o[g][e] += __shfl_xor_sync(0xffffffffu, o[g][e], 16);
-                if (lane < COLS) to[8 + g * DHP + lane * 4 + e] = o[g][e];
-            }
+            for (int e = 0; e < 4; e++) v[e] = SHARE == 2 ? o[g][e] + __shfl_xor_sync(0xffffffffu, o[g][e], 16) : o[g][e];
+            use(g, sum, v);
         }
+    }
+    __device__ __forceinline__ void finish(const PagedDesc& d, int b, int h0, int heads) const {
+        const int lane = threadIdx.x & 31;
+        each_head([&](int g, float sum, const float* v) {
+            if (g >= heads || lane >= COLS) return;
+#pragma unroll
+            for (int e = 0; e < 4; e++) put<float>(d, b, h0 + g, lane * 4 + e, m[g], sum, v[e]);
+        });
+    }
+    __device__ __forceinline__ void part(float* to) const {
+        const int lane = threadIdx.x & 31;
+        each_head([&](int g, float sum, const float* v) {
+            if (lane == 0) to[g] = m[g], to[HB + g] = sum;
+            if (lane >= COLS) return;
+#pragma unroll
+            for (int e = 0; e < 4; e++) to[2 * HB + g * DHP + lane * 4 + e] = v[e];
+        });
+    }
+    __device__ __forceinline__ void leave(float* to, int) const {
+        const int lane = threadIdx.x & 31;
+        each_head([&](int g, float sum, const float* v) {
+            if (lane == 0) to[g] = m[g], to[4 + g] = sum;
+            if (lane >= COLS) return;
+#pragma unroll
+            for (int e = 0; e < 4; e++) to[8 + g * DHP + lane * 4 + e] = v[e];
+        });
     }
 };
 
@@ -543,106 +640,118 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DHP>::PER_SM) paged_ring_ker
     sum_up(d, pre);
     __syncthreads();
     const int Hc = d.Hkv * a.chunks;
-    const long long W = (long long)pre[d.B] * Hc;
-    const long long per = max((long long)kMinTiles, (W + gridDim.x - 1) / gridDim.x);
+    const long long W = (long long)pre[d.B] * Hc, per = share(W, a.blocks * kWarps);
     if (blockIdx.x == 0) {
         for (int b = t; b <= d.B; b += kThreads) a.plan[1 + b] = pre[b];
         if (t == 0) a.plan[0] = (int)per;
     }
-    const long long begin = blockIdx.x * per, end = min(W, begin + per);
+    const long long first = (long long)blockIdx.x * kWarps * per;
+    if (first >= W) return;
+    const long long begin = min(W, first + warp * per), end = min(W, begin + per);
     const float s2 = d.scale * kLog2e;
-    if (begin >= end) return;
+    // whether all of the block's units are in one head's line
+    const Place f = locate(pre, d.B, Hc, first);
+    const bool together = f.i + (min(W, first + kWarps * per) - first) <= f.units;
 
-    Cursor c;  // of the tile to fetch
-    c.b = 0;
-    for (int step = 1 << 13; step; step >>= 1)
-        if (c.b + step < d.B && (long long)pre[c.b + step] * Hc <= begin) c.b += step;
-    c.tiles = pre[c.b + 1] - pre[c.b];
-    c.hc = (int)((begin - (long long)pre[c.b] * Hc) / c.tiles);
-    c.i = (int)(begin - (long long)pre[c.b] * Hc - (long long)c.hc * c.tiles);
-    c.s = seen_of(d, c.b);
-    int b = c.b, hc = c.hc, i = c.i, tiles = c.tiles;  // of the tile to add
-    long long ahead = begin;
-    look_up(a, c, true);
-    auto fetch_next = [&](int slot) {
-        if (ahead < end) {
-            fetch<T, DHP>(a, c, ring + slot * R::STAGE, mask + slot);
-            ahead++;
-            if (++c.i == c.tiles) {
-                c.i = 0;
-                if (++c.hc == Hc) {
-                    c.hc = 0;
-                    if (++c.b < d.B) {
-                        c.tiles = pre[c.b + 1] - pre[c.b];
-                        c.s = seen_of(d, c.b);
-                    }
-                }
-            }
-            look_up(a, c, ahead < end);  // a tile before it is wanted
+    Cursor c;  // of the next unit to look up
+    c.w = begin < W ? locate(pre, d.B, Hc, begin) : f;
+    c.s = seen_of(d, c.w.b);
+    Place w = c.w;  // of the next unit to add
+    Row ahead[R::STAGES - 1];
+    long long looked = begin, fetched = begin;
+#pragma unroll
+    for (int s = 0; s < R::STAGES - 1; s++)
+        if (looked < end) {
+            ahead[s] = c.look_up(a);
+            c.next(a, pre, Hc);
+            looked++;
+        }
+#pragma unroll
+    for (int s = 0; s < R::STAGES - 1; s++) {
+        if (fetched < end) {
+            fetch<T, DHP>(a, ahead[s], ring + s * R::STAGE, mask + s);
+            fetched++;
         }
         commit();
-    };
-    for (int s = 0; s < R::STAGES - 1; s++) fetch_next(s);
+    }
+    Row row = {};
+    if (looked < end) row = c.look_up(a);
 
     State<T, DHP, HB> state;
     int slot = 0;
     for (long long at = begin; at < end;) {
-        const int hk = hc / a.chunks, g0 = (hc - hk * a.chunks) * HB, h0 = hk * a.group + g0;
+        const int hk = w.hc / a.chunks, g0 = (w.hc - hk * a.chunks) * HB, h0 = hk * a.group + g0;
         const int heads = min(HB, a.group - g0);
-        const int i1 = (int)min((long long)tiles, i + (end - at));
-        const bool whole = i == 0 && i1 == tiles;
-        float* part = a.part + ((long long)blockIdx.x * 2 + (at == begin ? 0 : 1)) * (HB * (DHP + 2));
-        at += i1 - i;
-        state.start(d, b, h0, heads, queries);
-        for (; i < i1; i++) {
+        const int i1 = (int)min((long long)w.units, w.i + (end - at));
+        const bool whole = w.i == 0 && i1 == w.units;
+        const int which = 2 * warp + (at == begin ? 0 : 1);
+        at += i1 - w.i;
+        state.start(d, w.b, h0, heads, queries);
+        for (; w.i < i1; w.i++) {
             wait_but<R::STAGES - 2>();
             __syncwarp();  // every lane's pieces are there, and the slot before has been read
-            fetch_next(slot == 0 ? R::STAGES - 1 : slot - 1);
+            if (looked < end) {
+                const int to = slot == 0 ? R::STAGES - 1 : slot - 1;
+                fetch<T, DHP>(a, row, ring + to * R::STAGE, mask + to);
+                c.next(a, pre, Hc);
+                if (++looked < end) row = c.look_up(a);  // a unit before it is wanted
+            }
+            commit();
             if constexpr (std::is_same<T, float>::value) state.add(ring + slot * R::STAGE, mask[slot], s2, queries);
             else state.add(ptx::smem_u32(ring + slot * R::STAGE), mask[slot], s2, nullptr);
             slot = slot + 1 == R::STAGES ? 0 : slot + 1;
         }
-        // the warps meet, four heads at a time
-        for (int round = 0; round < ROUNDS; round++) {
-            __syncthreads();
-            state.leave(mine, round);
-            __syncthreads();
-            for (int e = t; e < MEET * DHP; e += kThreads) {
-                const int g = e / DHP, col = e % DHP, head = round * MEET + g;
-                float top = -INFINITY, sum = 0.f, val = 0.f;
-#pragma unroll
-                for (int w = 0; w < kWarps; w++) top = fmaxf(top, meet[w * R::MEET * (DHP + 2) + g]);
-                const float safe = top == -INFINITY ? 0.f : top;
-#pragma unroll
-                for (int w = 0; w < kWarps; w++) {
-                    const float* x = meet + w * R::MEET * (DHP + 2);
-                    const float f = exp2f(x[g] - safe);
-                    sum = fmaf(x[4 + g], f, sum);
-                    val = fmaf(x[8 + g * DHP + col], f, val);
-                }
-                if (head >= heads) continue;
-                if (whole) {
-                    put<T>(d, b, h0 + head, col, top, sum, val);
-                } else {
-                    part[2 * HB + head * DHP + col] = val;
-                    if (col == 0) part[head] = top, part[HB + head] = sum;
-                }
+        if (together) break;
+        if (whole) state.finish(d, w.b, h0, heads);
+        else state.part(a.part + ((long long)blockIdx.x * kSlots + which) * (HB * (DHP + 2)));
+        if (w.i == w.units) {
+            w.i = 0;
+            if (++w.hc == Hc) {
+                w.hc = 0;
+                if (++w.b < d.B) w.units = pre[w.b + 1] - pre[w.b];
             }
         }
-        if (i == tiles) {
-            i = 0;
-            if (++hc == Hc) {
-                hc = 0;
-                if (++b < d.B) tiles = pre[b + 1] - pre[b];
+    }
+    if (!together) return;
+    // the warps meet, four heads at a time
+    const int hk = f.hc / a.chunks, g0 = (f.hc - hk * a.chunks) * HB, h0 = hk * a.group + g0, heads = min(HB, a.group - g0);
+    const bool whole = f.i == 0 && min(W, first + kWarps * per) - first == f.units;
+    float* part = a.part + ((long long)blockIdx.x * kSlots + 2 * kWarps) * (HB * (DHP + 2));
+    if (begin >= end) state.start(d, f.b, h0, 0, queries);  // nothing of it
+    for (int round = 0; round < ROUNDS; round++) {
+        if (round) __syncthreads();
+        state.leave(mine, round);
+        __syncthreads();
+        for (int e = t; e < MEET * DHP; e += kThreads) {
+            const int g = e / DHP, col = e % DHP, head = round * MEET + g;
+            float top = -INFINITY, sum = 0.f, val = 0.f;
+#pragma unroll
+            for (int x = 0; x < kWarps; x++) top = fmaxf(top, meet[x * R::MEET * (DHP + 2) + g]);
+            const float safe = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int x = 0; x < kWarps; x++) {
+                const float* from = meet + x * R::MEET * (DHP + 2);
+                const float share = exp2f(from[g] - safe);
+                sum = fmaf(from[4 + g], share, sum);
+                val = fmaf(from[8 + g * DHP + col], share, val);
+            }
+            if (head >= heads) continue;
+            if (whole) {
+                put<T>(d, f.b, h0 + head, col, top, sum, val);
+            } else {
+                part[2 * HB + head * DHP + col] = val;
+                if (col == 0) part[head] = top, part[HB + head] = sum;
             }
         }
     }
 }
 
-// Joins what several blocks left of one head: eight warps take every eighth
-// part, and meet at the end.
+// Joins what several warps left of one head: eight warps take every eighth
+// part, and meet at the end. Parts are numbered through the blocks: one of a
+// block that is in the head's line with all of its units (where the blocks
+// meet, `together`), else its warps'.
 template <typename T, int DHP, int HB>
-__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedArgs a) {
+__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedArgs a, bool merges) {
     constexpr int C = DHP / 32;
     __shared__ float s_m[8], s_l[8], s_o[8][DHP];
     const PagedDesc& d = a.d;
@@ -650,23 +759,47 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     const int Hc = d.Hkv * a.chunks;
     const int b = blockIdx.x / Hc, hc = blockIdx.x - b * Hc, g = blockIdx.y;
     const int hk = hc / a.chunks, g0 = (hc - hk * a.chunks) * HB;
-    const long long per = a.plan[0];
-    const int before = a.plan[1 + b], tiles = a.plan[2 + b] - before;
-    const long long t0 = (long long)before * Hc + (long long)hc * tiles;
-    const int c0 = (int)(t0 / per), c1 = (int)((t0 + tiles - 1) / per);
-    if (c0 == c1 || g0 + g >= a.group) return;
+    if (g0 + g >= a.group) return;
+    const long long per = a.plan[0], block = per * kWarps, W = (long long)a.plan[1 + d.B] * Hc;
+    const int before = a.plan[1 + b], units = a.plan[2 + b] - before;
+    const long long t0 = (long long)before * Hc + (long long)hc * units, t1 = t0 + units;
+    const int c0 = (int)(t0 / block), c1 = (int)((t1 - 1) / block);
+    auto inside = [&](int c) { return merges && t0 <= c * block && min(W, (c + 1) * block) <= t1; };
+    const bool in0 = inside(c0), in1 = inside(c1);
+    if (c0 == c1 && in0) return;              // one block had it all,
+    if (t0 / per == (t1 - 1) / per) return;  // or one warp
+    const int n0 = in0 ? 1 : kWarps, n = c0 == c1 ? n0 : n0 + (c1 - c0 - 1) * (merges ? 1 : kWarps) + (in1 ? 1 : kWarps);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float m = -INFINITY, l = 0.f, o[C] = {};
-    for (int c = c0 + warp; c <= c1; c += 8) {
-        // in the first block the head begins behind others, unless at its very start
-        const float* part = a.part + ((long long)c * 2 + (c == c0 && t0 != c * per ? 1 : 0)) * (HB * (DHP + 2));
+    for (int x = warp; x < n; x += 8) {
+        int c, w;  // block, and warp of it (-1: all)
+        if (x < n0) {
+            c = c0;
+            w = in0 ? -1 : x;
+        } else if (merges && x < n0 + c1 - c0 - 1) {
+            c = c0 + 1 + x - n0;
+            w = -1;
+        } else if (merges) {
+            c = c1;
+            w = in1 ? -1 : x - (n0 + c1 - c0 - 1);
+        } else {
+            c = c0 + x / kWarps;
+            w = x % kWarps;
+        }
+        int slot = 2 * kWarps;
+        if (w >= 0) {
+            const long long from = c * block + w * per;
+            if (from >= t1 || from + per <= t0) continue;  // (a warp of this block in another head)
+            slot = 2 * w + (from < t0 ? 1 : 0);
+        }
+        const float* part = a.part + ((long long)c * kSlots + slot) * (HB * (DHP + 2));
         const float mc = part[g], lc = part[HB + g];
         const float top = fmaxf(m, mc), safe = top == -INFINITY ? 0.f : top;
-        const float turn = exp2f(m - safe), w = exp2f(mc - safe);
+        const float turn = exp2f(m - safe), share = exp2f(mc - safe);
         m = top;
-        l = fmaf(lc, w, l * turn);
+        l = fmaf(lc, share, l * turn);
 #pragma unroll
-        for (int j = 0; j < C; j++) o[j] = fmaf(part[2 * HB + g * DHP + lane + 32 * j], w, o[j] * turn);
+        for (int j = 0; j < C; j++) o[j] = fmaf(part[2 * HB + g * DHP + lane + 32 * j], share, o[j] * turn);
     }
     if (lane == 0) s_m[warp] = m, s_l[warp] = l;
 #pragma unroll
@@ -699,7 +832,7 @@ bool vectors(const void* p, long long a, long long b, long long c, int size) {
 
 size_t attention_paged_workspace(int B, int Hq, int Hkv, int dh) {
     if (B <= 0 || Hkv <= 0 || Hq < Hkv || Hq % Hkv || dh <= 0 || dh > kAttnMaxHead) return 0;
-    return plan_bytes(B) + (size_t)num_sms() * kPerSm * 2 * heads_a_block(Hq / Hkv, true) * (padded(dh) + 2) * sizeof(float);
+    return plan_bytes(B) + (size_t)num_sms() * kPerSm * kSlots * heads_a_block(Hq / Hkv, true) * (padded(dh) + 2) * sizeof(float);
 }
 
 int attention_paged_launches() { return 2; }
@@ -713,10 +846,10 @@ int attention_paged(const PagedDesc& d, cudaStream_t st) {
         return -1;
     if (d.B > kPagedMaxBatch) return -2;
     if (d.B == 0) return 0;
-    // tiles are counted in 32 bits, those of one block too
+    // units are counted in 32 bits, those of one warp too
     const long long room = (long long)d.width * d.page, seen = d.window ? (long long)d.window + d.sinks : room;
-    if ((room < seen ? room : seen) / kTile * d.B >= (1LL << 31) - kPagedMaxBatch ||
-        (room < seen ? room : seen) / kTile * d.B * d.Hq >= 1LL << 37)
+    if ((room < seen ? room : seen) / kKeys * d.B >= (1LL << 31) - kPagedMaxBatch ||
+        (room < seen ? room : seen) / kKeys * d.B * d.Hq >= 1LL << 39)
         return -2;
     if (!d.q.p || !d.out.p || !d.lens || (d.width && !d.table) || (d.pages && (!d.kc.p || !d.vc.p))) return -1;
     if (!d.workspace || reinterpret_cast<uintptr_t>(d.workspace) % 16 ||
@@ -726,6 +859,9 @@ int attention_paged(const PagedDesc& d, cudaStream_t st) {
     PagedArgs a;
     a.d = d;
     a.group = d.Hq / d.Hkv;
+    a.shift = -1;
+    for (int i = 0; i < 31; i++)
+        if (d.page == 1 << i) a.shift = i;
     a.plan = reinterpret_cast<int*>(d.workspace);
     a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(d.workspace) + plan_bytes(d.B));
     const int size = d.dtype == kBF16 ? 2 : 4;
@@ -742,9 +878,11 @@ int attention_paged(const PagedDesc& d, cudaStream_t st) {
             const size_t queries = std::is_same<T, float>::value ? (size_t)kWarps * HB * DHP * sizeof(float) : 0;
             const size_t bytes = R::BYTES + (size_t)((d.B + 4) & ~3) * sizeof(int) + queries;
             if (cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return -5;
-            f<<<num_sms() * R::PER_SM, kThreads, bytes, st>>>(a);
+            a.blocks = num_sms() * R::PER_SM;
+            f<<<a.blocks, kThreads, bytes, st>>>(a);
         } else {
-            paged_kernel<T, DHP, HB><<<num_sms() * kPerSm, kThreads, (d.B + 1) * sizeof(int), st>>>(a);
+            a.blocks = num_sms() * kPerSm;
+            paged_kernel<T, DHP, HB><<<a.blocks, kThreads, (d.B + 1) * sizeof(int), st>>>(a);
         }
         if (cudaGetLastError() != cudaSuccess) return -5;
         // the second kernel is launched while the first runs, and waits for it
@@ -757,7 +895,7 @@ int attention_paged(const PagedDesc& d, cudaStream_t st) {
         at.val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = &at;
         cfg.numAttrs = 1;
-        return cudaLaunchKernelEx(&cfg, paged_join_kernel<T, DHP, HB>, a) == cudaSuccess ? 0 : -5;
+        return cudaLaunchKernelEx(&cfg, paged_join_kernel<T, DHP, HB>, a, (bool)decltype(aligned)::value) == cudaSuccess ? 0 : -5;
     };
     using std::integral_constant;
     auto by_heads = [&](auto zero, auto wide) {
