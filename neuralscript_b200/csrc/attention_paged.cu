@@ -746,75 +746,94 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DHP>::PER_SM) paged_ring_ker
     }
 }
 
-// Joins what several warps left of one head: eight warps take every eighth
-// part, and meet at the end. Parts are numbered through the blocks: one of a
-// block that is in the head's line with all of its units (where the blocks
-// meet, `together`), else its warps'.
+// Joins what several warps left of one head. Parts are numbered through the
+// blocks: one of a block that is in the head's line with all of its units
+// (where the blocks meet, `together`), else its warps'. 256 parts at a time:
+// a thread each for maxima and sums, which gives every part its weight, then
+// eight warps add up every eighth part's values, whose loads wait for nothing.
 template <typename T, int DHP, int HB>
 __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedArgs a, bool merges) {
     constexpr int C = DHP / 32;
-    __shared__ float s_m[8], s_l[8], s_o[8][DHP];
+    __shared__ float s_top[8], s_sum[8], s_w[256], s_o[8][DHP];
+    __shared__ int s_at[256];
     const PagedDesc& d = a.d;
     cudaGridDependencySynchronize();
     const int Hc = d.Hkv * a.chunks;
     const int b = blockIdx.x / Hc, hc = blockIdx.x - b * Hc, g = blockIdx.y;
     const int hk = hc / a.chunks, g0 = (hc - hk * a.chunks) * HB;
     if (g0 + g >= a.group) return;
-    const long long per = a.plan[0], block = per * kWarps, W = (long long)a.plan[1 + d.B] * Hc;
     const int before = a.plan[1 + b], units = a.plan[2 + b] - before;
+    const long long per = a.plan[0], W = (long long)a.plan[1 + d.B] * Hc;
     const long long t0 = (long long)before * Hc + (long long)hc * units, t1 = t0 + units;
-    const int c0 = (int)(t0 / block), c1 = (int)((t1 - 1) / block);
+    const bool small = W < 0x7fffffff;  // (a division of 64 bits takes a hundred instructions)
+    const long long w0 = small ? (int)t0 / (int)per : t0 / per, w1 = small ? (int)(t1 - 1) / (int)per : (t1 - 1) / per;
+    if (w0 == w1) return;  // one warp had it all
+    const long long block = per * kWarps;
+    const int c0 = (int)(w0 / kWarps), c1 = (int)(w1 / kWarps);
     auto inside = [&](int c) { return merges && t0 <= c * block && min(W, (c + 1) * block) <= t1; };
     const bool in0 = inside(c0), in1 = inside(c1);
-    if (c0 == c1 && in0) return;              // one block had it all,
-    if (t0 / per == (t1 - 1) / per) return;  // or one warp
-    const int n0 = in0 ? 1 : kWarps, n = c0 == c1 ? n0 : n0 + (c1 - c0 - 1) * (merges ? 1 : kWarps) + (in1 ? 1 : kWarps);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (c0 == c1 && in0) return;  // or one block
+    // parts of the first block, of those between, and of the last
+    const int n0 = in0 ? 1 : kWarps, each = merges ? 1 : kWarps, n1 = c0 == c1 ? n0 : n0 + (c1 - c0 - 1) * each;
+    const int n = c0 == c1 ? n0 : n1 + (in1 ? 1 : kWarps);
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
     float m = -INFINITY, l = 0.f, o[C] = {};
-    for (int x = warp; x < n; x += 8) {
-        int c, w;  // block, and warp of it (-1: all)
-        if (x < n0) {
-            c = c0;
-            w = in0 ? -1 : x;
-        } else if (merges && x < n0 + c1 - c0 - 1) {
-            c = c0 + 1 + x - n0;
-            w = -1;
-        } else if (merges) {
-            c = c1;
-            w = in1 ? -1 : x - (n0 + c1 - c0 - 1);
-        } else {
-            c = c0 + x / kWarps;
-            w = x % kWarps;
-        }
-        int slot = 2 * kWarps;
-        if (w >= 0) {
+    for (int x0 = 0; x0 < n; x0 += 256) {
+        const int x = x0 + t;
+        int at = -1;
+        float mc = -INFINITY, lc = 0.f;
+        if (x < n) {
+            const int c = x < n0 ? c0 : x < n1 ? c0 + 1 + (x - n0) / each : c1;
+            const int w = x < n0 ? (in0 ? -1 : x) : x < n1 ? (merges ? -1 : (x - n0) % kWarps) : in1 ? -1 : x - n1;
             const long long from = c * block + w * per;
-            if (from >= t1 || from + per <= t0) continue;  // (a warp of this block in another head)
-            slot = 2 * w + (from < t0 ? 1 : 0);
+            if (w < 0) at = c * kSlots + 2 * kWarps;
+            else if (from < t1 && from + per > t0) at = c * kSlots + 2 * w + (from < t0 ? 1 : 0);  // else in another head
+            if (at >= 0) {
+                mc = a.part[(long long)at * (HB * (DHP + 2)) + g];
+                lc = a.part[(long long)at * (HB * (DHP + 2)) + HB + g];
+            }
         }
-        const float* part = a.part + ((long long)c * kSlots + slot) * (HB * (DHP + 2));
-        const float mc = part[g], lc = part[HB + g];
-        const float top = fmaxf(m, mc), safe = top == -INFINITY ? 0.f : top;
-        const float turn = exp2f(m - safe), share = exp2f(mc - safe);
-        m = top;
-        l = fmaf(lc, share, l * turn);
+        float top = mc;
 #pragma unroll
-        for (int j = 0; j < C; j++) o[j] = fmaf(part[2 * HB + g * DHP + lane + 32 * j], share, o[j] * turn);
+        for (int s = 1; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+        if (lane == 0) s_top[warp] = top;
+        __syncthreads();
+        top = m;
+#pragma unroll
+        for (int w = 0; w < 8; w++) top = fmaxf(top, s_top[w]);
+        const float safe = top == -INFINITY ? 0.f : top, turn = exp2f(m - safe), share = exp2f(mc - safe);
+        s_w[t] = share;
+        s_at[t] = at;
+        float sum = lc * share;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+        if (lane == 0) s_sum[warp] = sum;
+        __syncthreads();
+        m = top;
+        l *= turn;
+#pragma unroll
+        for (int w = 0; w < 8; w++) l += s_sum[w];
+#pragma unroll
+        for (int j = 0; j < C; j++) o[j] *= turn;
+#pragma unroll 4
+        for (int y = warp; y < min(256, n - x0); y += 8) {
+            const int from = s_at[y];
+            const float w = s_w[y];
+            if (from < 0) continue;
+#pragma unroll
+            for (int j = 0; j < C; j++)
+                o[j] = fmaf(a.part[(long long)from * (HB * (DHP + 2)) + 2 * HB + g * DHP + lane + 32 * j], w, o[j]);
+        }
+        __syncthreads();
     }
-    if (lane == 0) s_m[warp] = m, s_l[warp] = l;
 #pragma unroll
     for (int j = 0; j < C; j++) s_o[warp][lane + 32 * j] = o[j];
     __syncthreads();
-    if (threadIdx.x < DHP) {
-        float top = -INFINITY, sum = 0.f, val = 0.f;
-        for (int i = 0; i < 8; i++) top = fmaxf(top, s_m[i]);
-        const float safe = top == -INFINITY ? 0.f : top;
-        for (int i = 0; i < 8; i++) {
-            const float w = exp2f(s_m[i] - safe);
-            sum = fmaf(s_l[i], w, sum);
-            val = fmaf(s_o[i][threadIdx.x], w, val);
-        }
-        put<T>(d, b, hk * a.group + g0 + g, threadIdx.x, top, sum, val);
+    if (t < DHP) {
+        float val = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; w++) val += s_o[w][t];
+        put<T>(d, b, hk * a.group + g0 + g, t, m, l, val);
     }
 }
 
