@@ -31,7 +31,7 @@ namespace {
 constexpr int kKeys = 16;        // a unit
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
-constexpr int kPerSm = 2;        // most blocks an SM that the grid is made for
+constexpr int kPerSm = 3;        // most blocks an SM that the grid is made for
 constexpr int kMinUnits = 2;     // least units a warp: below, joining costs more than a warp saves
 constexpr int kSlots = 2 * kWarps + 1;  // parts that a block may leave: two a warp, or one
 constexpr float kLog2e = 1.4426950408889634f;
@@ -42,6 +42,7 @@ struct PagedArgs {
     int group;   // query heads that share a key head
     int chunks;  // shares of a group
     int blocks;
+    bool same;   // keys and values have the same strides
     int shift;   // log2 of a page's places, -1: no power of two
     int* plan;   // [0]: units a warp, [1 + b]: units before sequence b
     float* part; // [blocks][kSlots] maxima, sums [HB] and values [HB][DHP]
@@ -257,14 +258,18 @@ __global__ void __launch_bounds__(kThreads) paged_kernel(const __grid_constant__
 // fp32: on the fp32 units, two lanes a key for the scores, and four columns a
 // lane for the values.
 // ---------------------------------------------------------------------------
-template <typename T, int DHP>
+//
+// One unit ahead is enough (a unit's arithmetic takes longer than memory's
+// answer), and twelve warps an SM hide each other's latencies: with eight and
+// two units ahead the same arithmetic left 60 % of the issue slots empty.
+template <typename T, int DHP, int HB>
 struct Ring {
     static constexpr int ROW = DHP * (int)sizeof(T);
     static constexpr int STAGE = 2 * kKeys * ROW;  // keys, values
-    static constexpr int STAGES = ROW == 128 ? 6 : 3;
+    static constexpr int STAGES = ROW == 128 ? 4 : 2;
     static constexpr int MEET = 4;  // heads whose results meet at a time
     static constexpr int BYTES = kWarps * STAGES * STAGE + kWarps * MEET * (DHP + 2) * 4 + kWarps * STAGES * 4;
-    static constexpr int PER_SM = BYTES <= 108 * 1024 ? 2 : 1;
+    static constexpr int PER_SM = ROW == 512 ? 1 : HB * DHP > 1024 ? 2 : 3;  // by shared memory, and registers
 };
 
 // Of a unit to fetch, the page (from the table; -1: no such key) and the place
@@ -301,26 +306,54 @@ struct Cursor {
     }
 };
 
+// 16 bytes, zeros where `on` does not hold.
+__device__ __forceinline__ void ptx_copy(uint32_t to, const void* from, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Offsets are counted in pieces of 16 bytes: 32 bits reach 64 GB.
+constexpr uint32_t kNone = 0xffffffffu;
+
 template <typename T, int DHP>
-__device__ __forceinline__ void fetch(const PagedArgs& a, Row c, uint8_t* stage, uint32_t* mask) {
-    constexpr int PIECES = DHP * (int)sizeof(T) / 16, ROWS = 32 / PIECES > 0 ? 32 / PIECES : 1;
+__device__ __forceinline__ void fetch(const PagedArgs& a, Row c, uint32_t stage, uint32_t* mask) {
+    constexpr int ROW = DHP * (int)sizeof(T), PIECES = ROW / 16, ROWS = 32 / PIECES;
     const int lane = threadIdx.x & 31;
-    const Pages& mine = lane < kKeys ? a.d.kc : a.d.vc;
     const bool there_is = c.page >= 0 && c.page < a.d.pages;
-    const long long offset = there_is ? c.page * mine.page + c.place * mine.slot + c.hk * mine.head : -1;
     const uint32_t there = __ballot_sync(0xffffffffu, there_is);
     if (c.real && !there_is) atomicCAS(a.d.err, 0, kErrBadIndex);  // no such page: its keys are left out
     if (lane == 0) *mask = there;
     const int piece = lane % PIECES;
     const bool inside = piece * 16 < a.d.dh * (int)sizeof(T);
+    const char* nothing = (const char*)a.d.q.p;  // an address for copies of no bytes
+    const char *k = (const char*)a.d.kc.p + piece * 16, *v = (const char*)a.d.vc.p + piece * 16;
+    if (a.same) {  // keys and values lie alike
+        const uint32_t offset =
+            there_is ? (uint32_t)((c.page * a.d.kc.page + c.place * a.d.kc.slot + c.hk * a.d.kc.head) / (16 / (int)sizeof(T))) : kNone;
+#pragma unroll
+        for (int r0 = 0; r0 < kKeys; r0 += ROWS) {
+            const int row = r0 + lane / PIECES;
+            const uint32_t at = __shfl_sync(0xffffffffu, offset, row);
+            const bool on = at != kNone && inside;
+            const uint32_t to = stage + row * ROW + ((piece ^ (row & 7)) << 4);
+            ptx_copy(to, on ? k + (size_t)at * 16 : nothing, on);
+            ptx_copy(to + kKeys * ROW, on ? v + (size_t)at * 16 : nothing, on);
+        }
+        return;
+    }
+    const Pages& mine = lane < kKeys ? a.d.kc : a.d.vc;
+    const uint32_t offset =
+        there_is ? (uint32_t)((c.page * mine.page + c.place * mine.slot + c.hk * mine.head) / (16 / (int)sizeof(T))) : kNone;
 #pragma unroll
     for (int r0 = 0; r0 < 2 * kKeys; r0 += ROWS) {  // rows of the keys, then of the values
         const int row = r0 + lane / PIECES;
-        const long long at = __shfl_sync(0xffffffffu, offset, row);
-        const T* base = (const T*)(r0 < kKeys ? a.d.kc.p : a.d.vc.p);
-        const bool on = at >= 0 && inside;
-        ptx::cp_async16(stage + row * (DHP * (int)sizeof(T)) + ((piece ^ (row & 7)) << 4),
-                        on ? base + at + piece * (16 / (int)sizeof(T)) : (const T*)a.d.q.p, on ? 16 : 0);
+        const uint32_t at = __shfl_sync(0xffffffffu, offset, row);
+        const bool on = at != kNone && inside;
+        ptx_copy(stage + row * ROW + ((piece ^ (row & 7)) << 4), on ? (r0 < kKeys ? k : v) + (size_t)at * 16 : nothing, on);
     }
 }
 
@@ -408,11 +441,11 @@ struct State {
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                 top = fmaxf(top, m[n][e]);
                 const float safe = top == -INFINITY ? 0.f : top;
-                turn[n][e] = exp2f(m[n][e] - safe);
+                turn[n][e] = ex2(m[n][e] - safe);
                 rise |= top != m[n][e];
                 m[n][e] = top;
-                s[n][e] = exp2f(s[n][e] - safe);
-                s[n][2 + e] = exp2f(s[n][2 + e] - safe);
+                s[n][e] = ex2(s[n][e] - safe);
+                s[n][2 + e] = ex2(s[n][2 + e] - safe);
                 l[n][e] = fmaf(l[n][e], turn[n][e], s[n][e] + s[n][2 + e]);
             }
             const __nv_bfloat162 lo = __floats2bfloat162_rn(s[n][0], s[n][1]), hi = __floats2bfloat162_rn(s[n][2], s[n][3]);
@@ -560,8 +593,8 @@ struct State<float, DHP, HB> {
 #pragma unroll
             for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
             top = fmaxf(top, m[g]);
-            const float safe = top == -INFINITY ? 0.f : top, turn = exp2f(m[g] - safe);
-            p[g] = exp2f(z[g] - safe);
+            const float safe = top == -INFINITY ? 0.f : top, turn = ex2(m[g] - safe);
+            p[g] = ex2(z[g] - safe);
             m[g] = top;
             l[g] = fmaf(l[g], turn, p[g]);
 #pragma unroll
@@ -624,8 +657,8 @@ struct State<float, DHP, HB> {
 };
 
 template <typename T, int DHP, int HB>
-__global__ void __launch_bounds__(kThreads, Ring<T, DHP>::PER_SM) paged_ring_kernel(const __grid_constant__ PagedArgs a) {
-    using R = Ring<T, DHP>;
+__global__ void __launch_bounds__(kThreads, Ring<T, DHP, HB>::PER_SM) paged_ring_kernel(const __grid_constant__ PagedArgs a) {
+    using R = Ring<T, DHP, HB>;
     constexpr int ROUNDS = HB > R::MEET ? HB / R::MEET : 1, MEET = HB < R::MEET ? HB : R::MEET;
     extern __shared__ __align__(128) uint8_t smem[];
     float* meet = reinterpret_cast<float*>(smem + kWarps * R::STAGES * R::STAGE);
@@ -636,6 +669,7 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DHP>::PER_SM) paged_ring_ker
     float* mine = meet + warp * R::MEET * (DHP + 2);
     float* queries = reinterpret_cast<float*>(pre + ((d.B + 4) & ~3)) + warp * HB * DHP;  // (fp32)
     uint8_t* ring = smem + warp * R::STAGES * R::STAGE;
+    const uint32_t ring_at = ptx::smem_u32(ring);
     uint32_t* mask = masks + warp * R::STAGES;
     sum_up(d, pre);
     __syncthreads();
@@ -669,7 +703,7 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DHP>::PER_SM) paged_ring_ker
 #pragma unroll
     for (int s = 0; s < R::STAGES - 1; s++) {
         if (fetched < end) {
-            fetch<T, DHP>(a, ahead[s], ring + s * R::STAGE, mask + s);
+            fetch<T, DHP>(a, ahead[s], ring_at + s * R::STAGE, mask + s);
             fetched++;
         }
         commit();
@@ -692,13 +726,13 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DHP>::PER_SM) paged_ring_ker
             __syncwarp();  // every lane's pieces are there, and the slot before has been read
             if (looked < end) {
                 const int to = slot == 0 ? R::STAGES - 1 : slot - 1;
-                fetch<T, DHP>(a, row, ring + to * R::STAGE, mask + to);
+                fetch<T, DHP>(a, row, ring_at + to * R::STAGE, mask + to);
                 c.next(a, pre, Hc);
                 if (++looked < end) row = c.look_up(a);  // a unit before it is wanted
             }
             commit();
             if constexpr (std::is_same<T, float>::value) state.add(ring + slot * R::STAGE, mask[slot], s2, queries);
-            else state.add(ptx::smem_u32(ring + slot * R::STAGE), mask[slot], s2, nullptr);
+            else state.add(ring_at + slot * R::STAGE, mask[slot], s2, nullptr);
             slot = slot + 1 == R::STAGES ? 0 : slot + 1;
         }
         if (together) break;
@@ -884,7 +918,12 @@ int attention_paged(const PagedDesc& d, cudaStream_t st) {
     a.plan = reinterpret_cast<int*>(d.workspace);
     a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(d.workspace) + plan_bytes(d.B));
     const int size = d.dtype == kBF16 ? 2 : 4;
-    const bool vec = vectors(d.q.p, d.q.row, d.q.head, 0, size) && d.dh * size % 16 == 0 &&
+    a.same = d.kc.page == d.vc.page && d.kc.slot == d.vc.slot && d.kc.head == d.vc.head;
+    auto near = [&](const Pages& x) {  // offsets in pieces of 16 bytes fit 32 bits
+        return x.page >= 0 && x.slot >= 0 && x.head >= 0 &&
+               ((double)x.page * d.pages + (double)x.slot * d.page + (double)x.head * d.Hkv) * size / 16 < 4294967000.0;
+    };
+    const bool vec = near(d.kc) && near(d.vc) && vectors(d.q.p, d.q.row, d.q.head, 0, size) && d.dh * size % 16 == 0 &&
                      vectors(d.kc.p, d.kc.page, d.kc.slot, d.kc.head, size) &&
                      vectors(d.vc.p, d.vc.page, d.vc.slot, d.vc.head, size);
     auto go = [&](auto zero, auto wide, auto many, auto aligned) {
@@ -892,7 +931,7 @@ int attention_paged(const PagedDesc& d, cudaStream_t st) {
         constexpr int DHP = decltype(wide)::value, HB = decltype(many)::value;
         a.chunks = (a.group + HB - 1) / HB;
         if constexpr (decltype(aligned)::value) {
-            using R = Ring<T, DHP>;
+            using R = Ring<T, DHP, HB>;
             auto f = paged_ring_kernel<T, DHP, HB>;
             const size_t queries = std::is_same<T, float>::value ? (size_t)kWarps * HB * DHP * sizeof(float) : 0;
             const size_t bytes = R::BYTES + (size_t)((d.B + 4) & ~3) * sizeof(int) + queries;
