@@ -23,6 +23,7 @@
 #include "attention_cache.h"
 #include "gemm.h"
 #include "ptx.cuh"
+#include "shared_memory.h"
 
 namespace nsb {
 
@@ -153,6 +154,7 @@ __global__ void __launch_bounds__(kThreads) paged_kernel(const __grid_constant__
     extern __shared__ int pre[];
     const PagedDesc& d = a.d;
     const int t = threadIdx.x, sub = t & 7, warp = t >> 5;
+    cudaTriggerProgrammaticLaunchCompletion();  // the join's blocks take the places of those that end
     sum_up(d, pre);
     __syncthreads();
     const int Hc = d.Hkv * a.chunks;
@@ -307,8 +309,17 @@ struct Cursor {
 };
 
 // 16 bytes, zeros where `on` does not hold.
-__device__ __forceinline__ void ptx_copy(uint32_t to, const void* from, bool on) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(on ? 16 : 0) : "memory");
+// The cache is read once: it leaves L2 first, so that what is read again
+// (parts, tables, and the kernels' own code) stays.
+__device__ __forceinline__ uint64_t once() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool on, uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(to), "l"(from), "r"(on ? 16 : 0),
+                 "l"(policy)
+                 : "memory");
 }
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -320,7 +331,7 @@ __device__ __forceinline__ float ex2(float x) {
 constexpr uint32_t kNone = 0xffffffffu;
 
 template <typename T, int DHP>
-__device__ __forceinline__ void fetch(const PagedArgs& a, Row c, uint32_t stage, uint32_t* mask) {
+__device__ __forceinline__ void fetch(const PagedArgs& a, Row c, uint32_t stage, uint32_t* mask, uint64_t policy) {
     constexpr int ROW = DHP * (int)sizeof(T), PIECES = ROW / 16, ROWS = 32 / PIECES;
     const int lane = threadIdx.x & 31;
     const bool there_is = c.page >= 0 && c.page < a.d.pages;
@@ -340,8 +351,8 @@ __device__ __forceinline__ void fetch(const PagedArgs& a, Row c, uint32_t stage,
             const uint32_t at = __shfl_sync(0xffffffffu, offset, row);
             const bool on = at != kNone && inside;
             const uint32_t to = stage + row * ROW + ((piece ^ (row & 7)) << 4);
-            ptx_copy(to, on ? k + (size_t)at * 16 : nothing, on);
-            ptx_copy(to + kKeys * ROW, on ? v + (size_t)at * 16 : nothing, on);
+            copy16(to, on ? k + (size_t)at * 16 : nothing, on, policy);
+            copy16(to + kKeys * ROW, on ? v + (size_t)at * 16 : nothing, on, policy);
         }
         return;
     }
@@ -353,7 +364,8 @@ __device__ __forceinline__ void fetch(const PagedArgs& a, Row c, uint32_t stage,
         const int row = r0 + lane / PIECES;
         const uint32_t at = __shfl_sync(0xffffffffu, offset, row);
         const bool on = at != kNone && inside;
-        ptx_copy(stage + row * ROW + ((piece ^ (row & 7)) << 4), on ? (r0 < kKeys ? k : v) + (size_t)at * 16 : nothing, on);
+        copy16(stage + row * ROW + ((piece ^ (row & 7)) << 4), on ? (r0 < kKeys ? k : v) + (size_t)at * 16 : nothing, on,
+               policy);
     }
 }
 
@@ -671,6 +683,7 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DHP, HB>::PER_SM) paged_ring
     uint8_t* ring = smem + warp * R::STAGES * R::STAGE;
     const uint32_t ring_at = ptx::smem_u32(ring);
     uint32_t* mask = masks + warp * R::STAGES;
+    cudaTriggerProgrammaticLaunchCompletion();  // the join's blocks take the places of those that end
     sum_up(d, pre);
     __syncthreads();
     const int Hc = d.Hkv * a.chunks;
@@ -688,9 +701,12 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DHP, HB>::PER_SM) paged_ring
     const bool together = f.i + (min(W, first + kWarps * per) - first) <= f.units;
 
     Cursor c;  // of the next unit to look up
-    c.w = begin < W ? locate(pre, d.B, Hc, begin) : f;
+    c.w = f;
+    if (f.i + (begin - first) < f.units) c.w.i += (int)(begin - first);
+    else if (begin < W) c.w = locate(pre, d.B, Hc, begin);
     c.s = seen_of(d, c.w.b);
     Place w = c.w;  // of the next unit to add
+    const uint64_t policy = once();
     Row ahead[R::STAGES - 1];
     long long looked = begin, fetched = begin;
 #pragma unroll
@@ -703,7 +719,7 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DHP, HB>::PER_SM) paged_ring
 #pragma unroll
     for (int s = 0; s < R::STAGES - 1; s++) {
         if (fetched < end) {
-            fetch<T, DHP>(a, ahead[s], ring_at + s * R::STAGE, mask + s);
+            fetch<T, DHP>(a, ahead[s], ring_at + s * R::STAGE, mask + s, policy);
             fetched++;
         }
         commit();
@@ -726,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DHP, HB>::PER_SM) paged_ring
             __syncwarp();  // every lane's pieces are there, and the slot before has been read
             if (looked < end) {
                 const int to = slot == 0 ? R::STAGES - 1 : slot - 1;
-                fetch<T, DHP>(a, row, ring_at + to * R::STAGE, mask + to);
+                fetch<T, DHP>(a, row, ring_at + to * R::STAGE, mask + to, policy);
                 c.next(a, pre, Hc);
                 if (++looked < end) row = c.look_up(a);  // a unit before it is wanted
             }
@@ -849,14 +865,19 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
         for (int w = 0; w < 8; w++) l += s_sum[w];
 #pragma unroll
         for (int j = 0; j < C; j++) o[j] *= turn;
-#pragma unroll 4
-        for (int y = warp; y < min(256, n - x0); y += 8) {
-            const int from = s_at[y];
-            const float w = s_w[y];
-            if (from < 0) continue;
+        const float* values = a.part + 2 * HB + g * DHP + lane;
+        for (int y0 = warp; y0 < min(256, n - x0); y0 += 64) {  // eight parts' loads at once
+            float v[8][C];
 #pragma unroll
-            for (int j = 0; j < C; j++)
-                o[j] = fmaf(a.part[(long long)from * (HB * (DHP + 2)) + 2 * HB + g * DHP + lane + 32 * j], w, o[j]);
+            for (int u = 0; u < 8; u++) {
+                const int from = y0 + 8 * u < 256 ? s_at[y0 + 8 * u] : -1;
+#pragma unroll
+                for (int j = 0; j < C; j++) v[u][j] = from >= 0 ? values[(long long)from * (HB * (DHP + 2)) + 32 * j] : 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++)
+#pragma unroll
+                for (int j = 0; j < C; j++) o[j] = fmaf(v[u][j], y0 + 8 * u < 256 ? s_w[y0 + 8 * u] : 0.f, o[j]);
         }
         __syncthreads();
     }
@@ -935,7 +956,8 @@ int attention_paged(const PagedDesc& d, cudaStream_t st) {
             auto f = paged_ring_kernel<T, DHP, HB>;
             const size_t queries = std::is_same<T, float>::value ? (size_t)kWarps * HB * DHP * sizeof(float) : 0;
             const size_t bytes = R::BYTES + (size_t)((d.B + 4) & ~3) * sizeof(int) + queries;
-            if (cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return -5;
+            static size_t most[kMaxDevices];
+            if (!allow_shared(f, bytes, most)) return -5;
             a.blocks = num_sms() * R::PER_SM;
             f<<<a.blocks, kThreads, bytes, st>>>(a);
         } else {

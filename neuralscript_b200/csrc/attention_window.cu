@@ -22,6 +22,7 @@
 #include "attention_cache.h"
 #include "attention_window.cuh"
 #include "gemm.h"
+#include "shared_memory.h"
 
 namespace nsb {
 
@@ -314,13 +315,6 @@ constexpr int smem_of(int heads, int scores) {
     return (heads * kB * ld_of<DHP>() + scores * kB * kLdS) * (int)sizeof(float);
 }
 
-// Sets a kernel's shared memory on the current device (once would do, but
-// costs a table for each kernel; the call takes well below a microsecond).
-template <typename F>
-bool room(F f, int bytes) {
-    return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
-}
-
 int check(const WindowDesc& d) {
     if (d.T < 0 || d.Hkv <= 0 || d.Hq < d.Hkv || d.Hq % d.Hkv || d.dh <= 0 || d.dh > kAttnMaxHead ||
         (d.dtype != kF32 && d.dtype != kBF16) || d.B < 0 || d.window < 0 || d.sinks < 0 || !(d.scale > 0.f) ||
@@ -354,7 +348,8 @@ int attention_window(const WindowDesc& d, cudaStream_t st) {
     return by_type(d, [&](auto zero, auto wide) {
         using T = decltype(zero);
         constexpr int DHP = decltype(wide)::value, bytes = smem_of<DHP>(3, 1);
-        if (!room(window_fwd_kernel<T, DHP>, bytes)) return -5;
+        static size_t most[kMaxDevices];
+        if (!allow_shared(window_fwd_kernel<T, DHP>, bytes, most)) return -5;
         window_fwd_kernel<T, DHP><<<dim3((unsigned)tiles_of(d, kB), d.Hq), kThreads, bytes, st>>>(d);
         return cudaGetLastError() == cudaSuccess ? 0 : -5;
     });
@@ -385,7 +380,9 @@ int attention_window_bwd(const WindowDesc& given, cudaStream_t st) {
     return by_type(d, [&](auto zero, auto wide) {
         using T = decltype(zero);
         constexpr int DHP = decltype(wide)::value, bq = smem_of<DHP>(4, 1), bk = smem_of<DHP>(4, 2);
-        if (!room(window_bwd_q_kernel<T, DHP>, bq) || !room(window_bwd_kv_kernel<T, DHP>, bk)) return -5;
+        static size_t most_q[kMaxDevices], most_kv[kMaxDevices];
+        if (!allow_shared(window_bwd_q_kernel<T, DHP>, bq, most_q) || !allow_shared(window_bwd_kv_kernel<T, DHP>, bk, most_kv))
+            return -5;
         window_bwd_q_kernel<T, DHP><<<dim3((unsigned)tiles_of(d, kB), d.Hq), kThreads, bq, st>>>(d);
         window_bwd_kv_kernel<T, DHP><<<dim3((unsigned)tiles_of(d, kB), d.Hkv), kThreads, bk, st>>>(d);
         return cudaGetLastError() == cudaSuccess ? 0 : -5;

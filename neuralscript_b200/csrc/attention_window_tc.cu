@@ -15,6 +15,7 @@
 #include "common.cuh"
 #include "gemm.h"
 #include "ptx.cuh"
+#include "shared_memory.h"
 
 namespace nsb {
 
@@ -1144,11 +1145,6 @@ bool rows16(const Heads& x, int T, int H) {
     return reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && fits(x.row, T) && fits(x.head, H);
 }
 
-template <typename K>
-bool room(K kernel, int bytes) {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
-}
-
 long long tiles_of(const WindowDesc& d, int rows) { return ((long long)d.T + rows - 1) / rows + (d.offsets ? d.B : 0); }
 
 template <int DHP>
@@ -1156,7 +1152,8 @@ int fwd(const WindowDesc& d, cudaStream_t s) {
     CUtensorMap q, k, v;
     if (!make_map(&q, d.q, d.T, d.Hq, d.dh) || !make_map(&k, d.k, d.T, d.Hkv, d.dh) || !make_map(&v, d.v, d.T, d.Hkv, d.dh))
         return -2;
-    if (!room(window_tc_fwd_kernel<DHP>, Fwd<DHP>::SMEM)) return -5;
+    static size_t most[kMaxDevices];
+    if (!allow_shared(window_tc_fwd_kernel<DHP>, Fwd<DHP>::SMEM, most)) return -5;
     const long long blocks = tiles_of(d, 2 * kT) * d.Hq;
     if (blocks > 0x7fffffff) return -2;
     window_tc_fwd_kernel<DHP><<<(unsigned)blocks, kFwdThreads, Fwd<DHP>::SMEM, s>>>(q, k, v, d);
@@ -1169,7 +1166,9 @@ int bwd(const WindowDesc& d, cudaStream_t s) {
     if (!make_map(&q, d.q, d.T, d.Hq, d.dh) || !make_map(&k, d.k, d.T, d.Hkv, d.dh) || !make_map(&v, d.v, d.T, d.Hkv, d.dh) ||
         !make_map(&g, d.dout, d.T, d.Hq, d.dh))
         return -2;
-    if (!room(window_tc_bwd_q_kernel<DHP>, BwdQ<DHP>::SMEM) || !room(window_tc_bwd_kv_kernel<DHP>, BwdKv<DHP>::SMEM))
+    static size_t most_q[kMaxDevices], most_kv[kMaxDevices];
+    if (!allow_shared(window_tc_bwd_q_kernel<DHP>, BwdQ<DHP>::SMEM, most_q) ||
+        !allow_shared(window_tc_bwd_kv_kernel<DHP>, BwdKv<DHP>::SMEM, most_kv))
         return -5;
     const long long tiles = tiles_of(d, kT);
     if (tiles * d.Hq > 0x7fffffff) return -2;

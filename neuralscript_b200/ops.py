@@ -221,15 +221,16 @@ def moe_route(x, Wg, active, best, pb, probs=None):
 # anything is launched; see include/ns_b200_ops.h for the definitions.
 # ---------------------------------------------------------------------------
 _SCORE = {"softmax": 0, "sigmoid": 1}
-_f32 = _bf16 = _i32 = _u8 = _f8 = _stream_of = _device = None
+_f32 = _bf16 = _i32 = _u8 = _f8 = _stream_of = _device = _empty = None
 
 
 def _torch():
     """torch's names that every call below needs, looked up once (a decode step's kernels take a few microseconds)."""
-    global _f32, _bf16, _i32, _u8, _f8, _stream_of, _device
+    global _f32, _bf16, _i32, _u8, _f8, _stream_of, _device, _empty
     import torch
     lib = L()  # raises where the library is missing, in this call and in the next
     _stream_of, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+    _empty = torch.empty
     _bf16, _i32, _u8, _f8 = torch.bfloat16, torch.int32, torch.uint8, torch.float8_e4m3fn
     _f32 = torch.float32  # last: where it is set, other threads find all the rest
     return lib
@@ -521,6 +522,19 @@ def _ints(d, t, what, rows, cols):
     return _rows(d, t, what, _i32, rows, cols)
 
 
+def _workspace(need, d):
+    """Scratch of this call: the allocator hands it on to calls of the same stream alone, and a graph's keeps to itself."""
+    return _empty(need, dtype=_u8, device=_cuda[d])
+
+
+class _Devices(dict):
+    def __missing__(self, d):
+        import torch
+        self[d] = torch.device("cuda", d)
+        return self[d]
+
+
+_cuda = _Devices()
 _NO_TURN = (None, 0, 0, None, None, 0, 0, 1.0)
 
 
@@ -611,7 +625,6 @@ def attention_paged(q, k_cache, v_cache, table, lens, out, lse=None, window=0, s
     """out [B, Hq, dh] (and lse [B, Hq]) <- attention of one token a sequence, q [B, Hq, dh], over the first lens[b] keys
     of caches [pages, page, Hkv, dh] by table [B, width]: with window the last `window` of them and the first `sinks`.
     scale: 1 / sqrt(dh). workspace (uint8): attention_paged_workspace(...) bytes, allocated where it is not given."""
-    import torch
     lib = _bound if _f32 else _torch()
     d = _device()
     kind = _kind(q, "q")
@@ -621,7 +634,7 @@ def attention_paged(q, k_cache, v_cache, table, lens, out, lse=None, window=0, s
     width = table.shape[1]
     need = lib.nsb_op_attention_paged_workspace_bytes(B, Hq, Hkv, dh)
     if workspace is None:
-        workspace = torch.empty(need, dtype=_u8, device=q.device)
+        workspace = _workspace(need, d)
     have = workspace.numel()
     rc = lib.nsb_op_attention_paged(
         *_heads(d, q, "q", dt, B, Hq, dh), kind, B, Hq, Hkv, dh, *_pages(d, k_cache, "k_cache", dt, pages, page, Hkv, dh),
@@ -668,7 +681,6 @@ def attention_window_bwd(q, k, v, out, lse, dout, dq, dk, dv, offsets=None, wind
                          workspace=None):
     """dq [T, Hq, dh], dk, dv [T, Hkv, dh] <- the gradients of attention_window's q, k, v for out's gradient dout, from
     its out and lse. workspace (uint8): attention_window_bwd_workspace(...) bytes, allocated where it is not given."""
-    import torch
     lib = _bound if _f32 else _torch()
     d = _device()
     dt = q.dtype
@@ -677,7 +689,7 @@ def attention_window_bwd(q, k, v, out, lse, dout, dq, dk, dv, offsets=None, wind
     args = _packed(d, q, k, v, offsets, window, sinks, scale)
     if workspace is None:
         need = lib.nsb_op_attention_window_bwd_workspace_bytes(T, Hq, Hkv, dh, F32 if dt is _f32 else BF16)
-        workspace = torch.empty(need, dtype=_u8, device=q.device)
+        workspace = _workspace(need, d)
     have = workspace.numel()
     rc = lib.nsb_op_attention_window_bwd(
         *args, *_heads(d, out, "out", dt, T, Hq, dh), *_rows(d, lse, "lse", _f32, Hq, T),
