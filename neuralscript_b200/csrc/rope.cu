@@ -38,10 +38,26 @@ struct TurnJob {
     int turn, paged;
 };
 
+// Division of numbers below 2^31 by d: m = ceil(2^p / d) with p = 31 + ceil(log2 d)
+// gives floor(x m / 2^p) = floor(x / d), since m d - 2^p < d <= 2^(p - 31).
+struct Divisor {
+    uint32_t d, m, shift;
+    Divisor(uint32_t by = 1) : d(by), m(0), shift(0) {
+        int log = 0;
+        while ((1ull << log) < by) log++;
+        if (log) {  // (by 1: m 0)
+            m = (uint32_t)(((1ull << (31 + log)) + by - 1) / by);
+            shift = log - 1;
+        }
+    }
+    __device__ __forceinline__ int of(int x) const { return m ? (int)(__umulhi((uint32_t)x, m) >> shift) : x; }
+};
+
 struct TurnArgs {
     Turn r;
     TurnJob job[3];
     int jobs, T, dh, heads, tokens;
+    Divisor by_each, by_units, by_n;  // units a token, units a head, pairs
     const int *seq, *at, *table;
     long long ld_table;
     int B, width, pages, page;
@@ -72,17 +88,36 @@ __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float
 __device__ __forceinline__ void from_f(float& d, float v) { d = v; }
 __device__ __forceinline__ void from_f(__nv_bfloat16& d, float v) { d = __float2bfloat16_rn(v); }
 
-// P values a piece; a thread's unit is two pieces of one head.
-template <typename T, int P>
+// The pieces of a unit turned: pair e is (x0[e], x1[e]), or with SIDE pairs lie
+// side by side, through both pieces.
+template <int P, bool SIDE>
+__device__ __forceinline__ void turn_pairs(float* x0, float* x1, const float2* w, int pieces) {
+#pragma unroll
+    for (int e = 0; e < P; e++) {
+        float& p0 = SIDE && P > 1 ? (2 * e < P ? x0 : x1)[2 * e % P] : x0[e];
+        float& p1 = SIDE && P > 1 ? (2 * e < P ? x0 : x1)[(2 * e + 1) % P] : x1[e];
+        const float2 c = w[e / 2 * 2 * pieces + e % 2];
+        const float f0 = p0, f1 = p1;
+        p0 = f0 * c.x - f1 * c.y;
+        p1 = f1 * c.x + f0 * c.y;
+    }
+}
+
+// P values a piece; a thread's unit is two pieces of one head. Cosine and sine
+// of two neighbouring pairs lie together, those of all pieces' first two pairs
+// before those of the next two: neighbouring threads read neighbouring 16
+// bytes (pair by pair they met each bank four times, which bound the kernel:
+// 34 us a pass over 16384 x 20 x 128 in place of 31). ONE: there is one job.
+template <typename T, int P, bool SIDE, bool ONE>
 __global__ void __launch_bounds__(kTurnThreads) turn_kernel(const __grid_constant__ TurnArgs a) {
     using V = typename Piece<P * sizeof(T)>::type;
-    extern __shared__ float2 cs[];  // [tokens][n] cosine and sine
+    extern __shared__ __align__(16) float2 cs[];  // [tokens][n] cosine and sine
     __shared__ int s_page[kTurnTokens], s_place[kTurnTokens];
     const long long t0 = (long long)blockIdx.x * a.tokens;
     const int tokens = (int)min((long long)a.tokens, a.T - t0);
     const int n = a.r.n;
 
-    if ((int)threadIdx.x < tokens && a.seq) {
+    if (!ONE && (int)threadIdx.x < tokens) {
         const long long t = t0 + threadIdx.x;
         const int b = a.seq[t];
         int page = -1, place = 0;
@@ -99,48 +134,52 @@ __global__ void __launch_bounds__(kTurnThreads) turn_kernel(const __grid_constan
         s_page[threadIdx.x] = page;
         s_place[threadIdx.x] = place;
     }
+    const int units = a.dh / (2 * P), turned = n / P, each = a.heads * units;
     for (int e = threadIdx.x; e < tokens * n; e += kTurnThreads) {
-        const int t = e / n, i = e - t * n;
+        const int t = a.by_n.of(e), i = e - t * n;
         int axis = 0;
         while (axis + 1 < a.r.axes && i >= a.r.end[axis]) axis++;
         const double turns = (double)a.r.pos[axis * a.r.ld_pos + t0 + t] * ((double)a.r.freq[i] * 0.15915494309189533577);
         float s, c;
         sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
-        cs[e] = make_float2(c * a.r.scale, s * a.r.scale * a.r.sign);
+        const int piece = i / P, in = i - piece * P;
+        cs[t * n + (P > 1 ? (in / 2 * turned + piece) * 2 + in % 2 : i)] = make_float2(c * a.r.scale, s * a.r.scale * a.r.sign);
     }
     __syncthreads();
 
-    const int units = a.dh / (2 * P), turned = n / P, each = a.heads * units;
     for (int u = threadIdx.x; u < tokens * each; u += kTurnThreads) {
-        const int t = u / each, in = u - t * each;
-        int head = in / units;
+        const int t = a.by_each.of(u), in = u - t * each;
+        int head = a.by_units.of(in);
         const int piece = in - head * units;
-        const TurnJob& j = a.job[head >= a.job[2].first ? 2 : head >= a.job[1].first ? 1 : 0];
+        const TurnJob& j = a.job[ONE ? 0 : head >= a.job[2].first ? 2 : head >= a.job[1].first ? 1 : 0];
         head -= j.first;
-        if (a.seq && s_page[t] < 0) continue;
+        if (!ONE && s_page[t] < 0) continue;
         const bool turn = j.turn && piece < turned;
         int o0 = piece * 2 * P, o1 = o0 + P;
-        if (turn && !a.r.interleaved) {
+        if (turn && !SIDE) {
             o0 = piece * P;
             o1 = o0 + n;
         }
         const T* src = (const T*)j.src + (t0 + t) * j.src_row + head * j.src_head;
         T* dst = (T*)j.dst + head * j.dst_head +
-                 (j.paged ? s_page[t] * j.dst_page + s_place[t] * j.dst_row : (t0 + t) * j.dst_row);
+                 (!ONE && j.paged ? s_page[t] * j.dst_page + s_place[t] * j.dst_row : (t0 + t) * j.dst_row);
         V v0 = *reinterpret_cast<const V*>(src + o0), v1 = *reinterpret_cast<const V*>(src + o1);
         if (turn) {
             T* x0 = reinterpret_cast<T*>(&v0);
             T* x1 = reinterpret_cast<T*>(&v1);
-            const float2* w = cs + t * n + piece * P;
+            float f0[P], f1[P];
 #pragma unroll
-            for (int e = 0; e < P; e++) {
-                // interleaved: pair e lies in piece 2 e / P (P 1: one value a piece, as in halves)
-                T& p0 = !a.r.interleaved || P == 1 ? x0[e] : (2 * e < P ? x0 : x1)[2 * e % P];
-                T& p1 = !a.r.interleaved || P == 1 ? x1[e] : (2 * e < P ? x0 : x1)[(2 * e + 1) % P];
-                const float f0 = to_f(p0), f1 = to_f(p1);
-                const float2 c = w[e];
-                from_f(p0, f0 * c.x - f1 * c.y);
-                from_f(p1, f1 * c.x + f0 * c.y);
+            for (int e = 0; e < P; e++) f0[e] = to_f(x0[e]), f1[e] = to_f(x1[e]);
+            turn_pairs<P, SIDE>(f0, f1, cs + t * n + piece * (P > 1 ? 2 : 1), turned);
+            if constexpr (P > 1 && sizeof(T) == 2) {
+#pragma unroll
+                for (int e = 0; e < P; e += 2) {
+                    reinterpret_cast<__nv_bfloat162*>(x0)[e / 2] = __floats2bfloat162_rn(f0[e], f0[e + 1]);
+                    reinterpret_cast<__nv_bfloat162*>(x1)[e / 2] = __floats2bfloat162_rn(f1[e], f1[e + 1]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < P; e++) from_f(x0[e], f0[e]), from_f(x1[e], f1[e]);
             }
         }
         *reinterpret_cast<V*>(dst + o0) = v0;
@@ -188,8 +227,12 @@ int launch(TurnArgs& a, int dtype, cudaStream_t s) {
         a.tokens = 1;
         while (a.tokens < kTurnTokens && a.tokens * each < 4 * kTurnThreads && a.T / (2 * a.tokens) >= 4 * num_sms())
             a.tokens *= 2;
-        turn_kernel<T, P><<<(unsigned)(((long long)a.T + a.tokens - 1) / a.tokens), kTurnThreads,
-                            (size_t)a.tokens * a.r.n * sizeof(float2), s>>>(a);
+        a.by_each = Divisor((uint32_t)each);
+        a.by_units = Divisor(a.dh / (2 * P));
+        a.by_n = Divisor(a.r.n ? a.r.n : 1);
+        const auto f = a.seq ? (a.r.interleaved ? turn_kernel<T, P, true, false> : turn_kernel<T, P, false, false>)
+                             : (a.r.interleaved ? turn_kernel<T, P, true, true> : turn_kernel<T, P, false, true>);
+        f<<<(unsigned)(((long long)a.T + a.tokens - 1) / a.tokens), kTurnThreads, (size_t)a.tokens * a.r.n * sizeof(float2), s>>>(a);
         return cudaGetLastError() == cudaSuccess ? 0 : -5;
     };
     using std::integral_constant;

@@ -3,6 +3,7 @@ torch CUDA tensors; device memory comes from torch (plumbing only)."""
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 from . import lib as _core_lib
 
@@ -517,11 +518,6 @@ def _kind(t, what):
     return F32 if dt is _f32 else BF16
 
 
-def _ints(d, t, what, rows, cols):
-    """Address and leading dimension of an int32 matrix whose rows are contiguous."""
-    return _rows(d, t, what, _i32, rows, cols)
-
-
 def _workspace(need, d):
     """Scratch of this call: the allocator hands it on to calls of the same stream alone, and a graph's keeps to itself."""
     return _empty(need, dtype=_u8, device=_cuda[d])
@@ -538,45 +534,50 @@ _cuda = _Devices()
 _NO_TURN = (None, 0, 0, None, None, 0, 0, 1.0)
 
 
+@functools.lru_cache(maxsize=64)
+def _sections(sections, axes, pairs):
+    """Pairs of each axis as the entries take them."""
+    if len(sections) != axes or sum(sections) != pairs or min(sections) < 0:
+        raise ValueError(f"sections {sections} where {axes} of sum {pairs} are wanted")
+    return (C.c_int * axes)(*sections)
+
+
 def _turn(d, pos, freq, T, sections, interleaved, scale):
     """The arguments of a rotation: pos [T] or [axes, T], freq [pairs], sections: pairs of each axis."""
     if pos.dim() == 1:
         pos = pos[None]
     axes = pos.shape[0]
     pairs = freq.shape[0]
-    at, ld = _ints(d, pos, "pos", axes, T)
-    if sections is None:
-        if axes != 1:
-            raise ValueError(f"pos has {axes} axes: sections say how many pairs belong to each")
-    else:
-        sections = tuple(sections)
-        if len(sections) != axes or sum(sections) != pairs or min(sections) < 0:
-            raise ValueError(f"sections {sections} where {axes} of sum {pairs} are wanted")
-        sections = (C.c_int * axes)(*sections)
+    at, ld = _rows(d, pos, "pos", _i32, axes, T)
+    if sections is not None:
+        sections = _sections(tuple(sections), axes, pairs)
+    elif axes != 1:
+        raise ValueError(f"pos has {axes} axes: sections say how many pairs belong to each")
     return at, ld, axes, sections, _dense(d, freq, "freq", _f32, (pairs,)), pairs, interleaved, scale
 
 
-def _rope(name, x, pos, freq, y, sections, interleaved, scale):
-    lib = _bound if _f32 else _torch()
+def _rope(entry, x, pos, freq, y, sections, interleaved, scale):
     d = _device()
-    kind = _kind(x, "x")
+    dt = x.dtype
     T, H, dh = x.shape
-    at, row, head = _heads(d, x, "x", x.dtype, T, H, dh)
-    rc = getattr(lib, name)(at, kind, row, head, T, H, dh, *_turn(d, pos, freq, T, sections, interleaved, scale),
-                            *_heads(d, y, "y", x.dtype, T, H, dh), _stream_of(d))
+    at, row, head = _heads(d, x, "x", dt, T, H, dh)
+    rc = entry(at, _kind(x, "x"), row, head, T, H, dh, *_turn(d, pos, freq, T, sections, interleaved, scale),
+               *_heads(d, y, "y", dt, T, H, dh), _stream_of(d))
     if rc:
-        _check(rc, name)
+        _check(rc, entry.__name__)
 
 
 def rope(x, pos, freq, y, sections=None, interleaved=False, scale=1.0):
     """y [T, H, dh] <- x with the pairs of its heads turned by pos * freq: pos [T] or [axes, T] (int32), freq [pairs]
     (float32), a pair (i, i + pairs), or (2 i, 2 i + 1) where interleaved; sections: pairs of each axis. y may be x."""
-    _rope("nsb_op_rope", x, pos, freq, y, sections, interleaved, scale)
+    lib = _bound if _f32 else _torch()
+    _rope(lib.nsb_op_rope, x, pos, freq, y, sections, interleaved, scale)
 
 
 def rope_bwd(dy, pos, freq, dx, sections=None, interleaved=False, scale=1.0):
     """dx [T, H, dh] <- the gradient of rope's x. dx may be dy."""
-    _rope("nsb_op_rope_bwd", dy, pos, freq, dx, sections, interleaved, scale)
+    lib = _bound if _f32 else _torch()
+    _rope(lib.nsb_op_rope_bwd, dy, pos, freq, dx, sections, interleaved, scale)
 
 
 def _pages(d, t, what, dtype, pages, page, heads, dh):
@@ -606,7 +607,7 @@ def kv_append(k, v, seq, at, table, k_cache, v_cache, pos=None, freq=None, secti
     Hq = 0 if q is None else q.shape[1]
     rc = lib.nsb_op_kv_append(
         *_heads(d, k, "k", dt, T, Hkv, dh), *_heads(d, v, "v", dt, T, Hkv, dh), kind, T, Hkv, dh,
-        _dense(d, seq, "seq", _i32, (T,)), _dense(d, at, "at", _i32, (T,)), *_ints(d, table, "table", B, width), B, width,
+        _dense(d, seq, "seq", _i32, (T,)), _dense(d, at, "at", _i32, (T,)), *_rows(d, table, "table", _i32, B, width), B, width,
         pages, page, *_pages(d, k_cache, "k_cache", dt, pages, page, Hkv, dh),
         *_pages(d, v_cache, "v_cache", dt, pages, page, Hkv, dh),
         *(_NO_TURN if freq is None else _turn(d, pos, freq, T, sections, interleaved, scale)),
@@ -638,7 +639,7 @@ def attention_paged(q, k_cache, v_cache, table, lens, out, lse=None, window=0, s
     have = workspace.numel()
     rc = lib.nsb_op_attention_paged(
         *_heads(d, q, "q", dt, B, Hq, dh), kind, B, Hq, Hkv, dh, *_pages(d, k_cache, "k_cache", dt, pages, page, Hkv, dh),
-        *_pages(d, v_cache, "v_cache", dt, pages, page, Hkv, dh), pages, page, *_ints(d, table, "table", B, width), width,
+        *_pages(d, v_cache, "v_cache", dt, pages, page, Hkv, dh), pages, page, *_rows(d, table, "table", _i32, B, width), width,
         _dense(d, lens, "lens", _i32, (B,)), window, sinks, dh ** -0.5 if scale is None else scale,
         *_heads(d, out, "out", dt, B, Hq, dh), None if lse is None else _dense(d, lse, "lse", _f32, (B, Hq)),
         _dense(d, workspace, "workspace", _u8, (have,)), have, _stream_of(d))
