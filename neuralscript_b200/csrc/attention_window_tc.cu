@@ -32,8 +32,7 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// Waits of one block. `lane` is one thread's; the other is a whole warp's,
-// all of whose lanes go on or none.
+// Waits of one block, a whole warp's: all of its lanes go on or none.
 struct Waits {
     volatile int* failed;  // shared memory
     int* err;
@@ -47,19 +46,6 @@ struct Waits {
                 atomicCAS(err, 0, kErrTimeoutAttn);
             }
             if (__any_sync(0xffffffffu, late || *failed)) return false;
-        }
-        return true;
-    }
-    __device__ __forceinline__ bool lane(uint64_t* bar, uint32_t phase) const {
-        if (ptx::mbar_try_wait(bar, phase & 1)) return true;
-        const long long t0 = clock64();
-        while (!ptx::mbar_try_wait(bar, phase & 1)) {
-            if (*failed) return false;
-            if (clock64() - t0 > ptx::kWaitCycles) {
-                *failed = 1;
-                atomicCAS(err, 0, kErrTimeoutAttn);
-                return false;
-            }
         }
         return true;
     }
@@ -88,8 +74,9 @@ __device__ __forceinline__ void load_rows(uint8_t* to, const CUtensorMap* map, u
     for (int c = 0; c < DHP / 64; c++) ptx::tma_load_3d(to + c * kChunk, map, bar, c * 64, head, row);
 }
 
-// Zeros in the rows of a tile from `from` on, by one warp: what stands there
-// belongs to another sequence or to none, and 0 times an infinity is no 0.
+// Zeros in the rows of a tile from `from` on, by the warp that loads: what
+// stands there belongs to another sequence or to none, and 0 times an infinity
+// is no 0. Only a sequence's last tile has such rows.
 template <int DHP>
 __device__ __forceinline__ void zero_rows(uint8_t* tile, int from) {
     const int lane = threadIdx.x & 31;
@@ -98,8 +85,39 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int from) {
         for (int at = from * 128 + lane * 16; at < kChunk; at += 512)
             *reinterpret_cast<uint4*>(tile + c * kChunk + at) = make_uint4(0, 0, 0, 0);
     ptx::fence_proxy_async();
-    __syncwarp();
 }
+
+// A tile into a slot of the ring, by the whole warp that loads; where rows from
+// `end` on are to be zeros, the copy lands on a barrier of its own first.
+template <int DHP>
+__device__ __forceinline__ bool fill_slot(uint8_t* to, const CUtensorMap* map, uint64_t* full, uint64_t* landed, uint32_t& tails,
+                                          const Waits& wait, int head, int row, int end) {
+    const bool one = (threadIdx.x & 31) == 0;
+    if (end >= kT) {
+        if (one) load_rows<DHP>(to, map, full, head, row);
+        return true;
+    }
+    if (one) load_rows<DHP>(to, map, landed, head, row);
+    if (!wait(landed, tails++)) return false;
+    zero_rows<DHP>(to, end);
+    warp_arrive(full);
+    return true;
+}
+
+// A place in a ring of slots, and the phase of its barriers: it goes on by one
+// or two without a division.
+template <int SLOTS>
+struct Turnstile {
+    int slot = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void skip(int n) {
+        slot += n;
+        if (slot >= SLOTS) {
+            slot -= SLOTS;
+            phase ^= 1;
+        }
+    }
+};
 
 // Descriptors of a tile at shared address `at`: K-major (its rows are the rows
 // or columns of the product) and MN-major (its rows are summed over).
@@ -162,12 +180,14 @@ __device__ __forceinline__ bool all_seen(const WindowDesc& d, int q0, int k0) {
 
 // ---------------------------------------------------------------------------
 // Forward. A block has 256 neighbouring queries of one head, two tiles of 128:
-//   warp 9     TMA: the queries, then keys and values tile by tile through a
+//   warp 8     TMA: the queries, then keys and values tile by tile through a
 //              ring of slots
-//   warp 8     every MMA: S_g = Q_g K^T into TMEM columns [128 g, + 128),
+//   warp 9     every MMA: S_g = Q_g K^T into TMEM columns [128 g, + 128),
 //              O_g += P_g V into [256 + 128 g, ...), P_g (bf16) read from the
 //              columns that held S_g. While one tile of queries is in its
-//              softmax, the tensor cores run the other's products.
+//              softmax, the tensor cores run the other's products. (A warp for
+//              each tile's products ran 8192 rows in 298 us in place of 240:
+//              both then take turns on the tensor cores and end late.)
 //   warps 4 g .. 4 g + 3   softmax of tile g, a query a thread: the scores come
 //              from TMEM into registers once, weights go back as bf16 pairs
 //              (half a step of 2^-9; their fp32 sum is taken before).
@@ -201,7 +221,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     uint64_t* s_bar = empty + F::SLOTS;  // [2] scores of group g in TMEM
     uint64_t* p_bar = s_bar + 2;         // [2] weights of group g in TMEM (4 arrivals)
     uint64_t* o_bar = p_bar + 2;         // [2] product of group g added to O
-    uint64_t* drain = o_bar + 2;
+    uint64_t* landed = o_bar + 2;        // a copy with rows to clear
+    uint64_t* drain = landed + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     int* failed = reinterpret_cast<int*>(tmem_slot + 1);
 
@@ -224,11 +245,12 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             ptx::mbar_init(&p_bar[g], 4);
             ptx::mbar_init(&o_bar[g], 1);
         }
+        ptx::mbar_init(landed, 1);
         ptx::mbar_init(drain, 1);
         *failed = 0;
         ptx::fence_mbar_init();
     }
-    if (warp == 8) {
+    if (warp == 9) {
         ptx::tmem_alloc(tmem_slot, 512);
         ptx::tmem_relinquish();
     }
@@ -247,27 +269,33 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         return (g == 0 || two) && kt * kT <= first && (kt >= lo || kt < sink_tiles);
     };
 
-    if (warp == 9) {
-        if ((t & 31) == 0) {
+    if (warp == 8) {
+        const bool one = (t & 31) == 0;
+        if (one) {
             ptx::mbar_arrive_expect_tx(q_full, (two ? 2 : 1) * F::TILE);
             for (int g = 0; g < (two ? 2 : 1); g++)
                 for (int c = 0; c < DHP / 64; c++)
                     ptx::tma_load_3d(smem + g * F::TILE + c * kChunk, &tq, q_full, c * 64, h, row0 + q0 + g * kT);
-            int it = 0;
-            for (int x = 0; x < tiles.count && ok; x++) {
-                const int row = row0 + tiles.at(x) * kT;
-                for (int kv = 0; kv < 2; kv++, it++) {
-                    const int slot = it % F::SLOTS, round = it / F::SLOTS;
-                    if (round && !(ok = wait.lane(&empty[slot], round - 1))) break;
-                    load_rows<DHP>(ring + slot * F::TILE, kv ? &tv : &tk, &full[slot], hk, row);
-                }
+        }
+        int it = 0;
+        uint32_t tails = 0;
+        for (int x = 0; x < tiles.count && ok; x++) {
+            const int k0 = tiles.at(x) * kT;
+            for (int kv = 0; kv < 2; kv++, it++) {
+                const int slot = it % F::SLOTS, round = it / F::SLOTS;
+                if (round && !(ok = wait(&empty[slot], round - 1))) break;
+                if (!(ok = fill_slot<DHP>(ring + slot * F::TILE, kv ? &tv : &tk, &full[slot], landed, tails, wait, hk,
+                                          row0 + k0, kv ? w.n - k0 : kT)))
+                    break;
             }
-            // no copy may land after the block has left
+        }
+        // no copy may land after the block has left
+        if (one) {
             ptx::mbar_wait(q_full, 0, nullptr, 0);
             for (int i = max(0, it - F::SLOTS); i < it; i++)
                 ptx::mbar_wait(&full[i % F::SLOTS], (i / F::SLOTS) & 1, nullptr, 0);
         }
-    } else if (warp == 8) {
+    } else if (warp == 9) {
         const uint32_t aQ = ptx::smem_u32(smem), aR = ptx::smem_u32(ring);
         uint32_t given[2] = {0, 0};  // weights taken, by group
         ok = wait(q_full, 0);
@@ -275,10 +303,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             const int ik = 2 * x, iv = 2 * x - 1;  // what the ring's slots hold: K0 V0 K1 V1 ...
             const int sk = ik % F::SLOTS, sv = iv > 0 ? iv % F::SLOTS : 0;
             const int kt = x < tiles.count ? tiles.at(x) : 0, before = x > 0 ? tiles.at(x - 1) : 0;
-            if (x > 0) {
-                if (!(ok = wait(&full[sv], iv / F::SLOTS))) break;
-                if ((before + 1) * kT > w.n) zero_rows<DHP>(ring + sv * F::TILE, w.n - before * kT);
-            }
+            if (x > 0 && !(ok = wait(&full[sv], iv / F::SLOTS))) break;
             if (x < tiles.count && !(ok = wait(&full[sk], ik / F::SLOTS))) break;
 #pragma unroll
             for (int g = 0; g < 2; g++) {
@@ -401,7 +426,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     }
     ptx::tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 9) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc(tmem, 512);
     }
@@ -411,16 +436,16 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 // Gradient of the queries. A block has 128 queries of one head and walks the
 // tiles of keys that they see:
 //   warp 17    TMA: queries and dout, then keys and values through a ring
-//   warp 16    every MMA: S = Q K^T into TMEM columns [0, 128),
-//              dP = dout V^T into [128, 256), dQ += dS K into [256, ...), dS
-//              (bf16) read from [384, 448). The next tile's S and dP run while
-//              this one's dS is computed.
+//   warp 16    the MMAs S = Q K^T into TMEM columns [0, 128) and
+//              dP = dout V^T into [128, 256), a tile ahead of
+//   warp 18    dQ += dS K into [256, ...), dS (bf16) read from [384, 448) and
+//              [448, 512) in turn
 //   warps 0..15   dS = P (dP - D), four threads a query with 32 keys each: their
 //              registers hold both scores at once, and four warps a scheduler
 //              hide each other's latencies. Before the first tile they form D = rowdot(dout, out), which the second
 //              kernel reads too.
 // ---------------------------------------------------------------------------
-constexpr int kBwdQThreads = 576;
+constexpr int kBwdQThreads = 608;
 
 template <int DHP>
 struct BwdQ {
@@ -445,9 +470,10 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
     uint64_t* s_bar = empty + F::SLOTS;  // S and dP of a tile in TMEM
     uint64_t* r_bar = s_bar + 1;         // both read (16 arrivals)
     uint64_t* p_bar = r_bar + 1;         // dS in TMEM (16 arrivals)
-    uint64_t* o_bar = p_bar + 1;         // product added to dQ
-    uint64_t* drain = o_bar + 1;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    uint64_t* o_bar = p_bar + 1;         // [2] product added to dQ, of either dS
+    uint64_t* landed = o_bar + 2;        // a copy with rows to clear
+    uint64_t* drain = landed + 1;        // [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
     int* failed = reinterpret_cast<int*>(tmem_slot + 1);
 
     const int t = threadIdx.x, warp = t >> 5;
@@ -465,8 +491,11 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
         ptx::mbar_init(s_bar, 1);
         ptx::mbar_init(r_bar, 16);
         ptx::mbar_init(p_bar, 16);
-        ptx::mbar_init(o_bar, 1);
-        ptx::mbar_init(drain, 1);
+        ptx::mbar_init(&o_bar[0], 1);
+        ptx::mbar_init(&o_bar[1], 1);
+        ptx::mbar_init(landed, 1);
+        ptx::mbar_init(&drain[0], 1);
+        ptx::mbar_init(&drain[1], 1);
         *failed = 0;
         ptx::fence_mbar_init();
     }
@@ -483,57 +512,72 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
     const KeyTiles tiles(d, q0, min(q0 + kT, w.n), kT);
 
     if (warp == 17) {
-        if ((t & 31) == 0) {
+        const bool one = (t & 31) == 0;
+        if (one) {
             ptx::mbar_arrive_expect_tx(q_full, 2 * F::TILE);
             for (int c = 0; c < DHP / 64; c++) {
                 ptx::tma_load_3d(smem + c * kChunk, &tq, q_full, c * 64, h, row0 + q0);
                 ptx::tma_load_3d(smem + F::TILE + c * kChunk, &tg, q_full, c * 64, h, row0 + q0);
             }
-            int it = 0;
-            for (int x = 0; x < tiles.count && ok; x++) {
-                const int row = row0 + tiles.at(x) * kT;
-                for (int kv = 0; kv < 2; kv++, it++) {
-                    const int slot = it % F::SLOTS, round = it / F::SLOTS;
-                    if (round && !(ok = wait.lane(&empty[slot], round - 1))) break;
-                    load_rows<DHP>(ring + slot * F::TILE, kv ? &tv : &tk, &full[slot], hk, row);
-                }
+        }
+        int it = 0;
+        uint32_t tails = 0;
+        for (int x = 0; x < tiles.count && ok; x++) {
+            const int k0 = tiles.at(x) * kT;
+            for (int kv = 0; kv < 2; kv++, it++) {
+                const int slot = it % F::SLOTS, round = it / F::SLOTS;
+                if (round && !(ok = wait(&empty[slot], round - 1))) break;
+                if (!(ok = fill_slot<DHP>(ring + slot * F::TILE, kv ? &tv : &tk, &full[slot], landed, tails, wait, hk,
+                                          row0 + k0, kv ? kT : w.n - k0)))
+                    break;
             }
+        }
+        if (one) {
             ptx::mbar_wait(q_full, 0, nullptr, 0);
             for (int i = max(0, it - F::SLOTS); i < it; i++)
                 ptx::mbar_wait(&full[i % F::SLOTS], (i / F::SLOTS) & 1, nullptr, 0);
         }
     } else if (warp == 16) {
         const uint32_t aQ = ptx::smem_u32(smem), aG = aQ + F::TILE, aR = ptx::smem_u32(ring);
+        Turnstile<F::SLOTS> ts;
         ok = wait(q_full, 0);
-        for (int x = 0; x <= tiles.count && ok; x++) {
-            if (x < tiles.count) {
-                const int sk = 2 * x % F::SLOTS, sv = (2 * x + 1) % F::SLOTS, kt = tiles.at(x);
-                if (!(ok = wait(&full[sk], 2 * x / F::SLOTS) && wait(&full[sv], (2 * x + 1) / F::SLOTS))) break;
-                if ((kt + 1) * kT > w.n) zero_rows<DHP>(ring + sk * F::TILE, w.n - kt * kT);
-                if (x > 0 && !(ok = wait(r_bar, x - 1))) break;
-                ptx::tc_fence_after();
-                if (elect()) {
-                    mma_dot<DHP>(tmem, k_major(aQ), k_major(aR + sk * F::TILE));
-                    mma_dot<DHP>(tmem + 128, k_major(aG), k_major(aR + sv * F::TILE));
-                    ptx::mma_commit(s_bar);
-                    ptx::mma_commit(&empty[sv]);
-                }
-            }
-            if (x > 0) {
-                const int sk = 2 * (x - 1) % F::SLOTS;
-                if (!(ok = wait(p_bar, x - 1))) break;
-                ptx::tc_fence_after();
-                if (elect()) {
-                    mma_add<DHP>(tmem + 256, tmem + 384, 8, mn_major(aR + sk * F::TILE), x > 1);
-                    ptx::mma_commit(o_bar);
-                    ptx::mma_commit(&empty[sk]);
-                }
+        for (int x = 0; x < tiles.count && ok; x++) {
+            const uint32_t k_at = aR + ts.slot * F::TILE;
+            if (!(ok = wait(&full[ts.slot], ts.phase))) break;
+            ts.skip(1);
+            if (!(ok = wait(&full[ts.slot], ts.phase))) break;
+            if (x > 0 && !(ok = wait(r_bar, x - 1))) break;
+            ptx::tc_fence_after();
+            if (elect()) {
+                mma_dot<DHP>(tmem, k_major(aQ), k_major(k_at));
+                mma_dot<DHP>(tmem + 128, k_major(aG), k_major(aR + ts.slot * F::TILE));
+                ptx::mma_commit(s_bar);
+                ptx::mma_commit(&empty[ts.slot]);
             }
             __syncwarp();
+            ts.skip(1);
         }
         if (elect()) {
-            ptx::mma_commit(drain);
-            ptx::mbar_wait(drain, 0, nullptr, 0);
+            ptx::mma_commit(&drain[0]);
+            ptx::mbar_wait(&drain[0], 0, nullptr, 0);
+        }
+    } else if (warp == 18) {
+        const uint32_t aR = ptx::smem_u32(ring);
+        Turnstile<F::SLOTS> ts;
+        for (int x = 0; x < tiles.count && ok; x++) {
+            if (!(ok = wait(p_bar, x))) break;
+            ptx::tc_fence_after();
+            if (elect()) {
+                mma_add<DHP>(tmem + 256, tmem + 384 + 64 * (x & 1), 8, mn_major(aR + ts.slot * F::TILE), x > 0);
+                ptx::mma_commit(&o_bar[x & 1]);
+                ptx::mma_commit(&empty[ts.slot]);
+            }
+            __syncwarp();
+            ts.skip(2);
+        }
+        if (elect()) {
+            ptx::mma_commit(&drain[1]);
+            ptx::mbar_wait(&drain[1], 0, nullptr, 0);
         }
     } else {
         const int lg = warp & 3, part = warp >> 2, r = lg * 32 + (t & 31);
@@ -602,16 +646,17 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
                 const __nv_bfloat162 p = __floats2bfloat162_rn(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]));
                 pk[e] = *reinterpret_cast<const uint32_t*>(&p);
             }
-            if (x > 0) {
-                if (!(ok = wait(o_bar, x - 1))) break;  // the product before has read its dS
+            if (x > 1) {
+                if (!(ok = wait(&o_bar[x & 1], (x >> 1) - 1))) break;  // the product before the last has read its dS
                 ptx::tc_fence_after();
             }
-            ptx::tmem_st16(base + 384 + part * 16, pk);
+            ptx::tmem_st16(base + 384 + 64 * (x & 1) + part * 16, pk);
             ptx::tmem_st_wait();
             ptx::tc_fence_before();
             warp_arrive(p_bar);
         }
-        ok = ok && wait(o_bar, tiles.count - 1);
+        const int last = tiles.count - 1;
+        ok = ok && wait(&o_bar[last & 1], last >> 1);  // (the product before it was added before)
         ptx::tc_fence_after();
         if (ok) {
             __nv_bfloat16* to = (__nv_bfloat16*)d.dq.p + (w.row0 + i) * d.dq.row + h * d.dq.head;
@@ -649,15 +694,16 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
 // columns:
 //   warp 17    TMA: keys and values, then queries and dout through a ring
 //   warp 18    lse and D of each tile of queries, into a ring of their own
-//   warp 16    every MMA: S^T = K Q^T into TMEM columns [0, 128), dP^T = V dout^T
-//              into [128, 256), dV += P^T dout into [256, ...), dK += dS^T Q into
-//              [384, ...). P^T and dS^T (bf16) take the columns of the scores
-//              that they come from.
+//   warp 16    the MMAs S^T = K Q^T into TMEM columns [0, 128) and
+//              dV += P^T dout into [256, ...),
+//   warp 19    dP^T = V dout^T into [128, 256) and dK += dS^T Q into [384, ...).
+//              P^T and dS^T (bf16) take the columns of the scores that they
+//              come from.
 //   warps 0..15   P and dS, four threads a key with 32 queries each: while P is
 //              computed the tensor cores run dK and the next dP, while dS is,
 //              dV and the next S.
 // ---------------------------------------------------------------------------
-constexpr int kBwdKvThreads = 608;
+constexpr int kBwdKvThreads = 640;
 constexpr int kStats = 4;      // tiles of lse and D held
 constexpr int kMinSteps = 4;   // least steps a block: cutting a tile costs about two
 
@@ -781,7 +827,7 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
     uint8_t* ring = smem + 2 * F::TILE;
     float* stats = reinterpret_cast<float*>(ring + F::SLOTS * F::TILE);  // [kStats][lse | D][128]
     uint64_t* k_full = reinterpret_cast<uint64_t*>(stats + kStats * 2 * kT);
-    uint64_t* k_empty = k_full + 1;        // keys and values read by the last scores of a piece
+    uint64_t* k_empty = k_full + 1;        // read by the last scores of a piece, which all other warps have begun
     uint64_t* full = k_empty + 1;
     uint64_t* empty = full + F::SLOTS;
     uint64_t* st_full = empty + F::SLOTS;
@@ -792,9 +838,11 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
     uint64_t* ds_bar = p_bar + 1;          // dS^T in TMEM (16 arrivals)
     uint64_t* sum_bar = ds_bar + 1;        // a piece's sums in TMEM
     uint64_t* out_bar = sum_bar + 1;       // and read (16 arrivals)
-    uint64_t* drain = out_bar + 1;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    uint64_t* landed = out_bar + 1;        // a copy with rows to clear
+    uint64_t* drain = landed + 1;          // [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
     int* failed = reinterpret_cast<int*>(tmem_slot + 1);
+    Piece* pieces = reinterpret_cast<Piece*>(failed + 1);  // [2], written with a piece's keys
 
     const int t = threadIdx.x, warp = t >> 5;
     const int group = d.Hq / d.Hkv;
@@ -804,10 +852,10 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
 
     if (t == 0) {
         ptx::mbar_init(k_full, 1);
-        ptx::mbar_init(k_empty, 1);
+        ptx::mbar_init(k_empty, 2 + 17);
         for (int i = 0; i < F::SLOTS; i++) {
             ptx::mbar_init(&full[i], 1);
-            ptx::mbar_init(&empty[i], 1);
+            ptx::mbar_init(&empty[i], 1 + (i & 1));  // dout, in the odd slots, has two readers
         }
         for (int i = 0; i < kStats; i++) {
             ptx::mbar_init(&st_full[i], 1);
@@ -817,9 +865,11 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
         ptx::mbar_init(g_bar, 1);
         ptx::mbar_init(p_bar, 16);
         ptx::mbar_init(ds_bar, 16);
-        ptx::mbar_init(sum_bar, 1);
+        ptx::mbar_init(sum_bar, 2);
         ptx::mbar_init(out_bar, 16);
-        ptx::mbar_init(drain, 1);
+        ptx::mbar_init(landed, 1);
+        ptx::mbar_init(&drain[0], 1);
+        ptx::mbar_init(&drain[1], 1);
         *failed = 0;
         ptx::fence_mbar_init();
     }
@@ -836,29 +886,42 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
     // step: counted over all pieces; piece: likewise
     int step = 0, piece = 0;
 
+    // the next piece, once its keys are there; its steps go through the heads, and
+    // the tiles of queries of each
+    auto next_piece = [&](Piece& p) {
+        ok = wait(k_full, piece);
+        if (ok) p = pieces[piece & 1];
+        return ok;
+    };
     if (warp == 17) {
         const bool one = (t & 31) == 0;
         int keys = 0, copies = 0;  // loads started
+        uint32_t tails = 0;
         for (long long at = begin; at < end && ok; piece++) {
             const Piece p = piece_at(d, at, end);
             at += p.x1 - p.x0;
             if (piece && !(ok = wait(k_empty, piece - 1))) break;
             keys = piece + 1;
             if (one) {
+                pieces[piece & 1] = p;
                 ptx::mbar_arrive_expect_tx(k_full, 2 * F::TILE);
                 for (int c = 0; c < DHP / 64; c++) {
                     ptx::tma_load_3d(smem + c * kChunk, &tk, k_full, c * 64, p.hk, p.row0 + p.k0);
                     ptx::tma_load_3d(smem + F::TILE + c * kChunk, &tv, k_full, c * 64, p.hk, p.row0 + p.k0);
                 }
             }
+            int h = p.hk * group + p.x0 / p.each, q = p.x0 % p.each;
             for (int x = p.x0; x < p.x1 && ok; x++, step++) {
-                const int h = p.hk * group + x / p.each, row = p.row0 + (p.first + x % p.each) * kT;
+                const int q0 = (p.first + q) * kT;
                 for (int qg = 0; qg < 2; qg++) {
                     const int i = 2 * step + qg, slot = i % F::SLOTS, round = i / F::SLOTS;
                     if (round && !(ok = wait(&empty[slot], round - 1))) break;
-                    if (one) load_rows<DHP>(ring + slot * F::TILE, qg ? &tg : &tq, &full[slot], h, row);
                     copies = i + 1;
+                    if (!(ok = fill_slot<DHP>(ring + slot * F::TILE, qg ? &tg : &tq, &full[slot], landed, tails, wait, h,
+                                              p.row0 + q0, p.n - q0)))
+                        break;
                 }
+                if (++q == p.each) q = 0, h++;
             }
         }
         // no copy may land after the block has left
@@ -868,11 +931,13 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
                 ptx::mbar_wait(&full[i % F::SLOTS], (i / F::SLOTS) & 1, nullptr, 0);
         }
     } else if (warp == 18) {
-        for (long long at = begin; at < end && ok;) {
-            const Piece p = piece_at(d, at, end);
+        Piece p;
+        for (long long at = begin; at < end && next_piece(p); piece++) {
+            warp_arrive(k_empty);
             at += p.x1 - p.x0;
-            for (int x = p.x0; x < p.x1 && ok; x++, step++) {
-                const int slot = step % kStats, h = p.hk * group + x / p.each, q0 = (p.first + x % p.each) * kT;
+            int h = p.hk * group + p.x0 / p.each, q = p.x0 % p.each;
+            for (int x = p.x0; x < p.x1; x++, step++) {
+                const int slot = step % kStats, q0 = (p.first + q) * kT;
                 float l[4], D[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
@@ -893,85 +958,114 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
                     stats[slot * 2 * kT + kT + (t & 31) + 32 * e] = D[e];
                 }
                 warp_arrive(&st_full[slot]);
+                if (++q == p.each) q = 0, h++;
             }
+            if (!ok) break;
         }
     } else if (warp == 16) {
-        const uint32_t aK = ptx::smem_u32(smem), aV = aK + F::TILE, aR = ptx::smem_u32(ring);
-        for (long long at = begin; at < end && ok; piece++) {
-            const Piece p = piece_at(d, at, end);
+        const uint32_t aK = ptx::smem_u32(smem), aR = ptx::smem_u32(ring);
+        Turnstile<F::SLOTS> ts;  // queries of the next scores; their dout is one further
+        Piece p;
+        for (long long at = begin; at < end && next_piece(p); piece++) {
             at += p.x1 - p.x0;
-            // the slot that a step's queries (0) or dout (1) are in, with zeros behind the sequence's end
-            auto ready = [&](int x, int qg) {
-                const int i = 2 * (step + x - p.x0) + qg, slot = i % F::SLOTS, q0 = (p.first + x % p.each) * kT;
-                ok = wait(&full[slot], i / F::SLOTS);
-                if (ok && q0 + kT > p.n) zero_rows<DHP>(ring + slot * F::TILE, p.n - q0);
-                return aR + slot * F::TILE;
-            };
-            uint32_t aQ = 0, aG = 0;  // of the step whose weights are awaited
-            ok = wait(k_full, piece);
-            if (ok) aQ = ready(p.x0, 0);
-            if (ok) aG = ready(p.x0, 1);
-            if (ok && elect()) {
-                ptx::tc_fence_after();
-                mma_dot<DHP>(tmem, k_major(aK), k_major(aQ));
+            if (!(ok = wait(&full[ts.slot], ts.phase))) break;
+            ptx::tc_fence_after();
+            if (elect()) {
+                mma_dot<DHP>(tmem, k_major(aK), k_major(aR + ts.slot * F::TILE));
                 ptx::mma_commit(s_bar);
-                mma_dot<DHP>(tmem + 128, k_major(aV), k_major(aG));
-                ptx::mma_commit(g_bar);
+                if (p.x1 - p.x0 == 1) ptx::mma_commit(k_empty);
             }
             __syncwarp();
-            for (int x = p.x0; x < p.x1 && ok; x++) {
-                const bool more = x + 1 < p.x1;
-                const int i = 2 * (step + x - p.x0);
-                uint32_t nQ = 0, nG = 0;
-                if (more) nQ = ready(x + 1, 0);
-                if (!ok || !(ok = wait(p_bar, i / 2))) break;
+            for (int x = p.x0; x < p.x1; x++, step++) {
+                const int more = p.x1 - 1 - x;
+                ts.skip(1);
+                const int g_slot = ts.slot;
+                if (!(ok = wait(&full[g_slot], ts.phase))) break;
+                ts.skip(1);
+                if (more && !(ok = wait(&full[ts.slot], ts.phase))) break;
                 // the piece before has been read out of the sums
                 if (x == p.x0 && piece && !(ok = wait(out_bar, piece - 1))) break;
+                if (!(ok = wait(p_bar, step))) break;
+                ptx::tc_fence_after();
                 if (elect()) {
-                    ptx::tc_fence_after();
-                    mma_add<DHP>(tmem + 256, tmem, 24, mn_major(aG), x > p.x0);
-                    ptx::mma_commit(&empty[(i + 1) % F::SLOTS]);
+                    mma_add<DHP>(tmem + 256, tmem, 24, mn_major(aR + g_slot * F::TILE), x > p.x0);
                     if (more) {
-                        mma_dot<DHP>(tmem, k_major(aK), k_major(nQ));
+                        mma_dot<DHP>(tmem, k_major(aK), k_major(aR + ts.slot * F::TILE));
                         ptx::mma_commit(s_bar);
+                        if (more == 1) ptx::mma_commit(k_empty);
+                    } else {
+                        ptx::mma_commit(sum_bar);
                     }
+                    ptx::mma_commit(&empty[g_slot]);
                 }
                 __syncwarp();
-                if (more) nG = ready(x + 1, 1);
-                if (!ok || !(ok = wait(ds_bar, i / 2))) break;
-                if (elect()) {
-                    ptx::tc_fence_after();
-                    mma_add<DHP>(tmem + 384, tmem + 128, 24, mn_major(aQ), x > p.x0);
-                    ptx::mma_commit(&empty[i % F::SLOTS]);
-                    if (more) {
-                        mma_dot<DHP>(tmem + 128, k_major(aV), k_major(nG));
-                        ptx::mma_commit(g_bar);
-                    }
-                    if (x + 2 >= p.x1 && (more || p.x1 - p.x0 == 1)) ptx::mma_commit(k_empty);
-                    if (!more) ptx::mma_commit(sum_bar);
-                }
-                __syncwarp();
-                aQ = nQ;
-                aG = nG;
             }
-            step += p.x1 - p.x0;
+            if (!ok) break;
         }
         if (elect()) {
-            ptx::mma_commit(drain);
-            ptx::mbar_wait(drain, 0, nullptr, 0);
+            ptx::mma_commit(&drain[0]);
+            ptx::mbar_wait(&drain[0], 0, nullptr, 0);
+        }
+    } else if (warp == 19) {
+        const uint32_t aV = ptx::smem_u32(smem) + F::TILE, aR = ptx::smem_u32(ring);
+        Turnstile<F::SLOTS> ts;  // queries of the step whose dS is awaited
+        Piece p;
+        for (long long at = begin; at < end && next_piece(p); piece++) {
+            at += p.x1 - p.x0;
+            Turnstile<F::SLOTS> next = ts;  // dout of the next scores
+            next.skip(1);
+            if (!(ok = wait(&full[next.slot], next.phase))) break;
+            ptx::tc_fence_after();
+            if (elect()) {
+                mma_dot<DHP>(tmem + 128, k_major(aV), k_major(aR + next.slot * F::TILE));
+                ptx::mma_commit(g_bar);
+                ptx::mma_commit(&empty[next.slot]);
+                if (p.x1 - p.x0 == 1) ptx::mma_commit(k_empty);
+            }
+            __syncwarp();
+            for (int x = p.x0; x < p.x1; x++, step++) {
+                const int more = p.x1 - 1 - x;
+                next.skip(2);
+                if (more && !(ok = wait(&full[next.slot], next.phase))) break;
+                if (x == p.x0 && piece && !(ok = wait(out_bar, piece - 1))) break;
+                if (!(ok = wait(ds_bar, step))) break;
+                ptx::tc_fence_after();
+                if (elect()) {
+                    mma_add<DHP>(tmem + 384, tmem + 128, 24, mn_major(aR + ts.slot * F::TILE), x > p.x0);
+                    if (more) {
+                        mma_dot<DHP>(tmem + 128, k_major(aV), k_major(aR + next.slot * F::TILE));
+                        ptx::mma_commit(g_bar);
+                        ptx::mma_commit(&empty[next.slot]);
+                        if (more == 1) ptx::mma_commit(k_empty);
+                    } else {
+                        ptx::mma_commit(sum_bar);
+                    }
+                    ptx::mma_commit(&empty[ts.slot]);
+                }
+                __syncwarp();
+                ts.skip(2);
+            }
+            if (!ok) break;
+        }
+        if (elect()) {
+            ptx::mma_commit(&drain[1]);
+            ptx::mbar_wait(&drain[1], 0, nullptr, 0);
         }
     } else {
         const int lg = warp & 3, part = warp >> 2;
         const uint32_t row = tmem + ((uint32_t)(lg * 32) << 16), base = row + 32 * part;
         const float sl2 = d.scale * kLog2e;
         const uint64_t SL2 = f2_pack(sl2, sl2);
-        for (long long at = begin; at < end && ok; piece++) {
-            const Piece p = piece_at(d, at, end);
+        Piece p;
+        for (long long at = begin; at < end && next_piece(p); piece++) {
+            warp_arrive(k_empty);
             const int slot_of_part = at == begin ? 0 : 1;
             at += p.x1 - p.x0;
+            int q = p.x0 % p.each;
             const int j = p.k0 + lg * 32 + (t & 31);  // key of the sequence
             for (int x = p.x0; x < p.x1; x++, step++) {
-                const int slot = step % kStats, q0 = (p.first + x % p.each) * kT;
+                const int slot = step % kStats, q0 = (p.first + q) * kT;
+                if (++q == p.each) q = 0;
                 const float4* l4 = reinterpret_cast<const float4*>(stats + slot * 2 * kT + part * 32);
                 const float4* d4 = l4 + kT / 4;
                 if (!(ok = wait(&st_full[slot], step / kStats) && wait(s_bar, step))) break;
