@@ -781,8 +781,11 @@ __device__ __forceinline__ long long all_steps(const WindowDesc& d) {
     find_seq(d, &q, &tiles, &all, [](long long, long long) { return false; });
     return all * d.Hq;
 }
+__device__ __forceinline__ long long quotient(long long a, long long b) {  // (64 bits take a hundred instructions)
+    return a < 0x7fffffff && b < 0x7fffffff ? (int)a / (int)b : a / b;
+}
 __device__ __forceinline__ long long share(long long all, int blocks) {
-    return max((long long)kMinSteps, (all + blocks - 1) / blocks);
+    return max((long long)kMinSteps, quotient(all + blocks - 1, blocks));
 }
 
 // A piece of a block's share: steps [x0, x1) of `count` of one tile of keys.
@@ -802,7 +805,7 @@ __device__ __forceinline__ Piece piece_at(const WindowDesc& d, long long at, lon
     Piece p;
     p.row0 = q.row0;
     p.n = q.n;
-    p.hk = (int)(rest / head);
+    p.hk = (int)quotient(rest, head);
     rest -= p.hk * head;
     int t = 0;  // the last tile whose steps begin at or before `rest`
     for (int step = 1 << 24; step; step >>= 1)
@@ -1164,8 +1167,9 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
     }
 }
 
-// Joins the sums of a tile of keys that several blocks share: eight columns of
-// a key a thread, of dv and dk, block after block. grid (tiles of keys, Hkv).
+// Joins the sums of a tile of keys that several blocks share, block after
+// block: eight columns of a key's dv or dk a thread. grid (tiles of keys, Hkv,
+// shares of the columns).
 template <int DHP>
 __global__ void __launch_bounds__(256) window_tc_join_kernel(const __grid_constant__ WindowDesc d, int blocks) {
     cudaGridDependencySynchronize();
@@ -1177,27 +1181,28 @@ __global__ void __launch_bounds__(256) window_tc_join_kernel(const __grid_consta
     const Steps s(d, q.n);
     const int t = (int)(blockIdx.x - tiles);
     const long long from = q.before * d.Hq + hk * s.all() * group + s.before(t) * group, to = from + s.of(t) * group;
-    const int c0 = (int)(from / per), c1 = (int)((to - 1) / per);
+    const int c0 = (int)quotient(from, per), c1 = (int)quotient(to - 1, per);
     if (c0 == c1) return;
-    const int r = threadIdx.x & (kT - 1), j = t * kT + r;
-    for (int at = threadIdx.x / kT; at < 2 * (DHP / 8); at += 2) {
-        const int which = at / (DHP / 8), c = at % (DHP / 8) * 8;
-        float sum[8] = {};
-        for (int b = c0; b <= c1; b++) {
-            const float* rest = d.parts + ((long long)b * 2 + (b == c0 && from != b * per ? 1 : 0)) * (2 * DHP * kT) +
-                                (which * DHP + c) * kT + r;
+    const int r = threadIdx.x & (kT - 1), which = threadIdx.x / kT, j = t * kT + r;
+    if (j >= q.n) return;
+    constexpr long long kPart = 2 * DHP * kT;
+    const Heads& x = which ? d.dk : d.dv;
+    const float mul = which ? d.scale : 1.f;
+    for (int c = blockIdx.z * 8; c < d.dh; c += gridDim.z * 8) {
+        const float* parts = d.parts + (which * DHP + c) * kT + r;
+        const float* first = parts + ((long long)c0 * 2 + (from != c0 * per ? 1 : 0)) * kPart;
+        float sum[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) sum[e] += rest[e * kT];
-        }
-        if (j < q.n && c < d.dh) {
-            const Heads& x = which ? d.dk : d.dv;
-            const float mul = which ? d.scale : 1.f;
-            uint4 pk;
-            __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&pk);
+        for (int e = 0; e < 8; e++) sum[e] = first[e * kT];
+#pragma unroll 4
+        for (int b = c0 + 1; b <= c1; b++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) h[e] = __floats2bfloat162_rn(sum[2 * e] * mul, sum[2 * e + 1] * mul);
-            *reinterpret_cast<uint4*>((__nv_bfloat16*)x.p + (q.row0 + j) * x.row + hk * x.head + c) = pk;
-        }
+            for (int e = 0; e < 8; e++) sum[e] += parts[b * 2 * kPart + e * kT];
+        uint4 pk;
+        __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&pk);
+#pragma unroll
+        for (int e = 0; e < 4; e++) h[e] = __floats2bfloat162_rn(sum[2 * e] * mul, sum[2 * e + 1] * mul);
+        *reinterpret_cast<uint4*>((__nv_bfloat16*)x.p + (q.row0 + j) * x.row + hk * x.head + c) = pk;
     }
 }
 
@@ -1272,7 +1277,7 @@ int bwd(const WindowDesc& d, cudaStream_t s) {
     if (cudaGetLastError() != cudaSuccess) return -5;
     // launched while the kernel before runs, and waits for it
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)tiles, d.Hkv);
+    cfg.gridDim = dim3((unsigned)tiles, d.Hkv, 4);
     cfg.blockDim = dim3(256);
     cfg.stream = s;
     cudaLaunchAttribute at;
