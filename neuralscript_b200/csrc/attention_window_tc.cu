@@ -195,7 +195,7 @@ __device__ __forceinline__ bool all_seen(const WindowDesc& d, int q0, int k0) {
 // 2^8 above the one that its weights are taken against: smaller rises cost
 // neither range (fp32) nor precision (the weights are floating point).
 // ---------------------------------------------------------------------------
-constexpr int kFwdThreads = 320;
+constexpr int kFwdThreads = 384;  // (two of its warps idle: registers are split by groups of four)
 constexpr float kRise = 8.f;
 
 template <int DHP>
@@ -269,6 +269,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         return (g == 0 || two) && kt * kT <= first && (kt >= lo || kt < sink_tiles);
     };
 
+    // (all four warps of a group at one instruction; together what the block was
+    // launched with)
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 8) {
         const bool one = (t & 31) == 0;
         if (one) {
@@ -332,7 +336,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             ptx::mma_commit(drain);
             ptx::mbar_wait(drain, 0, nullptr, 0);
         }
-    } else if (warp < 4 || two) {
+    }
+    } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if (warp < 4 || two) {
         const int g = warp >> 2, lg = warp & 3;
         const int i = q0 + g * kT + lg * 32 + (t & 31);  // query of the sequence
         const uint32_t base = tmem + ((uint32_t)(lg * 32) << 16) + 128 * g;
@@ -423,6 +430,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             }
             if (i < w.n && d.lse) d.lse[h * d.ld_lse + w.row0 + i] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * kLn2;
         }
+    }
     }
     ptx::tc_fence_before();
     __syncthreads();
