@@ -134,14 +134,15 @@ __device__ __forceinline__ void mma_dot(uint32_t d, uint64_t a, uint64_t b) {
         ptx::mma_bf16(d, a + at, b + at, idesc, s > 0);
     }
 }
-// D (+)= A B, A [128, 128] in TMEM (16 of its columns in 8, `apart` from
-// sixteen to sixteen where two lie side by side), B an MN-major tile.
-template <int DHP>
-__device__ __forceinline__ void mma_add(uint32_t d, uint32_t a, int apart, uint64_t b, bool more) {
+// D (+)= A B, A [128, 128] in TMEM, B an MN-major tile. A's columns, two bf16 in
+// one of TMEM's, stand in runs of RUN columns that begin 2 RUN of TMEM's apart
+// (RUN 128: side by side).
+template <int DHP, int RUN>
+__device__ __forceinline__ void mma_add(uint32_t d, uint32_t a, uint64_t b, bool more) {
     constexpr uint32_t idesc = ptx::instr_desc(1, 0, 1, kT, DHP);
 #pragma unroll
     for (int s = 0; s < kT / 16; s++)
-        ptx::mma_bf16_ts(d, a + (s >> 1) * (8 + apart) + (s & 1) * 8, b + s * (2048 >> 4), idesc, more || s > 0);
+        ptx::mma_bf16_ts(d, a + 16 * s / RUN * RUN + 16 * s % RUN / 2, b + s * (2048 >> 4), idesc, more || s > 0);
 }
 
 // N columns of an output row, `cols` of which there are.
@@ -195,14 +196,15 @@ __device__ __forceinline__ bool all_seen(const WindowDesc& d, int q0, int k0) {
 // 2^8 above the one that its weights are taken against: smaller rises cost
 // neither range (fp32) nor precision (the weights are floating point).
 // ---------------------------------------------------------------------------
-constexpr int kFwdThreads = 384;  // (two of its warps idle: registers are split by groups of four)
+constexpr int kFwdThreads = 640;  // (two of its warps idle: registers are split by groups of four)
 constexpr float kRise = 8.f;
 
 template <int DHP>
 struct Fwd {
     static constexpr int TILE = DHP / 64 * kChunk;
     static constexpr int SLOTS = DHP == 128 ? 5 : 8;
-    static constexpr int SMEM = (2 + SLOTS) * TILE + 512 + 1024;
+    static constexpr int SMEM = (2 + SLOTS) * TILE + 4 * kT * 4 + 512;  // (no room to move its start)
+    static_assert(SMEM <= 227 * 1024, "above what a block may have");
 };
 
 }  // namespace
@@ -212,14 +214,18 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     window_tc_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                          const __grid_constant__ CUtensorMap tv, const __grid_constant__ WindowDesc d) {
     using F = Fwd<DHP>;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if (ptx::smem_u32(smem) & 1023) {  // tiles begin on multiples of 1024
+        if (threadIdx.x == 0) atomicCAS(d.err, 0, kErrBadShape);
+        return;
+    }
     uint8_t* ring = smem + 2 * F::TILE;
-    uint64_t* q_full = reinterpret_cast<uint64_t*>(ring + F::SLOTS * F::TILE);
+    float* tops = reinterpret_cast<float*>(ring + F::SLOTS * F::TILE);  // [2][2][128] of a group's halves
+    uint64_t* q_full = reinterpret_cast<uint64_t*>(tops + 4 * kT);
     uint64_t* full = q_full + 1;
     uint64_t* empty = full + F::SLOTS;
     uint64_t* s_bar = empty + F::SLOTS;  // [2] scores of group g in TMEM
-    uint64_t* p_bar = s_bar + 2;         // [2] weights of group g in TMEM (4 arrivals)
+    uint64_t* p_bar = s_bar + 2;         // [2] weights of group g in TMEM (8 arrivals)
     uint64_t* o_bar = p_bar + 2;         // [2] product of group g added to O
     uint64_t* landed = o_bar + 2;        // a copy with rows to clear
     uint64_t* drain = landed + 1;
@@ -242,7 +248,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         }
         for (int g = 0; g < 2; g++) {
             ptx::mbar_init(&s_bar[g], 1);
-            ptx::mbar_init(&p_bar[g], 4);
+            ptx::mbar_init(&p_bar[g], 8);
             ptx::mbar_init(&o_bar[g], 1);
         }
         ptx::mbar_init(landed, 1);
@@ -250,7 +256,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         *failed = 0;
         ptx::fence_mbar_init();
     }
-    if (warp == 9) {
+    if (warp == 17) {
         ptx::tmem_alloc(tmem_slot, 512);
         ptx::tmem_relinquish();
     }
@@ -271,9 +277,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 
     // (all four warps of a group at one instruction; together what the block was
     // launched with)
-    if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == 8) {
+    if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == 16) {
         const bool one = (t & 31) == 0;
         if (one) {
             ptx::mbar_arrive_expect_tx(q_full, (two ? 2 : 1) * F::TILE);
@@ -299,7 +305,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             for (int i = max(0, it - F::SLOTS); i < it; i++)
                 ptx::mbar_wait(&full[i % F::SLOTS], (i / F::SLOTS) & 1, nullptr, 0);
         }
-    } else if (warp == 9) {
+    } else if (warp == 17) {
         const uint32_t aQ = ptx::smem_u32(smem), aR = ptx::smem_u32(ring);
         uint32_t given[2] = {0, 0};  // weights taken, by group
         ok = wait(q_full, 0);
@@ -315,7 +321,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                     if (!(ok = wait(&p_bar[g], given[g]))) break;
                     ptx::tc_fence_after();
                     if (elect()) {
-                        mma_add<DHP>(tmem + 256 + 128 * g, tmem + 128 * g, 8, mn_major(aR + sv * F::TILE), given[g] > 0);
+                        mma_add<DHP, 64>(tmem + 256 + 128 * g, tmem + 128 * g, mn_major(aR + sv * F::TILE), given[g] > 0);
                         ptx::mma_commit(&o_bar[g]);
                     }
                     given[g]++;
@@ -338,29 +344,37 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         }
     }
     } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    if (warp < 4 || two) {
-        const int g = warp >> 2, lg = warp & 3;
-        const int i = q0 + g * kT + lg * 32 + (t & 31);  // query of the sequence
-        const uint32_t base = tmem + ((uint32_t)(lg * 32) << 16) + 128 * g;
-        const uint32_t o_at = tmem + ((uint32_t)(lg * 32) << 16) + 256 + 128 * g;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    if (warp < 8 || two) {
+        const int g = warp >> 3, half = warp >> 2 & 1, lg = warp & 3, r = lg * 32 + (t & 31);
+        const int i = q0 + g * kT + r;  // query of the sequence
+        const uint32_t lanes = tmem + ((uint32_t)(lg * 32) << 16);
+        const uint32_t base = lanes + 128 * g + 64 * half, o_at = lanes + 256 + 128 * g + half * (DHP / 2);
         const float sl2 = d.scale * kLog2e;
-        float ref = -INFINITY, sum = 0.f;  // what the weights are taken against (powers of two), their sum
+        float ref = -INFINITY, sum = 0.f;  // what the weights are taken against (powers of two), this half's sum
         uint32_t done = 0;                 // tiles behind
+        // What the thread of this row's other half has. (It has read what was here
+        // before: the scores that this thread waited for came after its weights.)
+        auto swap = [&](float mine) {
+            float* at = tops + g * 2 * kT;
+            at[half * kT + r] = mine;
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + lg) : "memory");
+            return at[(half ^ 1) * kT + r];
+        };
         for (int x = 0; x < tiles.count; x++) {
             const int kt = tiles.at(x), k0 = kt * kT;
             if (!uses(g, kt)) continue;
             if (!(ok = wait(&s_bar[g], done))) break;
             ptx::tc_fence_after();
-            uint32_t a[128];
-#pragma unroll
-            for (int c = 0; c < 4; c++) ptx::tmem_ld32(base + 32 * c, a + 32 * c);
-#pragma unroll
-            for (int c = 0; c < 4; c++) ptx::tmem_ld_wait_regs32(a + 32 * c);
+            uint32_t a[64];
+            ptx::tmem_ld32(base, a);
+            ptx::tmem_ld32(base + 32, a + 32);
+            ptx::tmem_ld_wait_regs32(a);
+            ptx::tmem_ld_wait_regs32(a + 32);
             if (!all_seen(d, q0 + g * kT, k0)) {
 #pragma unroll
-                for (int c = 0; c < 128; c += 32) {
-                    const uint32_t on = keys_seen(d, i, k0 + c);
+                for (int c = 0; c < 64; c += 32) {
+                    const uint32_t on = keys_seen(d, i, k0 + 64 * half + c);
 #pragma unroll
                     for (int e = 0; e < 32; e++)
                         if (!(on >> e & 1)) a[c + e] = 0xff800000u;
@@ -368,10 +382,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             }
             float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < 128; c += 2)
+            for (int c = 0; c < 64; c += 2)
                 m4[(c >> 1) & 3] = max3(m4[(c >> 1) & 3], __uint_as_float(a[c]), __uint_as_float(a[c + 1]));
-            const float top = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]) * sl2;  // (the scale is positive)
-            const bool rise = top > ref + kRise;  // ref -inf: the first finite score
+            float top = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]);
+            top = fmaxf(top, swap(top)) * sl2;  // (the scale is positive)
+            const bool rise = top > ref + kRise;          // ref -inf: the first finite score
             if (__any_sync(0xffffffffu, rise)) {
                 const float turn = rise ? ex2(ref - top) : 1.f;
                 if (rise) ref = top;
@@ -380,7 +395,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                     if (!(ok = wait(&o_bar[g], done - 1))) break;
                     ptx::tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < DHP; c += 16) {
+                    for (int c = 0; c < DHP / 2; c += 16) {
                         uint32_t o[16];
                         ptx::tmem_ld16(o_at + c, o);
                         ptx::tmem_ld_wait_regs16(o);
@@ -392,9 +407,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             }
             const float safe = ref == -INFINITY ? 0.f : ref;
             const uint64_t SL2 = f2_pack(sl2, sl2), NEG = f2_pack(-safe, -safe);
-            uint64_t s4[4] = {0, 0, 0, 0};
+            uint64_t s4[2] = {0, 0};
 #pragma unroll
-            for (int c = 0; c < 128; c += 32) {
+            for (int c = 0; c < 64; c += 32) {
                 uint32_t pk[16];
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
@@ -402,14 +417,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                     f2_unpack(f2_fma(f2_pack(__uint_as_float(a[c + 2 * e]), __uint_as_float(a[c + 2 * e + 1])), SL2, NEG), x0, x1);
                     x0 = ex2(x0);
                     x1 = ex2(x1);
-                    s4[e & 3] = f2_add(s4[e & 3], f2_pack(x0, x1));
+                    s4[e & 1] = f2_add(s4[e & 1], f2_pack(x0, x1));
                     const __nv_bfloat162 p = __floats2bfloat162_rn(x0, x1);
                     pk[e] = *reinterpret_cast<const uint32_t*>(&p);
                 }
                 ptx::tmem_st16(base + c / 2, pk);
             }
             float s0, s1;
-            f2_unpack(f2_add(f2_add(s4[0], s4[1]), f2_add(s4[2], s4[3])), s0, s1);
+            f2_unpack(f2_add(s4[0], s4[1]), s0, s1);
             sum += s0 + s1;
             ptx::tmem_st_wait();
             ptx::tc_fence_before();
@@ -419,22 +434,24 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         ok = ok && wait(&o_bar[g], done - 1);  // a query's own tile is always among its tiles
         ptx::tc_fence_after();
         if (ok) {
+            sum += swap(sum);
             const float mul = sum == 0.f ? 0.f : 1.f / sum;
             __nv_bfloat16* to = (__nv_bfloat16*)d.out.p + (w.row0 + i) * d.out.row + h * d.out.head;
 #pragma unroll 1
-            for (int c = 0; c < DHP; c += 32) {
+            for (int c = 0; c < DHP / 2; c += 32) {
                 uint32_t v[32];
                 ptx::tmem_ld32(o_at + c, v);
                 ptx::tmem_ld_wait_regs32(v);
-                if (i < w.n) store_cols<32>(to + c, v, mul, d.dh - c);
+                if (i < w.n) store_cols<32>(to + half * (DHP / 2) + c, v, mul, d.dh - half * (DHP / 2) - c);
             }
-            if (i < w.n && d.lse) d.lse[h * d.ld_lse + w.row0 + i] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * kLn2;
+            if (half == 0 && i < w.n && d.lse)
+                d.lse[h * d.ld_lse + w.row0 + i] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * kLn2;
         }
     }
     }
     ptx::tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == 17) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc(tmem, 512);
     }
@@ -576,7 +593,7 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
             if (!(ok = wait(p_bar, x))) break;
             ptx::tc_fence_after();
             if (elect()) {
-                mma_add<DHP>(tmem + 256, tmem + 384 + 64 * (x & 1), 8, mn_major(aR + ts.slot * F::TILE), x > 0);
+                mma_add<DHP, 128>(tmem + 256, tmem + 384 + 64 * (x & 1), mn_major(aR + ts.slot * F::TILE), x > 0);
                 ptx::mma_commit(&o_bar[x & 1]);
                 ptx::mma_commit(&empty[ts.slot]);
             }
@@ -999,7 +1016,7 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
                 if (!(ok = wait(p_bar, step))) break;
                 ptx::tc_fence_after();
                 if (elect()) {
-                    mma_add<DHP>(tmem + 256, tmem, 24, mn_major(aR + g_slot * F::TILE), x > p.x0);
+                    mma_add<DHP, 32>(tmem + 256, tmem, mn_major(aR + g_slot * F::TILE), x > p.x0);
                     if (more) {
                         mma_dot<DHP>(tmem, k_major(aK), k_major(aR + ts.slot * F::TILE));
                         ptx::mma_commit(s_bar);
@@ -1042,7 +1059,7 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
                 if (!(ok = wait(ds_bar, step))) break;
                 ptx::tc_fence_after();
                 if (elect()) {
-                    mma_add<DHP>(tmem + 384, tmem + 128, 24, mn_major(aR + ts.slot * F::TILE), x > p.x0);
+                    mma_add<DHP, 32>(tmem + 384, tmem + 128, mn_major(aR + ts.slot * F::TILE), x > p.x0);
                     if (more) {
                         mma_dot<DHP>(tmem + 128, k_major(aV), k_major(aR + next.slot * F::TILE));
                         ptx::mma_commit(g_bar);
