@@ -22,6 +22,7 @@
 #include "attention_cache.h"
 #include "attention_window.cuh"
 #include "gemm.h"
+#include "ptx.cuh"
 #include "shared_memory.h"
 
 namespace nsb {
@@ -42,14 +43,36 @@ constexpr int ld_of() {
     return DHP + 4;
 }
 
-// Rows [first, first + kB) of a head, zeros behind `end` and behind dh.
+// Rows [first, first + kB) of a head, zeros behind `end` and behind dh. fp32
+// rows on 16-byte boundaries are copied without passing through registers
+// (`land` waits for them), so that a tile's copies run beside the arithmetic of
+// the one before: 2 buffers, as far as shared memory reaches.
 template <typename T, int DHP>
 __device__ __forceinline__ void load_tile(float* s, const Heads& x, long long row0, int first, int end, int head, int dh) {
     const T* p = (const T*)x.p + head * x.head;
+    if constexpr (std::is_same<T, float>::value) {
+        if (((reinterpret_cast<uintptr_t>(x.p) >> 2 | x.row | x.head | dh) & 3) == 0) {
+            for (int e = threadIdx.x; e < kB * (DHP / 4); e += kThreads) {
+                const int r = e / (DHP / 4), c = e % (DHP / 4) * 4;
+                const bool on = first + r < end && c < dh;
+                ptx::cp_async16(s + r * ld_of<DHP>() + c, on ? p + (row0 + first + r) * x.row + c : (const float*)x.p, on ? 16 : 0);
+            }
+            return;
+        }
+    }
     for (int e = threadIdx.x; e < kB * DHP; e += kThreads) {
         const int r = e / DHP, c = e % DHP;
         s[r * ld_of<DHP>() + c] = first + r < end && c < dh ? ldf(p + (row0 + first + r) * x.row + c) : 0.f;
     }
+}
+
+__device__ __forceinline__ void land() {
+    ptx::cp_async_wait_all();
+    __syncthreads();
+}
+template <int DHP>
+constexpr int buffers(int heads, int scores) {  // of `heads` tiles, two of them twice where they fit
+    return ((heads + 2) * kB * ld_of<DHP>() + scores * kB * kLdS) * (int)sizeof(float) <= 227 * 1024 ? 2 : 1;
 }
 
 // acc[i][j] = sum over the head's columns of a[ty 4 + i] . b[tx + 16 j]
@@ -159,7 +182,8 @@ __device__ __forceinline__ float row_max(float v) {
 template <typename T, int DHP>
 __global__ void __launch_bounds__(kThreads) window_fwd_kernel(const __grid_constant__ WindowDesc d) {
     extern __shared__ float sm[];
-    float *sQ = sm, *sK = sQ + kB * ld_of<DHP>(), *sV = sK + kB * ld_of<DHP>(), *sP = sV + kB * ld_of<DHP>();
+    constexpr int TILE = kB * ld_of<DHP>(), BUFS = buffers<DHP>(3, 1);
+    float *sQ = sm, *sP = sQ + TILE, *ring = sP + kB * kLdS;  // keys and values of each buffer
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const Rows w = find_rows(d, gridDim.x - 1 - blockIdx.x, kB);
     if (w.n <= 0) return;
@@ -169,12 +193,21 @@ __global__ void __launch_bounds__(kThreads) window_fwd_kernel(const __grid_const
 #pragma unroll
     for (int i = 0; i < 4; i++) m[i] = -INFINITY, l[i] = 0.f;
     const KeyTiles kt(d, q0, min(q0 + kB, w.n), kB);
+    auto fetch = [&](int x) {
+        float* to = ring + x % BUFS * 2 * TILE;
+        load_tile<T, DHP>(to, d.k, w.row0, kt.at(x) * kB, w.n, hk, d.dh);
+        load_tile<T, DHP>(to + TILE, d.v, w.row0, kt.at(x) * kB, w.n, hk, d.dh);
+    };
+    if (BUFS == 2) fetch(0);
     for (int x = 0; x < kt.count; x++) {
         const int k0 = kt.at(x) * kB;
-        __syncthreads();
-        load_tile<T, DHP>(sK, d.k, w.row0, k0, w.n, hk, d.dh);
-        load_tile<T, DHP>(sV, d.v, w.row0, k0, w.n, hk, d.dh);
-        __syncthreads();
+        const float *sK = ring + x % BUFS * 2 * TILE, *sV = sK + TILE;
+        if (BUFS == 1) {
+            __syncthreads();
+            fetch(x);
+        }
+        land();
+        if (BUFS == 2 && x + 1 < kt.count) fetch(x + 1);
         float s[4][4];
         dot_tile<DHP>(s, sQ, sK, ty, tx);
 #pragma unroll
@@ -216,16 +249,16 @@ __global__ void __launch_bounds__(kThreads) window_fwd_kernel(const __grid_const
 template <typename T, int DHP>
 __global__ void __launch_bounds__(kThreads) window_bwd_q_kernel(const __grid_constant__ WindowDesc d) {
     extern __shared__ float sm[];
-    float *sQ = sm, *sG = sQ + kB * ld_of<DHP>(), *sK = sG + kB * ld_of<DHP>(), *sV = sK + kB * ld_of<DHP>(),
-          *sS = sV + kB * ld_of<DHP>();
+    constexpr int TILE = kB * ld_of<DHP>(), BUFS = buffers<DHP>(4, 1);
+    float *sQ = sm, *sG = sQ + TILE, *sS = sG + TILE, *ring = sS + kB * kLdS;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const Rows w = find_rows(d, gridDim.x - 1 - blockIdx.x, kB);
     if (w.n <= 0) return;
     const int h = blockIdx.y, hk = h / (d.Hq / d.Hkv), q0 = w.first;
     load_tile<T, DHP>(sQ, d.q, w.row0, q0, w.n, h, d.dh);
     load_tile<T, DHP>(sG, d.dout, w.row0, q0, w.n, h, d.dh);
-    load_tile<T, DHP>(sK, d.out, w.row0, q0, w.n, h, d.dh);
-    __syncthreads();
+    load_tile<T, DHP>(ring, d.out, w.row0, q0, w.n, h, d.dh);
+    land();
     float o[4][DHP / 16] = {}, lse[4], D[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -233,18 +266,30 @@ __global__ void __launch_bounds__(kThreads) window_bwd_q_kernel(const __grid_con
         float sum = 0.f;
 #pragma unroll
         for (int c = 0; c < DHP; c += 16)
-            sum = fmaf(sG[(ty * 4 + i) * ld_of<DHP>() + c + tx], sK[(ty * 4 + i) * ld_of<DHP>() + c + tx], sum);
+            sum = fmaf(sG[(ty * 4 + i) * ld_of<DHP>() + c + tx], ring[(ty * 4 + i) * ld_of<DHP>() + c + tx], sum);
         D[i] = row_sum(sum);
         lse[i] = r < w.n ? d.lse[h * d.ld_lse + w.row0 + r] : -INFINITY;
         if (tx == 0 && r < w.n) d.dvec[(long long)h * d.T + w.row0 + r] = D[i];
     }
     const KeyTiles kt(d, q0, min(q0 + kB, w.n), kB);
+    auto fetch = [&](int x) {
+        float* to = ring + x % BUFS * 2 * TILE;
+        load_tile<T, DHP>(to, d.k, w.row0, kt.at(x) * kB, w.n, hk, d.dh);
+        load_tile<T, DHP>(to + TILE, d.v, w.row0, kt.at(x) * kB, w.n, hk, d.dh);
+    };
+    if (BUFS == 2) {
+        __syncthreads();  // the outputs have been read
+        fetch(0);
+    }
     for (int x = 0; x < kt.count; x++) {
         const int k0 = kt.at(x) * kB;
-        __syncthreads();
-        load_tile<T, DHP>(sK, d.k, w.row0, k0, w.n, hk, d.dh);
-        load_tile<T, DHP>(sV, d.v, w.row0, k0, w.n, hk, d.dh);
-        __syncthreads();
+        const float *sK = ring + x % BUFS * 2 * TILE, *sV = sK + TILE;
+        if (BUFS == 1) {
+            __syncthreads();
+            fetch(x);
+        }
+        land();
+        if (BUFS == 2 && x + 1 < kt.count) fetch(x + 1);
         float s[4][4], g[4][4];
         dot_tile<DHP>(s, sQ, sK, ty, tx);
         dot_tile<DHP>(g, sG, sV, ty, tx);
@@ -266,8 +311,8 @@ __global__ void __launch_bounds__(kThreads) window_bwd_q_kernel(const __grid_con
 template <typename T, int DHP>
 __global__ void __launch_bounds__(kThreads) window_bwd_kv_kernel(const __grid_constant__ WindowDesc d) {
     extern __shared__ float sm[];
-    float *sK = sm, *sV = sK + kB * ld_of<DHP>(), *sQ = sV + kB * ld_of<DHP>(), *sG = sQ + kB * ld_of<DHP>(),
-          *sP = sG + kB * ld_of<DHP>(), *sS = sP + kB * kLdS;
+    constexpr int TILE = kB * ld_of<DHP>(), BUFS = buffers<DHP>(4, 2);
+    float *sK = sm, *sV = sK + TILE, *sP = sV + TILE, *sS = sP + kB * kLdS, *ring = sS + kB * kLdS;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const Rows w = find_rows(d, blockIdx.x, kB);
     if (w.n <= 0) return;
@@ -275,34 +320,43 @@ __global__ void __launch_bounds__(kThreads) window_bwd_kv_kernel(const __grid_co
     load_tile<T, DHP>(sK, d.k, w.row0, k0, w.n, hk, d.dh);
     load_tile<T, DHP>(sV, d.v, w.row0, k0, w.n, hk, d.dh);
     float dk[4][DHP / 16] = {}, dv[4][DHP / 16] = {};
-    const int last = query_tiles_end(d, k0, w.n, kB);
-    for (int h = hk * group; h < (hk + 1) * group; h++)
-        for (int x = k0 / kB; x < last; x++) {
-            const int q0 = x * kB;
+    const int first = k0 / kB, each = query_tiles_end(d, k0, w.n, kB) - first, count = each * group;
+    auto fetch = [&](int x) {
+        float* to = ring + x % BUFS * 2 * TILE;
+        const int h = hk * group + x / each, q0 = (first + x % each) * kB;
+        load_tile<T, DHP>(to, d.q, w.row0, q0, w.n, h, d.dh);
+        load_tile<T, DHP>(to + TILE, d.dout, w.row0, q0, w.n, h, d.dh);
+    };
+    if (BUFS == 2) fetch(0);
+    for (int x = 0; x < count; x++) {
+        const int h = hk * group + x / each, q0 = (first + x % each) * kB;
+        const float *sQ = ring + x % BUFS * 2 * TILE, *sG = sQ + TILE;
+        if (BUFS == 1) {
             __syncthreads();
-            load_tile<T, DHP>(sQ, d.q, w.row0, q0, w.n, h, d.dh);
-            load_tile<T, DHP>(sG, d.dout, w.row0, q0, w.n, h, d.dh);
-            __syncthreads();
-            float s[4][4], g[4][4];
-            dot_tile<DHP>(s, sQ, sK, ty, tx);
-            dot_tile<DHP>(g, sG, sV, ty, tx);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int r = q0 + ty * 4 + i;
-                const float lse = r < w.n ? d.lse[h * d.ld_lse + w.row0 + r] : -INFINITY;
-                const float D = r < w.n ? d.dvec[(long long)h * d.T + w.row0 + r] : 0.f;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const bool on = lse != -INFINITY && sees(d, r, k0 + tx + 16 * j);
-                    const float p = on ? expf(s[i][j] * d.scale - lse) : 0.f;
-                    sP[(ty * 4 + i) * kLdS + tx + 16 * j] = p;
-                    sS[(ty * 4 + i) * kLdS + tx + 16 * j] = on ? p * (g[i][j] - D) : 0.f;
-                }
-            }
-            __syncthreads();
-            add_cols<DHP>(dv, sP, sG, ty, tx);
-            add_cols<DHP>(dk, sS, sQ, ty, tx);
+            fetch(x);
         }
+        land();
+        if (BUFS == 2 && x + 1 < count) fetch(x + 1);
+        float s[4][4], g[4][4];
+        dot_tile<DHP>(s, sQ, sK, ty, tx);
+        dot_tile<DHP>(g, sG, sV, ty, tx);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = q0 + ty * 4 + i;
+            const float lse = r < w.n ? d.lse[h * d.ld_lse + w.row0 + r] : -INFINITY;
+            const float D = r < w.n ? d.dvec[(long long)h * d.T + w.row0 + r] : 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const bool on = lse != -INFINITY && sees(d, r, k0 + tx + 16 * j);
+                const float p = on ? expf(s[i][j] * d.scale - lse) : 0.f;
+                sP[(ty * 4 + i) * kLdS + tx + 16 * j] = p;
+                sS[(ty * 4 + i) * kLdS + tx + 16 * j] = on ? p * (g[i][j] - D) : 0.f;
+            }
+        }
+        __syncthreads();
+        add_cols<DHP>(dv, sP, sG, ty, tx);
+        add_cols<DHP>(dk, sS, sQ, ty, tx);
+    }
     const float one[4] = {1.f, 1.f, 1.f, 1.f}, mul[4] = {d.scale, d.scale, d.scale, d.scale};
     store_tile<T, DHP>(dv, one, d.dv, w.row0, k0, w.n, hk, d.dh, ty, tx);
     store_tile<T, DHP>(dk, mul, d.dk, w.row0, k0, w.n, hk, d.dh, ty, tx);
@@ -312,7 +366,7 @@ namespace {
 
 template <int DHP>
 constexpr int smem_of(int heads, int scores) {
-    return (heads * kB * ld_of<DHP>() + scores * kB * kLdS) * (int)sizeof(float);
+    return ((heads + (buffers<DHP>(heads, scores) - 1) * 2) * kB * ld_of<DHP>() + scores * kB * kLdS) * (int)sizeof(float);
 }
 
 int check(const WindowDesc& d) {
