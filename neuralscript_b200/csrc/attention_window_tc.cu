@@ -66,6 +66,20 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
     if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(bar);
 }
 
+// A barrier of N threads, by whole warps: whether one of them gave up. Who leaves
+// its loop meets it once more with `gone`, and who gets true leaves without: so
+// nobody stands at a barrier that another will not reach.
+template <int N>
+__device__ __forceinline__ bool meet(int id, bool gone) {
+    int any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %3, 0;\n\tbarrier.cta.red.or.pred q, %1, %2, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+        : "=r"(any)
+        : "r"(id), "n"(N), "r"((int)gone)
+        : "memory");
+    return any;
+}
+
 // 128 rows of a head from row `row` on, 64 columns a chunk.
 template <int DHP>
 __device__ __forceinline__ void load_rows(uint8_t* to, const CUtensorMap* map, uint64_t* bar, int head, int row) {
@@ -181,20 +195,31 @@ __device__ __forceinline__ bool all_seen(const WindowDesc& d, int q0, int k0) {
 
 // ---------------------------------------------------------------------------
 // Forward. A block has 256 neighbouring queries of one head, two tiles of 128:
-//   warp 8     TMA: the queries, then keys and values tile by tile through a
+//   warp 16    TMA: the queries, then keys and values tile by tile through a
 //              ring of slots
-//   warp 9     every MMA: S_g = Q_g K^T into TMEM columns [128 g, + 128),
+//   warp 17    every MMA: S_g = Q_g K^T into TMEM columns [128 g, + 128),
 //              O_g += P_g V into [256 + 128 g, ...), P_g (bf16) read from the
 //              columns that held S_g. While one tile of queries is in its
 //              softmax, the tensor cores run the other's products. (A warp for
 //              each tile's products ran 8192 rows in 298 us in place of 240:
 //              both then take turns on the tensor cores and end late.)
-//   warps 4 g .. 4 g + 3   softmax of tile g, a query a thread: the scores come
-//              from TMEM into registers once, weights go back as bf16 pairs
-//              (half a step of 2^-9; their fp32 sum is taken before).
+//   warps 8 g .. 8 g + 7   softmax of tile g, two threads a query with 64 keys
+//              each, which exchange their maxima through shared memory (8192
+//              rows: 246 us, a thread a query 279): the scores come from TMEM
+//              into registers once, weights go back as bf16 pairs (off by 2^-9
+//              of themselves at most; their fp32 sum is taken before).
 // O stays in TMEM. It is scaled only when a row's maximum rises by more than
 // 2^8 above the one that its weights are taken against: smaller rises cost
 // neither range (fp32) nor precision (the weights are floating point).
+//
+// Registers go from the warps that issue to those of the softmax, 64 and 104 a
+// thread of 96 at launch (246 to 243 us).
+//
+// Bound by the turn from a product to its softmax and back: tensor cores and
+// exponentials are each busy for 54 % of the time, and a tile's parts follow each
+// other, overlapped by the other tile's alone. 8192 rows of 16 heads of 128
+// columns, causal: 244 us, 1.13 PFLOP/s (0.68 of a measured library product);
+// 20000 rows of 4 heads of 64, window 4000: 134 us.
 // ---------------------------------------------------------------------------
 constexpr int kFwdThreads = 640;  // (two of its warps idle: registers are split by groups of four)
 constexpr float kRise = 8.f;
@@ -278,176 +303,184 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     // (all four warps of a group at one instruction; together what the block was
     // launched with)
     if (warp >= 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == 16) {
-        const bool one = (t & 31) == 0;
-        if (one) {
-            ptx::mbar_arrive_expect_tx(q_full, (two ? 2 : 1) * F::TILE);
-            for (int g = 0; g < (two ? 2 : 1); g++)
-                for (int c = 0; c < DHP / 64; c++)
-                    ptx::tma_load_3d(smem + g * F::TILE + c * kChunk, &tq, q_full, c * 64, h, row0 + q0 + g * kT);
-        }
-        int it = 0;
-        uint32_t tails = 0;
-        for (int x = 0; x < tiles.count && ok; x++) {
-            const int k0 = tiles.at(x) * kT;
-            for (int kv = 0; kv < 2; kv++, it++) {
-                const int slot = it % F::SLOTS, round = it / F::SLOTS;
-                if (round && !(ok = wait(&empty[slot], round - 1))) break;
-                if (!(ok = fill_slot<DHP>(ring + slot * F::TILE, kv ? &tv : &tk, &full[slot], landed, tails, wait, hk,
-                                          row0 + k0, kv ? w.n - k0 : kT)))
-                    break;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == 16) {
+            const bool one = (t & 31) == 0;
+            if (one) {
+                ptx::mbar_arrive_expect_tx(q_full, (two ? 2 : 1) * F::TILE);
+                for (int g = 0; g < (two ? 2 : 1); g++)
+                    for (int c = 0; c < DHP / 64; c++)
+                        ptx::tma_load_3d(smem + g * F::TILE + c * kChunk, &tq, q_full, c * 64, h, row0 + q0 + g * kT);
             }
-        }
-        // no copy may land after the block has left
-        if (one) {
-            ptx::mbar_wait(q_full, 0, nullptr, 0);
-            for (int i = max(0, it - F::SLOTS); i < it; i++)
-                ptx::mbar_wait(&full[i % F::SLOTS], (i / F::SLOTS) & 1, nullptr, 0);
-        }
-    } else if (warp == 17) {
-        const uint32_t aQ = ptx::smem_u32(smem), aR = ptx::smem_u32(ring);
-        uint32_t given[2] = {0, 0};  // weights taken, by group
-        ok = wait(q_full, 0);
-        for (int x = 0; x <= tiles.count && ok; x++) {
-            const int ik = 2 * x, iv = 2 * x - 1;  // what the ring's slots hold: K0 V0 K1 V1 ...
-            const int sk = ik % F::SLOTS, sv = iv > 0 ? iv % F::SLOTS : 0;
-            const int kt = x < tiles.count ? tiles.at(x) : 0, before = x > 0 ? tiles.at(x - 1) : 0;
-            if (x > 0 && !(ok = wait(&full[sv], iv / F::SLOTS))) break;
-            if (x < tiles.count && !(ok = wait(&full[sk], ik / F::SLOTS))) break;
+            int it = 0;
+            uint32_t tails = 0;
+            for (int x = 0; x < tiles.count && ok; x++) {
+                const int k0 = tiles.at(x) * kT;
+                for (int kv = 0; kv < 2; kv++, it++) {
+                    const int slot = it % F::SLOTS, round = it / F::SLOTS;
+                    if (round && !(ok = wait(&empty[slot], round - 1))) break;
+                    if (!(ok = fill_slot<DHP>(ring + slot * F::TILE, kv ? &tv : &tk, &full[slot], landed, tails, wait, hk,
+                                              row0 + k0, kv ? w.n - k0 : kT)))
+                        break;
+                }
+            }
+            // no copy may land after the block has left
+            if (one) {
+                ptx::mbar_wait(q_full, 0, nullptr, 0);
+                for (int i = max(0, it - F::SLOTS); i < it; i++)
+                    ptx::mbar_wait(&full[i % F::SLOTS], (i / F::SLOTS) & 1, nullptr, 0);
+            }
+        } else if (warp == 17) {
+            const uint32_t aQ = ptx::smem_u32(smem), aR = ptx::smem_u32(ring);
+            uint32_t given[2] = {0, 0};  // weights taken, by group
+            ok = wait(q_full, 0);
+            for (int x = 0; x <= tiles.count && ok; x++) {
+                const int ik = 2 * x, iv = 2 * x - 1;  // what the ring's slots hold: K0 V0 K1 V1 ...
+                const int sk = ik % F::SLOTS, sv = iv > 0 ? iv % F::SLOTS : 0;
+                const int kt = x < tiles.count ? tiles.at(x) : 0, before = x > 0 ? tiles.at(x - 1) : 0;
+                if (x > 0 && !(ok = wait(&full[sv], iv / F::SLOTS))) break;
+                if (x < tiles.count && !(ok = wait(&full[sk], ik / F::SLOTS))) break;
 #pragma unroll
-            for (int g = 0; g < 2; g++) {
-                if (x > 0 && uses(g, before)) {
-                    if (!(ok = wait(&p_bar[g], given[g]))) break;
-                    ptx::tc_fence_after();
-                    if (elect()) {
-                        mma_add<DHP, 64>(tmem + 256 + 128 * g, tmem + 128 * g, mn_major(aR + sv * F::TILE), given[g] > 0);
-                        ptx::mma_commit(&o_bar[g]);
+                for (int g = 0; g < 2; g++) {
+                    if (x > 0 && uses(g, before)) {
+                        if (!(ok = wait(&p_bar[g], given[g]))) break;
+                        ptx::tc_fence_after();
+                        if (elect()) {
+                            mma_add<DHP, 64>(tmem + 256 + 128 * g, tmem + 128 * g, mn_major(aR + sv * F::TILE), given[g] > 0);
+                            ptx::mma_commit(&o_bar[g]);
+                        }
+                        given[g]++;
                     }
-                    given[g]++;
+                    if (x < tiles.count && uses(g, kt) && elect()) {
+                        ptx::tc_fence_after();
+                        mma_dot<DHP>(tmem + 128 * g, k_major(aQ + g * F::TILE), k_major(aR + sk * F::TILE));
+                        ptx::mma_commit(&s_bar[g]);
+                    }
                 }
-                if (x < tiles.count && uses(g, kt) && elect()) {
-                    ptx::tc_fence_after();
-                    mma_dot<DHP>(tmem + 128 * g, k_major(aQ + g * F::TILE), k_major(aR + sk * F::TILE));
-                    ptx::mma_commit(&s_bar[g]);
+                if (ok && elect()) {
+                    if (x > 0) ptx::mma_commit(&empty[sv]);
+                    if (x < tiles.count) ptx::mma_commit(&empty[sk]);
                 }
+                __syncwarp();
             }
-            if (ok && elect()) {
-                if (x > 0) ptx::mma_commit(&empty[sv]);
-                if (x < tiles.count) ptx::mma_commit(&empty[sk]);
+            if (elect()) {
+                ptx::mma_commit(drain);
+                ptx::mbar_wait(drain, 0, nullptr, 0);
             }
-            __syncwarp();
         }
-        if (elect()) {
-            ptx::mma_commit(drain);
-            ptx::mbar_wait(drain, 0, nullptr, 0);
-        }
-    }
     } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
-    if (warp < 8 || two) {
-        const int g = warp >> 3, half = warp >> 2 & 1, lg = warp & 3, r = lg * 32 + (t & 31);
-        const int i = q0 + g * kT + r;  // query of the sequence
-        const uint32_t lanes = tmem + ((uint32_t)(lg * 32) << 16);
-        const uint32_t base = lanes + 128 * g + 64 * half, o_at = lanes + 256 + 128 * g + half * (DHP / 2);
-        const float sl2 = d.scale * kLog2e;
-        float ref = -INFINITY, sum = 0.f;  // what the weights are taken against (powers of two), this half's sum
-        uint32_t done = 0;                 // tiles behind
-        // What the thread of this row's other half has. (It has read what was here
-        // before: the scores that this thread waited for came after its weights.)
-        auto swap = [&](float mine) {
-            float* at = tops + g * 2 * kT;
-            at[half * kT + r] = mine;
-            asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + lg) : "memory");
-            return at[(half ^ 1) * kT + r];
-        };
-        for (int x = 0; x < tiles.count; x++) {
-            const int kt = tiles.at(x), k0 = kt * kT;
-            if (!uses(g, kt)) continue;
-            if (!(ok = wait(&s_bar[g], done))) break;
-            ptx::tc_fence_after();
-            uint32_t a[64];
-            ptx::tmem_ld32(base, a);
-            ptx::tmem_ld32(base + 32, a + 32);
-            ptx::tmem_ld_wait_regs32(a);
-            ptx::tmem_ld_wait_regs32(a + 32);
-            if (!all_seen(d, q0 + g * kT, k0)) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        if (warp < 8 || two) {
+            const int g = warp >> 3, half = warp >> 2 & 1, lg = warp & 3, r = lg * 32 + (t & 31);
+            const int i = q0 + g * kT + r;  // query of the sequence
+            const uint32_t lanes = tmem + ((uint32_t)(lg * 32) << 16);
+            const uint32_t base = lanes + 128 * g + 64 * half, o_at = lanes + 256 + 128 * g + half * (DHP / 2);
+            const float sl2 = d.scale * kLog2e;
+            float ref = -INFINITY, sum = 0.f;  // what the weights are taken against (powers of two), this half's sum
+            uint32_t done = 0;                 // tiles behind
+            // What the thread of this row's other half has. (It has read what was here
+            // before: the scores that this thread waited for came after its weights.)
+            auto swap = [&](float& v) {
+                float* at = tops + g * 2 * kT;
+                at[half * kT + r] = v;
+                ok = !meet<64>(1 + g * 4 + lg, false);
+                v = at[(half ^ 1) * kT + r];
+                return ok;
+            };
+            auto await = [&](uint64_t* bar, uint32_t phase) {
+                ok = wait(bar, phase);
+                if (!ok) meet<64>(1 + g * 4 + lg, true);
+                return ok;
+            };
+            for (int x = 0; x < tiles.count; x++) {
+                const int kt = tiles.at(x), k0 = kt * kT;
+                if (!uses(g, kt)) continue;
+                if (!await(&s_bar[g], done)) break;
+                ptx::tc_fence_after();
+                uint32_t a[64];
+                ptx::tmem_ld32(base, a);
+                ptx::tmem_ld32(base + 32, a + 32);
+                ptx::tmem_ld_wait_regs32(a);
+                ptx::tmem_ld_wait_regs32(a + 32);
+                if (!all_seen(d, q0 + g * kT, k0)) {
+#pragma unroll
+                    for (int c = 0; c < 64; c += 32) {
+                        const uint32_t on = keys_seen(d, i, k0 + 64 * half + c);
+#pragma unroll
+                        for (int e = 0; e < 32; e++)
+                            if (!(on >> e & 1)) a[c + e] = 0xff800000u;
+                    }
+                }
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 64; c += 2)
+                    m4[(c >> 1) & 3] = max3(m4[(c >> 1) & 3], __uint_as_float(a[c]), __uint_as_float(a[c + 1]));
+                const float mine = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]);
+                float top = mine;
+                if (!swap(top)) break;
+                top = fmaxf(top, mine) * sl2;  // (the scale is positive)
+                const bool rise = top > ref + kRise;          // ref -inf: the first finite score
+                if (__any_sync(0xffffffffu, rise)) {
+                    const float turn = rise ? ex2(ref - top) : 1.f;
+                    if (rise) ref = top;
+                    sum *= turn;
+                    if (done) {
+                        if (!await(&o_bar[g], done - 1)) break;
+                        ptx::tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < DHP / 2; c += 16) {
+                            uint32_t o[16];
+                            ptx::tmem_ld16(o_at + c, o);
+                            ptx::tmem_ld_wait_regs16(o);
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * turn);
+                            ptx::tmem_st16(o_at + c, o);
+                        }
+                    }
+                }
+                const float safe = ref == -INFINITY ? 0.f : ref;
+                const uint64_t SL2 = f2_pack(sl2, sl2), NEG = f2_pack(-safe, -safe);
+                uint64_t s4[2] = {0, 0};
 #pragma unroll
                 for (int c = 0; c < 64; c += 32) {
-                    const uint32_t on = keys_seen(d, i, k0 + 64 * half + c);
+                    uint32_t pk[16];
 #pragma unroll
-                    for (int e = 0; e < 32; e++)
-                        if (!(on >> e & 1)) a[c + e] = 0xff800000u;
-                }
-            }
-            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int c = 0; c < 64; c += 2)
-                m4[(c >> 1) & 3] = max3(m4[(c >> 1) & 3], __uint_as_float(a[c]), __uint_as_float(a[c + 1]));
-            float top = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]);
-            top = fmaxf(top, swap(top)) * sl2;  // (the scale is positive)
-            const bool rise = top > ref + kRise;          // ref -inf: the first finite score
-            if (__any_sync(0xffffffffu, rise)) {
-                const float turn = rise ? ex2(ref - top) : 1.f;
-                if (rise) ref = top;
-                sum *= turn;
-                if (done) {
-                    if (!(ok = wait(&o_bar[g], done - 1))) break;
-                    ptx::tc_fence_after();
-#pragma unroll 1
-                    for (int c = 0; c < DHP / 2; c += 16) {
-                        uint32_t o[16];
-                        ptx::tmem_ld16(o_at + c, o);
-                        ptx::tmem_ld_wait_regs16(o);
-#pragma unroll
-                        for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * turn);
-                        ptx::tmem_st16(o_at + c, o);
+                    for (int e = 0; e < 16; e++) {
+                        float x0, x1;
+                        f2_unpack(f2_fma(f2_pack(__uint_as_float(a[c + 2 * e]), __uint_as_float(a[c + 2 * e + 1])), SL2, NEG), x0, x1);
+                        x0 = ex2(x0);
+                        x1 = ex2(x1);
+                        s4[e & 1] = f2_add(s4[e & 1], f2_pack(x0, x1));
+                        const __nv_bfloat162 p = __floats2bfloat162_rn(x0, x1);
+                        pk[e] = *reinterpret_cast<const uint32_t*>(&p);
                     }
+                    ptx::tmem_st16(base + c / 2, pk);
                 }
+                float s0, s1;
+                f2_unpack(f2_add(s4[0], s4[1]), s0, s1);
+                sum += s0 + s1;
+                ptx::tmem_st_wait();
+                ptx::tc_fence_before();
+                warp_arrive(&p_bar[g]);
+                done++;
             }
-            const float safe = ref == -INFINITY ? 0.f : ref;
-            const uint64_t SL2 = f2_pack(sl2, sl2), NEG = f2_pack(-safe, -safe);
-            uint64_t s4[2] = {0, 0};
-#pragma unroll
-            for (int c = 0; c < 64; c += 32) {
-                uint32_t pk[16];
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    float x0, x1;
-                    f2_unpack(f2_fma(f2_pack(__uint_as_float(a[c + 2 * e]), __uint_as_float(a[c + 2 * e + 1])), SL2, NEG), x0, x1);
-                    x0 = ex2(x0);
-                    x1 = ex2(x1);
-                    s4[e & 1] = f2_add(s4[e & 1], f2_pack(x0, x1));
-                    const __nv_bfloat162 p = __floats2bfloat162_rn(x0, x1);
-                    pk[e] = *reinterpret_cast<const uint32_t*>(&p);
-                }
-                ptx::tmem_st16(base + c / 2, pk);
-            }
-            float s0, s1;
-            f2_unpack(f2_add(s4[0], s4[1]), s0, s1);
-            sum += s0 + s1;
-            ptx::tmem_st_wait();
-            ptx::tc_fence_before();
-            warp_arrive(&p_bar[g]);
-            done++;
-        }
-        ok = ok && wait(&o_bar[g], done - 1);  // a query's own tile is always among its tiles
-        ptx::tc_fence_after();
-        if (ok) {
-            sum += swap(sum);
-            const float mul = sum == 0.f ? 0.f : 1.f / sum;
-            __nv_bfloat16* to = (__nv_bfloat16*)d.out.p + (w.row0 + i) * d.out.row + h * d.out.head;
+            float rest = sum;
+            if (ok && await(&o_bar[g], done - 1) && swap(rest)) {  // a query's own tile is always among its tiles
+                ptx::tc_fence_after();
+                sum += rest;
+                const float mul = sum == 0.f ? 0.f : 1.f / sum;
+                __nv_bfloat16* to = (__nv_bfloat16*)d.out.p + (w.row0 + i) * d.out.row + h * d.out.head;
 #pragma unroll 1
-            for (int c = 0; c < DHP / 2; c += 32) {
-                uint32_t v[32];
-                ptx::tmem_ld32(o_at + c, v);
-                ptx::tmem_ld_wait_regs32(v);
-                if (i < w.n) store_cols<32>(to + half * (DHP / 2) + c, v, mul, d.dh - half * (DHP / 2) - c);
+                for (int c = 0; c < DHP / 2; c += 32) {
+                    uint32_t v[32];
+                    ptx::tmem_ld32(o_at + c, v);
+                    ptx::tmem_ld_wait_regs32(v);
+                    if (i < w.n) store_cols<32>(to + half * (DHP / 2) + c, v, mul, d.dh - half * (DHP / 2) - c);
+                }
+                if (half == 0 && i < w.n && d.lse)
+                    d.lse[h * d.ld_lse + w.row0 + i] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * kLn2;
             }
-            if (half == 0 && i < w.n && d.lse)
-                d.lse[h * d.ld_lse + w.row0 + i] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * kLn2;
         }
-    }
     }
     ptx::tc_fence_before();
     __syncthreads();
@@ -467,16 +500,30 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 //              [448, 512) in turn
 //   warps 0..15   dS = P (dP - D), four threads a query with 32 keys each: their
 //              registers hold both scores at once, and four warps a scheduler
-//              hide each other's latencies. Before the first tile they form D = rowdot(dout, out), which the second
-//              kernel reads too.
+//              hide each other's latencies. Before the first tile they form
+//              D = rowdot(dout, out), which the second kernel reads too.
+//
+// `out` is bf16, so that this D is off by up to 2^-9 |dout| |out|, and with it
+// every dS of the row by P times that. Where rows see few keys, dS itself is
+// small (one key: 0) and that is most of its error. There a pass before sums
+// dS: as the weights P add up to 1, the sum over a row of P (dP - D) is what D
+// is short of. Rounding dS to bf16 for the products remains (2^-9 of itself).
+// Error of dq and dk against 64 bits, in the norm: window of 2 keys 3.8e-3 to
+// 2.4e-3, sequences of 5 rows 3.9e-3 to 2.1e-3, and up to 2.5e-3 as in blocks of
+// many tiles, which go without; one pass more of a block costs 2/3 of its time.
+//
+// Bound by the products' issue and turns: 8192 rows in 3 sequences, 16 heads of
+// 128 columns, window 1024: 162 us, 0.52 PFLOP/s in S, dP and dQ.
 // ---------------------------------------------------------------------------
 constexpr int kBwdQThreads = 608;
+constexpr int kFewTiles = 2;  // tiles of keys for which the pass is made (none: dq 1 to 4 % faster, see above)
 
 template <int DHP>
 struct BwdQ {
     static constexpr int TILE = DHP / 64 * kChunk;
     static constexpr int SLOTS = DHP == 128 ? 5 : 8;
-    static constexpr int SMEM = (2 + SLOTS) * TILE + 128 * 4 + 512 + 1024;
+    static constexpr int SMEM = (2 + SLOTS) * TILE + 4 * kT * 4 + 512;  // (no room to move its start)
+    static_assert(SMEM <= 227 * 1024, "above what a block may have");
 };
 
 template <int DHP>
@@ -485,11 +532,14 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
                            const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tg,
                            const __grid_constant__ WindowDesc d) {
     using F = BwdQ<DHP>;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if (ptx::smem_u32(smem) & 1023) {  // tiles begin on multiples of 1024
+        if (threadIdx.x == 0) atomicCAS(d.err, 0, kErrBadShape);
+        return;
+    }
     uint8_t* ring = smem + 2 * F::TILE;
-    float* sums = reinterpret_cast<float*>(ring + F::SLOTS * F::TILE);  // [128] D
-    uint64_t* q_full = reinterpret_cast<uint64_t*>(sums + 128);
+    float* sums = reinterpret_cast<float*>(ring + F::SLOTS * F::TILE);  // [4][128] of a row's quarters
+    uint64_t* q_full = reinterpret_cast<uint64_t*>(sums + 4 * kT);
     uint64_t* full = q_full + 1;
     uint64_t* empty = full + F::SLOTS;
     uint64_t* s_bar = empty + F::SLOTS;  // S and dP of a tile in TMEM
@@ -535,6 +585,7 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
     const Waits wait{failed, d.err};
     bool ok = true;
     const KeyTiles tiles(d, q0, min(q0 + kT, w.n), kT);
+    const int first = tiles.count <= kFewTiles ? tiles.count : 0;  // steps of the pass that only sums
 
     if (warp == 17) {
         const bool one = (t & 31) == 0;
@@ -547,8 +598,8 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
         }
         int it = 0;
         uint32_t tails = 0;
-        for (int x = 0; x < tiles.count && ok; x++) {
-            const int k0 = tiles.at(x) * kT;
+        for (int x = -first; x < tiles.count && ok; x++) {
+            const int k0 = tiles.at(x < 0 ? x + first : x) * kT;
             for (int kv = 0; kv < 2; kv++, it++) {
                 const int slot = it % F::SLOTS, round = it / F::SLOTS;
                 if (round && !(ok = wait(&empty[slot], round - 1))) break;
@@ -566,22 +617,28 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
         const uint32_t aQ = ptx::smem_u32(smem), aG = aQ + F::TILE, aR = ptx::smem_u32(ring);
         Turnstile<F::SLOTS> ts;
         ok = wait(q_full, 0);
-        for (int x = 0; x < tiles.count && ok; x++) {
-            const uint32_t k_at = aR + ts.slot * F::TILE;
-            if (!(ok = wait(&full[ts.slot], ts.phase))) break;
+        auto both = [&](int step, bool keys) {  // keys: no other product reads them
+            const int slot = ts.slot;
+            const uint32_t k_at = aR + slot * F::TILE;
+            if (!(ok = wait(&full[slot], ts.phase))) return;
             ts.skip(1);
-            if (!(ok = wait(&full[ts.slot], ts.phase))) break;
-            if (x > 0 && !(ok = wait(r_bar, x - 1))) break;
+            if (!(ok = wait(&full[ts.slot], ts.phase))) return;
+            if (step > 0 && !(ok = wait(r_bar, step - 1))) return;
             ptx::tc_fence_after();
             if (elect()) {
                 mma_dot<DHP>(tmem, k_major(aQ), k_major(k_at));
                 mma_dot<DHP>(tmem + 128, k_major(aG), k_major(aR + ts.slot * F::TILE));
                 ptx::mma_commit(s_bar);
                 ptx::mma_commit(&empty[ts.slot]);
+                if (keys) ptx::mma_commit(&empty[slot]);
             }
             __syncwarp();
             ts.skip(1);
-        }
+        };
+#pragma unroll 1
+        for (int step = 0; step < first && ok; step++) both(step, true);
+#pragma unroll 1
+        for (int x = 0; x < tiles.count && ok; x++) both(first + x, false);
         if (elect()) {
             ptx::mma_commit(&drain[0]);
             ptx::mbar_wait(&drain[0], 0, nullptr, 0);
@@ -589,6 +646,7 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
     } else if (warp == 18) {
         const uint32_t aR = ptx::smem_u32(ring);
         Turnstile<F::SLOTS> ts;
+        for (int x = 0; x < first; x++) ts.skip(2);
         for (int x = 0; x < tiles.count && ok; x++) {
             if (!(ok = wait(p_bar, x))) break;
             ptx::tc_fence_after();
@@ -631,25 +689,31 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
                 }
             }
         }
-        for (int p = 0; p < 4; p++) {  // the quarters in order
-            if (p == part) sums[r] = p ? sums[r] + D : D;
-            asm volatile("bar.sync 1, 512;" ::: "memory");
-        }
-        D = sums[r];
-        if (part == 0 && i < w.n) d.dvec[(long long)h * d.T + w.row0 + i] = D;
-        const uint64_t SL2 = f2_pack(sl2, sl2), NEG = f2_pack(-lse2, -lse2), ND = f2_pack(-D, -D);
-        for (int x = 0; x < tiles.count; x++) {
-            const int k0 = tiles.at(x) * kT;
-            if (!(ok = wait(s_bar, x))) break;
+        // the sum of a row's four threads, in their order
+        auto add_up = [&](float& v) {
+            sums[part * kT + r] = v;
+            ok = !meet<512>(1, false);
+            v = ((sums[r] + sums[kT + r]) + sums[2 * kT + r]) + sums[3 * kT + r];
+            return ok;
+        };
+        auto await = [&](uint64_t* bar, uint32_t phase) {
+            ok = wait(bar, phase);
+            if (!ok) meet<512>(1, true);
+            return ok;
+        };
+        add_up(D);
+        const uint64_t SL2 = f2_pack(sl2, sl2), NEG = f2_pack(-lse2, -lse2);
+        uint32_t a[32], g[32];
+        auto gradients = [&](int step, int k0) {  // dS of the thread's 32 keys into g
+            if (!await(s_bar, step)) return false;
             ptx::tc_fence_after();
-            uint32_t a[32], g[32];
             ptx::tmem_ld32(base + part * 32, a);
             ptx::tmem_ld32(base + 128 + part * 32, g);
             ptx::tmem_ld_wait_regs32(a);
             ptx::tmem_ld_wait_regs32(g);
             ptx::tc_fence_before();
             warp_arrive(r_bar);
-            uint32_t pk[16];
+            const uint64_t ND = f2_pack(-D, -D);
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 float x0, x1, y0, y1;
@@ -666,13 +730,28 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
                 for (int e = 0; e < 32; e++)
                     if (!(on >> e & 1)) g[e] = 0u;
             }
+            return true;
+        };
+        if (first) {
+            float rest = 0.f;  // sum of dS: what D is short of
+#pragma unroll 1
+            for (int x = 0; x < first && gradients(x, tiles.at(x) * kT); x++)
+#pragma unroll
+                for (int e = 0; e < 32; e++) rest += __uint_as_float(g[e]);
+            ok = ok && !meet<512>(1, false);  // all have read the sums before
+            if (ok && add_up(rest)) D += rest;
+        }
+        if (part == 0 && i < w.n) d.dvec[(long long)h * d.T + w.row0 + i] = D;
+#pragma unroll 1
+        for (int x = 0; x < tiles.count && ok && gradients(first + x, tiles.at(x) * kT); x++) {
+            uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 const __nv_bfloat162 p = __floats2bfloat162_rn(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]));
                 pk[e] = *reinterpret_cast<const uint32_t*>(&p);
             }
             if (x > 1) {
-                if (!(ok = wait(&o_bar[x & 1], (x >> 1) - 1))) break;  // the product before the last has read its dS
+                if (!await(&o_bar[x & 1], (x >> 1) - 1)) break;  // the product before the last has read its dS
                 ptx::tc_fence_after();
             }
             ptx::tmem_st16(base + 384 + 64 * (x & 1) + part * 16, pk);
@@ -680,10 +759,9 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
             ptx::tc_fence_before();
             warp_arrive(p_bar);
         }
-        const int last = tiles.count - 1;
-        ok = ok && wait(&o_bar[last & 1], last >> 1);  // (the product before it was added before)
-        ptx::tc_fence_after();
-        if (ok) {
+        const int end = tiles.count - 1;
+        if (ok && await(&o_bar[end & 1], end >> 1)) {  // (the product before it was added before)
+            ptx::tc_fence_after();
             __nv_bfloat16* to = (__nv_bfloat16*)d.dq.p + (w.row0 + i) * d.dq.row + h * d.dq.head;
             if constexpr (DHP == 128) {
                 uint32_t v[32];
@@ -726,7 +804,12 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
 //              come from.
 //   warps 0..15   P and dS, four threads a key with 32 queries each: while P is
 //              computed the tensor cores run dK and the next dP, while dS is,
-//              dV and the next S.
+//              dV and the next S. P and dS are off by 2^-9 of themselves at most.
+//
+// Bound as the queries' gradient is, with one product more: 8192 rows in 3
+// sequences, 16 heads of 128 columns on 4 key heads, window 1024: 177 us,
+// 0.63 PFLOP/s, and 18 us to join the cut tiles; 20000 rows of 4 heads of 64 on
+// one, window 4000: 237 us and 9.
 // ---------------------------------------------------------------------------
 constexpr int kBwdKvThreads = 640;
 constexpr int kStats = 4;      // tiles of lse and D held
