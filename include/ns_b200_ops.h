@@ -279,7 +279,7 @@ int nsb_op_fp8_quantize_block(const void* x, int dtype, long long ld, int M, int
 
 /* What went wrong on the current device since the last call, in a product
  * below whose caller gave no dev_err or with an index past its tensor's rows:
- * 0, or the first error's code, which is cleared (101 to 103: a bounded wait
+ * 0, or the first error's code, which is cleared (101 to 104: a bounded wait
  * ran out and the product's result is not to be used; 111: an index was left
  * out). Waits for the stream; not inside a capture. */
 int nsb_op_device_error(int* code, void* stream);
@@ -347,7 +347,7 @@ int nsb_op_rope_bwd(const void* dy, int dtype, long long dy_row, long long dy_he
  * q). A token with a negative seq[t] is padding: nothing of it is read or
  * written. One whose place is outside the table or the cache is left out too,
  * and reported by nsb_op_device_error. No two tokens of one call go to the
- * same place. */
+ * same place. (2 Hkv + Hq) * dh is at most 2^26. */
 int nsb_op_kv_append(const void* k, long long k_row, long long k_head, const void* v, long long v_row, long long v_head,
                      int dtype, int T, int Hkv, int dh, const int* seq, const int* at, const int* table, long long ld_table,
                      int B, int width, int pages, int page, void* k_cache, long long kc_page, long long kc_slot,
@@ -364,7 +364,7 @@ int nsb_op_kv_append(const void* k, long long k_row, long long k_head, const voi
  * zeros and -inf. A length that the table has no room for is cut, and a page
  * outside the cache left out; both are reported by nsb_op_device_error. What
  * the cache holds behind a sequence's end is not looked at. dh <= 128,
- * B <= 8192, scale > 0. workspace (16-byte aligned) of at least
+ * B <= 8192, B * Hq < 2^31, scale > 0. workspace (16-byte aligned) of at least
  * nsb_op_attention_paged_workspace_bytes(...) bytes: of this call alone until
  * it is done. */
 size_t nsb_op_attention_paged_workspace_bytes(int B, int Hq, int Hkv, int dh);
@@ -382,8 +382,9 @@ int nsb_op_attention_paged(const void* q, long long q_row, long long q_head, int
  *   j <= i  and  (window == 0  or  i - j < window  or  j < sinks).
  * lse [Hq, ld_lse] receives the log-sum-exp (may be NULL). Rows behind the
  * last sequence are neither read nor written. Offsets that do not rise are
- * cut and reported by nsb_op_device_error. dh <= 128, scale > 0. A value of a
- * sequence that is infinite or NaN can reach its queries before it too. */
+ * cut and reported by nsb_op_device_error. dh <= 128, scale > 0, T <= 2^30,
+ * Hq <= 65535. A value of a sequence that is infinite or NaN can reach its
+ * queries before it too, and such a gradient its keys behind it. */
 int nsb_op_attention_window(const void* q, long long q_row, long long q_head, const void* k, long long k_row,
                             long long k_head, const void* v, long long v_row, long long v_head, int dtype, int T, int Hq,
                             int Hkv, int dh, const int* offsets, int B, int window, int sinks, float scale, void* out,

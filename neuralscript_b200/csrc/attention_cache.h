@@ -19,6 +19,7 @@ constexpr int kMaxAxes = 4;         // axes of a position
 constexpr int kTurnMaxHead = 1024;  // columns of a head that is rotated
 constexpr int kAttnMaxHead = 128;   // columns of a head in attention
 constexpr int kPagedMaxBatch = 8192;
+constexpr int kWindowMaxRows = 1 << 30;
 
 // A tensor of heads: row t, head h at p + t * row + h * head.
 struct Heads {
@@ -100,7 +101,7 @@ struct WindowDesc {
     void* workspace = nullptr;
     size_t workspace_bytes = 0;
     float* dvec = nullptr;    // in the workspace: [Hq, T] rowdot(dout, out)
-    float* parts = nullptr;   // and sums of tiles that several blocks share
+    float* parts = nullptr;   // on the tensor cores also sums of tiles that several blocks share
     int* err = nullptr;
 };
 int attention_window(const WindowDesc& d, cudaStream_t s);

@@ -918,7 +918,7 @@ int attention_paged(const PagedDesc& d, cudaStream_t st) {
     if (d.pages < 0 || d.page <= 0 || d.width < 0 || d.ld_table < d.width || d.window < 0 || d.sinks < 0 ||
         !(d.scale > 0.f) || !(d.scale < INFINITY))
         return -1;
-    if (d.B > kPagedMaxBatch) return -2;
+    if (d.B > kPagedMaxBatch || (long long)d.B * d.Hq > 0x7fffffff) return -2;
     if (d.B == 0) return 0;
     // units are counted in 32 bits, those of one warp too
     const long long room = (long long)d.width * d.page, seen = d.window ? (long long)d.window + d.sinks : room;

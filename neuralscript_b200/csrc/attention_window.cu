@@ -375,7 +375,8 @@ int check(const WindowDesc& d) {
         !(d.scale < INFINITY))
         return -1;
     if (!d.offsets && d.B != 1) return -1;
-    if (d.Hq > 65535) return -2;
+    // rows are counted in 32 bits, with room for a window's, and so are the steps of one tile of keys
+    if (d.Hq > 65535 || d.T > kWindowMaxRows || ((long long)d.T / kB + 1) * (d.Hq / d.Hkv) > 0x7fffffff) return -2;
     return 0;
 }
 

@@ -28,6 +28,7 @@ namespace {
 
 constexpr int kTurnThreads = 256;
 constexpr int kTurnTokens = 8;  // most tokens of a block
+constexpr int kTurnMaxRow = 1 << 26;  // columns of a token, all heads
 
 struct TurnJob {
     const void* src;
@@ -236,7 +237,7 @@ int launch(TurnArgs& a, int dtype, cudaStream_t s) {
         return cudaGetLastError() == cudaSuccess ? 0 : -5;
     };
     using std::integral_constant;
-    if ((long long)a.heads * a.dh > (1 << 26)) return -2;
+    if ((long long)a.heads * a.dh > kTurnMaxRow) return -2;
     if (dtype == kBF16) {
         if (fits(8)) return go(__nv_bfloat16(), integral_constant<int, 8>());
         if (fits(4)) return go(__nv_bfloat16(), integral_constant<int, 4>());
@@ -273,6 +274,7 @@ int rope(const Turn& t, int dtype, const Heads& x, const Heads& y, int T, int H,
 int kv_append(const AppendDesc& d, cudaStream_t s) {
     if (d.T < 0 || d.Hkv <= 0 || d.dh <= 0 || d.dh > kTurnMaxHead || (d.dh & 1) || (d.dtype != kF32 && d.dtype != kBF16))
         return -1;
+    if ((2LL * d.Hkv + (d.q.p ? d.Hq : 0)) * d.dh > kTurnMaxRow) return -2;
     if (d.B < 0 || d.width < 0 || d.ld_table < d.width || d.pages < 0 || d.page <= 0 || !turn_ok(d.turn, d.dh, d.T)) return -1;
     if ((d.q.p == nullptr) != (d.q_out.p == nullptr) || (d.q.p && d.Hq <= 0)) return -1;
     if (d.T == 0) return 0;

@@ -640,11 +640,18 @@ def attention_paged(q, k_cache, v_cache, table, lens, out, lse=None, window=0, s
     rc = lib.nsb_op_attention_paged(
         *_heads(d, q, "q", dt, B, Hq, dh), kind, B, Hq, Hkv, dh, *_pages(d, k_cache, "k_cache", dt, pages, page, Hkv, dh),
         *_pages(d, v_cache, "v_cache", dt, pages, page, Hkv, dh), pages, page, *_rows(d, table, "table", _i32, B, width), width,
-        _dense(d, lens, "lens", _i32, (B,)), window, sinks, dh ** -0.5 if scale is None else scale,
+        _dense(d, lens, "lens", _i32, (B,)), *_reach(window, sinks), dh ** -0.5 if scale is None else scale,
         *_heads(d, out, "out", dt, B, Hq, dh), None if lse is None else _dense(d, lse, "lse", _f32, (B, Hq)),
         _dense(d, workspace, "workspace", _u8, (have,)), have, _stream_of(d))
     if rc:
         _check(rc, "nsb_op_attention_paged")
+
+
+def _reach(window, sinks):
+    """Both as the entries take them: an int of 32 bits would drop the digits above."""
+    if not 0 <= window < 2147483648 or not 0 <= sinks < 2147483648:
+        raise ValueError(f"window {window}, sinks {sinks} where 0 to 2^31 - 1 is wanted")
+    return window, sinks
 
 
 def _packed(d, q, k, v, offsets, window, sinks, scale):
@@ -654,8 +661,8 @@ def _packed(d, q, k, v, offsets, window, sinks, scale):
     Hkv = k.shape[1]
     B = 1 if offsets is None else offsets.shape[0] - 1
     return (*_heads(d, q, "q", dt, T, Hq, dh), *_heads(d, k, "k", dt, T, Hkv, dh), *_heads(d, v, "v", dt, T, Hkv, dh), kind,
-            T, Hq, Hkv, dh, None if offsets is None else _dense(d, offsets, "offsets", _i32, (B + 1,)), B, window, sinks,
-            dh ** -0.5 if scale is None else scale)
+            T, Hq, Hkv, dh, None if offsets is None else _dense(d, offsets, "offsets", _i32, (B + 1,)), B,
+            *_reach(window, sinks), dh ** -0.5 if scale is None else scale)
 
 
 def attention_window(q, k, v, out, lse=None, offsets=None, window=0, sinks=0, scale=None):

@@ -28,8 +28,9 @@ def mask(n, m, window, sinks, device):
     return (j <= i) & ((i - j < window) | (j < sinks) if window else torch.ones_like(j <= i))
 
 
-def attend(q, k, v, seen, scale, dtype, dout=None):
-    """One head: q [n, dh], k, v [m, dh] in 64 bits. out, lse and with dout dq, dk, dv, each beside its tolerance."""
+def attend(q, k, v, seen, scale, dtype, dout=None, summed=False):
+    """One head: q [n, dh], k, v [m, dh] in 64 bits. out, lse and with dout dq, dk, dv, each beside its tolerance.
+    summed: D = sum_j p_j dP_j, not from the rounded out: it was that first, then the sum of P (dP - D) was added."""
     u, w = half_step(dtype), half_step(dtype)
     m, dh = k.shape
     e = 2.0 ** -24
@@ -49,6 +50,9 @@ def attend(q, k, v, seen, scale, dtype, dout=None):
     many = dh * e
     size_p, size_D = dout.abs() @ v.abs().t(), (dout.abs() * out.abs()).sum(1, keepdim=True)
     off_D = (dout.abs() * out_tol).sum(1, keepdim=True) + many * size_D
+    if summed:  # what was wrong before is left as far as the weights' sum is off 1
+        mean = (p * size_p).sum(1, keepdim=True)
+        off_D = off * (off_D + mean + size_D) + (many + m * e) * (2 * mean + size_D)
     off_s = (w + m * e) * ds.abs() + p * (off * (size_p + size_D) + many * size_p + off_D) + TINY * (size_p + size_D)
     got["dv"] = (p.t() @ dout, u * (p.t() @ dout).abs() + ((w + 2 * off) * p + TINY).t() @ dout.abs() + TINY)
     got["dq"] = (scale * ds @ k, u * (scale * ds @ k).abs() + scale * off_s @ k.abs() + TINY)
@@ -56,7 +60,7 @@ def attend(q, k, v, seen, scale, dtype, dout=None):
     return got
 
 
-def packed(q, k, v, offsets, window, sinks, scale, dtype, dout=None):
+def packed(q, k, v, offsets, window, sinks, scale, dtype, dout=None, summed=False):
     """All sequences and heads: {name: (value, tolerance)}, rows of no sequence 0."""
     T, Hq, dh = q.shape
     Hkv = k.shape[1]
@@ -72,7 +76,7 @@ def packed(q, k, v, offsets, window, sinks, scale, dtype, dout=None):
         for h in range(Hq):
             hk = h // (Hq // Hkv)
             got = attend(q[lo:hi, h].double(), k[lo:hi, hk].double(), v[lo:hi, hk].double(), seen, scale, dtype,
-                         None if dout is None else dout[lo:hi, h].double())
+                         None if dout is None else dout[lo:hi, h].double(), summed)
             for n, pair in got.items():
                 at = hk if n in ("dk", "dv") else h
                 for f, x in zip(full[n], pair):

@@ -53,6 +53,11 @@ def test_append_of_no_tokens():
     assert call("nsb_op_kv_append", APPEND, dict(T=0)) == 0
 
 
+@pytest.mark.parametrize("big", [dict(Hkv=1 << 30), dict(Hkv=(1 << 26) + 1), dict(Hq=(1 << 31) - 1), dict(Hq=1 << 20)])
+def test_append_limits(big):
+    assert call("nsb_op_kv_append", APPEND, big) == -2
+
+
 PAGED = dict(q=X, q_row=64, q_head=64, dtype=1, B=2, Hq=4, Hkv=2, dh=64, kc=X, kc_page=1024, kc_slot=64, kc_head=64, vc=X, vc_page=1024, vc_slot=64,
              vc_head=64, pages=9, page=16, table=X, ld_table=3, width=3, lens=X, window=0, sinks=0, scale=0.125, out=X, o_row=64, o_head=64,
              lse=X, workspace=X, bytes=1 << 30)
@@ -69,6 +74,7 @@ def test_paged_refuses(bad):
 def test_paged_limits():
     assert call("nsb_op_attention_paged", PAGED, dict(B=8193)) == -2
     assert call("nsb_op_attention_paged", PAGED, dict(B=8192, width=2 ** 30, ld_table=2 ** 30)) == -2
+    assert call("nsb_op_attention_paged", PAGED, dict(B=8192, Hq=1 << 20, Hkv=1 << 20, width=1)) == -2
     assert call("nsb_op_attention_paged", PAGED, dict(B=0)) == 0
     size = ops.L().nsb_op_attention_paged_workspace_bytes
     assert size(0, 4, 2, 64) == size(2, 3, 2, 64) == size(2, 4, 2, 129) == size(2, 4, 0, 64) == 0
@@ -100,3 +106,5 @@ def test_window_limits():
         assert call(name, ok, dict(T=0)) == 0
         assert call(name, ok, dict(B=0)) == 0
         assert call(name, ok, dict(Hq=131072, Hkv=65536)) == -2
+        assert call(name, ok, dict(T=(1 << 30) + 1, ld_lse=1 << 31)) == -2
+        assert call(name, ok, dict(T=1 << 30, Hq=65535, Hkv=1, ld_lse=1 << 31)) == -2

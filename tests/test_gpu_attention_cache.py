@@ -344,7 +344,7 @@ def test_paged_of_no_sequences():
 # ---------------------------------------------------------------------------
 # packed sequences with a window
 # ---------------------------------------------------------------------------
-def run_window(lens, Hq, Hkv, dh, window, sinks, dtype, train, spare=0, scale=None, amp=1.5, seed=1, lead=0):
+def run_window(lens, Hq, Hkv, dh, window, sinks, dtype, train, spare=0, scale=None, amp=1.5, seed=1, lead=0, summed=False):
     """Fills rows of no sequence with NaN, and checks that they stay."""
     offsets = [lead]
     for n in lens:
@@ -363,7 +363,7 @@ def run_window(lens, Hq, Hkv, dh, window, sinks, dtype, train, spare=0, scale=No
     if scale is None:
         scale = dh ** -0.5
     ops.attention_window(q, k, v, out, lse=lse, **kw)
-    want = packed(q, k, v, offsets, window, sinks, scale, dtype, dout if train else None)
+    want = packed(q, k, v, offsets, window, sinks, scale, dtype, dout if train else None, summed)
     mine = slice(offsets[0], offsets[-1])
     close(out[mine], *(x[mine] for x in want["out"]), "out")
     close(lse[:, mine], *(x[:, mine] for x in want["lse"]), "lse")
@@ -450,6 +450,12 @@ def test_window_unaligned(dtype):
         want = packed(q, k, v, [0, T], 77, 1, 0.125, dtype, dout)
         for name, x in dict(out=out, lse=lse, dq=dq, dk=dk, dv=dv).items():
             close(x, *want[name], name)
+
+
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("lens,window", [([2, 3, 5, 9, 40, 256], 0), ([700, 1, 130], 2), ([300, 129], 100)])
+def test_window_gradient_of_rows_with_few_keys(lens, window, dh):
+    run_window(lens, 4, 2, dh, window, 0, BF, True, summed=True)
 
 
 def test_window_gradient_against_differences():
@@ -639,6 +645,18 @@ def test_two_streams_at_once():
 # ---------------------------------------------------------------------------
 # refusals
 # ---------------------------------------------------------------------------
+@pytest.mark.parametrize("kw", [dict(window=2 ** 31), dict(window=2 ** 32 + 5), dict(sinks=2 ** 32), dict(sinks=-2 ** 32), dict(window=-1)])
+def test_window_past_32_bits(kw):
+    c = paged_case([20], 4, 2, 64, 8, BF)
+    with pytest.raises(ValueError):
+        ops.attention_paged(c["q"], c["kc"], c["vc"], c["table"], c["lens"], c["out"], **kw)
+    q, k, o, l = normal(4, 4, 64, dtype=BF), normal(4, 2, 64, dtype=BF), normal(4, 4, 64, dtype=BF), torch.empty(4, 4, device="cuda")
+    with pytest.raises(ValueError):
+        ops.attention_window(q, k, k, o, **kw)
+    with pytest.raises(ValueError):
+        ops.attention_window_bwd(q, k, k, o, l, o, q, k, k, **kw)
+
+
 def test_python_refusals():
     c = paged_case([20], 4, 2, 64, 8, BF)
     q, kc, vc, t, n, out = c["q"], c["kc"], c["vc"], c["table"], c["lens"], c["out"]
