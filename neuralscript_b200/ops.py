@@ -622,6 +622,12 @@ def attention_paged_workspace(B, Hq, Hkv, dh) -> int:
     return L().nsb_op_attention_paged_workspace_bytes(B, Hq, Hkv, dh)
 
 
+@functools.lru_cache(maxsize=256)
+def _paged_bytes(d, B, Hq, Hkv, dh):
+    """The same on device d (d: its multiprocessors count), without a call into the library a token."""
+    return attention_paged_workspace(B, Hq, Hkv, dh)
+
+
 def attention_paged(q, k_cache, v_cache, table, lens, out, lse=None, window=0, sinks=0, scale=None, workspace=None):
     """out [B, Hq, dh] (and lse [B, Hq]) <- attention of one token a sequence, q [B, Hq, dh], over the first lens[b] keys
     of caches [pages, page, Hkv, dh] by table [B, width]: with window the last `window` of them and the first `sinks`.
@@ -633,16 +639,19 @@ def attention_paged(q, k_cache, v_cache, table, lens, out, lse=None, window=0, s
     B, Hq, dh = q.shape
     pages, page, Hkv, _ = k_cache.shape
     width = table.shape[1]
-    need = lib.nsb_op_attention_paged_workspace_bytes(B, Hq, Hkv, dh)
     if workspace is None:
-        workspace = _workspace(need, d)
-    have = workspace.numel()
+        have = _paged_bytes(d, B, Hq, Hkv, dh)
+        workspace = _workspace(have, d)
+        room = workspace.data_ptr()
+    else:
+        have = workspace.numel()
+        room = _dense(d, workspace, "workspace", _u8, (have,))
     rc = lib.nsb_op_attention_paged(
         *_heads(d, q, "q", dt, B, Hq, dh), kind, B, Hq, Hkv, dh, *_pages(d, k_cache, "k_cache", dt, pages, page, Hkv, dh),
         *_pages(d, v_cache, "v_cache", dt, pages, page, Hkv, dh), pages, page, *_rows(d, table, "table", _i32, B, width), width,
         _dense(d, lens, "lens", _i32, (B,)), *_reach(window, sinks), dh ** -0.5 if scale is None else scale,
         *_heads(d, out, "out", dt, B, Hq, dh), None if lse is None else _dense(d, lse, "lse", _f32, (B, Hq)),
-        _dense(d, workspace, "workspace", _u8, (have,)), have, _stream_of(d))
+        room, have, _stream_of(d))
     if rc:
         _check(rc, "nsb_op_attention_paged")
 
