@@ -14,6 +14,12 @@
 // keeps queries and walks the keys (dq; it computes D on the way), one that
 // keeps keys and walks the queries of all heads that share them (dk, dv), so
 // that no sum needs an atomic addition.
+//
+// Bound by shared memory: 4 x 4 scores a thread take eight 16-byte reads for 64
+// FMAs, and 2 x 4 scores on 512 threads were slower (117 to 135 us below). fp32,
+// 4096 rows of 8 heads of 64 columns, causal, forward and backward: 3.3 ms, 18
+// TFLOP/s (of some 74); 700 rows in 6 sequences, window 100: 26 + 34 + 52 us, of
+// which some 39 pass in loading the first tiles and starting.
 #include <cuda_bf16.h>
 #include <math.h>
 
@@ -30,7 +36,8 @@ namespace nsb {
 namespace {
 
 constexpr int kB = 64;          // rows of a tile
-constexpr int kThreads = 256;   // 16 x 16, 4 x 4 scores each
+constexpr int kGroup = 256;     // threads of a product: 16 x 16, 4 x 4 scores each
+constexpr int kTwoGroups = 2 * kGroup;
 constexpr int kLdS = kB + 4;    // leading dimension of a tile of scores
 
 __device__ __forceinline__ float ldf(const float* p) { return *p; }
@@ -47,12 +54,12 @@ constexpr int ld_of() {
 // rows on 16-byte boundaries are copied without passing through registers
 // (`land` waits for them), so that a tile's copies run beside the arithmetic of
 // the one before: 2 buffers, as far as shared memory reaches.
-template <typename T, int DHP>
+template <typename T, int DHP, int THREADS>
 __device__ __forceinline__ void load_tile(float* s, const Heads& x, long long row0, int first, int end, int head, int dh) {
     const T* p = (const T*)x.p + head * x.head;
     if constexpr (std::is_same<T, float>::value) {
         if (((reinterpret_cast<uintptr_t>(x.p) >> 2 | x.row | x.head | dh) & 3) == 0) {
-            for (int e = threadIdx.x; e < kB * (DHP / 4); e += kThreads) {
+            for (int e = threadIdx.x; e < kB * (DHP / 4); e += THREADS) {
                 const int r = e / (DHP / 4), c = e % (DHP / 4) * 4;
                 const bool on = first + r < end && c < dh;
                 ptx::cp_async16(s + r * ld_of<DHP>() + c, on ? p + (row0 + first + r) * x.row + c : (const float*)x.p, on ? 16 : 0);
@@ -60,7 +67,7 @@ __device__ __forceinline__ void load_tile(float* s, const Heads& x, long long ro
             return;
         }
     }
-    for (int e = threadIdx.x; e < kB * DHP; e += kThreads) {
+    for (int e = threadIdx.x; e < kB * DHP; e += THREADS) {
         const int r = e / DHP, c = e % DHP;
         s[r * ld_of<DHP>() + c] = first + r < end && c < dh ? ldf(p + (row0 + first + r) * x.row + c) : 0.f;
     }
@@ -180,7 +187,7 @@ __device__ __forceinline__ float row_max(float v) {
 
 // grid (tiles, Hq)
 template <typename T, int DHP>
-__global__ void __launch_bounds__(kThreads) window_fwd_kernel(const __grid_constant__ WindowDesc d) {
+__global__ void __launch_bounds__(kGroup) window_fwd_kernel(const __grid_constant__ WindowDesc d) {
     extern __shared__ float sm[];
     constexpr int TILE = kB * ld_of<DHP>(), BUFS = buffers<DHP>(3, 1);
     float *sQ = sm, *sP = sQ + TILE, *ring = sP + kB * kLdS;  // keys and values of each buffer
@@ -188,15 +195,15 @@ __global__ void __launch_bounds__(kThreads) window_fwd_kernel(const __grid_const
     const Rows w = find_rows(d, gridDim.x - 1 - blockIdx.x, kB);
     if (w.n <= 0) return;
     const int h = blockIdx.y, hk = h / (d.Hq / d.Hkv), q0 = w.first;
-    load_tile<T, DHP>(sQ, d.q, w.row0, q0, w.n, h, d.dh);
+    load_tile<T, DHP, kGroup>(sQ, d.q, w.row0, q0, w.n, h, d.dh);
     float o[4][DHP / 16] = {}, m[4], l[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) m[i] = -INFINITY, l[i] = 0.f;
     const KeyTiles kt(d, q0, min(q0 + kB, w.n), kB);
     auto fetch = [&](int x) {
         float* to = ring + x % BUFS * 2 * TILE;
-        load_tile<T, DHP>(to, d.k, w.row0, kt.at(x) * kB, w.n, hk, d.dh);
-        load_tile<T, DHP>(to + TILE, d.v, w.row0, kt.at(x) * kB, w.n, hk, d.dh);
+        load_tile<T, DHP, kGroup>(to, d.k, w.row0, kt.at(x) * kB, w.n, hk, d.dh);
+        load_tile<T, DHP, kGroup>(to + TILE, d.v, w.row0, kt.at(x) * kB, w.n, hk, d.dh);
     };
     if (BUFS == 2) fetch(0);
     for (int x = 0; x < kt.count; x++) {
@@ -247,7 +254,7 @@ __global__ void __launch_bounds__(kThreads) window_fwd_kernel(const __grid_const
 
 // dq and D of 64 queries: grid (tiles, Hq)
 template <typename T, int DHP>
-__global__ void __launch_bounds__(kThreads) window_bwd_q_kernel(const __grid_constant__ WindowDesc d) {
+__global__ void __launch_bounds__(kGroup) window_bwd_q_kernel(const __grid_constant__ WindowDesc d) {
     extern __shared__ float sm[];
     constexpr int TILE = kB * ld_of<DHP>(), BUFS = buffers<DHP>(4, 1);
     float *sQ = sm, *sG = sQ + TILE, *sS = sG + TILE, *ring = sS + kB * kLdS;
@@ -255,9 +262,9 @@ __global__ void __launch_bounds__(kThreads) window_bwd_q_kernel(const __grid_con
     const Rows w = find_rows(d, gridDim.x - 1 - blockIdx.x, kB);
     if (w.n <= 0) return;
     const int h = blockIdx.y, hk = h / (d.Hq / d.Hkv), q0 = w.first;
-    load_tile<T, DHP>(sQ, d.q, w.row0, q0, w.n, h, d.dh);
-    load_tile<T, DHP>(sG, d.dout, w.row0, q0, w.n, h, d.dh);
-    load_tile<T, DHP>(ring, d.out, w.row0, q0, w.n, h, d.dh);
+    load_tile<T, DHP, kGroup>(sQ, d.q, w.row0, q0, w.n, h, d.dh);
+    load_tile<T, DHP, kGroup>(sG, d.dout, w.row0, q0, w.n, h, d.dh);
+    load_tile<T, DHP, kGroup>(ring, d.out, w.row0, q0, w.n, h, d.dh);
     land();
     float o[4][DHP / 16] = {}, lse[4], D[4];
 #pragma unroll
@@ -274,8 +281,8 @@ __global__ void __launch_bounds__(kThreads) window_bwd_q_kernel(const __grid_con
     const KeyTiles kt(d, q0, min(q0 + kB, w.n), kB);
     auto fetch = [&](int x) {
         float* to = ring + x % BUFS * 2 * TILE;
-        load_tile<T, DHP>(to, d.k, w.row0, kt.at(x) * kB, w.n, hk, d.dh);
-        load_tile<T, DHP>(to + TILE, d.v, w.row0, kt.at(x) * kB, w.n, hk, d.dh);
+        load_tile<T, DHP, kGroup>(to, d.k, w.row0, kt.at(x) * kB, w.n, hk, d.dh);
+        load_tile<T, DHP, kGroup>(to + TILE, d.v, w.row0, kt.at(x) * kB, w.n, hk, d.dh);
     };
     if (BUFS == 2) {
         __syncthreads();  // the outputs have been read
@@ -307,25 +314,29 @@ __global__ void __launch_bounds__(kThreads) window_bwd_q_kernel(const __grid_con
     store_tile<T, DHP>(o, mul, d.dq, w.row0, q0, w.n, h, d.dh, ty, tx);
 }
 
-// dk and dv of 64 keys: grid (tiles, Hkv)
+// dk and dv of 64 keys: grid (tiles, Hkv). The block has two groups of 256
+// threads: the first forms scores and weights, the second dP beside it and dS
+// from both, then the first adds to dv and the second to dk. (One group that did
+// all four left the SM with eight warps: 700 rows 58 us in place of 52. The
+// queries' gradient has three products and gains nothing: 35 us for 34.)
 template <typename T, int DHP>
-__global__ void __launch_bounds__(kThreads) window_bwd_kv_kernel(const __grid_constant__ WindowDesc d) {
+__global__ void __launch_bounds__(kTwoGroups) window_bwd_kv_kernel(const __grid_constant__ WindowDesc d) {
     extern __shared__ float sm[];
     constexpr int TILE = kB * ld_of<DHP>(), BUFS = buffers<DHP>(4, 2);
     float *sK = sm, *sV = sK + TILE, *sP = sV + TILE, *sS = sP + kB * kLdS, *ring = sS + kB * kLdS;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int half = threadIdx.x / kGroup, tx = threadIdx.x & 15, ty = threadIdx.x >> 4 & 15;
     const Rows w = find_rows(d, blockIdx.x, kB);
     if (w.n <= 0) return;
     const int hk = blockIdx.y, group = d.Hq / d.Hkv, k0 = w.first;
-    load_tile<T, DHP>(sK, d.k, w.row0, k0, w.n, hk, d.dh);
-    load_tile<T, DHP>(sV, d.v, w.row0, k0, w.n, hk, d.dh);
-    float dk[4][DHP / 16] = {}, dv[4][DHP / 16] = {};
+    load_tile<T, DHP, kTwoGroups>(sK, d.k, w.row0, k0, w.n, hk, d.dh);
+    load_tile<T, DHP, kTwoGroups>(sV, d.v, w.row0, k0, w.n, hk, d.dh);
+    float o[4][DHP / 16] = {};
     const int first = k0 / kB, each = query_tiles_end(d, k0, w.n, kB) - first, count = each * group;
     auto fetch = [&](int x) {
         float* to = ring + x % BUFS * 2 * TILE;
         const int h = hk * group + x / each, q0 = (first + x % each) * kB;
-        load_tile<T, DHP>(to, d.q, w.row0, q0, w.n, h, d.dh);
-        load_tile<T, DHP>(to + TILE, d.dout, w.row0, q0, w.n, h, d.dh);
+        load_tile<T, DHP, kTwoGroups>(to, d.q, w.row0, q0, w.n, h, d.dh);
+        load_tile<T, DHP, kTwoGroups>(to + TILE, d.dout, w.row0, q0, w.n, h, d.dh);
     };
     if (BUFS == 2) fetch(0);
     for (int x = 0; x < count; x++) {
@@ -335,31 +346,42 @@ __global__ void __launch_bounds__(kThreads) window_bwd_kv_kernel(const __grid_co
             __syncthreads();
             fetch(x);
         }
-        land();
-        if (BUFS == 2 && x + 1 < count) fetch(x + 1);
-        float s[4][4], g[4][4];
-        dot_tile<DHP>(s, sQ, sK, ty, tx);
-        dot_tile<DHP>(g, sG, sV, ty, tx);
+        float stat[4];  // lse in the first group, D in the second
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int r = q0 + ty * 4 + i;
-            const float lse = r < w.n ? d.lse[h * d.ld_lse + w.row0 + r] : -INFINITY;
-            const float D = r < w.n ? d.dvec[(long long)h * d.T + w.row0 + r] : 0.f;
+            stat[i] = half == 0 ? -INFINITY : 0.f;
+            if (r < w.n) stat[i] = half == 0 ? d.lse[h * d.ld_lse + w.row0 + r] : d.dvec[(long long)h * d.T + w.row0 + r];
+        }
+        land();
+        if (BUFS == 2 && x + 1 < count) fetch(x + 1);
+        float s[4][4];
+        dot_tile<DHP>(s, half ? sG : sQ, half ? sV : sK, ty, tx);
+        const int at = ty * 4 * kLdS + tx;
+        if (half == 0) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const bool on = lse != -INFINITY && sees(d, r, k0 + tx + 16 * j);
-                const float p = on ? expf(s[i][j] * d.scale - lse) : 0.f;
-                sP[(ty * 4 + i) * kLdS + tx + 16 * j] = p;
-                sS[(ty * 4 + i) * kLdS + tx + 16 * j] = on ? p * (g[i][j] - D) : 0.f;
-            }
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const bool on = stat[i] != -INFINITY && sees(d, q0 + ty * 4 + i, k0 + tx + 16 * j);
+                    sP[at + i * kLdS + 16 * j] = on ? expf(s[i][j] * d.scale - stat[i]) : 0.f;
+                }
         }
         __syncthreads();
-        add_cols<DHP>(dv, sP, sG, ty, tx);
-        add_cols<DHP>(dk, sS, sQ, ty, tx);
+        if (half == 1) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float p = sP[at + i * kLdS + 16 * j];  // 0 where the key is hidden, whatever its dP is
+                    sS[at + i * kLdS + 16 * j] = p == 0.f ? 0.f : p * (s[i][j] - stat[i]);
+                }
+            asm volatile("bar.sync 1, %0;" ::"n"(kGroup) : "memory");  // its group's dS
+        }
+        add_cols<DHP>(o, half ? sS : sP, half ? sQ : sG, ty, tx);
     }
-    const float one[4] = {1.f, 1.f, 1.f, 1.f}, mul[4] = {d.scale, d.scale, d.scale, d.scale};
-    store_tile<T, DHP>(dv, one, d.dv, w.row0, k0, w.n, hk, d.dh, ty, tx);
-    store_tile<T, DHP>(dk, mul, d.dk, w.row0, k0, w.n, hk, d.dh, ty, tx);
+    const float m = half ? d.scale : 1.f, mul[4] = {m, m, m, m};
+    store_tile<T, DHP>(o, mul, half ? d.dk : d.dv, w.row0, k0, w.n, hk, d.dh, ty, tx);
 }
 
 namespace {
@@ -405,7 +427,7 @@ int attention_window(const WindowDesc& d, cudaStream_t st) {
         constexpr int DHP = decltype(wide)::value, bytes = smem_of<DHP>(3, 1);
         static size_t most[kMaxDevices];
         if (!allow_shared(window_fwd_kernel<T, DHP>, bytes, most)) return -5;
-        window_fwd_kernel<T, DHP><<<dim3((unsigned)tiles_of(d, kB), d.Hq), kThreads, bytes, st>>>(d);
+        window_fwd_kernel<T, DHP><<<dim3((unsigned)tiles_of(d, kB), d.Hq), kGroup, bytes, st>>>(d);
         return cudaGetLastError() == cudaSuccess ? 0 : -5;
     });
 }
@@ -438,8 +460,8 @@ int attention_window_bwd(const WindowDesc& given, cudaStream_t st) {
         static size_t most_q[kMaxDevices], most_kv[kMaxDevices];
         if (!allow_shared(window_bwd_q_kernel<T, DHP>, bq, most_q) || !allow_shared(window_bwd_kv_kernel<T, DHP>, bk, most_kv))
             return -5;
-        window_bwd_q_kernel<T, DHP><<<dim3((unsigned)tiles_of(d, kB), d.Hq), kThreads, bq, st>>>(d);
-        window_bwd_kv_kernel<T, DHP><<<dim3((unsigned)tiles_of(d, kB), d.Hkv), kThreads, bk, st>>>(d);
+        window_bwd_q_kernel<T, DHP><<<dim3((unsigned)tiles_of(d, kB), d.Hq), kGroup, bq, st>>>(d);
+        window_bwd_kv_kernel<T, DHP><<<dim3((unsigned)tiles_of(d, kB), d.Hkv), kTwoGroups, bk, st>>>(d);
         return cudaGetLastError() == cudaSuccess ? 0 : -5;
     });
 }
