@@ -15,6 +15,12 @@
 // two halves of its pairs. kv_append is the same kernel with three tensors at
 // once (queries, keys, values), whose keys and values go to the cache's
 // places.
+//
+// Bound by HBM, with the issue slots close behind (64 %): 16384 rows of 20 heads
+// of 128 columns in bf16, 29.8 us a pass, 5.6 TB/s (a measured copy: 6.5); 9001 x
+// 12 x 80 in fp32, 14.4 us, 4.8 TB/s. Appending 32 tokens: 3.1 us, a launch; 8000
+// tokens of 8 heads of 64: 8.1 us, 4.1 TB/s, latency of one block's chain (place
+// of the token, angles, heads) in three rounds of blocks.
 #include <cuda_bf16.h>
 
 #include <type_traits>
@@ -108,7 +114,8 @@ __device__ __forceinline__ void turn_pairs(float* x0, float* x1, const float2* w
 // of two neighbouring pairs lie together, those of all pieces' first two pairs
 // before those of the next two: neighbouring threads read neighbouring 16
 // bytes (pair by pair they met each bank four times, which bound the kernel:
-// 34 us a pass over 16384 x 20 x 128 in place of 31). ONE: there is one job.
+// 34 us a pass over 16384 x 20 x 128 in place of 31). ONE: there is one job
+// (known when compiled, with divisions by multiplication: 31 to 30 us).
 template <typename T, int P, bool SIDE, bool ONE>
 __global__ void __launch_bounds__(kTurnThreads) turn_kernel(const __grid_constant__ TurnArgs a) {
     using V = typename Piece<P * sizeof(T)>::type;
