@@ -18,9 +18,9 @@
 //
 // Bound by HBM while it streams; the sum of lengths before it takes some 5 us,
 // the join behind it 2 to 9. 64 sequences of up to 4096 keys, 24 heads on 4 of
-// 128 columns, bf16: 45.8 us, 4.6 TB/s; two of 120000, 16 heads on 2: 43.9 us,
-// 4.6 TB/s; fp32, 96 behind a window of 1024, 8 heads of 64: 62.5 us, 5.7 TB/s;
-// one sequence of 900 keys, 8 heads of 64: 9.9 us, all of it latency.
+// 128 columns, bf16: 45.8 us, 4.6 TB/s; two of 120000, 16 heads on 2: 42.4 us,
+// 4.8 TB/s; fp32, 96 behind a window of 1024, 8 heads of 64: 62.5 us, 5.7 TB/s;
+// one sequence of 900 keys, 8 heads of 64: 9.7 us, all of it latency.
 #include <cuda_bf16.h>
 #include <math.h>
 
@@ -809,7 +809,11 @@ __global__ void __launch_bounds__(kThreads, Ring<T, DHP, HB>::PER_SM) paged_ring
 // (where the blocks meet, `together`), else its warps'. 256 parts at a time:
 // a thread each for maxima and sums, which gives every part its weight, then
 // eight warps add up every eighth part's values, whose loads wait for nothing.
-template <typename T, int DHP, int HB>
+// AHEAD: the first values are loaded while the weights are formed. That takes 76
+// registers for 44, so it is for grids that leave SMs room anyway (two sequences
+// of 120000 keys, 32 blocks: 44.2 to 42.4 us; 64 sequences, 1536 blocks: 46.2 to
+// 48.1).
+template <typename T, int DHP, int HB, bool AHEAD>
 __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedArgs a, bool merges) {
     constexpr int C = DHP / 32;
     __shared__ float s_top[8], s_sum[8], s_w[256], s_o[8][DHP];
@@ -851,6 +855,21 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
                 lc = a.part[(long long)at * (HB * (DHP + 2)) + HB + g];
             }
         }
+        s_at[t] = at;
+        const float* values = a.part + 2 * HB + g * DHP + lane;
+        float v[8][C];
+        auto load = [&](int y0) {  // eight parts' at once
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const int from = y0 + 8 * u < 256 ? s_at[y0 + 8 * u] : -1;
+#pragma unroll
+                for (int j = 0; j < C; j++) v[u][j] = from >= 0 ? values[(long long)from * (HB * (DHP + 2)) + 32 * j] : 0.f;
+            }
+        };
+        if (AHEAD) {
+            __syncthreads();
+            load(warp);
+        }
         float top = mc;
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
@@ -861,7 +880,6 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
         for (int w = 0; w < 8; w++) top = fmaxf(top, s_top[w]);
         const float safe = top == -INFINITY ? 0.f : top, turn = exp2f(m - safe), share = exp2f(mc - safe);
         s_w[t] = share;
-        s_at[t] = at;
         float sum = lc * share;
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
@@ -873,15 +891,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
         for (int w = 0; w < 8; w++) l += s_sum[w];
 #pragma unroll
         for (int j = 0; j < C; j++) o[j] *= turn;
-        const float* values = a.part + 2 * HB + g * DHP + lane;
-        for (int y0 = warp; y0 < min(256, n - x0); y0 += 64) {  // eight parts' loads at once
-            float v[8][C];
-#pragma unroll
-            for (int u = 0; u < 8; u++) {
-                const int from = y0 + 8 * u < 256 ? s_at[y0 + 8 * u] : -1;
-#pragma unroll
-                for (int j = 0; j < C; j++) v[u][j] = from >= 0 ? values[(long long)from * (HB * (DHP + 2)) + 32 * j] : 0.f;
-            }
+        for (int y0 = warp; y0 < min(256, n - x0); y0 += 64) {
+            if (!AHEAD || y0 != warp) load(y0);
 #pragma unroll
             for (int u = 0; u < 8; u++)
 #pragma unroll
@@ -983,7 +994,11 @@ int attention_paged(const PagedDesc& d, cudaStream_t st) {
         at.val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = &at;
         cfg.numAttrs = 1;
-        return cudaLaunchKernelEx(&cfg, paged_join_kernel<T, DHP, HB>, a, (bool)decltype(aligned)::value) == cudaSuccess ? 0 : -5;
+        const bool few = (long long)cfg.gridDim.x * cfg.gridDim.y <= 2 * num_sms();
+        return cudaLaunchKernelEx(&cfg, few ? paged_join_kernel<T, DHP, HB, true> : paged_join_kernel<T, DHP, HB, false>, a,
+                                  (bool)decltype(aligned)::value) == cudaSuccess
+                   ? 0
+                   : -5;
     };
     using std::integral_constant;
     auto by_heads = [&](auto zero, auto wide) {
