@@ -404,6 +404,18 @@ int nsb_op_attention_window_bwd(const void* q, long long q_row, long long q_head
                                 long long dv_row, long long dv_head, void* workspace, size_t workspace_bytes,
                                 void* stream);
 
+/* The calls from nsb_op_rope on with their arguments in one block, in order
+ * and each aligned as in a struct (`bytes` up to the end of the last), for
+ * bindings that pay by the argument. -1 where `which` or `bytes` does not
+ * fit. */
+#define NSB_CALL_ROPE 0
+#define NSB_CALL_ROPE_BWD 1
+#define NSB_CALL_KV_APPEND 2
+#define NSB_CALL_ATTENTION_PAGED 3
+#define NSB_CALL_ATTENTION_WINDOW 4
+#define NSB_CALL_ATTENTION_WINDOW_BWD 5
+int nsb_op_from_block(int which, const void* args, size_t bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -2,6 +2,9 @@
 // the launchers in gemm.cu, kernels.cu and attention.cu.
 #include <cuda_bf16.h>
 #include <math.h>
+#include <string.h>
+
+#include <tuple>
 
 #include "../../include/ns_b200_ops.h"
 #include "attention.h"
@@ -15,6 +18,21 @@
 #include "moe_topk.h"
 
 using namespace nsb;
+
+// A call of f with its arguments read from a block in which they stand in
+// order, each on a multiple of its size.
+template <typename... A>
+static int from_block(int (*f)(A...), const void* block, size_t bytes) {
+    std::tuple<A...> args{};
+    size_t at = 0;
+    auto next = [&](auto& to) {
+        at = (at + sizeof(to) - 1) / sizeof(to) * sizeof(to);
+        if (at + sizeof(to) <= bytes) memcpy(&to, static_cast<const char*>(block) + at, sizeof(to));
+        at += sizeof(to);
+    };
+    std::apply([&](auto&... to) { (next(to), ...); }, args);
+    return at == bytes ? std::apply(f, args) : -1;
+}
 
 static GemmDesc make_desc(int M, int N, int K, const void* A, int a_dtype, long long lda, int a_mn, const void* B,
                           int b_dtype, long long ldb, int b_mn, int engine) {
@@ -707,6 +725,19 @@ int nsb_op_attention_window_bwd(const void* q, long long q_row, long long q_head
     d.workspace_bytes = workspace_bytes;
     launch_counter() += attention_window_bwd_launches(d);
     return attention_window_bwd(d, (cudaStream_t)stream);
+}
+
+int nsb_op_from_block(int which, const void* args, size_t bytes) {
+    if (!args) return -1;
+    switch (which) {
+        case NSB_CALL_ROPE: return from_block(nsb_op_rope, args, bytes);
+        case NSB_CALL_ROPE_BWD: return from_block(nsb_op_rope_bwd, args, bytes);
+        case NSB_CALL_KV_APPEND: return from_block(nsb_op_kv_append, args, bytes);
+        case NSB_CALL_ATTENTION_PAGED: return from_block(nsb_op_attention_paged, args, bytes);
+        case NSB_CALL_ATTENTION_WINDOW: return from_block(nsb_op_attention_window, args, bytes);
+        case NSB_CALL_ATTENTION_WINDOW_BWD: return from_block(nsb_op_attention_window_bwd, args, bytes);
+    }
+    return -1;
 }
 
 }  // extern "C"

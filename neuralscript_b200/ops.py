@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import struct
 
 from . import lib as _core_lib
 
@@ -95,7 +96,14 @@ _sigs = {
     "nsb_op_attention_window_bwd": (C.c_int, _window_args + _heads_args + [C.c_void_p, C.c_longlong] + _heads_args * 4
                                     + [C.c_void_p, C.c_size_t, C.c_void_p]),
     "nsb_op_attention_window_bwd_workspace_bytes": (C.c_size_t, [C.c_int] * 5),
+    "nsb_op_from_block": (C.c_int, [C.c_int, C.c_char_p, C.c_size_t]),
 }
+_letters = {C.c_void_p: "P", C.POINTER(C.c_int): "P", C.c_int: "i", C.c_longlong: "q", C.c_float: "f", C.c_size_t: "N"}
+# entries that _call takes, in the order of the header's numbers, and what packs their arguments
+_BLOCKS = ("nsb_op_rope", "nsb_op_rope_bwd", "nsb_op_kv_append", "nsb_op_attention_paged", "nsb_op_attention_window",
+           "nsb_op_attention_window_bwd")
+_ROPE, _ROPE_BWD, _APPEND, _PAGED, _WINDOW, _WINDOW_BWD = range(6)
+_packs = [struct.Struct("".join(_letters[t] for t in _sigs[n][1])).pack for n in _BLOCKS]
 _bound = None
 
 
@@ -109,6 +117,14 @@ def L():
             f.argtypes = args
         _bound = lib
     return _bound
+
+
+def _call(lib, which, *args):
+    """An entry with its arguments in one block: ctypes takes 0.1 us for each of up to 60. Addresses are ints, 0: none."""
+    block = _packs[which](*args)
+    rc = lib.nsb_op_from_block(which, block, len(block))
+    if rc:
+        _check(rc, _BLOCKS[which])
 
 
 def p(t):
@@ -531,10 +547,10 @@ class _Devices(dict):
 
 
 _cuda = _Devices()
-_NO_TURN = (None, 0, 0, None, None, 0, 0, 1.0)
+_NO_TURN = (0, 0, 0, 0, 0, 0, 0, 1.0)
 
 
-@functools.lru_cache(maxsize=64)
+@functools.lru_cache(maxsize=None)  # (kept: entries are given the address)
 def _sections(sections, axes, pairs):
     """Pairs of each axis as the entries take them."""
     if len(sections) != axes or sum(sections) != pairs or min(sections) < 0:
@@ -550,34 +566,33 @@ def _turn(d, pos, freq, T, sections, interleaved, scale):
     pairs = freq.shape[0]
     at, ld = _rows(d, pos, "pos", _i32, axes, T)
     if sections is not None:
-        sections = _sections(tuple(sections), axes, pairs)
+        sections = C.addressof(_sections(tuple(sections), axes, pairs))
     elif axes != 1:
         raise ValueError(f"pos has {axes} axes: sections say how many pairs belong to each")
+    else:
+        sections = 0
     return at, ld, axes, sections, _dense(d, freq, "freq", _f32, (pairs,)), pairs, interleaved, scale
 
 
-def _rope(entry, x, pos, freq, y, sections, interleaved, scale):
+def _rope(which, x, pos, freq, y, sections, interleaved, scale):
+    lib = _bound if _f32 else _torch()
     d = _device()
     dt = x.dtype
     T, H, dh = x.shape
     at, row, head = _heads(d, x, "x", dt, T, H, dh)
-    rc = entry(at, _kind(x, "x"), row, head, T, H, dh, *_turn(d, pos, freq, T, sections, interleaved, scale),
-               *_heads(d, y, "y", dt, T, H, dh), _stream_of(d))
-    if rc:
-        _check(rc, entry.__name__)
+    _call(lib, which, at, _kind(x, "x"), row, head, T, H, dh, *_turn(d, pos, freq, T, sections, interleaved, scale),
+          *_heads(d, y, "y", dt, T, H, dh), _stream_of(d))
 
 
 def rope(x, pos, freq, y, sections=None, interleaved=False, scale=1.0):
     """y [T, H, dh] <- x with the pairs of its heads turned by pos * freq: pos [T] or [axes, T] (int32), freq [pairs]
     (float32), a pair (i, i + pairs), or (2 i, 2 i + 1) where interleaved; sections: pairs of each axis. y may be x."""
-    lib = _bound if _f32 else _torch()
-    _rope(lib.nsb_op_rope, x, pos, freq, y, sections, interleaved, scale)
+    _rope(_ROPE, x, pos, freq, y, sections, interleaved, scale)
 
 
 def rope_bwd(dy, pos, freq, dx, sections=None, interleaved=False, scale=1.0):
     """dx [T, H, dh] <- the gradient of rope's x. dx may be dy."""
-    lib = _bound if _f32 else _torch()
-    _rope(lib.nsb_op_rope_bwd, dy, pos, freq, dx, sections, interleaved, scale)
+    _rope(_ROPE_BWD, dy, pos, freq, dx, sections, interleaved, scale)
 
 
 def _pages(d, t, what, dtype, pages, page, heads, dh):
@@ -605,16 +620,14 @@ def kv_append(k, v, seq, at, table, k_cache, v_cache, pos=None, freq=None, secti
     if (q is None) != (q_out is None) or (pos is None) != (freq is None):
         raise ValueError("q goes with q_out, and pos with freq")
     Hq = 0 if q is None else q.shape[1]
-    rc = lib.nsb_op_kv_append(
-        *_heads(d, k, "k", dt, T, Hkv, dh), *_heads(d, v, "v", dt, T, Hkv, dh), kind, T, Hkv, dh,
+    _call(
+        lib, _APPEND, *_heads(d, k, "k", dt, T, Hkv, dh), *_heads(d, v, "v", dt, T, Hkv, dh), kind, T, Hkv, dh,
         _dense(d, seq, "seq", _i32, (T,)), _dense(d, at, "at", _i32, (T,)), *_rows(d, table, "table", _i32, B, width), B, width,
         pages, page, *_pages(d, k_cache, "k_cache", dt, pages, page, Hkv, dh),
         *_pages(d, v_cache, "v_cache", dt, pages, page, Hkv, dh),
         *(_NO_TURN if freq is None else _turn(d, pos, freq, T, sections, interleaved, scale)),
-        *((None, 0, 0) if q is None else _heads(d, q, "q", dt, T, Hq, dh)), Hq,
-        *((None, 0, 0) if q is None else _heads(d, q_out, "q_out", dt, T, Hq, dh)), _stream_of(d))
-    if rc:
-        _check(rc, "nsb_op_kv_append")
+        *((0, 0, 0) if q is None else _heads(d, q, "q", dt, T, Hq, dh)), Hq,
+        *((0, 0, 0) if q is None else _heads(d, q_out, "q_out", dt, T, Hq, dh)), _stream_of(d))
 
 
 def attention_paged_workspace(B, Hq, Hkv, dh) -> int:
@@ -646,14 +659,12 @@ def attention_paged(q, k_cache, v_cache, table, lens, out, lse=None, window=0, s
     else:
         have = workspace.numel()
         room = _dense(d, workspace, "workspace", _u8, (have,))
-    rc = lib.nsb_op_attention_paged(
-        *_heads(d, q, "q", dt, B, Hq, dh), kind, B, Hq, Hkv, dh, *_pages(d, k_cache, "k_cache", dt, pages, page, Hkv, dh),
+    _call(
+        lib, _PAGED, *_heads(d, q, "q", dt, B, Hq, dh), kind, B, Hq, Hkv, dh, *_pages(d, k_cache, "k_cache", dt, pages, page, Hkv, dh),
         *_pages(d, v_cache, "v_cache", dt, pages, page, Hkv, dh), pages, page, *_rows(d, table, "table", _i32, B, width), width,
         _dense(d, lens, "lens", _i32, (B,)), *_reach(window, sinks), dh ** -0.5 if scale is None else scale,
-        *_heads(d, out, "out", dt, B, Hq, dh), None if lse is None else _dense(d, lse, "lse", _f32, (B, Hq)),
+        *_heads(d, out, "out", dt, B, Hq, dh), 0 if lse is None else _dense(d, lse, "lse", _f32, (B, Hq)),
         room, have, _stream_of(d))
-    if rc:
-        _check(rc, "nsb_op_attention_paged")
 
 
 def _reach(window, sinks):
@@ -670,7 +681,7 @@ def _packed(d, q, k, v, offsets, window, sinks, scale):
     Hkv = k.shape[1]
     B = 1 if offsets is None else offsets.shape[0] - 1
     return (*_heads(d, q, "q", dt, T, Hq, dh), *_heads(d, k, "k", dt, T, Hkv, dh), *_heads(d, v, "v", dt, T, Hkv, dh), kind,
-            T, Hq, Hkv, dh, None if offsets is None else _dense(d, offsets, "offsets", _i32, (B + 1,)), B,
+            T, Hq, Hkv, dh, 0 if offsets is None else _dense(d, offsets, "offsets", _i32, (B + 1,)), B,
             *_reach(window, sinks), dh ** -0.5 if scale is None else scale)
 
 
@@ -681,11 +692,8 @@ def attention_window(q, k, v, out, lse=None, offsets=None, window=0, sinks=0, sc
     lib = _bound if _f32 else _torch()
     d = _device()
     T, Hq, dh = q.shape
-    rc = lib.nsb_op_attention_window(
-        *_packed(d, q, k, v, offsets, window, sinks, scale), *_heads(d, out, "out", q.dtype, T, Hq, dh),
-        *((None, 0) if lse is None else _rows(d, lse, "lse", _f32, Hq, T)), _stream_of(d))
-    if rc:
-        _check(rc, "nsb_op_attention_window")
+    _call(lib, _WINDOW, *_packed(d, q, k, v, offsets, window, sinks, scale), *_heads(d, out, "out", q.dtype, T, Hq, dh),
+          *((0, 0) if lse is None else _rows(d, lse, "lse", _f32, Hq, T)), _stream_of(d))
 
 
 def attention_window_bwd_workspace(T, Hq, Hkv, dh, dtype) -> int:
@@ -708,9 +716,7 @@ def attention_window_bwd(q, k, v, out, lse, dout, dq, dk, dv, offsets=None, wind
         need = lib.nsb_op_attention_window_bwd_workspace_bytes(T, Hq, Hkv, dh, F32 if dt is _f32 else BF16)
         workspace = _workspace(need, d)
     have = workspace.numel()
-    rc = lib.nsb_op_attention_window_bwd(
-        *args, *_heads(d, out, "out", dt, T, Hq, dh), *_rows(d, lse, "lse", _f32, Hq, T),
+    _call(
+        lib, _WINDOW_BWD, *args, *_heads(d, out, "out", dt, T, Hq, dh), *_rows(d, lse, "lse", _f32, Hq, T),
         *_heads(d, dout, "dout", dt, T, Hq, dh), *_heads(d, dq, "dq", dt, T, Hq, dh), *_heads(d, dk, "dk", dt, T, Hkv, dh),
         *_heads(d, dv, "dv", dt, T, Hkv, dh), _dense(d, workspace, "workspace", _u8, (have,)), have, _stream_of(d))
-    if rc:
-        _check(rc, "nsb_op_attention_window_bwd")

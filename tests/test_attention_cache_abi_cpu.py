@@ -81,6 +81,21 @@ def test_paged_limits():
     assert size(2, 4, 2, 64) > 0 and size(2, 4, 2, 64) % 8 == 0
 
 
+def test_block_of_arguments():
+    """The same refusals through the call that takes its arguments in one block, and those of the block."""
+    for which, (ok, cases) in enumerate([
+            (ROPE, [(dict(dh=63), -1), (dict(H=(1 << 20) + 1), -2), (dict(T=0), 0)]), (ROPE, [(dict(axes=5), -1), (dict(T=0), 0)]),
+            (APPEND, [(dict(page=0), -1), (dict(Hkv=1 << 30), -2), (dict(T=0), 0)]), (PAGED, [(dict(scale=0.0), -1), (dict(B=8193), -2), (dict(B=0), 0)]),
+            (WINDOW, [(dict(ld_lse=3), -1), (dict(Hq=131072, Hkv=65536), -2), (dict(T=0), 0)]),
+            (GRADS, [(dict(bytes=63), -1), (dict(Hq=131072, Hkv=65536), -2), (dict(B=0), 0)])]):
+        for bad, want in cases:
+            block = ops._packs[which](*(0 if v is None else v for v in (ok | bad).values()), 0)
+            call_block = ops.L().nsb_op_from_block
+            assert call_block(which, block, len(block)) == want, (which, bad)
+            assert call_block(which, block[:-1], len(block) - 1) == call_block(which, block + b"\0", len(block) + 1) == -1
+            assert call_block(which, None, len(block)) == call_block(6, block, len(block)) == call_block(-1, block, len(block)) == -1
+
+
 WINDOW = dict(q=X, q_row=64, q_head=64, k=X, k_row=64, k_head=64, v=X, v_row=64, v_head=64, dtype=1, T=4, Hq=4, Hkv=2, dh=64, offsets=X, B=2,
               window=0, sinks=0, scale=0.125, out=X, o_row=64, o_head=64, lse=X, ld_lse=4)
 GRADS = WINDOW | dict(dout=X, do_row=64, do_head=64, dq=X, dq_row=64, dq_head=64, dk=X, dk_row=64, dk_head=64, dv=X, dv_row=64, dv_head=64, workspace=X,
