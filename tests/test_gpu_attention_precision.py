@@ -1,0 +1,67 @@
+"""What attention keeps of its weights where tensors are bf16: against the
+definitions in 64 bits (attention_ref), with tolerances that leave no room for
+weights rounded to bf16."""
+import math
+
+import pytest
+import torch
+
+from attention_ref import close, half_step
+from neuralscript_b200 import ops
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+def normal(*shape, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return torch.randn(*shape, device="cuda", generator=g)
+
+
+@pytest.mark.parametrize("Hq,Hkv,dh", [(8, 8, 64), (8, 2, 128), (32, 2, 64), (24, 1, 128)])
+def test_weights_over_the_cache(Hq, Hkv, dh):
+    """A weight takes part to 2^-16 of itself (eight digits, and the next rounded to eight: 2^-7 2^-9), the result is
+    rounded once."""
+    lens, page = [3, 17, 40, 1, 300], 16
+    need = [-(-n // page) for n in lens]
+    table = torch.zeros(len(lens), max(need), dtype=torch.int32)
+    for b, n in enumerate(need):
+        table[b, :n] = torch.arange(n) + sum(need[:b])
+    kc, vc = (normal(sum(need), page, Hkv, dh, seed=s).to(BF) for s in (1, 2))
+    q = (0.25 * normal(len(lens), Hq, dh, seed=3)).to(BF)  # flat: weights that are no power of two
+    out, scale = torch.empty_like(q), dh ** -0.5
+    ops.attention_paged(q, kc, vc, table.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"), out)
+    for b, n in enumerate(lens):
+        pages = table[b, :need[b]].cuda().long()
+        k, v = (c[pages].reshape(-1, Hkv, dh)[:n].double().repeat_interleave(Hq // Hkv, 1) for c in (kc, vc))
+        z = scale * torch.einsum("hd,jhd->hj", q[b].double(), k)
+        size = scale * torch.einsum("hd,jhd->hj", q[b].double().abs(), k.abs()).amax(1)[:, None]
+        p = torch.softmax(z, 1)
+        want = torch.einsum("hj,jhd->hd", p, v)
+        # scores and sums in fp32, twice (weights and their sum), as attention_ref counts them
+        off = 4 * ((dh + 4) * size + n) * 2.0 ** -24 + 2.0 ** -19 + 2.0 ** -16
+        tol = half_step(BF) * want.abs() + off * torch.einsum("hj,jhd->hd", p, v.abs())
+        close(out[b], want, tol, f"out {b}")
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("lens", [[9], [9, 700], [2000]])  # finished by one warp, by a block, joined
+def test_infinite_values_over_the_cache(lens, dtype):
+    """An infinite value makes its column infinite, with its sign, also where its weight is a power of two; both: NaN."""
+    page, dh = 16, 64
+    pages = [-(-n // page) for n in lens]
+    table = torch.zeros(len(lens), max(pages), dtype=torch.int32)
+    for b, n in enumerate(pages):
+        table[b, :n] = torch.arange(n) + sum(pages[:b])
+    kc, vc = (normal(sum(pages), page, 1, dh, seed=s).to(dtype) for s in (1, 2))
+    kc *= 0.1
+    for q_of in (0.0, 1.0):  # equal weights, and any
+        q = (q_of * normal(len(lens), 2, dh, seed=3)).to(dtype)
+        for b, n in enumerate(lens):
+            for j, col, to in ((0, 5, math.inf), (n - 1, 6, -math.inf), (n // 2, 7, math.inf), (n - 2, 7, -math.inf)):
+                vc[int(table[b, j // page]), j % page, 0, col] = to
+        out = torch.empty_like(q)
+        ops.attention_paged(q, kc, vc, table.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"), out)
+        assert (out[..., 5] == math.inf).all() and (out[..., 6] == -math.inf).all() and out[..., 7].isnan().all()
+        assert out[..., [c for c in range(dh) if c not in (5, 6, 7)]].isfinite().all()
