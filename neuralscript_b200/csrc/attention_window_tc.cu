@@ -67,8 +67,10 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
 }
 
 // A barrier of N threads, by whole warps: whether one of them gave up. Who leaves
-// its loop meets it once more with `gone`, and who gets true leaves without: so
-// nobody stands at a barrier that another will not reach.
+// while the others will meet once more meets it with `gone`, and who gets true
+// leaves without: so nobody stands at a barrier that another will not reach. Behind
+// the last meeting of all a warp leaves by itself (and the flag ends the others'
+// waits).
 template <int N>
 __device__ __forceinline__ bool meet(int id, bool gone) {
     int any;
@@ -112,7 +114,11 @@ __device__ __forceinline__ bool fill_slot(uint8_t* to, const CUtensorMap* map, u
         return true;
     }
     if (one) load_rows<DHP>(to, map, landed, head, row);
-    if (!wait(landed, tails++)) return false;
+    if (!wait(landed, tails)) {
+        if (one) ptx::mbar_wait(landed, tails & 1, nullptr, 0);  // no copy may land after the block has left
+        return false;
+    }
+    tails++;
     zero_rows<DHP>(to, end);
     warp_arrive(full);
     return true;
@@ -696,9 +702,10 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
             v = ((sums[r] + sums[kT + r]) + sums[2 * kT + r]) + sums[3 * kT + r];
             return ok;
         };
+        bool last = first == 0;  // whether all have met for the last time
         auto await = [&](uint64_t* bar, uint32_t phase) {
             ok = wait(bar, phase);
-            if (!ok) meet<512>(1, true);
+            if (!ok && !last) meet<512>(1, true);
             return ok;
         };
         add_up(D);
@@ -740,6 +747,7 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
                 for (int e = 0; e < 32; e++) rest += __uint_as_float(g[e]);
             ok = ok && !meet<512>(1, false);  // all have read the sums before
             if (ok && add_up(rest)) D += rest;
+            last = true;
         }
         if (part == 0 && i < w.n) d.dvec[(long long)h * d.T + w.row0 + i] = D;
 #pragma unroll 1
@@ -1027,10 +1035,10 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
                 for (int qg = 0; qg < 2; qg++) {
                     const int i = 2 * step + qg, slot = i % F::SLOTS, round = i / F::SLOTS;
                     if (round && !(ok = wait(&empty[slot], round - 1))) break;
-                    copies = i + 1;
                     if (!(ok = fill_slot<DHP>(ring + slot * F::TILE, qg ? &tg : &tq, &full[slot], landed, tails, wait, h,
                                               p.row0 + q0, p.n - q0)))
                         break;
+                    copies = i + 1;
                 }
                 if (++q == p.each) q = 0, h++;
             }
