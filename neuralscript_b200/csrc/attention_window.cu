@@ -276,27 +276,31 @@ __global__ void __launch_bounds__(kGroup) window_bwd_q_kernel(const __grid_const
             sum = fmaf(sG[(ty * 4 + i) * ld_of<DHP>() + c + tx], ring[(ty * 4 + i) * ld_of<DHP>() + c + tx], sum);
         D[i] = row_sum(sum);
         lse[i] = r < w.n ? d.lse[h * d.ld_lse + w.row0 + r] : -INFINITY;
-        if (tx == 0 && r < w.n) d.dvec[(long long)h * d.T + w.row0 + r] = D[i];
     }
     const KeyTiles kt(d, q0, min(q0 + kB, w.n), kB);
+    // steps of the pass that only sums dS, for what D is short of
+    const int first = !std::is_same<T, float>::value && few_keys(d, q0, min(q0 + kB, w.n)) ? kt.count : 0;
+    const int steps = first + kt.count;
+    float rest[4] = {};
+    auto tile_of = [&](int x) { return kt.at(x < first ? x : x - first) * kB; };
     auto fetch = [&](int x) {
         float* to = ring + x % BUFS * 2 * TILE;
-        load_tile<T, DHP, kGroup>(to, d.k, w.row0, kt.at(x) * kB, w.n, hk, d.dh);
-        load_tile<T, DHP, kGroup>(to + TILE, d.v, w.row0, kt.at(x) * kB, w.n, hk, d.dh);
+        load_tile<T, DHP, kGroup>(to, d.k, w.row0, tile_of(x), w.n, hk, d.dh);
+        load_tile<T, DHP, kGroup>(to + TILE, d.v, w.row0, tile_of(x), w.n, hk, d.dh);
     };
     if (BUFS == 2) {
         __syncthreads();  // the outputs have been read
         fetch(0);
     }
-    for (int x = 0; x < kt.count; x++) {
-        const int k0 = kt.at(x) * kB;
+    for (int x = 0; x < steps; x++) {
+        const int k0 = tile_of(x);
         const float *sK = ring + x % BUFS * 2 * TILE, *sV = sK + TILE;
         if (BUFS == 1) {
             __syncthreads();
             fetch(x);
         }
         land();
-        if (BUFS == 2 && x + 1 < kt.count) fetch(x + 1);
+        if (BUFS == 2 && x + 1 < steps) fetch(x + 1);
         float s[4][4], g[4][4];
         dot_tile<DHP>(s, sQ, sK, ty, tx);
         dot_tile<DHP>(g, sG, sV, ty, tx);
@@ -305,10 +309,24 @@ __global__ void __launch_bounds__(kGroup) window_bwd_q_kernel(const __grid_const
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const bool on = lse[i] != -INFINITY && sees(d, q0 + ty * 4 + i, k0 + tx + 16 * j);
-                sS[(ty * 4 + i) * kLdS + tx + 16 * j] = on ? expf(s[i][j] * d.scale - lse[i]) * (g[i][j] - D[i]) : 0.f;
+                s[i][j] = on ? expf(s[i][j] * d.scale - lse[i]) * (g[i][j] - D[i]) : 0.f;
+                sS[(ty * 4 + i) * kLdS + tx + 16 * j] = s[i][j];
             }
+        if (x < first) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                rest[i] += (s[i][0] + s[i][1]) + (s[i][2] + s[i][3]);
+                if (x == first - 1) D[i] += row_sum(rest[i]);
+            }
+            continue;
+        }
         __syncwarp();
         add_rows<DHP>(o, sS, sK, ty, tx);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int r = q0 + ty * 4 + i;
+        if (tx == 0 && r < w.n) d.dvec[(long long)h * d.T + w.row0 + r] = D[i];
     }
     const float mul[4] = {d.scale, d.scale, d.scale, d.scale};
     store_tile<T, DHP>(o, mul, d.dq, w.row0, q0, w.n, h, d.dh, ty, tx);

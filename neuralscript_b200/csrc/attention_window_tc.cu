@@ -509,20 +509,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 //              hide each other's latencies. Before the first tile they form
 //              D = rowdot(dout, out), which the second kernel reads too.
 //
-// `out` is bf16, so that this D is off by up to 2^-9 |dout| |out|, and with it
-// every dS of the row by P times that. Where rows see few keys, dS itself is
-// small (one key: 0) and that is most of its error. There a pass before sums
-// dS: as the weights P add up to 1, the sum over a row of P (dP - D) is what D
-// is short of. Rounding dS to bf16 for the products remains (2^-9 of itself).
-// Error of dq and dk against 64 bits, in the norm: window of 2 keys 3.8e-3 to
-// 2.4e-3, sequences of 5 rows 3.9e-3 to 2.1e-3, and up to 2.5e-3 as in blocks of
-// many tiles, which go without; one pass more of a block costs 2/3 of its time.
+// Where few keys are seen (few_keys) a pass before sums dS, and D is corrected by
+// that; it costs 2/3 of the block's time. Rounding dS to bf16 for the products
+// remains (2^-9 of itself).
 //
 // Bound by the products' issue and turns: 8192 rows in 3 sequences, 16 heads of
 // 128 columns, window 1024: 162 us, 0.52 PFLOP/s in S, dP and dQ.
 // ---------------------------------------------------------------------------
 constexpr int kBwdQThreads = 608;
-constexpr int kFewTiles = 2;  // tiles of keys for which the pass is made (none: dq 1 to 4 % faster, see above)
 
 template <int DHP>
 struct BwdQ {
@@ -591,7 +585,7 @@ __global__ void __launch_bounds__(kBwdQThreads, 1)
     const Waits wait{failed, d.err};
     bool ok = true;
     const KeyTiles tiles(d, q0, min(q0 + kT, w.n), kT);
-    const int first = tiles.count <= kFewTiles ? tiles.count : 0;  // steps of the pass that only sums
+    const int first = few_keys(d, q0, min(q0 + kT, w.n)) ? tiles.count : 0;  // steps of the pass that only sums
 
     if (warp == 17) {
         const bool one = (t & 31) == 0;

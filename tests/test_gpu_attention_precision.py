@@ -8,6 +8,7 @@ import torch
 
 from attention_ref import close, half_step
 from neuralscript_b200 import ops
+from test_gpu_attention_cache import run_window
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -65,3 +66,10 @@ def test_infinite_values_over_the_cache(lens, dtype):
         ops.attention_paged(q, kc, vc, table.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"), out)
         assert (out[..., 5] == math.inf).all() and (out[..., 6] == -math.inf).all() and out[..., 7].isnan().all()
         assert out[..., [c for c in range(dh) if c not in (5, 6, 7)]].isfinite().all()
+
+
+@pytest.mark.parametrize("dh", [64, 128, 20, 100])  # (the last two: not on the tensor cores)
+@pytest.mark.parametrize("lens,window,sinks", [([700], 2, 1), ([700, 300], 9, 4), ([700], 50, 3), ([600], 1, 63), ([2, 3, 5, 9, 40, 256], 0, 0)])
+def test_gradients_of_rows_with_few_keys_and_first_tokens(lens, window, sinks, dh):
+    """D = sum P dP, not the rounded output's, wherever rows see few keys: first tokens beside the window, any alignment."""
+    run_window(lens, 4, 2, dh, window, sinks, BF, True, summed=True)
