@@ -361,10 +361,11 @@ int nsb_op_kv_append(const void* k, long long k_row, long long k_head, const voi
  *   out = sum_j p_j v_j,  p = softmax(scale * q . k_j),  lse = log sum_j exp(scale * q . k_j)
  * over j < lens[b] and, where window > 0, j >= lens[b] - window or j < sinks.
  * lse [B, Hq] may be NULL. Without a key (or with none but scores of -inf):
- * zeros and -inf. A length that the table has no room for is cut, and a page
- * outside the cache left out; both are reported by nsb_op_device_error. What
- * the cache holds behind a sequence's end is not looked at. dh <= 128,
- * B <= 8192, B * Hq < 2^31, scale > 0. workspace (16-byte aligned) of at least
+ * zeros and -inf; a negative length is one of 0. A length that the table has no
+ * room for, or above 2^31 - 16, is cut, and a page outside the cache left out;
+ * both are reported by nsb_op_device_error. What the cache holds behind a
+ * sequence's end is not looked at. dh <= 128, B <= 8192, B * Hq < 2^31,
+ * scale > 0. workspace (16-byte aligned) of at least
  * nsb_op_attention_paged_workspace_bytes(...) bytes: of this call alone until
  * it is done. */
 size_t nsb_op_attention_paged_workspace_bytes(int B, int Hq, int Hkv, int dh);

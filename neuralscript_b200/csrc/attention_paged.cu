@@ -39,6 +39,7 @@ constexpr int kKeys = 16;        // a unit
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kPerSm = 3;        // most blocks an SM that the grid is made for
+constexpr long long kMaxKeys = (1LL << 31) - kKeys;  // of a sequence: whole units of them are counted in 32 bits
 constexpr int kMinUnits = 2;     // least units a warp: below, joining costs more than a warp saves
 constexpr int kSlots = 2 * kWarps + 1;  // parts that a block may leave: two a warp, or one
 constexpr float kLog2e = 1.4426950408889634f;
@@ -62,7 +63,7 @@ struct Seen {
 };
 __device__ __forceinline__ Seen seen_of(const PagedDesc& d, int b) {
     int len = d.lens[b];
-    const long long room = min((long long)d.width * d.page, 0x7fffffffLL);
+    const long long room = min((long long)d.width * d.page, kMaxKeys);
     if (len < 0 || len > room) {
         if (len > 0) atomicCAS(d.err, 0, kErrBadIndex);
         len = len < 0 ? 0 : (int)room;
@@ -956,7 +957,8 @@ int attention_paged(const PagedDesc& d, cudaStream_t st) {
     if (d.B > kPagedMaxBatch || (long long)d.B * d.Hq > 0x7fffffff) return -2;
     if (d.B == 0) return 0;
     // units are counted in 32 bits, those of one warp too
-    const long long room = (long long)d.width * d.page, seen = d.window ? (long long)d.window + d.sinks : room;
+    const long long places = (long long)d.width * d.page, room = places < kMaxKeys ? places : kMaxKeys;
+    const long long seen = d.window ? (long long)d.window + d.sinks : room;
     if ((room < seen ? room : seen) / kKeys * d.B >= (1LL << 31) - kPagedMaxBatch ||
         (room < seen ? room : seen) / kKeys * d.B * d.Hq >= 1LL << 39)
         return -2;

@@ -688,3 +688,22 @@ def test_python_refusals():
             ops.attention_window(*a, **kw)
     with pytest.raises(ValueError):
         ops.attention_window_bwd(q, k, k, o, l, o, q, k, k[:2])
+
+
+@pytest.mark.parametrize("dtype,dh", [(BF, 8), (BF, 7), (F, 8)])
+def test_paged_of_the_longest_lengths(dtype, dh):
+    """2^31 - 1 keys, of pages that are all one: cut to 2^31 - 16 (units of 16 are counted in 32 bits) and reported."""
+    page, H = 1 << 20, 1
+    kc, vc = normal(1, page, H, dh, dtype=dtype), torch.ones(1, page, H, dh, dtype=dtype, device="cuda")
+    table = torch.zeros(1, (1 << 31) // page, dtype=torch.int32, device="cuda")
+    q, out, lse = torch.zeros(1, H, dh, dtype=dtype, device="cuda"), torch.empty(1, H, dh, dtype=dtype, device="cuda"), torch.empty(1, H, device="cuda")
+    for n, cut in ((2 ** 31 - 17, False), (2 ** 31 - 16, False), (2 ** 31 - 15, True), (2 ** 31 - 1, True)):
+        out.zero_()
+        ops.attention_paged(q, kc, vc, table, ints([n]), out, lse=lse)
+        if cut:
+            with pytest.raises(RuntimeError, match="index past"):
+                ops.check_errors()
+        ops.check_errors()
+        # equal scores: the mean of ones, and the logarithm of how many; sums of up to 2^13 parts in fp32
+        assert (out.double() - 1).abs().max() <= half_step(dtype) + 2.0 ** -11
+        assert abs(float(lse) - math.log(min(n, 2 ** 31 - 16))) <= 2.0 ** -10
