@@ -121,7 +121,10 @@ def L():
 
 def _call(lib, which, *args):
     """An entry with its arguments in one block: ctypes takes 0.1 us for each of up to 60. Addresses are ints, 0: none."""
-    block = _packs[which](*args)
+    try:
+        block = _packs[which](*args)
+    except struct.error as e:  # sizes past 32 bits, numbers that are none
+        raise ValueError(f"{_BLOCKS[which]}: {e}") from None
     rc = lib.nsb_op_from_block(which, block, len(block))
     if rc:
         _check(rc, _BLOCKS[which])

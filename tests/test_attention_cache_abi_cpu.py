@@ -123,3 +123,12 @@ def test_window_limits():
         assert call(name, ok, dict(Hq=131072, Hkv=65536)) == -2
         assert call(name, ok, dict(T=(1 << 30) + 1, ld_lse=1 << 31)) == -2
         assert call(name, ok, dict(T=1 << 30, Hq=65535, Hkv=1, ld_lse=1 << 31)) == -2
+
+
+@pytest.mark.parametrize("which,ok,bad", [(0, ROPE, dict(T=1 << 31)), (1, ROPE, dict(H=1 << 32)), (2, APPEND, dict(pages=1 << 31)), (3, PAGED, dict(B=1 << 31)),
+                                          (4, WINDOW, dict(T=1 << 31)), (4, WINDOW, dict(scale="0.1")),
+                                          (5, GRADS, dict(T=-(1 << 31) - 1)), (5, GRADS, dict(B=2.5))])
+def test_numbers_past_their_types_raise_value_errors(which, ok, bad):
+    """Before anything reaches the library."""
+    with pytest.raises(ValueError, match=ops._BLOCKS[which]):
+        ops._call(None, which, *(0 if v is None else v for v in (ok | bad).values()), 0)

@@ -707,3 +707,16 @@ def test_paged_of_the_longest_lengths(dtype, dh):
         # equal scores: the mean of ones, and the logarithm of how many; sums of up to 2^13 parts in fp32
         assert (out.double() - 1).abs().max() <= half_step(dtype) + 2.0 ** -11
         assert abs(float(lse) - math.log(min(n, 2 ** 31 - 16))) <= 2.0 ** -10
+
+
+def test_sizes_past_32_bits():
+    """ValueError from every entry that can meet them (the tensors have one row, seen 2^31 times)."""
+    n = 2 ** 31
+    x, many = torch.zeros(1, 1, 64, dtype=BF, device="cuda"), torch.zeros(1, 1, 64, dtype=BF, device="cuda").expand(n, 1, 64)
+    cache, i = torch.zeros(1, 1, 1, 64, dtype=BF, device="cuda").expand(n, 1, 1, 64), ints([0])
+    for call in (lambda: ops.rope(x.expand(1, n, 64), i, freqs(8), x.expand(1, n, 64)),
+                 lambda: ops.kv_append(x, x, i, i, i[None], cache, cache),
+                 lambda: ops.attention_paged(x, cache, cache, i[None], i, x),
+                 lambda: ops.attention_window(many, many, many, many)):
+        with pytest.raises(ValueError):
+            call()
