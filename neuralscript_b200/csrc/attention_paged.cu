@@ -533,7 +533,8 @@ struct State {
             for (int k = 0; k < KS; k++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    const __nv_bfloat162 v = __floats2bfloat162_rn(o[k][n][2 * e] * mul[0], o[k][n][2 * e + 1] * mul[1]);
+                    const __nv_bfloat162 v = __floats2bfloat162_rn(mul[0] == 0.f ? 0.f : o[k][n][2 * e] * mul[0],  // (0 times an infinity)
+                                                                   mul[1] == 0.f ? 0.f : o[k][n][2 * e + 1] * mul[1]);
                     const uint32_t w = turned(*reinterpret_cast<const uint32_t*>(&v));
                     const int c = 16 * k + 8 * e;
                     if (h >= heads || c + 2 * (lane & 3) >= d.dh) continue;

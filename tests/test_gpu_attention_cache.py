@@ -720,3 +720,18 @@ def test_sizes_past_32_bits():
                  lambda: ops.attention_window(many, many, many, many)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("n", [5, 16, 90, 3000])  # finished by a warp, by a block, joined
+def test_paged_infinite_values_of_scores_of_minus_infinity(n, dtype):
+    """Where every score is -inf nothing is seen, whatever the values are."""
+    c = paged_case([n, n], 4, 2, 64, 8, dtype)
+    c["q"].abs_()
+    for j in range(n):
+        c["kc"][int(c["table"][0, j // 8]), j % 8, 0] = -math.inf
+    c["vc"][int(c["table"][0, 0]), 0, 0, 3::4] = math.inf
+    c["vc"][int(c["table"][0, 0]), 1, 0, 2::4] = math.nan
+    run_paged(c, 0, 0)
+    assert (c["out"][0, :2] == 0).all() and (c["lse"][0, :2] == -math.inf).all()
+    assert c["out"][0, 2:].isfinite().all() and c["out"][1].isfinite().all()
