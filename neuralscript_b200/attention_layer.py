@@ -37,18 +37,36 @@ class PagedCache:
         self.width = pages if width is None else width  # fixed, so that a captured step finds its table again
         self.table = torch.zeros(B, self.width, dtype=torch.int32, device="cuda")
 
-    def grow(self, new):
-        """Room for new[b] tokens more of every sequence."""
-        for b, n in enumerate(new):
-            need = -(-(self.lens[b] + n) // self.page)
-            if need > self.width or need - len(self.host[b]) > len(self.free):
+    def chosen(self, which):
+        """The sequences' numbers: all, or those of `which`, each once."""
+        B = len(self.lens)
+        which = list(range(B) if which is None else which)
+        if len(set(which)) != len(which) or not all(0 <= b < B for b in which):
+            raise ValueError(f"sequences {which} where different ones of 0 to {B - 1} are wanted")
+        return which
+
+    def grow(self, new, which=None):
+        """Room for new[i] tokens more of sequence which[i] (of every sequence): of all of them or, where it does not
+        suffice, of none."""
+        which, new = self.chosen(which), list(new)
+        if len(new) != len(which) or min(new, default=0) < 0:
+            raise ValueError(f"{new} tokens for {len(which)} sequences")
+        places, left = [], len(self.free)
+        for b, n in zip(which, new):
+            had, need = len(self.host[b]), -(-(self.lens[b] + n) // self.page)
+            left -= max(0, need - had)
+            if need > self.width or left < 0:
                 raise ValueError(f"sequence {b}: no room for {self.lens[b] + n} tokens")
-            while len(self.host[b]) < need:
+            places += [(b, i) for i in range(had, need)]
+        if places:
+            for b, _ in places:
                 self.host[b].append(self.free.pop())
-                self.table[b, len(self.host[b]) - 1] = self.host[b][-1]
+            rows, cols = zip(*places)
+            rows, cols, pages = _ints([rows, cols, [self.host[b][i] for b, i in places]])
+            self.table[rows, cols] = pages
 
     def release(self, b):
-        """Gives sequence b's pages back."""
+        """Gives sequence b's pages back; a prompt or a token may begin it again."""
         self.free += self.host[b]
         self.host[b], self.lens[b] = [], 0
 
@@ -75,10 +93,13 @@ class AttentionLayer:
         """Rounds the weights to the products' type (after they change)."""
         self.wqkv16, self.wo16 = self.wqkv.to(BF16), self.wo.to(BF16)
 
-    def _heads(self, x):
-        """Queries, keys and values [T, Hq + 2 Hkv, dh] of x [T, D] (bf16, contiguous)."""
+    def _check(self, x):
         if x.dtype != BF16 or x.dim() != 2 or x.shape[1] != self.D or not x.is_contiguous():
             raise ValueError(f"x: {x.dtype} {tuple(x.shape)} where rows of {self.D} bfloat16 are wanted")
+
+    def _heads(self, x):
+        """Queries, keys and values [T, Hq + 2 Hkv, dh] of x [T, D] (bf16, contiguous)."""
+        self._check(x)
         T = x.shape[0]
         heads = torch.empty(T, self.N, dtype=BF16, device="cuda")
         ops.gemm(x, self.wqkv16, T, self.N, self.D, self.D, 0, self.D, 0, c16=heads)
@@ -136,31 +157,47 @@ class AttentionLayer:
         self.refresh()
         return loss
 
-    def prompt(self, cache, x, new):
-        """y [T, D] of the sequences' prompts x [T, D], new[b] rows of each, which enter the (empty) cache."""
-        if any(cache.lens):
+    def prompt(self, cache, x, new, which=None):
+        """y [T, D] of prompts x [T, D], new[i] rows of sequence which[i] (of every sequence), which enter the cache; it
+        holds nothing of these sequences yet."""
+        self._check(x)
+        which, new = cache.chosen(which), list(new)
+        if any(cache.lens[b] for b in which):
             raise ValueError("a prompt begins a sequence: its cache is empty")
-        cache.grow(new)
+        if sum(new) != x.shape[0]:
+            raise ValueError(f"{sum(new)} rows of prompts where x has {x.shape[0]}")
+        if not x.shape[0]:
+            return torch.empty(0, self.D, device="cuda")
+        cache.grow(new, which)
         at = _ints([i for n in new for i in range(n)])
-        seq = _ints([b for b, n in enumerate(new) for _ in range(n)])
-        offsets = _ints([sum(new[:b]) for b in range(len(new) + 1)])
+        seq = _ints([b for b, n in zip(which, new) for _ in range(n)])
+        offsets = _ints([sum(new[:i]) for i in range(len(new) + 1)])
         y, kept = self.forward(x, offsets, at)
         _, k, v = self._split(kept["heads"])
         ops.kv_append(k, v, seq, at, cache.table, cache.k, cache.v)  # (keys are rotated already)
-        cache.lens = list(new)
+        for b, n in zip(which, new):
+            cache.lens[b] = n
         return y
 
-    def token(self, cache, x):
-        """y [B, D] of one more token of every sequence, x [B, D]."""
-        B = x.shape[0]
-        cache.grow([1] * B)
-        at = _ints(cache.lens)
+    def token(self, cache, x, which=None):
+        """y [n, D] of one more token, x [n, D], of the sequences `which` (of every sequence, where one that the cache
+        holds nothing of begins with it)."""
+        self._check(x)
+        which = cache.chosen(which)
+        n = len(which)
+        if x.shape[0] != n:
+            raise ValueError(f"{x.shape[0]} rows of tokens for {n} sequences")
+        if not n:
+            return torch.empty(0, self.D, device="cuda")
+        cache.grow([1] * n, which)
+        at, seq = _ints([cache.lens[b] for b in which]), _ints(which)
         q, k, v = self._split(self._heads(x))
-        turned, ctx = (torch.empty(B, self.Hq, self.dh, dtype=BF16, device="cuda") for _ in "qc")
-        ops.kv_append(k, v, torch.arange(B, dtype=torch.int32, device="cuda"), at, cache.table, cache.k, cache.v, pos=at,
-                      freq=self.freq, q=q, q_out=turned)
-        cache.lens = [n + 1 for n in cache.lens]
-        ops.attention_paged(turned, cache.k, cache.v, cache.table, at + 1, ctx, **self.seen)
+        turned, ctx = (torch.empty(n, self.Hq, self.dh, dtype=BF16, device="cuda") for _ in "qc")
+        ops.kv_append(k, v, seq, at, cache.table, cache.k, cache.v, pos=at, freq=self.freq, q=q, q_out=turned)
+        for b in which:
+            cache.lens[b] += 1
+        table = cache.table if which == list(range(len(cache.lens))) else cache.table[seq]
+        ops.attention_paged(turned, cache.k, cache.v, table, at + 1, ctx, **self.seen)
         return self._out(ctx)
 
 

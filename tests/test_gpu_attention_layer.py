@@ -99,3 +99,62 @@ def test_refusals():
     for x in (torch.zeros(4, 96, device="cuda"), torch.zeros(4, 95, device="cuda", dtype=BF), torch.zeros(96, 4, device="cuda", dtype=BF).t()):
         with pytest.raises(ValueError):
             layer._heads(x)
+
+
+def state(cache):
+    return list(cache.lens), [list(h) for h in cache.host], sorted(cache.free), cache.table.clone()
+
+
+def same(a, b):
+    return a[:3] == b[:3] and torch.equal(a[3], b[3])
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (16, 2)])
+def test_sequences_come_and_go(window, sinks):
+    """A released sequence is served again beside one that goes on, with prompts and tokens of some sequences alone."""
+    from neuralscript_b200.attention_layer import PagedCache
+    layer = layer_of(window, sinks, seed=4)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(6)
+    a, b, c = (torch.randn(n, 96, device="cuda", generator=g).to(BF) for n in (70, 30, 40))
+    want = [whole(layer, r.double(), layer.wqkv16.double(), layer.wo16.double(), [r.shape[0]]) for r in (a, b, c)]
+    bound = 4 * half_step(BF)  # heads, their rotation, the weights, ctx
+    cache = PagedCache(layer, 3, pages=14, page=8)
+    y = layer.prompt(cache, torch.cat([a[:50], b[:20]]), [50, 20], which=[2, 0])
+    assert cache.lens == [20, 0, 50]
+    assert off(y, torch.cat([want[0][:50], want[1][:20]])) <= bound
+    for i in range(10):
+        y = layer.token(cache, torch.stack([b[20 + i], a[50 + i]]), which=[0, 2])
+        assert off(y, torch.stack([want[1][20 + i], want[0][50 + i]])) <= bound
+    cache.release(0)
+    y = layer.prompt(cache, c[:35], [35], which=[1])
+    assert off(y, want[2][:35]) <= bound
+    y = layer.token(cache, torch.stack([c[35], a[60], b[0]]), which=[1, 2, 0])  # (the third begins with its token)
+    assert off(y, torch.stack([want[2][35], want[0][60], want[1][0]])) <= bound
+    y = layer.token(cache, torch.stack([b[1], c[36], a[61]]))  # all of them, in order
+    assert off(y, torch.stack([want[1][1], want[2][36], want[0][61]])) <= bound
+    assert cache.lens == [2, 37, 62]
+
+
+def test_refused_calls_leave_the_cache_as_it_was():
+    from neuralscript_b200.attention_layer import PagedCache
+    layer = layer_of(0, 0)
+    x = torch.zeros(60, 96, device="cuda", dtype=BF)
+    cache = PagedCache(layer, 3, pages=6, page=8, width=5)
+    layer.prompt(cache, x[:9], [9], which=[1])
+    was = state(cache)
+    for call in (lambda: layer.prompt(cache, x[:9], [9], which=[1]), lambda: layer.prompt(cache, x[:9], [8], which=[0]),
+                 lambda: layer.prompt(cache, x[:9], [9], which=[3]), lambda: layer.prompt(cache, x[:9], [4, 5], which=[0, 0]),
+                 lambda: layer.prompt(cache, x[:9], [10, -1], which=[0, 2]), lambda: layer.prompt(cache, x[:9], [4, 5], which=[0]),
+                 lambda: layer.prompt(cache, x[:9].float(), [9], which=[0]), lambda: layer.prompt(cache, x[:40], [20, 20], which=[0, 2]),
+                 lambda: layer.prompt(cache, x[:41], [41], which=[0]), lambda: layer.prompt(cache, x[:9], [9]),
+                 lambda: layer.token(cache, x[:2]), lambda: layer.token(cache, x[:2], which=[1]), lambda: layer.token(cache, x[:2], which=[1, 1]),
+                 lambda: layer.token(cache, x[:1], which=[-1]), lambda: layer.token(cache, x[:1].float(), which=[1]),
+                 lambda: cache.grow([20, 20, 20]), lambda: cache.grow([1, 1])):
+        with pytest.raises(ValueError):
+            call()
+        assert same(state(cache), was)
+    assert layer.token(cache, x[:0], which=[]).shape == layer.prompt(cache, x[:0], [0, 0], which=[0, 2]).shape == (0, 96)
+    assert same(state(cache), was)
+    layer.token(cache, x[:3])
+    assert cache.lens == [1, 10, 1]
