@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from attention_ref import close, half_step
+from attention_ref import close, half_step, packed, turn, turn_tolerance
 from neuralscript_b200 import ops
 from test_gpu_attention_cache import run_window
 
@@ -73,3 +73,64 @@ def test_infinite_values_over_the_cache(lens, dtype):
 def test_gradients_of_rows_with_few_keys_and_first_tokens(lens, window, sinks, dh):
     """D = sum P dP, not the rounded output's, wherever rows see few keys: first tokens beside the window, any alignment."""
     run_window(lens, 4, 2, dh, window, sinks, BF, True, summed=True)
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (11, 2)])
+def test_prompt_then_tokens_by_the_rotated_heads(window, sinks, dtype):
+    """Prompts, then single tokens, through rotation, cache and both attentions, against the definition on the queries
+    that the calls gave and the keys and values that the cache holds: attention's tolerance alone. The same definition
+    on mistaken places, sequences or windows is far outside it."""
+    Hq, Hkv, dh, page, prompts, steps = 4, 2, 64, 8, [30, 5], 12
+    total = [p + steps for p in prompts]
+    whole = [normal(t, Hq + 2 * Hkv, dh, seed=b + 1).to(dtype) for b, t in enumerate(total)]
+    freq = (10000.0 ** (-torch.arange(32, dtype=torch.float64) / 32)).float().cuda()
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    empty = lambda *s: torch.empty(*s, dtype=dtype, device="cuda")  # noqa: E731
+    order = torch.randperm(sum(-(-t // page) for t in total), generator=torch.Generator().manual_seed(1)).tolist()
+    table = [[order.pop() for _ in range(-(-t // page))] for t in total]
+    pages, wide = sum(map(len, table)), max(map(len, table))
+    kc, vc = (torch.full((pages, page, Hkv, dh), math.nan, dtype=dtype, device="cuda") for _ in "kv")
+    on_device = ints([row + [-1] * (wide - len(row)) for row in table])
+    seen = dict(window=window, sinks=sinks)
+
+    def append(heads, seq, at):
+        q = empty(heads.shape[0], Hq, dh)
+        ops.kv_append(heads[:, Hq:Hq + Hkv], heads[:, Hq + Hkv:], seq, at, on_device, kc, vc, pos=at, freq=freq, q=heads[:, :Hq], q_out=q)
+        return q
+
+    heads = torch.cat([w[:p] for w, p in zip(whole, prompts)])
+    T, at = sum(prompts), ints([i for p in prompts for i in range(p)])
+    q = append(heads, ints([b for b, p in enumerate(prompts) for _ in range(p)]), at)
+    k, out = empty(T, Hkv, dh), empty(T, Hq, dh)
+    ops.rope(heads[:, Hq:Hq + Hkv], at, freq, k)
+    ops.attention_window(q, k, heads[:, Hq + Hkv:], out, offsets=ints([0, prompts[0], T]), **seen)
+    queries, found = ([[x[:prompts[0]]], [x[prompts[0]:]]] for x in (q, out))
+    for s in range(steps):
+        at = ints([p + s for p in prompts])
+        q = append(torch.stack([w[p + s] for w, p in zip(whole, prompts)]), ints([0, 1]), at)
+        out = empty(2, Hq, dh)
+        ops.attention_paged(q, kc, vc, on_device, at + 1, out, **seen)
+        for b in range(2):
+            queries[b].append(q[b:b + 1])
+            found[b].append(out[b:b + 1])
+    ops.check_errors()
+    queries, found = [torch.cat(x) for x in queries], [torch.cat(x) for x in found]
+    held = [[c[ints(table[b]).long()].flatten(0, 1)[:total[b]] for b in range(2)] for c in (kc, vc)]
+    for b, t in enumerate(total):
+        k, v = held[0][b], held[1][b]
+        assert torch.equal(v, whole[b][:, Hq + Hkv:])
+        x = whole[b]
+        turned = turn(x, torch.arange(t, device="cuda")[None], freq, torch.zeros(32, dtype=torch.long, device="cuda"), False, 1.0)
+        tol = turn_tolerance(x, 32, False, 1.0, dtype, turned)
+        close(queries[b], turned[:, :Hq], tol[:, :Hq], "queries")
+        close(k, turned[:, Hq:Hq + Hkv], tol[:, Hq:Hq + Hkv], "keys")
+        want, tol = packed(queries[b], k, v, [0, t], window, sinks, 0.125, dtype)["out"]
+        assert tol.max() < 0.05  # of values with a spread of 1
+        close(found[b], want, tol, "out")
+        wrong = [(k, v.roll(1, 0), window, sinks), (k.roll(1, 0), v, window, sinks), (k, v, 7, sinks), (k, v.flip(1), window, sinks)]
+        for other in wrong:
+            want, tol = packed(queries[b], *other[:2], [0, t], *other[2:], 0.125, dtype)["out"]
+            off = (found[b].double() - want).abs() > tol
+            # (row 9 is the first that a window of 7 and 2 first tokens changes: row 8 sees 2 to 8, and 0 and 1)
+            assert off[9:].any(-1).float().mean() > 0.9, other[2:]
