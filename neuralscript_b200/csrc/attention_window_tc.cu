@@ -1282,7 +1282,6 @@ __global__ void __launch_bounds__(kBwdKvThreads, 1)
 // shares of the columns).
 template <int DHP>
 __global__ void __launch_bounds__(256) window_tc_join_kernel(const __grid_constant__ WindowDesc d, int blocks) {
-    cudaGridDependencySynchronize();
     const int group = d.Hq / d.Hkv, hk = blockIdx.y;
     const long long per = share(all_steps(d), blocks);
     Seq q;
@@ -1384,18 +1383,8 @@ int bwd(const WindowDesc& d, cudaStream_t s) {
     const int blocks = num_sms();
     window_tc_bwd_q_kernel<DHP><<<(unsigned)(tiles * d.Hq), kBwdQThreads, BwdQ<DHP>::SMEM, s>>>(q, k, v, g, d);
     window_tc_bwd_kv_kernel<DHP><<<blocks, kBwdKvThreads, BwdKv<DHP>::SMEM, s>>>(q, k, v, g, d);
-    if (cudaGetLastError() != cudaSuccess) return -5;
-    // launched while the kernel before runs, and waits for it
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)tiles, d.Hkv, 4);
-    cfg.blockDim = dim3(256);
-    cfg.stream = s;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, window_tc_join_kernel<DHP>, d, blocks) == cudaSuccess ? 0 : -5;
+    window_tc_join_kernel<DHP><<<dim3((unsigned)tiles, d.Hkv, 4), 256, 0, s>>>(d, blocks);
+    return cudaGetLastError() == cudaSuccess ? 0 : -5;
 }
 
 }  // namespace
