@@ -344,8 +344,8 @@ int nsb_op_rope_bwd(const void* dy, int dtype, long long dy_row, long long dy_he
 /* Keys k and values v [T, Hkv, dh] into their caches, token t at key at[t] of
  * sequence seq[t], keys rotated as above on the way (pairs 0: as they are),
  * and queries q [T, Hq, dh], rotated, to q_out (both may be NULL; q_out may be
- * q). A token with a negative seq[t] is padding: nothing of it is read or
- * written. One whose place is outside the table or the cache is left out too,
+ * q). A token with a negative seq[t] is padding: nothing of its keys, values
+ * and queries is read or written. One whose place is outside the table or the cache is left out too,
  * and reported by nsb_op_device_error. No two tokens of one call go to the
  * same place. (2 Hkv + Hq) * dh is at most 2^26. */
 int nsb_op_kv_append(const void* k, long long k_row, long long k_head, const void* v, long long v_row, long long v_head,
@@ -384,8 +384,9 @@ int nsb_op_attention_paged(const void* q, long long q_row, long long q_head, int
  * lse [Hq, ld_lse] receives the log-sum-exp (may be NULL). Rows behind the
  * last sequence are neither read nor written. Offsets that do not rise are
  * cut and reported by nsb_op_device_error. dh <= 128, scale > 0, T <= 2^30,
- * Hq <= 65535. A value of a sequence that is infinite or NaN can reach its
- * queries before it too, and such a gradient its keys behind it. */
+ * Hq <= 65535. What is infinite or NaN in a sequence can reach its rows that it
+ * is hidden from too: values the outputs, keys the gradients of queries, queries
+ * and dout those of keys and values. */
 int nsb_op_attention_window(const void* q, long long q_row, long long q_head, const void* k, long long k_row,
                             long long k_head, const void* v, long long v_row, long long v_head, int dtype, int T, int Hq,
                             int Hkv, int dh, const int* offsets, int B, int window, int sinks, float scale, void* out,

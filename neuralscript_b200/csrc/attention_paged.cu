@@ -2,8 +2,10 @@
 //   out[b, h] = sum over visible j of p_j v_j,  p = softmax(scale * q[b, h] . k_j),
 // j visible where j < len and (no window, or j >= len - window, or j < sinks).
 //
-// Memory-bound: every visible key and value is read once, for all query heads
-// that share it. One pass with the running maximum and sum of the softmax.
+// Memory-bound: every visible key and value is read once for up to 16 query heads
+// that share it in bf16, and for up to 4 in fp32 (a warp's registers hold no more;
+// larger groups are cut into shares that each read it). One pass with the running
+// maximum and sum of the softmax.
 //
 // Work is cut without regard to where sequences end: the visible keys of every
 // (sequence, key head), counted in units of 16, stand in one line, and every
@@ -18,9 +20,17 @@
 //
 // Bound by HBM while it streams; the sum of lengths before it takes some 5 us,
 // the join behind it 2 to 9. 64 sequences of up to 4096 keys, 24 heads on 4 of
-// 128 columns, bf16: 47.2 us, 4.5 TB/s; two of 120000, 16 heads on 2: 41.8 us,
+// 128 columns, bf16: 46.9 us, 4.5 TB/s; two of 120000, 16 heads on 2: 41.9 us,
 // 4.8 TB/s; fp32, 96 behind a window of 1024, 8 heads of 64: 62.4 us, 5.7 TB/s;
-// one sequence of 900 keys, 8 heads of 64: 9.7 us, all of it latency.
+// one sequence of 900 keys, 8 heads of 64: 9.7 us, all of it latency. What the
+// forms cost that it suits less, 64 sequences of up to 4096 keys on 4 key heads:
+// fp32 of 64 columns, 4 query heads a key head 56 us (3.8 TB/s), 8 105, 16 196;
+// fp32 of 128 columns, whose ring leaves room for one block an SM, one query head
+// 84 us (5.0 TB/s), 6 223; bf16 of 128, 16 query heads 113, 24 188. Every block
+// holds a number for each sequence and sums all lengths up, and shares are cut for
+// as many blocks as a small batch's SMs hold: 512 sequences of up to 2048 keys,
+// 24 heads on 4 of 128, bf16, 182 us (5.0 TB/s), 1024 of up to 1024 251 us (3.5),
+// 4096 of up to 256 387 us (2.3).
 #include <cuda_bf16.h>
 #include <math.h>
 
@@ -38,7 +48,7 @@ namespace {
 constexpr int kKeys = 16;        // a unit
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
-constexpr int kPerSm = 3;        // most blocks an SM that the grid is made for
+constexpr int kPerSm = 3;        // most blocks an SM that the grid is made for (fewer fit beside some 700 sequences' sums)
 constexpr long long kMaxKeys = (1LL << 31) - kKeys;  // of a sequence: whole units of them are counted in 32 bits
 constexpr int kMinUnits = 2;     // least units a warp: below, joining costs more than a warp saves
 constexpr int kSlots = 2 * kWarps + 1;  // parts that a block may leave: two a warp, or one
@@ -266,7 +276,7 @@ __global__ void __launch_bounds__(kThreads) paged_kernel(const __grid_constant__
 // product's columns by a transpose in registers, O^T += V^T P^T. A weight goes in
 // as two bf16, its first eight digits and the next (2^-16 of it is lost; its sum
 // is taken before): the tensor pipe has room beside the bytes. 64 sequences
-// take 47.2 us for 45.5 with a rounded weight, and the result differs from one
+// take 46.9 us for 45.7 with a rounded weight, and the result differs from one
 // of fp32 weights by 8e-5 for 1.7e-3. Groups of fewer heads leave columns
 // empty, which costs nothing.
 // fp32: on the fp32 units, two lanes a key for the scores, and four columns a

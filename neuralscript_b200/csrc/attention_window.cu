@@ -252,7 +252,8 @@ __global__ void __launch_bounds__(kGroup) window_fwd_kernel(const __grid_constan
     store_tile<T, DHP>(o, mul, d.out, w.row0, q0, w.n, h, d.dh, ty, tx);
 }
 
-// dq and D of 64 queries: grid (tiles, Hq)
+// dq and D of 64 queries: grid (tiles, Hq). bf16: where few keys are seen, a pass
+// before corrects D (few_keys).
 template <typename T, int DHP>
 __global__ void __launch_bounds__(kGroup) window_bwd_q_kernel(const __grid_constant__ WindowDesc d) {
     extern __shared__ float sm[];

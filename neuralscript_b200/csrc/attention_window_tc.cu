@@ -211,9 +211,12 @@ __device__ __forceinline__ bool all_seen(const WindowDesc& d, int q0, int k0) {
 //              both then take turns on the tensor cores and end late.)
 //   warps 8 g .. 8 g + 7   softmax of tile g, two threads a query with 64 keys
 //              each, which exchange their maxima through shared memory (8192
-//              rows: 246 us, a thread a query 279): the scores come from TMEM
+//              rows: 242 us, a thread a query 243): the scores come from TMEM
 //              into registers once, weights go back as bf16 pairs (off by 2^-9
-//              of themselves at most; their fp32 sum is taken before).
+//              of themselves at most; their fp32 sum is taken before). Weights in
+//              two bf16, with a product of each, take 337 us in place of 244 and
+//              leave outputs 1.6e-3 off in place of 2.1e-3, of which 1.6e-3 is
+//              the rounding of outputs to bf16.
 // O stays in TMEM. It is scaled only when a row's maximum rises by more than
 // 2^8 above the one that its weights are taken against: smaller rises cost
 // neither range (fp32) nor precision (the weights are floating point).

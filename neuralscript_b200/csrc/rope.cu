@@ -18,9 +18,11 @@
 //
 // Bound by HBM, with the issue slots close behind (64 %): 16384 rows of 20 heads
 // of 128 columns in bf16, 29.8 us a pass, 5.6 TB/s (a measured copy: 6.5); 9001 x
-// 12 x 80 in fp32, 14.4 us, 4.8 TB/s. Appending 32 tokens: 3.1 us, a launch; 8000
-// tokens of 8 heads of 64: 8.1 us, 4.1 TB/s, latency of one block's chain (place
-// of the token, angles, heads) in three rounds of blocks.
+// 12 x 80 in fp32, 14.6 us, 4.7 TB/s: 1126 blocks are one round, so that all form
+// their angles first and HBM waits. Appending 32 tokens: 3.1 us, a launch (fp32
+// 3.2); 8000 tokens of 8 heads of 64: 8.1 us, 4.1 TB/s: one round of blocks and 122
+// more, whose chain (place of the token, angles, heads) passes by itself; in fp32,
+// twice the bytes, 10.6 us, 6.2 TB/s.
 #include <cuda_bf16.h>
 
 #include <type_traits>
