@@ -345,9 +345,9 @@ int nsb_op_rope_bwd(const void* dy, int dtype, long long dy_row, long long dy_he
  * sequence seq[t], keys rotated as above on the way (pairs 0: as they are),
  * and queries q [T, Hq, dh], rotated, to q_out (both may be NULL; q_out may be
  * q). A token with a negative seq[t] is padding: nothing of its keys, values
- * and queries is read or written. One whose place is outside the table or the cache is left out too,
- * and reported by nsb_op_device_error. No two tokens of one call go to the
- * same place. (2 Hkv + Hq) * dh is at most 2^26. */
+ * and queries is read or written. One whose place is outside the table or the
+ * cache is left out too, and reported by nsb_op_device_error. No two tokens of
+ * one call go to the same place. (2 Hkv + Hq) * dh is at most 2^26. */
 int nsb_op_kv_append(const void* k, long long k_row, long long k_head, const void* v, long long v_row, long long v_head,
                      int dtype, int T, int Hkv, int dh, const int* seq, const int* at, const int* table, long long ld_table,
                      int B, int width, int pages, int page, void* k_cache, long long kc_page, long long kc_slot,

@@ -735,3 +735,18 @@ def test_paged_infinite_values_of_scores_of_minus_infinity(n, dtype):
     run_paged(c, 0, 0)
     assert (c["out"][0, :2] == 0).all() and (c["lse"][0, :2] == -math.inf).all()
     assert c["out"][0, 2:].isfinite().all() and c["out"][1].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("B,Hq,Hkv,dh", [(900, 6, 2, 128), (2500, 4, 1, 64), (8192, 2, 1, 128)])
+def test_paged_of_large_batches(B, Hq, Hkv, dh, dtype):
+    """Up to the most sequences of a call, whose sums take shared memory from the rings."""
+    lens = [(37 * b) % 61 for b in range(B)]
+    lens[B // 2], lens[-1] = 900, 5
+    c = paged_case(lens, Hq, Hkv, dh, 16, dtype)
+    run_paged(c, 40, 3)
+    some = sorted({0, 1, B // 2, B - 1} | set(range(7, B, B // 40)))
+    part = {k: [c[k][b] for b in some] for k in ("k", "v")} | {k: c[k][some] for k in ("q", "out", "lse")}
+    check_paged(part, [lens[b] for b in some], Hq, Hkv, dh, dtype, 40, 3, dh ** -0.5)
+    assert c["out"].isfinite().all()
+    ops.check_errors()
